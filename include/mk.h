@@ -489,6 +489,197 @@ typedef struct mk_moe_ffn_args {
 int mk_moe_ffn_combine(const mk_moe_ffn_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Router of the MoE layer: top-k choice, gates, and (optionally) per-expert
+ * counts and the balance loss, in one pass over the logits.
+ *   topk_ids[t, i] = expert of the i-th largest logit of token t; equal logits
+ *     (-0 equals 0) go to the lowest expert index, NaN ranks above everything
+ *     and -inf is never chosen: a token with fewer than topk other logits has
+ *     id -1 and gate 0 in the places left (the index build skips such ids)
+ *   p[t, e]  = exp(logit - max) / sum over the token's experts   (fp32)
+ *   gates[t, i] = p of the choice, divided by the sum over the token's choices
+ *     when renorm is set.  A NaN or +inf among a token's logits makes all its
+ *     p and gates NaN.
+ * A token does not count when its token_mask byte is 0 (its logits are not
+ * read) or all its logits are -inf: ids -1, gates 0, nothing added below.
+ * With counts set (then all of prob_sum, tokens, loss and workspace):
+ *   counts[e] = choices of e,  prob_sum[e] = sum_t p[t, e],  tokens = n = tokens that count
+ *   loss = coef * num_experts / (topk * n^2) * sum_e counts[e] * prob_sum[e]
+ * (coef when every expert gets the same share of both; 0 when n = 0).  Sums
+ * are added in a fixed order: equal inputs give equal bits.  The workspace
+ * needs no clearing and holds nothing between calls.
+ * At most 1024 experts and 32 choices.  No counterpart in the reference, whose
+ * benches draw their routing on the host (bench/dispatch_gemm_bench.py:103-124). */
+typedef struct mk_moe_route_args {
+  const void* logits;          /* [num_tokens, ld]: the first num_experts of each row */
+  const uint8_t* token_mask;   /* [num_tokens] or NULL */
+  int32_t* topk_ids;           /* [num_tokens, topk] */
+  float* gates;                /* [num_tokens, topk] */
+  int64_t num_tokens, ld;
+  int32_t num_experts, topk;
+  int32_t logits_dtype;        /* 0 fp32, 1 bf16 */
+  int32_t renorm;
+  int32_t* counts;             /* [num_experts] or NULL: no balance outputs */
+  float* prob_sum;             /* [num_experts] */
+  int32_t* tokens;             /* [1] */
+  float* loss;                 /* [1] */
+  float coef;
+  void* workspace;             /* mk_moe_route_workspace_bytes bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+} mk_moe_route_args;
+int64_t mk_moe_route_workspace_bytes(int64_t num_tokens, int32_t num_experts);
+int mk_moe_route(const mk_moe_route_args* args, void* stream);
+
+/* Gradient of mk_moe_route's logits, from the gates' gradient and from the
+ * balance loss (either part may be left out: dgates or counts NULL).  With the
+ * forward's p and gates g of the choices c_i, recomputed here from the logits:
+ *   renorm:  dlogits[j]  = sum_i [c_i = j] g_i (dgates_i - sum_l g_l dgates_l)
+ *   else:    dlogits[j]  = sum_i [c_i = j] p_j dgates_i - p_j sum_l p_{c_l} dgates_l
+ *   balance: dlogits[j] += dloss * coef * E / (topk n^2) * p_j (counts[j] - sum_e counts[e] p_e)
+ * (the counts are constants of the loss; counts and n = tokens may be sums over
+ * several ranks).  Choices outside [0, num_experts) have no gradient; tokens
+ * that do not count get zeros.  dlogits has the logits' type and may be the
+ * logits themselves, with the same ld. */
+typedef struct mk_moe_route_backward_args {
+  const void* logits;          /* as in mk_moe_route */
+  const uint8_t* token_mask;
+  const int32_t* topk_ids;     /* [num_tokens, topk]; read when dgates is set */
+  const float* dgates;         /* [num_tokens, topk] or NULL */
+  const float* dloss;          /* [1] or NULL: 1 */
+  const int32_t* counts;       /* [num_experts] or NULL */
+  const int32_t* tokens;       /* [1]; read when counts is set */
+  void* dlogits;               /* [num_tokens, ld_out]: the first num_experts of each row are written */
+  int64_t num_tokens, ld, ld_out;
+  int32_t num_experts, topk;
+  int32_t logits_dtype;
+  int32_t renorm;
+  float coef;
+} mk_moe_route_backward_args;
+int mk_moe_route_backward(const mk_moe_route_backward_args* args, void* stream);
+
+/* Gradient of mk_moe_combine for one rank's experts [expert_begin,
+ * expert_begin + n_local), with the tables that mk_moe_build_indices(_dev)
+ * made from topk_ids at row_block 128:
+ *   dy_expert[r] = row_weight[r] * dy[t(r)]         (fp32 product, bf16; zero on padding rows)
+ *   dgates[t, j] = sum_h dy[t, h] * y_expert[r(t, j), h]   (fp32)
+ * dgates is 0 where topk_ids names no local expert (another rank has that
+ * part) or the row was not produced here (slot_to_row -1).  Rows at or past
+ * R_pad (sizes[1] when sizes is set, R_pad then being the capacity) are
+ * neither read nor written.  dy_expert may be NULL, and rb_rows then too.
+ * Each sum is added in a fixed order.  At most 32 choices.  No counterpart in
+ * the reference, which has no backward pass. */
+typedef struct mk_moe_combine_backward_args {
+  const void* dy;               /* [num_tokens, H] fp32 or bf16 */
+  const void* y_expert;         /* bf16 [R_pad, H] */
+  const int32_t* topk_ids;      /* [num_tokens, topk] */
+  const float* row_weight;      /* [R_pad] */
+  const int32_t* owner_offset;  /* [num_tokens + 1] */
+  const int32_t* slot_to_row;   /* [R] */
+  const int32_t* rb_rows;       /* [R_pad/128] */
+  void* dy_expert;              /* bf16 [R_pad, H] or NULL */
+  float* dgates;                /* [num_tokens, topk] */
+  int64_t num_tokens, H, R_pad;
+  int32_t topk, expert_begin, n_local;
+  int32_t dy_dtype;             /* 0 fp32, 1 bf16 */
+  const int64_t* sizes;         /* device {R, R_pad} or NULL */
+} mk_moe_combine_backward_args;
+int mk_moe_combine_backward(const mk_moe_combine_backward_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* 4-bit weights with group scales:
+ *   w[k, n] = (code[k, n] - zero[k / group, n]) * scale[k / group, n]
+ * codes and zero points 0 .. 15 (8 where there are no zero points), scales
+ * bf16, group 32, 64 or 128 rows of K, the last one shorter where K ends in
+ * it.  The products read them in an order of their own, laid out once by
+ * mk_w4_pack; E matrices (experts) of one shape lie one after another. */
+typedef struct mk_w4_weights {
+  void* packed;      /* mk_w4_packed_bytes bytes, 16-byte aligned */
+  void* scales;      /* bf16 [mk_w4_scale_count], 16-byte aligned */
+  void* zeros;       /* uint8 [mk_w4_scale_count], or NULL */
+  int64_t K, N;
+  int32_t group, num_experts;
+} mk_w4_weights;
+int64_t mk_w4_packed_bytes(int64_t K, int64_t N, int32_t num_experts);
+int64_t mk_w4_scale_count(int64_t K, int64_t N, int32_t num_experts, int32_t group);
+
+/* Lays out codes uint8 [E, K, N] (the low four bits of each byte), scales bf16
+ * [E, ceil(K / group), N] and zero points uint8 of the scales' shape. */
+typedef struct mk_w4_pack_args {
+  const void* codes;
+  const void* scales;
+  const void* zeros;    /* NULL exactly when out.zeros is */
+  mk_w4_weights out;
+} mk_w4_pack_args;
+int mk_w4_pack(const mk_w4_pack_args* args, void* stream);
+
+/* Codes and scales of bf16 weights [E, K, N], without zero points: scale =
+ * bf16(largest magnitude of the group / 7), code = round(w / scale) + 8 cut to
+ * 0 .. 15 (8 where the scale is 0). */
+typedef struct mk_w4_quantize_args {
+  const void* W;        /* bf16 [E, K, N] */
+  void* codes;          /* uint8 [E, K, N] */
+  void* scales;         /* bf16 [E, ceil(K / group), N] */
+  int64_t K, N;
+  int32_t group, num_experts;
+} mk_w4_quantize_args;
+int mk_w4_quantize(const mk_w4_quantize_args* args, void* stream);
+
+/* C[M, N] = A[M, K] @ w (num_experts 1), fp32 sums, bf16 output.  For few rows
+ * (it reads the weights once per 64 rows); K % 8 == 0, lda % 8 == 0, any M and
+ * N.  An infinity in a row of A makes that row of C NaN. */
+typedef struct mk_gemm_w4_args {
+  const void* A;        /* bf16 [M, lda] */
+  void* C;              /* bf16 [M, ldc] */
+  mk_w4_weights W;
+  int64_t M, lda, ldc;
+} mk_gemm_w4_args;
+int mk_gemm_w4(const mk_gemm_w4_args* args, void* stream);
+
+/* mk_moe_grouped_gemm with 4-bit weights, for the few rows per expert of a
+ * decode batch: out[r] = A[r] @ w[e(r)] (mode 0), or silu(h[:, :I]) * h[:, I:]
+ * of h = A[r] @ w[e(r)] with I = N / 2 a multiple of 16 (mode 1).  rb_expert
+ * names the expert of each 128-row block (blocks that name none are skipped);
+ * only the rb_rows real rows of a block are computed, other rows of out stay as
+ * they are.  gather_pull, n_src_rows, tokens_per_src, devs_per_node and sizes
+ * as in mk_moe_grouped_gemm_args. */
+typedef struct mk_moe_grouped_gemm_w4_args {
+  const void* A;               /* bf16 [R_pad, K], or the token buffer [n_src_rows, K] */
+  mk_w4_weights W;
+  void* out;                   /* bf16 [R_pad, N], mode 1: [R_pad, N / 2] */
+  const int32_t* rb_expert;    /* [R_pad/128] */
+  const int32_t* rb_rows;      /* [R_pad/128], or NULL: every row is real */
+  int64_t R_pad;
+  int32_t mode;
+  const int32_t* gather_pull;  /* [R_pad, 3] or NULL */
+  int64_t n_src_rows;
+  int32_t tokens_per_src, devs_per_node;
+  const int64_t* sizes;        /* device {R, R_pad} or NULL */
+} mk_moe_grouped_gemm_w4_args;
+int mk_moe_grouped_gemm_w4(const mk_moe_grouped_gemm_w4_args* args, void* stream);
+
+/* The local MoE layer with 4-bit expert weights: GEMM1 + SwiGLU (token rows
+ * read through the pull table) -> GEMM2 -> combine, three launches.  act and
+ * y_expert are written on real rows only. */
+typedef struct mk_moe_ffn_w4_args {
+  const void* tokens;           /* bf16 [n_src_rows, H] */
+  const int32_t* pull_indices;  /* [R_pad, 3] */
+  const int32_t* rb_expert;     /* [R_pad/128] */
+  const int32_t* rb_rows;       /* [R_pad/128], or NULL: every row is real */
+  const float* row_weight;      /* [R_pad] */
+  const int32_t* owner_offset;  /* [num_tokens + 1] */
+  const int32_t* slot_to_row;   /* [R] */
+  mk_w4_weights w1;             /* [E, H, 2I] (gate | up) */
+  mk_w4_weights w2;             /* [E, I, H] */
+  void* act;                    /* bf16 [R_pad, I] */
+  void* y_expert;               /* bf16 [R_pad, H] */
+  void* y_out;                  /* [num_tokens, H] fp32 or bf16 */
+  int64_t num_tokens, n_src_rows, R_pad;
+  int32_t tokens_per_src, devs_per_node;
+  int32_t out_dtype;            /* 0 fp32, 1 bf16 */
+  const int64_t* sizes;         /* device {R, R_pad} or NULL */
+} mk_moe_ffn_w4_args;
+int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* K-split workspace size.  When the output tiles do not fill the last round
  * of the persistent grid (tiles % compute workgroups != 0), the GEMM entry
  * points split each tile of that tail round along K over 2-4 workgroups;

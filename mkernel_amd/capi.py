@@ -34,6 +34,17 @@ EXPORTS = (
     "mk_moe_invert_slots",
     "mk_moe_tile_rows",
     "mk_moe_ffn_combine",
+    "mk_moe_route_workspace_bytes",
+    "mk_moe_route",
+    "mk_moe_route_backward",
+    "mk_moe_combine_backward",
+    "mk_w4_packed_bytes",
+    "mk_w4_scale_count",
+    "mk_w4_pack",
+    "mk_w4_quantize",
+    "mk_gemm_w4",
+    "mk_moe_grouped_gemm_w4",
+    "mk_moe_ffn_combine_w4",
     "mk_query_workspace_bytes",
     "mk_probe_mfma_ceiling",
     "mk_probe_threads",
@@ -47,6 +58,7 @@ vp = C.c_void_p
 i64 = C.c_int64
 i32 = C.c_int32
 u32 = C.c_uint32
+f32 = C.c_float
 
 
 class MkError(RuntimeError):
@@ -137,6 +149,57 @@ class MoeFfnArgs(C.Structure):
                 ("sizes", vp)]
 
 
+class MoeRouteArgs(C.Structure):
+    _fields_ = [("logits", vp), ("token_mask", vp), ("topk_ids", vp), ("gates", vp), ("num_tokens", i64), ("ld", i64),
+                ("num_experts", i32), ("topk", i32), ("logits_dtype", i32), ("renorm", i32), ("counts", vp),
+                ("prob_sum", vp), ("tokens", vp), ("loss", vp), ("coef", f32), ("workspace", vp),
+                ("workspace_bytes", i64)]
+
+
+class MoeRouteBackwardArgs(C.Structure):
+    _fields_ = [("logits", vp), ("token_mask", vp), ("topk_ids", vp), ("dgates", vp), ("dloss", vp), ("counts", vp),
+                ("tokens", vp), ("dlogits", vp), ("num_tokens", i64), ("ld", i64), ("ld_out", i64),
+                ("num_experts", i32), ("topk", i32), ("logits_dtype", i32), ("renorm", i32), ("coef", f32)]
+
+
+class MoeCombineBackwardArgs(C.Structure):
+    _fields_ = [("dy", vp), ("y_expert", vp), ("topk_ids", vp), ("row_weight", vp), ("owner_offset", vp),
+                ("slot_to_row", vp), ("rb_rows", vp), ("dy_expert", vp), ("dgates", vp), ("num_tokens", i64),
+                ("H", i64), ("R_pad", i64), ("topk", i32), ("expert_begin", i32), ("n_local", i32), ("dy_dtype", i32),
+                ("sizes", vp)]
+
+
+class W4WeightsC(C.Structure):
+    _fields_ = [("packed", vp), ("scales", vp), ("zeros", vp), ("K", i64), ("N", i64), ("group", i32),
+                ("num_experts", i32)]
+
+
+class W4PackArgs(C.Structure):
+    _fields_ = [("codes", vp), ("scales", vp), ("zeros", vp), ("out", W4WeightsC)]
+
+
+class W4QuantizeArgs(C.Structure):
+    _fields_ = [("W", vp), ("codes", vp), ("scales", vp), ("K", i64), ("N", i64), ("group", i32),
+                ("num_experts", i32)]
+
+
+class GemmW4Args(C.Structure):
+    _fields_ = [("A", vp), ("C", vp), ("W", W4WeightsC), ("M", i64), ("lda", i64), ("ldc", i64)]
+
+
+class MoeGroupedGemmW4Args(C.Structure):
+    _fields_ = [("A", vp), ("W", W4WeightsC), ("out", vp), ("rb_expert", vp), ("rb_rows", vp), ("R_pad", i64),
+                ("mode", i32), ("gather_pull", vp), ("n_src_rows", i64), ("tokens_per_src", i32),
+                ("devs_per_node", i32), ("sizes", vp)]
+
+
+class MoeFfnW4Args(C.Structure):
+    _fields_ = [("tokens", vp), ("pull_indices", vp), ("rb_expert", vp), ("rb_rows", vp), ("row_weight", vp),
+                ("owner_offset", vp), ("slot_to_row", vp), ("w1", W4WeightsC), ("w2", W4WeightsC), ("act", vp),
+                ("y_expert", vp), ("y_out", vp), ("num_tokens", i64), ("n_src_rows", i64), ("R_pad", i64),
+                ("tokens_per_src", i32), ("devs_per_node", i32), ("out_dtype", i32), ("sizes", vp)]
+
+
 _lib = None
 
 
@@ -149,7 +212,9 @@ def lib() -> C.CDLL:
                                "(or python -m mkernel_amd._build) first")
         L = C.CDLL(str(LIB_PATH))
         for name in ("mk_gemm", "mk_ag_gemm", "mk_ag_gemm_noalloc", "mk_gemm_rs", "mk_gemm_ar", "mk_gemm_ar_two_shot", "mk_moe_permute", "mk_moe_grouped_gemm",
-                     "mk_moe_combine", "mk_moe_ffn_combine"):
+                     "mk_moe_combine", "mk_moe_ffn_combine", "mk_moe_route", "mk_moe_route_backward",
+                     "mk_moe_combine_backward", "mk_w4_pack", "mk_w4_quantize", "mk_gemm_w4",
+                     "mk_moe_grouped_gemm_w4", "mk_moe_ffn_combine_w4"):
             getattr(L, name).argtypes = [vp, vp]
             getattr(L, name).restype = C.c_int
         L.mk_moe_index_sizes.argtypes = [vp, i32, i32, i32, i32, i32, C.POINTER(i64), C.POINTER(i64)]
@@ -158,6 +223,12 @@ def lib() -> C.CDLL:
         L.mk_moe_build_indices.restype = C.c_int
         L.mk_moe_index_workspace_bytes.argtypes = [i32, i32, i32]
         L.mk_moe_index_workspace_bytes.restype = i64
+        L.mk_moe_route_workspace_bytes.argtypes = [i64, i32]
+        L.mk_moe_route_workspace_bytes.restype = i64
+        L.mk_w4_packed_bytes.argtypes = [i64, i64, i32]
+        L.mk_w4_packed_bytes.restype = i64
+        L.mk_w4_scale_count.argtypes = [i64, i64, i32, i32]
+        L.mk_w4_scale_count.restype = i64
         L.mk_moe_build_indices_dev.argtypes = [vp, vp]
         L.mk_moe_build_indices_dev.restype = C.c_int
         L.mk_moe_invert_slots.argtypes = [vp, vp, i64, i32, i64, vp, vp, vp]
@@ -202,13 +273,19 @@ def call(fn: str, args: C.Structure, stream: int) -> None:
 # which the library and its launch take 3.8.  Values struct refuses (ctypes
 # wraps integers out of a field's range) go through the Structure, so every
 # call means what it meant.
-_FORMAT = {vp: "P", i64: "q", i32: "i", u32: "I"}
+_FORMAT = {vp: "P", i64: "q", i32: "i", u32: "I", f32: "f"}
 _packers: dict = {}
 _functions: dict = {}
 
 
+def _letters(cls):
+    return "".join(_FORMAT.get(t) or _letters(t) for _, t in cls._fields_)
+
+
 def _packer(cls):
-    fmt = "@" + "".join(_FORMAT[t] for _, t in cls._fields_)
+    # a nested block's values come one by one in their place (its alignment is
+    # that of its first field, its size a multiple of it)
+    fmt = "@" + _letters(cls)
     fmt += "x" * (C.sizeof(cls) - struct.calcsize(fmt))
     pack = _packers[cls] = struct.Struct(fmt).pack
     return pack
@@ -222,7 +299,9 @@ def call_values(fn: str, cls, stream: int, *values) -> None:
     pack = _packers.get(cls) or _packer(cls)
     try:
         args = pack(*values)
-    except struct.error:
+    except struct.error as err:
+        if len(values) != len(cls._fields_):
+            raise ValueError(f"{fn}: {err}") from None
         block = cls(*values)
         args = C.addressof(block)
     rc = f(args, stream or None)

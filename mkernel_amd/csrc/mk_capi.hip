@@ -1046,4 +1046,244 @@ int mk_moe_ffn_combine(const mk_moe_ffn_args* a, void* stream) {
   return mk_moe_combine(&ca, stream);
 }
 
+int64_t mk_moe_route_workspace_bytes(int64_t num_tokens, int32_t num_experts) {
+  if (num_tokens < 0 || num_experts <= 0 || num_experts > mk::kMaxExperts) return -1;
+  return mk::route_workspace_bytes(num_tokens, num_experts);
+}
+
+static int check_route(const char* fn, int64_t T, int64_t ld, int32_t E, int32_t topk, int32_t dtype) {
+  if (T < 0 || E <= 0 || topk <= 0) return fail(MK_EINVAL, "%s: bad sizes", fn);
+  if (dtype != 0 && dtype != 1) return fail(MK_EINVAL, "%s: logits_dtype must be 0 or 1", fn);
+  if (E > mk::kMaxExperts) return fail(MK_ESHAPE, "%s: at most %d experts", fn, mk::kMaxExperts);
+  if (topk > mk::kMaxTopk || topk > E)
+    return fail(MK_ESHAPE, "%s: topk must be at most %d and the number of experts", fn, mk::kMaxTopk);
+  if (ld < E && T > 1) return fail(MK_ESHAPE, "%s: ld must be at least num_experts", fn);
+  if (T > INT32_MAX / topk) return fail(MK_ESHAPE, "%s: too many choices for 32-bit counts", fn);
+  return MK_OK;
+}
+
+int mk_moe_route(const mk_moe_route_args* a, void* stream) {
+  if (!a) return fail(MK_EINVAL, "mk_moe_route: null argument");
+  if (int rc = check_route("mk_moe_route", a->num_tokens, a->ld, a->num_experts, a->topk, a->logits_dtype)) return rc;
+  if (a->num_tokens > 0 && (!a->logits || !a->topk_ids || !a->gates))
+    return fail(MK_EINVAL, "mk_moe_route: null argument");
+  if (a->counts) {
+    if (!a->prob_sum || !a->tokens || !a->loss || !a->workspace)
+      return fail(MK_EINVAL, "mk_moe_route: counts needs prob_sum, tokens, loss and workspace");
+    if (!aligned16(a->workspace) || a->workspace_bytes < mk::route_workspace_bytes(a->num_tokens, a->num_experts))
+      return fail(MK_EINVAL, "mk_moe_route: workspace not 16-byte aligned or smaller than mk_moe_route_workspace_bytes");
+  }
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  mk::RouteKParams p;
+  std::memset(&p, 0, sizeof p);
+  p.logits = a->logits; p.mask = a->token_mask; p.ids = a->topk_ids; p.gates = a->gates;
+  p.T = a->num_tokens; p.ld = a->ld; p.E = a->num_experts; p.k = a->topk;
+  p.bf16 = a->logits_dtype; p.renorm = a->renorm;
+  p.counts = a->counts; p.prob_sum = a->prob_sum; p.tokens = a->tokens; p.loss = a->loss; p.coef = a->coef;
+  hipError_t e = mk::launch_route(p, a->counts ? a->workspace : nullptr, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_route launch");
+}
+
+int mk_moe_route_backward(const mk_moe_route_backward_args* a, void* stream) {
+  if (!a) return fail(MK_EINVAL, "mk_moe_route_backward: null argument");
+  if (int rc = check_route("mk_moe_route_backward", a->num_tokens, a->ld, a->num_experts, a->topk, a->logits_dtype))
+    return rc;
+  if (a->ld_out < a->num_experts && a->num_tokens > 1)
+    return fail(MK_ESHAPE, "mk_moe_route_backward: ld_out must be at least num_experts");
+  if (!a->dgates && !a->counts) return fail(MK_EINVAL, "mk_moe_route_backward: dgates or counts must be set");
+  if (a->counts && !a->tokens) return fail(MK_EINVAL, "mk_moe_route_backward: counts needs tokens");
+  if (a->num_tokens == 0) return MK_OK;
+  if (!a->logits || !a->dlogits || (a->dgates && !a->topk_ids))
+    return fail(MK_EINVAL, "mk_moe_route_backward: null argument");
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  mk::RouteBwdKParams p{a->logits, a->token_mask, a->topk_ids, a->dgates, a->dloss, a->counts, a->tokens, a->dlogits,
+                        a->num_tokens, a->ld, a->ld_out, a->num_experts, a->topk, a->logits_dtype, a->renorm, a->coef};
+  hipError_t e = mk::launch_route_backward(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_route_backward launch");
+}
+
+int mk_moe_combine_backward(const mk_moe_combine_backward_args* a, void* stream) {
+  if (!a) return fail(MK_EINVAL, "mk_moe_combine_backward: null argument");
+  if (a->num_tokens < 0 || a->topk <= 0 || a->expert_begin < 0 || a->n_local <= 0)
+    return fail(MK_EINVAL, "mk_moe_combine_backward: bad sizes");
+  if (a->H <= 0 || a->H % 8) return fail(MK_ESHAPE, "mk_moe_combine_backward: H must be a positive multiple of 8");
+  if (a->R_pad < 0 || a->R_pad % MK_ROW_BLOCK)
+    return fail(MK_ESHAPE, "mk_moe_combine_backward: R_pad must be a multiple of %d", MK_ROW_BLOCK);
+  if (a->topk > mk::kMaxTopk) return fail(MK_ESHAPE, "mk_moe_combine_backward: topk must be at most %d", mk::kMaxTopk);
+  if (a->dy_dtype != 0 && a->dy_dtype != 1) return fail(MK_EINVAL, "mk_moe_combine_backward: dy_dtype must be 0 or 1");
+  if (a->num_tokens > INT32_MAX || a->R_pad > INT32_MAX)
+    return fail(MK_ESHAPE, "mk_moe_combine_backward: too many rows");
+  const bool rows = a->R_pad > 0;
+  if ((a->num_tokens > 0 && (!a->dy || !a->topk_ids || !a->owner_offset || !a->dgates)) ||
+      (rows && (!a->y_expert || !a->row_weight || !a->slot_to_row)) || (rows && a->dy_expert && !a->rb_rows))
+    return fail(MK_EINVAL, "mk_moe_combine_backward: null argument");
+  if (!aligned16(a->dy) || !aligned16(a->y_expert) || !aligned16(a->dy_expert))
+    return fail(MK_EINVAL, "mk_moe_combine_backward: dy, y_expert and dy_expert must be 16-byte aligned");
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  mk::CombineBwdKParams p{a->dy, static_cast<const uint16_t*>(a->y_expert), a->topk_ids, a->row_weight,
+                          a->owner_offset, a->slot_to_row, a->rb_rows, static_cast<uint16_t*>(a->dy_expert),
+                          a->dgates, a->num_tokens, a->H, a->R_pad, a->topk, a->expert_begin, a->n_local,
+                          a->dy_dtype, a->sizes ? a->sizes + 1 : nullptr};
+  hipError_t e = mk::launch_combine_backward(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_combine_backward launch");
+}
+
+// ---------------------------------------------------------------------------
+// 4-bit weights
+// ---------------------------------------------------------------------------
+
+static bool w4_sizes(int64_t K, int64_t N, int32_t E, int32_t group) {
+  return K > 0 && N > 0 && E > 0 && K <= (1LL << 24) && N <= (1LL << 24) && E <= 65536 &&
+         (group == 32 || group == 64 || group == 128);
+}
+
+int64_t mk_w4_packed_bytes(int64_t K, int64_t N, int32_t num_experts) {
+  return w4_sizes(K, N, num_experts, 128) ? 4 * mk::w4_packed_words(K, N, num_experts) : -1;
+}
+
+int64_t mk_w4_scale_count(int64_t K, int64_t N, int32_t num_experts, int32_t group) {
+  return w4_sizes(K, N, num_experts, group) ? mk::w4_scale_count(K, N, num_experts, group) : -1;
+}
+
+static int check_w4(const char* fn, const mk_w4_weights& w) {
+  if (!w.packed || !w.scales) return fail(MK_EINVAL, "%s: null weights", fn);
+  if (w.group != 32 && w.group != 64 && w.group != 128) return fail(MK_EINVAL, "%s: group must be 32, 64 or 128", fn);
+  if (!w4_sizes(w.K, w.N, w.num_experts, w.group)) return fail(MK_ESHAPE, "%s: bad weight sizes", fn);
+  if (!aligned16(w.packed) || !aligned16(w.scales))
+    return fail(MK_EINVAL, "%s: packed weights and scales must be 16-byte aligned", fn);
+  return MK_OK;
+}
+
+int mk_w4_pack(const mk_w4_pack_args* a, void* stream) {
+  if (!a || !a->codes || !a->scales) return fail(MK_EINVAL, "mk_w4_pack: null argument");
+  if (int rc = check_w4("mk_w4_pack", a->out)) return rc;
+  if (!a->zeros != !a->out.zeros) return fail(MK_EINVAL, "mk_w4_pack: zeros given on one side only");
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  hipError_t e = mk::launch_w4_pack(static_cast<const uint8_t*>(a->codes), static_cast<const uint16_t*>(a->scales),
+                                    static_cast<const uint8_t*>(a->zeros), a->out.K, a->out.N, a->out.num_experts,
+                                    a->out.group, static_cast<uint32_t*>(a->out.packed),
+                                    static_cast<uint16_t*>(a->out.scales), static_cast<uint8_t*>(a->out.zeros),
+                                    static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MK_OK : hip_fail(e, "mk_w4_pack launch");
+}
+
+int mk_w4_quantize(const mk_w4_quantize_args* a, void* stream) {
+  if (!a || !a->W || !a->codes || !a->scales) return fail(MK_EINVAL, "mk_w4_quantize: null argument");
+  if (a->group != 32 && a->group != 64 && a->group != 128)
+    return fail(MK_EINVAL, "mk_w4_quantize: group must be 32, 64 or 128");
+  if (!w4_sizes(a->K, a->N, a->num_experts, a->group)) return fail(MK_ESHAPE, "mk_w4_quantize: bad weight sizes");
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  hipError_t e = mk::launch_w4_quantize(static_cast<const uint16_t*>(a->W), a->K, a->N, a->num_experts, a->group,
+                                        static_cast<uint8_t*>(a->codes), static_cast<uint16_t*>(a->scales),
+                                        static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MK_OK : hip_fail(e, "mk_w4_quantize launch");
+}
+
+static mk::W4KParams w4_params(const mk_w4_weights& w, const void* A, void* C, int64_t M, int64_t lda, int64_t ldc) {
+  mk::W4KParams p;
+  std::memset(&p, 0, sizeof p);
+  p.w = {static_cast<const uint32_t*>(w.packed), static_cast<const uint16_t*>(w.scales),
+         static_cast<const uint8_t*>(w.zeros), w.K, w.N, w.group, w.num_experts};
+  p.A = static_cast<const uint16_t*>(A);
+  p.C = static_cast<uint16_t*>(C);
+  p.M = M; p.lda = lda; p.ldc = ldc;
+  p.tile_cols = (int)((w.N + 15) / 16);
+  return p;
+}
+
+int mk_gemm_w4(const mk_gemm_w4_args* a, void* stream) {
+  if (!a) return fail(MK_EINVAL, "mk_gemm_w4: null argument");
+  if (int rc = check_w4("mk_gemm_w4", a->W)) return rc;
+  if (a->W.num_experts != 1) return fail(MK_EINVAL, "mk_gemm_w4: the weights hold %d matrices", a->W.num_experts);
+  if (a->M < 0 || a->M > (1 << 20)) return fail(MK_ESHAPE, "mk_gemm_w4: M must be 0 .. 2^20");
+  if (a->W.K % 8) return fail(MK_ESHAPE, "mk_gemm_w4: K must be a multiple of 8");
+  if (a->lda < a->W.K || a->lda % 8 || a->ldc < a->W.N)
+    return fail(MK_ESHAPE, "mk_gemm_w4: lda must be a multiple of 8 of at least K, ldc at least N");
+  if (a->M == 0) return MK_OK;
+  if (!a->A || !a->C) return fail(MK_EINVAL, "mk_gemm_w4: null argument");
+  if (!aligned16(a->A) || !aligned16(a->C)) return fail(MK_EINVAL, "mk_gemm_w4: A and C must be 16-byte aligned");
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  mk::W4KParams p = w4_params(a->W, a->A, a->C, a->M, a->lda, a->ldc);
+  hipError_t e = mk::launch_w4(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MK_OK : hip_fail(e, "mk_gemm_w4 launch");
+}
+
+// Every check of the expert product, and its parameters.
+static int prepare_grouped_w4(const char* fn, const mk_moe_grouped_gemm_w4_args* a, mk::W4KParams* p) {
+  if (int rc = check_w4(fn, a->W)) return rc;
+  if (a->mode != 0 && a->mode != 1) return fail(MK_EINVAL, "%s: mode must be 0 or 1", fn);
+  if (a->W.K % 8) return fail(MK_ESHAPE, "%s: K must be a multiple of 8", fn);
+  if (a->mode == 1 && a->W.N % 32) return fail(MK_ESHAPE, "%s: N must be a multiple of 32 with SwiGLU", fn);
+  if (a->R_pad < 0 || a->R_pad % MK_ROW_BLOCK || a->R_pad > (1 << 21))
+    return fail(MK_ESHAPE, "%s: R_pad must be a multiple of %d up to 2^21", fn, MK_ROW_BLOCK);
+  if (a->R_pad > 0) {
+    if (!a->A || !a->out || !a->rb_expert) return fail(MK_EINVAL, "%s: null argument", fn);
+    if (!aligned16(a->A) || !aligned16(a->out)) return fail(MK_EINVAL, "%s: A and out must be 16-byte aligned", fn);
+    if (a->gather_pull && (a->n_src_rows <= 0 || a->tokens_per_src <= 0 || a->devs_per_node <= 0))
+      return fail(MK_EINVAL, "%s: gather_pull needs n_src_rows, tokens_per_src and devs_per_node > 0", fn);
+  }
+  const int64_t width = a->mode == 1 ? a->W.N / 2 : a->W.N;
+  *p = w4_params(a->W, a->A, a->out, a->R_pad, a->W.K, width);
+  p->swiglu = a->mode;
+  if (a->mode == 1) p->tile_cols = (int)(width / 16);
+  p->rb_expert = a->rb_expert;
+  p->rb_rows = a->rb_rows;
+  p->gather_pull = a->gather_pull;
+  p->gather_rows = a->n_src_rows;
+  p->gather_tps = a->tokens_per_src;
+  p->gather_devs = a->devs_per_node;
+  p->rows_dev = a->sizes ? a->sizes + 1 : nullptr;
+  return MK_OK;
+}
+
+int mk_moe_grouped_gemm_w4(const mk_moe_grouped_gemm_w4_args* a, void* stream) {
+  if (!a) return fail(MK_EINVAL, "mk_moe_grouped_gemm_w4: null argument");
+  mk::W4KParams p;
+  if (int rc = prepare_grouped_w4("mk_moe_grouped_gemm_w4", a, &p)) return rc;
+  if (a->R_pad == 0) return MK_OK;
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  hipError_t e = mk::launch_w4(p, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_grouped_gemm_w4 launch");
+}
+
+int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* a, void* stream) {
+  const char* fn = "mk_moe_ffn_combine_w4";
+  if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
+  const bool rows = a->R_pad > 0;
+  if ((rows && (!a->tokens || !a->pull_indices || !a->rb_expert || !a->row_weight || !a->slot_to_row || !a->act ||
+                !a->y_expert)) ||
+      (a->num_tokens > 0 && (!a->owner_offset || !a->y_out)))
+    return fail(MK_EINVAL, "%s: null argument", fn);
+  if (a->num_tokens < 0) return fail(MK_ESHAPE, "%s: num_tokens < 0", fn);
+  if (a->out_dtype != 0 && a->out_dtype != 1) return fail(MK_EINVAL, "%s: out_dtype must be 0 or 1", fn);
+  if (a->w1.num_experts != a->w2.num_experts || a->w1.K != a->w2.N || a->w1.N != 2 * a->w2.K)
+    return fail(MK_ESHAPE, "%s: w1 must be [E, H, 2I] and w2 [E, I, H]", fn);
+  // both products are checked before anything is queued
+  mk_moe_grouped_gemm_w4_args g1{a->tokens, a->w1, a->act, a->rb_expert, a->rb_rows, a->R_pad, 1, a->pull_indices,
+                                 a->n_src_rows, a->tokens_per_src, a->devs_per_node, a->sizes};
+  mk_moe_grouped_gemm_w4_args g2{a->act, a->w2, a->y_expert, a->rb_expert, a->rb_rows, a->R_pad, 0, nullptr,
+                                 0, 0, 0, a->sizes};
+  mk::W4KParams p1, p2;
+  if (int rc = prepare_grouped_w4(fn, &g1, &p1)) return rc;
+  if (int rc = prepare_grouped_w4(fn, &g2, &p2)) return rc;
+  mk_moe_combine_args ca{a->y_expert, a->row_weight, a->owner_offset, a->slot_to_row, a->y_out,
+                         a->num_tokens, a->w1.K, a->out_dtype};
+  if (a->num_tokens > 0 && !aligned16(a->y_out)) return fail(MK_EINVAL, "%s: y_out must be 16-byte aligned", fn);
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  if (rows) {
+    hipError_t e = mk::launch_w4(p1, static_cast<hipStream_t>(stream));
+    if (e == hipSuccess) e = mk::launch_w4(p2, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "mk_moe_ffn_combine_w4 launch");
+  }
+  return a->num_tokens > 0 ? mk_moe_combine(&ca, stream) : MK_OK;
+}
+
 }  // extern "C"

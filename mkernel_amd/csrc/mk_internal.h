@@ -14,6 +14,8 @@ enum PermMode : int { kPermNone = 0, kPermArrival = 1, kPermOwnedSpread = 2, kPe
 constexpr int kMaxTilesM = 512;
 constexpr int kMaxSplitListTiles = 4096;  // K-split with a permuted tile order: at most this many tiles
 constexpr int kMaxRounds = 64;   // cooperative staging between rounds: at most this many rounds
+constexpr int kMaxTopk = 32;     // choices per token of the router and of the combine's gradient
+constexpr int kMaxExperts = 1024; // experts of the router
 constexpr int kPieces = 16;  // cooperative staging: pieces per 128-row block
 
 struct GemmKParams {
@@ -160,6 +162,95 @@ struct CombineKParams {
 };
 hipError_t launch_combine(const CombineKParams& p, hipStream_t stream);
 hipError_t launch_tile_rows(const int* pull, int64_t R_pad, int* rb_rows, hipStream_t stream);
+
+// Gradient of the combine (mk_moe.hip).
+struct CombineBwdKParams {
+  const void* dy;
+  const uint16_t* y_expert;
+  const int* ids;
+  const float* row_weight;
+  const int* owner_offset;
+  const int* slot_to_row;
+  const int* rb_rows;
+  uint16_t* dy_expert;      // null: not computed
+  float* dgates;
+  int64_t T, H, R_pad;
+  int k, e0, n_local;
+  int dy_dtype;
+  const int64_t* rows_dev;
+};
+hipError_t launch_combine_backward(const CombineBwdKParams& p, hipStream_t stream);
+
+// Router (mk_route.hip).
+struct RouteKParams {
+  const void* logits;
+  const uint8_t* mask;
+  int* ids;
+  float* gates;
+  int64_t T, ld;
+  int E, k, bf16, renorm;
+  // balance sums (part_sum null: none)
+  int* counts;
+  float* prob_sum;
+  int* tokens;
+  float* loss;
+  float coef;
+  double* shares;      // an expert group's share of the loss, per workgroup of the second kernel
+  uint32_t* ticket;
+  float* part_sum;     // [workgroups][E]
+  int* part_cnt;       // [workgroups][E]
+  int* part_live;      // [workgroups]
+};
+struct RouteBwdKParams {
+  const void* logits;
+  const uint8_t* mask;
+  const int* ids;
+  const float* dgates;
+  const float* dloss;
+  const int* counts;
+  const int* tokens;
+  void* dlogits;
+  int64_t T, ld, ld_out;
+  int E, k, bf16, renorm;
+  float coef;
+};
+int64_t route_workspace_bytes(int64_t T, int E);
+// ws null: no balance sums
+hipError_t launch_route(RouteKParams p, void* ws, hipStream_t stream);
+hipError_t launch_route_backward(const RouteBwdKParams& p, hipStream_t stream);
+
+// Products with 4-bit weights (mk_w4.hip).
+struct W4Weights {
+  const uint32_t* packed;   // [E][tiles][blocks][64 lanes][4]
+  const uint16_t* scales;   // [E][tiles][groups][16]
+  const uint8_t* zeros;     // as scales, or null: 8
+  int64_t K, N;
+  int group, E;
+};
+struct W4KParams {
+  W4Weights w;
+  const uint16_t* A;
+  uint16_t* C;
+  int64_t lda, ldc, M;      // M: rows of A (dense) or of the tables
+  int tile_cols;            // output column tiles of 16
+  int swiglu;
+  // experts (rb_expert null: one dense product)
+  const int* rb_expert;
+  const int* rb_rows;
+  const int* gather_pull;
+  int64_t gather_rows;
+  int gather_tps, gather_devs;
+  const int64_t* rows_dev;
+};
+int64_t w4_packed_words(int64_t K, int64_t N, int64_t E);
+int64_t w4_scale_count(int64_t K, int64_t N, int64_t E, int group);
+hipError_t launch_w4(const W4KParams& p, hipStream_t stream);
+hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int64_t K, int64_t N,
+                          int64_t E, int group, uint32_t* packed, uint16_t* packed_scales, uint8_t* packed_zeros,
+                          hipStream_t stream);
+hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E, int group, uint8_t* codes,
+                              uint16_t* scales, hipStream_t stream);
+
 int64_t index_workspace_bytes(int T, int topk, int n_local);
 hipError_t launch_mfma_ceiling(int64_t iters, int n_wg, uint32_t seed, float* sink, uint64_t* clocks,
                                hipStream_t stream);

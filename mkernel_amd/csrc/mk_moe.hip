@@ -122,6 +122,99 @@ hipError_t launch_combine(const CombineKParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// Gradient of the combine: workgroup t < T has token t's, one that follows the
+// padding rows of a row block.
+//   dy_expert[r] = row_weight[r] * dy[t]            (one bf16 rounding)
+//   dgates[t, j] = sum_c dy[t, c] * y_expert[r, c]  (fp32), r the row of (t, j)
+// The row of (t, j) is found as the index build gave it out: the token's local
+// choices, ordered by (expert, j), have its slots in turn.
+template <class T>
+__global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineBwdKParams p) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  const int64_t R = p.rows_dev ? min(p.R_pad, *p.rows_dev) : p.R_pad;
+  const int64_t vec = p.H / 8;
+  if (blockIdx.x >= p.T) {
+    const int64_t b = blockIdx.x - p.T;
+    if (b * kFlagRows >= R) return;
+    const int real = min(max(p.rb_rows[b], 0), kFlagRows);
+    uint4* dst = reinterpret_cast<uint4*>(p.dy_expert + (b * kFlagRows + real) * p.H);
+    const uint4 z = {0u, 0u, 0u, 0u};
+    for (int64_t c = threadIdx.x; c < (kFlagRows - real) * vec; c += kThreads) dst[c] = z;
+    return;
+  }
+  const int64_t t = blockIdx.x;
+  __shared__ int rows[kMaxTopk];
+  __shared__ float part[kThreads / 64];
+  if (threadIdx.x < (unsigned)p.k) {
+    const int j = threadIdx.x, e = p.ids[t * p.k + j] - p.e0;
+    int row = -1;
+    if (e >= 0 && e < p.n_local) {
+      int slot = p.owner_offset[t];
+      for (int i = 0; i < p.k; ++i) {
+        const int o = p.ids[t * p.k + i] - p.e0;
+        slot += o >= 0 && o < p.n_local && (o < e || (o == e && i < j));
+      }
+      if (slot < p.owner_offset[t + 1]) row = p.slot_to_row[slot];
+      if (row >= R) row = -1;
+    }
+    rows[j] = row;
+  }
+  __syncthreads();
+  const T* dy = static_cast<const T*>(p.dy) + t * p.H;
+  for (int j = 0; j < p.k; ++j) {
+    const int row = rows[j];
+    float dot = 0.f;
+    if (row >= 0) {
+      const float w = p.row_weight[row];
+      for (int64_t c = threadIdx.x; c < vec; c += kThreads) {
+        float d[8];
+        if constexpr (sizeof(T) == 2) {
+          const words v = *reinterpret_cast<const words*>(dy + 8 * c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            d[2 * i] = bf16_lo(v[i]);
+            d[2 * i + 1] = bf16_hi(v[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(dy + 8 * c + 4 * i);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) d[4 * i + b] = v[b];
+          }
+        }
+        const words y = *reinterpret_cast<const words*>(p.y_expert + row * p.H + 8 * c);
+        words o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          dot += d[2 * i] * bf16_lo(y[i]);
+          dot += d[2 * i + 1] * bf16_hi(y[i]);
+          o[i] = pack_bf16x2(w * d[2 * i], w * d[2 * i + 1]);
+        }
+        if (p.dy_expert) *reinterpret_cast<words*>(p.dy_expert + row * p.H + 8 * c) = o;
+      }
+#pragma unroll
+      for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d, 64);
+      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
+      __syncthreads();
+      dot = 0.f;
+      for (int w2 = 0; w2 < kThreads / 64; ++w2) dot += part[w2];
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) p.dgates[t * p.k + j] = dot;
+  }
+}
+
+hipError_t launch_combine_backward(const CombineBwdKParams& p, hipStream_t stream) {
+  const int64_t blocks = p.T + (p.dy_expert ? p.R_pad / kFlagRows : 0);
+  if (blocks == 0) return hipSuccess;
+  if (p.dy_dtype == 0)
+    hipLaunchKernelGGL(combine_backward_kernel<float>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL(combine_backward_kernel<uint16_t>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
 // One workgroup per 128-row block: count rows with a real source token.
 __global__ __launch_bounds__(128) void tile_rows_kernel(const int* pull, int64_t R_pad, int* rb_rows) {
   const int64_t r = (int64_t)blockIdx.x * 128 + threadIdx.x;

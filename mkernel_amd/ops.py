@@ -6,14 +6,18 @@ Shape/argument problems raise :class:`mkernel_amd.capi.MkError`.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
+import math
+from typing import NamedTuple
 
 import numpy as np
 import torch
 
 from . import capi
-from .capi import (AgGemmArgs, GemmAr2Args, GemmArArgs, GemmArgs, GemmRsArgs, MoeCombineArgs, MoeFfnArgs, MoeGroupedGemmArgs,
-                   MoeIndex, MoeIndexDevArgs, MoePermuteArgs)
+from .capi import (AgGemmArgs, GemmAr2Args, GemmArArgs, GemmArgs, GemmRsArgs, GemmW4Args, MoeCombineArgs,
+                   MoeCombineBackwardArgs, MoeFfnArgs, MoeFfnW4Args, MoeGroupedGemmArgs, MoeGroupedGemmW4Args, MoeIndex,
+                   MoeIndexDevArgs, MoePermuteArgs, MoeRouteArgs, MoeRouteBackwardArgs, W4PackArgs, W4QuantizeArgs)
 
 
 def _ptr(t: torch.Tensor | None) -> int:
@@ -358,6 +362,363 @@ def moe_ffn_combine(tokens, pull, row_weight, owner_offset, slot_to_row, w1, w2,
                      tokens.shape[0], R_pad, H, I2 // 2, E, tps, devs_per_node, od, num_cus,
                      *_ws(split_ws, tokens.device), int(fuse_dispatch), tile_n, _ptr(sizes))
     return y_out
+
+
+# ------------------------------------------------------------------- router
+def _tensor(t, name: str, dtypes, shape=None, dim=None, rows=False, device=None) -> None:
+    """Checks one device tensor: type, shape (None: any size) and layout
+    (contiguous, or with `rows` a matrix whose rows are), on `device`."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor of type {' or '.join(str(d)[6:] for d in dtypes)}")
+    if dim is not None and t.dim() != dim:
+        raise ValueError(f"{name} must have {dim} dimensions")
+    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape))):
+        raise ValueError(f"{name} must have shape {tuple('any' if w is None else w for w in shape)}, not {tuple(t.shape)}")
+    if rows:
+        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError(f"{name} must be a matrix with contiguous rows that do not overlap")
+    elif not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride; of a matrix of one row, its width."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _on(device):
+    """The device as the current one for a launch, where it is not that already."""
+    return contextlib.nullcontext() if device.index == _device_index() else torch.cuda.device(device)
+
+
+_LOGITS = (torch.float32, torch.bfloat16)
+_F32, _BF16, _I32, _U8 = (torch.float32,), (torch.bfloat16,), (torch.int32,), (torch.uint8,)
+
+
+def _route_inputs(logits, topk, token_mask):
+    _tensor(logits, "logits", _LOGITS, rows=True)
+    if not 1 <= topk <= logits.shape[1]:
+        raise ValueError(f"topk must be 1 .. {logits.shape[1]}")
+    if token_mask is not None:
+        _tensor(token_mask, "token_mask", (torch.bool, torch.uint8), (logits.shape[0],), device=logits.device)
+
+
+def _coef(coef) -> float:
+    coef = float(coef)
+    if not math.isfinite(C.c_float(coef).value):
+        raise ValueError("coef must be finite in fp32")
+    return coef
+
+
+def moe_route(logits: torch.Tensor, topk: int, renorm: bool = True, token_mask: torch.Tensor | None = None) -> tuple:
+    """Top-k choice and gates of the router (mk_moe_route): (ids int32, gates
+    float32), both [T, topk], as moe_build_indices_dev takes them.  logits:
+    float32 or bfloat16 [T, E], rows contiguous (columns of a wider matrix are
+    fine).  Choices come in falling order, ties to the lowest expert; -inf is
+    never chosen (id -1, gate 0 in the places left).  gates: softmax over the
+    chosen logits, or with renorm=False the chosen entries of the softmax over
+    all.  token_mask (bool or uint8 [T]): tokens where it is 0 get ids -1."""
+    return _route(logits, topk, renorm, token_mask, None)[:2]
+
+
+def moe_route_balance(logits: torch.Tensor, topk: int, coef: float, renorm: bool = True,
+                      token_mask: torch.Tensor | None = None) -> dict:
+    """moe_route for training: ids and gates, and of the same pass "counts"
+    (int32 [E], choices of each expert), "prob_sum" (float32 [E], sum of its
+    probabilities over the tokens), "tokens" (int32 [1], tokens that count) and
+    "loss" (float32 [1]) = coef * E / (topk * tokens^2) * sum(counts * prob_sum).
+    Bitwise repeatable.  moe_route_backward has the gradient."""
+    ids, gates, loss, counts, prob_sum, tokens = _route(logits, topk, renorm, token_mask, _coef(coef))
+    return {"ids": ids, "gates": gates, "loss": loss, "counts": counts, "prob_sum": prob_sum, "tokens": tokens}
+
+
+def _route(logits, topk, renorm, token_mask, coef):
+    _route_inputs(logits, topk, token_mask)
+    T, E = logits.shape
+    dev = logits.device
+    with _on(dev):
+        ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
+        gates = torch.empty((T, topk), dtype=torch.float32, device=dev)
+        if coef is None:
+            extra, balance = (), (0, 0, 0, 0, 0.0, 0, 0)
+        else:
+            # loss, prob_sum | counts, tokens | workspace (made anew: it holds nothing between calls)
+            f = torch.empty(1 + E, dtype=torch.float32, device=dev)
+            i = torch.empty(1 + E, dtype=torch.int32, device=dev)
+            n = int(capi.lib().mk_moe_route_workspace_bytes(T, E))
+            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+            extra = (f[:1], i[:E], f[1:], i[E:])
+            balance = (i.data_ptr(), f.data_ptr() + 4, i.data_ptr() + 4 * E, f.data_ptr(), coef, ws.data_ptr(), n)
+        capi.call_values("mk_moe_route", MoeRouteArgs, _stream(), logits.data_ptr(), _ptr(token_mask), ids.data_ptr(),
+                         gates.data_ptr(), T, _ld(logits), E, topk, int(logits.dtype == torch.bfloat16), int(renorm),
+                         *balance)
+    return (ids, gates, *extra)
+
+
+def moe_route_backward(logits: torch.Tensor, ids: torch.Tensor, dgates: torch.Tensor | None = None,
+                       dloss: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                       tokens: torch.Tensor | None = None, coef: float = 0.0, renorm: bool = True,
+                       token_mask: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of the logits (mk_moe_route_backward), in their type: the
+    gates' part from dgates (float32 [T, topk]), the balance loss's part from
+    counts and tokens (as moe_route_balance gave them, or summed over ranks),
+    coef and dloss (one float32 on the device; None: 1).  Either part may be
+    left out.  ids, renorm and token_mask as in the forward call.  out: where
+    to write it; the logits themselves may be given."""
+    if ids is None or not isinstance(ids, torch.Tensor) or ids.dim() != 2:
+        raise ValueError("ids must be an int32 device tensor [T, topk]")
+    topk = ids.shape[1]
+    _route_inputs(logits, topk, token_mask)
+    T, E = logits.shape
+    dev = logits.device
+    _tensor(ids, "ids", _I32, (T, topk), device=dev)
+    if dgates is None and counts is None:
+        raise ValueError("dgates or counts must be given")
+    if dgates is not None:
+        _tensor(dgates, "dgates", _F32, (T, topk), device=dev)
+    if counts is not None:
+        _tensor(counts, "counts", _I32, (E,), device=dev)
+        if tokens is None:
+            raise ValueError("counts needs tokens")
+        _tensor(tokens, "tokens", _I32, device=dev)
+        if tokens.numel() != 1:
+            raise ValueError("tokens must hold one number")
+    if dloss is not None:
+        _tensor(dloss, "dloss", _F32, device=dev)
+        if dloss.numel() != 1:
+            raise ValueError("dloss must hold one number")
+    if out is not None:
+        _tensor(out, "out", (logits.dtype,), (T, E), rows=True, device=dev)
+    with _on(dev):
+        if out is None:
+            out = torch.empty((T, E), dtype=logits.dtype, device=dev)
+        capi.call_values("mk_moe_route_backward", MoeRouteBackwardArgs, _stream(), logits.data_ptr(), _ptr(token_mask),
+                         ids.data_ptr(), _ptr(dgates), _ptr(dloss), _ptr(counts), _ptr(tokens), out.data_ptr(), T,
+                         _ld(logits), _ld(out), E, topk, int(logits.dtype == torch.bfloat16), int(renorm), _coef(coef))
+    return out
+
+
+def moe_combine_backward(dy: torch.Tensor, y_expert: torch.Tensor, ids: torch.Tensor, row_weight: torch.Tensor,
+                         owner_offset: torch.Tensor, slot_to_row: torch.Tensor, rb_rows: torch.Tensor, e0: int,
+                         n_local: int, dy_expert: torch.Tensor | None = None, dgates: torch.Tensor | None = None,
+                         sizes: torch.Tensor | None = None) -> tuple:
+    """Gradient of moe_combine (mk_moe_combine_backward): (dy_expert bf16
+    [R_pad, H], dgates float32 [T, topk]) from dy ([T, H], the type of the
+    combine's output), with the tables of moe_build_indices(_dev)(ids, ...,
+    e0, n_local) at row_block 128.  dgates is 0 for experts of other ranks.
+    With sizes (moe_build_indices_dev(sync=False)) the rows are a capacity and
+    those behind the routed ones are left as they are."""
+    _tensor(dy, "dy", _LOGITS, dim=2)
+    dev = dy.device
+    T, H = dy.shape
+    _tensor(y_expert, "y_expert", _BF16, (None, H), device=dev)
+    R_pad = y_expert.shape[0]
+    _tensor(ids, "ids", _I32, (T, None), device=dev)
+    k = ids.shape[1]
+    _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)
+    _tensor(owner_offset, "owner_offset", _I32, (T + 1,), device=dev)
+    _tensor(slot_to_row, "slot_to_row", _I32, dim=1, device=dev)
+    _tensor(rb_rows, "rb_rows", _I32, dim=1, device=dev)
+    if row_weight.shape[0] < R_pad or rb_rows.shape[0] * capi.ROW_BLOCK < R_pad:
+        raise ValueError("row_weight and rb_rows must cover the rows of y_expert")
+    if sizes is not None:
+        _tensor(sizes, "sizes", (torch.int64,), (2,), device=dev)
+    if dy_expert is not None:
+        _tensor(dy_expert, "dy_expert", _BF16, (R_pad, H), device=dev)
+    if dgates is not None:
+        _tensor(dgates, "dgates", _F32, (T, k), device=dev)
+    with _on(dev):
+        if dy_expert is None:
+            dy_expert = torch.empty((R_pad, H), dtype=torch.bfloat16, device=dev)
+        if dgates is None:
+            dgates = torch.empty((T, k), dtype=torch.float32, device=dev)
+        capi.call_values("mk_moe_combine_backward", MoeCombineBackwardArgs, _stream(), dy.data_ptr(),
+                         y_expert.data_ptr(), ids.data_ptr(), row_weight.data_ptr(), owner_offset.data_ptr(),
+                         slot_to_row.data_ptr(), rb_rows.data_ptr(), dy_expert.data_ptr(), dgates.data_ptr(), T, H,
+                         R_pad, k, e0, n_local, int(dy.dtype == torch.bfloat16), _ptr(sizes))
+    return dy_expert, dgates
+
+
+# ------------------------------------------------------------------- 4-bit weights
+class W4Weights(NamedTuple):
+    """4-bit weights laid out by w4_pack: E matrices [K, N], values
+    (code - zero) * scale per `group` rows of K."""
+    packed: torch.Tensor
+    scales: torch.Tensor
+    zeros: torch.Tensor | None
+    K: int
+    N: int
+    group: int
+    experts: int
+
+    def _values(self) -> tuple:
+        return (self.packed.data_ptr(), self.scales.data_ptr(), _ptr(self.zeros), self.K, self.N, self.group,
+                self.experts)
+
+
+def _groups(K: int, group: int) -> int:
+    if group not in (32, 64, 128):
+        raise ValueError("group must be 32, 64 or 128")
+    return (K + group - 1) // group
+
+
+def _matrices(t, name, dtypes):
+    _tensor(t, name, dtypes)
+    if t.dim() not in (2, 3) or 0 in t.shape:
+        raise ValueError(f"{name} must be [K, N] or [E, K, N], not empty")
+    return (1, *t.shape) if t.dim() == 2 else tuple(t.shape)
+
+
+def w4_pack(codes: torch.Tensor, scales: torch.Tensor, group: int, zeros: torch.Tensor | None = None) -> W4Weights:
+    """Lays 4-bit weights out for gemm_w4 and the expert products (mk_w4_pack;
+    once, when a model is loaded).  codes: uint8 [K, N] or [E, K, N], one code
+    0 .. 15 a byte; scales: bf16 [.., ceil(K / group), N]; zeros: uint8 of the
+    scales' shape, or None (8)."""
+    E, K, N = _matrices(codes, "codes", _U8)
+    shape = (*codes.shape[:-2], _groups(K, group), N)
+    _tensor(scales, "scales", _BF16, shape, device=codes.device)
+    if zeros is not None:
+        _tensor(zeros, "zeros", _U8, shape, device=codes.device)
+    L = capi.lib()
+    dev = codes.device
+    words, count = int(L.mk_w4_packed_bytes(K, N, E)), int(L.mk_w4_scale_count(K, N, E, group))
+    if words < 0 or count < 0:
+        raise ValueError(f"weights of {E} x {K} x {N} are too large")
+    with _on(dev):
+        w = W4Weights(torch.empty(words, dtype=torch.uint8, device=dev),
+                      torch.empty(count, dtype=torch.bfloat16, device=dev),
+                      None if zeros is None else torch.empty(count, dtype=torch.uint8, device=dev), K, N, group, E)
+        capi.call_values("mk_w4_pack", W4PackArgs, _stream(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros),
+                         *w._values())
+    return w
+
+
+def w4_quantize(W: torch.Tensor, group: int) -> tuple:
+    """(codes, scales) of bf16 weights [K, N] or [E, K, N] for w4_pack
+    (mk_w4_quantize): per group scale = bf16(largest magnitude / 7), code =
+    round(w / scale) + 8."""
+    E, K, N = _matrices(W, "W", _BF16)
+    dev = W.device
+    with _on(dev):
+        codes = torch.empty(W.shape, dtype=torch.uint8, device=dev)
+        scales = torch.empty((*W.shape[:-2], _groups(K, group), N), dtype=torch.bfloat16, device=dev)
+        capi.call_values("mk_w4_quantize", W4QuantizeArgs, _stream(), W.data_ptr(), codes.data_ptr(),
+                         scales.data_ptr(), K, N, group, E)
+    return codes, scales
+
+
+def _w4(W, name, device, experts=None) -> None:
+    if not isinstance(W, W4Weights):
+        raise ValueError(f"{name} must be W4Weights (w4_pack)")
+    if W.packed.device != device:
+        raise ValueError(f"{name} is on {W.packed.device}, not on {device}")
+    if experts is not None and W.experts != experts:
+        raise ValueError(f"{name} holds {W.experts} matrices, not {experts}")
+
+
+def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> torch.Tensor:
+    """C = A @ w for few rows (mk_gemm_w4): A bf16 [M, K], w 4-bit weights of
+    w4_pack; fp32 sums of exact products, scaled group by group in fp32, bf16
+    out.  K a multiple of 8, any M and N; rows of A (a multiple of 8 elements
+    apart) and of out need only be contiguous each.  The weights are read once
+    per 64 rows: from a few hundred rows on, gemm is faster."""
+    _tensor(A, "A", _BF16, rows=True)
+    dev = A.device
+    _w4(W, "W", dev, 1)
+    M, K = A.shape
+    if K != W.K:
+        raise ValueError(f"A has {K} columns, the weights {W.K} rows")
+    if out is not None:
+        _tensor(out, "out", _BF16, (M, W.N), rows=True, device=dev)
+    with _on(dev):
+        if out is None:
+            out = torch.empty((M, W.N), dtype=torch.bfloat16, device=dev)
+        capi.call_values("mk_gemm_w4", GemmW4Args, _stream(), A.data_ptr(), out.data_ptr(), *W._values(), M, _ld(A),
+                         _ld(out))
+    return out
+
+
+def _block_tables(rb_expert, rb_rows, R_pad, sizes, dev):
+    if R_pad % capi.ROW_BLOCK:
+        raise ValueError(f"the tables' rows must be a multiple of {capi.ROW_BLOCK}")
+    _tensor(rb_expert, "rb_expert", _I32, dim=1, device=dev)
+    if rb_rows is not None:
+        _tensor(rb_rows, "rb_rows", _I32, dim=1, device=dev)
+    for t in (rb_expert, rb_rows):
+        if t is not None and t.shape[0] * capi.ROW_BLOCK < R_pad:
+            raise ValueError("rb_expert and rb_rows must cover the rows")
+    if sizes is not None:
+        _tensor(sizes, "sizes", (torch.int64,), (2,), device=dev)
+
+
+def moe_grouped_gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor, rb_expert: torch.Tensor,
+                        rb_rows: torch.Tensor | None = None, mode: int = 0,
+                        gather_pull: torch.Tensor | None = None, tokens_per_src: int | None = None,
+                        devs_per_node: int = 1, sizes: torch.Tensor | None = None) -> torch.Tensor:
+    """moe_grouped_gemm with 4-bit expert weights (mk_moe_grouped_gemm_w4), for
+    the few rows per expert of a decode batch.  mode 0: out = A @ w[e]; mode 1:
+    out = silu(h[:, :I]) * h[:, I:], h = A @ w[e].  Only the real rows (rb_rows)
+    of the 128-row blocks are computed and written."""
+    _tensor(A, "A", _BF16, dim=2)
+    dev = A.device
+    _w4(W, "W", dev)
+    if mode not in (0, 1):
+        raise ValueError("mode must be 0 or 1")
+    R_pad = A.shape[0] if gather_pull is None else gather_pull.shape[0]
+    if A.shape[1] != W.K:
+        raise ValueError(f"A has {A.shape[1]} columns, the weights {W.K} rows")
+    _tensor(out, "out", _BF16, (R_pad, W.N // 2 if mode else W.N), device=dev)
+    _block_tables(rb_expert, rb_rows, R_pad, sizes, dev)
+    if gather_pull is not None:
+        _tensor(gather_pull, "gather_pull", _I32, (R_pad, 3), device=dev)
+    tps = A.shape[0] if tokens_per_src is None else tokens_per_src
+    with _on(dev):
+        capi.call_values("mk_moe_grouped_gemm_w4", MoeGroupedGemmW4Args, _stream(), A.data_ptr(), *W._values(),
+                         out.data_ptr(), rb_expert.data_ptr(), _ptr(rb_rows), R_pad, mode, _ptr(gather_pull),
+                         A.shape[0], tps, devs_per_node, _ptr(sizes))
+    return out
+
+
+def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: torch.Tensor, owner_offset: torch.Tensor,
+                       slot_to_row: torch.Tensor, w1: W4Weights, w2: W4Weights, act: torch.Tensor,
+                       y_expert: torch.Tensor, y_out: torch.Tensor, rb_expert: torch.Tensor,
+                       rb_rows: torch.Tensor | None = None, tokens_per_src: int | None = None, devs_per_node: int = 1,
+                       sizes: torch.Tensor | None = None) -> torch.Tensor:
+    """moe_ffn_combine with 4-bit expert weights w1 [E, H, 2I] and w2 [E, I, H]
+    (mk_moe_ffn_combine_w4), for decode batches: grouped GEMM1 + SwiGLU (reads
+    the tokens through the pull table) -> grouped GEMM2 -> combine.  act
+    [R_pad, I] and y_expert [R_pad, H] are scratch; sizes as in
+    moe_ffn_combine."""
+    _tensor(tokens, "tokens", _BF16, dim=2)
+    dev = tokens.device
+    _w4(w1, "w1", dev)
+    _w4(w2, "w2", dev, w1.experts)
+    H, I = w1.K, w2.K
+    if w1.N != 2 * I or w2.N != H or tokens.shape[1] != H:
+        raise ValueError("w1 must be [E, H, 2I], w2 [E, I, H] and tokens [n, H]")
+    _tensor(pull, "pull", _I32, (None, 3), device=dev)
+    R_pad = pull.shape[0]
+    _tensor(act, "act", _BF16, (R_pad, I), device=dev)
+    _tensor(y_expert, "y_expert", _BF16, (R_pad, H), device=dev)
+    _tensor(y_out, "y_out", _LOGITS, (None, H), device=dev)
+    T = y_out.shape[0]
+    _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)
+    _tensor(owner_offset, "owner_offset", _I32, (T + 1,), device=dev)
+    _tensor(slot_to_row, "slot_to_row", _I32, dim=1, device=dev)
+    if row_weight.shape[0] < R_pad:
+        raise ValueError("row_weight must cover the rows")
+    _block_tables(rb_expert, rb_rows, R_pad, sizes, dev)
+    tps = tokens.shape[0] if tokens_per_src is None else tokens_per_src
+    with _on(dev):
+        capi.call_values("mk_moe_ffn_combine_w4", MoeFfnW4Args, _stream(), tokens.data_ptr(), pull.data_ptr(),
+                         rb_expert.data_ptr(), _ptr(rb_rows), row_weight.data_ptr(), owner_offset.data_ptr(),
+                         slot_to_row.data_ptr(), *w1._values(), *w2._values(), act.data_ptr(), y_expert.data_ptr(),
+                         y_out.data_ptr(), T, tokens.shape[0], R_pad, tps, devs_per_node,
+                         int(y_out.dtype == torch.bfloat16), _ptr(sizes))
+    return y_out
+
 
 
 def probe_mfma_ceiling(iters: int = 20000, num_wg: int = 0, reps: int = 3) -> dict:

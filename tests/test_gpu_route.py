@@ -1,0 +1,370 @@
+"""The router (choices, gates, counts, balance loss), its gradient and the
+combine's gradient, against plain 64-bit forms.
+
+Tolerances (u = 2^-24, half an fp32 step): an exponential of x - max carries
+|x - max| u from the difference's rounding, at most 32 u here (logits within 32
+of the maximum), 4 u of its own; a sum of at most 1024 positive terms, 16 per
+lane and 6 steps across, 22 u; quotient 1 u: below 64 u = 2^-18 for a
+probability and for a gate.  A gradient adds at most as much once more per
+product and sum, relative to the sum of its terms' magnitudes: 2^-17.  Sums
+over tokens add their own roundings, at most (T / 4096 + 8) u in a lane."""
+import numpy as np
+import pytest
+import torch
+
+from mkernel_amd import ops, workloads as wl
+
+pytestmark = pytest.mark.gpu
+INF, NAN = float("inf"), float("nan")
+D = torch.float64
+
+
+def _say(*a):
+    print("[case]", *a, flush=True)
+
+
+def _logits(T, E, dtype, seed, spread=4.0, pad=0):
+    g = torch.Generator().manual_seed(seed)
+    wide = torch.randn((T, E + pad), generator=g).mul_(spread).clamp_(-14, 14).to(dtype)
+    return wide
+
+
+def _choose(x, k):
+    """The k largest, ties to the lowest index, NaN largest; -1 where only -inf is left.  numpy, on the host."""
+    x = x.double().numpy()
+    key = np.where(np.isnan(x), np.inf, x)
+    ids = np.full((x.shape[0], k), -1, dtype=np.int64)
+    for t in range(x.shape[0]):
+        order = sorted(range(x.shape[1]), key=lambda e: (not np.isnan(x[t, e]), -key[t, e], e))
+        n = 0
+        for e in order[:k]:
+            if x[t, e] != -np.inf:
+                ids[t, n] = e
+                n += 1
+    return torch.from_numpy(ids)
+
+
+def _softmax(x):
+    m = x.amax(1, keepdim=True)
+    e = torch.where(x == -INF, torch.zeros_like(x), torch.exp(x - torch.where(m == -INF, torch.zeros_like(m), m)))
+    return e / torch.where(m == -INF, torch.ones_like(m), e.sum(1, keepdim=True))
+
+
+def _reference(x, k, renorm, mask, coef):
+    """ids, gates, p, counts, n, loss in 64 bits."""
+    x = x.to(D).clone()
+    if mask is not None:
+        x[~mask.bool()] = -INF
+    ids = _choose(x, k)
+    p = _softmax(x)
+    on = ids >= 0
+    g = torch.where(on, p.gather(1, ids.clamp(min=0)), torch.zeros(1, dtype=D))
+    if renorm:
+        g = torch.where(on, g / torch.where(on.any(1, keepdim=True), g.sum(1, keepdim=True), torch.ones(1, dtype=D)), g)
+    E = x.shape[1]
+    counts = torch.bincount(ids[on], minlength=E)
+    n = int(on.any(1).sum())
+    loss = coef * E / (k * max(n, 1) ** 2) * (counts.to(D) * p.sum(0)).sum()
+    return ids, g, p, counts, n, loss
+
+
+SIZES = [(1, 1, 1, 0), (1, 256, 8, 0), (3, 7, 7, 0), (5, 64, 6, 192), (64, 256, 8, 0), (17, 65, 1, 3), (130, 128, 32, 0),
+         (129, 60, 4, 5), (33, 255, 9, 1), (40, 257, 16, 7), (20, 512, 10, 0), (9, 1000, 32, 24), (7, 1024, 8, 0),
+         (1027, 16, 2, 0), (4099, 32, 4, 0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("T,E,k,pad", SIZES)
+def test_route_and_balance(dev, T, E, k, pad, renorm, dtype):
+    _say("route", T, E, k, pad, renorm, dtype)
+    wide = _logits(T, E, dtype, 3 * T + E, pad=pad)
+    x = wide[:, :E]
+    g = torch.Generator().manual_seed(1)
+    for mask in (None, torch.rand(T, generator=g) < 0.7):
+        if mask is not None:
+            x = x.clone()
+            x[~mask] = NAN
+        ids, gates, p, counts, n, loss = _reference(x, k, renorm, mask, 0.25)
+        d = wide.to(dev)[:, :E] if mask is None else torch.cat([x, x[:, :pad]], 1).to(dev)[:, :E]
+        dm = None if mask is None else mask.to(dev)
+        got = ops.moe_route(d, k, renorm=renorm, token_mask=dm)
+        r = ops.moe_route_balance(d, k, 0.25, renorm=renorm, token_mask=None if dm is None else dm.to(torch.uint8))
+        torch.cuda.synchronize()
+        assert torch.equal(got[0].cpu().long(), ids)
+        assert torch.allclose(got[1].cpu().to(D), gates, rtol=2 ** -18, atol=1e-37)
+        assert torch.equal(r["ids"], got[0]) and torch.equal(r["gates"], got[1])
+        assert torch.equal(r["counts"].cpu().long(), counts) and int(r["tokens"]) == n
+        rtol = 2 ** -18 + (T / 4096 + 8) * 2 ** -24
+        assert torch.allclose(r["prob_sum"].cpu().to(D), p.sum(0), rtol=rtol, atol=1e-37)
+        assert abs(float(r["loss"]) - float(loss)) <= rtol * float(loss)
+
+
+@pytest.mark.parametrize("T", [0, 1])
+def test_no_tokens(dev, T):
+    """Nothing to route, or nothing that counts: no choice, sums and loss zero, no division by zero."""
+    _say("no tokens", T)
+    x = torch.full((T, 40), NAN, device=dev)
+    mask = torch.zeros(T, dtype=torch.bool, device=dev)
+    r = ops.moe_route_balance(x, 4, 1.0, token_mask=mask)
+    assert r["ids"].shape == (T, 4) and bool((r["ids"] == -1).all()) and bool((r["gates"] == 0).all())
+    assert not r["counts"].any() and not r["prob_sum"].any() and int(r["tokens"]) == 0 and float(r["loss"]) == 0
+    d = ops.moe_route_backward(x, r["ids"], dgates=torch.ones((T, 4), device=dev), counts=r["counts"],
+                               tokens=r["tokens"], coef=1.0, token_mask=mask)
+    assert d.shape == (T, 40) and not d.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E", [6, 100, 300, 700])
+def test_ties_signs_and_masked_experts(dev, E, dtype):
+    """Equal logits go to the lowest expert (-0 equals 0); -inf is never chosen; a row of -inf alone
+    does not count; the type's lowest value can be chosen; NaN ranks first and spreads over its row only."""
+    _say("ties", E, dtype)
+    k, low = 5, torch.finfo(dtype).min
+    rows = [torch.zeros(E), torch.where(torch.arange(E) % 2 == 0, -0.0, 0.0), torch.full((E,), -INF),
+            torch.full((E,), low), torch.full((E,), -INF), torch.arange(E).float() % 3, torch.full((E,), low),
+            torch.full((E,), 2.0), torch.linspace(-1, 1, E), torch.linspace(1, -1, E)]
+    rows[4][E - 2] = 1.5                       # one expert left
+    rows[6][E // 2] = torch.finfo(dtype).max   # the difference to the others overflows
+    rows[8][E - 3] = NAN
+    rows[9][1] = INF
+    x = torch.stack(rows).to(dtype)
+    want = _choose(x, k)
+    ids, gates = ops.moe_route(x.to(dev), k)
+    r = ops.moe_route_balance(x[:8].to(dev), k, 1.0)
+    full = ops.moe_route(x.to(dev), k, renorm=False)[1].cpu()
+    ids, gates = ids.cpu().long(), gates.cpu()
+    assert torch.equal(ids, want)
+    assert ids[1].tolist() == list(range(5)) and ids[2].tolist() == [-1] * 5 and ids[4].tolist() == [E - 2] + [-1] * 4
+    assert ids[8, 0] == E - 3 and ids[9, 0] == 1
+    for g in (gates, full):
+        assert torch.isfinite(g[:8]).all() and torch.isnan(g[8:]).all()
+        assert not g[2].any() and g[4].tolist() == [1, 0, 0, 0, 0] and g[6].tolist() == [1, 0, 0, 0, 0]
+    assert torch.allclose(gates[0].to(D), torch.full((5,), 0.2, dtype=D), rtol=2 ** -18, atol=0)
+    assert torch.allclose(full[0].to(D), torch.full((5,), 1 / E, dtype=D), rtol=2 ** -18, atol=0)
+    assert int(r["tokens"]) == 7 and int(r["counts"].sum()) == 6 * 5 + 1
+    assert abs(float(r["prob_sum"].sum().double()) - 7) < 7 * 2 ** -17
+    # the gradient of the same rows: finite, zero where nothing may flow, NaN in the NaN rows only
+    d = ops.moe_route_backward(x.to(dev), ids.int().to(dev), dgates=torch.ones_like(gates).to(dev), counts=r["counts"],
+                               tokens=r["tokens"], coef=1.0).float().cpu()
+    assert torch.isfinite(d[:8]).all() and not d[2].any() and d[4][E - 2] == 0 and torch.isnan(d[8:]).all()
+
+
+def _gradient(x, ids, dg, counts, n, coef, dloss, renorm):
+    """The formula in 64 bits, and the sum of its terms' magnitudes."""
+    p = _softmax(x)
+    T, E = x.shape
+    k = ids.shape[1]
+    on = (ids >= 0) & (ids < E)
+    at = ids.clamp(0, E - 1)
+    zero = torch.zeros(1, dtype=D)
+    dg = torch.where(on, dg.to(D), zero)
+    d, mag = torch.zeros_like(x), torch.zeros_like(x)
+    if renorm:
+        xc = torch.where(on, x.gather(1, at), torch.full((1,), -INF, dtype=D))
+        g = _softmax(xc)
+        d.scatter_add_(1, at, torch.where(on, g * (dg - (g * dg).sum(1, keepdim=True)), zero))
+        mag.scatter_add_(1, at, torch.where(on, g * (dg.abs() + (g * dg.abs()).sum(1, keepdim=True)), zero))
+    else:
+        g = torch.where(on, p.gather(1, at), zero)
+        d -= p * (g * dg).sum(1, keepdim=True)
+        mag += p * (g * dg.abs()).sum(1, keepdim=True)
+        d.scatter_add_(1, at, torch.where(on, g * dg, zero))
+        mag.scatter_add_(1, at, torch.where(on, g * dg.abs(), zero))
+    if counts is not None and n:
+        c = dloss * coef * E / (k * n * n)
+        f = counts.to(D)
+        s = (p * f).sum(1, keepdim=True)
+        d += c * p * (f - s)
+        mag += abs(c) * p * (f + s)
+    return d, mag
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("T,E,k,pad", SIZES)
+def test_route_backward(dev, T, E, k, pad, renorm, dtype):
+    _say("route backward", T, E, k, pad, renorm, dtype)
+    wide = _logits(T, E, dtype, T + 7 * E, pad=pad)
+    g = torch.Generator().manual_seed(2)
+    mask = torch.rand(T, generator=g) < 0.8
+    x = wide[:, :E].clone()
+    if E > 4:
+        x[:, 2] = -INF
+    ids = _reference(x, k, renorm, mask, 1.0)[0]
+    dg = torch.randn((T, k), generator=g)
+    dg[ids < 0] = NAN  # nobody's gradient
+    counts = torch.bincount(ids[ids >= 0], minlength=E) * 3  # as summed over three ranks
+    n = 3 * int(mask.sum())
+    to = lambda t: t.to(dev)
+    whole = torch.cat([x, wide[:, E:]], 1).to(dev)
+    xd, tokens = whole[:, :E], torch.tensor([n], dtype=torch.int32, device=dev)
+    common = dict(renorm=renorm, token_mask=to(mask))
+    both = dict(dgates=to(dg), counts=to(counts.int()), tokens=tokens, coef=0.5, dloss=torch.tensor([-1.5], device=dev))
+    for parts in (both, {"dgates": both["dgates"]}, {k_: v for k_, v in both.items() if k_ != "dgates"}):
+        got = ops.moe_route_backward(xd, to(ids.int()), **common, **parts)
+        torch.cuda.synchronize()
+        assert got.dtype == dtype and got.shape == (T, E)
+        gates = dg if "dgates" in parts else torch.zeros_like(dg)
+        want, mag = _gradient(x.to(D), ids, gates, counts if "counts" in parts else None, n, 0.5, -1.5, renorm)
+        want[~mask], mag[~mask] = 0, 0
+        tol = 2 ** -17 * mag + 1e-37 + (2 ** -8 * want.abs() if dtype is torch.bfloat16 else 0)
+        assert bool(((got.cpu().to(D) - want).abs() <= tol).all())
+    # in place, leaving the columns behind the experts alone
+    behind = whole[:, E:].clone()
+    first = ops.moe_route_backward(xd, to(ids.int()), **common, **both)
+    out = ops.moe_route_backward(xd, to(ids.int()), **common, **both, out=xd)
+    assert out.data_ptr() == xd.data_ptr() and torch.equal(out, first) and torch.equal(whole[:, E:], behind)
+
+
+def test_backward_against_differences(dev):
+    """The gradient of sum(gates * w) + loss by central differences of the 64-bit formula, with the counts held."""
+    _say("differences")
+    T, E, k = 6, 24, 4
+    x = _logits(T, E, torch.float32, 5, spread=1.5).to(D)
+    w = torch.randn((T, k), generator=torch.Generator().manual_seed(8))
+    for renorm in (True, False):
+        ids, _, _, counts, n, _ = _reference(x, k, renorm, None, 0.7)
+
+        def value(y):
+            p = _softmax(y)
+            g = p.gather(1, ids)
+            if renorm:
+                g = g / g.sum(1, keepdim=True)
+            return float((g * w.to(D)).sum() + 0.7 * E / (k * n * n) * (counts.to(D) * p.sum(0)).sum())
+
+        got = ops.moe_route_backward(x.float().to(dev), ids.int().to(dev), dgates=w.to(dev), counts=counts.int().to(dev),
+                                     tokens=torch.tensor([n], dtype=torch.int32, device=dev), coef=0.7, renorm=renorm)
+        h = 1e-4
+        for t in range(T):
+            for e in range(E):
+                a, b = x.clone(), x.clone()
+                a[t, e] += h
+                b[t, e] -= h
+                # h^2 / 6 times a third derivative of a few units, and 2^-17 of magnitudes below 4
+                assert abs(float(got[t, e]) - (value(a) - value(b)) / (2 * h)) < 1e-7 + 2 ** -15
+
+
+def test_backward_odd_choices(dev):
+    """Choices that the forward pass would not make: out of range (no gradient, nothing read or written there), the
+    same expert twice (both count), experts at -inf, all of them left out."""
+    _say("odd choices")
+    E = 10
+    x = _logits(5, E, torch.float32, 9)
+    x[3, 4] = -INF
+    ids = torch.tensor([[3, 3, 7], [1 << 30, -5, 2], [E, E, -1], [4, 4, 4], [0, 9, 0]])
+    dg = torch.tensor([[1.0, 2.0, 3.0], [9.0, 9.0, 4.0], [5.0, 6.0, 7.0], [1.0, 1.0, 2.0], [1.0, -2.0, 0.5]])
+    for renorm in (True, False):
+        got = ops.moe_route_backward(x.to(dev), ids.int().to(dev), dgates=dg.to(dev), renorm=renorm).cpu().to(D)
+        want, mag = _gradient(x.to(D), ids, dg, None, 0, 0, 0, renorm)
+        want = torch.nan_to_num(want)
+        assert bool(((got - want).abs() <= 2 ** -17 * torch.nan_to_num(mag) + 1e-37).all())
+
+
+def _combine_case(dev, T, H, E, e0, n_local, k, dtype, seed, same=False):
+    rng = np.random.default_rng(seed)
+    ids = np.stack([rng.permutation(E)[:k] for _ in range(T)]).astype(np.int32) if T else np.zeros((0, k), np.int32)
+    if same:
+        ids[:] = ids[:, :1]  # one expert k times
+    gates = rng.random((T, k), dtype=np.float32)
+    ids, gates = torch.from_numpy(ids), torch.from_numpy(gates)
+    dy = torch.randn((T, H), generator=torch.Generator().manual_seed(seed)).to(dtype)
+    return ids, gates, dy
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,H,E,e0,n_local,k,same", [
+    (1, 8, 4, 0, 4, 2, False), (7, 2056, 40, 8, 16, 8, False), (300, 1032, 12, 0, 12, 3, False), (64, 7168, 256, 32, 32, 8, False),
+    (5, 512, 40, 0, 40, 32, False), (9, 264, 6, 0, 6, 4, True), (50, 128, 64, 60, 4, 2, False)])
+def test_combine_backward(dev, T, H, E, e0, n_local, k, same, dtype):
+    _say("combine backward", T, H, E, e0, n_local, k, same, dtype)
+    ids, gates, dy = _combine_case(dev, T, H, E, e0, n_local, k, dtype, T + H, same)
+    idd, gd, dyd = ids.to(dev), gates.to(dev), dy.to(dev)
+    t = ops.moe_build_indices_dev(idd, gd, e0, n_local)
+    pull, w = t["pull_indices"].cpu(), t["row_weight"].cpu()
+    ye = wl.randn_bf16((t["R_pad"], H), 5)
+    a, dg = ops.moe_combine_backward(dyd, ye.to(dev), idd, t["row_weight"], t["owner_offset"], t["slot_to_row"],
+                                     t["rb_rows"], e0, n_local)
+    # a capacity, the row count on the device; rows behind it stay
+    c = ops.moe_build_indices_dev(idd, gd, e0, n_local, sync=False)
+    cap = c["pull_indices"].shape[0]
+    yc = torch.zeros((cap, H), dtype=torch.bfloat16, device=dev)
+    yc[:t["R_pad"]] = ye.to(dev)
+    keep = torch.full((cap, H), 7.0, dtype=torch.bfloat16, device=dev)
+    b, dg2 = ops.moe_combine_backward(dyd, yc, idd, c["row_weight"], c["owner_offset"], c["slot_to_row"], c["rb_rows"],
+                                      e0, n_local, dy_expert=keep, sizes=c["sizes"])
+    torch.cuda.synchronize()
+    assert torch.equal(b[:t["R_pad"]], a) and bool((b[t["R_pad"]:] == 7).all()) and torch.equal(dg, dg2)
+    # dy_expert: one fp32 product, one rounding: the same bits
+    tok = pull[:, 2].clamp(min=0).long()
+    want = torch.where((pull[:, 0] >= 0)[:, None], w[:, None] * dy.float()[tok], torch.zeros(1)).to(torch.bfloat16)
+    assert torch.equal(a.cpu(), want)
+    # dgates by the order of the rows of each expert
+    ref, mag = torch.zeros((T, k), dtype=D), torch.zeros((T, k), dtype=D)
+    row = 0
+    for e in range(n_local):
+        at = (ids == e0 + e).nonzero()
+        for i, (tt, j) in enumerate(at.tolist()):
+            v = dy[tt].to(D) * ye[row + i].to(D)
+            ref[tt, j], mag[tt, j] = v.sum(), v.abs().sum()
+        row += (at.shape[0] + 127) // 128 * 128
+    # a lane's chain of at most H / 32 + 8 products and sums (each rounded), and 12 sums across
+    assert bool(((dg.cpu().to(D) - ref).abs() <= (2 * (H / 32 + 8) + 12) * 2 ** -24 * mag).all())
+    local = (ids >= e0) & (ids < e0 + n_local)
+    assert not dg.cpu()[~local].any()
+
+
+def test_combine_backward_no_rows(dev):
+    """A rank that no token was routed to, a batch of no tokens, and rows that another owner holds."""
+    _say("combine backward without rows")
+    ids = torch.zeros((6, 2), dtype=torch.int32, device=dev)
+    gates = torch.ones((6, 2), device=dev)
+    t = ops.moe_build_indices_dev(ids, gates, 5, 3)
+    dy = torch.full((6, 64), NAN, device=dev)
+    a, dg = ops.moe_combine_backward(dy, torch.empty((0, 64), dtype=torch.bfloat16, device=dev), ids, t["row_weight"],
+                                     t["owner_offset"], t["slot_to_row"], t["rb_rows"], 5, 3)
+    assert a.shape == (0, 64) and not dg.any()
+    t = ops.moe_build_indices_dev(ids, gates, 0, 3)
+    t["slot_to_row"].fill_(-1)
+    ye = torch.zeros((t["R_pad"], 64), dtype=torch.bfloat16, device=dev)
+    a, dg = ops.moe_combine_backward(dy, ye, ids, t["row_weight"], t["owner_offset"], t["slot_to_row"], t["rb_rows"], 0, 3)
+    assert not dg.any() and not a[12:].any()
+    none = ids[:0]
+    a, dg = ops.moe_combine_backward(dy[:0], ye, none, t["row_weight"], torch.zeros(1, dtype=torch.int32, device=dev),
+                                     t["slot_to_row"], t["rb_rows"], 0, 3)
+    assert dg.shape == (0, 2)
+
+
+def test_repeatable_on_other_streams_and_in_a_graph(dev):
+    """Equal bits on another stream, beside another call, and in replays of a captured graph with new inputs."""
+    _say("streams and graph")
+    T, E, k = 3000, 60, 4
+    xs = [_logits(T, E, torch.float32, s).to(dev) for s in range(3)]
+    dg = torch.randn((T, k), device=dev)
+
+    def step(x):
+        r = ops.moe_route_balance(x, k, 0.1)
+        d = ops.moe_route_backward(x, r["ids"], dgates=dg, counts=r["counts"], tokens=r["tokens"], coef=0.1)
+        return [r["ids"], r["gates"], r["loss"], r["counts"], r["prob_sum"], r["tokens"], d]
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for s, x in zip(side, xs):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(step(x))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+    x = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x)
+    for rep in range(4):
+        x.copy_(xs[rep % 3])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, v) for u, v in zip(out, want[rep % 3])), rep
+        step(xs[1])  # eager work between the replays

@@ -1,0 +1,293 @@
+"""Products with 4-bit weights, dense and for routed experts, against 64-bit
+plain forms.
+
+Two kinds of input.  Whole numbers and scales that are powers of two make every
+product and sum exact in fp32 (a group's sum stays below 128 * 3 * 143 * 2 <
+2^24), so the result is the exact one rounded once: equal bits, whatever the
+order of the sums.  Normal inputs: one rounding to bf16 (2^-8 of the value), and
+fp32 roundings of a group's sums, at most 2 per product of magnitude up to 143
+|x| s (the code's offset included) on a chain of a group's 2 * 128 products, and
+one per group and wave sum."""
+import numpy as np
+import pytest
+import torch
+
+from mkernel_amd import ops, workloads as wl
+
+pytestmark = pytest.mark.gpu
+D = torch.float64
+
+
+def _say(*a):
+    print("[case]", *a, flush=True)
+
+
+def _weights(shape, group, seed, zeros, exact):
+    g = torch.Generator().manual_seed(seed)
+    *lead, K, N = shape
+    gs = (*lead, (K + group - 1) // group, N)
+    codes = torch.randint(0, 16, shape, generator=g, dtype=torch.uint8)
+    if exact:
+        scales = 2.0 ** torch.randint(-3, 1, gs, generator=g)
+    else:
+        scales = (torch.rand(gs, generator=g) + 0.5) * K ** -0.5 / 4.6
+    z = torch.randint(0, 16, gs, generator=g, dtype=torch.uint8) if zeros else None
+    return codes, scales.to(torch.bfloat16), z
+
+
+def _dense(codes, scales, z, group):
+    at = torch.arange(codes.shape[-2]) // group
+    zz = 8.0 if z is None else z[..., at, :].to(D)
+    return (codes.to(D) - zz) * scales[..., at, :].to(D)
+
+
+def _pack(dev, w, group):
+    return ops.w4_pack(w[0].to(dev), w[1].to(dev), group, zeros=None if w[2] is None else w[2].to(dev))
+
+
+def _whole(shape, seed):
+    return torch.randint(-3, 4, shape, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16)
+
+
+def _bound(x, w, group, want):
+    """2^-8 of the value, and 256 + ceil(K / 128) + 8 fp32 roundings of the sum of |x| 143 s."""
+    s = w[1][..., torch.arange(w[0].shape[-2]) // group, :].to(D)
+    mag = x.to(D).abs() @ (143.0 * s)
+    n = 256 + (w[0].shape[-2] + 127) // 128 + 8
+    return 2.0 ** -8 * want.abs() + n * 2.0 ** -24 * mag + 1e-37
+
+
+SHAPES = [(1, 8, 1), (1, 128, 16), (1, 2048, 2048), (2, 136, 17), (5, 5608, 2811), (16, 1024, 100), (17, 264, 33),
+          (33, 96, 50), (48, 520, 2064), (64, 3584, 512), (65, 1032, 70), (130, 384, 40), (1, 8192, 3584), (3, 16384, 64),
+          (0, 64, 64)]
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_gemm_exact(dev, M, K, N, group, zeros):
+    _say("gemm_w4 exact", M, K, N, group, zeros)
+    w = _weights((K, N), group, K + N, zeros, True)
+    x = _whole((M, K), M)
+    want = (x.to(D) @ _dense(*w, group)).float().to(torch.bfloat16)
+    p = _pack(dev, w, group)
+    assert torch.equal(ops.gemm_w4(x.to(dev), p).cpu(), want)
+    # rows of wider matrices; what lies beside the result stays
+    wide = torch.full((M, K + 24), float("nan"), dtype=torch.bfloat16, device=dev)
+    wide[:, 8:8 + K] = x.to(dev)
+    out = torch.full((M, N + 5), 3.0, dtype=torch.bfloat16, device=dev)
+    if M > 1:
+        got = ops.gemm_w4(wide[:, 8:8 + K], p, out=out[:, :N])
+        assert torch.equal(got.cpu(), want) and bool((out[:, N:] == 3).all())
+
+
+@pytest.mark.parametrize("M,K,N,group,zeros", [(1, 8192, 3584, 128, False), (1, 2048, 2048, 32, True), (7, 5608, 2811, 32, True),
+                                               (64, 3584, 8192, 64, False), (16, 7168, 4096, 128, True), (100, 1000, 300, 64, False)])
+def test_gemm_normal(dev, M, K, N, group, zeros):
+    _say("gemm_w4 normal", M, K, N, group, zeros)
+    w = _weights((K, N), group, 1, zeros, False)
+    x = wl.randn_bf16((M, K), 2)
+    want = x.to(D) @ _dense(*w, group)
+    p = _pack(dev, w, group)
+    got = ops.gemm_w4(x.to(dev), p)
+    err = (got.cpu().to(D) - want).abs()
+    assert bool((err <= _bound(x, w, group, want)).all())
+    assert float(err.norm() / want.norm()) < 2.0 ** -8  # one rounding's norm, the fp32 sums' far below
+    # a batch's rows do not depend on each other, nor a row on the batch's size (within a tile height)
+    again = ops.gemm_w4(x.to(dev), p)
+    assert torch.equal(got, again)
+    x[0] = float("nan")
+    bad = ops.gemm_w4(x.to(dev), p)
+    assert torch.isnan(bad[0]).all() and torch.equal(bad[1:], got[1:])
+
+
+@pytest.mark.parametrize("shape", [(200, 33), (3, 128, 48), (7, 64)])
+@pytest.mark.parametrize("group", [32, 128])
+def test_quantize(dev, shape, group):
+    """Scales and codes by the definition, bit by bit; the values within half a step of the weights."""
+    _say("quantize", shape, group)
+    W = wl.randn_bf16(shape, 3)
+    W[..., 0] = 0
+    codes, scales = (t.cpu() for t in ops.w4_quantize(W.to(dev), group))
+    K = shape[-2]
+    at = torch.arange(K) // group
+    for g in range((K + group - 1) // group):
+        most = W[..., at == g, :].float().abs().amax(-2)
+        assert torch.equal(scales[..., g, :], (most / 7).to(torch.bfloat16))
+    s = scales[..., at, :].float()
+    q = torch.where(s > 0, W.float() / s, torch.zeros(1)).round().clamp(-8, 7) + 8
+    assert torch.equal(codes.float(), q)
+    # half a step of the code; the largest magnitudes lie up to 7 (1 + 2^-8) steps out
+    back = (codes.float() - 8) * s
+    assert bool(((back - W.float()).abs() <= s * (0.5 + 7 * 2 ** -8)).all())
+    if len(shape) == 2 and K % 8 == 0:
+        x = wl.randn_bf16((4, K), 4)
+        want = x.to(D) @ back.to(D)
+        got = ops.gemm_w4(x.to(dev), ops.w4_pack(codes.to(dev), scales.to(dev), group)).cpu().to(D)
+        assert bool(((got - want).abs() <= _bound(x, (codes, scales), group, want)).all())
+
+
+def _tables(dev, counts, E):
+    """Tables of experts with these row counts, in 128-row blocks."""
+    blocks = [(c + 127) // 128 for c in counts]
+    rb_expert = torch.tensor([e for e in range(E) for _ in range(blocks[e])], dtype=torch.int32)
+    rb_rows = torch.tensor([min(128, counts[e] - 128 * b) for e in range(E) for b in range(blocks[e])], dtype=torch.int32)
+    return rb_expert.to(dev), rb_rows.to(dev)
+
+
+@pytest.mark.parametrize("counts", [[1, 0, 3], [0, 0, 0], [16, 17, 64, 65], [128, 1, 129, 300], [2] * 7])
+@pytest.mark.parametrize("K,N,mode,group,zeros", [(128, 64, 0, 128, False), (264, 96, 1, 32, False), (520, 50, 0, 64, True),
+                                                  (1024, 544, 1, 128, True)])
+def test_grouped(dev, counts, K, N, mode, group, zeros):
+    _say("grouped_w4", counts, K, N, mode, group, zeros)
+    E = len(counts)
+    w = _weights((E, K, N), group, 5, zeros, True)
+    p = _pack(dev, w, group)
+    rb_expert, rb_rows = _tables(dev, counts, E)
+    R, width = 128 * rb_expert.shape[0], N // 2 if mode else N
+    A = _whole((R, K), 6)
+    real = torch.zeros(R, dtype=torch.bool)
+    for b, n in enumerate(rb_rows.tolist()):
+        real[128 * b:128 * b + n] = True
+    Ad = A.clone()
+    Ad[~real] = float("nan")
+    out = torch.full((R + 128, width), 7.0, dtype=torch.bfloat16, device=dev)
+    ops.moe_grouped_gemm_w4(Ad.to(dev), p, out[:R], rb_expert, rb_rows, mode=mode)
+    got = out.cpu()
+    assert bool((got[R:] == 7).all()) and bool((got[:R][~real] == 7).all())
+    dense = _dense(*w, group)
+    for b in range(R // 128):
+        rows = slice(128 * b, 128 * b + int(rb_rows[b]))
+        h = A[rows].to(D) @ dense[int(rb_expert[b])]
+        if mode == 0:
+            assert torch.equal(got[rows], h.float().to(torch.bfloat16)), b
+        else:
+            want = torch.nn.functional.silu(h[:, :width]) * h[:, width:]
+            # one rounding, and 8 fp32 roundings of the SwiGLU (of exact sums)
+            assert torch.allclose(got[rows].to(D), want, rtol=2 ** -8 + 2 ** -20, atol=1e-30), b
+    # rows of a token buffer through a pull table, the row count on the device, blocks behind it and bad experts skipped
+    tokens = _whole((40, K), 7)
+    pick = torch.randint(0, 40, (R,), generator=torch.Generator().manual_seed(8))
+    pull = torch.stack([torch.zeros(R, dtype=torch.int64), torch.zeros(R, dtype=torch.int64), pick], 1)
+    pull[~real] = -1
+    direct = torch.full((R, width), 7.0, dtype=torch.bfloat16, device=dev)
+    ops.moe_grouped_gemm_w4(tokens[pick].to(dev), p, direct, rb_expert, rb_rows, mode=mode)
+    bad = torch.tensor([E, -1], dtype=torch.int32, device=dev)
+    more_pull = torch.cat([pull, torch.zeros((256, 3), dtype=torch.int64)]).int().to(dev)
+    more = torch.full((R + 256, width), 7.0, dtype=torch.bfloat16, device=dev)
+    ops.moe_grouped_gemm_w4(tokens.to(dev), p, more, torch.cat([rb_expert, bad]),
+                            torch.cat([rb_rows, torch.full((2,), 128, dtype=torch.int32, device=dev)]), mode=mode,
+                            gather_pull=more_pull, sizes=torch.tensor([R, R + 128], dtype=torch.int64, device=dev))
+    assert torch.equal(more[:R], direct) and bool((more[R:] == 7).all())
+
+
+def _layer(dev, T, H, I, E, e0, n_local, k, group, seed, zeros=False):
+    g = torch.Generator().manual_seed(seed)
+    x = wl.randn_bf16((T, H), seed)
+    logits = torch.randn((T, E), generator=g)
+    w1, w2 = _weights((n_local, H, 2 * I), group, seed + 1, zeros, False), _weights((n_local, I, H), group, seed + 2, zeros, False)
+    return x, logits, w1, w2
+
+
+def _run_layer(dev, x, logits, p1, p2, e0, n_local, k, out, bufs=None):
+    """Logits to layer output, as a decode step runs it."""
+    ids, gates = ops.moe_route(logits, k)
+    t = ops.moe_build_indices_dev(ids, gates, e0, n_local, sync=False)
+    cap = t["pull_indices"].shape[0]
+    act = torch.empty((cap, p2.K), dtype=torch.bfloat16, device=dev)
+    ye = torch.empty((cap, p1.K), dtype=torch.bfloat16, device=dev)
+    y = torch.empty(x.shape, dtype=out, device=dev)
+    ops.moe_ffn_combine_w4(x, t["pull_indices"], t["row_weight"], t["owner_offset"], t["slot_to_row"], p1, p2, act, ye,
+                           y, t["rb_expert"], t["rb_rows"], sizes=t["sizes"])
+    return y, ids, gates
+
+
+@pytest.mark.parametrize("T,H,I,E,e0,n_local,k,group,zeros,out", [
+    (1, 512, 128, 16, 0, 16, 4, 128, False, torch.bfloat16), (5, 264, 48, 8, 2, 4, 2, 32, True, torch.float32),
+    (64, 1024, 256, 64, 8, 8, 8, 64, False, torch.bfloat16), (300, 256, 112, 4, 0, 4, 2, 128, False, torch.float32),
+    (3, 512, 128, 16, 12, 4, 1, 128, False, torch.bfloat16)])
+def test_layer_from_logits(dev, T, H, I, E, e0, n_local, k, group, zeros, out):
+    """Router, index build and 4-bit expert layer together, in 64 bits: activation, expert rows and (bf16)
+    output are rounded to bf16, each by at most 2^-8 of its value."""
+    _say("layer", T, H, I, E, e0, n_local, k, group, zeros, out)
+    x, logits, w1, w2 = _layer(dev, T, H, I, E, e0, n_local, k, group, 11, zeros)
+    p1, p2 = _pack(dev, w1, group), _pack(dev, w2, group)
+    y, ids, gates = _run_layer(dev, x.to(dev), logits.to(dev), p1, p2, e0, n_local, k, out)
+    ids, gates = ids.cpu(), gates.cpu()
+    d1, d2 = _dense(*w1, group), _dense(*w2, group)
+    ref, mag = torch.zeros((T, H), dtype=D), torch.zeros((T, H), dtype=D)
+    for t in range(T):
+        for j in range(k):
+            e = int(ids[t, j]) - e0
+            if 0 <= e < n_local:
+                h = x[t].to(D) @ d1[e]
+                a = torch.nn.functional.silu(h[:I]) * h[I:]
+                ref[t] += gates[t, j].to(D) * (a @ d2[e])
+                mag[t] += gates[t, j].to(D) * (a.abs() @ d2[e].abs())
+    got = y.cpu().to(D)
+    # 2^-8 of every activation and of every expert row (at most mag); half as much again for fp32; the output's own
+    tol = (2 + 1) * 2.0 ** -8 * mag + (2.0 ** -8 * ref.abs() if out is torch.bfloat16 else 0) + 1e-30
+    assert bool(((got - ref).abs() <= tol).all())
+    assert not got[mag.sum(1) == 0].any()
+    if mag.any():
+        assert float((got - ref).norm() / ref.norm()) < 3 * 2.0 ** -8
+
+
+def test_layer_graph_and_streams(dev):
+    """The decode step captured and replayed with new tokens, eager steps between; two streams at once."""
+    _say("layer graph")
+    T, H, I, E, k = 24, 512, 128, 32, 4
+    x, logits, w1, w2 = _layer(dev, T, H, I, E, 0, E, k, 128, 21)
+    p1, p2 = _pack(dev, w1, 128), _pack(dev, w2, 128)
+    data = [(wl.randn_bf16((T, H), s).to(dev), torch.randn((T, E), generator=torch.Generator().manual_seed(s)).to(dev))
+            for s in range(3)]
+    want = [_run_layer(dev, a, b, p1, p2, 0, E, k, torch.bfloat16) for a, b in data]
+    torch.cuda.synchronize()
+    sx, sl = data[0][0].clone(), data[0][1].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _run_layer(dev, sx, sl, p1, p2, 0, E, k, torch.bfloat16)
+    for rep in range(4):
+        sx.copy_(data[rep % 3][0])
+        sl.copy_(data[rep % 3][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, v) for u, v in zip(out, want[rep % 3])), rep
+        _run_layer(dev, *data[1], p1, p2, 0, E, k, torch.bfloat16)
+    got = []
+    for (a, b) in data[:2]:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(_run_layer(dev, a, b, p1, p2, 0, E, k, torch.bfloat16))
+    torch.cuda.synchronize()
+    for u, v in zip(got, want):
+        assert all(torch.equal(i, j) for i, j in zip(u, v))
+
+
+def test_python_refusals(dev):
+    _say("refusals")
+    codes = torch.zeros((64, 32), dtype=torch.uint8, device=dev)
+    scales = torch.ones((2, 32), dtype=torch.bfloat16, device=dev)
+    p = ops.w4_pack(codes, scales, 32)
+    x = torch.zeros((2, 64), dtype=torch.bfloat16, device=dev)
+    two = ops.w4_pack(codes.repeat(2, 1, 1), scales.repeat(2, 1, 1), 32)
+    rb = torch.zeros(1, dtype=torch.int32, device=dev)
+    out = torch.zeros((128, 32), dtype=torch.bfloat16, device=dev)
+    for call in (lambda: ops.w4_pack(codes, scales, 48), lambda: ops.w4_pack(codes, scales[:1], 32),
+                 lambda: ops.w4_pack(codes.t(), scales, 32), lambda: ops.w4_pack(codes, scales.float(), 32),
+                 lambda: ops.w4_pack(codes[:0], scales[:0], 32), lambda: ops.gemm_w4(x[:, :56], p),
+                 lambda: ops.gemm_w4(x.t().contiguous().t(), p), lambda: ops.gemm_w4(x, two), lambda: ops.gemm_w4(x.float(), p),
+                 lambda: ops.gemm_w4(x, p, out=out[:2, :31]), lambda: ops.gemm_w4(x.expand(2, 64)[:1].expand(4, 64), p),
+                 lambda: ops.moe_grouped_gemm_w4(x, two, out, rb), lambda: ops.moe_grouped_gemm_w4(out, two, out, rb)):
+        with pytest.raises(ValueError):
+            call()
+    logits = torch.zeros((3, 8), device=dev)
+    ids = torch.zeros((3, 2), dtype=torch.int32, device=dev)
+    for call in (lambda: ops.moe_route(logits, 9), lambda: ops.moe_route(logits, 0), lambda: ops.moe_route(logits.t(), 1),
+                 lambda: ops.moe_route(logits.half(), 1), lambda: ops.moe_route(logits, 1, token_mask=ids[:, 0]),
+                 lambda: ops.moe_route_balance(logits, 1, float("inf")), lambda: ops.moe_route_balance(logits, 1, 1e39),
+                 lambda: ops.moe_route_backward(logits, ids), lambda: ops.moe_route_backward(logits, ids, counts=ids[0]),
+                 lambda: ops.moe_route_backward(logits, ids, dgates=torch.zeros((2, 2), device=dev))):
+        with pytest.raises((ValueError, OverflowError)):
+            call()
