@@ -200,7 +200,7 @@ def prepare(case, seed):
         s["ye"][: s["where"].shape[0]] = _randn((s["where"].shape[0], c["H"]), seed, 2, 1.0)
         s["dye"] = torch.zeros_like(s["ye"])
         if own:  # the tables that the forward pass was run with
-            s["t"] = s["ops"].moe_build_indices_dev(s["ids"], s["gates"], 0, c["E"] // c["ep"], sync=False)
+            s["t"] = s["ops"].moe_build_indices_dev(s["ids"], s["gates"].float(), 0, c["E"] // c["ep"], sync=False)
     elif op == "w4":
         s["x"] = _randn((c["M"], c["K"]), seed, 1, 1.0)
         s["w"] = _codes((c["K"], c["N"]), c["group"], seed, 10, c["zeros"])
