@@ -215,8 +215,8 @@ def prepare(case, seed):
         if own:
             s["p1"] = s["ops"].w4_pack(s["w1"][0], s["w1"][1], c["group"])
             s["p2"] = s["ops"].w4_pack(s["w2"][0], s["w2"][1], c["group"])
-            s["act"] = torch.empty((_capacity(c), I), dtype=BF16, device=DEV)
-            s["ye"] = torch.empty((_capacity(c), H), dtype=BF16, device=DEV)
+            s["act"] = torch.empty((_capacity(c), 2 * I), dtype=BF16, device=DEV)
+            s["ye"] = torch.empty((_capacity(c), H), dtype=F32, device=DEV)
             s["y"] = torch.empty((c["T"], H), dtype=BF16, device=DEV)
     return s
 
