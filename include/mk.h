@@ -623,14 +623,15 @@ typedef struct mk_w4_quantize_args {
 } mk_w4_quantize_args;
 int mk_w4_quantize(const mk_w4_quantize_args* args, void* stream);
 
-/* C[M, N] = A[M, K] @ w (num_experts 1), fp32 sums, bf16 output.  For few rows
+/* C[M, N] = A[M, K] @ w (num_experts 1), fp32 sums, bf16 or fp32 output.  For few rows
  * (it reads the weights once per 64 rows); K % 8 == 0, lda % 8 == 0, any M and
  * N.  An infinity in a row of A makes that row of C NaN. */
 typedef struct mk_gemm_w4_args {
   const void* A;        /* bf16 [M, lda] */
-  void* C;              /* bf16 [M, ldc] */
+  void* C;              /* [M, ldc] */
   mk_w4_weights W;
   int64_t M, lda, ldc;
+  int32_t out_type;     /* 0 fp32, 1 bf16 */
 } mk_gemm_w4_args;
 int mk_gemm_w4(const mk_gemm_w4_args* args, void* stream);
 
@@ -639,26 +640,32 @@ int mk_gemm_w4(const mk_gemm_w4_args* args, void* stream);
  * of h = A[r] @ w[e(r)] with I = N / 2 a multiple of 16 (mode 1).  rb_expert
  * names the expert of each 128-row block (blocks that name none are skipped);
  * only the rb_rows real rows of a block are computed, other rows of out stay as
- * they are.  gather_pull, n_src_rows, tokens_per_src, devs_per_node and sizes
+ * they are.  out is fp32, bf16, or a bf16 pair: a row holds its values rounded
+ * to bf16 and behind them what the rounding left, again in bf16 (17 bits of
+ * significand, so that an activation between two products loses nothing that a
+ * bf16 result shows); such rows are read with a_parts 2.  gather_pull, n_src_rows, tokens_per_src, devs_per_node and sizes
  * as in mk_moe_grouped_gemm_args. */
 typedef struct mk_moe_grouped_gemm_w4_args {
-  const void* A;               /* bf16 [R_pad, K], or the token buffer [n_src_rows, K] */
+  const void* A;               /* bf16 [R_pad, K * a_parts], or the token buffer [n_src_rows, K] */
   mk_w4_weights W;
-  void* out;                   /* bf16 [R_pad, N], mode 1: [R_pad, N / 2] */
+  void* out;                   /* [R_pad, N], mode 1: [R_pad, N / 2]; twice as wide as a pair */
   const int32_t* rb_expert;    /* [R_pad/128] */
   const int32_t* rb_rows;      /* [R_pad/128], or NULL: every row is real */
   int64_t R_pad;
   int32_t mode;
+  int32_t a_parts;             /* 1, or 2: A holds pairs (without gather_pull) */
+  int32_t out_type;            /* 0 fp32, 1 bf16, 2 bf16 pair */
   const int32_t* gather_pull;  /* [R_pad, 3] or NULL */
-  int64_t n_src_rows;
+  int64_t n_src_rows;          /* n_src_rows * K * 2 below 2 GiB */
   int32_t tokens_per_src, devs_per_node;
   const int64_t* sizes;        /* device {R, R_pad} or NULL */
 } mk_moe_grouped_gemm_w4_args;
 int mk_moe_grouped_gemm_w4(const mk_moe_grouped_gemm_w4_args* args, void* stream);
 
 /* The local MoE layer with 4-bit expert weights: GEMM1 + SwiGLU (token rows
- * read through the pull table) -> GEMM2 -> combine, three launches.  act and
- * y_expert are written on real rows only. */
+ * read through the pull table) -> GEMM2 -> combine, three launches.  The
+ * activation goes as a bf16 pair and the expert rows in fp32, so y_out is
+ * rounded once.  act and y_expert are written on real rows only. */
 typedef struct mk_moe_ffn_w4_args {
   const void* tokens;           /* bf16 [n_src_rows, H] */
   const int32_t* pull_indices;  /* [R_pad, 3] */
@@ -669,8 +676,8 @@ typedef struct mk_moe_ffn_w4_args {
   const int32_t* slot_to_row;   /* [R] */
   mk_w4_weights w1;             /* [E, H, 2I] (gate | up) */
   mk_w4_weights w2;             /* [E, I, H] */
-  void* act;                    /* bf16 [R_pad, I] */
-  void* y_expert;               /* bf16 [R_pad, H] */
+  void* act;                    /* bf16 [R_pad, 2I] */
+  void* y_expert;               /* fp32 [R_pad, H] */
   void* y_out;                  /* [num_tokens, H] fp32 or bf16 */
   int64_t num_tokens, n_src_rows, R_pad;
   int32_t tokens_per_src, devs_per_node;

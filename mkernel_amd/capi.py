@@ -184,13 +184,14 @@ class W4QuantizeArgs(C.Structure):
 
 
 class GemmW4Args(C.Structure):
-    _fields_ = [("A", vp), ("C", vp), ("W", W4WeightsC), ("M", i64), ("lda", i64), ("ldc", i64)]
+    _fields_ = [("A", vp), ("C", vp), ("W", W4WeightsC), ("M", i64), ("lda", i64), ("ldc", i64),
+                ("out_type", i32)]
 
 
 class MoeGroupedGemmW4Args(C.Structure):
     _fields_ = [("A", vp), ("W", W4WeightsC), ("out", vp), ("rb_expert", vp), ("rb_rows", vp), ("R_pad", i64),
-                ("mode", i32), ("gather_pull", vp), ("n_src_rows", i64), ("tokens_per_src", i32),
-                ("devs_per_node", i32), ("sizes", vp)]
+                ("mode", i32), ("a_parts", i32), ("out_type", i32), ("gather_pull", vp), ("n_src_rows", i64),
+                ("tokens_per_src", i32), ("devs_per_node", i32), ("sizes", vp)]
 
 
 class MoeFfnW4Args(C.Structure):

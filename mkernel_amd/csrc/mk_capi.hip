@@ -954,8 +954,8 @@ int mk_moe_combine(const mk_moe_combine_args* a, void* stream) {
   if (a->out_dtype != 0 && a->out_dtype != 1) return fail(MK_EINVAL, "mk_moe_combine: out_dtype must be 0 or 1");
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
-  mk::CombineKParams p{static_cast<const uint16_t*>(a->y_expert), a->row_weight, a->owner_offset, a->slot_to_row,
-                       a->y_out, a->num_tokens, a->H, a->out_dtype};
+  mk::CombineKParams p{a->y_expert, a->row_weight, a->owner_offset, a->slot_to_row,
+                       a->y_out, a->num_tokens, a->H, a->out_dtype, 0};
   hipError_t e = mk::launch_combine(p, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_combine launch");
 }
@@ -1190,8 +1190,9 @@ static mk::W4KParams w4_params(const mk_w4_weights& w, const void* A, void* C, i
   p.w = {static_cast<const uint32_t*>(w.packed), static_cast<const uint16_t*>(w.scales),
          static_cast<const uint8_t*>(w.zeros), w.K, w.N, w.group, w.num_experts};
   p.A = static_cast<const uint16_t*>(A);
-  p.C = static_cast<uint16_t*>(C);
+  p.C = C;
   p.M = M; p.lda = lda; p.ldc = ldc;
+  p.parts = 1;
   p.tile_cols = (int)((w.N + 15) / 16);
   return p;
 }
@@ -1204,13 +1205,16 @@ int mk_gemm_w4(const mk_gemm_w4_args* a, void* stream) {
   if (a->W.K % 8) return fail(MK_ESHAPE, "mk_gemm_w4: K must be a multiple of 8");
   if (a->lda < a->W.K || a->lda % 8 || a->ldc < a->W.N)
     return fail(MK_ESHAPE, "mk_gemm_w4: lda must be a multiple of 8 of at least K, ldc at least N");
+  if (a->lda > (1 << 24)) return fail(MK_ESHAPE, "mk_gemm_w4: lda must be at most 2^24");  // 32-bit offsets in a row tile
+  if (a->out_type != 0 && a->out_type != 1) return fail(MK_EINVAL, "mk_gemm_w4: out_type must be 0 or 1");
   if (a->M == 0) return MK_OK;
   if (!a->A || !a->C) return fail(MK_EINVAL, "mk_gemm_w4: null argument");
   if (!aligned16(a->A) || !aligned16(a->C)) return fail(MK_EINVAL, "mk_gemm_w4: A and C must be 16-byte aligned");
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   mk::W4KParams p = w4_params(a->W, a->A, a->C, a->M, a->lda, a->ldc);
-  hipError_t e = mk::launch_w4(p, static_cast<hipStream_t>(stream));
+  p.out_type = a->out_type;
+  hipError_t e = mk::launch_w4(p, d.cus, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? MK_OK : hip_fail(e, "mk_gemm_w4 launch");
 }
 
@@ -1218,18 +1222,24 @@ int mk_gemm_w4(const mk_gemm_w4_args* a, void* stream) {
 static int prepare_grouped_w4(const char* fn, const mk_moe_grouped_gemm_w4_args* a, mk::W4KParams* p) {
   if (int rc = check_w4(fn, a->W)) return rc;
   if (a->mode != 0 && a->mode != 1) return fail(MK_EINVAL, "%s: mode must be 0 or 1", fn);
-  if (a->W.K % 8) return fail(MK_ESHAPE, "%s: K must be a multiple of 8", fn);
+  if (a->a_parts != 1 && a->a_parts != 2) return fail(MK_EINVAL, "%s: a_parts must be 1 or 2", fn);
+  if (a->out_type < 0 || a->out_type > 2) return fail(MK_EINVAL, "%s: out_type must be 0, 1 or 2", fn);
+  if (a->W.K % 8 || a->W.K > (1 << 21)) return fail(MK_ESHAPE, "%s: K must be a multiple of 8 up to 2^21", fn);
   if (a->mode == 1 && a->W.N % 32) return fail(MK_ESHAPE, "%s: N must be a multiple of 32 with SwiGLU", fn);
   if (a->R_pad < 0 || a->R_pad % MK_ROW_BLOCK || a->R_pad > (1 << 21))
     return fail(MK_ESHAPE, "%s: R_pad must be a multiple of %d up to 2^21", fn, MK_ROW_BLOCK);
   if (a->R_pad > 0) {
     if (!a->A || !a->out || !a->rb_expert) return fail(MK_EINVAL, "%s: null argument", fn);
     if (!aligned16(a->A) || !aligned16(a->out)) return fail(MK_EINVAL, "%s: A and out must be 16-byte aligned", fn);
-    if (a->gather_pull && (a->n_src_rows <= 0 || a->tokens_per_src <= 0 || a->devs_per_node <= 0))
-      return fail(MK_EINVAL, "%s: gather_pull needs n_src_rows, tokens_per_src and devs_per_node > 0", fn);
+    if (a->gather_pull && (a->n_src_rows <= 0 || a->tokens_per_src <= 0 || a->devs_per_node <= 0 || a->a_parts != 1 ||
+                           a->n_src_rows >= (1LL << 30) / a->W.K))
+      return fail(MK_EINVAL, "%s: gather_pull needs n_src_rows, tokens_per_src and devs_per_node > 0, a_parts 1 and "
+                             "a token buffer below 2 GiB", fn);
   }
   const int64_t width = a->mode == 1 ? a->W.N / 2 : a->W.N;
-  *p = w4_params(a->W, a->A, a->out, a->R_pad, a->W.K, width);
+  *p = w4_params(a->W, a->A, a->out, a->R_pad, a->W.K * a->a_parts, width * (a->out_type == 2 ? 2 : 1));
+  p->parts = a->a_parts;
+  p->out_type = a->out_type;
   p->swiglu = a->mode;
   if (a->mode == 1) p->tile_cols = (int)(width / 16);
   p->rb_expert = a->rb_expert;
@@ -1249,7 +1259,7 @@ int mk_moe_grouped_gemm_w4(const mk_moe_grouped_gemm_w4_args* a, void* stream) {
   if (a->R_pad == 0) return MK_OK;
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
-  hipError_t e = mk::launch_w4(p, static_cast<hipStream_t>(stream));
+  hipError_t e = mk::launch_w4(p, d.cus, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_grouped_gemm_w4 launch");
 }
 
@@ -1266,24 +1276,24 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* a, void* stream) {
   if (a->w1.num_experts != a->w2.num_experts || a->w1.K != a->w2.N || a->w1.N != 2 * a->w2.K)
     return fail(MK_ESHAPE, "%s: w1 must be [E, H, 2I] and w2 [E, I, H]", fn);
   // both products are checked before anything is queued
-  mk_moe_grouped_gemm_w4_args g1{a->tokens, a->w1, a->act, a->rb_expert, a->rb_rows, a->R_pad, 1, a->pull_indices,
-                                 a->n_src_rows, a->tokens_per_src, a->devs_per_node, a->sizes};
-  mk_moe_grouped_gemm_w4_args g2{a->act, a->w2, a->y_expert, a->rb_expert, a->rb_rows, a->R_pad, 0, nullptr,
-                                 0, 0, 0, a->sizes};
+  mk_moe_grouped_gemm_w4_args g1{a->tokens, a->w1, a->act, a->rb_expert, a->rb_rows, a->R_pad, 1, 1, 2,
+                                 a->pull_indices, a->n_src_rows, a->tokens_per_src, a->devs_per_node, a->sizes};
+  mk_moe_grouped_gemm_w4_args g2{a->act, a->w2, a->y_expert, a->rb_expert, a->rb_rows, a->R_pad, 0, 2, 0,
+                                 nullptr, 0, 0, 0, a->sizes};
   mk::W4KParams p1, p2;
   if (int rc = prepare_grouped_w4(fn, &g1, &p1)) return rc;
   if (int rc = prepare_grouped_w4(fn, &g2, &p2)) return rc;
-  mk_moe_combine_args ca{a->y_expert, a->row_weight, a->owner_offset, a->slot_to_row, a->y_out,
-                         a->num_tokens, a->w1.K, a->out_dtype};
+  const mk::CombineKParams pc{a->y_expert, a->row_weight, a->owner_offset, a->slot_to_row, a->y_out,
+                              a->num_tokens, a->w1.K, a->out_dtype, 1};
   if (a->num_tokens > 0 && !aligned16(a->y_out)) return fail(MK_EINVAL, "%s: y_out must be 16-byte aligned", fn);
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
-  if (rows) {
-    hipError_t e = mk::launch_w4(p1, static_cast<hipStream_t>(stream));
-    if (e == hipSuccess) e = mk::launch_w4(p2, static_cast<hipStream_t>(stream));
-    if (e != hipSuccess) return hip_fail(e, "mk_moe_ffn_combine_w4 launch");
-  }
-  return a->num_tokens > 0 ? mk_moe_combine(&ca, stream) : MK_OK;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e = hipSuccess;
+  if (rows) e = mk::launch_w4(p1, d.cus, st);
+  if (rows && e == hipSuccess) e = mk::launch_w4(p2, d.cus, st);
+  if (e == hipSuccess) e = mk::launch_combine(pc, st);
+  return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_ffn_combine_w4 launch");
 }
 
 }  // extern "C"

@@ -152,13 +152,14 @@ struct PermuteKParams {
 hipError_t launch_permute(const PermuteKParams& p, hipStream_t stream);
 
 struct CombineKParams {
-  const uint16_t* y_expert;
+  const void* y_expert;
   const float* row_weight;
   const int* owner_offset;
   const int* slot_to_row;
   void* y_out;
   int64_t num_tokens, H;
   int out_dtype;
+  int f32_rows;             // y_expert holds fp32
 };
 hipError_t launch_combine(const CombineKParams& p, hipStream_t stream);
 hipError_t launch_tile_rows(const int* pull, int64_t R_pad, int* rb_rows, hipStream_t stream);
@@ -222,18 +223,22 @@ hipError_t launch_route_backward(const RouteBwdKParams& p, hipStream_t stream);
 // Products with 4-bit weights (mk_w4.hip).
 struct W4Weights {
   const uint32_t* packed;   // [E][tiles][blocks][64 lanes][4]
-  const uint16_t* scales;   // [E][tiles][groups][16]
-  const uint8_t* zeros;     // as scales, or null: 8
+  const uint16_t* scales;   // [E][tiles][blocks][4 quads][groups of a block][4 columns]
+  const uint8_t* zeros;     // [E][tiles][blocks][16 columns][groups of a block], or null: 8
   int64_t K, N;
   int group, E;
 };
+enum W4Out : int { kW4F32 = 0, kW4Bf16 = 1, kW4Pair = 2 };
 struct W4KParams {
   W4Weights w;
   const uint16_t* A;
-  uint16_t* C;
-  int64_t lda, ldc, M;      // M: rows of A (dense) or of the tables
+  void* C;
+  int64_t lda, ldc, M;      // elements; M: rows of A (dense) or of the tables
   int tile_cols;            // output column tiles of 16
   int swiglu;
+  int parts;                // 2: a row of A is two bf16 rows of K whose sum it stands for
+  int out_type;             // W4Out; a pair is two bf16 rows of the result's width
+  int64_t row_blocks;       // set by the launch
   // experts (rb_expert null: one dense product)
   const int* rb_expert;
   const int* rb_rows;
@@ -244,7 +249,7 @@ struct W4KParams {
 };
 int64_t w4_packed_words(int64_t K, int64_t N, int64_t E);
 int64_t w4_scale_count(int64_t K, int64_t N, int64_t E, int group);
-hipError_t launch_w4(const W4KParams& p, hipStream_t stream);
+hipError_t launch_w4(const W4KParams& p, int cus, hipStream_t stream);
 hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int64_t K, int64_t N,
                           int64_t E, int group, uint32_t* packed, uint16_t* packed_scales, uint8_t* packed_zeros,
                           hipStream_t stream);

@@ -49,9 +49,11 @@ hipError_t launch_permute(const PermuteKParams& p, hipStream_t stream) {
 // kernel is latency-bound, and the dependent owner -> slot -> row -> data
 // chain per column chunk made it so.  Sums stay in slot order
 // (deterministic, bit-identical to the plain loop).
-template <int V>
+// Rows are bf16, or fp32 (F32: the 4-bit expert layer's, which are not rounded
+// before the sum).
+template <int V, bool F32>
 __global__ __launch_bounds__(kThreads) void combine_kernel(CombineKParams p) {
-  constexpr int kMaxSlots = 8, kWords = V / 2;  // 32-bit words of a row chunk
+  constexpr int kMaxSlots = 8, kWords = F32 ? V : V / 2;  // 32-bit words of a row chunk
   typedef uint32_t words __attribute__((ext_vector_type(kWords)));
   const int64_t t = blockIdx.x;
   const int s0 = p.owner_offset[t], s1 = p.owner_offset[t + 1];
@@ -75,11 +77,17 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineKParams p) {
     auto add = [&](float w, const words& v) {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
-        acc[2 * i] += w * bf16_lo(v[i]);
-        acc[2 * i + 1] += w * bf16_hi(v[i]);
+        if constexpr (F32) {
+          acc[i] += w * __uint_as_float(v[i]);
+        } else {
+          acc[2 * i] += w * bf16_lo(v[i]);
+          acc[2 * i + 1] += w * bf16_hi(v[i]);
+        }
       }
     };
-    auto load = [&](int64_t row) { return *reinterpret_cast<const words*>(p.y_expert + row * p.H + c * V); };
+    auto load = [&](int64_t row) {
+      return *reinterpret_cast<const words*>(static_cast<const char*>(p.y_expert) + (row * p.H + c * V) * (F32 ? 4 : 2));
+    };
     if (few) {
       words v[kMaxSlots];
 #pragma unroll
@@ -115,10 +123,9 @@ hipError_t launch_combine(const CombineKParams& p, hipStream_t stream) {
   const int64_t chunks = (p.H / v + kThreads - 1) / kThreads;
   // workgroups per token: enough for 1024 in all, at most one per column chunk
   const unsigned split = (unsigned)std::max<int64_t>(1, std::min<int64_t>(chunks, 1024 / p.num_tokens));
-  if (v == 4)
-    hipLaunchKernelGGL(combine_kernel<4>, dim3((unsigned)p.num_tokens, split), dim3(kThreads), 0, stream, p);
-  else
-    hipLaunchKernelGGL(combine_kernel<8>, dim3((unsigned)p.num_tokens, split), dim3(kThreads), 0, stream, p);
+  auto* kernel = p.f32_rows ? (v == 4 ? combine_kernel<4, true> : combine_kernel<8, true>)
+                            : (v == 4 ? combine_kernel<4, false> : combine_kernel<8, false>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)p.num_tokens, split), dim3(kThreads), 0, stream, p);
   return hipGetLastError();
 }
 

@@ -33,11 +33,12 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // Eight codes of one word as bf16 128 + q: nibbles i and i + 4 are elements
-// 2i and 2i + 1.
-__device__ __forceinline__ bf16x8 expand(uint32_t w) {
+// 2i and 2i + 1.  `mask` and `bias` are 0x000f000f and 0x43004300 in registers,
+// so that a pair is one v_and_or_b32 (with literals it is two instructions).
+__device__ __forceinline__ bf16x8 expand(uint32_t w, uint32_t mask, uint32_t bias) {
   u32x4 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+  for (int i = 0; i < 4; ++i) v[i] = ((w >> (4 * i)) & mask) | bias;
   return __builtin_bit_cast(bf16x8, v);
 }
 
@@ -49,142 +50,374 @@ __device__ __forceinline__ bf16x8 minus_offset(uint32_t z) {
 
 __device__ __forceinline__ float silu(float x) { return x / (1.f + __expf(-x)); }
 
-// MT tiles of 16 rows of x, NT weight tiles (2 with SwiGLU: gate and up), W
-// waves, SUB 32-row steps of K per scale.
-template <int MT, int NT, int W, int SUB, bool ZEROS>
-__global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
-  extern __shared__ f32x4 red[];  // [W][NT][MT][64]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = lane & 15, quad = lane >> 4;
-  const int64_t KB = (p.w.K + kBlock - 1) / kBlock, tiles = (p.w.N + kTile - 1) / kTile;
-  const int64_t groups = KB * (4 / SUB);
+// Loads past a range give zeros without traffic: offsets from here on are past
+// every range (all are checked to span less).
+constexpr uint32_t kNowhere = 0x80000000u;
 
-  // rows of this workgroup
-  int64_t row0 = (int64_t)blockIdx.y * 16 * MT, rows = p.M - row0;
-  int64_t expert = 0;
-  if (p.rb_expert) {
-    const int64_t b = blockIdx.y / (kFlagRows / (16 * MT)), part = blockIdx.y % (kFlagRows / (16 * MT));
-    if (b * kFlagRows >= (p.rows_dev ? min(p.M, *p.rows_dev) : p.M)) return;
-    expert = p.rb_expert[b];
-    if (expert < 0 || expert >= p.w.E) return;
-    rows = (p.rb_rows ? min(p.rb_rows[b], kFlagRows) : kFlagRows) - part * 16 * MT;
-    row0 = b * kFlagRows + part * 16 * MT;
-  }
-  if (rows <= 0) return;
-  rows = min(rows, (int64_t)16 * MT);
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
 
-  // this lane's row of x in each row tile; lanes past the last row read it
-  // again, and their results are not stored
-  const uint16_t* x[MT];
-  bool have[MT];
+// What one step of 128 rows of K needs: packed codes, scales (of this lane's
+// four columns, group by group), zero points (of its one column) and x.
+template <int MT, int NT, int SUB, bool ZEROS, int PARTS>
+struct Step {
+  u32x4 w[NT];
+  uint32_t s[NT][2 * (4 / SUB)];
+  uint32_t z[ZEROS ? NT : 1];
+  u32x4 x[PARTS][MT][4];
+};
+
+// Descriptors of a wave's column tiles (each tile's codes, scales and zeros are
+// one piece) and of its rows of x.
+template <int MT, int NT>
+struct Source {
+  __amdgpu_buffer_rsrc_t w[NT], x;
+  const char* s[NT];
+  const uint8_t* z[NT];
+  uint32_t last;     // last step
+  uint32_t row[MT];  // byte offset of this lane's row, kNowhere where there is none
+  int32_t most;      // last multiple of 8 below K, less this lane's first k in a step
+  uint32_t K;
+};
+
+template <int MT, int NT, int SUB, bool ZEROS, int PARTS>
+__device__ __forceinline__ void load(Step<MT, NT, SUB, ZEROS, PARTS>& st, const Source<MT, NT>& t, uint32_t kb, int lane) {
+  constexpr int G = 4 / SUB;
+  // scales past the last step are the last one's: they multiply zeros
+  const uint32_t sb = min(kb, t.last);
+  const uint32_t at = sb * (32 * G) + (lane >> 4) * (8 * G), zt = sb * (16 * G) + (lane & 15) * G;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int64_t r = row0 + min(rows - 1, (int64_t)16 * m + col);
-    int64_t src = r;
-    have[m] = true;
-    if (p.gather_pull) {
-      const int* pr = p.gather_pull + 3 * r;
-      src = ((int64_t)pr[0] * p.gather_devs + pr[1]) * p.gather_tps + pr[2];
-      have[m] = pr[0] >= 0 && src >= 0 && src < p.gather_rows;
-      if (!have[m]) src = 0;
+  for (int n = 0; n < NT; ++n) st.w[n] = load16(t.w[n], kb * 1024 + lane * 16);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    typedef uint32_t words __attribute__((ext_vector_type(G == 4 ? 4 : 2 * G)));
+#pragma unroll
+    for (int h = 0; h < (G == 4 ? 2 : 1); ++h) {
+      const words v = *reinterpret_cast<const words*>(t.s[n] + at + 16 * h);
+#pragma unroll
+      for (int i = 0; i < (G == 4 ? 4 : 2 * G); ++i) st.s[n][4 * h + i] = v[i];
     }
-    x[m] = p.A + src * p.lda;
+    if constexpr (ZEROS) {
+      if constexpr (G == 1) st.z[n] = t.z[n][zt];
+      else if constexpr (G == 2) st.z[n] = *reinterpret_cast<const uint16_t*>(t.z[n] + zt);
+      else st.z[n] = *reinterpret_cast<const uint32_t*>(t.z[n] + zt);
+    }
   }
-  int64_t tile[NT];
-  tile[0] = blockIdx.x * (p.swiglu ? 1 : NT);
-  if constexpr (NT == 2) tile[1] = p.swiglu ? tile[0] + p.tile_cols : min(tile[0] + 1, tiles - 1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool in = (int32_t)(kb * kBlock) + j * 32 <= t.most;
+#pragma unroll
+    for (int h = 0; h < PARTS; ++h)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        st.x[h][m][j] = load16(t.x, in ? t.row[m] + kb * 256 + 2 * (j * 32 + h * t.K) : kNowhere);
+  }
+}
 
-  f32x4 acc[NT][MT];
+template <int MT, int NT, int SUB, bool ZEROS, int PARTS>
+__device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, PARTS>& st, uint32_t mask, uint32_t bias,
+                                         f32x4 (&acc)[NT][MT]) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int g = 0; g < 4 / SUB; ++g) {
+    f32x4 base[MT];  // sum of -136 x: the same for every column where there are no zero points
+    if constexpr (!ZEROS) {
+      const bf16x8 off = minus_offset(8u);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  for (int64_t kb = wave; kb < KB; kb += W) {
-    u32x4 w[NT];
+      for (int m = 0; m < MT; ++m) {
+        base[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      w[n] = *reinterpret_cast<const u32x4*>(p.w.packed + (((expert * tiles + tile[n]) * KB + kb) * 64 + lane) * 4);
-    bf16x8 xv[MT][4];
+        for (int i = 0; i < SUB; ++i)
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t k = kb * kBlock + j * 32 + quad * 8;
-        u32x4 v = {0u, 0u, 0u, 0u};
-        if (k < p.w.K && have[m]) v = *reinterpret_cast<const u32x4*>(x[m] + k);
-        xv[m][j] = __builtin_bit_cast(bf16x8, v);
+          for (int h = 0; h < PARTS; ++h)
+            base[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(off, __builtin_bit_cast(bf16x8, st.x[h][m][g * SUB + i]), base[m], 0, 0, 0);
       }
+    }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+      f32x4 part[MT];
 #pragma unroll
-      for (int g = 0; g < 4 / SUB; ++g) {
-        const int64_t at = ((expert * tiles + tile[n]) * groups + kb * (4 / SUB) + g) * kTile;
-        const u32x2 sw = *reinterpret_cast<const u32x2*>(p.w.scales + at + 4 * quad);
-        const bf16x8 off = minus_offset(ZEROS ? p.w.zeros[at + col] : 8u);
-        const f32x4 s = {bf16_lo(sw[0]), bf16_hi(sw[0]), bf16_lo(sw[1]), bf16_hi(sw[1])};
-        f32x4 part[MT];
+      for (int m = 0; m < MT; ++m) part[m] = ZEROS ? f32x4{0.f, 0.f, 0.f, 0.f} : base[m];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) part[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < SUB; ++i) {
-          const bf16x8 q = expand(w[n][g * SUB + i]);
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(off, xv[m][g * SUB + i], part[m], 0, 0, 0);
-            part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, xv[m][g * SUB + i], part[m], 0, 0, 0);
-          }
-        }
+      for (int i = 0; i < SUB; ++i) {
+        const bf16x8 q = expand(st.w[n][g * SUB + i], mask, bias);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(s[r], part[m][r], acc[n][m][r]);
+          for (int h = 0; h < PARTS; ++h) {
+            const bf16x8 xv = __builtin_bit_cast(bf16x8, st.x[h][m][g * SUB + i]);
+            if constexpr (ZEROS)
+              part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus_offset((st.z[n] >> (8 * g)) & 255u), xv, part[m], 0, 0, 0);
+            part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, xv, part[m], 0, 0, 0);
+          }
       }
-  }
-
+      const f32x4 s = {bf16_lo(st.s[n][2 * g]), bf16_hi(st.s[n][2 * g]), bf16_lo(st.s[n][2 * g + 1]), bf16_hi(st.s[n][2 * g + 1])};
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) red[((wave * NT + n) * MT + m) * 64 + lane] = acc[n][m];
-  __syncthreads();
-  auto total = [&](int n, int m) {
-    f32x4 v = red[(n * MT + m) * 64 + lane];
-#pragma unroll
-    for (int o = 1; o < W; ++o) v += red[((o * NT + n) * MT + m) * 64 + lane];
-    return v;
-  };
-  const int64_t width = p.swiglu ? (int64_t)p.tile_cols * kTile : p.w.N;
-  const int units = p.swiglu ? MT : NT * MT;
-  for (int u = wave; u < units; u += W) {
-    const int m = u % MT, n = u / MT;
-    if (16 * m + col >= rows) continue;
-    f32x4 v = total(n, m);
-    if constexpr (NT == 2)
-      if (p.swiglu) {
-        const f32x4 up = total(1, m);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = silu(v[r]) * up[r];
-      }
-    if (!p.swiglu && tile[0] + n >= tiles) continue;
-    const int64_t c = (tile[0] + n) * kTile + 4 * quad;
-    uint16_t* out = p.C + (row0 + 16 * m + col) * p.ldc + c;
-    if (c + 4 <= width && p.ldc % 4 == 0) {
-      *reinterpret_cast<u32x2*>(out) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (c + r < width) out[r] = __builtin_bit_cast(uint16_t, (__bf16)v[r]);
+        for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(s[r], part[m][r], acc[n][m][r]);
     }
   }
 }
 
-template <int MT, int NT, int SUB, bool ZEROS>
-void launch(const W4KParams& p, hipStream_t stream) {
-  constexpr int W = 8;
-  const unsigned gx = (unsigned)(p.swiglu ? p.tile_cols : (p.tile_cols + NT - 1) / NT);
-  const unsigned gy = (unsigned)(p.rb_expert ? p.M / (16 * MT) : (p.M + 16 * MT - 1) / (16 * MT));
-  hipLaunchKernelGGL((w4_kernel<MT, NT, W, SUB, ZEROS>), dim3(gx, gy), dim3(64 * W), W * NT * MT * 64 * sizeof(f32x4),
-                     stream, p);
+// The steps kb = first, first + stride, ... of a wave's tiles and rows: a ring
+// of P steps in registers (loads past the last step cost nothing and add
+// zeros).  The barriers keep a step's loads behind the step before, in order:
+// loads return in the order of their issue, so a step waits for its own only.
+template <int MT, int NT, int SUB, bool ZEROS, int PARTS, int P>
+__device__ __forceinline__ void sweep(const Source<MT, NT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
+                                      f32x4 (&acc)[NT][MT]) {
+  uint32_t mask = 0x000f000fu, bias = 0x43004300u;
+  asm volatile("" : "+s"(mask));
+  asm volatile("" : "+v"(bias));
+  Step<MT, NT, SUB, ZEROS, PARTS> st[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    load(st[i], t, first + i * stride, lane);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t kb = first; kb < KB; kb += P * stride) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      multiply(st[i], mask, bias, acc);
+      __builtin_amdgcn_sched_barrier(0);
+      load(st[i], t, kb + (i + P) * stride, lane);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// One unit of the result: 16 columns of 16 rows, this lane's four columns `c` ..
+// of row `r`.
+__device__ __forceinline__ void store(const W4KParams& p, int64_t r, int64_t c, int64_t width, f32x4 v) {
+  if (p.out_type == kW4F32) {
+    float* out = static_cast<float*>(p.C) + r * p.ldc + c;
+    if (c + 4 <= width && p.ldc % 4 == 0) {
+      *reinterpret_cast<f32x4*>(out) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < width) out[i] = v[i];
+    }
+    return;
+  }
+  uint16_t* out = static_cast<uint16_t*>(p.C) + r * p.ldc + c;
+  for (int h = 0; h < (p.out_type == kW4Pair ? 2 : 1); ++h) {
+    const u32x2 o = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    if (c + 4 <= width && p.ldc % 4 == 0 && width % 4 == 0) {
+      *reinterpret_cast<u32x2*>(out) = o;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < width) out[i] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
+    }
+    // what the rounding left, in the second half of the row
+    v = f32x4{v[0] - bf16_lo(o[0]), v[1] - bf16_hi(o[0]), v[2] - bf16_lo(o[1]), v[3] - bf16_hi(o[1])};
+    out += width;
+  }
+}
+
+// How many of a workgroup's W waves share an item's K: few items are cut into
+// more parts so that all waves have work, many are left whole; between, what
+// needs the fewest steps in the longest wave (a round costs about kRoundSteps
+// steps beside its own: row tables, first loads, the sum over waves).
+constexpr int kRoundSteps = 3;
+__device__ __forceinline__ int choose_split(int64_t items, int64_t waves, int KB, int W) {
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= W; s *= 2) {
+    const int64_t cost = (items * s + waves - 1) / waves * ((KB + s - 1) / s + kRoundSteps);
+    if (cost < least) least = cost, best = s;
+  }
+  return best;
+}
+
+// The row passes (16 rows each) of the real rows of up to kListed row blocks.
+constexpr int kListed = 512, kPasses = kFlagRows / 16;
+struct PassList {
+  int first[kListed + 1];             // first pass of each block
+  uint16_t block[kListed * kPasses];  // block of each pass
+  int scratch[17];
+};
+
+// Inclusive prefix sum over the workgroup's 64 W threads.
+template <int W>
+__device__ __forceinline__ int prefix(int v, int* s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(v, d, 64);
+    if (lane >= d) v += y;
+  }
+  if (lane == 63) s[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v += s[w];
+  return v;
+}
+
+__device__ __forceinline__ int block_rows(const W4KParams& p, int64_t b) {
+  const int e = p.rb_expert[b];
+  if (e < 0 || e >= p.w.E) return 0;
+  return p.rb_rows ? max(0, min(p.rb_rows[b], kFlagRows)) : kFlagRows;
+}
+
+// W waves.  An item is NT column tiles (with SwiGLU: the first half gate tiles,
+// the second the matching up tiles) of 16 MT rows; `split` waves share its K.
+// The workgroups of the grid walk the items in turn, as many as the device's
+// row count and tables say there are.
+template <int MT, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS>
+__global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
+  extern __shared__ f32x4 red[];  // [W][NT * MT][64], used where K is split
+  __shared__ PassList list;
+  static_assert(!EXPERTS || MT == 1, "passes of 16 rows");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const uint32_t KB = (uint32_t)((p.w.K + kBlock - 1) / kBlock);
+  const int tiles = (int)((p.w.N + kTile - 1) / kTile);
+  const int64_t groups = (int64_t)KB * (4 / SUB);
+  const int per_item = p.swiglu ? NT / 2 : NT;  // output tiles
+  const int col_items = (p.tile_cols + per_item - 1) / per_item;
+  const int64_t width = p.swiglu ? (int64_t)p.tile_cols * kTile : p.w.N;
+  int64_t blocks = p.row_blocks, passes = p.row_blocks;
+  bool listed = false;
+  if constexpr (EXPERTS) {
+    if (p.rows_dev) blocks = min(blocks, max((int64_t)0, *p.rows_dev / kFlagRows));
+    listed = blocks <= kListed;
+    passes = blocks * kPasses;
+    if (listed) {
+      constexpr int per = kListed / (64 * W) > 0 ? kListed / (64 * W) : 1;
+      int n[per], sum = 0;
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        const int64_t b = threadIdx.x * per + i;
+        n[i] = b < blocks ? (block_rows(p, b) + 15) / 16 : 0;
+        sum += n[i];
+      }
+      int at = prefix<W>(sum, list.scratch);
+      if (threadIdx.x == 64 * W - 1) list.scratch[16] = at;
+      at -= sum;
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        const int b = threadIdx.x * per + i;
+        if (b <= kListed) list.first[b] = at;
+        for (int j = 0; j < n[i]; ++j) list.block[at + j] = (uint16_t)b;
+        at += n[i];
+      }
+      if (threadIdx.x == 64 * W - 1) list.first[kListed] = at;
+      __syncthreads();
+      passes = list.scratch[16];
+    }
+  }
+  const int64_t items = passes * col_items;
+  const int split = __builtin_amdgcn_readfirstlane(choose_split(items, (int64_t)gridDim.x * W, KB, W));
+  const int per = W / split, ks = wave % split;
+  for (int64_t it0 = (int64_t)blockIdx.x * per; it0 < items; it0 += (int64_t)gridDim.x * per) {
+    const int64_t it = it0 + wave / split;
+    int64_t row0 = 0, expert = 0;
+    int ci = 0, left = 0;
+    if (it < items) {
+      if constexpr (EXPERTS) {
+        // the passes of one column item side by side: they read the same weights
+        int64_t q = it / col_items, b;
+        int np = kPasses, pass;
+        if (listed) {
+          b = __builtin_amdgcn_readfirstlane((int)list.block[q]);
+          const int first = __builtin_amdgcn_readfirstlane(list.first[b]);
+          np = __builtin_amdgcn_readfirstlane(list.first[b + 1]) - first;
+          q = first;
+        } else {
+          b = q / kPasses;
+          q = b * kPasses;
+        }
+        const int local = (int)(it - q * col_items);
+        ci = local / np;
+        pass = local - ci * np;
+        left = __builtin_amdgcn_readfirstlane(block_rows(p, b)) - 16 * pass;
+        expert = __builtin_amdgcn_readfirstlane(p.rb_expert[b]);
+        row0 = b * kFlagRows + 16 * pass;
+      } else {
+        const int64_t b = it / col_items;
+        ci = (int)(it - b * col_items);
+        row0 = b * 16 * MT;
+        left = (int)min(p.M - row0, (int64_t)16 * MT);
+      }
+    }
+    Source<MT, NT> t;
+    int tile[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool up = p.swiglu && n >= NT / 2;
+      tile[n] = min(ci * per_item + (up ? n - NT / 2 : n), p.tile_cols - 1) + (up ? p.tile_cols : 0);
+      const int64_t at = left > 0 ? expert * tiles + tile[n] : 0;
+      t.w[n] = make_rsrc(p.w.packed + at * KB * 256, KB * 1024);
+      t.s[n] = reinterpret_cast<const char*>(p.w.scales + at * groups * kTile);
+      if constexpr (ZEROS) t.z[n] = p.w.zeros + at * groups * kTile;
+    }
+    t.last = KB - 1;
+    t.K = (uint32_t)p.w.K;
+    t.most = (int32_t)p.w.K - 8 - quad * 8;
+    // lanes past the last row read nothing; their results are not stored
+    if (EXPERTS && p.gather_pull) {
+      t.x = make_rsrc(p.A, (uint32_t)(p.gather_rows * p.lda * 2));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        t.row[m] = kNowhere;
+        if (16 * m + col < left) {
+          const int* pr = p.gather_pull + 3 * (row0 + 16 * m + col);
+          const int64_t src = ((int64_t)pr[0] * p.gather_devs + pr[1]) * p.gather_tps + pr[2];
+          if (pr[0] >= 0 && pr[2] >= 0 && src >= 0 && src < p.gather_rows) t.row[m] = (uint32_t)(src * p.lda * 2) + quad * 16;
+        }
+      }
+    } else {
+      t.x = make_rsrc(p.A + row0 * p.lda, (uint32_t)(min(max(left, 0), 16 * MT) * p.lda * 2));
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        t.row[m] = 16 * m + col < left ? (uint32_t)((16 * m + col) * p.lda * 2) + quad * 16 : kNowhere;
+    }
+    f32x4 acc[NT][MT];
+    sweep<MT, NT, SUB, ZEROS, PARTS, (MT * PARTS * NT == 1 ? 3 : 2)>(t, KB, left > 0 ? ks : KB, split, lane, acc);
+    auto finish = [&](int n, int m, f32x4 v, f32x4 up) {
+      if (16 * m + col >= left || ci * per_item + n >= p.tile_cols) return;
+      if constexpr (NT >= 2)
+        if (p.swiglu)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = silu(v[r]) * up[r];
+      store(p, row0 + 16 * m + col, (int64_t)(ci * per_item + n) * kTile + 4 * quad, width, v);
+    };
+    if (split == 1) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if (n < per_item) finish(n, m, acc[n][m], acc[NT >= 2 ? (n + NT / 2) % NT : n][m]);
+      continue;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) red[(wave * NT * MT + n * MT + m) * 64 + lane] = acc[n][m];
+    __syncthreads();
+    auto total = [&](int u) {
+      f32x4 v = red[((wave - ks) * NT * MT + u) * 64 + lane];
+      for (int o = 1; o < split; ++o) v += red[((wave - ks + o) * NT * MT + u) * 64 + lane];
+      return v;
+    };
+    for (int u = ks; u < per_item * MT; u += split) {
+      const f32x4 v = total(u);
+      finish(u / MT, u % MT, v, p.swiglu ? total(u + (NT / 2) * MT) : v);
+    }
+    __syncthreads();
+  }
+}
+
+template <int MT, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS>
+void launch(const W4KParams& p, int grid, hipStream_t stream) {
+  hipLaunchKernelGGL((w4_kernel<MT, NT, W, SUB, ZEROS, PARTS, EXPERTS>), dim3(grid), dim3(64 * W),
+                     W * NT * MT * 64 * sizeof(f32x4), stream, p);
 }
 
 __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, int64_t K, int64_t N, int64_t KB,
@@ -205,15 +438,22 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, int6
 }
 
 __global__ __launch_bounds__(256) void w4_pack_groups_kernel(const uint16_t* scales, const uint8_t* zeros, int64_t N,
-                                                             int64_t given, int64_t groups, int64_t tiles,
+                                                             int64_t given, int64_t groups, int per, int64_t tiles,
                                                              int64_t count, uint16_t* out_scales, uint8_t* out_zeros) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= count) return;
-  const int64_t g = i / kTile % groups, tile = i / kTile / groups % tiles, e = i / kTile / groups / tiles;
-  const int64_t n = tile * kTile + i % kTile, at = (e * given + g) * N + n;
-  const bool in = g < given && n < N;
-  out_scales[i] = in ? scales[at] : 0;
-  if (out_zeros) out_zeros[i] = in ? zeros[at] & 15u : 8u;
+  // scales: [tile][block][4 quads][per block][4 columns]; zeros: [tile][block][16 columns][per block]
+  const int64_t unit = kTile * per, block = i / unit, in_block = i % unit;
+  const int64_t kb = block % (groups / per), tile = block / (groups / per) % tiles, e = block / (groups / per) / tiles;
+  auto source = [&](int64_t g, int64_t n) {
+    return g < given && n < N ? (e * given + g) * N + n : (int64_t)-1;
+  };
+  const int64_t at = source(kb * per + in_block / 4 % per, tile * kTile + in_block / (4 * per) * 4 + in_block % 4);
+  out_scales[i] = at >= 0 ? scales[at] : 0;
+  if (out_zeros) {
+    const int64_t zt = source(kb * per + in_block % per, tile * kTile + in_block / per);
+    out_zeros[i] = zt >= 0 ? zeros[zt] & 15u : 8u;
+  }
 }
 
 // One thread per group and column: scale = bf16(largest magnitude / 7), code =
@@ -256,7 +496,7 @@ hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const ui
   const int64_t words = w4_packed_words(K, N, E), count = w4_scale_count(K, N, E, group);
   hipLaunchKernelGGL(w4_pack_kernel, dim3(blocks256(words)), dim3(256), 0, stream, codes, K, N, KB, tiles, words, packed);
   hipLaunchKernelGGL(w4_pack_groups_kernel, dim3(blocks256(count)), dim3(256), 0, stream, scales, zeros, N,
-                     (K + group - 1) / group, KB * (kBlock / group), tiles, count, packed_scales, packed_zeros);
+                     (K + group - 1) / group, KB * (kBlock / group), kBlock / group, tiles, count, packed_scales, packed_zeros);
   return hipGetLastError();
 }
 
@@ -268,24 +508,43 @@ hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E
   return hipGetLastError();
 }
 
-hipError_t launch_w4(const W4KParams& p, hipStream_t stream) {
-  if (p.M == 0) return hipSuccess;
-  auto zeros = [&](auto mt, auto nt, auto sub) {
-    if (p.w.zeros) launch<decltype(mt)::value, decltype(nt)::value, decltype(sub)::value, true>(p, stream);
-    else launch<decltype(mt)::value, decltype(nt)::value, decltype(sub)::value, false>(p, stream);
+hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
+  if (args.M == 0) return hipSuccess;
+  W4KParams p = args;
+  const bool experts = p.rb_expert != nullptr;
+  auto go = [&](auto mt, auto nt, auto w, auto sub, auto zeros, auto parts, auto ex) {
+    constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, W = decltype(w)::value;
+    p.row_blocks = decltype(ex)::value ? p.M / kFlagRows : (p.M + 16 * MT - 1) / (16 * MT);
+    const int per_item = p.swiglu ? NT / 2 : NT;
+    const int64_t items = p.row_blocks * (decltype(ex)::value ? kPasses : 1) * ((p.tile_cols + per_item - 1) / per_item);
+    const int64_t grid = std::min<int64_t>(items, (int64_t)cus * (decltype(ex)::value ? 12 : 16) / W);
+    launch<MT, NT, W, decltype(sub)::value, decltype(zeros)::value, decltype(parts)::value, decltype(ex)::value>(
+        p, (int)grid, stream);
   };
-  auto sub = [&](auto mt, auto nt) {
-    if (p.w.group == 32) zeros(mt, nt, std::integral_constant<int, 1>());
-    else if (p.w.group == 64) zeros(mt, nt, std::integral_constant<int, 2>());
-    else zeros(mt, nt, std::integral_constant<int, 4>());
+  using std::integral_constant;
+  auto with_zeros = [&](auto mt, auto nt, auto w, auto sub, auto parts, auto ex) {
+    if (p.w.zeros) go(mt, nt, w, sub, std::true_type(), parts, ex);
+    else go(mt, nt, w, sub, std::false_type(), parts, ex);
   };
-  auto nt = [&](auto mt) {
-    if (p.swiglu) sub(mt, std::integral_constant<int, 2>());
-    else sub(mt, std::integral_constant<int, 1>());
+  auto with_group = [&](auto mt, auto nt, auto w, auto parts, auto ex) {
+    if (p.w.group == 32) with_zeros(mt, nt, w, integral_constant<int, 1>(), parts, ex);
+    else if (p.w.group == 64) with_zeros(mt, nt, w, integral_constant<int, 2>(), parts, ex);
+    else with_zeros(mt, nt, w, integral_constant<int, 4>(), parts, ex);
   };
-  if (p.M <= 16 && !p.rb_expert) nt(std::integral_constant<int, 1>());
-  else if (p.M <= 32 && !p.rb_expert) nt(std::integral_constant<int, 2>());
-  else nt(std::integral_constant<int, 4>());
+  constexpr integral_constant<int, 1> one;
+  constexpr integral_constant<int, 2> two;
+  constexpr integral_constant<int, 4> four;
+  constexpr integral_constant<int, 8> eight;
+  if (experts) {
+    if (p.parts == 2) with_group(one, four, four, two, std::true_type());
+    else with_group(one, four, four, one, std::true_type());
+  } else if (p.M <= 16) {
+    with_group(one, one, eight, one, std::false_type());
+  } else if (p.M <= 32) {
+    with_group(two, one, eight, one, std::false_type());
+  } else {
+    with_group(four, one, eight, one, std::false_type());
+  }
   return hipGetLastError();
 }
 

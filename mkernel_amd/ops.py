@@ -620,8 +620,8 @@ def _w4(W, name, device, experts=None) -> None:
 
 def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> torch.Tensor:
     """C = A @ w for few rows (mk_gemm_w4): A bf16 [M, K], w 4-bit weights of
-    w4_pack; fp32 sums of exact products, scaled group by group in fp32, bf16
-    out.  K a multiple of 8, any M and N; rows of A (a multiple of 8 elements
+    w4_pack; fp32 sums of exact products, scaled group by group in fp32; out
+    bf16 (what is made where none is given) or float32.  K a multiple of 8, any M and N; rows of A (a multiple of 8 elements
     apart) and of out need only be contiguous each.  The weights are read once
     per 64 rows: from a few hundred rows on, gemm is faster."""
     _tensor(A, "A", _BF16, rows=True)
@@ -631,12 +631,12 @@ def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> t
     if K != W.K:
         raise ValueError(f"A has {K} columns, the weights {W.K} rows")
     if out is not None:
-        _tensor(out, "out", _BF16, (M, W.N), rows=True, device=dev)
+        _tensor(out, "out", _LOGITS, (M, W.N), rows=True, device=dev)
     with _on(dev):
         if out is None:
             out = torch.empty((M, W.N), dtype=torch.bfloat16, device=dev)
         capi.call_values("mk_gemm_w4", GemmW4Args, _stream(), A.data_ptr(), out.data_ptr(), *W._values(), M, _ld(A),
-                         _ld(out))
+                         _ld(out), int(out.dtype == torch.bfloat16))
     return out
 
 
@@ -660,24 +660,32 @@ def moe_grouped_gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor, rb_exp
     """moe_grouped_gemm with 4-bit expert weights (mk_moe_grouped_gemm_w4), for
     the few rows per expert of a decode batch.  mode 0: out = A @ w[e]; mode 1:
     out = silu(h[:, :I]) * h[:, I:], h = A @ w[e].  Only the real rows (rb_rows)
-    of the 128-row blocks are computed and written."""
+    of the 128-row blocks are computed and written.  out is float32, bfloat16 or,
+    with twice the columns, a bfloat16 pair: the rounded values and behind them
+    what the rounding left; A may hold such pairs ([R_pad, 2 K])."""
     _tensor(A, "A", _BF16, dim=2)
     dev = A.device
     _w4(W, "W", dev)
     if mode not in (0, 1):
         raise ValueError("mode must be 0 or 1")
     R_pad = A.shape[0] if gather_pull is None else gather_pull.shape[0]
-    if A.shape[1] != W.K:
+    parts = 2 if gather_pull is None and A.shape[1] == 2 * W.K else 1
+    if A.shape[1] != W.K * parts:
         raise ValueError(f"A has {A.shape[1]} columns, the weights {W.K} rows")
-    _tensor(out, "out", _BF16, (R_pad, W.N // 2 if mode else W.N), device=dev)
+    width = W.N // 2 if mode else W.N
+    _tensor(out, "out", _LOGITS, (R_pad, None), device=dev)
+    pair = out.dtype == torch.bfloat16 and out.shape[1] == 2 * width
+    if out.shape[1] != width and not pair:
+        raise ValueError(f"out has {out.shape[1]} columns, not {width}")
     _block_tables(rb_expert, rb_rows, R_pad, sizes, dev)
     if gather_pull is not None:
         _tensor(gather_pull, "gather_pull", _I32, (R_pad, 3), device=dev)
     tps = A.shape[0] if tokens_per_src is None else tokens_per_src
     with _on(dev):
         capi.call_values("mk_moe_grouped_gemm_w4", MoeGroupedGemmW4Args, _stream(), A.data_ptr(), *W._values(),
-                         out.data_ptr(), rb_expert.data_ptr(), _ptr(rb_rows), R_pad, mode, _ptr(gather_pull),
-                         A.shape[0], tps, devs_per_node, _ptr(sizes))
+                         out.data_ptr(), rb_expert.data_ptr(), _ptr(rb_rows), R_pad, mode, parts,
+                         2 if pair else int(out.dtype == torch.bfloat16), _ptr(gather_pull), A.shape[0], tps,
+                         devs_per_node, _ptr(sizes))
     return out
 
 
@@ -689,8 +697,9 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
     """moe_ffn_combine with 4-bit expert weights w1 [E, H, 2I] and w2 [E, I, H]
     (mk_moe_ffn_combine_w4), for decode batches: grouped GEMM1 + SwiGLU (reads
     the tokens through the pull table) -> grouped GEMM2 -> combine.  act
-    [R_pad, I] and y_expert [R_pad, H] are scratch; sizes as in
-    moe_ffn_combine."""
+    (bfloat16 [R_pad, 2 I]: rounded values and what the rounding left) and
+    y_expert (float32 [R_pad, H]) are scratch; y_out, bfloat16 or float32, is
+    the only rounding; sizes as in moe_ffn_combine."""
     _tensor(tokens, "tokens", _BF16, dim=2)
     dev = tokens.device
     _w4(w1, "w1", dev)
@@ -700,8 +709,8 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
         raise ValueError("w1 must be [E, H, 2I], w2 [E, I, H] and tokens [n, H]")
     _tensor(pull, "pull", _I32, (None, 3), device=dev)
     R_pad = pull.shape[0]
-    _tensor(act, "act", _BF16, (R_pad, I), device=dev)
-    _tensor(y_expert, "y_expert", _BF16, (R_pad, H), device=dev)
+    _tensor(act, "act", _BF16, (R_pad, 2 * I), device=dev)
+    _tensor(y_expert, "y_expert", _F32, (R_pad, H), device=dev)
     _tensor(y_out, "y_out", _LOGITS, (None, H), device=dev)
     T = y_out.shape[0]
     _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)

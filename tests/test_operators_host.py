@@ -138,13 +138,14 @@ def test_weight_refusals(change, code, match):
     _refused("mk_w4_pack", _args(capi.W4PackArgs, dict(codes=P, scales=P, out=w), {}), code, match)
 
 
-GEMM = dict(A=P, C=P, M=1, lda=256, ldc=64)
+GEMM = dict(A=P, C=P, M=1, lda=256, ldc=64, out_type=1)
 
 
 @pytest.mark.parametrize("weights,change,code,match", [
     ({}, dict(M=-1), ESHAPE, "M must"), ({}, dict(M=(1 << 20) + 1), ESHAPE, "M must"), (dict(K=252), {}, ESHAPE, "K must"),
     ({}, dict(lda=248), ESHAPE, "lda"), ({}, dict(lda=260), ESHAPE, "lda"), ({}, dict(ldc=63), ESHAPE, "lda"),
-    (dict(num_experts=2), {}, EINVAL, "matrices"), ({}, dict(A=0), EINVAL, "null"), ({}, dict(A=P + 2), EINVAL, "aligned")])
+    (dict(num_experts=2), {}, EINVAL, "matrices"), ({}, dict(out_type=2), EINVAL, "out_type"),
+    ({}, dict(lda=1 << 25), ESHAPE, "lda"), ({}, dict(A=0), EINVAL, "null"), ({}, dict(A=P + 2), EINVAL, "aligned")])
 def test_gemm_w4_refusals(weights, change, code, match):
     _refused("mk_gemm_w4", _args(capi.GemmW4Args, dict(GEMM, W=_weights(**weights)), change), code, match)
 
@@ -155,12 +156,15 @@ def test_pack_refusals():
                                      {}), EINVAL, "group")
 
 
-GROUPED = dict(A=P, out=P, rb_expert=P, R_pad=128, mode=0)
+GROUPED = dict(A=P, out=P, rb_expert=P, R_pad=128, mode=0, a_parts=1, out_type=1)
+PULL = dict(gather_pull=P, n_src_rows=1, tokens_per_src=1, devs_per_node=1)
 
 
 @pytest.mark.parametrize("weights,change,code,match", [
     ({}, dict(mode=2), EINVAL, "mode"), ({}, dict(R_pad=64), ESHAPE, "R_pad"), ({}, dict(rb_expert=0), EINVAL, "null"),
     (dict(N=48), dict(mode=1), ESHAPE, "SwiGLU"), ({}, dict(gather_pull=P), EINVAL, "gather_pull"),
+    ({}, dict(PULL, a_parts=2), EINVAL, "gather_pull"), ({}, dict(PULL, n_src_rows=1 << 22), EINVAL, "2 GiB"),
+    ({}, dict(a_parts=0), EINVAL, "a_parts"), ({}, dict(out_type=3), EINVAL, "out_type"),
     ({}, dict(R_pad=1 << 22), ESHAPE, "R_pad"), (dict(K=100), {}, ESHAPE, "K must")])
 def test_grouped_w4_refusals(weights, change, code, match):
     _refused("mk_moe_grouped_gemm_w4", _args(capi.MoeGroupedGemmW4Args, dict(GROUPED, W=_weights(**weights)), change),
