@@ -1205,6 +1205,7 @@ int mk_gemm_w4(const mk_gemm_w4_args* a, void* stream) {
   if (a->W.K % 8) return fail(MK_ESHAPE, "mk_gemm_w4: K must be a multiple of 8");
   if (a->lda < a->W.K || a->lda % 8 || a->ldc < a->W.N)
     return fail(MK_ESHAPE, "mk_gemm_w4: lda must be a multiple of 8 of at least K, ldc at least N");
+  if ((a->M + 15) / 16 * ((a->W.N + 15) / 16) >= (1LL << 31)) return fail(MK_ESHAPE, "mk_gemm_w4: M x N too large");
   if (a->lda > (1 << 24)) return fail(MK_ESHAPE, "mk_gemm_w4: lda must be at most 2^24");  // 32-bit offsets in a row tile
   if (a->out_type != 0 && a->out_type != 1) return fail(MK_EINVAL, "mk_gemm_w4: out_type must be 0 or 1");
   if (a->M == 0) return MK_OK;
@@ -1228,6 +1229,7 @@ static int prepare_grouped_w4(const char* fn, const mk_moe_grouped_gemm_w4_args*
   if (a->mode == 1 && a->W.N % 32) return fail(MK_ESHAPE, "%s: N must be a multiple of 32 with SwiGLU", fn);
   if (a->R_pad < 0 || a->R_pad % MK_ROW_BLOCK || a->R_pad > (1 << 21))
     return fail(MK_ESHAPE, "%s: R_pad must be a multiple of %d up to 2^21", fn, MK_ROW_BLOCK);
+  if (a->R_pad / 16 * ((a->W.N + 15) / 16) >= (1LL << 31)) return fail(MK_ESHAPE, "%s: R_pad x N too large", fn);
   if (a->R_pad > 0) {
     if (!a->A || !a->out || !a->rb_expert) return fail(MK_EINVAL, "%s: null argument", fn);
     if (!aligned16(a->A) || !aligned16(a->out)) return fail(MK_EINVAL, "%s: A and out must be 16-byte aligned", fn);

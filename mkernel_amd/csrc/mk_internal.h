@@ -238,7 +238,7 @@ struct W4KParams {
   int swiglu;
   int parts;                // 2: a row of A is two bf16 rows of K whose sum it stands for
   int out_type;             // W4Out; a pair is two bf16 rows of the result's width
-  int64_t row_blocks;       // set by the launch
+  int row_blocks, split;    // set by the launch
   // experts (rb_expert null: one dense product)
   const int* rb_expert;
   const int* rb_rows;

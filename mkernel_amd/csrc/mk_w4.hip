@@ -23,6 +23,13 @@
 #include "mk_device.h"
 #include "mk_internal.h"
 
+#ifndef W4_NT
+#define W4_NT 1
+#define W4_W 8
+#define W4_NT2 4
+#define W4_W2 8
+#define W4_P1 3
+#endif
 namespace mk {
 namespace {
 
@@ -161,9 +168,11 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, PARTS>& 
 }
 
 // The steps kb = first, first + stride, ... of a wave's tiles and rows: a ring
-// of P steps in registers (loads past the last step cost nothing and add
-// zeros).  The barriers keep a step's loads behind the step before, in order:
-// loads return in the order of their issue, so a step waits for its own only.
+// of P steps in registers.  The barriers keep a step's loads behind the step
+// before, in order: loads return in the order of their issue, so a step waits
+// for its own only.  The last P steps load nothing more (a load that nobody
+// needs would still be waited for before its registers are used again); those
+// past the end found zeros.
 template <int MT, int NT, int SUB, bool ZEROS, int PARTS, int P>
 __device__ __forceinline__ void sweep(const Source<MT, NT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
                                       f32x4 (&acc)[NT][MT]) {
@@ -180,7 +189,8 @@ __device__ __forceinline__ void sweep(const Source<MT, NT>& t, uint32_t KB, uint
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (uint32_t kb = first; kb < KB; kb += P * stride) {
+  uint32_t kb = first;
+  for (; kb + P * stride < KB; kb += P * stride) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       multiply(st[i], mask, bias, acc);
@@ -189,6 +199,8 @@ __device__ __forceinline__ void sweep(const Source<MT, NT>& t, uint32_t KB, uint
       __builtin_amdgcn_sched_barrier(0);
     }
   }
+#pragma unroll
+  for (int i = 0; i < P; ++i) multiply(st[i], mask, bias, acc);
 }
 
 // One unit of the result: 16 columns of 16 rows, this lane's four columns `c` ..
@@ -226,12 +238,14 @@ __device__ __forceinline__ void store(const W4KParams& p, int64_t r, int64_t c, 
 // needs the fewest steps in the longest wave (a round costs about kRoundSteps
 // steps beside its own: row tables, first loads, the sum over waves).
 constexpr int kRoundSteps = 3;
-__device__ __forceinline__ int choose_split(int64_t items, int64_t waves, int KB, int W) {
+__host__ __device__ __forceinline__ int choose_split(uint32_t items, uint32_t waves, uint32_t KB, int W) {
   int best = 1;
-  int64_t least = INT64_MAX;
-  for (int s = 1; s <= W; s *= 2) {
-    const int64_t cost = (items * s + waves - 1) / waves * ((KB + s - 1) / s + kRoundSteps);
-    if (cost < least) least = cost, best = s;
+  uint64_t least = ~0ull;
+  for (int log = 0; 1 << log <= W; ++log) {
+    // rounds of items << log wave tasks; items < 2^31, so a wave's items are counted first
+    const uint32_t each = waves >> log ? waves >> log : 1;
+    const uint64_t cost = (uint64_t)((items + each - 1) / each) * (((KB + (1u << log) - 1) >> log) + kRoundSteps);
+    if (cost < least) least = cost, best = 1 << log;
   }
   return best;
 }
@@ -282,10 +296,11 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
   const int per_item = p.swiglu ? NT / 2 : NT;  // output tiles
   const int col_items = (p.tile_cols + per_item - 1) / per_item;
   const int64_t width = p.swiglu ? (int64_t)p.tile_cols * kTile : p.w.N;
-  int64_t blocks = p.row_blocks, passes = p.row_blocks;
+  int blocks = p.row_blocks;
+  uint32_t passes = p.row_blocks;
   bool listed = false;
   if constexpr (EXPERTS) {
-    if (p.rows_dev) blocks = min(blocks, max((int64_t)0, *p.rows_dev / kFlagRows));
+    if (p.rows_dev) blocks = (int)min((int64_t)blocks, max((int64_t)0, *p.rows_dev / kFlagRows));
     listed = blocks <= kListed;
     passes = blocks * kPasses;
     if (listed) {
@@ -293,7 +308,7 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
       int n[per], sum = 0;
 #pragma unroll
       for (int i = 0; i < per; ++i) {
-        const int64_t b = threadIdx.x * per + i;
+        const int b = threadIdx.x * per + i;
         n[i] = b < blocks ? (block_rows(p, b) + 15) / 16 : 0;
         sum += n[i];
       }
@@ -312,18 +327,19 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
       passes = list.scratch[16];
     }
   }
-  const int64_t items = passes * col_items;
-  const int split = __builtin_amdgcn_readfirstlane(choose_split(items, (int64_t)gridDim.x * W, KB, W));
-  const int per = W / split, ks = wave % split;
-  for (int64_t it0 = (int64_t)blockIdx.x * per; it0 < items; it0 += (int64_t)gridDim.x * per) {
-    const int64_t it = it0 + wave / split;
+  const uint32_t items = passes * col_items;
+  // (a dense launch knows its items on the host)
+  const int split = EXPERTS ? __builtin_amdgcn_readfirstlane(choose_split(items, gridDim.x * W, KB, W)) : p.split;
+  const int log = __builtin_ctz(split), per = W >> log, ks = wave & (split - 1);
+  for (uint32_t it0 = blockIdx.x * per; it0 < items; it0 += gridDim.x * per) {
+    const uint32_t it = it0 + (wave >> log);
     int64_t row0 = 0, expert = 0;
     int ci = 0, left = 0;
     if (it < items) {
       if constexpr (EXPERTS) {
         // the passes of one column item side by side: they read the same weights
-        int64_t q = it / col_items, b;
-        int np = kPasses, pass;
+        uint32_t q = it / col_items;
+        int np = kPasses, pass, b;
         if (listed) {
           b = __builtin_amdgcn_readfirstlane((int)list.block[q]);
           const int first = __builtin_amdgcn_readfirstlane(list.first[b]);
@@ -338,11 +354,11 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
         pass = local - ci * np;
         left = __builtin_amdgcn_readfirstlane(block_rows(p, b)) - 16 * pass;
         expert = __builtin_amdgcn_readfirstlane(p.rb_expert[b]);
-        row0 = b * kFlagRows + 16 * pass;
+        row0 = (int64_t)b * kFlagRows + 16 * pass;
       } else {
-        const int64_t b = it / col_items;
+        const uint32_t b = it / col_items;
         ci = (int)(it - b * col_items);
-        row0 = b * 16 * MT;
+        row0 = (int64_t)b * 16 * MT;
         left = (int)min(p.M - row0, (int64_t)16 * MT);
       }
     }
@@ -379,7 +395,7 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
         t.row[m] = 16 * m + col < left ? (uint32_t)((16 * m + col) * p.lda * 2) + quad * 16 : kNowhere;
     }
     f32x4 acc[NT][MT];
-    sweep<MT, NT, SUB, ZEROS, PARTS, (MT * PARTS * NT == 1 ? 3 : 2)>(t, KB, left > 0 ? ks : KB, split, lane, acc);
+    sweep<MT, NT, SUB, ZEROS, PARTS, (MT * PARTS * NT == 1 ? W4_P1 : 2)>(t, KB, left > 0 ? ks : KB, split, lane, acc);
     auto finish = [&](int n, int m, f32x4 v, f32x4 up) {
       if (16 * m + col >= left || ci * per_item + n >= p.tile_cols) return;
       if constexpr (NT >= 2)
@@ -508,16 +524,26 @@ hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E
   return hipGetLastError();
 }
 
+// Waves that a CU holds (by registers), the grid of a launch.
+constexpr int waves_per_cu(int mt, int nt, int parts) {
+  return nt == 4 ? (mt * parts == 1 ? 12 : 8) : (mt == 1 ? 16 : 12);
+}
+
 hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
   if (args.M == 0) return hipSuccess;
   W4KParams p = args;
   const bool experts = p.rb_expert != nullptr;
   auto go = [&](auto mt, auto nt, auto w, auto sub, auto zeros, auto parts, auto ex) {
     constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, W = decltype(w)::value;
-    p.row_blocks = decltype(ex)::value ? p.M / kFlagRows : (p.M + 16 * MT - 1) / (16 * MT);
+    p.row_blocks = (int)(decltype(ex)::value ? p.M / kFlagRows : (p.M + 16 * MT - 1) / (16 * MT));
     const int per_item = p.swiglu ? NT / 2 : NT;
-    const int64_t items = p.row_blocks * (decltype(ex)::value ? kPasses : 1) * ((p.tile_cols + per_item - 1) / per_item);
-    const int64_t grid = std::min<int64_t>(items, (int64_t)cus * (decltype(ex)::value ? 12 : 16) / W);
+    const int64_t items = (int64_t)p.row_blocks * (decltype(ex)::value ? kPasses : 1) * ((p.tile_cols + per_item - 1) / per_item);
+    const int64_t most = (int64_t)cus * waves_per_cu(MT, NT, decltype(parts)::value) / W;
+    int64_t grid = std::min<int64_t>(items, most);
+    if (!decltype(ex)::value) {
+      p.split = choose_split((uint32_t)items, (uint32_t)(most * W), (uint32_t)((p.w.K + kBlock - 1) / kBlock), W);
+      grid = std::min<int64_t>(most, (items * p.split + W - 1) / W);
+    }
     launch<MT, NT, W, decltype(sub)::value, decltype(zeros)::value, decltype(parts)::value, decltype(ex)::value>(
         p, (int)grid, stream);
   };
@@ -539,11 +565,9 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
     if (p.parts == 2) with_group(one, four, four, two, std::true_type());
     else with_group(one, four, four, one, std::true_type());
   } else if (p.M <= 16) {
-    with_group(one, one, eight, one, std::false_type());
-  } else if (p.M <= 32) {
-    with_group(two, one, eight, one, std::false_type());
+    with_group(one, integral_constant<int, W4_NT>(), integral_constant<int, W4_W>(), one, std::false_type());
   } else {
-    with_group(four, one, eight, one, std::false_type());
+    with_group(two, integral_constant<int, W4_NT2>(), integral_constant<int, W4_W2>(), one, std::false_type());
   }
   return hipGetLastError();
 }
