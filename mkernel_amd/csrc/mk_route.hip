@@ -2,14 +2,16 @@
 // per-expert counts and the balance loss in one pass over the logits, and the
 // gradient of the logits.
 //
-// One wavefront per token; lane l holds experts l, l + 64, ... in registers.
-// A choice is the maximum over (ordered bits of the logit, lowest index), so
-// ids do not depend on how a sum is ordered, and ties go to the lowest index.
+// 16 logits per lane in registers, so 4 lanes (up to 64 experts) to 64 per token
+// and 16 tokens to one per wavefront.  A choice is the maximum over (ordered
+// bits of the logit, lowest index) as one number, so ids do not depend on how a
+// sum is ordered, and ties go to the lowest index.
 // The balance loss needs sums over all tokens: every workgroup writes its
 // tokens' sums to the workspace and a second kernel adds them in workgroup
 // order, so results do not depend on timing either.
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "mk_device.h"
 #include "mk_internal.h"
@@ -18,55 +20,214 @@ namespace mk {
 namespace {
 
 constexpr int kWaves = 4, kThreadsR = 64 * kWaves;
-constexpr int kMaxBlocks = 1024;   // workgroups of a launch with balance sums
-constexpr int kFinishExperts = 16; // experts per workgroup of the second kernel
-
-// Bits of x ordered as unsigned integers: -0 equals +0, NaN above all.
-__device__ __forceinline__ uint32_t ordered(float x) {
-  if (x != x) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(x + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-constexpr uint32_t kOrderedNegInf = 0x007fffffu;
+constexpr int kMaxBlocks = 1024;    // workgroups of a launch with balance sums, and
+constexpr int kMaxParts = 1 << 17;  // at most this many sums of one expert and workgroup
+constexpr int kFinishExperts = 8;   // experts per workgroup of the second kernel
 
 // exp(x) for x <= 0 to about an ulp: the product with log2 e carried in two
-// parts, since one rounding of it is |x| times as large in the result.
+// parts, since one rounding of it is |x| times as large in the result.  Below
+// -200 (and for -inf and NaN) the result is 0.
 __device__ __forceinline__ float exp_neg(float x) {
   constexpr float kLog2e = 1.44269502162933349609375f, kLog2eLo = 1.92596299112661746887e-8f;
+  x = fmaxf(x, -200.f);
   const float hi = x * kLog2e;
-  float lo = fmaf(x, kLog2e, -hi);
-  lo = fmaf(x, kLog2eLo, lo);
+  const float lo = fmaf(x, kLog2eLo, fmaf(x, kLog2e, -hi));
   const float e = __builtin_amdgcn_exp2f(hi);
-  return hi == -INFINITY ? 0.f : fmaf(e, lo * 0.693147182464599609375f, e);
+  return fmaf(e, lo * 0.693147182464599609375f, e);
+}
+
+// Keys: numbers whose order is that of (logit, lowest index): -0 equals +0, NaN
+// above all.  A bf16 logit leaves room for its index in 32 bits.  A float takes
+// 44, as the fraction of a double in [1, 2), so that one v_max_f64 compares
+// both at the rate of a 32-bit one.
+template <class T>
+struct Key;
+template <>
+struct Key<uint16_t> {
+  using type = uint32_t;
+  static constexpr type kNone = 0;
+  static __device__ __forceinline__ type make(float x, uint32_t index) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    const uint32_t o = x != x ? 0xffff0000u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    return (o & 0xffff0000u) | (0xffffu - index);
+  }
+  static __device__ __forceinline__ uint32_t index(type k) { return 0xffffu - (k & 0xffffu); }
+  static __device__ __forceinline__ float value(type k) {
+    const uint32_t o = k & 0xffff0000u;
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o & 0xffff0000u);
+  }
+  static __device__ __forceinline__ type top(type a, type b) { return max(a, b); }
+  static __device__ __forceinline__ type low(type a, type b) { return min(a, b); }
+  template <int CTRL>
+  static __device__ __forceinline__ type dpp(type k) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)k, CTRL, 0xf, 0xf, true);
+  }
+  static __device__ __forceinline__ type shuffle(type k, int mask) { return (uint32_t)__shfl_xor((int)k, mask, 64); }
+};
+template <>
+struct Key<float> {
+  using type = double;
+  static constexpr type kNone = 0.0;
+  static __device__ __forceinline__ type pack(uint32_t hi, uint32_t lo) {
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  }
+  static __device__ __forceinline__ type make(float x, uint32_t index) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    const uint32_t o = x != x ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    return pack(0x3ff00000u | o >> 12, o << 20 | (0xfffffu - index));
+  }
+  static __device__ __forceinline__ uint32_t index(type k) {
+    return 0xfffffu - ((uint32_t)__builtin_bit_cast(uint64_t, k) & 0xfffffu);
+  }
+  static __device__ __forceinline__ float value(type k) {
+    const uint32_t o = (uint32_t)(__builtin_bit_cast(uint64_t, k) >> 20);
+    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+  }
+  static __device__ __forceinline__ type top(type a, type b) { return __builtin_fmax(a, b); }
+  static __device__ __forceinline__ type low(type a, type b) { return __builtin_fmin(a, b); }
+  template <int CTRL>
+  static __device__ __forceinline__ type dpp(type k) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, k);
+    return pack((uint32_t)__builtin_amdgcn_mov_dpp((int)(b >> 32), CTRL, 0xf, 0xf, true),
+                (uint32_t)__builtin_amdgcn_mov_dpp((int)b, CTRL, 0xf, 0xf, true));
+  }
+  static __device__ __forceinline__ type shuffle(type k, int mask) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, k);
+    return pack((uint32_t)__shfl_xor((int)(b >> 32), mask, 64), (uint32_t)__shfl_xor((int)b, mask, 64));
+  }
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// All of the L neighbouring lanes of a token get op over their values.  Inside a
+// row of 16 lanes the partner comes as a DPP operand: lane ^ 1, lane ^ 2, then
+// mirrored halves (whose quads, and whose halves, hold one value by then).
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+template <int L, class V, class Op, class Dpp, class Shuffle>
+__device__ __forceinline__ V across(V v, Op op, Dpp d, Shuffle sh) {
+  using std::integral_constant;
+  v = op(v, d(v, integral_constant<int, kXor1>()));
+  v = op(v, d(v, integral_constant<int, kXor2>()));
+  if constexpr (L >= 8) v = op(v, d(v, integral_constant<int, kHalfMirror>()));
+  if constexpr (L >= 16) v = op(v, d(v, integral_constant<int, kMirror>()));
+  if constexpr (L >= 32) v = op(v, sh(v, 16));
+  if constexpr (L >= 64) v = op(v, sh(v, 32));
+  return v;
+}
+
+template <int L, class Op>
+__device__ __forceinline__ float row_float(float v, Op op) {
+  return across<L>(v, op, [](float x, auto c) { return dpp<decltype(c)::value>(x); },
+                   [](float x, int m) { return __shfl_xor(x, m, 64); });
+}
+template <int L>
+__device__ __forceinline__ float row_sum(float v) {
+  return row_float<L>(v, [](float a, float b) { return a + b; });
+}
+template <int L>
+__device__ __forceinline__ float row_max(float v) {
+  return row_float<L>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int L, class T>
+__device__ __forceinline__ typename Key<T>::type row_top(typename Key<T>::type v) {
+  using K = Key<T>;
+  using V = typename K::type;
+  return across<L>(v, [](V a, V b) { return K::top(a, b); },
+                   [](V x, auto c) { return K::template dpp<decltype(c)::value>(x); },
+                   [](V x, int m) { return K::shuffle(x, m); });
+}
+
+// The exchanges of a sorting network of V (a power of two) by odd-even merges,
+// made by the compiler: every index is a constant, so keys stay in registers.
+template <int V>
+struct Network {
+  int n = 0, a[V * V / 2 + 1] = {}, b[V * V / 2 + 1] = {};
+  constexpr Network() {
+    for (int p = 1; p < V; p *= 2)
+      for (int k = p; k >= 1; k /= 2)
+        for (int j = k % p; j + k < V; j += 2 * k)
+          for (int i = 0; i < k; ++i)
+            if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+              a[n] = i + j;
+              b[n++] = i + j + k;
+            }
+  }
+};
+
+template <class T, int V, size_t... I>
+__device__ __forceinline__ void exchange(typename Key<T>::type (&a)[V], std::index_sequence<I...>) {
+  constexpr Network<V> net;
+  auto one = [&](int hi, int lo) {
+    const auto x = a[hi], y = a[lo];
+    a[hi] = Key<T>::top(x, y);
+    a[lo] = Key<T>::low(x, y);
+  };
+  (one(net.a[I], net.b[I]), ...);
+}
+
+// Falling order of a lane's V keys.
+template <class T, int V>
+__device__ __forceinline__ void sort_keys(typename Key<T>::type (&a)[V]) {
+  constexpr Network<V> net;
+  exchange<T, V>(a, std::make_index_sequence<net.n>());
+}
+
+// Where a lane's values lie: V of them in pieces of C neighbours.
+template <int L, int C>
+__device__ __forceinline__ int expert_of(int lane, int j) {
+  return (j / C) * (L * C) + lane * C + j % C;
 }
 
 template <class T>
-__device__ __forceinline__ float load_logit(const T* p) {
+__device__ __forceinline__ float load_one(const T* p) {
   if constexpr (sizeof(T) == 2) return __uint_as_float((uint32_t)*p << 16);
   else return *p;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
+template <class T, int V, int L, int C>
+__device__ __forceinline__ void load_row(float (&x)[V], const T* row, int E, int lane, bool on) {
 #pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
+  for (int j = 0; j < V; j += C) {
+    const int e = expert_of<L, C>(lane, j);
+    if (on && e < E) {  // (C > 1: E is a multiple of it)
+      if constexpr (C == 1) {
+        x[j] = load_one(row + e);
+      } else if constexpr (sizeof(T) == 2) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 v = *reinterpret_cast<const u32x2*>(row + e);
+        x[j] = bf16_lo(v[0]);
+        x[j + 1] = bf16_hi(v[0]);
+        x[j + 2] = bf16_lo(v[1]);
+        x[j + 3] = bf16_hi(v[1]);
+      } else {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(row + e);
 #pragma unroll
-  for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
-  return v;
+        for (int i = 0; i < 4; ++i) x[j + i] = v[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) x[j + i] = -INFINITY;
+    }
+  }
 }
 
-// V values per lane (64 V >= E).
-template <class T, int V>
+// V values per lane, L lanes per token, KM the most choices (a lane keeps its
+// KM largest, sorted; the winner of a round of maxima leaves its lane's list).
+template <class T, int V, int L, int C, int KM>
 __global__ __launch_bounds__(kThreadsR) void route_kernel(RouteKParams p) {
-  __shared__ float psum[kWaves][64 * V];
-  __shared__ int cnt[64 * V];
+  using K = Key<T>;
+  using KeyT = typename K::type;
+  constexpr int R = 64 / L, S = (KM + L - 1) / L, D = V < KM ? V : KM;
+  __shared__ float psum[kWaves][L * V];
+  __shared__ int cnt[L * V];
   __shared__ int live_s;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & (L - 1), sub = (threadIdx.x & 63) / L;
   const bool balance = p.part_sum != nullptr;
   if (balance) {
-    for (int e = threadIdx.x; e < 64 * V; e += kThreadsR) cnt[e] = 0;
+    for (int e = threadIdx.x; e < L * V; e += kThreadsR) cnt[e] = 0;
     if (threadIdx.x == 0) live_s = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
     __syncthreads();
@@ -75,76 +236,90 @@ __global__ __launch_bounds__(kThreadsR) void route_kernel(RouteKParams p) {
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
   int live = 0;
-  for (int64_t t = (int64_t)blockIdx.x * kWaves + wave; t < p.T; t += (int64_t)gridDim.x * kWaves) {
-    if (p.mask && !p.mask[t]) {
-      if (lane < p.k) {
-        p.ids[t * p.k + lane] = -1;
-        p.gates[t * p.k + lane] = 0.f;
-      }
-      continue;
-    }
-    const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+  const int64_t stride = (int64_t)gridDim.x * kWaves * R;
+  int64_t t = ((int64_t)blockIdx.x * kWaves + wave) * R + sub;
+  auto present = [&](int64_t u) { return u < p.T && (!p.mask || p.mask[u]); };
+  float next[V];
+  load_row<T, V, L, C>(next, static_cast<const T*>(p.logits) + t * p.ld, p.E, lane, present(t));
+  for (; t - sub < p.T; t += stride) {
     float x[V];
-    uint64_t key[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = lane + 64 * j;
-      x[j] = e < p.E ? load_logit(row + e) : -INFINITY;
-      key[j] = (uint64_t)ordered(x[j]) << 32 | (uint32_t)(0xffff - e);
-    }
-    int my_id = -1;
-    float my_x = -INFINITY, m = -INFINITY;
+    for (int j = 0; j < V; ++j) x[j] = next[j];
+    // the next token's logits are on their way while this one's are ranked
+    if (t - sub + stride < p.T)
+      load_row<T, V, L, C>(next, static_cast<const T*>(p.logits) + (t + stride) * p.ld, p.E, lane, present(t + stride));
+    KeyT key[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = K::make(x[j], expert_of<L, C>(lane, j));
+    sort_keys<T, V>(key);
+    int id[S];
+    float top[S], m = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < S; ++s) id[s] = -1, top[s] = -INFINITY;
     for (int r = 0; r < p.k; ++r) {
-      uint64_t best = 0;
+      const KeyT best = row_top<L, T>(key[0]);
+      const bool won = key[0] == best;
 #pragma unroll
-      for (int j = 0; j < V; ++j) best = key[j] > best ? key[j] : best;
-#pragma unroll
-      for (int d = 32; d; d >>= 1) {
-        const uint64_t o = (uint64_t)__shfl_xor((uint32_t)(best >> 32), d, 64) << 32 | __shfl_xor((uint32_t)best, d, 64);
-        best = o > best ? o : best;
+      for (int i = 0; i < D; ++i) {
+        // (by value: a choice between two elements would index the array)
+        const KeyT here = key[i], then = i + 1 < D ? +key[i + 1 < D ? i + 1 : i] : K::kNone;
+        key[i] = won ? then : here;
       }
-      if ((uint32_t)(best >> 32) <= kOrderedNegInf) break;
-      const int id = 0xffff - (int)(uint32_t)best;
-      float v = 0.f;
+      const float v = K::value(best);
+      if (r == 0) m = best == K::kNone ? -INFINITY : v;
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (key[j] == best) {
-          key[j] = 0;
-          v = x[j];
+      for (int s = 0; s < S; ++s)
+        if (lane + s * L == r && best != K::kNone && v != -INFINITY) {
+          id[s] = (int)K::index(best);
+          top[s] = v;
         }
-      v = __shfl(v, id & 63, 64);
-      if (r == 0) m = v;
-      if (lane == r) {
-        my_id = id;
-        my_x = v;
-      }
     }
     const bool alive = m != -INFINITY;
-    float e[V], z = 0.f;
+    float e[V], z = 1.f;
+    if (balance || !p.renorm) {
+      z = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      e[j] = alive ? exp_neg(x[j] - m) : 0.f;
-      z += e[j];
+      for (int j = 0; j < V; ++j) {
+        e[j] = exp_neg(x[j] - m);  // (a row with NaN or +inf: all 0, and 0 / 0 below)
+        z += e[j];
+      }
+      z = row_sum<L>(z);
     }
-    z = wave_sum(z);
-    float g = my_id >= 0 ? exp_neg(my_x - m) : 0.f;
-    const float zg = p.renorm ? wave_sum(g) : z;
-    if (my_id >= 0) g /= zg;
-    if (lane < p.k) {
-      p.ids[t * p.k + lane] = my_id;
-      p.gates[t * p.k + lane] = g;
+    float g[S], zg = z;
+#pragma unroll
+    for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? exp_neg(top[s] - m) : 0.f;
+    if (p.renorm) {
+      zg = 0.f;
+#pragma unroll
+      for (int s = 0; s < S; ++s) zg += g[s];
+      zg = row_sum<L>(zg);
+    }
+    if (t < p.T) {
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (lane + s * L < p.k) {
+          p.ids[t * p.k + lane + s * L] = id[s];
+          p.gates[t * p.k + lane + s * L] = id[s] >= 0 ? g[s] / zg : 0.f;
+        }
     }
     if (balance && alive) {
-      ++live;
+      live += lane == 0;
+      const float inv = 1.f / z;
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] += e[j] / z;
-      if (my_id >= 0) atomicAdd(&cnt[my_id], 1);
+      for (int j = 0; j < V; ++j) acc[j] += e[j] * inv;
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (id[s] >= 0) atomicAdd(&cnt[id[s]], 1);
     }
   }
   if (!balance) return;
-  if (lane == 0) atomicAdd(&live_s, live);
+  if (live) atomicAdd(&live_s, live);
 #pragma unroll
-  for (int j = 0; j < V; ++j) psum[wave][lane + 64 * j] = acc[j];
+  for (int j = 0; j < V; ++j) {
+#pragma unroll
+    for (int d = L; d < 64; d *= 2) acc[j] += __shfl_xor(acc[j], d, 64);
+    if (sub == 0) psum[wave][expert_of<L, C>(lane, j)] = acc[j];
+  }
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += kThreadsR) {
     float s = 0.f;
@@ -159,22 +334,36 @@ __global__ __launch_bounds__(kThreadsR) void route_kernel(RouteKParams p) {
 // Sums the workgroups' parts in order, kFinishExperts experts per workgroup;
 // the last workgroup to finish adds the experts' shares of the loss.
 __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int nparts) {
-  constexpr int kSlices = 256 / kFinishExperts;
+  constexpr int kSlices = 256 / kFinishExperts, kAhead = 8;
   __shared__ double sums[kSlices][kFinishExperts];
   __shared__ int cnts[kSlices][kFinishExperts];
-  __shared__ int last;
+  __shared__ int last, total;
   const int x = threadIdx.x % kFinishExperts, slice = threadIdx.x / kFinishExperts;
   const int e = blockIdx.x * kFinishExperts + x;
   double s = 0.0;
-  int c = 0;
-  if (e < p.E)
-    for (int b = slice; b < nparts; b += kSlices) {
-      s += p.part_sum[(int64_t)b * p.E + e];
-      c += p.part_cnt[(int64_t)b * p.E + e];
+  int c = 0, n = 0;
+  if (threadIdx.x == 0) total = 0;
+  for (int b0 = slice; b0 < nparts; b0 += kAhead * kSlices) {
+    float ps[kAhead];
+    int pc[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int b = b0 + i * kSlices;
+      const bool in = e < p.E && b < nparts;
+      ps[i] = in ? p.part_sum[(int64_t)b * p.E + e] : 0.f;
+      pc[i] = in ? p.part_cnt[(int64_t)b * p.E + e] : 0;
     }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      s += ps[i];
+      c += pc[i];
+    }
+  }
+  for (int b = threadIdx.x; b < nparts; b += 256) n += p.part_live[b];
   sums[slice][x] = s;
   cnts[slice][x] = c;
   __syncthreads();
+  atomicAdd(&total, n);
   if (slice == 0) {
     for (int i = 1; i < kSlices; ++i) {
       s += sums[i][x];
@@ -194,179 +383,260 @@ __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int n
     last = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
   }
   __syncthreads();
-  if (!last) return;
-  int n = 0;
-  for (int b = threadIdx.x; b < nparts; b += 256) n += p.part_live[b];
-  __shared__ int total;
-  if (threadIdx.x == 0) total = 0;
-  __syncthreads();
-  atomicAdd(&total, n);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double sum = 0.0;
-    for (int b = 0; b < (int)gridDim.x; ++b)
-      sum += __hip_atomic_load(p.shares + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *p.tokens = total;
-    *p.loss = total ? (float)((double)p.coef * p.E * sum / ((double)p.k * total * total)) : 0.f;
-  }
+  if (!last || threadIdx.x >= 64) return;
+  double sum = 0.0;  // at most kMaxExperts / kFinishExperts shares: two per lane
+  for (int b = threadIdx.x; b < (int)gridDim.x; b += 64)
+    sum += __hip_atomic_load(p.shares + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+  if (threadIdx.x != 0) return;
+  *p.tokens = total;
+  *p.loss = total ? (float)((double)p.coef * p.E * sum / ((double)p.k * total * total)) : 0.f;
 }
 
-template <class T, int V>
+template <class T, int V, int L, int C, int KM>
 __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKParams p) {
-  __shared__ float add[kWaves][64 * V];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int R = 64 / L, S = (KM + L - 1) / L;
+  // the gates' part of the gradient, by expert; zero but between a token's writes and reads
+  __shared__ __align__(16) float add_s[kWaves * R][L * V];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & (L - 1), sub = (threadIdx.x & 63) / L;
+  float* add = add_s[wave * R + sub];
+  const int64_t stride = (int64_t)gridDim.x * kWaves * R;
+  int64_t t = ((int64_t)blockIdx.x * kWaves + wave) * R + sub;
+  auto present = [&](int64_t u) { return u < p.T && (!p.mask || p.mask[u]); };
+  // a token's logits, choices and their gates' gradients
+  struct Token {
+    float x[V], dg[S];
+    int id[S];
+    bool on;
+  } next;
+  auto fetch = [&](int64_t u) {
+    next.on = present(u);
+    load_row<T, V, L, C>(next.x, static_cast<const T*>(p.logits) + u * p.ld, p.E, lane, next.on);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int i = lane + s * L;
+      const bool in = p.dgates && next.on && i < p.k;
+      next.id[s] = in ? p.ids[u * p.k + i] : -1;
+      next.dg[s] = in ? p.dgates[u * p.k + i] : 0.f;
+    }
+  };
+  fetch(t);
   // counts, and what a probability's gradient is multiplied with
   float f[V], scale = 0.f;
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = 0.f;
+  for (int j = 0; j < V; ++j) {
+    const int e = expert_of<L, C>(lane, j);
+    f[j] = p.counts && e < p.E ? (float)p.counts[e] : 0.f;
+    add[e] = 0.f;
+  }
   if (p.counts) {
     const double n = *p.tokens;
     if (n > 0) scale = (float)((double)p.coef * (p.dloss ? *p.dloss : 1.f) * p.E / ((double)p.k * n * n));
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = lane + 64 * j;
-      if (e < p.E) f[j] = (float)p.counts[e];
-    }
   }
-  for (int64_t t = (int64_t)blockIdx.x * kWaves + wave; t < p.T; t += (int64_t)gridDim.x * kWaves) {
-    T* out = static_cast<T*>(p.dlogits) + t * p.ld_out;
-    auto store = [&](int e, float v) {
-      if constexpr (sizeof(T) == 2) out[e] = __builtin_bit_cast(uint16_t, (__bf16)v);
-      else out[e] = v;
-    };
+  for (; t - sub < p.T; t += stride) {
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-    float x[V], m = -INFINITY;
-    const bool on = !p.mask || p.mask[t];
-    bool nan = false;
+    float x[V], dg[S], xc[S];
+    int id[S];
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = next.x[j];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      id[s] = next.id[s] < p.E ? next.id[s] : -1;
+      dg[s] = id[s] >= 0 ? next.dg[s] : 0.f;
+      xc[s] = id[s] >= 0 ? load_one(row + id[s]) : -INFINITY;
+    }
+    // the next token's are on their way meanwhile (an output over the logits
+    // does not reach them: every row is read and written by the same lanes)
+    if (t - sub + stride < p.T) fetch(t + stride);
+    float m = -INFINITY;
+    int odd = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int e = lane + 64 * j;
-      x[j] = on && e < p.E ? load_logit(row + e) : -INFINITY;
-      nan |= x[j] != x[j];
       m = fmaxf(m, x[j]);
+      odd |= x[j] != x[j];
     }
-    m = __any(nan) ? NAN : wave_max(m);
-    if (m == -INFINITY) {  // a token that does not count, or that no expert is left for
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (lane + 64 * j < p.E) store(lane + 64 * j, 0.f);
-      continue;
-    }
-    float pr[V], z = 0.f;
+    m = row_max<L>(m);
+    odd = row_max<L>(odd ? 1.f : 0.f) != 0.f || m == INFINITY;  // a NaN or +inf: the whole row is NaN
+    const bool alive = m != -INFINITY || odd;  // else the token does not count, or no expert is left for it
+    float pr[V], z = 0.f, s0 = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       pr[j] = exp_neg(x[j] - m);
       z += pr[j];
+      s0 += pr[j] * f[j];
     }
-    z = wave_sum(z);
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      pr[j] /= z;
-      s += pr[j] * f[j];
-    }
-    s = wave_sum(s);
-    // the gates' part: lane i has choice i
-    int id = -1;
-    float dg = 0.f, v = 0.f, dense = 0.f;
+    z = row_sum<L>(z);
+    const float inv = odd ? NAN : alive ? 1.f / z : 0.f;
+    s0 = row_sum<L>(s0) * inv;
+    float v[S], dense = 0.f;
     if (p.dgates) {
-      if (lane < p.k) id = p.ids[t * p.k + lane];
-      if (id >= p.E) id = -1;
-      float xc = -INFINITY;
-      if (id >= 0) {
-        dg = p.dgates[t * p.k + lane];
-        xc = load_logit(row + id);
-      }
+      float g[S], sum = 0.f, dot = 0.f;
       if (p.renorm) {
-        const float mc = wave_max(xc);
-        float g = id >= 0 && mc != -INFINITY ? exp_neg(xc - mc) : 0.f;
-        g /= fmaxf(wave_sum(g), 1e-30f);
-        if (z != z) g = z;
-        const float dot = wave_sum(id >= 0 ? g * dg : 0.f);
-        v = id >= 0 ? g * (dg - dot) : 0.f;
+        float mc = xc[0];
+#pragma unroll
+        for (int s = 1; s < S; ++s) mc = fmaxf(mc, xc[s]);
+        mc = row_max<L>(mc);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          g[s] = xc[s] != -INFINITY ? exp_neg(xc[s] - mc) : 0.f;
+          sum += g[s];
+        }
+        sum = row_sum<L>(sum);
+        sum = sum > 0.f ? 1.f / sum : 0.f;
       } else {
-        const float g = id >= 0 ? exp_neg(xc - m) / z : 0.f;
-        v = g * dg;
-        dense = wave_sum(v);
+        sum = inv;
+#pragma unroll
+        for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? exp_neg(xc[s] - m) : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) add[wave][lane + 64 * j] = 0.f;
-      // an expert named twice: its first lane adds all, in lane order
-      float all = 0.f;
-      bool first = id >= 0;
-      for (int i = 0; i < p.k; ++i) {
-        const int oi = __shfl(id, i, 64);
-        const float ov = __shfl(v, i, 64);
-        if (oi == id) {
-          all += ov;
-          if (i < lane) first = false;
+      for (int s = 0; s < S; ++s) {
+        g[s] *= sum;
+        dot += g[s] * dg[s];
+      }
+      dot = row_sum<L>(dot);
+      if (!p.renorm) dense = dot;
+#pragma unroll
+      for (int s = 0; s < S; ++s) v[s] = g[s] * (p.renorm ? dg[s] - dot : dg[s]);
+      // An expert named twice gets the sum, in the order of the choices: every
+      // choice leaves its number at its expert's place, and only where one does
+      // not find its own there again are they added one after another.
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (id[s] >= 0) add[id[s]] = __int_as_float(lane + s * L);
+      __builtin_amdgcn_wave_barrier();
+      bool twice = false;
+#pragma unroll
+      for (int s = 0; s < S; ++s) twice |= id[s] >= 0 && __float_as_int(add[id[s]]) != lane + s * L;
+      __builtin_amdgcn_wave_barrier();
+      if (!__any(twice)) {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+          if (id[s] >= 0) add[id[s]] = v[s];
+      } else {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+          if (id[s] >= 0) add[id[s]] = 0.f;
+        for (int i = 0; i < p.k; ++i) {
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+            if (id[s] >= 0 && lane + s * L == i) add[id[s]] += v[s];
         }
       }
       __builtin_amdgcn_wave_barrier();
-      if (first) add[wave][id] = all;
-      __builtin_amdgcn_wave_barrier();
     }
+    float d[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int e = lane + 64 * j;
-      float d = pr[j] * (scale * (f[j] - s) - dense);
-      if (p.dgates) d += add[wave][e];
-      if (e < p.E) store(e, d);
+      d[j] = alive ? pr[j] * inv * (scale * (f[j] - s0) - dense) : 0.f;
+      if (p.dgates) d[j] += add[expert_of<L, C>(lane, j)];
+      if (odd) d[j] = NAN;
+    }
+    if (p.dgates) {
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        if (id[s] >= 0) add[id[s]] = 0.f;
+    }
+    if (t >= p.T) continue;
+    T* out = static_cast<T*>(p.dlogits) + t * p.ld_out;
+#pragma unroll
+    for (int j = 0; j < V; j += C) {
+      const int e = expert_of<L, C>(lane, j);
+      if (e >= p.E) continue;
+      if constexpr (C == 1) {
+        if constexpr (sizeof(T) == 2) out[e] = __builtin_bit_cast(uint16_t, (__bf16)d[j]);
+        else out[e] = d[j];
+      } else if constexpr (sizeof(T) == 2) {
+        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+        *reinterpret_cast<u32x2*>(out + e) = u32x2{pack_bf16x2(d[j], d[j + 1]), pack_bf16x2(d[j + 2], d[j + 3])};
+      } else {
+        *reinterpret_cast<f32x4*>(out + e) = f32x4{d[j], d[j + 1], d[j + 2], d[j + 3]};
+      }
     }
   }
 }
 
-int route_blocks(int64_t T, bool balance) {
-  const int64_t all = (T + kWaves - 1) / kWaves;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(all, balance ? kMaxBlocks : 1 << 20));
+// Lanes and values per lane for E experts, pieces of C, and at most 8 or
+// kMaxTopk choices.
+template <class F>
+void by_shape(int E, bool vector, int k, F&& f) {
+  using std::integral_constant;
+  auto choices = [&](auto v, auto l, auto c) {
+    if (k <= 8) f(v, l, c, integral_constant<int, 8>());
+    else f(v, l, c, integral_constant<int, kMaxTopk>());
+  };
+  auto pieces = [&](auto v, auto l) {
+    if (vector) choices(v, l, integral_constant<int, 4>());
+    else choices(v, l, integral_constant<int, 1>());
+  };
+  constexpr integral_constant<int, 16> v;
+  if (E <= 64) pieces(v, integral_constant<int, 4>());
+  else if (E <= 128) pieces(v, integral_constant<int, 8>());
+  else if (E <= 256) pieces(v, integral_constant<int, 16>());
+  else if (E <= 512) pieces(v, integral_constant<int, 32>());
+  else pieces(v, integral_constant<int, 64>());
 }
 
-template <class F>
-void by_width(int E, F&& f) {
-  if (E <= 64) f(std::integral_constant<int, 1>());
-  else if (E <= 128) f(std::integral_constant<int, 2>());
-  else if (E <= 256) f(std::integral_constant<int, 4>());
-  else if (E <= 512) f(std::integral_constant<int, 8>());
-  else f(std::integral_constant<int, 16>());
+int tokens_per_block(int E) { return kWaves * (E <= 64 ? 16 : E <= 128 ? 8 : E <= 256 ? 4 : E <= 512 ? 2 : 1); }
+
+int route_blocks(int64_t T, int E) {
+  const int64_t all = (T + tokens_per_block(E) - 1) / tokens_per_block(E);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({all, kMaxBlocks, kMaxParts / E}));
+}
+
+// Whether rows can be read (written) in pieces of four neighbours.
+bool pieces_of_four(const void* rows, int64_t ld, int E, int bf16) {
+  const int size = bf16 ? 2 : 4;
+  return E % 4 == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(rows) % (4 * size) == 0;
 }
 
 }  // namespace
 
 int64_t route_workspace_bytes(int64_t T, int E) {
-  const int64_t nb = route_blocks(T, true);
+  const int64_t nb = route_blocks(T, E);
   const int64_t shares = (E + kFinishExperts - 1) / kFinishExperts;
   return (8 * shares + 8 + nb * (8 * (int64_t)E + 4) + 255) / 256 * 256;
 }
 
 hipError_t launch_route(RouteKParams p, void* ws, hipStream_t stream) {
   const bool balance = ws != nullptr;
-  const int nb = route_blocks(p.T, balance);
+  int64_t nb = route_blocks(p.T, p.E);
   const int shares = (p.E + kFinishExperts - 1) / kFinishExperts;
   if (balance) {
     p.shares = static_cast<double*>(ws);
     p.ticket = reinterpret_cast<uint32_t*>(p.shares + shares);
     p.part_sum = reinterpret_cast<float*>(p.ticket + 2);
-    p.part_cnt = reinterpret_cast<int*>(p.part_sum + (int64_t)nb * p.E);
-    p.part_live = p.part_cnt + (int64_t)nb * p.E;
+    p.part_cnt = reinterpret_cast<int*>(p.part_sum + nb * p.E);
+    p.part_live = p.part_cnt + nb * p.E;
   } else if (p.T == 0) {
     return hipSuccess;
+  } else {
+    nb = std::min<int64_t>((p.T + tokens_per_block(p.E) - 1) / tokens_per_block(p.E), kMaxBlocks);
   }
-  by_width(p.E, [&](auto v) {
-    constexpr int V = decltype(v)::value;
-    if (p.bf16) hipLaunchKernelGGL((route_kernel<uint16_t, V>), dim3(nb), dim3(kThreadsR), 0, stream, p);
-    else hipLaunchKernelGGL((route_kernel<float, V>), dim3(nb), dim3(kThreadsR), 0, stream, p);
+  by_shape(p.E, pieces_of_four(p.logits, p.ld, p.E, p.bf16), p.k, [&](auto v, auto l, auto c, auto km) {
+    constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value, KM = decltype(km)::value;
+    if (p.bf16)
+      hipLaunchKernelGGL((route_kernel<uint16_t, V, L, C, KM>), dim3((unsigned)nb), dim3(kThreadsR), 0, stream, p);
+    else
+      hipLaunchKernelGGL((route_kernel<float, V, L, C, KM>), dim3((unsigned)nb), dim3(kThreadsR), 0, stream, p);
   });
-  if (balance) hipLaunchKernelGGL(route_finish_kernel, dim3(shares), dim3(256), 0, stream, p, nb);
+  if (balance) hipLaunchKernelGGL(route_finish_kernel, dim3(shares), dim3(256), 0, stream, p, (int)nb);
   return hipGetLastError();
 }
 
 hipError_t launch_route_backward(const RouteBwdKParams& p, hipStream_t stream) {
   if (p.T == 0) return hipSuccess;
-  const int nb = route_blocks(p.T, false);
-  by_width(p.E, [&](auto v) {
-    constexpr int V = decltype(v)::value;
-    if (p.bf16) hipLaunchKernelGGL((route_backward_kernel<uint16_t, V>), dim3(nb), dim3(kThreadsR), 0, stream, p);
-    else hipLaunchKernelGGL((route_backward_kernel<float, V>), dim3(nb), dim3(kThreadsR), 0, stream, p);
+  const int64_t nb = std::min<int64_t>((p.T + tokens_per_block(p.E) - 1) / tokens_per_block(p.E), 2 * kMaxBlocks);
+  const bool vector = pieces_of_four(p.logits, p.ld, p.E, p.bf16) && pieces_of_four(p.dlogits, p.ld_out, p.E, p.bf16);
+  by_shape(p.E, vector, p.k, [&](auto v, auto l, auto c, auto km) {
+    constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value, KM = decltype(km)::value;
+    if (p.bf16)
+      hipLaunchKernelGGL((route_backward_kernel<uint16_t, V, L, C, KM>), dim3((unsigned)nb), dim3(kThreadsR), 0, stream, p);
+    else
+      hipLaunchKernelGGL((route_backward_kernel<float, V, L, C, KM>), dim3((unsigned)nb), dim3(kThreadsR), 0, stream, p);
   });
   return hipGetLastError();
 }
