@@ -20,21 +20,28 @@ namespace mk {
 namespace {
 
 constexpr int kWaves = 4, kThreadsR = 64 * kWaves;
-constexpr int kMaxBlocks = 1024;    // workgroups of a launch with balance sums, and
-constexpr int kMaxParts = 1 << 17;  // at most this many sums of one expert and workgroup
-constexpr int kFinishExperts = 8;   // experts per workgroup of the second kernel
+constexpr int kWavesSum = 8;        // with balance sums: fewer workgroups, so fewer parts to add
+constexpr int kMaxBlocks = 2048;
+constexpr int kMaxParts = 512;      // workgroups with balance sums
+constexpr int kFinishExperts = 4;   // experts per workgroup of the second kernel
 
-// exp(x) for x <= 0 to about an ulp: the product with log2 e carried in two
-// parts, since one rounding of it is |x| times as large in the result.  Below
-// -200 (and for -inf and NaN) the result is 0.
-__device__ __forceinline__ float exp_neg(float x) {
-  constexpr float kLog2e = 1.44269502162933349609375f, kLog2eLo = 1.92596299112661746887e-8f;
-  x = fmaxf(x, -200.f);
-  const float hi = x * kLog2e;
-  const float lo = fmaf(x, kLog2eLo, fmaf(x, kLog2e, -hi));
-  const float e = __builtin_amdgcn_exp2f(hi);
-  return fmaf(e, lo * 0.693147182464599609375f, e);
-}
+// exp(x - m) for every x of a token, m their maximum (and not -inf): 2^(x c - m c)
+// with c = log2 e.  The product m c is rounded once, to `shift`; that error is
+// one factor of all of a token's exponentials and cancels in their quotients.
+// What is left is one rounding of the exponent: |x - m| half steps of the
+// result, as much as the rounding of a difference x - m, and 0.3 as much from
+// c.  Where m c overflows (|m| > 2^127), the difference is taken first instead.
+// A row with NaN or +inf gives NaN.
+constexpr float kLog2e = 1.44269502162933349609375f;
+struct ExpOf {
+  float m, shift;
+  bool far;
+  __device__ __forceinline__ explicit ExpOf(float m_) : m(m_), shift(m_ * kLog2e), far(__any(fabsf(m_) > 0x1p127f)) {}
+  __device__ __forceinline__ float operator()(float x) const {
+    if (far) return __builtin_amdgcn_exp2f((x - m) * kLog2e);
+    return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -shift));
+  }
+};
 
 // Keys: numbers whose order is that of (logit, lowest index): -0 equals +0, NaN
 // above all.  A bf16 logit leaves room for its index in 32 bits.  A float takes
@@ -217,17 +224,17 @@ __device__ __forceinline__ void load_row(float (&x)[V], const T* row, int E, int
 // V values per lane, L lanes per token, KM the most choices (a lane keeps its
 // KM largest, sorted; the winner of a round of maxima leaves its lane's list).
 template <class T, int V, int L, int C, int KM>
-__global__ __launch_bounds__(kThreadsR) void route_kernel(RouteKParams p) {
+__global__ __launch_bounds__(64 * kWavesSum) void route_kernel(RouteKParams p) {
   using K = Key<T>;
   using KeyT = typename K::type;
   constexpr int R = 64 / L, S = (KM + L - 1) / L, D = V < KM ? V : KM;
-  __shared__ float psum[kWaves][L * V];
+  extern __shared__ float psum[];  // [waves][L * V], with balance sums
   __shared__ int cnt[L * V];
   __shared__ int live_s;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & (L - 1), sub = (threadIdx.x & 63) / L;
+  const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & (L - 1), sub = (threadIdx.x & 63) / L;
   const bool balance = p.part_sum != nullptr;
   if (balance) {
-    for (int e = threadIdx.x; e < L * V; e += kThreadsR) cnt[e] = 0;
+    for (int e = threadIdx.x; e < L * V; e += blockDim.x) cnt[e] = 0;
     if (threadIdx.x == 0) live_s = 0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.ticket = 0;
     __syncthreads();
@@ -236,8 +243,8 @@ __global__ __launch_bounds__(kThreadsR) void route_kernel(RouteKParams p) {
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
   int live = 0;
-  const int64_t stride = (int64_t)gridDim.x * kWaves * R;
-  int64_t t = ((int64_t)blockIdx.x * kWaves + wave) * R + sub;
+  const int64_t stride = (int64_t)gridDim.x * waves * R;
+  int64_t t = ((int64_t)blockIdx.x * waves + wave) * R + sub;
   auto present = [&](int64_t u) { return u < p.T && (!p.mask || p.mask[u]); };
   float next[V];
   load_row<T, V, L, C>(next, static_cast<const T*>(p.logits) + t * p.ld, p.E, lane, present(t));
@@ -275,19 +282,20 @@ __global__ __launch_bounds__(kThreadsR) void route_kernel(RouteKParams p) {
         }
     }
     const bool alive = m != -INFINITY;
+    const ExpOf exp_of(alive ? m : 0.f);
     float e[V], z = 1.f;
     if (balance || !p.renorm) {
       z = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        e[j] = exp_neg(x[j] - m);  // (a row with NaN or +inf: all 0, and 0 / 0 below)
+        e[j] = exp_of(x[j]);
         z += e[j];
       }
       z = row_sum<L>(z);
     }
     float g[S], zg = z;
 #pragma unroll
-    for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? exp_neg(top[s] - m) : 0.f;
+    for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? exp_of(top[s]) : 0.f;
     if (p.renorm) {
       zg = 0.f;
 #pragma unroll
@@ -318,13 +326,12 @@ __global__ __launch_bounds__(kThreadsR) void route_kernel(RouteKParams p) {
   for (int j = 0; j < V; ++j) {
 #pragma unroll
     for (int d = L; d < 64; d *= 2) acc[j] += __shfl_xor(acc[j], d, 64);
-    if (sub == 0) psum[wave][expert_of<L, C>(lane, j)] = acc[j];
+    if (sub == 0) psum[wave * (L * V) + expert_of<L, C>(lane, j)] = acc[j];
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < p.E; e += kThreadsR) {
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += psum[w][e];
+    for (int w = 0; w < waves; ++w) s += psum[w * (L * V) + e];
     p.part_sum[(int64_t)blockIdx.x * p.E + e] = s;
     p.part_cnt[(int64_t)blockIdx.x * p.E + e] = cnt[e];
   }
@@ -334,7 +341,7 @@ __global__ __launch_bounds__(kThreadsR) void route_kernel(RouteKParams p) {
 // Sums the workgroups' parts in order, kFinishExperts experts per workgroup;
 // the last workgroup to finish adds the experts' shares of the loss.
 __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int nparts) {
-  constexpr int kSlices = 256 / kFinishExperts, kAhead = 8;
+  constexpr int kSlices = 256 / kFinishExperts, kAhead = 16;
   __shared__ double sums[kSlices][kFinishExperts];
   __shared__ int cnts[kSlices][kFinishExperts];
   __shared__ int last, total;
@@ -379,12 +386,14 @@ __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int n
   if (threadIdx.x == 0) {
     double share = 0.0;
     for (int i = 0; i < kFinishExperts; ++i) share += sums[0][i];
+    // written through to agent scope and waited for: a plain ticket orders it
     __hip_atomic_store(p.shares + blockIdx.x, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    wait_vmem_all();
+    last = __hip_atomic_fetch_add(p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
   }
   __syncthreads();
   if (!last || threadIdx.x >= 64) return;
-  double sum = 0.0;  // at most kMaxExperts / kFinishExperts shares: two per lane
+  double sum = 0.0;  // one share per kFinishExperts experts
   for (int b = threadIdx.x; b < (int)gridDim.x; b += 64)
     sum += __hip_atomic_load(p.shares + b, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
@@ -459,10 +468,11 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
     m = row_max<L>(m);
     odd = row_max<L>(odd ? 1.f : 0.f) != 0.f || m == INFINITY;  // a NaN or +inf: the whole row is NaN
     const bool alive = m != -INFINITY || odd;  // else the token does not count, or no expert is left for it
+    const ExpOf exp_of(alive ? m : 0.f);
     float pr[V], z = 0.f, s0 = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      pr[j] = exp_neg(x[j] - m);
+      pr[j] = exp_of(x[j]);
       z += pr[j];
       s0 += pr[j] * f[j];
     }
@@ -477,9 +487,10 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
 #pragma unroll
         for (int s = 1; s < S; ++s) mc = fmaxf(mc, xc[s]);
         mc = row_max<L>(mc);
+        const ExpOf exp_c(mc != -INFINITY ? mc : 0.f);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-          g[s] = xc[s] != -INFINITY ? exp_neg(xc[s] - mc) : 0.f;
+          g[s] = xc[s] != -INFINITY ? exp_c(xc[s]) : 0.f;
           sum += g[s];
         }
         sum = row_sum<L>(sum);
@@ -487,7 +498,7 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
       } else {
         sum = inv;
 #pragma unroll
-        for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? exp_neg(xc[s] - m) : 0.f;
+        for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? exp_of(xc[s]) : 0.f;
       }
 #pragma unroll
       for (int s = 0; s < S; ++s) {
@@ -580,11 +591,12 @@ void by_shape(int E, bool vector, int k, F&& f) {
   else pieces(v, integral_constant<int, 64>());
 }
 
-int tokens_per_block(int E) { return kWaves * (E <= 64 ? 16 : E <= 128 ? 8 : E <= 256 ? 4 : E <= 512 ? 2 : 1); }
+int tokens_per_wave(int E) { return E <= 64 ? 16 : E <= 128 ? 8 : E <= 256 ? 4 : E <= 512 ? 2 : 1; }
 
-int route_blocks(int64_t T, int E) {
-  const int64_t all = (T + tokens_per_block(E) - 1) / tokens_per_block(E);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({all, kMaxBlocks, kMaxParts / E}));
+// Workgroups of `waves` waves, one token group per wave where that many are allowed.
+int route_blocks(int64_t T, int E, int waves, int most) {
+  const int64_t each = tokens_per_wave(E) * waves;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((T + each - 1) / each, most));
 }
 
 // Whether rows can be read (written) in pieces of four neighbours.
@@ -596,14 +608,15 @@ bool pieces_of_four(const void* rows, int64_t ld, int E, int bf16) {
 }  // namespace
 
 int64_t route_workspace_bytes(int64_t T, int E) {
-  const int64_t nb = route_blocks(T, E);
+  const int64_t nb = route_blocks(T, E, kWavesSum, kMaxParts);
   const int64_t shares = (E + kFinishExperts - 1) / kFinishExperts;
   return (8 * shares + 8 + nb * (8 * (int64_t)E + 4) + 255) / 256 * 256;
 }
 
 hipError_t launch_route(RouteKParams p, void* ws, hipStream_t stream) {
   const bool balance = ws != nullptr;
-  int64_t nb = route_blocks(p.T, p.E);
+  const int waves = balance ? kWavesSum : kWaves;
+  const int64_t nb = route_blocks(p.T, p.E, waves, balance ? kMaxParts : kMaxBlocks);
   const int shares = (p.E + kFinishExperts - 1) / kFinishExperts;
   if (balance) {
     p.shares = static_cast<double*>(ws);
@@ -613,15 +626,14 @@ hipError_t launch_route(RouteKParams p, void* ws, hipStream_t stream) {
     p.part_live = p.part_cnt + nb * p.E;
   } else if (p.T == 0) {
     return hipSuccess;
-  } else {
-    nb = std::min<int64_t>((p.T + tokens_per_block(p.E) - 1) / tokens_per_block(p.E), kMaxBlocks);
   }
   by_shape(p.E, pieces_of_four(p.logits, p.ld, p.E, p.bf16), p.k, [&](auto v, auto l, auto c, auto km) {
     constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value, KM = decltype(km)::value;
+    const unsigned lds = balance ? waves * L * V * sizeof(float) : 0;
     if (p.bf16)
-      hipLaunchKernelGGL((route_kernel<uint16_t, V, L, C, KM>), dim3((unsigned)nb), dim3(kThreadsR), 0, stream, p);
+      hipLaunchKernelGGL((route_kernel<uint16_t, V, L, C, KM>), dim3((unsigned)nb), dim3(64 * waves), lds, stream, p);
     else
-      hipLaunchKernelGGL((route_kernel<float, V, L, C, KM>), dim3((unsigned)nb), dim3(kThreadsR), 0, stream, p);
+      hipLaunchKernelGGL((route_kernel<float, V, L, C, KM>), dim3((unsigned)nb), dim3(64 * waves), lds, stream, p);
   });
   if (balance) hipLaunchKernelGGL(route_finish_kernel, dim3(shares), dim3(256), 0, stream, p, (int)nb);
   return hipGetLastError();
@@ -629,14 +641,14 @@ hipError_t launch_route(RouteKParams p, void* ws, hipStream_t stream) {
 
 hipError_t launch_route_backward(const RouteBwdKParams& p, hipStream_t stream) {
   if (p.T == 0) return hipSuccess;
-  const int64_t nb = std::min<int64_t>((p.T + tokens_per_block(p.E) - 1) / tokens_per_block(p.E), 2 * kMaxBlocks);
+  const int nb = route_blocks(p.T, p.E, kWaves, kMaxBlocks / 2);
   const bool vector = pieces_of_four(p.logits, p.ld, p.E, p.bf16) && pieces_of_four(p.dlogits, p.ld_out, p.E, p.bf16);
   by_shape(p.E, vector, p.k, [&](auto v, auto l, auto c, auto km) {
     constexpr int V = decltype(v)::value, L = decltype(l)::value, C = decltype(c)::value, KM = decltype(km)::value;
     if (p.bf16)
-      hipLaunchKernelGGL((route_backward_kernel<uint16_t, V, L, C, KM>), dim3((unsigned)nb), dim3(kThreadsR), 0, stream, p);
+      hipLaunchKernelGGL((route_backward_kernel<uint16_t, V, L, C, KM>), dim3(nb), dim3(kThreadsR), 0, stream, p);
     else
-      hipLaunchKernelGGL((route_backward_kernel<float, V, L, C, KM>), dim3((unsigned)nb), dim3(kThreadsR), 0, stream, p);
+      hipLaunchKernelGGL((route_backward_kernel<float, V, L, C, KM>), dim3(nb), dim3(kThreadsR), 0, stream, p);
   });
   return hipGetLastError();
 }

@@ -383,6 +383,12 @@ def _tensor(t, name: str, dtypes, shape=None, dim=None, rows=False, device=None)
         raise ValueError(f"{name} is on {t.device}, not on {device}")
 
 
+def _is(t, dtype, shape, device) -> bool:
+    """The usual case of _tensor, in a third of its time."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device
+            and t.is_contiguous())
+
+
 def _ld(t: torch.Tensor) -> int:
     """Row stride; of a matrix of one row, its width."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -398,11 +404,15 @@ _F32, _BF16, _I32, _U8 = (torch.float32,), (torch.bfloat16,), (torch.int32,), (t
 
 
 def _route_inputs(logits, topk, token_mask):
-    _tensor(logits, "logits", _LOGITS, rows=True)
-    if not 1 <= topk <= logits.shape[1]:
-        raise ValueError(f"topk must be 1 .. {logits.shape[1]}")
-    if token_mask is not None:
-        _tensor(token_mask, "token_mask", (torch.bool, torch.uint8), (logits.shape[0],), device=logits.device)
+    if not (isinstance(logits, torch.Tensor) and logits.dtype in _LOGITS and logits.is_cuda and logits.dim() == 2
+            and logits.is_contiguous()):
+        _tensor(logits, "logits", _LOGITS, rows=True)
+    T, E = logits.shape
+    if not 1 <= topk <= E:
+        raise ValueError(f"topk must be 1 .. {E}")
+    if token_mask is not None and not _is(token_mask, torch.bool, (T,), logits.device):
+        _tensor(token_mask, "token_mask", (torch.bool, torch.uint8), (T,), device=logits.device)
+    return T, E, logits.device
 
 
 def _coef(coef) -> float:
@@ -435,26 +445,27 @@ def moe_route_balance(logits: torch.Tensor, topk: int, coef: float, renorm: bool
 
 
 def _route(logits, topk, renorm, token_mask, coef):
-    _route_inputs(logits, topk, token_mask)
-    T, E = logits.shape
-    dev = logits.device
-    with _on(dev):
-        ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
-        gates = torch.empty((T, topk), dtype=torch.float32, device=dev)
-        if coef is None:
-            extra, balance = (), (0, 0, 0, 0, 0.0, 0, 0)
-        else:
-            # loss, prob_sum | counts, tokens | workspace (made anew: it holds nothing between calls)
-            f = torch.empty(1 + E, dtype=torch.float32, device=dev)
-            i = torch.empty(1 + E, dtype=torch.int32, device=dev)
-            n = int(capi.lib().mk_moe_route_workspace_bytes(T, E))
-            ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
-            extra = (f[:1], i[:E], f[1:], i[E:])
-            balance = (i.data_ptr(), f.data_ptr() + 4, i.data_ptr() + 4 * E, f.data_ptr(), coef, ws.data_ptr(), n)
-        capi.call_values("mk_moe_route", MoeRouteArgs, _stream(), logits.data_ptr(), _ptr(token_mask), ids.data_ptr(),
-                         gates.data_ptr(), T, _ld(logits), E, topk, int(logits.dtype == torch.bfloat16), int(renorm),
-                         *balance)
-    return (ids, gates, *extra)
+    T, E, dev = _route_inputs(logits, topk, token_mask)
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return _route(logits, topk, renorm, token_mask, coef)
+    ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
+    gates = torch.empty((T, topk), dtype=torch.float32, device=dev)
+    out, balance = (ids, gates), (0, 0, 0, 0, 0.0, 0, 0)
+    if coef is not None:
+        # loss, prob_sum | counts, tokens | workspace (made anew: it holds nothing between calls)
+        f = torch.empty(1 + E, dtype=torch.float32, device=dev)
+        i = torch.empty(E + 1, dtype=torch.int32, device=dev)
+        n = capi.lib().mk_moe_route_workspace_bytes(T, E)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+        fp, ip = f.data_ptr(), i.data_ptr()
+        balance = (ip, fp + 4, ip + 4 * E, fp, coef, ws.data_ptr(), n)
+        loss, prob_sum = f.split_with_sizes((1, E))
+        counts, tokens = i.split_with_sizes((E, 1))
+        out += (loss, counts, prob_sum, tokens)
+    capi.call_values("mk_moe_route", MoeRouteArgs, _stream(), logits.data_ptr(), _ptr(token_mask), ids.data_ptr(),
+                     gates.data_ptr(), T, _ld(logits), E, topk, logits.dtype is torch.bfloat16, bool(renorm), *balance)
+    return out
 
 
 def moe_route_backward(logits: torch.Tensor, ids: torch.Tensor, dgates: torch.Tensor | None = None,
@@ -467,36 +478,39 @@ def moe_route_backward(logits: torch.Tensor, ids: torch.Tensor, dgates: torch.Te
     coef and dloss (one float32 on the device; None: 1).  Either part may be
     left out.  ids, renorm and token_mask as in the forward call.  out: where
     to write it; the logits themselves may be given."""
-    if ids is None or not isinstance(ids, torch.Tensor) or ids.dim() != 2:
+    if not isinstance(ids, torch.Tensor) or ids.dim() != 2:
         raise ValueError("ids must be an int32 device tensor [T, topk]")
     topk = ids.shape[1]
-    _route_inputs(logits, topk, token_mask)
-    T, E = logits.shape
-    dev = logits.device
-    _tensor(ids, "ids", _I32, (T, topk), device=dev)
+    T, E, dev = _route_inputs(logits, topk, token_mask)
+    if not _is(ids, torch.int32, (T, topk), dev):
+        _tensor(ids, "ids", _I32, (T, topk), device=dev)
     if dgates is None and counts is None:
         raise ValueError("dgates or counts must be given")
-    if dgates is not None:
+    if dgates is not None and not _is(dgates, torch.float32, (T, topk), dev):
         _tensor(dgates, "dgates", _F32, (T, topk), device=dev)
     if counts is not None:
-        _tensor(counts, "counts", _I32, (E,), device=dev)
-        if tokens is None:
-            raise ValueError("counts needs tokens")
-        _tensor(tokens, "tokens", _I32, device=dev)
-        if tokens.numel() != 1:
-            raise ValueError("tokens must hold one number")
-    if dloss is not None:
+        if not _is(counts, torch.int32, (E,), dev):
+            _tensor(counts, "counts", _I32, (E,), device=dev)
+        if not _is(tokens, torch.int32, (1,), dev):
+            if tokens is None:
+                raise ValueError("counts needs tokens")
+            _tensor(tokens, "tokens", _I32, device=dev)
+            if tokens.numel() != 1:
+                raise ValueError("tokens must hold one number")
+    if dloss is not None and not _is(dloss, torch.float32, (1,), dev):
         _tensor(dloss, "dloss", _F32, device=dev)
         if dloss.numel() != 1:
             raise ValueError("dloss must hold one number")
     if out is not None:
         _tensor(out, "out", (logits.dtype,), (T, E), rows=True, device=dev)
-    with _on(dev):
-        if out is None:
-            out = torch.empty((T, E), dtype=logits.dtype, device=dev)
-        capi.call_values("mk_moe_route_backward", MoeRouteBackwardArgs, _stream(), logits.data_ptr(), _ptr(token_mask),
-                         ids.data_ptr(), _ptr(dgates), _ptr(dloss), _ptr(counts), _ptr(tokens), out.data_ptr(), T,
-                         _ld(logits), _ld(out), E, topk, int(logits.dtype == torch.bfloat16), int(renorm), _coef(coef))
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return moe_route_backward(logits, ids, dgates, dloss, counts, tokens, coef, renorm, token_mask, out)
+    if out is None:
+        out = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    capi.call_values("mk_moe_route_backward", MoeRouteBackwardArgs, _stream(), logits.data_ptr(), _ptr(token_mask),
+                     ids.data_ptr(), _ptr(dgates), _ptr(dloss), _ptr(counts), _ptr(tokens), out.data_ptr(), T,
+                     _ld(logits), _ld(out), E, topk, logits.dtype is torch.bfloat16, bool(renorm), _coef(coef))
     return out
 
 
@@ -518,16 +532,17 @@ def moe_combine_backward(dy: torch.Tensor, y_expert: torch.Tensor, ids: torch.Te
     _tensor(ids, "ids", _I32, (T, None), device=dev)
     k = ids.shape[1]
     _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)
-    _tensor(owner_offset, "owner_offset", _I32, (T + 1,), device=dev)
+    if not _is(owner_offset, torch.int32, (T + 1,), dev):
+        _tensor(owner_offset, "owner_offset", _I32, (T + 1,), device=dev)
     _tensor(slot_to_row, "slot_to_row", _I32, dim=1, device=dev)
     _tensor(rb_rows, "rb_rows", _I32, dim=1, device=dev)
     if row_weight.shape[0] < R_pad or rb_rows.shape[0] * capi.ROW_BLOCK < R_pad:
         raise ValueError("row_weight and rb_rows must cover the rows of y_expert")
-    if sizes is not None:
+    if sizes is not None and not _is(sizes, torch.int64, (2,), dev):
         _tensor(sizes, "sizes", (torch.int64,), (2,), device=dev)
-    if dy_expert is not None:
+    if dy_expert is not None and not _is(dy_expert, torch.bfloat16, (R_pad, H), dev):
         _tensor(dy_expert, "dy_expert", _BF16, (R_pad, H), device=dev)
-    if dgates is not None:
+    if dgates is not None and not _is(dgates, torch.float32, (T, k), dev):
         _tensor(dgates, "dgates", _F32, (T, k), device=dev)
     with _on(dev):
         if dy_expert is None:
@@ -537,7 +552,7 @@ def moe_combine_backward(dy: torch.Tensor, y_expert: torch.Tensor, ids: torch.Te
         capi.call_values("mk_moe_combine_backward", MoeCombineBackwardArgs, _stream(), dy.data_ptr(),
                          y_expert.data_ptr(), ids.data_ptr(), row_weight.data_ptr(), owner_offset.data_ptr(),
                          slot_to_row.data_ptr(), rb_rows.data_ptr(), dy_expert.data_ptr(), dgates.data_ptr(), T, H,
-                         R_pad, k, e0, n_local, int(dy.dtype == torch.bfloat16), _ptr(sizes))
+                         R_pad, k, e0, n_local, dy.dtype is torch.bfloat16, _ptr(sizes))
     return dy_expert, dgates
 
 
@@ -624,7 +639,9 @@ def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> t
     bf16 (what is made where none is given) or float32.  K a multiple of 8, any M and N; rows of A (a multiple of 8 elements
     apart) and of out need only be contiguous each.  The weights are read once
     per 64 rows: from a few hundred rows on, gemm is faster."""
-    _tensor(A, "A", _BF16, rows=True)
+    if not (isinstance(A, torch.Tensor) and A.dtype is torch.bfloat16 and A.is_cuda and A.dim() == 2
+            and A.is_contiguous()):
+        _tensor(A, "A", _BF16, rows=True)
     dev = A.device
     _w4(W, "W", dev, 1)
     M, K = A.shape
@@ -632,11 +649,13 @@ def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> t
         raise ValueError(f"A has {K} columns, the weights {W.K} rows")
     if out is not None:
         _tensor(out, "out", _LOGITS, (M, W.N), rows=True, device=dev)
-    with _on(dev):
-        if out is None:
-            out = torch.empty((M, W.N), dtype=torch.bfloat16, device=dev)
-        capi.call_values("mk_gemm_w4", GemmW4Args, _stream(), A.data_ptr(), out.data_ptr(), *W._values(), M, _ld(A),
-                         _ld(out), int(out.dtype == torch.bfloat16))
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return gemm_w4(A, W, out)
+    if out is None:
+        out = torch.empty((M, W.N), dtype=torch.bfloat16, device=dev)
+    capi.call_values("mk_gemm_w4", GemmW4Args, _stream(), A.data_ptr(), out.data_ptr(), *W._values(), M, _ld(A),
+                     _ld(out), out.dtype is torch.bfloat16)
     return out
 
 
