@@ -1229,7 +1229,7 @@ static int prepare_grouped_w4(const char* fn, const mk_moe_grouped_gemm_w4_args*
   if (a->mode == 1 && a->W.N % 32) return fail(MK_ESHAPE, "%s: N must be a multiple of 32 with SwiGLU", fn);
   if (a->R_pad < 0 || a->R_pad % MK_ROW_BLOCK || a->R_pad > (1 << 21))
     return fail(MK_ESHAPE, "%s: R_pad must be a multiple of %d up to 2^21", fn, MK_ROW_BLOCK);
-  if (a->R_pad / 16 * ((a->W.N + 15) / 16) >= (1LL << 31)) return fail(MK_ESHAPE, "%s: R_pad x N too large", fn);
+  if (a->R_pad / 8 * ((a->W.N + 15) / 16) >= (1LL << 31)) return fail(MK_ESHAPE, "%s: R_pad x N too large", fn);
   if (a->R_pad > 0) {
     if (!a->A || !a->out || !a->rb_expert) return fail(MK_EINVAL, "%s: null argument", fn);
     if (!aligned16(a->A) || !aligned16(a->out)) return fail(MK_EINVAL, "%s: A and out must be 16-byte aligned", fn);

@@ -67,12 +67,12 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) 
 
 // What one step of 128 rows of K needs: packed codes, scales (of this lane's
 // four columns, group by group), zero points (of its one column) and x.
-template <int MT, int NT, int SUB, bool ZEROS, int PARTS>
+template <int MT, int NT, int SUB, bool ZEROS>
 struct Step {
   u32x4 w[NT];
   uint32_t s[NT][2 * (4 / SUB)];
   uint32_t z[ZEROS ? NT : 1];
-  u32x4 x[PARTS][MT][4];
+  u32x4 x[MT][4];
 };
 
 // Descriptors of a wave's column tiles (each tile's codes, scales and zeros are
@@ -85,11 +85,10 @@ struct Source {
   uint32_t last;     // last step
   uint32_t row[MT];  // byte offset of this lane's row, kNowhere where there is none
   int32_t most;      // last multiple of 8 below K, less this lane's first k in a step
-  uint32_t K;
 };
 
-template <int MT, int NT, int SUB, bool ZEROS, int PARTS>
-__device__ __forceinline__ void load(Step<MT, NT, SUB, ZEROS, PARTS>& st, const Source<MT, NT>& t, uint32_t kb, int lane) {
+template <int MT, int NT, int SUB, bool ZEROS>
+__device__ __forceinline__ void load(Step<MT, NT, SUB, ZEROS>& st, const Source<MT, NT>& t, uint32_t kb, int lane) {
   constexpr int G = 4 / SUB;
   // scales past the last step are the last one's: they multiply zeros
   const uint32_t sb = min(kb, t.last);
@@ -115,15 +114,12 @@ __device__ __forceinline__ void load(Step<MT, NT, SUB, ZEROS, PARTS>& st, const 
   for (int j = 0; j < 4; ++j) {
     const bool in = (int32_t)(kb * kBlock) + j * 32 <= t.most;
 #pragma unroll
-    for (int h = 0; h < PARTS; ++h)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        st.x[h][m][j] = load16(t.x, in ? t.row[m] + kb * 256 + 2 * (j * 32 + h * t.K) : kNowhere);
+    for (int m = 0; m < MT; ++m) st.x[m][j] = load16(t.x, in ? t.row[m] + kb * 256 + 64 * j : kNowhere);
   }
 }
 
-template <int MT, int NT, int SUB, bool ZEROS, int PARTS>
-__device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, PARTS>& st, uint32_t mask, uint32_t bias,
+template <int MT, int NT, int SUB, bool ZEROS>
+__device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS>& st, uint32_t mask, uint32_t bias,
                                          f32x4 (&acc)[NT][MT]) {
 #pragma unroll
   for (int g = 0; g < 4 / SUB; ++g) {
@@ -135,9 +131,7 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, PARTS>& 
         base[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < SUB; ++i)
-#pragma unroll
-          for (int h = 0; h < PARTS; ++h)
-            base[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(off, __builtin_bit_cast(bf16x8, st.x[h][m][g * SUB + i]), base[m], 0, 0, 0);
+          base[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(off, __builtin_bit_cast(bf16x8, st.x[m][g * SUB + i]), base[m], 0, 0, 0);
       }
     }
 #pragma unroll
@@ -149,14 +143,12 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, PARTS>& 
       for (int i = 0; i < SUB; ++i) {
         const bf16x8 q = expand(st.w[n][g * SUB + i], mask, bias);
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int h = 0; h < PARTS; ++h) {
-            const bf16x8 xv = __builtin_bit_cast(bf16x8, st.x[h][m][g * SUB + i]);
-            if constexpr (ZEROS)
-              part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus_offset((st.z[n] >> (8 * g)) & 255u), xv, part[m], 0, 0, 0);
-            part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, xv, part[m], 0, 0, 0);
-          }
+        for (int m = 0; m < MT; ++m) {
+          const bf16x8 xv = __builtin_bit_cast(bf16x8, st.x[m][g * SUB + i]);
+          if constexpr (ZEROS)
+            part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus_offset((st.z[n] >> (8 * g)) & 255u), xv, part[m], 0, 0, 0);
+          part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, xv, part[m], 0, 0, 0);
+        }
       }
       const f32x4 s = {bf16_lo(st.s[n][2 * g]), bf16_hi(st.s[n][2 * g]), bf16_lo(st.s[n][2 * g + 1]), bf16_hi(st.s[n][2 * g + 1])};
 #pragma unroll
@@ -173,13 +165,13 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, PARTS>& 
 // for its own only.  The last P steps load nothing more (a load that nobody
 // needs would still be waited for before its registers are used again); those
 // past the end found zeros.
-template <int MT, int NT, int SUB, bool ZEROS, int PARTS, int P>
+template <int MT, int NT, int SUB, bool ZEROS, int P>
 __device__ __forceinline__ void sweep(const Source<MT, NT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
                                       f32x4 (&acc)[NT][MT]) {
   uint32_t mask = 0x000f000fu, bias = 0x43004300u;
   asm volatile("" : "+s"(mask));
   asm volatile("" : "+v"(bias));
-  Step<MT, NT, SUB, ZEROS, PARTS> st[P];
+  Step<MT, NT, SUB, ZEROS> st[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     load(st[i], t, first + i * stride, lane);
@@ -250,11 +242,14 @@ __host__ __device__ __forceinline__ int choose_split(uint32_t items, uint32_t wa
   return best;
 }
 
-// The row passes (16 rows each) of the real rows of up to kListed row blocks.
-constexpr int kListed = 512, kPasses = kFlagRows / 16;
+// The row passes of the real rows of up to kListed row blocks: 16 rows each, or
+// 8 where x goes as bf16 pairs, whose second halves take the other 8 lanes (the
+// two sums of a row are added at the end).
+constexpr int kListed = 512;
+template <int ROWS>
 struct PassList {
-  int first[kListed + 1];             // first pass of each block
-  uint16_t block[kListed * kPasses];  // block of each pass
+  int first[kListed + 1];                        // first pass of each block
+  uint16_t block[kListed * (kFlagRows / ROWS)];  // block of each pass
   int scratch[17];
 };
 
@@ -286,8 +281,9 @@ __device__ __forceinline__ int block_rows(const W4KParams& p, int64_t b) {
 template <int MT, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS>
 __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
   extern __shared__ f32x4 red[];  // [W][NT * MT][64], used where K is split
-  __shared__ PassList list;
-  static_assert(!EXPERTS || MT == 1, "passes of 16 rows");
+  constexpr int ROWS = PARTS == 2 ? 8 : 16, kPasses = kFlagRows / ROWS;  // of a pass over experts' rows
+  __shared__ PassList<ROWS> list;
+  static_assert(MT == 1 || (!EXPERTS && PARTS == 1), "passes of 16 rows");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const uint32_t KB = (uint32_t)((p.w.K + kBlock - 1) / kBlock);
@@ -309,7 +305,7 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
 #pragma unroll
       for (int i = 0; i < per; ++i) {
         const int b = threadIdx.x * per + i;
-        n[i] = b < blocks ? (block_rows(p, b) + 15) / 16 : 0;
+        n[i] = b < blocks ? (block_rows(p, b) + ROWS - 1) / ROWS : 0;
         sum += n[i];
       }
       int at = prefix<W>(sum, list.scratch);
@@ -352,9 +348,9 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
         const int local = (int)(it - q * col_items);
         ci = local / np;
         pass = local - ci * np;
-        left = __builtin_amdgcn_readfirstlane(block_rows(p, b)) - 16 * pass;
+        left = __builtin_amdgcn_readfirstlane(block_rows(p, b)) - ROWS * pass;
         expert = __builtin_amdgcn_readfirstlane(p.rb_expert[b]);
-        row0 = (int64_t)b * kFlagRows + 16 * pass;
+        row0 = (int64_t)b * kFlagRows + ROWS * pass;
       } else {
         const uint32_t b = it / col_items;
         ci = (int)(it - b * col_items);
@@ -374,7 +370,6 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
       if constexpr (ZEROS) t.z[n] = p.w.zeros + at * groups * kTile;
     }
     t.last = KB - 1;
-    t.K = (uint32_t)p.w.K;
     t.most = (int32_t)p.w.K - 8 - quad * 8;
     // lanes past the last row read nothing; their results are not stored
     if (EXPERTS && p.gather_pull) {
@@ -390,13 +385,22 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
       }
     } else {
       t.x = make_rsrc(p.A + row0 * p.lda, (uint32_t)(min(max(left, 0), 16 * MT) * p.lda * 2));
+      const int r = PARTS == 2 ? col & 7 : col;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
-        t.row[m] = 16 * m + col < left ? (uint32_t)((16 * m + col) * p.lda * 2) + quad * 16 : kNowhere;
+        t.row[m] = 16 * m + r < left ? (uint32_t)((16 * m + r) * p.lda * 2 + (r < col ? 2 * p.w.K : 0)) + quad * 16 : kNowhere;
     }
     f32x4 acc[NT][MT];
-    sweep<MT, NT, SUB, ZEROS, PARTS, (MT * PARTS * NT == 1 ? W4_P1 : 2)>(t, KB, left > 0 ? ks : KB, split, lane, acc);
+    sweep<MT, NT, SUB, ZEROS, (MT * NT == 1 ? W4_P1 : 2)>(t, KB, left > 0 ? ks : KB, split, lane, acc);
     auto finish = [&](int n, int m, f32x4 v, f32x4 up) {
+      if constexpr (PARTS == 2) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          v[r] += __shfl_xor(v[r], 8, 64);
+          up[r] += __shfl_xor(up[r], 8, 64);
+        }
+        if (col >= 8) return;
+      }
       if (16 * m + col >= left || ci * per_item + n >= p.tile_cols) return;
       if constexpr (NT >= 2)
         if (p.swiglu)
@@ -525,8 +529,8 @@ hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E
 }
 
 // Waves that a CU holds (by registers), the grid of a launch.
-constexpr int waves_per_cu(int mt, int nt, int parts) {
-  return nt == 4 ? (mt * parts == 1 ? 12 : 8) : (mt == 1 ? 16 : 12);
+constexpr int waves_per_cu(int mt, int nt) {
+  return nt == 4 ? (mt == 1 ? 12 : 8) : (mt == 1 ? 16 : 12);
 }
 
 hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
@@ -537,8 +541,9 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
     constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, W = decltype(w)::value;
     p.row_blocks = (int)(decltype(ex)::value ? p.M / kFlagRows : (p.M + 16 * MT - 1) / (16 * MT));
     const int per_item = p.swiglu ? NT / 2 : NT;
-    const int64_t items = (int64_t)p.row_blocks * (decltype(ex)::value ? kPasses : 1) * ((p.tile_cols + per_item - 1) / per_item);
-    const int64_t most = (int64_t)cus * waves_per_cu(MT, NT, decltype(parts)::value) / W;
+    const int passes = decltype(ex)::value ? kFlagRows / (decltype(parts)::value == 2 ? 8 : 16) : 1;
+    const int64_t items = (int64_t)p.row_blocks * passes * ((p.tile_cols + per_item - 1) / per_item);
+    const int64_t most = (int64_t)cus * waves_per_cu(MT, NT) / W;
     int64_t grid = std::min<int64_t>(items, most);
     if (!decltype(ex)::value) {
       p.split = choose_split((uint32_t)items, (uint32_t)(most * W), (uint32_t)((p.w.K + kBlock - 1) / kBlock), W);
