@@ -592,21 +592,19 @@ int mk_moe_combine_backward(const mk_moe_combine_backward_args* args, void* stre
  * it.  The products read them in an order of their own, laid out once by
  * mk_w4_pack; E matrices (experts) of one shape lie one after another. */
 typedef struct mk_w4_weights {
-  void* packed;      /* mk_w4_packed_bytes bytes, 16-byte aligned */
-  void* scales;      /* bf16 [mk_w4_scale_count], 16-byte aligned */
-  void* zeros;       /* uint8 [mk_w4_scale_count], or NULL */
+  void* packed;      /* mk_w4_packed_bytes bytes, 16-byte aligned: codes, scales and zero points */
   int64_t K, N;
   int32_t group, num_experts;
+  int32_t has_zeros; /* 0: the zero point is 8 */
 } mk_w4_weights;
-int64_t mk_w4_packed_bytes(int64_t K, int64_t N, int32_t num_experts);
-int64_t mk_w4_scale_count(int64_t K, int64_t N, int32_t num_experts, int32_t group);
+int64_t mk_w4_packed_bytes(int64_t K, int64_t N, int32_t num_experts, int32_t group, int32_t has_zeros);
 
 /* Lays out codes uint8 [E, K, N] (the low four bits of each byte), scales bf16
  * [E, ceil(K / group), N] and zero points uint8 of the scales' shape. */
 typedef struct mk_w4_pack_args {
   const void* codes;
   const void* scales;
-  const void* zeros;    /* NULL exactly when out.zeros is */
+  const void* zeros;    /* set exactly when out.has_zeros is */
   mk_w4_weights out;
 } mk_w4_pack_args;
 int mk_w4_pack(const mk_w4_pack_args* args, void* stream);

@@ -39,7 +39,6 @@ EXPORTS = (
     "mk_moe_route_backward",
     "mk_moe_combine_backward",
     "mk_w4_packed_bytes",
-    "mk_w4_scale_count",
     "mk_w4_pack",
     "mk_w4_quantize",
     "mk_gemm_w4",
@@ -170,8 +169,7 @@ class MoeCombineBackwardArgs(C.Structure):
 
 
 class W4WeightsC(C.Structure):
-    _fields_ = [("packed", vp), ("scales", vp), ("zeros", vp), ("K", i64), ("N", i64), ("group", i32),
-                ("num_experts", i32)]
+    _fields_ = [("packed", vp), ("K", i64), ("N", i64), ("group", i32), ("num_experts", i32), ("has_zeros", i32)]
 
 
 class W4PackArgs(C.Structure):
@@ -226,10 +224,8 @@ def lib() -> C.CDLL:
         L.mk_moe_index_workspace_bytes.restype = i64
         L.mk_moe_route_workspace_bytes.argtypes = [i64, i32]
         L.mk_moe_route_workspace_bytes.restype = i64
-        L.mk_w4_packed_bytes.argtypes = [i64, i64, i32]
+        L.mk_w4_packed_bytes.argtypes = [i64, i64, i32, i32, i32]
         L.mk_w4_packed_bytes.restype = i64
-        L.mk_w4_scale_count.argtypes = [i64, i64, i32, i32]
-        L.mk_w4_scale_count.restype = i64
         L.mk_moe_build_indices_dev.argtypes = [vp, vp]
         L.mk_moe_build_indices_dev.restype = C.c_int
         L.mk_moe_invert_slots.argtypes = [vp, vp, i64, i32, i64, vp, vp, vp]
@@ -280,12 +276,19 @@ _functions: dict = {}
 
 
 def _letters(cls):
-    return "".join(_FORMAT.get(t) or _letters(t) for _, t in cls._fields_)
+    # a nested block's values come one by one in their place (it starts at its
+    # first field's alignment), then the bytes that fill it up
+    fmt = ""
+    for _, t in cls._fields_:
+        inner = _FORMAT.get(t)
+        if inner is None:
+            inner = _letters(t)
+            inner += "x" * (C.sizeof(t) - struct.calcsize("@" + inner))
+        fmt += inner
+    return fmt
 
 
 def _packer(cls):
-    # a nested block's values come one by one in their place (its alignment is
-    # that of its first field, its size a multiple of it)
     fmt = "@" + _letters(cls)
     fmt += "x" * (C.sizeof(cls) - struct.calcsize(fmt))
     pack = _packers[cls] = struct.Struct(fmt).pack

@@ -1140,33 +1140,27 @@ static bool w4_sizes(int64_t K, int64_t N, int32_t E, int32_t group) {
          (group == 32 || group == 64 || group == 128);
 }
 
-int64_t mk_w4_packed_bytes(int64_t K, int64_t N, int32_t num_experts) {
-  return w4_sizes(K, N, num_experts, 128) ? 4 * mk::w4_packed_words(K, N, num_experts) : -1;
-}
-
-int64_t mk_w4_scale_count(int64_t K, int64_t N, int32_t num_experts, int32_t group) {
-  return w4_sizes(K, N, num_experts, group) ? mk::w4_scale_count(K, N, num_experts, group) : -1;
+int64_t mk_w4_packed_bytes(int64_t K, int64_t N, int32_t num_experts, int32_t group, int32_t has_zeros) {
+  return w4_sizes(K, N, num_experts, group) ? mk::w4_packed_bytes(K, N, num_experts, group, has_zeros != 0) : -1;
 }
 
 static int check_w4(const char* fn, const mk_w4_weights& w) {
-  if (!w.packed || !w.scales) return fail(MK_EINVAL, "%s: null weights", fn);
+  if (!w.packed) return fail(MK_EINVAL, "%s: null weights", fn);
   if (w.group != 32 && w.group != 64 && w.group != 128) return fail(MK_EINVAL, "%s: group must be 32, 64 or 128", fn);
   if (!w4_sizes(w.K, w.N, w.num_experts, w.group)) return fail(MK_ESHAPE, "%s: bad weight sizes", fn);
-  if (!aligned16(w.packed) || !aligned16(w.scales))
-    return fail(MK_EINVAL, "%s: packed weights and scales must be 16-byte aligned", fn);
+  if (!aligned16(w.packed)) return fail(MK_EINVAL, "%s: packed weights must be 16-byte aligned", fn);
   return MK_OK;
 }
 
 int mk_w4_pack(const mk_w4_pack_args* a, void* stream) {
   if (!a || !a->codes || !a->scales) return fail(MK_EINVAL, "mk_w4_pack: null argument");
   if (int rc = check_w4("mk_w4_pack", a->out)) return rc;
-  if (!a->zeros != !a->out.zeros) return fail(MK_EINVAL, "mk_w4_pack: zeros given on one side only");
+  if (!a->zeros != !a->out.has_zeros) return fail(MK_EINVAL, "mk_w4_pack: zeros given on one side only");
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   hipError_t e = mk::launch_w4_pack(static_cast<const uint8_t*>(a->codes), static_cast<const uint16_t*>(a->scales),
                                     static_cast<const uint8_t*>(a->zeros), a->out.K, a->out.N, a->out.num_experts,
-                                    a->out.group, static_cast<uint32_t*>(a->out.packed),
-                                    static_cast<uint16_t*>(a->out.scales), static_cast<uint8_t*>(a->out.zeros),
+                                    a->out.group, static_cast<unsigned char*>(a->out.packed),
                                     static_cast<hipStream_t>(stream));
   return e == hipSuccess ? MK_OK : hip_fail(e, "mk_w4_pack launch");
 }
@@ -1187,8 +1181,7 @@ int mk_w4_quantize(const mk_w4_quantize_args* a, void* stream) {
 static mk::W4KParams w4_params(const mk_w4_weights& w, const void* A, void* C, int64_t M, int64_t lda, int64_t ldc) {
   mk::W4KParams p;
   std::memset(&p, 0, sizeof p);
-  p.w = {static_cast<const uint32_t*>(w.packed), static_cast<const uint16_t*>(w.scales),
-         static_cast<const uint8_t*>(w.zeros), w.K, w.N, w.group, w.num_experts};
+  p.w = {static_cast<const unsigned char*>(w.packed), w.K, w.N, w.group, w.num_experts, w.has_zeros != 0};
   p.A = static_cast<const uint16_t*>(A);
   p.C = C;
   p.M = M; p.lda = lda; p.ldc = ldc;

@@ -222,11 +222,10 @@ hipError_t launch_route_backward(const RouteBwdKParams& p, hipStream_t stream);
 
 // Products with 4-bit weights (mk_w4.hip).
 struct W4Weights {
-  const uint32_t* packed;   // [E][tiles][blocks][64 lanes][4]
-  const uint16_t* scales;   // [E][tiles][blocks][4 quads][groups of a block][4 columns]
-  const uint8_t* zeros;     // [E][tiles][blocks][16 columns][groups of a block], or null: 8
+  const unsigned char* packed;   // [E][tile pairs][blocks] of two tiles' codes, scales and zero points
   int64_t K, N;
   int group, E;
+  bool zeros;                    // whether there are zero points (else 8)
 };
 enum W4Out : int { kW4F32 = 0, kW4Bf16 = 1, kW4Pair = 2 };
 struct W4KParams {
@@ -247,12 +246,10 @@ struct W4KParams {
   int gather_tps, gather_devs;
   const int64_t* rows_dev;
 };
-int64_t w4_packed_words(int64_t K, int64_t N, int64_t E);
-int64_t w4_scale_count(int64_t K, int64_t N, int64_t E, int group);
+int64_t w4_packed_bytes(int64_t K, int64_t N, int64_t E, int group, bool zeros);
 hipError_t launch_w4(const W4KParams& p, int cus, hipStream_t stream);
 hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int64_t K, int64_t N,
-                          int64_t E, int group, uint32_t* packed, uint16_t* packed_scales, uint8_t* packed_zeros,
-                          hipStream_t stream);
+                          int64_t E, int group, unsigned char* packed, hipStream_t stream);
 hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E, int group, uint8_t* codes,
                               uint16_t* scales, hipStream_t stream);
 

@@ -7,15 +7,17 @@
 // in the order in which the matrix instruction reads them: a 16-byte unit per
 // lane holds the 32 codes that lane feeds to four 16 x 16 x 32 MFMAs (16
 // columns, 128 rows of K), so a wave reads 1 KB in one piece and nothing goes
-// through LDS on the way in.
+// through LDS on the way in.  Two such tiles of neighbouring columns and their
+// scales and zero points are one block, the blocks of a pair of tiles one run
+// along K: a wave's reads stay in few pages.
 //
 // A code becomes the bf16 number 128 + q by setting bits (0x4300 | q, exact);
 // the product with the constant -(128 + z) is one more MFMA into the same
 // accumulator.  A group's sum of x * (q - z) is then multiplied with its scale
 // in fp32: no rounding but the fp32 sums' and the one of the result.
 //
-// The weights are the first operand, so a lane of the result holds four
-// neighbouring columns of one row of x.  The waves of a workgroup share a
+// x is the first operand, so a lane of the result holds one column of four rows
+// of x, and needs that column's scale only.  The waves of a workgroup share a
 // column tile and split K; their sums meet in LDS in wave order.
 #include <algorithm>
 #include <type_traits>
@@ -23,13 +25,6 @@
 #include "mk_device.h"
 #include "mk_internal.h"
 
-#ifndef W4_NT
-#define W4_NT 1
-#define W4_W 8
-#define W4_NT2 4
-#define W4_W2 8
-#define W4_P1 3
-#endif
 namespace mk {
 namespace {
 
@@ -65,62 +60,101 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) 
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
 }
 
-// What one step of 128 rows of K needs: packed codes, scales (of this lane's
-// four columns, group by group), zero points (of its one column) and x.
-template <int MT, int NT, int SUB, bool ZEROS>
+// What one step of 128 rows of K needs: packed codes, scales and zero points of
+// this lane's column (a word has both tiles of a pair, group by group), and x.
+//
+// An MFMA takes x as 16 rows by 32 of K, 16 bytes per lane; the step's four are
+// XQ = 4 loads.  With at most 4 rows three quarters of those lanes would load
+// nothing, so one load (XQ = 1) brings the four MFMAs' parts at once, lane
+// 4 j + r of 16 the part of row r for MFMA j, and a rotation by 4 j lanes moves
+// them in place (the other lanes then hold parts of other MFMAs, which end in
+// rows that are not stored).  The loads of x, mostly empty, were the largest
+// cost of a decode step beside the weights: 12 of 67 us.
+template <int MT, int NT, int SUB, bool ZEROS, int XQ>
 struct Step {
   u32x4 w[NT];
-  uint32_t s[NT][2 * (4 / SUB)];
-  uint32_t z[ZEROS ? NT : 1];
-  u32x4 x[MT][4];
+  static constexpr int PAIRS = NT == 4 ? 2 : NT;  // four tiles are two pairs; else each tile reads its pair's
+  uint32_t s[PAIRS][4 / SUB];
+  uint32_t z[ZEROS ? PAIRS : 1][SUB == 1 ? 2 : 1];
+  u32x4 x[MT][XQ];
 };
 
-// Descriptors of a wave's column tiles (each tile's codes, scales and zeros are
-// one piece) and of its rows of x.
+// Lane i of each 16 gets lane i + 4 J.
+template <int J>
+__device__ __forceinline__ u32x4 from_quarter(u32x4 v) {
+  if constexpr (J > 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = (uint32_t)__builtin_amdgcn_mov_dpp((int)v[i], 0x120 + 16 - 4 * J /* row_ror */, 0xf, 0xf, true);
+  }
+  return v;
+}
+
+// Bytes of a block: two tiles' codes, their scales [16 columns][groups][2 tiles]
+// and zero points (the same order).
+constexpr uint32_t block_bytes(int groups, bool zeros) { return 2048u + 64u * groups + (zeros ? 32u * groups : 0u); }
+
+// A wave's pairs of column tiles (the run of blocks of each) and its rows of x.
 template <int MT, int NT>
 struct Source {
-  __amdgpu_buffer_rsrc_t w[NT], x;
-  const char* s[NT];
-  const uint8_t* z[NT];
-  uint32_t last;     // last step
+  __amdgpu_buffer_rsrc_t w[NT == 4 ? 2 : NT], x;
+  int odd[NT];       // which of its pair a tile is
   uint32_t row[MT];  // byte offset of this lane's row, kNowhere where there is none
   int32_t most;      // last multiple of 8 below K, less this lane's first k in a step
 };
 
-template <int MT, int NT, int SUB, bool ZEROS>
-__device__ __forceinline__ void load(Step<MT, NT, SUB, ZEROS>& st, const Source<MT, NT>& t, uint32_t kb, int lane) {
+template <int MT, int NT, int SUB, bool ZEROS, int XQ>
+__device__ __forceinline__ void load(Step<MT, NT, SUB, ZEROS, XQ>& st, const Source<MT, NT>& t, uint32_t kb, int lane) {
   constexpr int G = 4 / SUB;
-  // scales past the last step are the last one's: they multiply zeros
-  const uint32_t sb = min(kb, t.last);
-  const uint32_t at = sb * (32 * G) + (lane >> 4) * (8 * G), zt = sb * (16 * G) + (lane & 15) * G;
+  const uint32_t at = kb * block_bytes(G, ZEROS), sat = at + (lane & 15) * (4 * G), zat = at + (lane & 15) * (2 * G);
 #pragma unroll
-  for (int n = 0; n < NT; ++n) st.w[n] = load16(t.w[n], kb * 1024 + lane * 16);
+  for (int n = 0; n < NT; ++n)
+    st.w[n] = load16(t.w[NT == 4 ? n / 2 : n], at + lane * 16 + 1024 * (NT == 4 ? n % 2 : t.odd[n]));
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    typedef uint32_t words __attribute__((ext_vector_type(G == 4 ? 4 : 2 * G)));
+  for (int n = 0; n < st.PAIRS; ++n) {
+    if constexpr (G == 1) {
+      st.s[n][0] = __builtin_amdgcn_raw_buffer_load_b32(t.w[n], (int)sat + 2048, 0, 0);
+    } else if constexpr (G == 2) {
+      const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t.w[n], (int)sat + 2048, 0, 0));
+      st.s[n][0] = v[0];
+      st.s[n][1] = v[1];
+    } else {
+      const u32x4 v = load16(t.w[n], sat + 2048);
 #pragma unroll
-    for (int h = 0; h < (G == 4 ? 2 : 1); ++h) {
-      const words v = *reinterpret_cast<const words*>(t.s[n] + at + 16 * h);
-#pragma unroll
-      for (int i = 0; i < (G == 4 ? 4 : 2 * G); ++i) st.s[n][4 * h + i] = v[i];
+      for (int i = 0; i < 4; ++i) st.s[n][i] = v[i];
     }
     if constexpr (ZEROS) {
-      if constexpr (G == 1) st.z[n] = t.z[n][zt];
-      else if constexpr (G == 2) st.z[n] = *reinterpret_cast<const uint16_t*>(t.z[n] + zt);
-      else st.z[n] = *reinterpret_cast<const uint32_t*>(t.z[n] + zt);
+      const int zo = (int)zat + 2048 + 64 * G;
+      if constexpr (G == 1) {
+        st.z[n][0] = __builtin_amdgcn_raw_buffer_load_b16(t.w[n], zo, 0, 0);
+      } else if constexpr (G == 2) {
+        st.z[n][0] = __builtin_amdgcn_raw_buffer_load_b32(t.w[n], zo, 0, 0);
+      } else {
+        const u32x2 zv = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t.w[n], zo, 0, 0));
+        st.z[n][0] = zv[0];
+        st.z[n][1] = zv[1];
+      }
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < XQ; ++j) {
     const bool in = (int32_t)(kb * kBlock) + j * 32 <= t.most;
 #pragma unroll
     for (int m = 0; m < MT; ++m) st.x[m][j] = load16(t.x, in ? t.row[m] + kb * 256 + 64 * j : kNowhere);
   }
 }
 
-template <int MT, int NT, int SUB, bool ZEROS>
-__device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS>& st, uint32_t mask, uint32_t bias,
-                                         f32x4 (&acc)[NT][MT]) {
+template <int MT, int NT, int SUB, bool ZEROS, int XQ>
+__device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, XQ>& st, const int (&odd)[NT], uint32_t mask,
+                                         uint32_t bias, f32x4 (&acc)[NT][MT]) {
+  bf16x8 x[MT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    x[m][0] = __builtin_bit_cast(bf16x8, st.x[m][0]);
+    x[m][1] = __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<1>(st.x[m][0]) : st.x[m][1 % XQ]);
+    x[m][2] = __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<2>(st.x[m][0]) : st.x[m][2 % XQ]);
+    x[m][3] = __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<3>(st.x[m][0]) : st.x[m][3 % XQ]);
+  }
 #pragma unroll
   for (int g = 0; g < 4 / SUB; ++g) {
     f32x4 base[MT];  // sum of -136 x: the same for every column where there are no zero points
@@ -131,11 +165,17 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS>& st, uin
         base[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < SUB; ++i)
-          base[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(off, __builtin_bit_cast(bf16x8, st.x[m][g * SUB + i]), base[m], 0, 0, 0);
+          base[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[m][g * SUB + i], off, base[m], 0, 0, 0);
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      // this lane's column: scale (and zero point) of the tile in its pair's word
+      const int pair = NT == 4 ? n / 2 : n;
+      const uint32_t sw = st.s[pair][g];
+      const float s = __uint_as_float(NT == 4 ? (n % 2 ? sw & 0xffff0000u : sw << 16) : sw >> (16 * odd[n]) << 16);
+      bf16x8 off;
+      if constexpr (ZEROS) off = minus_offset(st.z[pair][g / 2] >> (16 * (g % 2) + 8 * (NT == 4 ? n % 2 : odd[n])) & 255u);
       f32x4 part[MT];
 #pragma unroll
       for (int m = 0; m < MT; ++m) part[m] = ZEROS ? f32x4{0.f, 0.f, 0.f, 0.f} : base[m];
@@ -144,17 +184,15 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS>& st, uin
         const bf16x8 q = expand(st.w[n][g * SUB + i], mask, bias);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const bf16x8 xv = __builtin_bit_cast(bf16x8, st.x[m][g * SUB + i]);
-          if constexpr (ZEROS)
-            part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus_offset((st.z[n] >> (8 * g)) & 255u), xv, part[m], 0, 0, 0);
-          part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q, xv, part[m], 0, 0, 0);
+          const bf16x8 xv = x[m][g * SUB + i];
+          if constexpr (ZEROS) part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, off, part[m], 0, 0, 0);
+          part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, q, part[m], 0, 0, 0);
         }
       }
-      const f32x4 s = {bf16_lo(st.s[n][2 * g]), bf16_hi(st.s[n][2 * g]), bf16_lo(st.s[n][2 * g + 1]), bf16_hi(st.s[n][2 * g + 1])};
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(s[r], part[m][r], acc[n][m][r]);
+        for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(s, part[m][r], acc[n][m][r]);
     }
   }
 }
@@ -165,13 +203,13 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS>& st, uin
 // for its own only.  The last P steps load nothing more (a load that nobody
 // needs would still be waited for before its registers are used again); those
 // past the end found zeros.
-template <int MT, int NT, int SUB, bool ZEROS, int P>
+template <int MT, int NT, int SUB, bool ZEROS, int XQ, int P>
 __device__ __forceinline__ void sweep(const Source<MT, NT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
                                       f32x4 (&acc)[NT][MT]) {
   uint32_t mask = 0x000f000fu, bias = 0x43004300u;
   asm volatile("" : "+s"(mask));
   asm volatile("" : "+v"(bias));
-  Step<MT, NT, SUB, ZEROS> st[P];
+  Step<MT, NT, SUB, ZEROS, XQ> st[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     load(st[i], t, first + i * stride, lane);
@@ -185,44 +223,27 @@ __device__ __forceinline__ void sweep(const Source<MT, NT>& t, uint32_t KB, uint
   for (; kb + P * stride < KB; kb += P * stride) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-      multiply(st[i], mask, bias, acc);
+      multiply(st[i], t.odd, mask, bias, acc);
       __builtin_amdgcn_sched_barrier(0);
       load(st[i], t, kb + (i + P) * stride, lane);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
 #pragma unroll
-  for (int i = 0; i < P; ++i) multiply(st[i], mask, bias, acc);
+  for (int i = 0; i < P; ++i) multiply(st[i], t.odd, mask, bias, acc);
 }
 
-// One unit of the result: 16 columns of 16 rows, this lane's four columns `c` ..
-// of row `r`.
-__device__ __forceinline__ void store(const W4KParams& p, int64_t r, int64_t c, int64_t width, f32x4 v) {
+// One value of the result.
+__device__ __forceinline__ void store(const W4KParams& p, int64_t r, int64_t c, int64_t width, float v) {
   if (p.out_type == kW4F32) {
-    float* out = static_cast<float*>(p.C) + r * p.ldc + c;
-    if (c + 4 <= width && p.ldc % 4 == 0) {
-      *reinterpret_cast<f32x4*>(out) = v;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + i < width) out[i] = v[i];
-    }
+    static_cast<float*>(p.C)[r * p.ldc + c] = v;
     return;
   }
   uint16_t* out = static_cast<uint16_t*>(p.C) + r * p.ldc + c;
-  for (int h = 0; h < (p.out_type == kW4Pair ? 2 : 1); ++h) {
-    const u32x2 o = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    if (c + 4 <= width && p.ldc % 4 == 0 && width % 4 == 0) {
-      *reinterpret_cast<u32x2*>(out) = o;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + i < width) out[i] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
-    }
-    // what the rounding left, in the second half of the row
-    v = f32x4{v[0] - bf16_lo(o[0]), v[1] - bf16_hi(o[0]), v[2] - bf16_lo(o[1]), v[3] - bf16_hi(o[1])};
-    out += width;
-  }
+  const __bf16 hi = (__bf16)v;
+  out[0] = __builtin_bit_cast(uint16_t, hi);
+  // what the rounding left, in the second half of the row
+  if (p.out_type == kW4Pair) out[width] = __builtin_bit_cast(uint16_t, (__bf16)(v - (float)hi));
 }
 
 // How many of a workgroup's W waves share an item's K: few items are cut into
@@ -242,13 +263,14 @@ __host__ __device__ __forceinline__ int choose_split(uint32_t items, uint32_t wa
   return best;
 }
 
-// The row passes of the real rows of up to kListed row blocks: 16 rows each, or
-// 8 where x goes as bf16 pairs, whose second halves take the other 8 lanes (the
-// two sums of a row are added at the end).
+// The real row blocks' experts and rows, and the passes of ROWS rows that they
+// take, for up to kListed blocks: read once per workgroup, so that an item
+// starts without a chain of loads.
 constexpr int kListed = 512;
 template <int ROWS>
 struct PassList {
-  int first[kListed + 1];                        // first pass of each block
+  int expert[kListed];
+  uint16_t rows[kListed], first[kListed + 1];    // first pass of each block
   uint16_t block[kListed * (kFlagRows / ROWS)];  // block of each pass
   int scratch[17];
 };
@@ -274,51 +296,67 @@ __device__ __forceinline__ int block_rows(const W4KParams& p, int64_t b) {
   return p.rb_rows ? max(0, min(p.rb_rows[b], kFlagRows)) : kFlagRows;
 }
 
+// Steps in flight per wave: what 120 registers hold, at least two.
+constexpr int steps_ahead(int mt, int nt, int sub, bool zeros, int xq) {
+  const int pairs = nt == 4 ? 2 : nt;
+  const int regs = 4 * nt + pairs * (4 / sub) + (zeros ? pairs * (sub == 1 ? 2 : 1) : 0) + 4 * mt * xq;
+  return 120 / regs < 2 ? 2 : 120 / regs > 6 ? 6 : 120 / regs;
+}
+
 // W waves.  An item is NT column tiles (with SwiGLU: the first half gate tiles,
-// the second the matching up tiles) of 16 MT rows; `split` waves share its K.
-// The workgroups of the grid walk the items in turn, as many as the device's
-// row count and tables say there are.
-template <int MT, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS>
-__global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
-  extern __shared__ f32x4 red[];  // [W][NT * MT][64], used where K is split
-  constexpr int ROWS = PARTS == 2 ? 8 : 16, kPasses = kFlagRows / ROWS;  // of a pass over experts' rows
-  __shared__ PassList<ROWS> list;
-  static_assert(MT == 1 || (!EXPERTS && PARTS == 1), "passes of 16 rows");
+// the second the matching up tiles) of a pass of up to 16 MTX rows; `split`
+// waves share its K.  Where x goes as bf16 pairs (PARTS 2) the halves of a row
+// take two lanes of a row tile, and their two sums are added at the end.  The
+// workgroups of the grid walk the items in turn, as many as the device's row
+// count and tables say there are.  FEW, MANY: whether passes of at most 4 row
+// lanes, and of more, come (see Step).
+template <int MTX, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS, bool FEW, bool MANY>
+__global__ __launch_bounds__(64 * W, NT == 4 ? 2 : 1) void w4_kernel(W4KParams p) {
+  extern __shared__ f32x4 red[];  // [W][NT * MTX][64], used where K is split
+  constexpr int ROWS = 16 * MTX / PARTS, kPasses = EXPERTS ? kFlagRows / ROWS : 1;
+  __shared__ PassList<EXPERTS ? ROWS : kFlagRows> list;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const uint32_t KB = (uint32_t)((p.w.K + kBlock - 1) / kBlock);
-  const int tiles = (int)((p.w.N + kTile - 1) / kTile);
-  const int64_t groups = (int64_t)KB * (4 / SUB);
+  const int64_t pairs = (p.w.N + 2 * kTile - 1) / (2 * kTile), tile_run = (int64_t)KB * block_bytes(4 / SUB, ZEROS);
   const int per_item = p.swiglu ? NT / 2 : NT;  // output tiles
   const int col_items = (p.tile_cols + per_item - 1) / per_item;
   const int64_t width = p.swiglu ? (int64_t)p.tile_cols * kTile : p.w.N;
-  int blocks = p.row_blocks;
   uint32_t passes = p.row_blocks;
   bool listed = false;
   if constexpr (EXPERTS) {
-    if (p.rows_dev) blocks = (int)min((int64_t)blocks, max((int64_t)0, *p.rows_dev / kFlagRows));
+    constexpr int per = (kListed + 64 * W - 1) / (64 * W);
+    int n[per], sum = 0, blocks = p.row_blocks;
+    int64_t rows_dev = p.rows_dev ? *p.rows_dev : p.M;
+#pragma unroll
+    for (int i = 0; i < per; ++i) {  // (not held back by the row count)
+      const int b = threadIdx.x * per + i;
+      n[i] = b < min(p.row_blocks, kListed) ? block_rows(p, b) : 0;
+      if (b < min(p.row_blocks, kListed)) list.expert[b] = p.rb_expert[b];
+    }
+    blocks = (int)min((int64_t)blocks, max((int64_t)0, rows_dev / kFlagRows));
     listed = blocks <= kListed;
     passes = blocks * kPasses;
     if (listed) {
-      constexpr int per = kListed / (64 * W) > 0 ? kListed / (64 * W) : 1;
-      int n[per], sum = 0;
 #pragma unroll
       for (int i = 0; i < per; ++i) {
-        const int b = threadIdx.x * per + i;
-        n[i] = b < blocks ? (block_rows(p, b) + ROWS - 1) / ROWS : 0;
-        sum += n[i];
+        if ((int)threadIdx.x * per + i >= blocks) n[i] = 0;
+        sum += (n[i] + ROWS - 1) / ROWS;
       }
       int at = prefix<W>(sum, list.scratch);
-      if (threadIdx.x == 64 * W - 1) list.scratch[16] = at;
+      if (threadIdx.x == 64 * W - 1) {
+        list.scratch[16] = at;
+        list.first[kListed] = (uint16_t)at;
+      }
       at -= sum;
 #pragma unroll
       for (int i = 0; i < per; ++i) {
         const int b = threadIdx.x * per + i;
-        if (b <= kListed) list.first[b] = at;
-        for (int j = 0; j < n[i]; ++j) list.block[at + j] = (uint16_t)b;
-        at += n[i];
+        if (b >= kListed) break;
+        list.first[b] = (uint16_t)at;
+        list.rows[b] = (uint16_t)n[i];
+        for (int j = 0; j < (n[i] + ROWS - 1) / ROWS; ++j) list.block[at++] = (uint16_t)b;
       }
-      if (threadIdx.x == 64 * W - 1) list.first[kListed] = at;
       __syncthreads();
       passes = list.scratch[16];
     }
@@ -332,148 +370,183 @@ __global__ __launch_bounds__(64 * W) void w4_kernel(W4KParams p) {
     int64_t row0 = 0, expert = 0;
     int ci = 0, left = 0;
     if (it < items) {
+      uint32_t q = it / col_items;
       if constexpr (EXPERTS) {
         // the passes of one column item side by side: they read the same weights
-        uint32_t q = it / col_items;
-        int np = kPasses, pass, b;
+        int np = kPasses, b;
         if (listed) {
           b = __builtin_amdgcn_readfirstlane((int)list.block[q]);
-          const int first = __builtin_amdgcn_readfirstlane(list.first[b]);
-          np = __builtin_amdgcn_readfirstlane(list.first[b + 1]) - first;
-          q = first;
+          q = __builtin_amdgcn_readfirstlane((int)list.first[b]);
+          np = __builtin_amdgcn_readfirstlane((int)list.first[b + 1]) - (int)q;
+          left = __builtin_amdgcn_readfirstlane((int)list.rows[b]);
+          expert = __builtin_amdgcn_readfirstlane(list.expert[b]);
         } else {
           b = q / kPasses;
           q = b * kPasses;
+          left = __builtin_amdgcn_readfirstlane(block_rows(p, b));
+          expert = __builtin_amdgcn_readfirstlane(p.rb_expert[b]);
         }
-        const int local = (int)(it - q * col_items);
+        const int local = (int)(it - q * col_items), pass = local % np;
         ci = local / np;
-        pass = local - ci * np;
-        left = __builtin_amdgcn_readfirstlane(block_rows(p, b)) - ROWS * pass;
-        expert = __builtin_amdgcn_readfirstlane(p.rb_expert[b]);
+        left = min(left - ROWS * pass, ROWS);
         row0 = (int64_t)b * kFlagRows + ROWS * pass;
       } else {
-        const uint32_t b = it / col_items;
-        ci = (int)(it - b * col_items);
-        row0 = (int64_t)b * 16 * MT;
-        left = (int)min(p.M - row0, (int64_t)16 * MT);
+        ci = (int)(it - q * col_items);
+        row0 = (int64_t)q * ROWS;
+        left = (int)min(p.M - row0, (int64_t)ROWS);
       }
     }
-    Source<MT, NT> t;
-    int tile[NT];
+    const bool any = left > 0, few = FEW && left <= 4 / PARTS;
+    const int lanes = few ? 4 : 16;  // of a row tile
+    f32x4 acc[NT][MTX];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const bool up = p.swiglu && n >= NT / 2;
-      tile[n] = min(ci * per_item + (up ? n - NT / 2 : n), p.tile_cols - 1) + (up ? p.tile_cols : 0);
-      const int64_t at = left > 0 ? expert * tiles + tile[n] : 0;
-      t.w[n] = make_rsrc(p.w.packed + at * KB * 256, KB * 1024);
-      t.s[n] = reinterpret_cast<const char*>(p.w.scales + at * groups * kTile);
-      if constexpr (ZEROS) t.z[n] = p.w.zeros + at * groups * kTile;
-    }
-    t.last = KB - 1;
-    t.most = (int32_t)p.w.K - 8 - quad * 8;
-    // lanes past the last row read nothing; their results are not stored
-    if (EXPERTS && p.gather_pull) {
-      t.x = make_rsrc(p.A, (uint32_t)(p.gather_rows * p.lda * 2));
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        t.row[m] = kNowhere;
-        if (16 * m + col < left) {
-          const int* pr = p.gather_pull + 3 * (row0 + 16 * m + col);
-          const int64_t src = ((int64_t)pr[0] * p.gather_devs + pr[1]) * p.gather_tps + pr[2];
-          if (pr[0] >= 0 && pr[2] >= 0 && src >= 0 && src < p.gather_rows) t.row[m] = (uint32_t)(src * p.lda * 2) + quad * 16;
+      for (int m = 0; m < MTX; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto run = [&](auto mt, auto xq) {
+      constexpr int MT = decltype(mt)::value, XQ = decltype(xq)::value;
+      Source<MT, NT> t;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const bool up = p.swiglu && n >= NT / 2;
+        // (a last item's missing tile: its pair's other one again, which is not stored)
+        const int tile = min(ci * per_item + (up ? n - NT / 2 : n), p.tile_cols - 1) + (up ? p.tile_cols : 0);
+        t.odd[n] = tile & 1;
+        if (NT < 4 || n % 2 == 0)
+          t.w[NT == 4 ? n / 2 : n] = make_rsrc(p.w.packed + (expert * pairs + tile / 2) * tile_run, (uint32_t)tile_run);
+      }
+      // This lane's row of a tile, which half of a pair, and its first k in a step
+      // (see Step).  Lanes past the last row read nothing; their results are not
+      // stored.
+      constexpr int LANES = XQ == 1 ? 4 : 16, EACH = LANES / PARTS;
+      const int r = col % EACH, half = col % LANES / EACH, k0 = (XQ == 1 ? col / 4 * 32 : 0) + quad * 8;
+      t.most = (int32_t)p.w.K - 8 - k0;
+      const uint32_t in_row = 2 * (uint32_t)(k0 + half * p.w.K);
+      if (EXPERTS && p.gather_pull) {
+        t.x = make_rsrc(p.A, (uint32_t)(p.gather_rows * p.lda * 2));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          t.row[m] = kNowhere;
+          if (EACH * m + r < left) {
+            const int* pr = p.gather_pull + 3 * (row0 + EACH * m + r);
+            const int64_t src = ((int64_t)pr[0] * p.gather_devs + pr[1]) * p.gather_tps + pr[2];
+            if (pr[0] >= 0 && pr[2] >= 0 && src >= 0 && src < p.gather_rows) t.row[m] = (uint32_t)(src * p.lda * 2) + in_row;
+          }
         }
-      }
-    } else {
-      t.x = make_rsrc(p.A + row0 * p.lda, (uint32_t)(min(max(left, 0), 16 * MT) * p.lda * 2));
-      const int r = PARTS == 2 ? col & 7 : col;
+      } else {
+        t.x = make_rsrc(p.A + row0 * p.lda, (uint32_t)(left * p.lda * 2));
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        t.row[m] = 16 * m + r < left ? (uint32_t)((16 * m + r) * p.lda * 2 + (r < col ? 2 * p.w.K : 0)) + quad * 16 : kNowhere;
+        for (int m = 0; m < MT; ++m) t.row[m] = EACH * m + r < left ? (uint32_t)((EACH * m + r) * p.lda * 2) + in_row : kNowhere;
+      }
+      f32x4 a[NT][MT];
+      sweep<MT, NT, SUB, ZEROS, XQ, steps_ahead(MT, NT, SUB, ZEROS, XQ)>(t, KB, ks, split, lane, a);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if constexpr (PARTS == 2 && XQ == 1) {  // rows 0 and 1, then their second halves
+            a[n][m][0] += a[n][m][2];
+            a[n][m][1] += a[n][m][3];
+          } else if constexpr (PARTS == 2) {  // second halves: rows 8 to 15, two quads on
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[n][m][i] += __shfl_xor(a[n][m][i], 32, 64);
+          }
+          acc[n][m] = a[n][m];
+        }
+    };
+    using std::integral_constant;
+    int mt = 1;
+    if (any) {
+      if (FEW && (few || !MANY)) {
+        if constexpr (FEW) run(integral_constant<int, 1>(), integral_constant<int, 1>());
+      } else if (MTX == 1 || left <= 16 / PARTS) {
+        if constexpr (MANY) run(integral_constant<int, 1>(), integral_constant<int, 4>());
+      } else {
+        mt = MTX;
+        if constexpr (MANY && MTX > 1) run(integral_constant<int, MTX>(), integral_constant<int, 4>());
+      }
     }
-    f32x4 acc[NT][MT];
-    sweep<MT, NT, SUB, ZEROS, (MT * NT == 1 ? W4_P1 : 2)>(t, KB, left > 0 ? ks : KB, split, lane, acc);
     auto finish = [&](int n, int m, f32x4 v, f32x4 up) {
-      if constexpr (PARTS == 2) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          v[r] += __shfl_xor(v[r], 8, 64);
-          up[r] += __shfl_xor(up[r], 8, 64);
-        }
-        if (col >= 8) return;
-      }
-      if (16 * m + col >= left || ci * per_item + n >= p.tile_cols) return;
+      const int64_t c = (int64_t)(ci * per_item + n) * kTile + col;
+      if (c >= width) return;
       if constexpr (NT >= 2)
         if (p.swiglu)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = silu(v[r]) * up[r];
-      store(p, row0 + 16 * m + col, (int64_t)(ci * per_item + n) * kTile + 4 * quad, width, v);
+          for (int i = 0; i < 4; ++i) v[i] = silu(v[i]) * up[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * quad + i;
+        if (r < lanes / PARTS && lanes / PARTS * m + r < left) store(p, row0 + lanes / PARTS * m + r, c, width, v[i]);
+      }
     };
     if (split == 1) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (n < per_item) finish(n, m, acc[n][m], acc[NT >= 2 ? (n + NT / 2) % NT : n][m]);
+        for (int m = 0; m < MTX; ++m)
+          if (n < per_item && m < mt) finish(n, m, acc[n][m], acc[NT >= 2 ? (n + NT / 2) % NT : n][m]);
       continue;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) red[(wave * NT * MT + n * MT + m) * 64 + lane] = acc[n][m];
+      for (int m = 0; m < MTX; ++m)
+        if (m < mt) red[(wave * NT * MTX + n * MTX + m) * 64 + lane] = acc[n][m];
     __syncthreads();
     auto total = [&](int u) {
-      f32x4 v = red[((wave - ks) * NT * MT + u) * 64 + lane];
-      for (int o = 1; o < split; ++o) v += red[((wave - ks + o) * NT * MT + u) * 64 + lane];
+      f32x4 v = red[((wave - ks) * NT * MTX + u) * 64 + lane];
+      for (int o = 1; o < split; ++o) v += red[((wave - ks + o) * NT * MTX + u) * 64 + lane];
       return v;
     };
-    for (int u = ks; u < per_item * MT; u += split) {
-      const f32x4 v = total(u);
-      finish(u / MT, u % MT, v, p.swiglu ? total(u + (NT / 2) * MT) : v);
-    }
+    if (any)
+      for (int u = ks; u < per_item * mt; u += split) {
+        const int n = u / mt, m = u - n * mt;
+        const f32x4 v = total(n * MTX + m);
+        finish(n, m, v, p.swiglu ? total((n + NT / 2) * MTX + m) : v);
+      }
     __syncthreads();
   }
 }
 
-template <int MT, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS>
+template <int MTX, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS, bool FEW, bool MANY>
 void launch(const W4KParams& p, int grid, hipStream_t stream) {
-  hipLaunchKernelGGL((w4_kernel<MT, NT, W, SUB, ZEROS, PARTS, EXPERTS>), dim3(grid), dim3(64 * W),
-                     W * NT * MT * 64 * sizeof(f32x4), stream, p);
+  hipLaunchKernelGGL((w4_kernel<MTX, NT, W, SUB, ZEROS, PARTS, EXPERTS, FEW, MANY>), dim3(grid), dim3(64 * W),
+                     W * NT * MTX * 64 * sizeof(f32x4), stream, p);
 }
 
-__global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, int64_t K, int64_t N, int64_t KB,
-                                                      int64_t tiles, int64_t words, uint32_t* out) {
+// One thread per 4 bytes of the packed weights.
+__global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros,
+                                                      int64_t K, int64_t N, int64_t KB, int64_t pairs, int64_t given,
+                                                      int groups, int64_t words, uint32_t* out) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= words) return;
-  const int j = (int)(i & 3), lane = (int)((i >> 2) & 63);
-  const int64_t block = i >> 8, kb = block % KB, tile = block / KB % tiles, e = block / KB / tiles;
-  const int64_t n = tile * kTile + (lane & 15), k0 = kb * kBlock + j * 32 + (lane >> 4) * 8;
+  const int unit = (int)(block_bytes(groups, zeros != nullptr) / 4);
+  const int64_t block = i / unit, kb = block % KB, pair = block / KB % pairs, e = block / KB / pairs;
+  const int at = (int)(i - block * unit);
   uint32_t w = 0;
+  if (at < 512) {  // codes: [2 tiles][64 lanes][4 MFMAs], see expand()
+    const int j = at & 3, lane = (at >> 2) & 63;
+    const int64_t n = (2 * pair + (at >> 8)) * kTile + (lane & 15), k0 = kb * kBlock + j * 32 + (lane >> 4) * 8;
 #pragma unroll
-  for (int o = 0; o < 8; ++o) {
-    const int64_t k = k0 + o;
-    const uint32_t q = k < K && n < N ? codes[(e * K + k) * N + n] & 15u : 8u;
-    w |= q << (4 * ((o & 1) * 4 + (o >> 1)));
+    for (int o = 0; o < 8; ++o) {
+      const int64_t k = k0 + o;
+      const uint32_t q = k < K && n < N ? codes[(e * K + k) * N + n] & 15u : 8u;
+      w |= q << (4 * ((o & 1) * 4 + (o >> 1)));
+    }
+  } else {
+    // scales, two to a word, then zero points, four: [16 columns][groups][2 tiles]
+    const bool zero = at >= 512 + 16 * groups;
+    const int first = zero ? 4 * (at - 512 - 16 * groups) : 2 * (at - 512);
+    for (int o = 0; o < (zero ? 4 : 2); ++o) {
+      const int u = first + o;
+      const int64_t n = (2 * pair + u % 2) * kTile + u / (2 * groups), g = kb * groups + u / 2 % groups;
+      const bool in = g < given && n < N;
+      const int64_t src = (e * given + g) * N + n;
+      if (zero) w |= (in ? zeros[src] & 15u : 8u) << (8 * o);
+      else w |= (in ? (uint32_t)scales[src] : 0u) << (16 * o);
+    }
   }
   out[i] = w;
-}
-
-__global__ __launch_bounds__(256) void w4_pack_groups_kernel(const uint16_t* scales, const uint8_t* zeros, int64_t N,
-                                                             int64_t given, int64_t groups, int per, int64_t tiles,
-                                                             int64_t count, uint16_t* out_scales, uint8_t* out_zeros) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= count) return;
-  // scales: [tile][block][4 quads][per block][4 columns]; zeros: [tile][block][16 columns][per block]
-  const int64_t unit = kTile * per, block = i / unit, in_block = i % unit;
-  const int64_t kb = block % (groups / per), tile = block / (groups / per) % tiles, e = block / (groups / per) / tiles;
-  auto source = [&](int64_t g, int64_t n) {
-    return g < given && n < N ? (e * given + g) * N + n : (int64_t)-1;
-  };
-  const int64_t at = source(kb * per + in_block / 4 % per, tile * kTile + in_block / (4 * per) * 4 + in_block % 4);
-  out_scales[i] = at >= 0 ? scales[at] : 0;
-  if (out_zeros) {
-    const int64_t zt = source(kb * per + in_block % per, tile * kTile + in_block / per);
-    out_zeros[i] = zt >= 0 ? zeros[zt] & 15u : 8u;
-  }
 }
 
 // One thread per group and column: scale = bf16(largest magnitude / 7), code =
@@ -501,22 +574,16 @@ unsigned blocks256(int64_t n) { return (unsigned)((n + 255) / 256); }
 
 }  // namespace
 
-int64_t w4_packed_words(int64_t K, int64_t N, int64_t E) {
-  return E * ((N + kTile - 1) / kTile) * ((K + kBlock - 1) / kBlock) * 256;
-}
-
-int64_t w4_scale_count(int64_t K, int64_t N, int64_t E, int group) {
-  return E * ((N + kTile - 1) / kTile) * ((K + kBlock - 1) / kBlock) * (kBlock / group) * kTile;
+int64_t w4_packed_bytes(int64_t K, int64_t N, int64_t E, int group, bool zeros) {
+  return E * ((N + 2 * kTile - 1) / (2 * kTile)) * ((K + kBlock - 1) / kBlock) * block_bytes(kBlock / group, zeros);
 }
 
 hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int64_t K, int64_t N,
-                          int64_t E, int group, uint32_t* packed, uint16_t* packed_scales, uint8_t* packed_zeros,
-                          hipStream_t stream) {
-  const int64_t KB = (K + kBlock - 1) / kBlock, tiles = (N + kTile - 1) / kTile;
-  const int64_t words = w4_packed_words(K, N, E), count = w4_scale_count(K, N, E, group);
-  hipLaunchKernelGGL(w4_pack_kernel, dim3(blocks256(words)), dim3(256), 0, stream, codes, K, N, KB, tiles, words, packed);
-  hipLaunchKernelGGL(w4_pack_groups_kernel, dim3(blocks256(count)), dim3(256), 0, stream, scales, zeros, N,
-                     (K + group - 1) / group, KB * (kBlock / group), kBlock / group, tiles, count, packed_scales, packed_zeros);
+                          int64_t E, int group, unsigned char* packed, hipStream_t stream) {
+  const int64_t KB = (K + kBlock - 1) / kBlock, pairs = (N + 2 * kTile - 1) / (2 * kTile);
+  const int64_t words = w4_packed_bytes(K, N, E, group, zeros != nullptr) / 4;
+  hipLaunchKernelGGL(w4_pack_kernel, dim3(blocks256(words)), dim3(256), 0, stream, codes, scales, zeros, K, N, KB, pairs,
+                     (K + group - 1) / group, kBlock / group, words, reinterpret_cast<uint32_t*>(packed));
   return hipGetLastError();
 }
 
@@ -541,7 +608,7 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
     constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, W = decltype(w)::value;
     p.row_blocks = (int)(decltype(ex)::value ? p.M / kFlagRows : (p.M + 16 * MT - 1) / (16 * MT));
     const int per_item = p.swiglu ? NT / 2 : NT;
-    const int passes = decltype(ex)::value ? kFlagRows / (decltype(parts)::value == 2 ? 8 : 16) : 1;
+    const int passes = decltype(ex)::value ? kFlagRows * decltype(parts)::value / (16 * MT) : 1;
     const int64_t items = (int64_t)p.row_blocks * passes * ((p.tile_cols + per_item - 1) / per_item);
     const int64_t most = (int64_t)cus * waves_per_cu(MT, NT) / W;
     int64_t grid = std::min<int64_t>(items, most);
@@ -549,8 +616,16 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
       p.split = choose_split((uint32_t)items, (uint32_t)(most * W), (uint32_t)((p.w.K + kBlock - 1) / kBlock), W);
       grid = std::min<int64_t>(most, (items * p.split + W - 1) / W);
     }
-    launch<MT, NT, W, decltype(sub)::value, decltype(zeros)::value, decltype(parts)::value, decltype(ex)::value>(
-        p, (int)grid, stream);
+    constexpr int SUB = decltype(sub)::value, PARTS = decltype(parts)::value;
+    constexpr bool ZEROS = decltype(zeros)::value;
+    if constexpr (decltype(ex)::value) {
+      launch<MT, NT, W, SUB, ZEROS, PARTS, true, true, true>(p, (int)grid, stream);
+    } else if constexpr (MT == 1) {
+      if (p.M <= 4) launch<MT, NT, W, SUB, ZEROS, PARTS, false, true, false>(p, (int)grid, stream);
+      else launch<MT, NT, W, SUB, ZEROS, PARTS, false, false, true>(p, (int)grid, stream);
+    } else {
+      launch<MT, NT, W, SUB, ZEROS, PARTS, false, false, true>(p, (int)grid, stream);
+    }
   };
   using std::integral_constant;
   auto with_zeros = [&](auto mt, auto nt, auto w, auto sub, auto parts, auto ex) {
@@ -567,12 +642,16 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
   constexpr integral_constant<int, 4> four;
   constexpr integral_constant<int, 8> eight;
   if (experts) {
-    if (p.parts == 2) with_group(one, four, four, two, std::true_type());
-    else with_group(one, four, four, one, std::true_type());
+    // SwiGLU's gate and up tiles go in pairs where the width is a whole number of them
+    const bool pairs = !p.swiglu || p.tile_cols % 2 == 0;
+    if (p.parts == 2 && pairs) with_group(two, four, four, two, std::true_type());
+    else if (p.parts == 2) with_group(two, two, four, two, std::true_type());
+    else if (pairs) with_group(two, four, four, one, std::true_type());
+    else with_group(two, two, four, one, std::true_type());
   } else if (p.M <= 16) {
-    with_group(one, integral_constant<int, W4_NT>(), integral_constant<int, W4_W>(), one, std::false_type());
+    with_group(one, one, eight, one, std::false_type());
   } else {
-    with_group(two, integral_constant<int, W4_NT2>(), integral_constant<int, W4_W2>(), one, std::false_type());
+    with_group(two, four, eight, one, std::false_type());
   }
   return hipGetLastError();
 }

@@ -560,17 +560,15 @@ def moe_combine_backward(dy: torch.Tensor, y_expert: torch.Tensor, ids: torch.Te
 class W4Weights(NamedTuple):
     """4-bit weights laid out by w4_pack: E matrices [K, N], values
     (code - zero) * scale per `group` rows of K."""
-    packed: torch.Tensor
-    scales: torch.Tensor
-    zeros: torch.Tensor | None
+    packed: torch.Tensor  # codes, scales and zero points
     K: int
     N: int
     group: int
     experts: int
+    zeros: bool           # whether there are zero points
 
     def _values(self) -> tuple:
-        return (self.packed.data_ptr(), self.scales.data_ptr(), _ptr(self.zeros), self.K, self.N, self.group,
-                self.experts)
+        return self.packed.data_ptr(), self.K, self.N, self.group, self.experts, self.zeros
 
 
 def _groups(K: int, group: int) -> int:
@@ -596,15 +594,12 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, group: int, zeros: torch.
     _tensor(scales, "scales", _BF16, shape, device=codes.device)
     if zeros is not None:
         _tensor(zeros, "zeros", _U8, shape, device=codes.device)
-    L = capi.lib()
     dev = codes.device
-    words, count = int(L.mk_w4_packed_bytes(K, N, E)), int(L.mk_w4_scale_count(K, N, E, group))
-    if words < 0 or count < 0:
+    n = capi.lib().mk_w4_packed_bytes(K, N, E, group, zeros is not None)
+    if n < 0:
         raise ValueError(f"weights of {E} x {K} x {N} are too large")
     with _on(dev):
-        w = W4Weights(torch.empty(words, dtype=torch.uint8, device=dev),
-                      torch.empty(count, dtype=torch.bfloat16, device=dev),
-                      None if zeros is None else torch.empty(count, dtype=torch.uint8, device=dev), K, N, group, E)
+        w = W4Weights(torch.empty(n, dtype=torch.uint8, device=dev), K, N, group, E, zeros is not None)
         capi.call_values("mk_w4_pack", W4PackArgs, _stream(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros),
                          *w._values())
     return w

@@ -126,12 +126,12 @@ def test_combine_backward_refusals(change, code, match):
 
 
 def _weights(**change):
-    return _args(capi.W4WeightsC, dict(packed=P, scales=P, K=256, N=64, group=128, num_experts=1), change)
+    return _args(capi.W4WeightsC, dict(packed=P, K=256, N=64, group=128, num_experts=1), change)
 
 
 @pytest.mark.parametrize("change,code,match", [
     (dict(packed=0), EINVAL, "null"), (dict(group=48), EINVAL, "group"), (dict(K=0), ESHAPE, "sizes"),
-    (dict(N=1 << 25), ESHAPE, "sizes"), (dict(scales=P + 2), EINVAL, "aligned")])
+    (dict(N=1 << 25), ESHAPE, "sizes"), (dict(packed=P + 2), EINVAL, "aligned")])
 def test_weight_refusals(change, code, match):
     w = _weights(**change)
     _refused("mk_gemm_w4", _args(capi.GemmW4Args, dict(A=P, C=P, M=1, lda=256, ldc=64, W=w), {}), code, match)
@@ -186,10 +186,10 @@ def test_ffn_w4_refusals(w2, change, code, match):
 
 def test_sizes():
     L = capi.lib()
-    assert L.mk_w4_packed_bytes(256, 64, 1) == 256 * 64 // 2
-    assert L.mk_w4_packed_bytes(129, 17, 3) == 3 * 256 * 32 // 2  # whole 128 x 16 blocks
-    assert L.mk_w4_scale_count(129, 17, 3, 32) == 3 * 8 * 32
-    assert L.mk_w4_packed_bytes(0, 64, 1) < 0 and L.mk_w4_scale_count(64, 64, 1, 16) < 0
+    assert L.mk_w4_packed_bytes(256, 64, 1, 128, 0) == 256 * 64 // 2 + 2 * 64 * 2
+    # whole blocks of 128 rows by two tiles of 16 columns; a byte per zero point
+    assert L.mk_w4_packed_bytes(129, 33, 3, 32, 1) == 3 * (256 * 64 // 2 + 8 * 64 * 3)
+    assert L.mk_w4_packed_bytes(0, 64, 1, 128, 0) < 0 and L.mk_w4_packed_bytes(64, 64, 1, 16, 0) < 0
     assert L.mk_moe_route_workspace_bytes(-1, 8) < 0 and L.mk_moe_route_workspace_bytes(1, 1025) < 0
     assert L.mk_moe_route_workspace_bytes(0, 8) > 0
     # bounded however long the batch is
