@@ -237,7 +237,8 @@ struct W4KParams {
   int swiglu;
   int parts;                // 2: a row of A is two bf16 rows of K whose sum it stands for
   int out_type;             // W4Out; a pair is two bf16 rows of the result's width
-  int row_blocks, split;    // set by the launch
+  uint32_t passes;          // set by the launch: row passes,
+  int split;                // and waves that share an item's K (dense)
   // experts (rb_expert null: one dense product)
   const int* rb_expert;
   const int* rb_rows;

@@ -70,13 +70,13 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) 
 // them in place (the other lanes then hold parts of other MFMAs, which end in
 // rows that are not stored).  The loads of x, mostly empty, were the largest
 // cost of a decode step beside the weights: 12 of 67 us.
-template <int MT, int NT, int SUB, bool ZEROS, int XQ>
+template <int NT, int SUB, bool ZEROS, int XQ>
 struct Step {
   u32x4 w[NT];
   static constexpr int PAIRS = NT == 4 ? 2 : NT;  // four tiles are two pairs; else each tile reads its pair's
   uint32_t s[PAIRS][4 / SUB];
   uint32_t z[ZEROS ? PAIRS : 1][SUB == 1 ? 2 : 1];
-  u32x4 x[MT][XQ];
+  u32x4 x[XQ];
 };
 
 // Lane i of each 16 gets lane i + 4 J.
@@ -95,16 +95,16 @@ __device__ __forceinline__ u32x4 from_quarter(u32x4 v) {
 constexpr uint32_t block_bytes(int groups, bool zeros) { return 2048u + 64u * groups + (zeros ? 32u * groups : 0u); }
 
 // A wave's pairs of column tiles (the run of blocks of each) and its rows of x.
-template <int MT, int NT>
+template <int NT>
 struct Source {
   __amdgpu_buffer_rsrc_t w[NT == 4 ? 2 : NT], x;
   int odd[NT];       // which of its pair a tile is
-  uint32_t row[MT];  // byte offset of this lane's row, kNowhere where there is none
+  uint32_t row;      // byte offset of this lane's row, kNowhere where there is none
   int32_t most;      // last multiple of 8 below K, less this lane's first k in a step
 };
 
-template <int MT, int NT, int SUB, bool ZEROS, int XQ>
-__device__ __forceinline__ void load(Step<MT, NT, SUB, ZEROS, XQ>& st, const Source<MT, NT>& t, uint32_t kb, int lane) {
+template <int NT, int SUB, bool ZEROS, int XQ>
+__device__ __forceinline__ void load(Step<NT, SUB, ZEROS, XQ>& st, const Source<NT>& t, uint32_t kb, int lane) {
   constexpr int G = 4 / SUB;
   const uint32_t at = kb * block_bytes(G, ZEROS), sat = at + (lane & 15) * (4 * G), zat = at + (lane & 15) * (2 * G);
 #pragma unroll
@@ -139,34 +139,25 @@ __device__ __forceinline__ void load(Step<MT, NT, SUB, ZEROS, XQ>& st, const Sou
 #pragma unroll
   for (int j = 0; j < XQ; ++j) {
     const bool in = (int32_t)(kb * kBlock) + j * 32 <= t.most;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) st.x[m][j] = load16(t.x, in ? t.row[m] + kb * 256 + 64 * j : kNowhere);
+    st.x[j] = load16(t.x, in ? t.row + kb * 256 + 64 * j : kNowhere);
   }
 }
 
-template <int MT, int NT, int SUB, bool ZEROS, int XQ>
-__device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, XQ>& st, const int (&odd)[NT], uint32_t mask,
-                                         uint32_t bias, f32x4 (&acc)[NT][MT]) {
-  bf16x8 x[MT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    x[m][0] = __builtin_bit_cast(bf16x8, st.x[m][0]);
-    x[m][1] = __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<1>(st.x[m][0]) : st.x[m][1 % XQ]);
-    x[m][2] = __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<2>(st.x[m][0]) : st.x[m][2 % XQ]);
-    x[m][3] = __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<3>(st.x[m][0]) : st.x[m][3 % XQ]);
-  }
+template <int NT, int SUB, bool ZEROS, int XQ>
+__device__ __forceinline__ void multiply(const Step<NT, SUB, ZEROS, XQ>& st, const int (&odd)[NT], uint32_t mask,
+                                         uint32_t bias, f32x4 (&acc)[NT]) {
+  const bf16x8 x[4] = {
+      __builtin_bit_cast(bf16x8, st.x[0]),
+      __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<1>(st.x[0]) : st.x[1 % XQ]),
+      __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<2>(st.x[0]) : st.x[2 % XQ]),
+      __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<3>(st.x[0]) : st.x[3 % XQ])};
 #pragma unroll
   for (int g = 0; g < 4 / SUB; ++g) {
-    f32x4 base[MT];  // sum of -136 x: the same for every column where there are no zero points
+    f32x4 base = {0.f, 0.f, 0.f, 0.f};  // sum of -136 x: the same for every column where there are no zero points
     if constexpr (!ZEROS) {
       const bf16x8 off = minus_offset(8u);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        base[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < SUB; ++i)
-          base[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[m][g * SUB + i], off, base[m], 0, 0, 0);
-      }
+      for (int i = 0; i < SUB; ++i) base = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[g * SUB + i], off, base, 0, 0, 0);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -176,23 +167,14 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, XQ>& st,
       const float s = __uint_as_float(NT == 4 ? (n % 2 ? sw & 0xffff0000u : sw << 16) : sw >> (16 * odd[n]) << 16);
       bf16x8 off;
       if constexpr (ZEROS) off = minus_offset(st.z[pair][g / 2] >> (16 * (g % 2) + 8 * (NT == 4 ? n % 2 : odd[n])) & 255u);
-      f32x4 part[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) part[m] = ZEROS ? f32x4{0.f, 0.f, 0.f, 0.f} : base[m];
+      f32x4 part = base;
 #pragma unroll
       for (int i = 0; i < SUB; ++i) {
-        const bf16x8 q = expand(st.w[n][g * SUB + i], mask, bias);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const bf16x8 xv = x[m][g * SUB + i];
-          if constexpr (ZEROS) part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, off, part[m], 0, 0, 0);
-          part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv, q, part[m], 0, 0, 0);
-        }
+        if constexpr (ZEROS) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[g * SUB + i], off, part, 0, 0, 0);
+        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[g * SUB + i], expand(st.w[n][g * SUB + i], mask, bias), part, 0, 0, 0);
       }
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[n][m][r] = fmaf(s, part[m][r], acc[n][m][r]);
+      for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(s, part[r], acc[n][r]);
     }
   }
 }
@@ -203,22 +185,18 @@ __device__ __forceinline__ void multiply(const Step<MT, NT, SUB, ZEROS, XQ>& st,
 // for its own only.  The last P steps load nothing more (a load that nobody
 // needs would still be waited for before its registers are used again); those
 // past the end found zeros.
-template <int MT, int NT, int SUB, bool ZEROS, int XQ, int P>
-__device__ __forceinline__ void sweep(const Source<MT, NT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
-                                      f32x4 (&acc)[NT][MT]) {
+template <int NT, int SUB, bool ZEROS, int XQ, int P>
+__device__ __forceinline__ void sweep(const Source<NT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
+                                      f32x4 (&acc)[NT]) {
   uint32_t mask = 0x000f000fu, bias = 0x43004300u;
   asm volatile("" : "+s"(mask));
   asm volatile("" : "+v"(bias));
-  Step<MT, NT, SUB, ZEROS, XQ> st[P];
+  Step<NT, SUB, ZEROS, XQ> st[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     load(st[i], t, first + i * stride, lane);
     __builtin_amdgcn_sched_barrier(0);
   }
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
   uint32_t kb = first;
   for (; kb + P * stride < KB; kb += P * stride) {
 #pragma unroll
@@ -251,7 +229,7 @@ __device__ __forceinline__ void store(const W4KParams& p, int64_t r, int64_t c, 
 // needs the fewest steps in the longest wave (a round costs about kRoundSteps
 // steps beside its own: row tables, first loads, the sum over waves).
 constexpr int kRoundSteps = 3;
-__host__ __device__ __forceinline__ int choose_split(uint32_t items, uint32_t waves, uint32_t KB, int W) {
+__host__ __device__ inline int choose_split(uint32_t items, uint32_t waves, uint32_t KB, int W) {
   int best = 1;
   uint64_t least = ~0ull;
   for (int log = 0; 1 << log <= W; ++log) {
@@ -296,24 +274,29 @@ __device__ __forceinline__ int block_rows(const W4KParams& p, int64_t b) {
   return p.rb_rows ? max(0, min(p.rb_rows[b], kFlagRows)) : kFlagRows;
 }
 
-// Steps in flight per wave: what 120 registers hold, at least two.
-constexpr int steps_ahead(int mt, int nt, int sub, bool zeros, int xq) {
-  const int pairs = nt == 4 ? 2 : nt;
-  const int regs = 4 * nt + pairs * (4 / sub) + (zeros ? pairs * (sub == 1 ? 2 : 1) : 0) + 4 * mt * xq;
-  return 120 / regs < 2 ? 2 : 120 / regs > 6 ? 6 : 120 / regs;
-}
+// Waves of a workgroup, and those that a CU holds (by registers): the grid of a launch.
+constexpr int group_waves(int nt) { return nt == 1 ? 8 : 4; }
+constexpr int waves_per_cu(int nt) { return nt == 1 ? 16 : 12; }
 
-// W waves.  An item is NT column tiles (with SwiGLU: the first half gate tiles,
-// the second the matching up tiles) of a pass of up to 16 MTX rows; `split`
-// waves share its K.  Where x goes as bf16 pairs (PARTS 2) the halves of a row
-// take two lanes of a row tile, and their two sums are added at the end.  The
-// workgroups of the grid walk the items in turn, as many as the device's row
-// count and tables say there are.  FEW, MANY: whether passes of at most 4 row
-// lanes, and of more, come (see Step).
-template <int MTX, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS, bool FEW, bool MANY>
-__global__ __launch_bounds__(64 * W, NT == 4 ? 2 : 1) void w4_kernel(W4KParams p) {
-  extern __shared__ f32x4 red[];  // [W][NT * MTX][64], used where K is split
-  constexpr int ROWS = 16 * MTX / PARTS, kPasses = EXPERTS ? kFlagRows / ROWS : 1;
+// Steps in flight per wave.  More than about 96 KB on their way into a CU is
+// slower, not faster (64 tokens on 32 experts, GEMM1 / GEMM2: 12 waves of 2
+// steps of 4 KB 59 / 36 us, 12 of 4 steps 72 / 45, 16 of 2 steps 69 / 42, 8 of
+// 2 steps 63 / 41; 1 x 8192 x 3584: 2 steps 5.9 us, 6 steps 7.5).
+constexpr int kAhead = 2;
+
+// An item is NT column tiles (with SwiGLU: the first half gate tiles, the second
+// the matching up tiles) of a pass of up to 16 rows; `split` waves of a
+// workgroup share its K.  Where x goes as bf16 pairs (PARTS 2) the halves of a
+// row take two lanes of the row tile, and their two sums are added at the end.
+// The workgroups of the grid walk the items in turn, as many as the device's row
+// count and tables say there are; the passes of one column item lie side by
+// side, since they read the same weights.  (32-row passes, two row tiles per
+// step, are slower: 32 x 8192 x 8192 22.3 us instead of 15.3.)  FEW, MANY:
+// whether passes of at most 4 row lanes, and of more, come (see Step).
+template <int NT, int SUB, bool ZEROS, int PARTS, bool EXPERTS, bool FEW, bool MANY>
+__global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4_kernel(W4KParams p) {
+  extern __shared__ f32x4 red[];  // [W][NT][64], used where K is split
+  constexpr int W = group_waves(NT), ROWS = 16 / PARTS, kPasses = kFlagRows / ROWS;
   __shared__ PassList<EXPERTS ? ROWS : kFlagRows> list;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -322,19 +305,20 @@ __global__ __launch_bounds__(64 * W, NT == 4 ? 2 : 1) void w4_kernel(W4KParams p
   const int per_item = p.swiglu ? NT / 2 : NT;  // output tiles
   const int col_items = (p.tile_cols + per_item - 1) / per_item;
   const int64_t width = p.swiglu ? (int64_t)p.tile_cols * kTile : p.w.N;
-  uint32_t passes = p.row_blocks;
+  uint32_t passes = p.passes;
   bool listed = false;
   if constexpr (EXPERTS) {
     constexpr int per = (kListed + 64 * W - 1) / (64 * W);
-    int n[per], sum = 0, blocks = p.row_blocks;
+    const int most = (int)(p.M / kFlagRows);
+    int n[per], sum = 0;
     int64_t rows_dev = p.rows_dev ? *p.rows_dev : p.M;
 #pragma unroll
     for (int i = 0; i < per; ++i) {  // (not held back by the row count)
       const int b = threadIdx.x * per + i;
-      n[i] = b < min(p.row_blocks, kListed) ? block_rows(p, b) : 0;
-      if (b < min(p.row_blocks, kListed)) list.expert[b] = p.rb_expert[b];
+      n[i] = b < min(most, kListed) ? block_rows(p, b) : 0;
+      if (b < min(most, kListed)) list.expert[b] = p.rb_expert[b];
     }
-    blocks = (int)min((int64_t)blocks, max((int64_t)0, rows_dev / kFlagRows));
+    const int blocks = (int)min((int64_t)most, max((int64_t)0, rows_dev / kFlagRows));
     listed = blocks <= kListed;
     passes = blocks * kPasses;
     if (listed) {
@@ -370,9 +354,8 @@ __global__ __launch_bounds__(64 * W, NT == 4 ? 2 : 1) void w4_kernel(W4KParams p
     int64_t row0 = 0, expert = 0;
     int ci = 0, left = 0;
     if (it < items) {
-      uint32_t q = it / col_items;
       if constexpr (EXPERTS) {
-        // the passes of one column item side by side: they read the same weights
+        uint32_t q = it / col_items;  // a pass of the item's block
         int np = kPasses, b;
         if (listed) {
           b = __builtin_amdgcn_readfirstlane((int)list.block[q]);
@@ -391,21 +374,19 @@ __global__ __launch_bounds__(64 * W, NT == 4 ? 2 : 1) void w4_kernel(W4KParams p
         left = min(left - ROWS * pass, ROWS);
         row0 = (int64_t)b * kFlagRows + ROWS * pass;
       } else {
-        ci = (int)(it - q * col_items);
-        row0 = (int64_t)q * ROWS;
+        ci = (int)(it / passes);
+        row0 = (int64_t)(it - ci * passes) * ROWS;
         left = (int)min(p.M - row0, (int64_t)ROWS);
       }
     }
     const bool any = left > 0, few = FEW && left <= 4 / PARTS;
     const int lanes = few ? 4 : 16;  // of a row tile
-    f32x4 acc[NT][MTX];
+    f32x4 acc[NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int m = 0; m < MTX; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto run = [&](auto mt, auto xq) {
-      constexpr int MT = decltype(mt)::value, XQ = decltype(xq)::value;
-      Source<MT, NT> t;
+    for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto run = [&](auto xq) {
+      constexpr int XQ = decltype(xq)::value;
+      Source<NT> t;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const bool up = p.swiglu && n >= NT / 2;
@@ -422,51 +403,40 @@ __global__ __launch_bounds__(64 * W, NT == 4 ? 2 : 1) void w4_kernel(W4KParams p
       const int r = col % EACH, half = col % LANES / EACH, k0 = (XQ == 1 ? col / 4 * 32 : 0) + quad * 8;
       t.most = (int32_t)p.w.K - 8 - k0;
       const uint32_t in_row = 2 * (uint32_t)(k0 + half * p.w.K);
+      t.row = kNowhere;
       if (EXPERTS && p.gather_pull) {
         t.x = make_rsrc(p.A, (uint32_t)(p.gather_rows * p.lda * 2));
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          t.row[m] = kNowhere;
-          if (EACH * m + r < left) {
-            const int* pr = p.gather_pull + 3 * (row0 + EACH * m + r);
-            const int64_t src = ((int64_t)pr[0] * p.gather_devs + pr[1]) * p.gather_tps + pr[2];
-            if (pr[0] >= 0 && pr[2] >= 0 && src >= 0 && src < p.gather_rows) t.row[m] = (uint32_t)(src * p.lda * 2) + in_row;
-          }
+        if (r < left) {
+          const int* pr = p.gather_pull + 3 * (row0 + r);
+          const int64_t src = ((int64_t)pr[0] * p.gather_devs + pr[1]) * p.gather_tps + pr[2];
+          if (pr[0] >= 0 && pr[2] >= 0 && src >= 0 && src < p.gather_rows) t.row = (uint32_t)(src * p.lda * 2) + in_row;
         }
       } else {
         t.x = make_rsrc(p.A + row0 * p.lda, (uint32_t)(left * p.lda * 2));
-#pragma unroll
-        for (int m = 0; m < MT; ++m) t.row[m] = EACH * m + r < left ? (uint32_t)((EACH * m + r) * p.lda * 2) + in_row : kNowhere;
+        if (r < left) t.row = (uint32_t)(r * p.lda * 2) + in_row;
       }
-      f32x4 a[NT][MT];
-      sweep<MT, NT, SUB, ZEROS, XQ, steps_ahead(MT, NT, SUB, ZEROS, XQ)>(t, KB, ks, split, lane, a);
+      sweep<NT, SUB, ZEROS, XQ, kAhead>(t, KB, ks, split, lane, acc);
+      if constexpr (PARTS == 2) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (XQ == 1) {  // rows 0 and 1, then their second halves
+            acc[n][0] += acc[n][2];
+            acc[n][1] += acc[n][3];
+          } else {  // second halves: rows 8 to 15, two quads on
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if constexpr (PARTS == 2 && XQ == 1) {  // rows 0 and 1, then their second halves
-            a[n][m][0] += a[n][m][2];
-            a[n][m][1] += a[n][m][3];
-          } else if constexpr (PARTS == 2) {  // second halves: rows 8 to 15, two quads on
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[n][m][i] += __shfl_xor(a[n][m][i], 32, 64);
+            for (int i = 0; i < 4; ++i) acc[n][i] += __shfl_xor(acc[n][i], 32, 64);
           }
-          acc[n][m] = a[n][m];
         }
+      }
     };
-    using std::integral_constant;
-    int mt = 1;
     if (any) {
       if (FEW && (few || !MANY)) {
-        if constexpr (FEW) run(integral_constant<int, 1>(), integral_constant<int, 1>());
-      } else if (MTX == 1 || left <= 16 / PARTS) {
-        if constexpr (MANY) run(integral_constant<int, 1>(), integral_constant<int, 4>());
+        if constexpr (FEW) run(std::integral_constant<int, 1>());
       } else {
-        mt = MTX;
-        if constexpr (MANY && MTX > 1) run(integral_constant<int, MTX>(), integral_constant<int, 4>());
+        if constexpr (MANY) run(std::integral_constant<int, 4>());
       }
     }
-    auto finish = [&](int n, int m, f32x4 v, f32x4 up) {
+    auto finish = [&](int n, f32x4 v, f32x4 up) {
       const int64_t c = (int64_t)(ci * per_item + n) * kTile + col;
       if (c >= width) return;
       if constexpr (NT >= 2)
@@ -474,47 +444,32 @@ __global__ __launch_bounds__(64 * W, NT == 4 ? 2 : 1) void w4_kernel(W4KParams p
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] = silu(v[i]) * up[i];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * quad + i;
-        if (r < lanes / PARTS && lanes / PARTS * m + r < left) store(p, row0 + lanes / PARTS * m + r, c, width, v[i]);
-      }
+      for (int i = 0; i < 4; ++i)
+        if (4 * quad + i < min(left, lanes / PARTS)) store(p, row0 + 4 * quad + i, c, width, v[i]);
     };
     if (split == 1) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int m = 0; m < MTX; ++m)
-          if (n < per_item && m < mt) finish(n, m, acc[n][m], acc[NT >= 2 ? (n + NT / 2) % NT : n][m]);
+        if (n < per_item) finish(n, acc[n], acc[NT >= 2 ? (n + NT / 2) % NT : n]);
       continue;
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int m = 0; m < MTX; ++m)
-        if (m < mt) red[(wave * NT * MTX + n * MTX + m) * 64 + lane] = acc[n][m];
+    for (int n = 0; n < NT; ++n) red[(wave * NT + n) * 64 + lane] = acc[n];
     __syncthreads();
-    auto total = [&](int u) {
-      f32x4 v = red[((wave - ks) * NT * MTX + u) * 64 + lane];
-      for (int o = 1; o < split; ++o) v += red[((wave - ks + o) * NT * MTX + u) * 64 + lane];
+    auto total = [&](int n) {
+      f32x4 v = red[((wave - ks) * NT + n) * 64 + lane];
+      for (int o = 1; o < split; ++o) v += red[((wave - ks + o) * NT + n) * 64 + lane];
       return v;
     };
     if (any)
-      for (int u = ks; u < per_item * mt; u += split) {
-        const int n = u / mt, m = u - n * mt;
-        const f32x4 v = total(n * MTX + m);
-        finish(n, m, v, p.swiglu ? total((n + NT / 2) * MTX + m) : v);
+      for (int n = ks; n < per_item; n += split) {
+        const f32x4 v = total(n);
+        finish(n, v, p.swiglu ? total(n + NT / 2) : v);
       }
     __syncthreads();
   }
 }
 
-template <int MTX, int NT, int W, int SUB, bool ZEROS, int PARTS, bool EXPERTS, bool FEW, bool MANY>
-void launch(const W4KParams& p, int grid, hipStream_t stream) {
-  hipLaunchKernelGGL((w4_kernel<MTX, NT, W, SUB, ZEROS, PARTS, EXPERTS, FEW, MANY>), dim3(grid), dim3(64 * W),
-                     W * NT * MTX * 64 * sizeof(f32x4), stream, p);
-}
-
-// One thread per 4 bytes of the packed weights.
 __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros,
                                                       int64_t K, int64_t N, int64_t KB, int64_t pairs, int64_t given,
                                                       int groups, int64_t words, uint32_t* out) {
@@ -595,64 +550,53 @@ hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E
   return hipGetLastError();
 }
 
-// Waves that a CU holds (by registers), the grid of a launch.
-constexpr int waves_per_cu(int mt, int nt) {
-  return nt == 4 ? (mt == 1 ? 12 : 8) : (mt == 1 ? 16 : 12);
-}
-
 hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
   if (args.M == 0) return hipSuccess;
   W4KParams p = args;
-  const bool experts = p.rb_expert != nullptr;
-  auto go = [&](auto mt, auto nt, auto w, auto sub, auto zeros, auto parts, auto ex) {
-    constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value, W = decltype(w)::value;
-    p.row_blocks = (int)(decltype(ex)::value ? p.M / kFlagRows : (p.M + 16 * MT - 1) / (16 * MT));
-    const int per_item = p.swiglu ? NT / 2 : NT;
-    const int passes = decltype(ex)::value ? kFlagRows * decltype(parts)::value / (16 * MT) : 1;
-    const int64_t items = (int64_t)p.row_blocks * passes * ((p.tile_cols + per_item - 1) / per_item);
-    const int64_t most = (int64_t)cus * waves_per_cu(MT, NT) / W;
-    int64_t grid = std::min<int64_t>(items, most);
-    if (!decltype(ex)::value) {
-      p.split = choose_split((uint32_t)items, (uint32_t)(most * W), (uint32_t)((p.w.K + kBlock - 1) / kBlock), W);
-      grid = std::min<int64_t>(most, (items * p.split + W - 1) / W);
-    }
-    constexpr int SUB = decltype(sub)::value, PARTS = decltype(parts)::value;
-    constexpr bool ZEROS = decltype(zeros)::value;
-    if constexpr (decltype(ex)::value) {
-      launch<MT, NT, W, SUB, ZEROS, PARTS, true, true, true>(p, (int)grid, stream);
-    } else if constexpr (MT == 1) {
-      if (p.M <= 4) launch<MT, NT, W, SUB, ZEROS, PARTS, false, true, false>(p, (int)grid, stream);
-      else launch<MT, NT, W, SUB, ZEROS, PARTS, false, false, true>(p, (int)grid, stream);
-    } else {
-      launch<MT, NT, W, SUB, ZEROS, PARTS, false, false, true>(p, (int)grid, stream);
-    }
-  };
   using std::integral_constant;
-  auto with_zeros = [&](auto mt, auto nt, auto w, auto sub, auto parts, auto ex) {
-    if (p.w.zeros) go(mt, nt, w, sub, std::true_type(), parts, ex);
-    else go(mt, nt, w, sub, std::false_type(), parts, ex);
+  auto launch = [&](auto kernel, int nt, bool experts) {
+    const int w = group_waves(nt), rows = 16 / p.parts, per_item = p.swiglu ? nt / 2 : nt;
+    p.passes = (uint32_t)((p.M + rows - 1) / rows);  // (experts: at most so many)
+    const int64_t items = (int64_t)p.passes * ((p.tile_cols + per_item - 1) / per_item);
+    const int64_t most = (int64_t)cus * waves_per_cu(nt) / w;
+    int64_t grid = std::min<int64_t>(items, most);
+    if (!experts) {
+      p.split = choose_split((uint32_t)items, (uint32_t)(most * w), (uint32_t)((p.w.K + kBlock - 1) / kBlock), w);
+      grid = std::min<int64_t>(most, (items * p.split + w - 1) / w);
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * w), w * nt * 64 * sizeof(f32x4), stream, p);
   };
-  auto with_group = [&](auto mt, auto nt, auto w, auto parts, auto ex) {
-    if (p.w.group == 32) with_zeros(mt, nt, w, integral_constant<int, 1>(), parts, ex);
-    else if (p.w.group == 64) with_zeros(mt, nt, w, integral_constant<int, 2>(), parts, ex);
-    else with_zeros(mt, nt, w, integral_constant<int, 4>(), parts, ex);
+  auto go = [&](auto nt, auto sub, auto zeros) {
+    constexpr int NT = decltype(nt)::value, SUB = decltype(sub)::value;
+    constexpr bool Z = decltype(zeros)::value;
+    if (!p.rb_expert) {
+      if constexpr (NT == 1)
+        if (p.M <= 4) return launch(w4_kernel<1, SUB, Z, 1, false, true, false>, 1, false);
+      if constexpr (NT != 2) launch(w4_kernel<NT, SUB, Z, 1, false, false, true>, NT, false);
+    } else if constexpr (NT != 1) {
+      if (p.parts == 2) launch(w4_kernel<NT, SUB, Z, 2, true, true, true>, NT, true);
+      else launch(w4_kernel<NT, SUB, Z, 1, true, true, true>, NT, true);
+    }
   };
-  constexpr integral_constant<int, 1> one;
-  constexpr integral_constant<int, 2> two;
-  constexpr integral_constant<int, 4> four;
-  constexpr integral_constant<int, 8> eight;
-  if (experts) {
-    // SwiGLU's gate and up tiles go in pairs where the width is a whole number of them
-    const bool pairs = !p.swiglu || p.tile_cols % 2 == 0;
-    if (p.parts == 2 && pairs) with_group(two, four, four, two, std::true_type());
-    else if (p.parts == 2) with_group(two, two, four, two, std::true_type());
-    else if (pairs) with_group(two, four, four, one, std::true_type());
-    else with_group(two, two, four, one, std::true_type());
-  } else if (p.M <= 16) {
-    with_group(one, one, eight, one, std::false_type());
-  } else {
-    with_group(two, four, eight, one, std::false_type());
-  }
+  auto with_zeros = [&](auto nt, auto sub) {
+    if (p.w.zeros) go(nt, sub, std::true_type());
+    else go(nt, sub, std::false_type());
+  };
+  auto with_group = [&](auto nt) {
+    if (p.w.group == 32) with_zeros(nt, integral_constant<int, 1>());
+    else if (p.w.group == 64) with_zeros(nt, integral_constant<int, 2>());
+    else with_zeros(nt, integral_constant<int, 4>());
+  };
+  // Column tiles of an item.  Experts: four, or two (one gate, one up) where
+  // SwiGLU's tiles are no whole pairs.  Dense: with more than 4 rows, x is read
+  // once per item and four tiles pay from kWideItems row tiles x column tiles on
+  // (16 x 8192 x 8192 19.9 us with one, 13.6 with four; 16 x 7168 x 4096 11.1
+  // and 12.0); up to 4 rows one tile, and more waves, always (1 x 8192 x 8192
+  // 8.6 us, with four 11.2).
+  constexpr int64_t kWideItems = 384;
+  if (p.rb_expert ? p.swiglu && p.tile_cols % 2 : false) with_group(integral_constant<int, 2>());
+  else if (p.rb_expert || (p.M > 4 && (p.M + 15) / 16 * p.tile_cols >= kWideItems)) with_group(integral_constant<int, 4>());
+  else with_group(integral_constant<int, 1>());
   return hipGetLastError();
 }
 
