@@ -1113,7 +1113,7 @@ int mk_moe_combine_backward(const mk_moe_combine_backward_args* a, void* stream)
     return fail(MK_ESHAPE, "mk_moe_combine_backward: R_pad must be a multiple of %d", MK_ROW_BLOCK);
   if (a->topk > mk::kMaxTopk) return fail(MK_ESHAPE, "mk_moe_combine_backward: topk must be at most %d", mk::kMaxTopk);
   if (a->dy_dtype != 0 && a->dy_dtype != 1) return fail(MK_EINVAL, "mk_moe_combine_backward: dy_dtype must be 0 or 1");
-  if (a->num_tokens > INT32_MAX || a->R_pad > INT32_MAX)
+  if (a->num_tokens > INT32_MAX / 2 || a->R_pad > INT32_MAX)
     return fail(MK_ESHAPE, "mk_moe_combine_backward: too many rows");
   const bool rows = a->R_pad > 0;
   if ((a->num_tokens > 0 && (!a->dy || !a->topk_ids || !a->owner_offset || !a->dgates)) ||
@@ -1126,7 +1126,7 @@ int mk_moe_combine_backward(const mk_moe_combine_backward_args* a, void* stream)
   mk::CombineBwdKParams p{a->dy, static_cast<const uint16_t*>(a->y_expert), a->topk_ids, a->row_weight,
                           a->owner_offset, a->slot_to_row, a->rb_rows, static_cast<uint16_t*>(a->dy_expert),
                           a->dgates, a->num_tokens, a->H, a->R_pad, a->topk, a->expert_begin, a->n_local,
-                          a->dy_dtype, a->sizes ? a->sizes + 1 : nullptr};
+                          a->dy_dtype, a->sizes ? a->sizes + 1 : nullptr, 0};
   hipError_t e = mk::launch_combine_backward(p, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_combine_backward launch");
 }

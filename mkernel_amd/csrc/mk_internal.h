@@ -179,8 +179,9 @@ struct CombineBwdKParams {
   int k, e0, n_local;
   int dy_dtype;
   const int64_t* rows_dev;
+  int pad_blocks;           // set by the launch
 };
-hipError_t launch_combine_backward(const CombineBwdKParams& p, hipStream_t stream);
+hipError_t launch_combine_backward(CombineBwdKParams p, hipStream_t stream);
 
 // Router (mk_route.hip).
 struct RouteKParams {

@@ -129,91 +129,129 @@ hipError_t launch_combine(const CombineKParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Gradient of the combine: workgroup t < T has token t's, one that follows the
-// padding rows of a row block.
+// Gradient of the combine.
 //   dy_expert[r] = row_weight[r] * dy[t]            (one bf16 rounding)
 //   dgates[t, j] = sum_c dy[t, c] * y_expert[r, c]  (fp32), r the row of (t, j)
+// Bound by its bytes (dy and the routed rows read, dy_expert's whole row blocks
+// written).  Workgroup p.pad_blocks + t has token t's rows, kAtOnce of them
+// against one read of dy; the first p.pad_blocks zero kPadRows padding rows
+// each (a whole row block's in one workgroup was the longest of the launch).
 // The row of (t, j) is found as the index build gave it out: the token's local
 // choices, ordered by (expert, j), have its slots in turn.
+constexpr int kAtOnce = 4, kPadRows = 8;
 template <class T>
 __global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineBwdKParams p) {
   typedef uint32_t words __attribute__((ext_vector_type(4)));
+  constexpr int U = 4;  // pieces of 8 columns a thread has on their way
   const int64_t R = p.rows_dev ? min(p.R_pad, *p.rows_dev) : p.R_pad;
   const int64_t vec = p.H / 8;
-  if (blockIdx.x >= p.T) {
-    const int64_t b = blockIdx.x - p.T;
-    if (b * kFlagRows >= R) return;
-    const int real = min(max(p.rb_rows[b], 0), kFlagRows);
-    uint4* dst = reinterpret_cast<uint4*>(p.dy_expert + (b * kFlagRows + real) * p.H);
-    const uint4 z = {0u, 0u, 0u, 0u};
-    for (int64_t c = threadIdx.x; c < (kFlagRows - real) * vec; c += kThreads) dst[c] = z;
+  if ((int)blockIdx.x < p.pad_blocks) {
+    const int64_t r0 = (int64_t)blockIdx.x * kPadRows, b = r0 / kFlagRows;
+    if (r0 >= R) return;
+    const int64_t from = max(r0, b * kFlagRows + min(max(p.rb_rows[b], 0), kFlagRows));
+    words* dst = reinterpret_cast<words*>(p.dy_expert);
+    for (int64_t c = from * vec + threadIdx.x; c < (r0 + kPadRows) * vec; c += kThreads) dst[c] = words{0u, 0u, 0u, 0u};
     return;
   }
-  const int64_t t = blockIdx.x;
-  __shared__ int rows[kMaxTopk];
-  __shared__ float part[kThreads / 64];
-  if (threadIdx.x < (unsigned)p.k) {
-    const int j = threadIdx.x, e = p.ids[t * p.k + j] - p.e0;
-    int row = -1;
-    if (e >= 0 && e < p.n_local) {
-      int slot = p.owner_offset[t];
-      for (int i = 0; i < p.k; ++i) {
-        const int o = p.ids[t * p.k + i] - p.e0;
-        slot += o >= 0 && o < p.n_local && (o < e || (o == e && i < j));
-      }
-      if (slot < p.owner_offset[t + 1]) row = p.slot_to_row[slot];
-      if (row >= R) row = -1;
+  const int64_t t = (int)blockIdx.x - p.pad_blocks;
+  __shared__ int rows[kMaxTopk], choice[kMaxTopk], count;
+  __shared__ float part[kThreads / 64][kAtOnce];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (wave == 0) {
+    const int e = lane < p.k ? p.ids[t * p.k + lane] - p.e0 : -1;
+    const bool local = e >= 0 && e < p.n_local;
+    int slot = p.owner_offset[t], row = -1;
+    for (int i = 0; i < p.k; ++i) {
+      const int o = __shfl(e, i, 64);
+      slot += o >= 0 && o < p.n_local && (o < e || (o == e && i < lane));
     }
-    rows[j] = row;
+    if (local && slot < p.owner_offset[t + 1]) row = p.slot_to_row[slot];
+    if (row >= R) row = -1;
+    const uint64_t there = __ballot(row >= 0);
+    const int at = __popcll(there & ((1ull << lane) - 1));
+    if (row >= 0) {
+      rows[at] = row;
+      choice[at] = lane;
+    } else if (lane < p.k) {
+      p.dgates[t * p.k + lane] = 0.f;
+    }
+    if (lane == 0) count = __popcll(there);
   }
   __syncthreads();
   const T* dy = static_cast<const T*>(p.dy) + t * p.H;
-  for (int j = 0; j < p.k; ++j) {
-    const int row = rows[j];
-    float dot = 0.f;
-    if (row >= 0) {
-      const float w = p.row_weight[row];
-      for (int64_t c = threadIdx.x; c < vec; c += kThreads) {
-        float d[8];
+  for (int j0 = 0; j0 < count; j0 += kAtOnce) {
+    const int n = min(count - j0, kAtOnce);
+    int64_t row[kAtOnce];
+    float w[kAtOnce], dot[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      row[j] = rows[min(j0 + j, count - 1)];
+      w[j] = p.row_weight[row[j]];
+      dot[j] = 0.f;
+    }
+    for (int64_t c0 = threadIdx.x; c0 < vec; c0 += U * kThreads) {
+      float d[U][8];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t c = c0 + u * kThreads;
+        if (c >= vec) continue;
         if constexpr (sizeof(T) == 2) {
           const words v = *reinterpret_cast<const words*>(dy + 8 * c);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            d[2 * i] = bf16_lo(v[i]);
-            d[2 * i + 1] = bf16_hi(v[i]);
+            d[u][2 * i] = bf16_lo(v[i]);
+            d[u][2 * i + 1] = bf16_hi(v[i]);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const f32x4 v = *reinterpret_cast<const f32x4*>(dy + 8 * c + 4 * i);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) d[4 * i + b] = v[b];
+            for (int b = 0; b < 4; ++b) d[u][4 * i + b] = v[b];
           }
         }
-        const words y = *reinterpret_cast<const words*>(p.y_expert + row * p.H + 8 * c);
-        words o;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          dot += d[2 * i] * bf16_lo(y[i]);
-          dot += d[2 * i + 1] * bf16_hi(y[i]);
-          o[i] = pack_bf16x2(w * d[2 * i], w * d[2 * i + 1]);
-        }
-        if (p.dy_expert) *reinterpret_cast<words*>(p.dy_expert + row * p.H + 8 * c) = o;
       }
 #pragma unroll
-      for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d, 64);
-      if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
-      __syncthreads();
-      dot = 0.f;
-      for (int w2 = 0; w2 < kThreads / 64; ++w2) dot += part[w2];
-      __syncthreads();
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (j >= n) continue;
+        words y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + u * kThreads < vec) y[u] = *reinterpret_cast<const words*>(p.y_expert + row[j] * p.H + 8 * (c0 + u * kThreads));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t c = c0 + u * kThreads;
+          if (c >= vec) continue;
+          words o;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            dot[j] += d[u][2 * i] * bf16_lo(y[u][i]);
+            dot[j] += d[u][2 * i + 1] * bf16_hi(y[u][i]);
+            o[i] = pack_bf16x2(w[j] * d[u][2 * i], w[j] * d[u][2 * i + 1]);
+          }
+          if (p.dy_expert) *reinterpret_cast<words*>(p.dy_expert + row[j] * p.H + 8 * c) = o;
+        }
+      }
     }
-    if (threadIdx.x == 0) p.dgates[t * p.k + j] = dot;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+#pragma unroll
+      for (int s = 32; s; s >>= 1) dot[j] += __shfl_xor(dot[j], s, 64);
+      if (lane == 0) part[wave][j] = dot[j];
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+      float sum = 0.f;
+      for (int v = 0; v < kThreads / 64; ++v) sum += part[v][threadIdx.x];
+      p.dgates[t * p.k + choice[j0 + threadIdx.x]] = sum;
+    }
+    __syncthreads();
   }
 }
 
-hipError_t launch_combine_backward(const CombineBwdKParams& p, hipStream_t stream) {
-  const int64_t blocks = p.T + (p.dy_expert ? p.R_pad / kFlagRows : 0);
+hipError_t launch_combine_backward(CombineBwdKParams p, hipStream_t stream) {
+  p.pad_blocks = p.dy_expert ? (int)(p.R_pad / kPadRows) : 0;
+  const int64_t blocks = p.T + p.pad_blocks;
   if (blocks == 0) return hipSuccess;
   if (p.dy_dtype == 0)
     hipLaunchKernelGGL(combine_backward_kernel<float>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);

@@ -250,26 +250,18 @@ def moe_build_indices_dev(topk_ids: torch.Tensor, gates: torch.Tensor, e0: int, 
     # row count for the grouped GEMMs
     cap = (T * k + n_local * (row_block - 1) + row_block - 1) // row_block * row_block
     i32 = dict(dtype=torch.int32, device=dev)
-    t = {
-        "padded_tokens_per_expert": torch.empty(n_local, **i32),
-        "local_rb_per_expert": torch.empty(n_local, **i32),
-        "pull_indices": torch.empty((cap, 3), **i32),
-        "row_expert": torch.empty(cap, **i32),
-        "rb_expert": torch.empty((cap + row_block - 1) // row_block, **i32),
-        "rb_rows": torch.empty((cap + row_block - 1) // row_block, **i32),
-        "row_weight": torch.empty(cap, dtype=torch.float32, device=dev),
-        "owner_offset": torch.empty(T + 1, **i32),
-        "row_to_slot": torch.empty(cap, **i32),
-        "row_to_owner": torch.empty(cap, **i32),
-        "slot_to_row": torch.empty(max(cap, 1), **i32),
-    }
     L = capi.lib()
     wsb = int(L.mk_moe_index_workspace_bytes(T, k, n_local))
-    ws = torch.empty(max(wsb, 4), dtype=torch.uint8, device=dev)
+    # one allocation for the tables and the workspace: 13 took most of the call
+    nb = (cap + row_block - 1) // row_block
+    padded, local_rb, pull, row_expert, rb_expert, rb_rows, weight, offset, to_slot, to_owner, to_row, ws = torch.empty(
+        2 * n_local + 2 * nb + 7 * cap + T + 1 + max(cap, 1) + max(wsb, 4) // 4, **i32).split_with_sizes(
+        (n_local, n_local, 3 * cap, cap, nb, nb, cap, T + 1, cap, cap, max(cap, 1), max(wsb, 4) // 4))
+    t = dict(zip(_INDEX_TABLES, (padded, local_rb, pull.view(cap, 3), row_expert, rb_expert, rb_rows,
+                                 weight.view(torch.float32), offset, to_slot, to_owner, to_row)))
     sizes = torch.empty(2, dtype=torch.int64, device=dev)  # both words are written by the build
-    idx = MoeIndex(*[_ptr(t[f]) for f, _ in MoeIndex._fields_])
-    args = MoeIndexDevArgs(_ptr(ids), _ptr(g), T, k, e0, n_local, row_block, cap, _ptr(ws), wsb, _ptr(sizes), idx)
-    capi.call("mk_moe_build_indices_dev", args, _stream())
+    capi.call_values("mk_moe_build_indices_dev", MoeIndexDevArgs, _stream(), _ptr(ids), _ptr(g), T, k, e0, n_local,
+                     row_block, cap, _ptr(ws), wsb, _ptr(sizes), *[t[f].data_ptr() for f in _INDEX_TABLES])
     if not sync:
         t["sizes"] = sizes
         return t
@@ -655,15 +647,16 @@ def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> t
 
 
 def _block_tables(rb_expert, rb_rows, R_pad, sizes, dev):
+    n = R_pad // capi.ROW_BLOCK
     if R_pad % capi.ROW_BLOCK:
         raise ValueError(f"the tables' rows must be a multiple of {capi.ROW_BLOCK}")
-    _tensor(rb_expert, "rb_expert", _I32, dim=1, device=dev)
-    if rb_rows is not None:
-        _tensor(rb_rows, "rb_rows", _I32, dim=1, device=dev)
-    for t in (rb_expert, rb_rows):
-        if t is not None and t.shape[0] * capi.ROW_BLOCK < R_pad:
-            raise ValueError("rb_expert and rb_rows must cover the rows")
-    if sizes is not None:
+    for t, name in ((rb_expert, "rb_expert"), (rb_rows, "rb_rows")):
+        if (t is None and name == "rb_rows") or _is(t, torch.int32, (n,), dev):
+            continue
+        _tensor(t, name, _I32, dim=1, device=dev)
+        if t.shape[0] < n:
+            raise ValueError(f"{name} must cover the rows")
+    if sizes is not None and not _is(sizes, torch.int64, (2,), dev):
         _tensor(sizes, "sizes", (torch.int64,), (2,), device=dev)
 
 
@@ -718,30 +711,36 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
     dev = tokens.device
     _w4(w1, "w1", dev)
     _w4(w2, "w2", dev, w1.experts)
-    H, I = w1.K, w2.K
-    if w1.N != 2 * I or w2.N != H or tokens.shape[1] != H:
+    n, H = tokens.shape
+    I = w2.K
+    if w1.N != 2 * I or w2.N != H or w1.K != H:
         raise ValueError("w1 must be [E, H, 2I], w2 [E, I, H] and tokens [n, H]")
     _tensor(pull, "pull", _I32, (None, 3), device=dev)
     R_pad = pull.shape[0]
-    _tensor(act, "act", _BF16, (R_pad, 2 * I), device=dev)
-    _tensor(y_expert, "y_expert", _F32, (R_pad, H), device=dev)
+    if not _is(act, torch.bfloat16, (R_pad, 2 * I), dev):
+        _tensor(act, "act", _BF16, (R_pad, 2 * I), device=dev)
+    if not _is(y_expert, torch.float32, (R_pad, H), dev):
+        _tensor(y_expert, "y_expert", _F32, (R_pad, H), device=dev)
     _tensor(y_out, "y_out", _LOGITS, (None, H), device=dev)
     T = y_out.shape[0]
-    _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)
-    _tensor(owner_offset, "owner_offset", _I32, (T + 1,), device=dev)
+    if not _is(row_weight, torch.float32, (R_pad,), dev):
+        _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)
+        if row_weight.shape[0] < R_pad:
+            raise ValueError("row_weight must cover the rows")
+    if not _is(owner_offset, torch.int32, (T + 1,), dev):
+        _tensor(owner_offset, "owner_offset", _I32, (T + 1,), device=dev)
     _tensor(slot_to_row, "slot_to_row", _I32, dim=1, device=dev)
-    if row_weight.shape[0] < R_pad:
-        raise ValueError("row_weight must cover the rows")
     _block_tables(rb_expert, rb_rows, R_pad, sizes, dev)
-    tps = tokens.shape[0] if tokens_per_src is None else tokens_per_src
-    with _on(dev):
-        capi.call_values("mk_moe_ffn_combine_w4", MoeFfnW4Args, _stream(), tokens.data_ptr(), pull.data_ptr(),
-                         rb_expert.data_ptr(), _ptr(rb_rows), row_weight.data_ptr(), owner_offset.data_ptr(),
-                         slot_to_row.data_ptr(), *w1._values(), *w2._values(), act.data_ptr(), y_expert.data_ptr(),
-                         y_out.data_ptr(), T, tokens.shape[0], R_pad, tps, devs_per_node,
-                         int(y_out.dtype == torch.bfloat16), _ptr(sizes))
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return moe_ffn_combine_w4(tokens, pull, row_weight, owner_offset, slot_to_row, w1, w2, act, y_expert,
+                                      y_out, rb_expert, rb_rows, tokens_per_src, devs_per_node, sizes)
+    capi.call_values("mk_moe_ffn_combine_w4", MoeFfnW4Args, _stream(), tokens.data_ptr(), pull.data_ptr(),
+                     rb_expert.data_ptr(), _ptr(rb_rows), row_weight.data_ptr(), owner_offset.data_ptr(),
+                     slot_to_row.data_ptr(), *w1._values(), *w2._values(), act.data_ptr(), y_expert.data_ptr(),
+                     y_out.data_ptr(), T, n, R_pad, n if tokens_per_src is None else tokens_per_src, devs_per_node,
+                     y_out.dtype is torch.bfloat16, _ptr(sizes))
     return y_out
-
 
 
 def probe_mfma_ceiling(iters: int = 20000, num_wg: int = 0, reps: int = 3) -> dict:
