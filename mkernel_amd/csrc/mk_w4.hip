@@ -470,6 +470,7 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
   }
 }
 
+// One thread per 4 bytes of the packed weights.
 __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros,
                                                       int64_t K, int64_t N, int64_t KB, int64_t pairs, int64_t given,
                                                       int groups, int64_t words, uint32_t* out) {
