@@ -474,35 +474,35 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
 __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros,
                                                       int64_t K, int64_t N, int64_t KB, int64_t pairs, int64_t given,
                                                       int groups, int64_t words, uint32_t* out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= words) return;
   const int unit = (int)(block_bytes(groups, zeros != nullptr) / 4);
-  const int64_t block = i / unit, kb = block % KB, pair = block / KB % pairs, e = block / KB / pairs;
-  const int at = (int)(i - block * unit);
-  uint32_t w = 0;
-  if (at < 512) {  // codes: [2 tiles][64 lanes][4 MFMAs], see expand()
-    const int j = at & 3, lane = (at >> 2) & 63;
-    const int64_t n = (2 * pair + (at >> 8)) * kTile + (lane & 15), k0 = kb * kBlock + j * 32 + (lane >> 4) * 8;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
+    const int64_t block = i / unit, kb = block % KB, pair = block / KB % pairs, e = block / KB / pairs;
+    const int at = (int)(i - block * unit);
+    uint32_t w = 0;
+    if (at < 512) {  // codes: [2 tiles][64 lanes][4 MFMAs], see expand()
+      const int j = at & 3, lane = (at >> 2) & 63;
+      const int64_t n = (2 * pair + (at >> 8)) * kTile + (lane & 15), k0 = kb * kBlock + j * 32 + (lane >> 4) * 8;
 #pragma unroll
-    for (int o = 0; o < 8; ++o) {
-      const int64_t k = k0 + o;
-      const uint32_t q = k < K && n < N ? codes[(e * K + k) * N + n] & 15u : 8u;
-      w |= q << (4 * ((o & 1) * 4 + (o >> 1)));
+      for (int o = 0; o < 8; ++o) {
+        const int64_t k = k0 + o;
+        const uint32_t q = k < K && n < N ? codes[(e * K + k) * N + n] & 15u : 8u;
+        w |= q << (4 * ((o & 1) * 4 + (o >> 1)));
+      }
+    } else {
+      // scales, two to a word, then zero points, four: [16 columns][groups][2 tiles]
+      const bool zero = at >= 512 + 16 * groups;
+      const int first = zero ? 4 * (at - 512 - 16 * groups) : 2 * (at - 512);
+      for (int o = 0; o < (zero ? 4 : 2); ++o) {
+        const int u = first + o;
+        const int64_t n = (2 * pair + u % 2) * kTile + u / (2 * groups), g = kb * groups + u / 2 % groups;
+        const bool in = g < given && n < N;
+        const int64_t src = (e * given + g) * N + n;
+        if (zero) w |= (in ? zeros[src] & 15u : 8u) << (8 * o);
+        else w |= (in ? (uint32_t)scales[src] : 0u) << (16 * o);
+      }
     }
-  } else {
-    // scales, two to a word, then zero points, four: [16 columns][groups][2 tiles]
-    const bool zero = at >= 512 + 16 * groups;
-    const int first = zero ? 4 * (at - 512 - 16 * groups) : 2 * (at - 512);
-    for (int o = 0; o < (zero ? 4 : 2); ++o) {
-      const int u = first + o;
-      const int64_t n = (2 * pair + u % 2) * kTile + u / (2 * groups), g = kb * groups + u / 2 % groups;
-      const bool in = g < given && n < N;
-      const int64_t src = (e * given + g) * N + n;
-      if (zero) w |= (in ? zeros[src] & 15u : 8u) << (8 * o);
-      else w |= (in ? (uint32_t)scales[src] : 0u) << (16 * o);
-    }
+    out[i] = w;
   }
-  out[i] = w;
 }
 
 // One thread per group and column: scale = bf16(largest magnitude / 7), code =
@@ -510,23 +510,23 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, cons
 __global__ __launch_bounds__(256) void w4_quantize_kernel(const uint16_t* W, int64_t K, int64_t N, int group,
                                                           int64_t groups, int64_t count, uint8_t* codes,
                                                           uint16_t* scales) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= count) return;
-  const int64_t n = i % N, g = i / N % groups, e = i / N / groups;
-  const int64_t k0 = g * group, k1 = min(K, k0 + group);
-  auto value = [&](int64_t k) { return __uint_as_float((uint32_t)W[(e * K + k) * N + n] << 16); };
-  float most = 0.f;
-  for (int64_t k = k0; k < k1; ++k) most = fmaxf(most, fabsf(value(k)));
-  const __bf16 s = (__bf16)(most / 7.f);
-  const float scale = (float)s;
-  scales[i] = __builtin_bit_cast(uint16_t, s);
-  for (int64_t k = k0; k < k1; ++k) {
-    const float q = scale > 0.f ? rintf(value(k) / scale) : 0.f;
-    codes[(e * K + k) * N + n] = (uint8_t)((int)fminf(fmaxf(q, -8.f), 7.f) + 8);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i % N, g = i / N % groups, e = i / N / groups;
+    const int64_t k0 = g * group, k1 = min(K, k0 + group);
+    auto value = [&](int64_t k) { return __uint_as_float((uint32_t)W[(e * K + k) * N + n] << 16); };
+    float most = 0.f;
+    for (int64_t k = k0; k < k1; ++k) most = fmaxf(most, fabsf(value(k)));
+    const __bf16 s = (__bf16)(most / 7.f);
+    const float scale = (float)s;
+    scales[i] = __builtin_bit_cast(uint16_t, s);
+    for (int64_t k = k0; k < k1; ++k) {
+      const float q = scale > 0.f ? rintf(value(k) / scale) : 0.f;
+      codes[(e * K + k) * N + n] = (uint8_t)((int)fminf(fmaxf(q, -8.f), 7.f) + 8);
+    }
   }
 }
 
-unsigned blocks256(int64_t n) { return (unsigned)((n + 255) / 256); }
+unsigned blocks256(int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, 1 << 22); }
 
 }  // namespace
 

@@ -9,7 +9,6 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import math
-from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -549,15 +548,20 @@ def moe_combine_backward(dy: torch.Tensor, y_expert: torch.Tensor, ids: torch.Te
 
 
 # ------------------------------------------------------------------- 4-bit weights
-class W4Weights(NamedTuple):
-    """4-bit weights laid out by w4_pack: E matrices [K, N], values
-    (code - zero) * scale per `group` rows of K."""
-    packed: torch.Tensor  # codes, scales and zero points
-    K: int
-    N: int
-    group: int
-    experts: int
-    zeros: bool           # whether there are zero points
+class W4Weights:
+    """4-bit weights laid out by w4_pack: ``experts`` matrices [K, N], values
+    (code - zero) * scale per ``group`` rows of K, in one uint8 tensor
+    ``packed`` that may be stored and made W4Weights again."""
+    __slots__ = ("packed", "K", "N", "group", "experts", "zeros")
+
+    def __init__(self, packed: torch.Tensor, K: int, N: int, group: int, experts: int = 1, zeros: bool = False):
+        _tensor(packed, "packed", _U8, dim=1)
+        n = capi.lib().mk_w4_packed_bytes(K, N, experts, group, bool(zeros))
+        if n < 0:
+            raise ValueError(f"no 4-bit weights of {experts} x {K} x {N} in groups of {group}")
+        if packed.numel() != n:
+            raise ValueError(f"packed holds {packed.numel()} bytes, {experts} x {K} x {N} takes {n}")
+        self.packed, self.K, self.N, self.group, self.experts, self.zeros = packed, K, N, group, experts, bool(zeros)
 
     def _values(self) -> tuple:
         return self.packed.data_ptr(), self.K, self.N, self.group, self.experts, self.zeros
@@ -588,10 +592,8 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, group: int, zeros: torch.
         _tensor(zeros, "zeros", _U8, shape, device=codes.device)
     dev = codes.device
     n = capi.lib().mk_w4_packed_bytes(K, N, E, group, zeros is not None)
-    if n < 0:
-        raise ValueError(f"weights of {E} x {K} x {N} are too large")
     with _on(dev):
-        w = W4Weights(torch.empty(n, dtype=torch.uint8, device=dev), K, N, group, E, zeros is not None)
+        w = W4Weights(torch.empty(max(n, 0), dtype=torch.uint8, device=dev), K, N, group, E, zeros is not None)
         capi.call_values("mk_w4_pack", W4PackArgs, _stream(), codes.data_ptr(), scales.data_ptr(), _ptr(zeros),
                          *w._values())
     return w
@@ -723,6 +725,8 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
         _tensor(y_expert, "y_expert", _F32, (R_pad, H), device=dev)
     _tensor(y_out, "y_out", _LOGITS, (None, H), device=dev)
     T = y_out.shape[0]
+    if T == 0 and n == 0:
+        return y_out
     if not _is(row_weight, torch.float32, (R_pad,), dev):
         _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)
         if row_weight.shape[0] < R_pad:

@@ -100,6 +100,114 @@ def test_route_and_balance(dev, T, E, k, pad, renorm, dtype):
         assert abs(float(r["loss"]) - float(loss)) <= rtol * float(loss)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k", [(70001, 24, 3), (9001, 250, 8), (40000, 700, 2)])
+def test_long_batches(dev, T, E, k, dtype):
+    """Several tokens per wave, and as many workgroups as there may be."""
+    _say("long", T, E, k, dtype)
+    g = torch.Generator(device=dev).manual_seed(T)
+    x = torch.randn((T, E), generator=g, device=dev).mul_(3).clamp_(-14, 14).to(dtype)
+    top, ids = torch.sort(x, dim=1, descending=True, stable=True)
+    p = torch.softmax(x.to(D), 1)
+    r = ops.moe_route_balance(x, k, 0.5)
+    assert torch.equal(r["ids"].long(), ids[:, :k])
+    assert torch.allclose(r["gates"].to(D), torch.softmax(top[:, :k].to(D), 1), rtol=2 ** -18, atol=0)
+    counts = torch.bincount(ids[:, :k].reshape(-1), minlength=E)
+    rtol = 2 ** -18 + (T / 4096 + 8) * 2 ** -24
+    assert torch.equal(r["counts"].long(), counts) and int(r["tokens"]) == T
+    assert torch.allclose(r["prob_sum"].to(D), p.sum(0), rtol=rtol, atol=0)
+    loss = 0.5 * E / (k * T * T) * (counts.to(D) * p.sum(0)).sum()
+    assert abs(float(r["loss"]) - float(loss)) <= rtol * float(loss)
+    again = ops.moe_route_balance(x, k, 0.5)
+    assert all(torch.equal(r[f], again[f]) for f in r)
+    dg = torch.randn((T, k), generator=g, device=dev)
+    d = ops.moe_route_backward(x, r["ids"], dgates=dg, counts=r["counts"], tokens=r["tokens"], coef=0.5)
+    want, mag = _gradient(x.to(D).cpu(), ids[:, :k].cpu(), dg.cpu(), counts.cpu(), T, 0.5, 1.0, True)
+    tol = 2 ** -17 * mag + 1e-37 + (2 ** -8 * want.abs() if dtype is torch.bfloat16 else 0)
+    assert bool(((d.cpu().to(D) - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_columns_of_a_wider_matrix(dev, dtype):
+    """Logits, and their gradient, at column offsets and row strides of every alignment: nothing beside them is read or
+    written. Sums over a token's experts go in another order where they are loaded in other pieces."""
+    _say("columns", dtype)
+    T, E, k = 37, 60, 4
+    x = _logits(T, E, dtype, 4).to(dev)
+    dg = torch.randn((T, k), generator=torch.Generator().manual_seed(3)).to(dev)
+    r = ops.moe_route_balance(x, k, 0.5)
+    kw = dict(dgates=dg, counts=r["counts"], tokens=r["tokens"], coef=0.5)
+    want, mag = _gradient(x.to(D).cpu(), r["ids"].cpu().long(), dg.cpu(), r["counts"].cpu(), T, 0.5, 1.0, True)
+    tol = 2 ** -17 * mag + 1e-37 + (2 ** -8 * want.abs() if dtype is torch.bfloat16 else 0)
+    for first, width in ((0, 64), (1, 61), (2, 66), (4, 64), (3, 68), (4, 71), (8, 128)):
+        wide = torch.full((T, width + first), float("nan"), dtype=dtype, device=dev)
+        wide[:, first:first + E] = x
+        view = wide[:, first:first + E]
+        q = ops.moe_route_balance(view, k, 0.5)
+        assert torch.equal(q["ids"], r["ids"]) and torch.equal(q["counts"], r["counts"])
+        assert torch.allclose(q["gates"], r["gates"], rtol=2 ** -17, atol=0)  # 2^-18 each
+        out = torch.full((T, width + first), 7.0, dtype=dtype, device=dev)
+        got = ops.moe_route_backward(view, r["ids"], **kw, out=out[:, first:first + E])
+        assert bool(((got.cpu().to(D) - want).abs() <= tol).all())
+        out[:, first:first + E] = 7
+        assert bool((out == 7).all())
+
+
+def test_training_step(dev):
+    """Router, index build, combine and their gradients together, as the router of a training step runs them, against
+    64-bit automatic differentiation of sum(y G) + loss with the expert rows and the counts as constants."""
+    _say("training step")
+    T, E, k, H, e0, n_local, coef = 50, 24, 4, 64, 8, 12, 0.3
+    logits = _logits(T, E, torch.float32, 6, spread=1.5)
+    G = torch.randn((T, H), generator=torch.Generator().manual_seed(7)) * 0.1
+    for renorm in (True, False):
+        x = logits.to(dev)
+        r = ops.moe_route_balance(x, k, coef, renorm=renorm)
+        t = ops.moe_build_indices_dev(r["ids"], r["gates"], e0, n_local)
+        ye = wl.randn_bf16((t["R_pad"], H), 8).to(dev)
+        y = torch.empty((T, H), device=dev)
+        ops.moe_combine(ye, t["row_weight"], t["owner_offset"], t["slot_to_row"], y)
+        dye, dg = ops.moe_combine_backward(G.to(dev), ye, r["ids"], t["row_weight"], t["owner_offset"], t["slot_to_row"],
+                                           t["rb_rows"], e0, n_local)
+        d = ops.moe_route_backward(x, r["ids"], dgates=dg, counts=r["counts"], tokens=r["tokens"], coef=coef,
+                                   renorm=renorm)
+        # the same on the host
+        z = logits.to(D).requires_grad_()
+        ids = r["ids"].cpu().long()
+        p = torch.softmax(z, 1)
+        g = p.gather(1, ids)
+        if renorm:
+            g = g / g.sum(1, keepdim=True)
+        rows = torch.zeros((T, k, H), dtype=D)
+        at, row = {}, 0
+        for e in range(n_local):
+            mine = (ids == e0 + e).nonzero().tolist()
+            at.update({(tt, j): row + i for i, (tt, j) in enumerate(mine)})
+            row += (len(mine) + 127) // 128 * 128
+        for (tt, j), i in at.items():
+            rows[tt, j] = ye[i].cpu().to(D)
+        rows.requires_grad_()
+        out = (g[..., None] * rows).sum(1)
+        f = torch.bincount(ids.reshape(-1), minlength=E).to(D)
+        loss = coef * E / (k * T * T) * (f * p.sum(0)).sum()
+        ((out * G.to(D)).sum() + loss).backward()
+        # y: gates (2^-18, below 1 in sum), k products and sums. dlogits: 2^-17 of the terms g dg and g sum(g dg), each
+        # at most the largest sum over the columns of |G y|, which also bounds the error of dg itself (64 sums of fp32
+        # in pieces: below 2^-20 of it), and of the balance term, below 1
+        assert torch.allclose(y.cpu().to(D), out.detach(), rtol=0, atol=2 ** -17 * float(rows.detach().abs().max()))
+        most = float((rows.detach().abs() * G.to(D).abs()[:, None]).sum(2).max())
+        assert abs(float(r["loss"]) - float(loss.detach())) <= 2 ** -17 * float(loss.detach())
+        assert torch.allclose(d.cpu().to(D), z.grad, rtol=0, atol=2 ** -17 * (2 * most + 1))
+        got = dye.cpu().to(D)
+        for (tt, j), i in at.items():
+            want = rows.grad[tt, j]
+            # the gate's own rounding, 2^-18, and one of bf16
+            assert bool(((got[i] - want).abs() <= (2 ** -8 + 2 ** -17) * want.abs()).all())
+        rest = torch.ones(t["R_pad"], dtype=torch.bool)
+        rest[list(at.values())] = False
+        assert not got[rest].any()
+
+
 @pytest.mark.parametrize("T", [0, 1])
 def test_no_tokens(dev, T):
     """Nothing to route, or nothing that counts: no choice, sums and loss zero, no division by zero."""

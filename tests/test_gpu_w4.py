@@ -295,6 +295,66 @@ def test_layer_graph_and_streams(dev):
         assert all(torch.equal(i, j) for i, j in zip(u, v))
 
 
+def test_many_blocks(dev):
+    """More row blocks than a workgroup lists, a few rows in each (none in some), and rows at a block's end only."""
+    _say("many blocks")
+    E, K, N, B = 3, 96, 40, 700
+    w = _weights((E, K, N), 32, 1, False, True)
+    p = _pack(dev, w, 32)
+    g = torch.Generator().manual_seed(4)
+    rb_expert = torch.randint(0, E, (B,), generator=g)
+    rb_rows = torch.randint(0, 20, (B,), generator=g)
+    rb_rows[::97] = 128
+    A = _whole((B * 128, K), 5)
+    out = torch.full((B * 128, N), 7.0, dtype=torch.bfloat16, device=dev)
+    ops.moe_grouped_gemm_w4(A.to(dev), p, out, rb_expert.int().to(dev), rb_rows.int().to(dev))
+    got, dense = out.cpu(), _dense(*w, 32)
+    for b in range(B):
+        n = int(rb_rows[b])
+        rows = slice(128 * b, 128 * b + n)
+        assert torch.equal(got[rows], (A[rows].to(D) @ dense[int(rb_expert[b])]).float().to(torch.bfloat16)), b
+        assert bool((got[128 * b + n:128 * b + 128] == 7).all()), b
+    # the same with the row count on the device, below what is listed and above
+    for rows in (128 * 300, 128 * 600):
+        part = torch.full_like(out, 7.0)
+        ops.moe_grouped_gemm_w4(A.to(dev), p, part, rb_expert.int().to(dev), rb_rows.int().to(dev),
+                                sizes=torch.tensor([1, rows], dtype=torch.int64, device=dev))
+        assert torch.equal(part[:rows], out[:rows]) and bool((part[rows:] == 7).all())
+
+
+def test_no_tokens(dev):
+    _say("layer without tokens, product without rows")
+    w1, w2 = _weights((2, 64, 64), 32, 1, False, False), _weights((2, 32, 64), 32, 2, False, False)
+    p1, p2 = _pack(dev, w1, 32), _pack(dev, w2, 32)
+    e = lambda *s, t=torch.int32: torch.zeros(s, dtype=t, device=dev)
+    bf = torch.bfloat16
+    y = ops.moe_ffn_combine_w4(e(0, 64, t=bf), e(128, 3), e(128, t=torch.float32), e(1), e(1), p1, p2, e(128, 64, t=bf),
+                               e(128, 64, t=torch.float32), e(0, 64, t=bf), e(1), e(1))
+    assert y.shape == (0, 64)
+    # no rows routed here: zeros, whatever the scratch holds
+    nan = torch.full((0, 64), float("nan"), device=dev)
+    y = torch.full((3, 64), 5.0, device=dev)
+    ops.moe_ffn_combine_w4(torch.ones((3, 64), dtype=bf, device=dev), e(0, 3), e(0, t=torch.float32), e(4), e(1), p1, p2,
+                           e(0, 64, t=bf), nan, y, e(0), e(0))
+    assert not y.any()
+
+
+def test_weights_as_a_tensor(dev):
+    """Packed weights stored and loaded; only the low four bits of a code count; a wrong size is refused."""
+    _say("packed tensor")
+    w = _weights((200, 50), 64, 3, True, True)
+    p = _pack(dev, w, 64)
+    again = ops.w4_pack((w[0] + 16 * (w[0] % 5)).to(dev), w[1].to(dev), 64, zeros=(w[2] + 32).to(dev))
+    assert torch.equal(p.packed, again.packed)
+    loaded = ops.W4Weights(p.packed.cpu().to(dev), 200, 50, 64, zeros=True)
+    x = _whole((3, 200), 1).to(dev)
+    assert torch.equal(ops.gemm_w4(x, loaded), ops.gemm_w4(x, p))
+    for bad in ((p.packed, 200, 50, 64), (p.packed, 200, 50, 32, 1, True), (p.packed[:-16], 200, 50, 64, 1, True),
+                (p.packed, 200, 50, 48, 1, True), (p.packed.cpu(), 200, 50, 64, 1, True), (p.packed, 0, 50, 64, 1, True)):
+        with pytest.raises(ValueError):
+            ops.W4Weights(*bad)
+
+
 def test_python_refusals(dev):
     _say("refusals")
     codes = torch.zeros((64, 32), dtype=torch.uint8, device=dev)
