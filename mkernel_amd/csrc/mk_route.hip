@@ -30,16 +30,21 @@ constexpr int kFinishExperts = 4;   // experts per workgroup of the second kerne
 // one factor of all of a token's exponentials and cancels in their quotients.
 // What is left is one rounding of the exponent: |x - m| half steps of the
 // result, as much as the rounding of a difference x - m, and 0.3 as much from
-// c.  Where m c overflows (|m| > 2^127), the difference is taken first instead.
+// c.  The factor is 2 to the power of shift's error, up to |m| 2^-23: beyond
+// kFar, where it would reach 2^(1/8) and later pass the range, the difference
+// is taken first (the product then rounds once more).  Which form a token takes
+// depends on its own logits only; the branch is taken where one of a wave does.
 // A row with NaN or +inf gives NaN.
-constexpr float kLog2e = 1.44269502162933349609375f;
+constexpr float kLog2e = 1.44269502162933349609375f, kFar = 0x1p20f;
 struct ExpOf {
   float m, shift;
-  bool far;
-  __device__ __forceinline__ explicit ExpOf(float m_) : m(m_), shift(m_ * kLog2e), far(__any(fabsf(m_) > 0x1p127f)) {}
+  bool far, any;
+  __device__ __forceinline__ explicit ExpOf(float m_)
+      : m(m_), shift(m_ * kLog2e), far(fabsf(m_) > kFar), any(__any(far)) {}
   __device__ __forceinline__ float operator()(float x) const {
-    if (far) return __builtin_amdgcn_exp2f((x - m) * kLog2e);
-    return __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -shift));
+    float e = fmaf(x, kLog2e, -shift);
+    if (any) e = far ? (x - m) * kLog2e : e;
+    return __builtin_amdgcn_exp2f(e);
   }
 };
 

@@ -2,10 +2,10 @@
 combine's gradient, against plain 64-bit forms.
 
 Tolerances (u = 2^-24, half an fp32 step): an exponential of x - max carries
-|x - max| u from the difference's rounding, at most 32 u here (logits within 32
-of the maximum), 4 u of its own; a sum of at most 1024 positive terms, 16 per
-lane and 6 steps across, 22 u; quotient 1 u: below 64 u = 2^-18 for a
-probability and for a gate.  A gradient adds at most as much once more per
+1.3 |x - max| u from the rounding of its exponent and of the constant in it, at
+most 37 u here (logits within 28 of the maximum), 2 u of its own; a sum of at
+most 1024 positive terms, 16 per lane and 6 steps across, 22 u; quotient 1 u:
+below 64 u = 2^-18 for a probability and for a gate.  A gradient adds at most as much once more per
 product and sum, relative to the sum of its terms' magnitudes: 2^-17.  Sums
 over tokens add their own roundings, at most (T / 4096 + 8) u in a lane."""
 import numpy as np
@@ -125,6 +125,42 @@ def test_long_batches(dev, T, E, k, dtype):
     want, mag = _gradient(x.to(D).cpu(), ids[:, :k].cpu(), dg.cpu(), counts.cpu(), T, 0.5, 1.0, True)
     tol = 2 ** -17 * mag + 1e-37 + (2 ** -8 * want.abs() if dtype is torch.bfloat16 else 0)
     assert bool(((d.cpu().to(D) - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_common_offsets(dev, dtype, renorm):
+    """Logits around one far value per token, of both signs up to the type's largest: a softmax does not see it, and a
+    token's results are the same bits whatever its neighbours are."""
+    _say("offsets", dtype, renorm)
+    E, k = 40, 6
+    g = torch.Generator().manual_seed(12)
+    offsets = [0.0, 3.0, -100.0, 1e3, -3e3, 1e5, -9e5, 1.1e6, -1e7, 1e8, 1e9, -1e12, 1e20, -1e30, 3e38, -3e38]
+    x = torch.stack([(torch.randn(E, generator=g).clamp_(-3, 3) + o) for o in offsets]).to(dtype)
+    x[::3, 5:9] = x[::3].amax(1, keepdim=True)
+    x[3::4, 11] = -INF
+    x[5::4, 12] = torch.finfo(dtype).min
+    ids, want, p, counts, n, loss = _reference(x, k, renorm, None, 0.25)
+    r = ops.moe_route_balance(x.to(dev), k, 0.25, renorm=renorm)
+    assert torch.equal(r["ids"].cpu().long(), ids)
+    # as in the docstring above, for |x - max| below 42 and with a second rounding of the exponent where the difference is
+    # taken first: 2.3 x 42 u + 25 u
+    got = r["gates"].cpu().to(D)
+    near = want > 1e-18
+    assert bool(((got - want).abs() <= 2 ** -17 * want)[near].all()) and bool((got[~near] <= 2e-18).all())
+    assert bool(((r["prob_sum"].cpu().to(D) - p.sum(0)).abs() <= 2 ** -17 * p.sum(0) + 1e-16).all())
+    dg = torch.randn((len(offsets), k), generator=g)
+    kw = dict(coef=0.25, counts=r["counts"], tokens=r["tokens"], renorm=renorm)
+    d = ops.moe_route_backward(x.to(dev), r["ids"], dgates=dg.to(dev), **kw)
+    ref, mag = _gradient(x.to(D), ids, dg, counts, n, 0.25, 1.0, renorm)
+    # a gate twice in a product, 122 u each, and 10 u of sums and products; gates below 1e-18 times gradients below 10
+    tol = 2 ** -16 * mag + 1e-16 + (2 ** -8 * ref.abs() if dtype is torch.bfloat16 else 0)
+    assert bool(((d.cpu().to(D) - ref).abs() <= tol).all())
+    for t in range(len(offsets)):
+        i, gate = ops.moe_route(x[t:t + 1].to(dev), k, renorm=renorm)
+        assert torch.equal(i, r["ids"][t:t + 1]) and torch.equal(gate, r["gates"][t:t + 1])
+        one = ops.moe_route_backward(x[t:t + 1].to(dev), i, dgates=dg[t:t + 1].to(dev), **kw)
+        assert torch.equal(one, d[t:t + 1])
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -420,6 +456,58 @@ def test_combine_backward(dev, T, H, E, e0, n_local, k, same, dtype):
     assert bool(((dg.cpu().to(D) - ref).abs() <= (2 * (H / 32 + 8) + 12) * 2 ** -24 * mag).all())
     local = (ids >= e0) & (ids < e0 + n_local)
     assert not dg.cpu()[~local].any()
+
+
+def test_combine_backward_in_place(dev):
+    """dy_expert over y_expert, gates' gradient alone, tables with nonsense behind the routed rows, rows beyond the
+    capacity of the given buffers, and two calls captured and replayed beside eager ones."""
+    _say("combine backward in place")
+    T, H, E, e0, n_local, k = 90, 520, 24, 4, 9, 5
+    ids, gates, dy = _combine_case(dev, T, H, E, e0, n_local, k, torch.float32, 3, False)
+    idd, gd, dyd = ids.to(dev), gates.to(dev), dy.to(dev)
+    t = ops.moe_build_indices_dev(idd, gd, e0, n_local)
+    tables = [t[n] for n in ("row_weight", "owner_offset", "slot_to_row", "rb_rows")]
+    R = t["R_pad"]
+    ye = wl.randn_bf16((R, H), 5).to(dev)
+    a, dg = ops.moe_combine_backward(dyd, ye, idd, *tables, e0, n_local)
+    over = ye.clone()
+    b, dg2 = ops.moe_combine_backward(dyd, over, idd, *tables, e0, n_local, dy_expert=over)
+    assert b.data_ptr() == over.data_ptr() and torch.equal(a, b) and torch.equal(dg, dg2)
+    # a capacity whose tables hold nonsense where no row is
+    c = ops.moe_build_indices_dev(idd, gd, e0, n_local, sync=False)
+    cap = c["pull_indices"].shape[0]
+    c["row_weight"][R:] = NAN
+    c["rb_rows"][R // 128:] = -(1 << 30)
+    c["slot_to_row"][int(c["sizes"][0]):] = 1 << 30
+    wide = torch.full((cap, H), NAN, dtype=torch.bfloat16, device=dev)
+    wide[:R] = ye
+    keep = torch.full((cap, H), 7.0, dtype=torch.bfloat16, device=dev)
+    tables_c = [c[n] for n in ("row_weight", "owner_offset", "slot_to_row", "rb_rows")]
+    kw = dict(dy_expert=keep, sizes=c["sizes"])
+    b, dg2 = ops.moe_combine_backward(dyd, wide, idd, *tables_c, e0, n_local, **kw)
+    assert torch.equal(b[:R], a) and bool((b[R:] == 7).all()) and torch.equal(dg, dg2)
+    # fewer rows than were routed: those behind them have no gradient and are not reached
+    half = R // 256 * 128
+    b, dg2 = ops.moe_combine_backward(dyd, ye[:half], idd, *tables, e0, n_local)
+    assert torch.equal(b, a[:half])
+    rows = torch.full((T, k), -1, dtype=torch.long)
+    row = 0
+    for e in range(n_local):
+        at = (ids == e0 + e).nonzero()
+        rows[at[:, 0], at[:, 1]] = row + torch.arange(at.shape[0])
+        row += (at.shape[0] + 127) // 128 * 128
+    assert torch.equal(dg2, torch.where((rows < half).to(dev), dg, torch.zeros(1, device=dev)))
+    # captured
+    graph, d = torch.cuda.CUDAGraph(), dyd.clone()
+    with torch.cuda.graph(graph):
+        one = ops.moe_combine_backward(d, ye, idd, *tables, e0, n_local)
+        two = ops.moe_combine_backward(d.bfloat16(), ye, idd, *tables, e0, n_local)
+    for rep in range(3):
+        d.copy_(dyd if rep != 1 else 2 * dyd)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = [ops.moe_combine_backward(x, ye, idd, *tables, e0, n_local) for x in (d, d.bfloat16())]
+        assert all(torch.equal(u, v) for i, j in zip((one, two), want) for u, v in zip(i, j)), rep
 
 
 def test_combine_backward_no_rows(dev):
