@@ -538,7 +538,7 @@ int mk_moe_route(const mk_moe_route_args* args, void* stream);
  * (the counts are constants of the loss; counts and n = tokens may be sums over
  * several ranks).  Choices outside [0, num_experts) have no gradient; tokens
  * that do not count get zeros.  dlogits has the logits' type and may be the
- * logits themselves, with the same ld. */
+ * logits themselves, with the same ld, but share no other element with them. */
 typedef struct mk_moe_route_backward_args {
   const void* logits;          /* as in mk_moe_route */
   const uint8_t* token_mask;
@@ -564,7 +564,8 @@ int mk_moe_route_backward(const mk_moe_route_backward_args* args, void* stream);
  * dgates is 0 where topk_ids names no local expert (another rank has that
  * part) or the row was not produced here (slot_to_row -1).  Rows at or past
  * R_pad (sizes[1] when sizes is set, R_pad then being the capacity) are
- * neither read nor written.  dy_expert may be NULL, and rb_rows then too.
+ * neither read nor written.  dy_expert may be NULL, and rb_rows then too; it
+ * may be y_expert itself, whose padding rows are then zeroed as well.
  * Each sum is added in a fixed order.  At most 32 choices.  No counterpart in
  * the reference, which has no backward pass. */
 typedef struct mk_moe_combine_backward_args {
@@ -589,7 +590,7 @@ int mk_moe_combine_backward(const mk_moe_combine_backward_args* args, void* stre
  *   w[k, n] = (code[k, n] - zero[k / group, n]) * scale[k / group, n]
  * codes and zero points 0 .. 15 (8 where there are no zero points), scales
  * bf16, group 32, 64 or 128 rows of K, the last one shorter where K ends in
- * it.  The products read them in an order of their own, laid out once by
+ * it; K and N up to 2^24, 2^40 weights in all.  The products read them in an order of their own, laid out once by
  * mk_w4_pack; E matrices (experts) of one shape lie one after another. */
 typedef struct mk_w4_weights {
   void* packed;      /* mk_w4_packed_bytes bytes, 16-byte aligned: codes, scales and zero points */
@@ -621,9 +622,12 @@ typedef struct mk_w4_quantize_args {
 } mk_w4_quantize_args;
 int mk_w4_quantize(const mk_w4_quantize_args* args, void* stream);
 
-/* C[M, N] = A[M, K] @ w (num_experts 1), fp32 sums, bf16 or fp32 output.  For few rows
- * (it reads the weights once per 64 rows); K % 8 == 0, lda % 8 == 0, any M and
- * N.  An infinity in a row of A makes that row of C NaN. */
+/* C[M, N] = A[M, K] @ w (num_experts 1), fp32 sums, bf16 or fp32 output.  For
+ * few rows (16 at a time, and the weights expanded for each 16); K % 8 == 0,
+ * lda % 8 == 0, any M up to 2^20 and any N.  A group's sum is that of
+ * A * (128 + code) - A * (128 + zero), exact products: its fp32 roundings are
+ * relative to 143 times the group's largest |A|, and an infinity in a row of A,
+ * or a magnitude above 2^120, makes that row of C NaN or infinite. */
 typedef struct mk_gemm_w4_args {
   const void* A;        /* bf16 [M, lda] */
   void* C;              /* [M, ldc] */
@@ -641,8 +645,9 @@ int mk_gemm_w4(const mk_gemm_w4_args* args, void* stream);
  * they are.  out is fp32, bf16, or a bf16 pair: a row holds its values rounded
  * to bf16 and behind them what the rounding left, again in bf16 (17 bits of
  * significand, so that an activation between two products loses nothing that a
- * bf16 result shows); such rows are read with a_parts 2.  gather_pull, n_src_rows, tokens_per_src, devs_per_node and sizes
- * as in mk_moe_grouped_gemm_args. */
+ * bf16 result shows); such rows are read with a_parts 2.  gather_pull,
+ * n_src_rows, tokens_per_src, devs_per_node and sizes as in
+ * mk_moe_grouped_gemm_args. */
 typedef struct mk_moe_grouped_gemm_w4_args {
   const void* A;               /* bf16 [R_pad, K * a_parts], or the token buffer [n_src_rows, K] */
   mk_w4_weights W;

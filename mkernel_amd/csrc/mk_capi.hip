@@ -1085,6 +1085,17 @@ int mk_moe_route(const mk_moe_route_args* a, void* stream) {
   return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_route launch");
 }
 
+// Whether two matrices of T rows of E elements share none, or are one and the same.
+static bool apart_or_same(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t T, int64_t E, int64_t size) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  if (x == y && (lda == ldb || T == 1)) return true;
+  const uintptr_t bytes_a = (uintptr_t)(((T - 1) * lda + E) * size), bytes_b = (uintptr_t)(((T - 1) * ldb + E) * size);
+  if (x + bytes_a <= y || y + bytes_b <= x) return true;
+  // columns of one wider matrix
+  const uintptr_t ld = (uintptr_t)(lda * size), at = (x < y ? y - x : x - y) % (ld ? ld : 1), row = (uintptr_t)(E * size);
+  return T > 1 && lda == ldb && at >= row && at + row <= ld;
+}
+
 int mk_moe_route_backward(const mk_moe_route_backward_args* a, void* stream) {
   if (!a) return fail(MK_EINVAL, "mk_moe_route_backward: null argument");
   if (int rc = check_route("mk_moe_route_backward", a->num_tokens, a->ld, a->num_experts, a->topk, a->logits_dtype))
@@ -1096,6 +1107,8 @@ int mk_moe_route_backward(const mk_moe_route_backward_args* a, void* stream) {
   if (a->num_tokens == 0) return MK_OK;
   if (!a->logits || !a->dlogits || (a->dgates && !a->topk_ids))
     return fail(MK_EINVAL, "mk_moe_route_backward: null argument");
+  if (!apart_or_same(a->logits, a->ld, a->dlogits, a->ld_out, a->num_tokens, a->num_experts, a->logits_dtype ? 2 : 4))
+    return fail(MK_EINVAL, "mk_moe_route_backward: dlogits overlaps the logits");
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   mk::RouteBwdKParams p{a->logits, a->token_mask, a->topk_ids, a->dgates, a->dloss, a->counts, a->tokens, a->dlogits,
@@ -1136,7 +1149,8 @@ int mk_moe_combine_backward(const mk_moe_combine_backward_args* a, void* stream)
 // ---------------------------------------------------------------------------
 
 static bool w4_sizes(int64_t K, int64_t N, int32_t E, int32_t group) {
-  return K > 0 && N > 0 && E > 0 && K <= (1LL << 24) && N <= (1LL << 24) && E <= 65536 &&
+  // (2^40 weights are past any device's memory, and byte counts stay in range)
+  return K > 0 && N > 0 && E > 0 && K <= (1LL << 24) && N <= (1LL << 24) && E <= 65536 && K * N <= (1LL << 40) / E &&
          (group == 32 || group == 64 || group == 128);
 }
 

@@ -468,7 +468,8 @@ def moe_route_backward(logits: torch.Tensor, ids: torch.Tensor, dgates: torch.Te
     counts and tokens (as moe_route_balance gave them, or summed over ranks),
     coef and dloss (one float32 on the device; None: 1).  Either part may be
     left out.  ids, renorm and token_mask as in the forward call.  out: where
-    to write it; the logits themselves may be given."""
+    to write it; the logits themselves may be given, but no other tensor that
+    shares elements with them."""
     if not isinstance(ids, torch.Tensor) or ids.dim() != 2:
         raise ValueError("ids must be an int32 device tensor [T, topk]")
     topk = ids.shape[1]
@@ -625,9 +626,10 @@ def _w4(W, name, device, experts=None) -> None:
 def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> torch.Tensor:
     """C = A @ w for few rows (mk_gemm_w4): A bf16 [M, K], w 4-bit weights of
     w4_pack; fp32 sums of exact products, scaled group by group in fp32; out
-    bf16 (what is made where none is given) or float32.  K a multiple of 8, any M and N; rows of A (a multiple of 8 elements
-    apart) and of out need only be contiguous each.  The weights are read once
-    per 64 rows: from a few hundred rows on, gemm is faster."""
+    bf16 (what is made where none is given) or float32.  K a multiple of 8, any
+    M and N; rows of A (a multiple of 8 elements apart) and of out need only be
+    contiguous each.  The weights are expanded for every 16 rows: from a few
+    hundred rows on, gemm with bf16 weights is faster."""
     if not (isinstance(A, torch.Tensor) and A.dtype is torch.bfloat16 and A.is_cuda and A.dim() == 2
             and A.is_contiguous()):
         _tensor(A, "A", _BF16, rows=True)

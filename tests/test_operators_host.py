@@ -112,6 +112,15 @@ def test_route_backward_refusals(change, code, match):
     _refused("mk_moe_route_backward", _args(capi.MoeRouteBackwardArgs, BACK, change), code, match)
 
 
+@pytest.mark.parametrize("change", [
+    dict(dlogits=P + 4), dict(dlogits=P + 255), dict(ld_out=68), dict(dlogits=P + 256, ld_out=65),
+    dict(ld=128, ld_out=128, dlogits=P + 252), dict(ld=128, ld_out=128, dlogits=P + 260), dict(dlogits=P - 4),
+    dict(dlogits=P + 4 * 255), dict(num_tokens=1, dlogits=P + 4), dict(ld=128, ld_out=128, dlogits=P + 508)])
+def test_route_backward_overlap(change):
+    """An output that shares elements with the logits and is not the logits."""
+    _refused("mk_moe_route_backward", _args(capi.MoeRouteBackwardArgs, BACK, change), EINVAL, "overlaps")
+
+
 COMBINE = dict(dy=P, y_expert=P, topk_ids=P, row_weight=P, owner_offset=P, slot_to_row=P, rb_rows=P, dy_expert=P,
                dgates=P, num_tokens=4, H=64, R_pad=128, topk=2, expert_begin=0, n_local=4)
 
@@ -190,6 +199,9 @@ def test_sizes():
     # whole blocks of 128 rows by two tiles of 16 columns; a byte per zero point
     assert L.mk_w4_packed_bytes(129, 33, 3, 32, 1) == 3 * (256 * 64 // 2 + 8 * 64 * 3)
     assert L.mk_w4_packed_bytes(0, 64, 1, 128, 0) < 0 and L.mk_w4_packed_bytes(64, 64, 1, 16, 0) < 0
+    # more weights than any memory holds: no byte count that wraps round
+    assert L.mk_w4_packed_bytes(1 << 24, 1 << 24, 65536, 128, 0) < 0 and L.mk_w4_packed_bytes(1 << 20, 1 << 20, 2, 32, 1) < 0
+    assert L.mk_w4_packed_bytes(1 << 20, 1 << 20, 1, 128, 0) == (1 << 39) + (1 << 34)
     assert L.mk_moe_route_workspace_bytes(-1, 8) < 0 and L.mk_moe_route_workspace_bytes(1, 1025) < 0
     assert L.mk_moe_route_workspace_bytes(0, 8) > 0
     # bounded however long the batch is
