@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import itertools
 import math
 
 import numpy as np
@@ -248,19 +249,19 @@ def moe_build_indices_dev(topk_ids: torch.Tensor, gates: torch.Tensor, e0: int, 
     # worst case, rounded to whole row blocks so the capacity is a valid
     # row count for the grouped GEMMs
     cap = (T * k + n_local * (row_block - 1) + row_block - 1) // row_block * row_block
-    i32 = dict(dtype=torch.int32, device=dev)
-    L = capi.lib()
-    wsb = int(L.mk_moe_index_workspace_bytes(T, k, n_local))
+    wsb = int(capi.lib().mk_moe_index_workspace_bytes(T, k, n_local))
     # one allocation for the tables and the workspace: 13 took most of the call
     nb = (cap + row_block - 1) // row_block
-    padded, local_rb, pull, row_expert, rb_expert, rb_rows, weight, offset, to_slot, to_owner, to_row, ws = torch.empty(
-        2 * n_local + 2 * nb + 7 * cap + T + 1 + max(cap, 1) + max(wsb, 4) // 4, **i32).split_with_sizes(
-        (n_local, n_local, 3 * cap, cap, nb, nb, cap, T + 1, cap, cap, max(cap, 1), max(wsb, 4) // 4))
+    parts = (4, n_local, n_local, 3 * cap, cap, nb, nb, cap, T + 1, cap, cap, max(cap, 1), max(wsb, 4) // 4)
+    buf = torch.empty(sum(parts), dtype=torch.int32, device=dev)
+    sizes, padded, local_rb, pull, row_expert, rb_expert, rb_rows, weight, offset, to_slot, to_owner, to_row, _ = \
+        buf.split_with_sizes(parts)
     t = dict(zip(_INDEX_TABLES, (padded, local_rb, pull.view(cap, 3), row_expert, rb_expert, rb_rows,
                                  weight.view(torch.float32), offset, to_slot, to_owner, to_row)))
-    sizes = torch.empty(2, dtype=torch.int64, device=dev)  # both words are written by the build
-    capi.call_values("mk_moe_build_indices_dev", MoeIndexDevArgs, _stream(), _ptr(ids), _ptr(g), T, k, e0, n_local,
-                     row_block, cap, _ptr(ws), wsb, _ptr(sizes), *[t[f].data_ptr() for f in _INDEX_TABLES])
+    sizes = sizes.view(torch.int64)  # both words are written by the build
+    at, *tables, ws = itertools.accumulate((4 * n for n in parts[:-1]), initial=buf.data_ptr())
+    capi.call_values("mk_moe_build_indices_dev", MoeIndexDevArgs, _stream(), ids.data_ptr(), g.data_ptr(), T, k, e0,
+                     n_local, row_block, cap, ws, wsb, at, *tables)
     if not sync:
         t["sizes"] = sizes
         return t
@@ -380,6 +381,13 @@ def _is(t, dtype, shape, device) -> bool:
             and t.is_contiguous())
 
 
+def _vector(t, name: str, device) -> None:
+    """An int32 table of any length."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1 and t.device == device
+            and t.is_contiguous()):
+        _tensor(t, name, _I32, dim=1, device=device)
+
+
 def _ld(t: torch.Tensor) -> int:
     """Row stride; of a matrix of one row, its width."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -392,6 +400,9 @@ def _on(device):
 
 _LOGITS = (torch.float32, torch.bfloat16)
 _F32, _BF16, _I32, _U8 = (torch.float32,), (torch.bfloat16,), (torch.int32,), (torch.uint8,)
+
+
+_NO_BALANCE = (0, 0, 0, 0, 0.0, 0, 0)
 
 
 def _route_inputs(logits, topk, token_mask):
@@ -440,22 +451,21 @@ def _route(logits, topk, renorm, token_mask, coef):
     if dev.index != _device_index():
         with torch.cuda.device(dev):
             return _route(logits, topk, renorm, token_mask, coef)
-    ids = torch.empty((T, topk), dtype=torch.int32, device=dev)
-    gates = torch.empty((T, topk), dtype=torch.float32, device=dev)
-    out, balance = (ids, gates), (0, 0, 0, 0, 0.0, 0, 0)
+    ids = torch.empty(T, topk, dtype=torch.int32, device=dev)
+    gates = torch.empty_like(ids, dtype=torch.float32)
+    out, balance = (ids, gates), _NO_BALANCE
     if coef is not None:
-        # loss, prob_sum | counts, tokens | workspace (made anew: it holds nothing between calls)
-        f = torch.empty(1 + E, dtype=torch.float32, device=dev)
-        i = torch.empty(E + 1, dtype=torch.int32, device=dev)
+        # loss, prob_sum, counts and tokens in one tensor; the workspace in another (it holds nothing between calls)
+        sums = torch.empty(2 * E + 2, dtype=torch.int32, device=dev)
         n = capi.lib().mk_moe_route_workspace_bytes(T, E)
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
-        fp, ip = f.data_ptr(), i.data_ptr()
-        balance = (ip, fp + 4, ip + 4 * E, fp, coef, ws.data_ptr(), n)
-        loss, prob_sum = f.split_with_sizes((1, E))
-        counts, tokens = i.split_with_sizes((E, 1))
-        out += (loss, counts, prob_sum, tokens)
-    capi.call_values("mk_moe_route", MoeRouteArgs, _stream(), logits.data_ptr(), _ptr(token_mask), ids.data_ptr(),
-                     gates.data_ptr(), T, _ld(logits), E, topk, logits.dtype is torch.bfloat16, bool(renorm), *balance)
+        at = sums.data_ptr()
+        balance = (at + 4 + 4 * E, at + 4, at + 4 + 8 * E, at, coef, ws.data_ptr(), n)
+        loss, prob_sum, counts, tokens = sums.split_with_sizes((1, E, E, 1))
+        out += (loss.view(torch.float32), counts, prob_sum.view(torch.float32), tokens)
+    capi.call_values("mk_moe_route", MoeRouteArgs, _raw_stream(dev.index), logits.data_ptr(), _ptr(token_mask),
+                     ids.data_ptr(), gates.data_ptr(), T, _ld(logits), E, topk, logits.dtype is torch.bfloat16,
+                     bool(renorm), *balance)
     return out
 
 
@@ -499,8 +509,8 @@ def moe_route_backward(logits: torch.Tensor, ids: torch.Tensor, dgates: torch.Te
         with torch.cuda.device(dev):
             return moe_route_backward(logits, ids, dgates, dloss, counts, tokens, coef, renorm, token_mask, out)
     if out is None:
-        out = torch.empty((T, E), dtype=logits.dtype, device=dev)
-    capi.call_values("mk_moe_route_backward", MoeRouteBackwardArgs, _stream(), logits.data_ptr(), _ptr(token_mask),
+        out = logits.new_empty(T, E)
+    capi.call_values("mk_moe_route_backward", MoeRouteBackwardArgs, _raw_stream(dev.index), logits.data_ptr(), _ptr(token_mask),
                      ids.data_ptr(), _ptr(dgates), _ptr(dloss), _ptr(counts), _ptr(tokens), out.data_ptr(), T,
                      _ld(logits), _ld(out), E, topk, logits.dtype is torch.bfloat16, bool(renorm), _coef(coef))
     return out
@@ -519,32 +529,36 @@ def moe_combine_backward(dy: torch.Tensor, y_expert: torch.Tensor, ids: torch.Te
     _tensor(dy, "dy", _LOGITS, dim=2)
     dev = dy.device
     T, H = dy.shape
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return moe_combine_backward(dy, y_expert, ids, row_weight, owner_offset, slot_to_row, rb_rows, e0, n_local,
+                                        dy_expert, dgates, sizes)
     _tensor(y_expert, "y_expert", _BF16, (None, H), device=dev)
     R_pad = y_expert.shape[0]
     _tensor(ids, "ids", _I32, (T, None), device=dev)
     k = ids.shape[1]
-    _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)
+    if not _is(row_weight, torch.float32, (R_pad,), dev):
+        _tensor(row_weight, "row_weight", _F32, dim=1, device=dev)
     if not _is(owner_offset, torch.int32, (T + 1,), dev):
         _tensor(owner_offset, "owner_offset", _I32, (T + 1,), device=dev)
-    _tensor(slot_to_row, "slot_to_row", _I32, dim=1, device=dev)
-    _tensor(rb_rows, "rb_rows", _I32, dim=1, device=dev)
+    _vector(slot_to_row, "slot_to_row", dev)
+    _vector(rb_rows, "rb_rows", dev)
     if row_weight.shape[0] < R_pad or rb_rows.shape[0] * capi.ROW_BLOCK < R_pad:
         raise ValueError("row_weight and rb_rows must cover the rows of y_expert")
     if sizes is not None and not _is(sizes, torch.int64, (2,), dev):
         _tensor(sizes, "sizes", (torch.int64,), (2,), device=dev)
-    if dy_expert is not None and not _is(dy_expert, torch.bfloat16, (R_pad, H), dev):
+    if dy_expert is None:
+        dy_expert = torch.empty_like(y_expert)
+    elif not _is(dy_expert, torch.bfloat16, (R_pad, H), dev):
         _tensor(dy_expert, "dy_expert", _BF16, (R_pad, H), device=dev)
-    if dgates is not None and not _is(dgates, torch.float32, (T, k), dev):
+    if dgates is None:
+        dgates = torch.empty_like(ids, dtype=torch.float32)
+    elif not _is(dgates, torch.float32, (T, k), dev):
         _tensor(dgates, "dgates", _F32, (T, k), device=dev)
-    with _on(dev):
-        if dy_expert is None:
-            dy_expert = torch.empty((R_pad, H), dtype=torch.bfloat16, device=dev)
-        if dgates is None:
-            dgates = torch.empty((T, k), dtype=torch.float32, device=dev)
-        capi.call_values("mk_moe_combine_backward", MoeCombineBackwardArgs, _stream(), dy.data_ptr(),
-                         y_expert.data_ptr(), ids.data_ptr(), row_weight.data_ptr(), owner_offset.data_ptr(),
-                         slot_to_row.data_ptr(), rb_rows.data_ptr(), dy_expert.data_ptr(), dgates.data_ptr(), T, H,
-                         R_pad, k, e0, n_local, dy.dtype is torch.bfloat16, _ptr(sizes))
+    capi.call_values("mk_moe_combine_backward", MoeCombineBackwardArgs, _raw_stream(dev.index), dy.data_ptr(),
+                     y_expert.data_ptr(), ids.data_ptr(), row_weight.data_ptr(), owner_offset.data_ptr(),
+                     slot_to_row.data_ptr(), rb_rows.data_ptr(), dy_expert.data_ptr(), dgates.data_ptr(), T, H,
+                     R_pad, k, e0, n_local, dy.dtype is torch.bfloat16, _ptr(sizes))
     return dy_expert, dgates
 
 
@@ -644,8 +658,8 @@ def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> t
         with torch.cuda.device(dev):
             return gemm_w4(A, W, out)
     if out is None:
-        out = torch.empty((M, W.N), dtype=torch.bfloat16, device=dev)
-    capi.call_values("mk_gemm_w4", GemmW4Args, _stream(), A.data_ptr(), out.data_ptr(), *W._values(), M, _ld(A),
+        out = A.new_empty(M, W.N)
+    capi.call_values("mk_gemm_w4", GemmW4Args, _raw_stream(dev.index), A.data_ptr(), out.data_ptr(), *W._values(), M, _ld(A),
                      _ld(out), out.dtype is torch.bfloat16)
     return out
 
@@ -711,7 +725,9 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
     (bfloat16 [R_pad, 2 I]: rounded values and what the rounding left) and
     y_expert (float32 [R_pad, H]) are scratch; y_out, bfloat16 or float32, is
     the only rounding; sizes as in moe_ffn_combine."""
-    _tensor(tokens, "tokens", _BF16, dim=2)
+    if not (isinstance(tokens, torch.Tensor) and tokens.dtype is torch.bfloat16 and tokens.is_cuda
+            and tokens.dim() == 2 and tokens.is_contiguous()):
+        _tensor(tokens, "tokens", _BF16, dim=2)
     dev = tokens.device
     _w4(w1, "w1", dev)
     _w4(w2, "w2", dev, w1.experts)
@@ -719,7 +735,8 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
     I = w2.K
     if w1.N != 2 * I or w2.N != H or w1.K != H:
         raise ValueError("w1 must be [E, H, 2I], w2 [E, I, H] and tokens [n, H]")
-    _tensor(pull, "pull", _I32, (None, 3), device=dev)
+    if not (isinstance(pull, torch.Tensor) and _is(pull, torch.int32, (*pull.shape[:1], 3), dev)):
+        _tensor(pull, "pull", _I32, (None, 3), device=dev)
     R_pad = pull.shape[0]
     if not _is(act, torch.bfloat16, (R_pad, 2 * I), dev):
         _tensor(act, "act", _BF16, (R_pad, 2 * I), device=dev)
@@ -735,13 +752,13 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
             raise ValueError("row_weight must cover the rows")
     if not _is(owner_offset, torch.int32, (T + 1,), dev):
         _tensor(owner_offset, "owner_offset", _I32, (T + 1,), device=dev)
-    _tensor(slot_to_row, "slot_to_row", _I32, dim=1, device=dev)
+    _vector(slot_to_row, "slot_to_row", dev)
     _block_tables(rb_expert, rb_rows, R_pad, sizes, dev)
     if dev.index != _device_index():
         with torch.cuda.device(dev):
             return moe_ffn_combine_w4(tokens, pull, row_weight, owner_offset, slot_to_row, w1, w2, act, y_expert,
                                       y_out, rb_expert, rb_rows, tokens_per_src, devs_per_node, sizes)
-    capi.call_values("mk_moe_ffn_combine_w4", MoeFfnW4Args, _stream(), tokens.data_ptr(), pull.data_ptr(),
+    capi.call_values("mk_moe_ffn_combine_w4", MoeFfnW4Args, _raw_stream(dev.index), tokens.data_ptr(), pull.data_ptr(),
                      rb_expert.data_ptr(), _ptr(rb_rows), row_weight.data_ptr(), owner_offset.data_ptr(),
                      slot_to_row.data_ptr(), *w1._values(), *w2._values(), act.data_ptr(), y_expert.data_ptr(),
                      y_out.data_ptr(), T, n, R_pad, n if tokens_per_src is None else tokens_per_src, devs_per_node,
