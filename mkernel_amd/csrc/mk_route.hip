@@ -41,55 +41,110 @@ struct ExpOf {
   bool far, any;
   __device__ __forceinline__ explicit ExpOf(float m_)
       : m(m_), shift(m_ * kLog2e), far(fabsf(m_) > kFar), any(__any(far)) {}
-  __device__ __forceinline__ float operator()(float x) const {
-    float e = fmaf(x, kLog2e, -shift);
-    if (any) e = far ? (x - m) * kLog2e : e;
-    return __builtin_amdgcn_exp2f(e);
+  template <int N>
+  __device__ __forceinline__ void operator()(const float (&x)[N], float (&e)[N]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = fmaf(x[i], kLog2e, -shift);
+    if (__builtin_expect(any, 0)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) e[i] = far ? (x[i] - m) * kLog2e : e[i];
+      asm volatile("");  // keeps this a branch: as selects it is 3 instructions per value
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = __builtin_amdgcn_exp2f(e[i]);
+  }
+};
+
+// A lane's V logits of a row as they lie in memory: a bf16 pair a word, or fp32.
+template <class T, int V>
+struct Raw {
+  static constexpr int kWords = sizeof(T) == 2 ? V / 2 : V;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void values(float (&x)[V]) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        x[2 * i] = bf16_lo(w[i]);
+        x[2 * i + 1] = bf16_hi(w[i]);
+      } else {
+        x[i] = __uint_as_float(w[i]);
+      }
+    }
   }
 };
 
 // Keys: numbers whose order is that of (logit, lowest index): -0 equals +0, NaN
-// above all.  A bf16 logit leaves room for its index in 32 bits.  A float takes
-// 44, as the fraction of a double in [1, 2), so that one v_max_f64 compares
-// both at the rate of a 32-bit one.
+// above all.  A bf16 logit leaves room for its index in 32 bits: 16 bits in
+// two's complement (two logits of a word at a time) above the inverted index.
+// A float takes 44, as the fraction of a double in [1, 2), so that one
+// v_max_f64 compares both at the rate of a 32-bit one.
 template <class T>
 struct Key;
 template <>
 struct Key<uint16_t> {
-  using type = uint32_t;
-  static constexpr type kNone = 0;
-  static __device__ __forceinline__ type make(float x, uint32_t index) {
-    const uint32_t u = __float_as_uint(x + 0.f);
-    const uint32_t o = x != x ? 0xffff0000u : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-    return (o & 0xffff0000u) | (0xffffu - index);
+  using type = int32_t;
+  static constexpr type kNone = INT32_MIN;  // (the least logit is -0x7fff)
+  static constexpr uint32_t kCode = 0xffffu;  // less the index: a key's low bits
+  typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  template <int V>
+  static __device__ __forceinline__ void make(const Raw<uint16_t, V>& raw, const uint32_t (&code)[V], type (&key)[V]) {
+    s16x2 o[V / 2];
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const s16x2 sign = __builtin_bit_cast(s16x2, raw.w[i]) >> 15;
+      o[i] = __builtin_bit_cast(s16x2, raw.w[i] ^ (__builtin_bit_cast(uint32_t, sign) & 0x7fff7fffu)) - sign;
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, raw.w[i] & 0x7fff7fffu));
+    }
+    if (__builtin_expect(__any(most[0] > 0x7f80 || most[1] > 0x7f80), 0)) {  // NaN of either sign: the greatest
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        if ((raw.w[i] & 0x7fffu) > 0x7f80u) o[i][0] = 0x7fff;
+        if ((raw.w[i] >> 16 & 0x7fffu) > 0x7f80u) o[i][1] = 0x7fff;
+      }
+      asm volatile("");  // (stays a branch)
+    }
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const uint32_t w = __builtin_bit_cast(uint32_t, o[i]);
+      key[2 * i] = (int32_t)(w << 16 | code[2 * i]);
+      key[2 * i + 1] = (int32_t)((w & 0xffff0000u) | code[2 * i + 1]);
+    }
   }
-  static __device__ __forceinline__ uint32_t index(type k) { return 0xffffu - (k & 0xffffu); }
+  static __device__ __forceinline__ uint32_t index(type k) { return kCode - ((uint32_t)k & kCode); }
   static __device__ __forceinline__ float value(type k) {
-    const uint32_t o = k & 0xffff0000u;
-    return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o & 0xffff0000u);
+    const int32_t o = k >> 16;
+    return __uint_as_float((uint32_t)(o < 0 ? -o | 0x8000 : o) << 16);
   }
   static __device__ __forceinline__ type top(type a, type b) { return max(a, b); }
   static __device__ __forceinline__ type low(type a, type b) { return min(a, b); }
   template <int CTRL>
   static __device__ __forceinline__ type dpp(type k) {
-    return (uint32_t)__builtin_amdgcn_mov_dpp((int)k, CTRL, 0xf, 0xf, true);
+    return __builtin_amdgcn_mov_dpp(k, CTRL, 0xf, 0xf, true);
   }
-  static __device__ __forceinline__ type shuffle(type k, int mask) { return (uint32_t)__shfl_xor((int)k, mask, 64); }
+  static __device__ __forceinline__ type shuffle(type k, int mask) { return __shfl_xor(k, mask, 64); }
 };
 template <>
 struct Key<float> {
   using type = double;
   static constexpr type kNone = 0.0;
+  static constexpr uint32_t kCode = 0xfffffu;
   static __device__ __forceinline__ type pack(uint32_t hi, uint32_t lo) {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
   }
-  static __device__ __forceinline__ type make(float x, uint32_t index) {
-    const uint32_t u = __float_as_uint(x + 0.f);
-    const uint32_t o = x != x ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-    return pack(0x3ff00000u | o >> 12, o << 20 | (0xfffffu - index));
+  template <int V>
+  static __device__ __forceinline__ void make(const Raw<float, V>& raw, const uint32_t (&code)[V], type (&key)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float x = __uint_as_float(raw.w[j]);
+      const uint32_t u = __float_as_uint(x + 0.f);
+      const uint32_t o = x != x ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+      key[j] = pack(0x3ff00000u | o >> 12, o << 20 | code[j]);
+    }
   }
   static __device__ __forceinline__ uint32_t index(type k) {
-    return 0xfffffu - ((uint32_t)__builtin_bit_cast(uint64_t, k) & 0xfffffu);
+    return kCode - ((uint32_t)__builtin_bit_cast(uint64_t, k) & kCode);
   }
   static __device__ __forceinline__ float value(type k) {
     const uint32_t o = (uint32_t)(__builtin_bit_cast(uint64_t, k) >> 20);
@@ -169,22 +224,47 @@ struct Network {
   }
 };
 
-template <class T, int V, size_t... I>
-__device__ __forceinline__ void exchange(typename Key<T>::type (&a)[V], std::index_sequence<I...>) {
+template <class T, int V, int N, size_t... I>
+__device__ __forceinline__ void exchange(typename Key<T>::type (&a)[N], int at, std::index_sequence<I...>) {
   constexpr Network<V> net;
   auto one = [&](int hi, int lo) {
-    const auto x = a[hi], y = a[lo];
-    a[hi] = Key<T>::top(x, y);
-    a[lo] = Key<T>::low(x, y);
+    const auto x = a[at + hi], y = a[at + lo];
+    a[at + hi] = Key<T>::top(x, y);
+    a[at + lo] = Key<T>::low(x, y);
   };
   (one(net.a[I], net.b[I]), ...);
 }
 
-// Falling order of a lane's V keys.
-template <class T, int V>
+// The D largest of a lane's V keys in falling order, in a[0 .. D): runs of D are
+// sorted, then two runs at a time become one (the larger of each pair of a run
+// and the other one reversed, put in order by halves).  V = 16: 126 minima and
+// maxima for D = 16, 108 for 8, 76 for 4.
+template <class T, int D, int V>
 __device__ __forceinline__ void sort_keys(typename Key<T>::type (&a)[V]) {
-  constexpr Network<V> net;
-  exchange<T, V>(a, std::make_index_sequence<net.n>());
+  using K = Key<T>;
+  constexpr Network<D> net;
+#pragma unroll
+  for (int g = 0; g < V; g += D) exchange<T, D>(a, g, std::make_index_sequence<net.n>());
+#pragma unroll
+  for (int runs = V / D; runs > 1; runs /= 2) {
+#pragma unroll
+    for (int g = 0; g < runs / 2; ++g) {
+      typename K::type c[D];
+#pragma unroll
+      for (int i = 0; i < D; ++i) c[i] = K::top(a[2 * g * D + i], a[2 * g * D + 2 * D - 1 - i]);
+#pragma unroll
+      for (int d = D / 2; d >= 1; d /= 2)
+#pragma unroll
+        for (int i = 0; i < D; ++i)
+          if ((i & d) == 0) {
+            const auto x = c[i], y = c[i + d];
+            c[i] = K::top(x, y);
+            c[i + d] = K::low(x, y);
+          }
+#pragma unroll
+      for (int i = 0; i < D; ++i) a[g * D + i] = c[i];
+    }
+  }
 }
 
 // Where a lane's values lie: V of them in pieces of C neighbours.
@@ -199,29 +279,26 @@ __device__ __forceinline__ float load_one(const T* p) {
   else return *p;
 }
 
-template <class T, int V, int L, int C>
-__device__ __forceinline__ void load_row(float (&x)[V], const T* row, int E, int lane, bool on) {
+template <int V, int L, int C, class T>
+__device__ __forceinline__ void load_row(Raw<T, V>& x, const T* row, int E, int lane, bool on) {
+  constexpr uint32_t kNothing = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
+  constexpr int kEach = sizeof(T) == 2 ? 2 : 1;                              // values of a word
+#pragma unroll
+  for (int i = 0; i < x.kWords; ++i) x.w[i] = kNothing;
 #pragma unroll
   for (int j = 0; j < V; j += C) {
     const int e = expert_of<L, C>(lane, j);
     if (on && e < E) {  // (C > 1: E is a multiple of it)
-      if constexpr (C == 1) {
-        x[j] = load_one(row + e);
-      } else if constexpr (sizeof(T) == 2) {
-        typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-        const u32x2 v = *reinterpret_cast<const u32x2*>(row + e);
-        x[j] = bf16_lo(v[0]);
-        x[j + 1] = bf16_hi(v[0]);
-        x[j + 2] = bf16_lo(v[1]);
-        x[j + 3] = bf16_hi(v[1]);
+      if constexpr (C == 1 && sizeof(T) == 2) {
+        x.w[j / 2] = j % 2 ? (x.w[j / 2] & 0xffffu) | (uint32_t)row[e] << 16 : (x.w[j / 2] & 0xffff0000u) | row[e];
+      } else if constexpr (C == 1) {
+        x.w[j] = __float_as_uint(row[e]);
       } else {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(row + e);
+        typedef uint32_t words __attribute__((ext_vector_type(C / kEach)));
+        const words v = *reinterpret_cast<const words*>(row + e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[j + i] = v[i];
+        for (int i = 0; i < C / kEach; ++i) x.w[j / kEach + i] = v[i];
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) x[j + i] = -INFINITY;
     }
   }
 }
@@ -251,25 +328,29 @@ __global__ __launch_bounds__(64 * kWavesSum) void route_kernel(RouteKParams p) {
   const int64_t stride = (int64_t)gridDim.x * waves * R;
   int64_t t = ((int64_t)blockIdx.x * waves + wave) * R + sub;
   auto present = [&](int64_t u) { return u < p.T && (!p.mask || p.mask[u]); };
-  float next[V];
-  load_row<T, V, L, C>(next, static_cast<const T*>(p.logits) + t * p.ld, p.E, lane, present(t));
+  // (in registers of their own: worked out anew they are one more instruction per key)
+  uint32_t code[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    code[j] = K::kCode - expert_of<L, C>(lane, j);
+    asm volatile("" : "+v"(code[j]));
+  }
+  Raw<T, V> next;
+  load_row<V, L, C>(next, static_cast<const T*>(p.logits) + t * p.ld, p.E, lane, present(t));
   for (; t - sub < p.T; t += stride) {
     float x[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = next[j];
+    next.values(x);
+    KeyT key[V], kept[S];
+    K::make(next, code, key);
     // the next token's logits are on their way while this one's are ranked
     if (t - sub + stride < p.T)
-      load_row<T, V, L, C>(next, static_cast<const T*>(p.logits) + (t + stride) * p.ld, p.E, lane, present(t + stride));
-    KeyT key[V];
+      load_row<V, L, C>(next, static_cast<const T*>(p.logits) + (t + stride) * p.ld, p.E, lane, present(t + stride));
+    sort_keys<T, D>(key);
 #pragma unroll
-    for (int j = 0; j < V; ++j) key[j] = K::make(x[j], expert_of<L, C>(lane, j));
-    sort_keys<T, V>(key);
-    int id[S];
-    float top[S], m = -INFINITY;
-#pragma unroll
-    for (int s = 0; s < S; ++s) id[s] = -1, top[s] = -INFINITY;
-    for (int r = 0; r < p.k; ++r) {
-      const KeyT best = row_top<L, T>(key[0]);
+    for (int s = 0; s < S; ++s) kept[s] = K::kNone;
+    KeyT best = row_top<L, T>(key[0]);
+    const float m = K::value(best);
+    for (int r = 0;;) {
       const bool won = key[0] == best;
 #pragma unroll
       for (int i = 0; i < D; ++i) {
@@ -277,30 +358,34 @@ __global__ __launch_bounds__(64 * kWavesSum) void route_kernel(RouteKParams p) {
         const KeyT here = key[i], then = i + 1 < D ? +key[i + 1 < D ? i + 1 : i] : K::kNone;
         key[i] = won ? then : here;
       }
-      const float v = K::value(best);
-      if (r == 0) m = best == K::kNone ? -INFINITY : v;
 #pragma unroll
-      for (int s = 0; s < S; ++s)
-        if (lane + s * L == r && best != K::kNone && v != -INFINITY) {
-          id[s] = (int)K::index(best);
-          top[s] = v;
-        }
+      for (int s = 0; s < S; ++s) kept[s] = lane + s * L == r ? best : +kept[s];
+      if (++r == p.k) break;
+      best = row_top<L, T>(key[0]);
+    }
+    int id[S];
+    float top[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const float v = K::value(kept[s]);
+      const bool chosen = kept[s] != K::kNone && v != -INFINITY;
+      id[s] = chosen ? (int)K::index(kept[s]) : -1;
+      top[s] = chosen ? v : -INFINITY;
     }
     const bool alive = m != -INFINITY;
     const ExpOf exp_of(alive ? m : 0.f);
     float e[V], z = 1.f;
     if (balance || !p.renorm) {
       z = 0.f;
+      exp_of(x, e);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        e[j] = exp_of(x[j]);
-        z += e[j];
-      }
+      for (int j = 0; j < V; ++j) z += e[j];
       z = row_sum<L>(z);
     }
     float g[S], zg = z;
+    exp_of(top, g);  // (-inf where there is no choice: 0, but NaN beside a NaN or +inf)
 #pragma unroll
-    for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? exp_of(top[s]) : 0.f;
+    for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? g[s] : 0.f;
     if (p.renorm) {
       zg = 0.f;
 #pragma unroll
@@ -347,14 +432,13 @@ __global__ __launch_bounds__(64 * kWavesSum) void route_kernel(RouteKParams p) {
 // the last workgroup to finish adds the experts' shares of the loss.
 __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int nparts) {
   constexpr int kSlices = 256 / kFinishExperts, kAhead = 16;
-  __shared__ double sums[kSlices][kFinishExperts];
-  __shared__ int cnts[kSlices][kFinishExperts];
-  __shared__ int last, total;
+  __shared__ double sums[4][kFinishExperts];
+  __shared__ int cnts[4][kFinishExperts], lives[4];
+  __shared__ int last;
   const int x = threadIdx.x % kFinishExperts, slice = threadIdx.x / kFinishExperts;
   const int e = blockIdx.x * kFinishExperts + x;
   double s = 0.0;
   int c = 0, n = 0;
-  if (threadIdx.x == 0) total = 0;
   for (int b0 = slice; b0 < nparts; b0 += kAhead * kSlices) {
     float ps[kAhead];
     int pc[kAhead];
@@ -372,12 +456,22 @@ __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int n
     }
   }
   for (int b = threadIdx.x; b < nparts; b += 256) n += p.part_live[b];
-  sums[slice][x] = s;
-  cnts[slice][x] = c;
+#pragma unroll
+  for (int d = kFinishExperts; d < 64; d *= 2) {
+    s += __shfl_xor(s, d, 64);
+    c += __shfl_xor(c, d, 64);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d, 64);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) < kFinishExperts) {
+    sums[wave][x] = s;
+    cnts[wave][x] = c;
+    if (x == 0) lives[wave] = n;
+  }
   __syncthreads();
-  atomicAdd(&total, n);
   if (slice == 0) {
-    for (int i = 1; i < kSlices; ++i) {
+    for (int i = 1; i < 4; ++i) {
       s += sums[i][x];
       c += cnts[i][x];
     }
@@ -385,12 +479,14 @@ __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int n
       p.prob_sum[e] = (float)s;
       p.counts[e] = c;
     }
-    sums[0][x] = e < p.E ? s * c : 0.0;
+    double share = e < p.E ? s * c : 0.0;
+#pragma unroll
+    for (int d = 1; d < kFinishExperts; d *= 2) share += __shfl_xor(share, d, 64);
+    sums[0][x] = share;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    double share = 0.0;
-    for (int i = 0; i < kFinishExperts; ++i) share += sums[0][i];
+    const double share = sums[0][0];
     // written through to agent scope and waited for: a plain ticket orders it
     __hip_atomic_store(p.shares + blockIdx.x, share, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     wait_vmem_all();
@@ -404,6 +500,7 @@ __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int n
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
   if (threadIdx.x != 0) return;
+  const int total = lives[0] + lives[1] + lives[2] + lives[3];
   *p.tokens = total;
   *p.loss = total ? (float)((double)p.coef * p.E * sum / ((double)p.k * total * total)) : 0.f;
 }
@@ -420,13 +517,14 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
   auto present = [&](int64_t u) { return u < p.T && (!p.mask || p.mask[u]); };
   // a token's logits, choices and their gates' gradients
   struct Token {
-    float x[V], dg[S];
+    Raw<T, V> x;
+    float dg[S];
     int id[S];
     bool on;
   } next;
   auto fetch = [&](int64_t u) {
     next.on = present(u);
-    load_row<T, V, L, C>(next.x, static_cast<const T*>(p.logits) + u * p.ld, p.E, lane, next.on);
+    load_row<V, L, C>(next.x, static_cast<const T*>(p.logits) + u * p.ld, p.E, lane, next.on);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const int i = lane + s * L;
@@ -452,8 +550,7 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
     const T* row = static_cast<const T*>(p.logits) + t * p.ld;
     float x[V], dg[S], xc[S];
     int id[S];
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = next.x[j];
+    next.x.values(x);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       id[s] = next.id[s] < p.E ? next.id[s] : -1;
@@ -475,9 +572,9 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
     const bool alive = m != -INFINITY || odd;  // else the token does not count, or no expert is left for it
     const ExpOf exp_of(alive ? m : 0.f);
     float pr[V], z = 0.f, s0 = 0.f;
+    exp_of(x, pr);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      pr[j] = exp_of(x[j]);
       z += pr[j];
       s0 += pr[j] * f[j];
     }
@@ -493,17 +590,19 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
         for (int s = 1; s < S; ++s) mc = fmaxf(mc, xc[s]);
         mc = row_max<L>(mc);
         const ExpOf exp_c(mc != -INFINITY ? mc : 0.f);
+        exp_c(xc, g);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-          g[s] = xc[s] != -INFINITY ? exp_c(xc[s]) : 0.f;
+          g[s] = xc[s] != -INFINITY ? g[s] : 0.f;
           sum += g[s];
         }
         sum = row_sum<L>(sum);
         sum = sum > 0.f ? 1.f / sum : 0.f;
       } else {
         sum = inv;
+        exp_of(xc, g);
 #pragma unroll
-        for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? exp_of(xc[s]) : 0.f;
+        for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? g[s] : 0.f;
       }
 #pragma unroll
       for (int s = 0; s < S; ++s) {
@@ -575,13 +674,14 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
   }
 }
 
-// Lanes and values per lane for E experts, pieces of C, and at most 8 or
+// Lanes and values per lane for E experts, pieces of C, and at most 4, 8 or
 // kMaxTopk choices.
 template <class F>
 void by_shape(int E, bool vector, int k, F&& f) {
   using std::integral_constant;
   auto choices = [&](auto v, auto l, auto c) {
-    if (k <= 8) f(v, l, c, integral_constant<int, 8>());
+    if (k <= 4) f(v, l, c, integral_constant<int, 4>());
+    else if (k <= 8) f(v, l, c, integral_constant<int, 8>());
     else f(v, l, c, integral_constant<int, kMaxTopk>());
   };
   auto pieces = [&](auto v, auto l) {
