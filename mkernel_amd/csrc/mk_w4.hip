@@ -68,9 +68,15 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) 
 // nothing, so one load (XQ = 1) brings the four MFMAs' parts at once, lane
 // 4 j + r of 16 the part of row r for MFMA j, and a rotation by 4 j lanes moves
 // them in place (the other lanes then hold parts of other MFMAs, which end in
-// rows that are not stored).  The loads of x, mostly empty, were the largest
-// cost of a decode step beside the weights: 12 of 67 us.
-template <int NT, int SUB, bool ZEROS, int XQ>
+// rows that are not stored).
+//
+// FLIP: odd rows load the step's parts 1, 0, 3, 2 instead of 0, 1, 2, 3, and are
+// put in order by 16 selects.  Rows lie a multiple of 128 bytes apart as a rule,
+// and 64 bytes of each in one load come from the same half of a cache line: its
+// banks are read one row after another (64 x 8192 x 8192 25 us, flipped 21, and
+// 20 as it is where rows are 16 bytes off).  The experts' kernel is slower with
+// it where few rows come (64 tokens, GEMM1: 60 us, flipped 65).
+template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP>
 struct Step {
   u32x4 w[NT];
   static constexpr int PAIRS = NT == 4 ? 2 : NT;  // four tiles are two pairs; else each tile reads its pair's
@@ -103,8 +109,8 @@ struct Source {
   int32_t most;      // last multiple of 8 below K, less this lane's first k in a step
 };
 
-template <int NT, int SUB, bool ZEROS, int XQ>
-__device__ __forceinline__ void load(Step<NT, SUB, ZEROS, XQ>& st, const Source<NT>& t, uint32_t kb, int lane) {
+template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP>
+__device__ __forceinline__ void load(Step<NT, SUB, ZEROS, XQ, FLIP>& st, const Source<NT>& t, uint32_t kb, int lane) {
   constexpr int G = 4 / SUB;
   const uint32_t at = kb * block_bytes(G, ZEROS), sat = at + (lane & 15) * (4 * G), zat = at + (lane & 15) * (2 * G);
 #pragma unroll
@@ -138,19 +144,37 @@ __device__ __forceinline__ void load(Step<NT, SUB, ZEROS, XQ>& st, const Source<
   }
 #pragma unroll
   for (int j = 0; j < XQ; ++j) {
-    const bool in = (int32_t)(kb * kBlock) + j * 32 <= t.most;
-    st.x[j] = load16(t.x, in ? t.row + kb * 256 + 64 * j : kNowhere);
+    const int part = FLIP ? j + (j % 2 ? -(lane & 1) : lane & 1) : j;
+    const bool in = (int32_t)(kb * kBlock) + part * 32 <= t.most;
+    st.x[j] = load16(t.x, in ? t.row + kb * 256 + 64 * part : kNowhere);
   }
 }
 
-template <int NT, int SUB, bool ZEROS, int XQ>
-__device__ __forceinline__ void multiply(const Step<NT, SUB, ZEROS, XQ>& st, const int (&odd)[NT], uint32_t mask,
+template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP>
+__device__ __forceinline__ void multiply(const Step<NT, SUB, ZEROS, XQ, FLIP>& st, const int (&odd)[NT], uint32_t mask,
                                          uint32_t bias, f32x4 (&acc)[NT]) {
-  const bf16x8 x[4] = {
-      __builtin_bit_cast(bf16x8, st.x[0]),
-      __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<1>(st.x[0]) : st.x[1 % XQ]),
-      __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<2>(st.x[0]) : st.x[2 % XQ]),
-      __builtin_bit_cast(bf16x8, XQ == 1 ? from_quarter<3>(st.x[0]) : st.x[3 % XQ])};
+  bf16x8 x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(bf16x8, st.x[j % XQ]);
+  if constexpr (XQ == 1) {
+    x[1] = __builtin_bit_cast(bf16x8, from_quarter<1>(st.x[0]));
+    x[2] = __builtin_bit_cast(bf16x8, from_quarter<2>(st.x[0]));
+    x[3] = __builtin_bit_cast(bf16x8, from_quarter<3>(st.x[0]));
+  } else if constexpr (FLIP) {
+    const bool flipped = threadIdx.x & 1;
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      u32x4 a, b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u = st.x[j][i], v = st.x[j + 1][i];
+        a[i] = flipped ? v : u;
+        b[i] = flipped ? u : v;
+      }
+      x[j] = __builtin_bit_cast(bf16x8, a);
+      x[j + 1] = __builtin_bit_cast(bf16x8, b);
+    }
+  }
 #pragma unroll
   for (int g = 0; g < 4 / SUB; ++g) {
     f32x4 base = {0.f, 0.f, 0.f, 0.f};  // sum of -136 x: the same for every column where there are no zero points
@@ -185,13 +209,13 @@ __device__ __forceinline__ void multiply(const Step<NT, SUB, ZEROS, XQ>& st, con
 // for its own only.  The last P steps load nothing more (a load that nobody
 // needs would still be waited for before its registers are used again); those
 // past the end found zeros.
-template <int NT, int SUB, bool ZEROS, int XQ, int P>
+template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP, int P>
 __device__ __forceinline__ void sweep(const Source<NT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
                                       f32x4 (&acc)[NT]) {
   uint32_t mask = 0x000f000fu, bias = 0x43004300u;
   asm volatile("" : "+s"(mask));
   asm volatile("" : "+v"(bias));
-  Step<NT, SUB, ZEROS, XQ> st[P];
+  Step<NT, SUB, ZEROS, XQ, FLIP> st[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     load(st[i], t, first + i * stride, lane);
@@ -349,7 +373,13 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
   // (a dense launch knows its items on the host)
   const int split = EXPERTS ? __builtin_amdgcn_readfirstlane(choose_split(items, gridDim.x * W, KB, W)) : p.split;
   const int log = __builtin_ctz(split), per = W >> log, ks = wave & (split - 1);
-  for (uint32_t it0 = blockIdx.x * per; it0 < items; it0 += gridDim.x * per) {
+  // Dense passes of one column item read the same weights: neighbouring ids lie
+  // on one XCD (64 x 3584 x 8192 14.9 us, as launched 15.5).  Experts' seldom
+  // have several, and are faster with neighbours on all XCDs (16 tokens, GEMM1:
+  // 19 us and 32, 64 tokens 60 and 65).
+  const uint32_t xcd = blockIdx.x & 7, G = gridDim.x;
+  const uint32_t id = EXPERTS ? blockIdx.x : xcd * (G >> 3) + min(xcd, G & 7) + (blockIdx.x >> 3);
+  for (uint32_t it0 = id * per; it0 < items; it0 += G * per) {
     const uint32_t it = it0 + (wave >> log);
     int64_t row0 = 0, expert = 0;
     int ci = 0, left = 0;
@@ -415,7 +445,7 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
         t.x = make_rsrc(p.A + row0 * p.lda, (uint32_t)(left * p.lda * 2));
         if (r < left) t.row = (uint32_t)(r * p.lda * 2) + in_row;
       }
-      sweep<NT, SUB, ZEROS, XQ, kAhead>(t, KB, ks, split, lane, acc);
+      sweep<NT, SUB, ZEROS, XQ, XQ == 4 && !EXPERTS, kAhead>(t, KB, ks, split, lane, acc);
       if constexpr (PARTS == 2) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
