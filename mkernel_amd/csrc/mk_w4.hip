@@ -603,7 +603,7 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
     if (!p.rb_expert) {
       if constexpr (NT == 1)
         if (p.M <= 4) return launch(w4_kernel<1, SUB, Z, 1, false, true, false>, 1, false);
-      if constexpr (NT != 2) launch(w4_kernel<NT, SUB, Z, 1, false, false, true>, NT, false);
+      launch(w4_kernel<NT, SUB, Z, 1, false, false, true>, NT, false);
     } else if constexpr (NT != 1) {
       if (p.parts == 2) launch(w4_kernel<NT, SUB, Z, 2, true, true, true>, NT, true);
       else launch(w4_kernel<NT, SUB, Z, 1, true, true, true>, NT, true);
@@ -619,15 +619,19 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
     else with_zeros(nt, integral_constant<int, 4>());
   };
   // Column tiles of an item.  Experts: four, or two (one gate, one up) where
-  // SwiGLU's tiles are no whole pairs.  Dense: with more than 4 rows, x is read
-  // once per item and four tiles pay from kWideItems row tiles x column tiles on
-  // (16 x 8192 x 8192 19.9 us with one, 13.6 with four; 16 x 7168 x 4096 11.1
-  // and 12.0); up to 4 rows one tile, and more waves, always (1 x 8192 x 8192
-  // 8.6 us, with four 11.2).
-  constexpr int64_t kWideItems = 384;
-  if (p.rb_expert ? p.swiglu && p.tile_cols % 2 : false) with_group(integral_constant<int, 2>());
-  else if (p.rb_expert || (p.M > 4 && (p.M + 15) / 16 * p.tile_cols >= kWideItems)) with_group(integral_constant<int, 4>());
-  else with_group(integral_constant<int, 1>());
+  // SwiGLU's tiles are no whole pairs.  Dense up to 4 rows: one tile, and more
+  // waves (1 x 8192 x 8192 8.6 us, with four tiles 11.2).  Dense with more rows:
+  // x is read once per item, so as many tiles as leave an item for every CU.  Row
+  // tiles x column tiles, and us with 1, 2, 4 tiles an item: 256 (32 x 3584 x
+  // 2048) 5.9, 6.3, 8.0; 320 (16 x 4096 x 5120) 7.9, 6.2, 8.1; 512 (64 x 7168 x
+  // 2048) 13.9, 9.3, 11.6; 640 (16 x 4096 x 10240) 12.3, 9.4, 8.6; 1024 (128 x
+  // 2048 x 2048) 7.7, 6.4, 6.0.
+  const int64_t tiles = (p.M + 15) / 16 * p.tile_cols;
+  const int wide = p.rb_expert ? (p.swiglu && p.tile_cols % 2 ? 2 : 4)
+                   : p.M <= 4 || tiles <= cus ? 1 : tiles <= 2 * (int64_t)cus ? 2 : 4;
+  if (wide == 1) with_group(integral_constant<int, 1>());
+  else if (wide == 2) with_group(integral_constant<int, 2>());
+  else with_group(integral_constant<int, 4>());
   return hipGetLastError();
 }
 
