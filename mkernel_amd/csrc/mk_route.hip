@@ -38,22 +38,35 @@ constexpr int kFinishExperts = 4;   // experts per workgroup of the second kerne
 constexpr float kLog2e = 1.44269502162933349609375f, kFar = 0x1p20f;
 struct ExpOf {
   float m, shift;
-  bool far, any;
-  __device__ __forceinline__ explicit ExpOf(float m_)
-      : m(m_), shift(m_ * kLog2e), far(fabsf(m_) > kFar), any(__any(far)) {}
+  bool far;
+  __device__ __forceinline__ explicit ExpOf(float m_) : m(m_), shift(m_ * kLog2e), far(fabsf(m_) > kFar) {}
   template <int N>
-  __device__ __forceinline__ void operator()(const float (&x)[N], float (&e)[N]) const {
+  __device__ __forceinline__ void near_form(const float (&x)[N], float (&e)[N]) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) e[i] = fmaf(x[i], kLog2e, -shift);
-    if (__builtin_expect(any, 0)) {
+  }
+  template <int N>
+  __device__ __forceinline__ void far_form(const float (&x)[N], float (&e)[N]) const {
 #pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = far ? (x[i] - m) * kLog2e : e[i];
-      asm volatile("");  // keeps this a branch: as selects it is 3 instructions per value
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) e[i] = __builtin_amdgcn_exp2f(e[i]);
+    for (int i = 0; i < N; ++i) e[i] = far ? (x[i] - m) * kLog2e : e[i];
   }
 };
+// e = exp_a(x), g = exp_b(y), with one branch for both.
+template <int N, int M>
+__device__ __forceinline__ void exps(const ExpOf& a, const float (&x)[N], float (&e)[N], const ExpOf& b,
+                                     const float (&y)[M], float (&g)[M]) {
+  a.near_form(x, e);
+  b.near_form(y, g);
+  if (__builtin_expect(__any(a.far || b.far), 0)) {
+    a.far_form(x, e);
+    b.far_form(y, g);
+    asm volatile("");  // keeps this a branch: as selects it is 3 instructions per value
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) e[i] = __builtin_amdgcn_exp2f(e[i]);
+#pragma unroll
+  for (int i = 0; i < M; ++i) g[i] = __builtin_amdgcn_exp2f(g[i]);
+}
 
 // A lane's V logits of a row as they lie in memory: a bf16 pair a word, or fp32.
 template <class T, int V>
@@ -374,16 +387,19 @@ __global__ __launch_bounds__(64 * kWavesSum) void route_kernel(RouteKParams p) {
     }
     const bool alive = m != -INFINITY;
     const ExpOf exp_of(alive ? m : 0.f);
-    float e[V], z = 1.f;
+    // (top is -inf where there is no choice: 0, but NaN beside a NaN or +inf)
+    float e[V], z = 1.f, g[S];
     if (balance || !p.renorm) {
+      exps(exp_of, x, e, exp_of, top, g);
       z = 0.f;
-      exp_of(x, e);
 #pragma unroll
       for (int j = 0; j < V; ++j) z += e[j];
       z = row_sum<L>(z);
+    } else {
+      float none[1] = {0.f}, unused[1];
+      exps(exp_of, none, unused, exp_of, top, g);
     }
-    float g[S], zg = z;
-    exp_of(top, g);  // (-inf where there is no choice: 0, but NaN beside a NaN or +inf)
+    float zg = z;
 #pragma unroll
     for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? g[s] : 0.f;
     if (p.renorm) {
@@ -570,9 +586,14 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
     m = row_max<L>(m);
     odd = row_max<L>(odd ? 1.f : 0.f) != 0.f || m == INFINITY;  // a NaN or +inf: the whole row is NaN
     const bool alive = m != -INFINITY || odd;  // else the token does not count, or no expert is left for it
-    const ExpOf exp_of(alive ? m : 0.f);
-    float pr[V], z = 0.f, s0 = 0.f;
-    exp_of(x, pr);
+    // the gates: softmax over the choices, or over all
+    float mc = xc[0];
+#pragma unroll
+    for (int s = 1; s < S; ++s) mc = fmaxf(mc, xc[s]);
+    mc = row_max<L>(mc);
+    if (!p.renorm) mc = m;
+    float pr[V], g[S], z = 0.f, s0 = 0.f;
+    exps(ExpOf(alive ? m : 0.f), x, pr, ExpOf(mc != -INFINITY ? mc : 0.f), xc, g);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       z += pr[j];
@@ -583,26 +604,17 @@ __global__ __launch_bounds__(kThreadsR) void route_backward_kernel(RouteBwdKPara
     s0 = row_sum<L>(s0) * inv;
     float v[S], dense = 0.f;
     if (p.dgates) {
-      float g[S], sum = 0.f, dot = 0.f;
+      float sum = 0.f, dot = 0.f;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        g[s] = id[s] >= 0 && xc[s] != -INFINITY ? g[s] : 0.f;
+        sum += g[s];
+      }
       if (p.renorm) {
-        float mc = xc[0];
-#pragma unroll
-        for (int s = 1; s < S; ++s) mc = fmaxf(mc, xc[s]);
-        mc = row_max<L>(mc);
-        const ExpOf exp_c(mc != -INFINITY ? mc : 0.f);
-        exp_c(xc, g);
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          g[s] = xc[s] != -INFINITY ? g[s] : 0.f;
-          sum += g[s];
-        }
         sum = row_sum<L>(sum);
         sum = sum > 0.f ? 1.f / sum : 0.f;
       } else {
         sum = inv;
-        exp_of(xc, g);
-#pragma unroll
-        for (int s = 0; s < S; ++s) g[s] = id[s] >= 0 ? g[s] : 0.f;
       }
 #pragma unroll
       for (int s = 0; s < S; ++s) {
