@@ -463,9 +463,9 @@ def _route(logits, topk, renorm, token_mask, coef):
         balance = (at + 4 + 4 * E, at + 4, at + 4 + 8 * E, at, coef, ws.data_ptr(), n)
         loss, prob_sum, counts, tokens = sums.split_with_sizes((1, E, E, 1))
         out += (loss.view(torch.float32), counts, prob_sum.view(torch.float32), tokens)
-    capi.call_values("mk_moe_route", MoeRouteArgs, _raw_stream(dev.index), logits.data_ptr(), _ptr(token_mask),
-                     ids.data_ptr(), gates.data_ptr(), T, _ld(logits), E, topk, logits.dtype is torch.bfloat16,
-                     bool(renorm), *balance)
+    capi.call_values("mk_moe_route", MoeRouteArgs, _raw_stream(dev.index), logits.data_ptr(),
+                     0 if token_mask is None else token_mask.data_ptr(), ids.data_ptr(), gates.data_ptr(), T,
+                     logits.stride(0) if T > 1 else E, E, topk, logits.dtype is torch.bfloat16, bool(renorm), *balance)
     return out
 
 
@@ -545,6 +545,8 @@ def moe_combine_backward(dy: torch.Tensor, y_expert: torch.Tensor, ids: torch.Te
     _vector(rb_rows, "rb_rows", dev)
     if row_weight.shape[0] < R_pad or rb_rows.shape[0] * capi.ROW_BLOCK < R_pad:
         raise ValueError("row_weight and rb_rows must cover the rows of y_expert")
+    if not (0 <= e0 < 2**31 and 0 < n_local < 2**31):
+        raise ValueError("experts e0 .. e0 + n_local must be numbers of 32 bits")
     if sizes is not None and not _is(sizes, torch.int64, (2,), dev):
         _tensor(sizes, "sizes", (torch.int64,), (2,), device=dev)
     if dy_expert is None:
@@ -648,19 +650,24 @@ def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> t
             and A.is_contiguous()):
         _tensor(A, "A", _BF16, rows=True)
     dev = A.device
-    _w4(W, "W", dev, 1)
+    if type(W) is not W4Weights or W.experts != 1 or W.packed.device != dev:
+        _w4(W, "W", dev, 1)
     M, K = A.shape
+    N = W.N
     if K != W.K:
         raise ValueError(f"A has {K} columns, the weights {W.K} rows")
     if out is not None:
-        _tensor(out, "out", _LOGITS, (M, W.N), rows=True, device=dev)
-    if dev.index != _device_index():
+        _tensor(out, "out", _LOGITS, (M, N), rows=True, device=dev)
+    index = dev.index
+    if index != _device_index():
         with torch.cuda.device(dev):
             return gemm_w4(A, W, out)
     if out is None:
-        out = A.new_empty(M, W.N)
-    capi.call_values("mk_gemm_w4", GemmW4Args, _raw_stream(dev.index), A.data_ptr(), out.data_ptr(), *W._values(), M, _ld(A),
-                     _ld(out), out.dtype is torch.bfloat16)
+        out, ldc, bf16 = A.new_empty(M, N), N, True
+    else:
+        ldc, bf16 = _ld(out), out.dtype is torch.bfloat16
+    capi.call_values("mk_gemm_w4", GemmW4Args, _raw_stream(index), A.data_ptr(), out.data_ptr(), *W._values(), M,
+                     A.stride(0) if M > 1 else K, ldc, bf16)
     return out
 
 
