@@ -7,8 +7,16 @@
 // bits of the logit, lowest index) as one number, so ids do not depend on how a
 // sum is ordered, and ties go to the lowest index.
 // The balance loss needs sums over all tokens: every workgroup writes its
-// tokens' sums to the workspace and a second kernel adds them in workgroup
-// order, so results do not depend on timing either.
+// tokens' sums to the workspace and a second kernel adds them in a fixed order,
+// so results do not depend on timing either.
+//
+// What bounds it: a small batch the chain of launch, loads, ranking and stores
+// (1 x 256, 8 choices 3.1 us; 4096 x 256 fp32 with sums 8 and 6 us, gradient 8),
+// a large one the vector instructions: 131001 x 60 bf16, 4 choices, with sums,
+// 13.8 us, 477 of them per 16 tokens, which keep the units busy for four fifths
+// of a wave's life (its 20 MB are 4 us); the sums over workgroups 7.2 us, the
+// gradient 14.3 (447 instructions, and two dependent loads before them).  16384
+// x 256 bf16, 8 choices, without sums: 6.6 us.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -444,8 +452,11 @@ __global__ __launch_bounds__(64 * kWavesSum) void route_kernel(RouteKParams p) {
   if (threadIdx.x == 0) p.part_live[blockIdx.x] = live_s;
 }
 
-// Sums the workgroups' parts in order, kFinishExperts experts per workgroup;
-// the last workgroup to finish adds the experts' shares of the loss.
+// Sums the workgroups' parts, kFinishExperts experts per workgroup, in an order
+// that the launch's size alone decides; the last workgroup to finish adds the
+// experts' shares of the loss.  All latency: two loads' worth of memory, the
+// store and ticket, and the shares (131001 x 60, 512 parts 7.2 us, one workgroup
+// for everything 15; the sums in LDS one after another 9.5).
 __global__ __launch_bounds__(256) void route_finish_kernel(RouteKParams p, int nparts) {
   constexpr int kSlices = 256 / kFinishExperts, kAhead = 16;
   __shared__ double sums[4][kFinishExperts];

@@ -19,6 +19,13 @@
 // x is the first operand, so a lane of the result holds one column of four rows
 // of x, and needs that column's scale only.  The waves of a workgroup share a
 // column tile and split K; their sums meet in LDS in wave order.
+//
+// What bounds it: for few rows the weights' bytes.  1 x 8192 x 3584: 5.7 us for
+// 15 MB, 3 of them launch and first loads; 64 tokens on 18 experts of 7168 x
+// 4096 (273 MB, not in a cache): 62 us, 4.4 TB/s, where a kernel that only reads
+// them takes 46.  With more rows a step's instructions beside (128 x 64 weights
+// against 16 rows: 170 vector instructions, most of them the expansion, and 20
+// MFMAs): 64 x 3584 x 8192 in 13 us is 290 TFLOP/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -75,7 +82,8 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) 
 // and 64 bytes of each in one load come from the same half of a cache line: its
 // banks are read one row after another (64 x 8192 x 8192 25 us, flipped 21, and
 // 20 as it is where rows are 16 bytes off).  The experts' kernel is slower with
-// it where few rows come (64 tokens, GEMM1: 60 us, flipped 65).
+// it where few rows come (64 tokens, GEMM1 / GEMM2: 62 / 37 us, flipped 65 / 39)
+// and no faster where many do (256 tokens: 142 / 93 and 143 / 92).
 template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP>
 struct Step {
   u32x4 w[NT];
@@ -374,9 +382,9 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
   const int split = EXPERTS ? __builtin_amdgcn_readfirstlane(choose_split(items, gridDim.x * W, KB, W)) : p.split;
   const int log = __builtin_ctz(split), per = W >> log, ks = wave & (split - 1);
   // Dense passes of one column item read the same weights: neighbouring ids lie
-  // on one XCD (64 x 3584 x 8192 14.9 us, as launched 15.5).  Experts' seldom
+  // on one XCD (64 x 3584 x 8192 13.6 us, as launched 15.1).  Experts' seldom
   // have several, and are faster with neighbours on all XCDs (16 tokens, GEMM1:
-  // 19 us and 32, 64 tokens 60 and 65).
+  // 21 us and 33, 64 tokens 62 and 66).
   const uint32_t xcd = blockIdx.x & 7, G = gridDim.x;
   const uint32_t id = EXPERTS ? blockIdx.x : xcd * (G >> 3) + min(xcd, G & 7) + (blockIdx.x >> 3);
   for (uint32_t it0 = id * per; it0 < items; it0 += G * per) {
