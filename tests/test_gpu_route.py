@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from mkernel_amd import ops, workloads as wl
+from mkernel_amd import capi, ops, workloads as wl
 
 pytestmark = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
@@ -508,6 +508,58 @@ def test_combine_backward_in_place(dev):
         torch.cuda.synchronize()
         want = [ops.moe_combine_backward(x, ye, idd, *tables, e0, n_local) for x in (d, d.bfloat16())]
         assert all(torch.equal(u, v) for i, j in zip((one, two), want) for u, v in zip(i, j)), rep
+
+
+def test_gates_gradient_alone(dev):
+    """The C entry without dy_expert and rb_rows: the same gates' gradient."""
+    _say("combine backward, gates alone")
+    T, H, E, e0, n_local, k = 33, 264, 10, 2, 5, 3
+    ids, gates, dy = _combine_case(dev, T, H, E, e0, n_local, k, torch.bfloat16, 9, False)
+    idd, dyd = ids.to(dev), dy.to(dev)
+    t = ops.moe_build_indices_dev(idd, gates.to(dev), e0, n_local)
+    ye = wl.randn_bf16((t["R_pad"], H), 5).to(dev)
+    _, dg = ops.moe_combine_backward(dyd, ye, idd, t["row_weight"], t["owner_offset"], t["slot_to_row"], t["rb_rows"], e0,
+                                     n_local)
+    alone = torch.full((T, k), 7.0, device=dev)
+    capi.call_values("mk_moe_combine_backward", capi.MoeCombineBackwardArgs, ops._stream(), dyd.data_ptr(), ye.data_ptr(),
+                     idd.data_ptr(), t["row_weight"].data_ptr(), t["owner_offset"].data_ptr(),
+                     t["slot_to_row"].data_ptr(), 0, 0, alone.data_ptr(), T, H, t["R_pad"], k, e0, n_local, 1, 0)
+    assert torch.equal(alone, dg)
+
+
+def test_past_32_bits(dev):
+    """Logits and expert rows more than 2^31 elements into their buffers."""
+    _say("offsets past 32 bits")
+    T, E, k, ld = 60000, 40, 4, 40000
+    assert (T - 1) * ld > 2**31
+    wide = torch.empty((T, ld), dtype=torch.bfloat16, device=dev)
+    x = _logits(T, E, torch.bfloat16, 3).to(dev)
+    wide[:, 8:8 + E] = x
+    view = wide[:, 8:8 + E]
+    a, b = ops.moe_route_balance(view, k, 0.5), ops.moe_route_balance(x, k, 0.5)
+    assert all(torch.equal(a[f], b[f]) for f in a)
+    kw = dict(dgates=torch.randn((T, k), device=dev), counts=a["counts"], tokens=a["tokens"], coef=0.5)
+    want = ops.moe_route_backward(x, b["ids"], **kw)
+    ops.moe_route_backward(view, a["ids"], **kw, out=view)
+    assert torch.equal(view, want)
+    del wide, view
+    # one token per expert: a padded row block each
+    n, H = 2400, 7168
+    assert n * 128 * H > 2**31
+    ids = torch.randperm(n, generator=torch.Generator().manual_seed(1)).int().view(n, 1).to(dev)
+    gates = torch.rand((n, 1), device=dev) + 0.5
+    t = ops.moe_build_indices_dev(ids, gates, 0, n)
+    assert t["R_pad"] == n * 128
+    ye = torch.zeros((n * 128, H), dtype=torch.bfloat16, device=dev)
+    rows = ids[:, 0].long() * 128
+    ye[rows] = wl.randn_bf16((n, H), 2).to(dev)
+    dy = wl.randn_bf16((n, H), 3).to(dev)
+    dye, dg = ops.moe_combine_backward(dy, ye, ids, t["row_weight"], t["owner_offset"], t["slot_to_row"], t["rb_rows"], 0, n)
+    assert torch.equal(dye[rows], (gates * dy.float()).to(torch.bfloat16))
+    ref = (dy.to(D) * ye[rows].to(D))
+    assert bool(((dg[:, 0].to(D) - ref.sum(1)).abs() <= (2 * (H / 32 + 8) + 12) * 2 ** -24 * ref.abs().sum(1)).all())
+    dye[rows] = 0
+    assert not dye.any()
 
 
 def test_combine_backward_no_rows(dev):

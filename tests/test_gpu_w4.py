@@ -323,6 +323,36 @@ def test_many_blocks(dev):
         assert torch.equal(part[:rows], out[:rows]) and bool((part[rows:] == 7).all())
 
 
+def test_past_32_bits(dev):
+    """Packed weights of more than 4 GiB: the last experts' are the same as packed alone.  Rows of x and of the result
+    more than 2^31 elements into their buffers."""
+    _say("offsets past 32 bits")
+    E, K, N, group = 36, 16384, 16384, 128
+    g = torch.Generator(device=dev).manual_seed(5)
+    codes = torch.randint(0, 16, (E, K, N), generator=g, dtype=torch.uint8, device=dev)
+    scales = 2.0 ** torch.randint(-3, 1, (E, K // group, N), generator=g, device=dev).to(torch.bfloat16)
+    p = ops.w4_pack(codes, scales, group)
+    assert p.packed.numel() > 2**32
+    x = _whole((256, K), 6).to(dev)
+    rb_expert, rb_rows = torch.tensor([E - 1, 1], dtype=torch.int32, device=dev), torch.tensor([3, 2], dtype=torch.int32, device=dev)
+    out = torch.zeros((256, N), device=dev)
+    ops.moe_grouped_gemm_w4(x, p, out, rb_expert, rb_rows)
+    for e, rows in ((E - 1, slice(0, 3)), (1, slice(128, 130))):
+        one = ops.w4_pack(codes[e], scales[e], group)
+        assert torch.equal(out[rows], ops.gemm_w4(x[rows], one, out=torch.empty((rows.stop - rows.start, N), device=dev)))
+    del codes, p
+    # strided rows
+    M, K, N, ld = 70, 256, 96, 1 << 24
+    w = _pack(dev, _weights((K, N), 64, 1, False, True), 64)
+    wide = torch.empty((M, ld), dtype=torch.bfloat16, device=dev)
+    assert (M - 1) * ld < 2**31 < 2 * (M - 1) * ld
+    wide[:, :K] = _whole((M, K), 2).to(dev)
+    assert torch.equal(ops.gemm_w4(wide[:, :K], w), ops.gemm_w4(wide[:, :K].contiguous(), w))
+    far = torch.empty((M, 1 << 25), dtype=torch.bfloat16, device=dev)
+    assert (M - 1) * (1 << 25) > 2**31
+    assert torch.equal(ops.gemm_w4(wide[:, :K], w, out=far[:, :N]), ops.gemm_w4(wide[:, :K].contiguous(), w))
+
+
 def test_no_tokens(dev):
     _say("layer without tokens, product without rows")
     w1, w2 = _weights((2, 64, 64), 32, 1, False, False), _weights((2, 32, 64), 32, 2, False, False)
