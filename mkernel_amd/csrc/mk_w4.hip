@@ -24,8 +24,9 @@
 // 15 MB, 3 of them launch and first loads; 64 tokens on 18 experts of 7168 x
 // 4096 (273 MB, not in a cache): 62 us, 4.4 TB/s, where a kernel that only reads
 // them takes 46.  With more rows a step's instructions beside (128 x 64 weights
-// against 16 rows: 170 vector instructions, most of them the expansion, and 20
-// MFMAs): 64 x 3584 x 8192 in 13 us is 290 TFLOP/s.
+// against 16 rows: 170 vector instructions, two thirds of them the expansion, and
+// 20 MFMAs; against 32 rows 250 and 40): 64 x 3584 x 8192 in 11.2 us is 335
+// TFLOP/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -80,17 +81,17 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) 
 // FLIP: odd rows load the step's parts 1, 0, 3, 2 instead of 0, 1, 2, 3, and are
 // put in order by 16 selects.  Rows lie a multiple of 128 bytes apart as a rule,
 // and 64 bytes of each in one load come from the same half of a cache line: its
-// banks are read one row after another (64 x 8192 x 8192 25 us, flipped 21, and
-// 20 as it is where rows are 16 bytes off).  The experts' kernel is slower with
+// banks are read one row after another (64 x 8192 x 8192 with one row tile 25 us,
+// flipped 21, and 20 as it is where rows are 16 bytes off).  The experts' kernel is slower with
 // it where few rows come (64 tokens, GEMM1 / GEMM2: 62 / 37 us, flipped 65 / 39)
 // and no faster where many do (256 tokens: 142 / 93 and 143 / 92).
-template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP>
+template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP, int MT>
 struct Step {
   u32x4 w[NT];
   static constexpr int PAIRS = NT == 4 ? 2 : NT;  // four tiles are two pairs; else each tile reads its pair's
   uint32_t s[PAIRS][4 / SUB];
   uint32_t z[ZEROS ? PAIRS : 1][SUB == 1 ? 2 : 1];
-  u32x4 x[XQ];
+  u32x4 x[MT][XQ];
 };
 
 // Lane i of each 16 gets lane i + 4 J.
@@ -109,16 +110,16 @@ __device__ __forceinline__ u32x4 from_quarter(u32x4 v) {
 constexpr uint32_t block_bytes(int groups, bool zeros) { return 2048u + 64u * groups + (zeros ? 32u * groups : 0u); }
 
 // A wave's pairs of column tiles (the run of blocks of each) and its rows of x.
-template <int NT>
+template <int NT, int MT>
 struct Source {
   __amdgpu_buffer_rsrc_t w[NT == 4 ? 2 : NT], x;
   int odd[NT];       // which of its pair a tile is
-  uint32_t row;      // byte offset of this lane's row, kNowhere where there is none
+  uint32_t row[MT];  // byte offset of this lane's row, kNowhere where there is none
   int32_t most;      // last multiple of 8 below K, less this lane's first k in a step
 };
 
-template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP>
-__device__ __forceinline__ void load(Step<NT, SUB, ZEROS, XQ, FLIP>& st, const Source<NT>& t, uint32_t kb, int lane) {
+template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP, int MT>
+__device__ __forceinline__ void load(Step<NT, SUB, ZEROS, XQ, FLIP, MT>& st, const Source<NT, MT>& t, uint32_t kb, int lane) {
   constexpr int G = 4 / SUB;
   const uint32_t at = kb * block_bytes(G, ZEROS), sat = at + (lane & 15) * (4 * G), zat = at + (lane & 15) * (2 * G);
 #pragma unroll
@@ -154,42 +155,51 @@ __device__ __forceinline__ void load(Step<NT, SUB, ZEROS, XQ, FLIP>& st, const S
   for (int j = 0; j < XQ; ++j) {
     const int part = FLIP ? j + (j % 2 ? -(lane & 1) : lane & 1) : j;
     const bool in = (int32_t)(kb * kBlock) + part * 32 <= t.most;
-    st.x[j] = load16(t.x, in ? t.row + kb * 256 + 64 * part : kNowhere);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) st.x[m][j] = load16(t.x, in ? t.row[m] + kb * 256 + 64 * part : kNowhere);
   }
 }
 
-template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP>
-__device__ __forceinline__ void multiply(const Step<NT, SUB, ZEROS, XQ, FLIP>& st, const int (&odd)[NT], uint32_t mask,
-                                         uint32_t bias, f32x4 (&acc)[NT]) {
-  bf16x8 x[4];
+template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP, int MT>
+__device__ __forceinline__ void multiply(const Step<NT, SUB, ZEROS, XQ, FLIP, MT>& st, const int (&odd)[NT], uint32_t mask,
+                                         uint32_t bias, f32x4 (&acc)[MT][NT]) {
+  bf16x8 x[MT][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(bf16x8, st.x[j % XQ]);
-  if constexpr (XQ == 1) {
-    x[1] = __builtin_bit_cast(bf16x8, from_quarter<1>(st.x[0]));
-    x[2] = __builtin_bit_cast(bf16x8, from_quarter<2>(st.x[0]));
-    x[3] = __builtin_bit_cast(bf16x8, from_quarter<3>(st.x[0]));
-  } else if constexpr (FLIP) {
-    const bool flipped = threadIdx.x & 1;
+  for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      u32x4 a, b;
+    for (int j = 0; j < 4; ++j) x[m][j] = __builtin_bit_cast(bf16x8, st.x[m][j % XQ]);
+    if constexpr (XQ == 1) {
+      x[m][1] = __builtin_bit_cast(bf16x8, from_quarter<1>(st.x[m][0]));
+      x[m][2] = __builtin_bit_cast(bf16x8, from_quarter<2>(st.x[m][0]));
+      x[m][3] = __builtin_bit_cast(bf16x8, from_quarter<3>(st.x[m][0]));
+    } else if constexpr (FLIP) {
+      const bool flipped = threadIdx.x & 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t u = st.x[j][i], v = st.x[j + 1][i];
-        a[i] = flipped ? v : u;
-        b[i] = flipped ? u : v;
+      for (int j = 0; j < 4; j += 2) {
+        u32x4 a, b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u = st.x[m][j][i], v = st.x[m][j + 1][i];
+          a[i] = flipped ? v : u;
+          b[i] = flipped ? u : v;
+        }
+        x[m][j] = __builtin_bit_cast(bf16x8, a);
+        x[m][j + 1] = __builtin_bit_cast(bf16x8, b);
       }
-      x[j] = __builtin_bit_cast(bf16x8, a);
-      x[j + 1] = __builtin_bit_cast(bf16x8, b);
     }
   }
 #pragma unroll
   for (int g = 0; g < 4 / SUB; ++g) {
-    f32x4 base = {0.f, 0.f, 0.f, 0.f};  // sum of -136 x: the same for every column where there are no zero points
-    if constexpr (!ZEROS) {
-      const bf16x8 off = minus_offset(8u);
+    f32x4 base[MT];  // sum of -136 x: the same for every column where there are no zero points
 #pragma unroll
-      for (int i = 0; i < SUB; ++i) base = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[g * SUB + i], off, base, 0, 0, 0);
+    for (int m = 0; m < MT; ++m) {
+      base[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (!ZEROS) {
+        const bf16x8 off = minus_offset(8u);
+#pragma unroll
+        for (int i = 0; i < SUB; ++i)
+          base[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[m][g * SUB + i], off, base[m], 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -199,14 +209,22 @@ __device__ __forceinline__ void multiply(const Step<NT, SUB, ZEROS, XQ, FLIP>& s
       const float s = __uint_as_float(NT == 4 ? (n % 2 ? sw & 0xffff0000u : sw << 16) : sw >> (16 * odd[n]) << 16);
       bf16x8 off;
       if constexpr (ZEROS) off = minus_offset(st.z[pair][g / 2] >> (16 * (g % 2) + 8 * (NT == 4 ? n % 2 : odd[n])) & 255u);
-      f32x4 part = base;
+      f32x4 part[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) part[m] = base[m];
 #pragma unroll
       for (int i = 0; i < SUB; ++i) {
-        if constexpr (ZEROS) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[g * SUB + i], off, part, 0, 0, 0);
-        part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[g * SUB + i], expand(st.w[n][g * SUB + i], mask, bias), part, 0, 0, 0);
+        const bf16x8 q = expand(st.w[n][g * SUB + i], mask, bias);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if constexpr (ZEROS) part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[m][g * SUB + i], off, part[m], 0, 0, 0);
+          part[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[m][g * SUB + i], q, part[m], 0, 0, 0);
+        }
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[n][r] = fmaf(s, part[r], acc[n][r]);
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(s, part[m][r], acc[m][n][r]);
     }
   }
 }
@@ -217,13 +235,13 @@ __device__ __forceinline__ void multiply(const Step<NT, SUB, ZEROS, XQ, FLIP>& s
 // for its own only.  The last P steps load nothing more (a load that nobody
 // needs would still be waited for before its registers are used again); those
 // past the end found zeros.
-template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP, int P>
-__device__ __forceinline__ void sweep(const Source<NT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
-                                      f32x4 (&acc)[NT]) {
+template <int NT, int SUB, bool ZEROS, int XQ, bool FLIP, int P, int MT>
+__device__ __forceinline__ void sweep(const Source<NT, MT>& t, uint32_t KB, uint32_t first, uint32_t stride, int lane,
+                                      f32x4 (&acc)[MT][NT]) {
   uint32_t mask = 0x000f000fu, bias = 0x43004300u;
   asm volatile("" : "+s"(mask));
   asm volatile("" : "+v"(bias));
-  Step<NT, SUB, ZEROS, XQ, FLIP> st[P];
+  Step<NT, SUB, ZEROS, XQ, FLIP, MT> st[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     load(st[i], t, first + i * stride, lane);
@@ -306,29 +324,33 @@ __device__ __forceinline__ int block_rows(const W4KParams& p, int64_t b) {
   return p.rb_rows ? max(0, min(p.rb_rows[b], kFlagRows)) : kFlagRows;
 }
 
-// Waves of a workgroup, and those that a CU holds (by registers): the grid of a launch.
-constexpr int group_waves(int nt) { return nt == 1 ? 8 : 4; }
-constexpr int waves_per_cu(int nt) { return nt == 1 ? 16 : 12; }
+// Waves of a workgroup, and those that a CU holds (by registers): the grid of a
+// launch.  Items of two row tiles with 12 waves spill (64 x 3584 x 8192 12.9 us,
+// with 8 11.2).
+constexpr int group_waves(int nt, int mt) { return nt == 1 || mt == 2 ? 8 : 4; }
+constexpr int waves_per_cu(int nt, int mt) { return nt == 1 ? 16 : mt == 2 ? 8 : 12; }
 
 // Steps in flight per wave.  More than about 96 KB on their way into a CU is
 // slower, not faster (64 tokens on 32 experts, GEMM1 / GEMM2: 12 waves of 2
 // steps of 4 KB 59 / 36 us, 12 of 4 steps 72 / 45, 16 of 2 steps 69 / 42, 8 of
-// 2 steps 63 / 41; 1 x 8192 x 3584: 2 steps 5.9 us, 6 steps 7.5).
-constexpr int kAhead = 2;
+// 2 steps 63 / 41; 1 x 8192 x 3584: 2 steps 5.9 us, 6 steps 7.5).  With two row
+// tiles a step is 12 KB and one is enough (64 x 3584 x 8192 11.3 us, two 12.5;
+// 64 x 8192 x 8192 19.4 and 19.1).
+constexpr int kAhead = 2, kAheadWide = 1;
 
 // An item is NT column tiles (with SwiGLU: the first half gate tiles, the second
-// the matching up tiles) of a pass of up to 16 rows; `split` waves of a
-// workgroup share its K.  Where x goes as bf16 pairs (PARTS 2) the halves of a
-// row take two lanes of the row tile, and their two sums are added at the end.
-// The workgroups of the grid walk the items in turn, as many as the device's row
-// count and tables say there are; the passes of one column item lie side by
-// side, since they read the same weights.  (32-row passes, two row tiles per
-// step, are slower: 32 x 8192 x 8192 22.3 us instead of 15.3.)  FEW, MANY:
-// whether passes of at most 4 row lanes, and of more, come (see Step).
-template <int NT, int SUB, bool ZEROS, int PARTS, bool EXPERTS, bool FEW, bool MANY>
-__global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4_kernel(W4KParams p) {
+// the matching up tiles) of a pass of up to 16 MT rows; `split` waves of a
+// workgroup share its K.  MT = 2 expands a code once for two row tiles.  Where x
+// goes as bf16 pairs (PARTS 2) the halves of a row take two lanes of the row
+// tile, and their two sums are added at the end.  The workgroups of the grid walk
+// the items in turn, as many as the device's row count and tables say there are;
+// the passes of one column item lie side by side, since they read the same
+// weights.  FEW, MANY: whether passes of at most 4 row lanes, and of more, come
+// (see Step).
+template <int NT, int SUB, bool ZEROS, int PARTS, bool EXPERTS, bool FEW, bool MANY, int MT>
+__global__ __launch_bounds__(64 * group_waves(NT, MT), waves_per_cu(NT, MT) / 4) void w4_kernel(W4KParams p) {
   extern __shared__ f32x4 red[];  // [W][NT][64], used where K is split
-  constexpr int W = group_waves(NT), ROWS = 16 / PARTS, kPasses = kFlagRows / ROWS;
+  constexpr int W = group_waves(NT, MT), ROWS = 16 * MT / PARTS, kPasses = kFlagRows / ROWS;
   __shared__ PassList<EXPERTS ? ROWS : kFlagRows> list;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -382,7 +404,7 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
   const int split = EXPERTS ? __builtin_amdgcn_readfirstlane(choose_split(items, gridDim.x * W, KB, W)) : p.split;
   const int log = __builtin_ctz(split), per = W >> log, ks = wave & (split - 1);
   // Dense passes of one column item read the same weights: neighbouring ids lie
-  // on one XCD (64 x 3584 x 8192 13.6 us, as launched 15.1).  Experts' seldom
+  // on one XCD (64 x 3584 x 8192 with one row tile 13.6 us, as launched 15.1).  Experts' seldom
   // have several, and are faster with neighbours on all XCDs (16 tokens, GEMM1:
   // 21 us and 33, 64 tokens 62 and 66).
   const uint32_t xcd = blockIdx.x & 7, G = gridDim.x;
@@ -419,12 +441,12 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
     }
     const bool any = left > 0, few = FEW && left <= 4 / PARTS;
     const int lanes = few ? 4 : 16;  // of a row tile
-    f32x4 acc[NT];
+    f32x4 acc[MT][NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < MT * NT; ++n) acc[n / NT][n % NT] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto run = [&](auto xq) {
       constexpr int XQ = decltype(xq)::value;
-      Source<NT> t;
+      Source<NT, MT> t;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const bool up = p.swiglu && n >= NT / 2;
@@ -441,28 +463,31 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
       const int r = col % EACH, half = col % LANES / EACH, k0 = (XQ == 1 ? col / 4 * 32 : 0) + quad * 8;
       t.most = (int32_t)p.w.K - 8 - k0;
       const uint32_t in_row = 2 * (uint32_t)(k0 + half * p.w.K);
-      t.row = kNowhere;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) t.row[m] = kNowhere;
       if (EXPERTS && p.gather_pull) {
         t.x = make_rsrc(p.A, (uint32_t)(p.gather_rows * p.lda * 2));
         if (r < left) {
           const int* pr = p.gather_pull + 3 * (row0 + r);
           const int64_t src = ((int64_t)pr[0] * p.gather_devs + pr[1]) * p.gather_tps + pr[2];
-          if (pr[0] >= 0 && pr[2] >= 0 && src >= 0 && src < p.gather_rows) t.row = (uint32_t)(src * p.lda * 2) + in_row;
+          if (pr[0] >= 0 && pr[2] >= 0 && src >= 0 && src < p.gather_rows) t.row[0] = (uint32_t)(src * p.lda * 2) + in_row;
         }
       } else {
         t.x = make_rsrc(p.A + row0 * p.lda, (uint32_t)(left * p.lda * 2));
-        if (r < left) t.row = (uint32_t)(r * p.lda * 2) + in_row;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if (r + 16 * m < left) t.row[m] = (uint32_t)((r + 16 * m) * p.lda * 2) + in_row;
       }
-      sweep<NT, SUB, ZEROS, XQ, XQ == 4 && !EXPERTS, kAhead>(t, KB, ks, split, lane, acc);
+      sweep<NT, SUB, ZEROS, XQ, XQ == 4 && !EXPERTS, MT == 2 ? kAheadWide : kAhead, MT>(t, KB, ks, split, lane, acc);
       if constexpr (PARTS == 2) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if constexpr (XQ == 1) {  // rows 0 and 1, then their second halves
-            acc[n][0] += acc[n][2];
-            acc[n][1] += acc[n][3];
+            acc[0][n][0] += acc[0][n][2];
+            acc[0][n][1] += acc[0][n][3];
           } else {  // second halves: rows 8 to 15, two quads on
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][i] += __shfl_xor(acc[n][i], 32, 64);
+            for (int i = 0; i < 4; ++i) acc[0][n][i] += __shfl_xor(acc[0][n][i], 32, 64);
           }
         }
       }
@@ -474,7 +499,7 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
         if constexpr (MANY) run(std::integral_constant<int, 4>());
       }
     }
-    auto finish = [&](int n, f32x4 v, f32x4 up) {
+    auto finish = [&](int m, int n, f32x4 v, f32x4 up) {
       const int64_t c = (int64_t)(ci * per_item + n) * kTile + col;
       if (c >= width) return;
       if constexpr (NT >= 2)
@@ -483,27 +508,38 @@ __global__ __launch_bounds__(64 * group_waves(NT), waves_per_cu(NT) / 4) void w4
           for (int i = 0; i < 4; ++i) v[i] = silu(v[i]) * up[i];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (4 * quad + i < min(left, lanes / PARTS)) store(p, row0 + 4 * quad + i, c, width, v[i]);
+        if (MT == 1 ? 4 * quad + i < min(left, lanes / PARTS) : 16 * m + 4 * quad + i < left)
+          store(p, row0 + 16 * m + 4 * quad + i, c, width, v[i]);
     };
     if (split == 1) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (n < per_item) finish(n, acc[n], acc[NT >= 2 ? (n + NT / 2) % NT : n]);
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          if (n < per_item) finish(m, n, acc[m][n], acc[m][NT >= 2 ? (n + NT / 2) % NT : n]);
       continue;
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) red[(wave * NT + n) * 64 + lane] = acc[n];
+    for (int n = 0; n < MT * NT; ++n) red[(wave * MT * NT + n) * 64 + lane] = acc[n / NT][n % NT];
     __syncthreads();
     auto total = [&](int n) {
-      f32x4 v = red[((wave - ks) * NT + n) * 64 + lane];
-      for (int o = 1; o < split; ++o) v += red[((wave - ks + o) * NT + n) * 64 + lane];
+      f32x4 v = red[((wave - ks) * MT * NT + n) * 64 + lane];
+      for (int o = 1; o < split; ++o) v += red[((wave - ks + o) * MT * NT + n) * 64 + lane];
       return v;
     };
-    if (any)
-      for (int n = ks; n < per_item; n += split) {
-        const f32x4 v = total(n);
-        finish(n, v, p.swiglu ? total(n + NT / 2) : v);
+    if (any) {
+      if constexpr (MT == 1) {
+        for (int n = ks; n < per_item; n += split) {
+          const f32x4 v = total(n);
+          finish(0, n, v, p.swiglu ? total(n + NT / 2) : v);
+        }
+      } else {  // (dense: no SwiGLU)
+        for (int n = ks; n < MT * NT; n += split) {
+          const f32x4 v = total(n);
+          finish(n / NT, n % NT, v, v);
+        }
       }
+    }
     __syncthreads();
   }
 }
@@ -593,28 +629,31 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
   if (args.M == 0) return hipSuccess;
   W4KParams p = args;
   using std::integral_constant;
-  auto launch = [&](auto kernel, int nt, bool experts) {
-    const int w = group_waves(nt), rows = 16 / p.parts, per_item = p.swiglu ? nt / 2 : nt;
+  auto launch = [&](auto kernel, int nt, bool experts, int mt = 1) {
+    const int w = group_waves(nt, mt), rows = 16 * mt / p.parts, per_item = p.swiglu ? nt / 2 : nt;
     p.passes = (uint32_t)((p.M + rows - 1) / rows);  // (experts: at most so many)
     const int64_t items = (int64_t)p.passes * ((p.tile_cols + per_item - 1) / per_item);
-    const int64_t most = (int64_t)cus * waves_per_cu(nt) / w;
+    const int64_t most = (int64_t)cus * waves_per_cu(nt, mt) / w;
     int64_t grid = std::min<int64_t>(items, most);
     if (!experts) {
       p.split = choose_split((uint32_t)items, (uint32_t)(most * w), (uint32_t)((p.w.K + kBlock - 1) / kBlock), w);
       grid = std::min<int64_t>(most, (items * p.split + w - 1) / w);
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * w), w * nt * 64 * sizeof(f32x4), stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * w), w * nt * mt * 64 * sizeof(f32x4), stream, p);
   };
+  bool two_rows = false;
   auto go = [&](auto nt, auto sub, auto zeros) {
     constexpr int NT = decltype(nt)::value, SUB = decltype(sub)::value;
     constexpr bool Z = decltype(zeros)::value;
     if (!p.rb_expert) {
       if constexpr (NT == 1)
-        if (p.M <= 4) return launch(w4_kernel<1, SUB, Z, 1, false, true, false>, 1, false);
-      launch(w4_kernel<NT, SUB, Z, 1, false, false, true>, NT, false);
+        if (p.M <= 4) return launch(w4_kernel<1, SUB, Z, 1, false, true, false, 1>, 1, false);
+      if constexpr (NT == 4)
+        if (two_rows) return launch(w4_kernel<4, SUB, Z, 1, false, false, true, 2>, 4, false, 2);
+      launch(w4_kernel<NT, SUB, Z, 1, false, false, true, 1>, NT, false);
     } else if constexpr (NT != 1) {
-      if (p.parts == 2) launch(w4_kernel<NT, SUB, Z, 2, true, true, true>, NT, true);
-      else launch(w4_kernel<NT, SUB, Z, 1, true, true, true>, NT, true);
+      if (p.parts == 2) launch(w4_kernel<NT, SUB, Z, 2, true, true, true, 1>, NT, true);
+      else launch(w4_kernel<NT, SUB, Z, 1, true, true, true, 1>, NT, true);
     }
   };
   auto with_zeros = [&](auto nt, auto sub) {
@@ -629,14 +668,17 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
   // Column tiles of an item.  Experts: four, or two (one gate, one up) where
   // SwiGLU's tiles are no whole pairs.  Dense up to 4 rows: one tile, and more
   // waves (1 x 8192 x 8192 8.6 us, with four tiles 11.2).  Dense with more rows:
-  // x is read once per item, so as many tiles as leave an item for every CU.  Row
-  // tiles x column tiles, and us with 1, 2, 4 tiles an item: 256 (32 x 3584 x
-  // 2048) 5.9, 6.3, 8.0; 320 (16 x 4096 x 5120) 7.9, 6.2, 8.1; 512 (64 x 7168 x
-  // 2048) 13.9, 9.3, 11.6; 640 (16 x 4096 x 10240) 12.3, 9.4, 8.6; 1024 (128 x
-  // 2048 x 2048) 7.7, 6.4, 6.0.
+  // x is read once per item and codes are expanded once per row tile or two, so
+  // as many tiles an item as leave one for every CU.  Row tiles x column tiles,
+  // and us with 1, 2, 4 column tiles an item and with 4 times two row tiles: 256
+  // (32 x 3584 x 2048) 5.9, 6.3, 8.0; 320 (16 x 4096 x 5120) 7.9, 6.2, 8.1; 512
+  // (64 x 7168 x 2048) 13.9, 9.3, 11.6; 640 (16 x 4096 x 10240) 12.3, 9.4, 8.6;
+  // 1024 (32 x 3584 x 8192) -, 10.3, 8.2, 10.1; 1280 (64 x 3584 x 5120) -, -,
+  // 12.2, 10.1; 2048 (64 x 3584 x 8192) -, 16.7, 13.6, 11.2.
   const int64_t tiles = (p.M + 15) / 16 * p.tile_cols;
   const int wide = p.rb_expert ? (p.swiglu && p.tile_cols % 2 ? 2 : 4)
                    : p.M <= 4 || tiles <= cus ? 1 : tiles <= 2 * (int64_t)cus ? 2 : 4;
+  two_rows = p.M > 16 && tiles > 4 * (int64_t)cus;
   if (wide == 1) with_group(integral_constant<int, 1>());
   else if (wide == 2) with_group(integral_constant<int, 2>());
   else with_group(integral_constant<int, 4>());

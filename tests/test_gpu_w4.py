@@ -60,7 +60,8 @@ def _bound(x, w, group, want):
 SHAPES = [(1, 8, 1), (1, 128, 16), (1, 2048, 2048), (2, 136, 17), (5, 5608, 2811), (16, 1024, 100), (17, 264, 33),
           (33, 96, 50), (48, 520, 2064), (64, 3584, 512), (65, 1032, 70), (130, 384, 40), (1, 8192, 3584), (3, 16384, 64),
           (0, 64, 64), (4, 136, 50), (5, 264, 6168), (20, 136, 3090), (16, 392, 4090),
-          (16, 136, 8210), (40, 1032, 1370)]
+          (16, 136, 8210), (40, 1032, 1370), (33, 264, 8200),
+          (130, 136, 4090), (17, 1032, 16400), (1000, 40, 300)]
 
 
 @pytest.mark.parametrize("zeros", [False, True])
