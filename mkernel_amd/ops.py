@@ -254,8 +254,9 @@ def moe_build_indices_dev(topk_ids: torch.Tensor, gates: torch.Tensor, e0: int, 
     nb = (cap + row_block - 1) // row_block
     parts = (4, n_local, n_local, 3 * cap, cap, nb, nb, cap, T + 1, cap, cap, max(cap, 1), max(wsb, 4) // 4)
     buf = torch.empty(sum(parts), dtype=torch.int32, device=dev)
+    # ("unsafe": pieces that autograd does not know as views, which tables need not be; 4.1 us with views, so 2.9)
     sizes, padded, local_rb, pull, row_expert, rb_expert, rb_rows, weight, offset, to_slot, to_owner, to_row, _ = \
-        buf.split_with_sizes(parts)
+        torch.unsafe_split_with_sizes(buf, parts)
     t = dict(zip(_INDEX_TABLES, (padded, local_rb, pull.view(cap, 3), row_expert, rb_expert, rb_rows,
                                  weight.view(torch.float32), offset, to_slot, to_owner, to_row)))
     sizes = sizes.view(torch.int64)  # both words are written by the build
@@ -461,7 +462,7 @@ def _route(logits, topk, renorm, token_mask, coef):
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
         at = sums.data_ptr()
         balance = (at + 4 + 4 * E, at + 4, at + 4 + 8 * E, at, coef, ws.data_ptr(), n)
-        loss, prob_sum, counts, tokens = sums.split_with_sizes((1, E, E, 1))
+        loss, prob_sum, counts, tokens = torch.unsafe_split_with_sizes(sums, (1, E, E, 1))
         out += (loss.view(torch.float32), counts, prob_sum.view(torch.float32), tokens)
     capi.call_values("mk_moe_route", MoeRouteArgs, _raw_stream(dev.index), logits.data_ptr(),
                      0 if token_mask is None else token_mask.data_ptr(), ids.data_ptr(), gates.data_ptr(), T,
