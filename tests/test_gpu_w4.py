@@ -324,6 +324,64 @@ def test_many_blocks(dev):
         assert torch.equal(part[:rows], out[:rows]) and bool((part[rows:] == 7).all())
 
 
+def test_every_row_real_and_several_sources(dev):
+    """No rb_rows: all 128 rows of a block, as rb_rows of 128 gives them, for single values and pairs; tokens of several
+    sources through the pull table, entries outside them read as zeros."""
+    _say("whole blocks, sources")
+    E, K, N, B = 3, 264, 96, 4
+    w = _weights((E, K, N), 32, 1, True, True)
+    p = _pack(dev, w, 32)
+    rb_expert = torch.tensor([2, 0, 1, 0], dtype=torch.int32, device=dev)
+    full = torch.full((B,), 128, dtype=torch.int32, device=dev)
+    A = _whole((B * 128, K), 5).to(dev)
+    for mode, a in ((0, A), (1, A), (0, torch.cat([A, A * 2 ** -9], 1))):
+        width = N // 2 if mode else N
+        got, want = (torch.full((B * 128, width), 7.0, device=dev) for _ in range(2))
+        ops.moe_grouped_gemm_w4(a, p, got, rb_expert, mode=mode)
+        ops.moe_grouped_gemm_w4(a, p, want, rb_expert, full, mode=mode)
+        assert torch.equal(got, want)
+        if mode == 0:
+            x = a.cpu().to(D).view(B, 128, -1, K).sum(2)
+            dense = _dense(*w, 32)
+            ref = torch.cat([x[b] @ dense[int(rb_expert[b])] for b in range(B)])
+            assert torch.equal(got.cpu(), ref.float())
+    tokens = _whole((6 * 20, K), 7).to(dev)  # 3 nodes of 2 devices with 20 tokens each
+    g = torch.Generator().manual_seed(3)
+    R = B * 128
+    pull = torch.stack([torch.randint(0, 3, (R,), generator=g), torch.randint(0, 2, (R,), generator=g),
+                        torch.randint(0, 20, (R,), generator=g)], 1)
+    at = (pull[:, 0] * 2 + pull[:, 1]) * 20 + pull[:, 2]
+    rows = tokens.cpu()[at]
+    pull[7] = torch.tensor([9, 0, 0])      # past the buffer
+    pull[200] = torch.tensor([-1, -1, -1])  # a padding row
+    rows[7] = rows[200] = 0
+    got, want = (torch.full((R, N), 7.0, device=dev) for _ in range(2))
+    ops.moe_grouped_gemm_w4(tokens, p, got, rb_expert, gather_pull=pull.int().to(dev), tokens_per_src=20, devs_per_node=2)
+    ops.moe_grouped_gemm_w4(rows.to(dev), p, want, rb_expert)
+    assert torch.equal(got, want)
+
+
+def test_layer_with_host_sizes(dev):
+    """Tables trimmed on the host: the bits of the device's row count; without rb_rows, padding rows as zeros."""
+    _say("layer, host sizes")
+    T, H, I, E, k = 40, 264, 48, 10, 3
+    x, logits, w1, w2 = _layer(dev, T, H, I, E, 0, E, k, 64, 5)
+    p1, p2 = _pack(dev, w1, 64), _pack(dev, w2, 64)
+    want, ids, gates = _run_layer(dev, x.to(dev), logits.to(dev), p1, p2, 0, E, k, torch.float32)
+    t = ops.moe_build_indices_dev(ids, gates, 0, E)
+    R = t["R_pad"]
+    for rb_rows in (t["rb_rows"], None):
+        act = torch.full((R, 2 * I), float("nan"), dtype=torch.bfloat16, device=dev)
+        ye = torch.full((R, H), float("nan"), device=dev)
+        y = torch.empty((T, H), device=dev)
+        ops.moe_ffn_combine_w4(x.to(dev), t["pull_indices"], t["row_weight"], t["owner_offset"], t["slot_to_row"], p1, p2,
+                               act, ye, y, t["rb_expert"], rb_rows)
+        if rb_rows is not None:
+            assert torch.equal(y, want)
+        else:  # other passes of the same rows: other sums of the same terms, an activation within 2^-16 of each
+            assert float((y - want).norm() / want.norm()) < 2.0 ** -15
+
+
 def test_past_32_bits(dev):
     """Packed weights of more than 4 GiB: the last experts' are the same as packed alone.  Rows of x and of the result
     more than 2^31 elements into their buffers."""
