@@ -625,9 +625,10 @@ int mk_w4_quantize(const mk_w4_quantize_args* args, void* stream);
 /* C[M, N] = A[M, K] @ w (num_experts 1), fp32 sums, bf16 or fp32 output.  For
  * few rows (16 at a time, and the weights expanded for each 16); K % 8 == 0,
  * lda % 8 == 0, any M up to 2^20 and any N.  A group's sum is that of
- * A * (128 + code) - A * (128 + zero), exact products: its fp32 roundings are
- * relative to 143 times the group's largest |A|, and an infinity in a row of A,
- * or a magnitude above 2^120, makes that row of C NaN or infinite. */
+ * A * (16 + code) - A * (16 + zero), exact products: its fp32 roundings are
+ * relative to at most 31 times the group's sum of |A|, and an infinity in a row
+ * of A, or a group whose |A| sum to more than 2^123, makes that row of C NaN or
+ * infinite. */
 typedef struct mk_gemm_w4_args {
   const void* A;        /* bf16 [M, lda] */
   void* C;              /* [M, ldc] */

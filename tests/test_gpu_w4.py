@@ -83,6 +83,44 @@ def test_gemm_exact(dev, M, K, N, group, zeros):
         assert torch.equal(got.cpu(), want) and bool((out[:, N:] == 3).all())
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N", [(1, 512, 200), (3, 256, 50), (5, 264, 40), (16, 512, 2064), (40, 256, 8210)])
+def test_small_beside_large(dev, M, K, N, group, zeros):
+    """Half of x odd numbers up to 3, half multiples of 32 up to 6144, all positive: a group's partial sums of
+    x (16 + code) and x (16 + zero), codes and zeros up to 15, are whole numbers up to 31 * 64 * (6144 + 3) < 2^24,
+    so nothing is rounded in fp32 and nothing of the small x may be missing from a float32 result; so the total,
+    15 * 256 * 6147 at most in a sum over 512 rows, of codes that lie around the zero point."""
+    _say("small beside large", M, K, N, group, zeros)
+    g = torch.Generator().manual_seed(M + N)
+    codes, scales, z = _weights((K, N), group, K + N, zeros, True)
+    scales = torch.ones_like(scales)
+    if zeros:
+        z = torch.randint(6, 10, z.shape, generator=g, dtype=torch.uint8)
+    x = 32.0 * torch.randint(160, 193, (M, K), generator=g)
+    x[:, 1::2] = 2.0 * torch.randint(0, 2, (M, K // 2), generator=g) + 1
+    assert torch.equal(x.to(torch.bfloat16).float(), x)
+    w = _dense(codes, scales, z, group)
+    for g0 in range(0, K, group):  # (the running total over groups)
+        assert float((x[:, :g0 + group].to(D) @ w[:g0 + group]).abs().max()) < 2 ** 24
+    want = x.to(D) @ w
+    out = torch.empty((M, N), device=dev)
+    ops.gemm_w4(x.to(torch.bfloat16).to(dev), _pack(dev, (codes, scales, z), group), out=out)
+    assert torch.equal(out.cpu().to(D), want)
+    E = 3  # the experts' product: one expert's rows, and the halves of a pair (the large and the small numbers)
+    p = ops.w4_pack(*(t.expand(E, *t.shape).contiguous().to(dev) for t in (codes, scales)), group,
+                    zeros=None if z is None else z.expand(E, *z.shape).contiguous().to(dev))
+    A = torch.zeros((128, K))
+    A[:M] = x
+    one, rows = torch.tensor([1], dtype=torch.int32, device=dev), torch.tensor([M], dtype=torch.int32, device=dev)
+    small = torch.zeros_like(A)
+    small[:, 1::2] = A[:, 1::2]
+    for a in (A, torch.cat([A - small, small], 1)):
+        y = torch.zeros((128, N), device=dev)
+        ops.moe_grouped_gemm_w4(a.to(torch.bfloat16).to(dev), p, y, one, rows)
+        assert torch.equal(y[:M].cpu().to(D), want)
+
+
 @pytest.mark.parametrize("M,K,N,group,zeros", [(1, 8192, 3584, 128, False), (1, 2048, 2048, 32, True), (7, 5608, 2811, 32, True),
                                                (64, 3584, 8192, 64, False), (16, 7168, 4096, 128, True), (100, 1000, 300, 64, False)])
 def test_gemm_normal(dev, M, K, N, group, zeros):
