@@ -564,8 +564,9 @@ int mk_moe_route_backward(const mk_moe_route_backward_args* args, void* stream);
  * dgates is 0 where topk_ids names no local expert (another rank has that
  * part) or the row was not produced here (slot_to_row -1).  Rows at or past
  * R_pad (sizes[1] when sizes is set, R_pad then being the capacity) are
- * neither read nor written.  dy_expert may be NULL, and rb_rows then too; it
- * may be y_expert itself, whose padding rows are then zeroed as well.
+ * neither read nor written; with R_pad 0 every table of rows may be NULL, and
+ * dgates is 0.  dy_expert may be NULL, and rb_rows then too; it may be y_expert
+ * itself, whose padding rows are then zeroed as well.
  * Each sum is added in a fixed order.  At most 32 choices.  No counterpart in
  * the reference, which has no backward pass. */
 typedef struct mk_moe_combine_backward_args {

@@ -166,7 +166,8 @@ __global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineBwdKP
       const int o = __shfl(e, i, 64);
       slot += o >= 0 && o < p.n_local && (o < e || (o == e && i < lane));
     }
-    if (local && slot < p.owner_offset[t + 1]) row = p.slot_to_row[slot];
+    // (without rows there may be no slot_to_row either)
+    if (R > 0 && local && slot < p.owner_offset[t + 1]) row = p.slot_to_row[slot];
     if (row >= R) row = -1;
     const uint64_t there = __ballot(row >= 0);
     const int at = __popcll(there & ((1ull << lane) - 1));

@@ -583,6 +583,28 @@ def test_combine_backward_no_rows(dev):
     assert dg.shape == (0, 2)
 
 
+def test_combine_backward_offsets_without_rows(dev):
+    """Owner offsets of routed tokens, but no rows here: no table of rows is read, and dgates is 0."""
+    _say("combine backward, offsets without rows")
+    T, H, k = 6, 64, 2
+    ids = torch.arange(T * k, dtype=torch.int32, device=dev).view(T, k) % 3
+    t = ops.moe_build_indices_dev(ids, torch.ones((T, k), device=dev), 0, 3)
+    dy = torch.ones((T, H), device=dev)
+    none = torch.empty(0, dtype=torch.int32, device=dev)
+    assert none.data_ptr() == 0 and int(t["owner_offset"][-1]) == T * k
+    a, dg = ops.moe_combine_backward(dy, torch.empty((0, H), dtype=torch.bfloat16, device=dev), ids, t["row_weight"][:0],
+                                     t["owner_offset"], none, none, 0, 3, dgates=torch.full((T, k), NAN, device=dev))
+    assert a.shape == (0, H) and not dg.any()
+    # a capacity of one block, of which the device counts no row
+    ye = torch.full((128, H), NAN, dtype=torch.bfloat16, device=dev)
+    keep = torch.full((128, H), 7.0, dtype=torch.bfloat16, device=dev)
+    _, dg = ops.moe_combine_backward(dy, ye, ids, torch.ones(128, device=dev), t["owner_offset"], t["slot_to_row"],
+                                     torch.zeros(1, dtype=torch.int32, device=dev), 0, 3, dy_expert=keep,
+                                     dgates=torch.full((T, k), NAN, device=dev),
+                                     sizes=torch.zeros(2, dtype=torch.int64, device=dev))
+    assert not dg.any() and bool((keep == 7).all())
+
+
 def test_repeatable_on_other_streams_and_in_a_graph(dev):
     """Equal bits on another stream, beside another call, and in replays of a captured graph with new inputs."""
     _say("streams and graph")
