@@ -944,9 +944,8 @@ int mk_moe_grouped_gemm(const mk_moe_grouped_gemm_args* a, void* stream) {
                            static_cast<hipStream_t>(stream));
 }
 
-int mk_moe_combine(const mk_moe_combine_args* a, void* stream) {
-  // y_expert, row_weight and slot_to_row are read only inside owner_offset's
-  // ranges: with no routed rows (every range empty) they may be NULL.
+// `rows`: how many y_expert has (0: it, row_weight and slot_to_row may be NULL).
+static int combine_impl(const mk_moe_combine_args* a, int64_t rows, void* stream) {
   if (!a || !a->owner_offset || (!a->y_out && a->num_tokens > 0))
     return fail(MK_EINVAL, "mk_moe_combine: null argument");
   if (a->num_tokens < 0) return fail(MK_ESHAPE, "mk_moe_combine: num_tokens < 0");
@@ -955,9 +954,13 @@ int mk_moe_combine(const mk_moe_combine_args* a, void* stream) {
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   mk::CombineKParams p{a->y_expert, a->row_weight, a->owner_offset, a->slot_to_row,
-                       a->y_out, a->num_tokens, a->H, a->out_dtype, 0};
+                       a->y_out, a->num_tokens, a->H, a->out_dtype, 0, (uint32_t)std::min<int64_t>(rows, INT32_MAX)};
   hipError_t e = mk::launch_combine(p, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_combine launch");
+}
+
+int mk_moe_combine(const mk_moe_combine_args* a, void* stream) {
+  return combine_impl(a, a && a->y_expert && a->row_weight && a->slot_to_row ? INT32_MAX : 0, stream);
 }
 
 int mk_moe_invert_slots(const int32_t* row_to_slot, const int32_t* row_to_owner, int64_t R_pad, int32_t owner,
@@ -1043,7 +1046,7 @@ int mk_moe_ffn_combine(const mk_moe_ffn_args* a, void* stream) {
     return rc;
   mk_moe_combine_args ca{a->y_expert, a->row_weight, a->owner_offset, a->slot_to_row, a->y_out,
                          a->num_tokens, a->H, a->out_dtype};
-  return mk_moe_combine(&ca, stream);
+  return combine_impl(&ca, a->R_pad, stream);
 }
 
 int64_t mk_moe_route_workspace_bytes(int64_t num_tokens, int32_t num_experts) {
@@ -1293,7 +1296,7 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* a, void* stream) {
   if (int rc = prepare_grouped_w4(fn, &g1, &p1)) return rc;
   if (int rc = prepare_grouped_w4(fn, &g2, &p2)) return rc;
   const mk::CombineKParams pc{a->y_expert, a->row_weight, a->owner_offset, a->slot_to_row, a->y_out,
-                              a->num_tokens, a->w1.K, a->out_dtype, 1};
+                              a->num_tokens, a->w1.K, a->out_dtype, 1, (uint32_t)a->R_pad};
   if (a->num_tokens > 0 && !aligned16(a->y_out)) return fail(MK_EINVAL, "%s: y_out must be 16-byte aligned", fn);
   DevInfo d;
   if (int rc = device_info(&d)) return rc;

@@ -160,6 +160,7 @@ struct CombineKParams {
   int64_t num_tokens, H;
   int out_dtype;
   int f32_rows;             // y_expert holds fp32
+  uint32_t rows;            // rows of y_expert: others contribute nothing; 0: no table of rows is read
 };
 hipError_t launch_combine(const CombineKParams& p, hipStream_t stream);
 hipError_t launch_tile_rows(const int* pull, int64_t R_pad, int* rb_rows, hipStream_t stream);

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineKParams p) {
   typedef uint32_t words __attribute__((ext_vector_type(kWords)));
   const int64_t t = blockIdx.x;
   const int s0 = p.owner_offset[t], s1 = p.owner_offset[t + 1];
-  const int n = s1 - s0;
+  const int n = p.rows > 0 ? s1 - s0 : 0;  // (without rows the tables may be NULL)
   const int64_t vec = p.H / V;
   int rows[kMaxSlots];
   float wts[kMaxSlots];
@@ -66,10 +66,12 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineKParams p) {
   for (int k = 0; k < kMaxSlots; ++k)
     if (few && k < n) rows[k] = p.slot_to_row[s0 + k];
   // a slot whose row is -1 was not produced on this GPU (another owner's
-  // combine covers it): it contributes nothing
+  // combine covers it), and one at or past the rows' count not at all: it
+  // contributes nothing (as unsigned numbers both are at or past the count)
+  auto has = [&](int row) { return (uint32_t)row < p.rows; };
 #pragma unroll
   for (int k = 0; k < kMaxSlots; ++k)
-    if (few && k < n) wts[k] = rows[k] >= 0 ? p.row_weight[rows[k]] : 0.f;
+    if (few && k < n) wts[k] = has(rows[k]) ? p.row_weight[rows[k]] : 0.f;
   for (int64_t c = (int64_t)blockIdx.y * kThreads + threadIdx.x; c < vec; c += (int64_t)gridDim.y * kThreads) {
     float acc[V];
 #pragma unroll
@@ -92,14 +94,14 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(CombineKParams p) {
       words v[kMaxSlots];
 #pragma unroll
       for (int k = 0; k < kMaxSlots; ++k)
-        if (k < n && rows[k] >= 0) v[k] = load(rows[k]);
+        if (k < n && has(rows[k])) v[k] = load(rows[k]);
 #pragma unroll
       for (int k = 0; k < kMaxSlots; ++k)
-        if (k < n && rows[k] >= 0) add(wts[k], v[k]);
+        if (k < n && has(rows[k])) add(wts[k], v[k]);
     } else {
       for (int s = s0; s < s1; ++s) {
         const int row = p.slot_to_row[s];
-        if (row < 0) continue;
+        if (!has(row)) continue;
         add(p.row_weight[row], load(row));
       }
     }

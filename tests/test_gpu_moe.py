@@ -458,3 +458,34 @@ def test_ffn_combine_random_layers(dev):
             assert rel_fro(ys[0], y_ref) < TOL, f"case {case}: y"
         routed = torch.from_numpy(np.diff(np.asarray(idx["owner_offset"])) > 0)
         assert (ys[0][~routed] == 0).all(), f"case {case}: unrouted tokens"
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("topk", [2, 9])
+def test_layer_rows_behind_the_buffers(dev, topk, out):
+    """Owner offsets of a routed batch with fewer rows than were routed, and with none: what has no row adds
+    nothing, and no table of rows is read where there are no rows (the layer, and the combine by itself)."""
+    _say(f"moe layer, slots without rows, topk {topk}, {out}")
+    T, H, I = 6, 256, 128
+    ids = torch.arange(topk, dtype=torch.int32, device=dev).expand(T, topk).contiguous()
+    gates = torch.full((T, topk), 0.5, device=dev)
+    x = wl.randn_bf16((T, H), 3).to(dev)
+    w1, w2 = wl.randn_bf16((topk, H, 2 * I), 4, H ** -0.5).to(dev), wl.randn_bf16((topk, I, H), 5, I ** -0.5).to(dev)
+    all_, first = (ops.moe_build_indices_dev(ids, gates, 0, n) for n in (topk, 1))
+    assert all_["R_pad"] == 128 * topk and first["R_pad"] == 128
+
+    def layer(t, rows, n):
+        y = torch.full((T, H), float("nan"), dtype=out, device=dev)
+        ye = torch.full((128 * topk, H), float("nan"), dtype=torch.bfloat16, device=dev)
+        ops.moe_ffn_combine(x, t["pull_indices"][:rows], t["row_weight"][:rows], t["owner_offset"],
+                            t["slot_to_row"] if rows else t["slot_to_row"][:0].clone(), w1[:n], w2[:n], None,
+                            torch.empty((rows, I), dtype=torch.bfloat16, device=dev), ye[:rows], y,
+                            rb_expert=t["rb_expert"][:rows // 128], rb_rows=t["rb_rows"][:rows // 128], fuse_dispatch=True)
+        return y
+
+    assert torch.equal(layer(all_, 128, topk), layer(first, 128, 1))
+    assert not layer(all_, 0, topk).any()
+    y = torch.full((T, H), float("nan"), dtype=out, device=dev)
+    ops.moe_combine(torch.empty((0, H), dtype=torch.bfloat16, device=dev), all_["row_weight"][:0].clone(),
+                    all_["owner_offset"], all_["slot_to_row"][:0].clone(), y)
+    assert not y.any()

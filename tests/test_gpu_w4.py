@@ -467,6 +467,32 @@ def test_no_tokens(dev):
     assert not y.any()
 
 
+def test_layer_rows_behind_the_buffers(dev):
+    """Owner offsets of a routed batch with fewer rows than were routed, and with none: what has no row adds
+    nothing, and no table of rows is read where there are no rows."""
+    _say("layer, slots without rows")
+    T, H, I, bf = 6, 64, 32, torch.bfloat16
+    w1, w2 = _weights((2, H, 2 * I), 32, 1, False, False), _weights((2, I, H), 32, 2, False, False)
+    ids = torch.tensor([[0, 1]] * T, dtype=torch.int32, device=dev)
+    gates = torch.full((T, 2), 0.5, device=dev)
+    x = wl.randn_bf16((T, H), 3).to(dev)
+    both, first = ops.moe_build_indices_dev(ids, gates, 0, 2), ops.moe_build_indices_dev(ids, gates, 0, 1)
+    assert both["R_pad"] == 256 and first["R_pad"] == 128
+
+    def layer(t, rows, n):
+        y = torch.full((T, H), float("nan"), device=dev)
+        ye = torch.full((256, H), float("nan"), device=dev)  # (behind the rows: what may not be read)
+        pack = lambda w: _pack(dev, (w[0][:n], w[1][:n], None), 32)
+        ops.moe_ffn_combine_w4(x, t["pull_indices"][:rows], t["row_weight"][:rows], t["owner_offset"],
+                               t["slot_to_row"] if rows else t["slot_to_row"][:0].clone(), pack(w1), pack(w2),
+                               torch.empty((rows, 2 * I), dtype=bf, device=dev), ye[:rows], y, t["rb_expert"][:rows // 128],
+                               t["rb_rows"][:rows // 128])
+        return y
+
+    assert torch.equal(layer(both, 128, 2), layer(first, 128, 1))
+    assert not layer(both, 0, 2).any()
+
+
 def test_weights_as_a_tensor(dev):
     """Packed weights stored and loaded; only the low four bits of a code count; a wrong size is refused."""
     _say("packed tensor")
