@@ -627,7 +627,8 @@ int mk_w4_quantize(const mk_w4_quantize_args* args, void* stream);
 
 /* C[M, N] = A[M, K] @ w (num_experts 1), fp32 sums, bf16 or fp32 output.  For
  * few rows (16 at a time, and the weights expanded for each 16); K % 8 == 0,
- * lda % 8 == 0, any M up to 2^20 and any N.  A group's sum is that of
+ * lda % 8 == 0, A 16-byte aligned; C aligned to its elements; any M up to 2^20
+ * and any N.  A group's sum is that of
  * A * (16 + code) - A * (16 + zero), exact products: its fp32 roundings are
  * relative to at most 31 times the group's sum of |A|, and an infinity in a row
  * of A, or a group whose |A| sum to more than 2^123, makes that row of C NaN or
@@ -649,7 +650,8 @@ int mk_gemm_w4(const mk_gemm_w4_args* args, void* stream);
  * they are.  out is fp32, bf16, or a bf16 pair: a row holds its values rounded
  * to bf16 and behind them what the rounding left, again in bf16 (17 bits of
  * significand, so that an activation between two products loses nothing that a
- * bf16 result shows); such rows are read with a_parts 2.  gather_pull,
+ * bf16 result shows); such rows are read with a_parts 2.  A is 16-byte aligned,
+ * out to its elements.  gather_pull,
  * n_src_rows, tokens_per_src, devs_per_node and sizes as in
  * mk_moe_grouped_gemm_args. */
 typedef struct mk_moe_grouped_gemm_w4_args {

@@ -1207,6 +1207,11 @@ static mk::W4KParams w4_params(const mk_w4_weights& w, const void* A, void* C, i
   return p;
 }
 
+// Results of the 4-bit products are stored element by element.
+static bool w4_out_aligned(const void* out, int out_type) {
+  return reinterpret_cast<uintptr_t>(out) % (out_type == 0 ? 4 : 2) == 0;
+}
+
 int mk_gemm_w4(const mk_gemm_w4_args* a, void* stream) {
   if (!a) return fail(MK_EINVAL, "mk_gemm_w4: null argument");
   if (int rc = check_w4("mk_gemm_w4", a->W)) return rc;
@@ -1220,7 +1225,8 @@ int mk_gemm_w4(const mk_gemm_w4_args* a, void* stream) {
   if (a->out_type != 0 && a->out_type != 1) return fail(MK_EINVAL, "mk_gemm_w4: out_type must be 0 or 1");
   if (a->M == 0) return MK_OK;
   if (!a->A || !a->C) return fail(MK_EINVAL, "mk_gemm_w4: null argument");
-  if (!aligned16(a->A) || !aligned16(a->C)) return fail(MK_EINVAL, "mk_gemm_w4: A and C must be 16-byte aligned");
+  if (!aligned16(a->A)) return fail(MK_EINVAL, "mk_gemm_w4: A must be 16-byte aligned");
+  if (!w4_out_aligned(a->C, a->out_type)) return fail(MK_EINVAL, "mk_gemm_w4: C must be aligned to its elements");
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   mk::W4KParams p = w4_params(a->W, a->A, a->C, a->M, a->lda, a->ldc);
@@ -1242,7 +1248,8 @@ static int prepare_grouped_w4(const char* fn, const mk_moe_grouped_gemm_w4_args*
   if (a->R_pad / 8 * ((a->W.N + 15) / 16) >= (1LL << 31)) return fail(MK_ESHAPE, "%s: R_pad x N too large", fn);
   if (a->R_pad > 0) {
     if (!a->A || !a->out || !a->rb_expert) return fail(MK_EINVAL, "%s: null argument", fn);
-    if (!aligned16(a->A) || !aligned16(a->out)) return fail(MK_EINVAL, "%s: A and out must be 16-byte aligned", fn);
+    if (!aligned16(a->A)) return fail(MK_EINVAL, "%s: A must be 16-byte aligned", fn);
+    if (!w4_out_aligned(a->out, a->out_type)) return fail(MK_EINVAL, "%s: out must be aligned to its elements", fn);
     if (a->gather_pull && (a->n_src_rows <= 0 || a->tokens_per_src <= 0 || a->devs_per_node <= 0 || a->a_parts != 1 ||
                            a->n_src_rows >= (1LL << 30) / a->W.K))
       return fail(MK_EINVAL, "%s: gather_pull needs n_src_rows, tokens_per_src and devs_per_node > 0, a_parts 1 and "
@@ -1297,6 +1304,7 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* a, void* stream) {
   if (int rc = prepare_grouped_w4(fn, &g2, &p2)) return rc;
   const mk::CombineKParams pc{a->y_expert, a->row_weight, a->owner_offset, a->slot_to_row, a->y_out,
                               a->num_tokens, a->w1.K, a->out_dtype, 1, (uint32_t)a->R_pad};
+  if (rows && !aligned16(a->y_expert)) return fail(MK_EINVAL, "%s: y_expert must be 16-byte aligned", fn);
   if (a->num_tokens > 0 && !aligned16(a->y_out)) return fail(MK_EINVAL, "%s: y_out must be 16-byte aligned", fn);
   DevInfo d;
   if (int rc = device_info(&d)) return rc;

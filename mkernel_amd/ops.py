@@ -644,8 +644,8 @@ def gemm_w4(A: torch.Tensor, W: W4Weights, out: torch.Tensor | None = None) -> t
     """C = A @ w for few rows (mk_gemm_w4): A bf16 [M, K], w 4-bit weights of
     w4_pack; fp32 sums of exact products, scaled group by group in fp32; out
     bf16 (what is made where none is given) or float32.  K a multiple of 8, any
-    M and N; rows of A (a multiple of 8 elements apart) and of out need only be
-    contiguous each.  The weights are expanded for every 16 rows: from a few
+    M and N; rows of A (a multiple of 8 elements apart, the first 16-byte
+    aligned) and of out need only be contiguous each.  The weights are expanded for every 16 rows: from a few
     hundred rows on, gemm with bf16 weights is faster."""
     if not (isinstance(A, torch.Tensor) and A.dtype is torch.bfloat16 and A.is_cuda and A.dim() == 2
             and A.is_contiguous()):

@@ -450,6 +450,32 @@ def test_past_32_bits(dev):
     assert torch.equal(ops.gemm_w4(wide[:, :K], w, out=far[:, :N]), ops.gemm_w4(wide[:, :K].contiguous(), w))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_outputs_at_odd_places(dev, dtype):
+    """Results that start at any element: columns from an odd one on, rows behind an odd width, for both products
+    and for a pair; what lies beside them stays."""
+    _say("outputs at odd places", dtype)
+    for M, K, N in ((1, 136, 33), (5, 264, 2811), (40, 136, 8211)):
+        w = _weights((K, N), 64, M, True, True)
+        p, x = _pack(dev, w, 64), _whole((M, K), 1).to(dev)
+        want = ops.gemm_w4(x, p, out=torch.empty((M, N), dtype=dtype, device=dev))
+        for out in (torch.full((M, N + 3), 7.0, dtype=dtype, device=dev)[:, 1:N + 1],
+                    torch.full((M + 2, N), 7.0, dtype=dtype, device=dev)[1:M + 1]):
+            assert out.data_ptr() % 16
+            assert torch.equal(ops.gemm_w4(x, p, out=out), want)
+            whole = out._base if out._base is not None else out
+            assert int((whole != 7).sum()) == int((want != 7).sum())
+    K, N = 136, 96
+    w = _weights((1, K, N), 64, 5, False, True)
+    p, x = _pack(dev, w, 64), _whole((128, K), 1).to(dev)
+    rb = torch.zeros(1, dtype=torch.int32, device=dev)
+    for width in (N,) if dtype is torch.float32 else (N, 2 * N):
+        want = ops.moe_grouped_gemm_w4(x, p, torch.empty((128, width), dtype=dtype, device=dev), rb)
+        flat = torch.full((128 * width + 2,), 7.0, dtype=dtype, device=dev)
+        got = ops.moe_grouped_gemm_w4(x, p, flat[1:-1].view(128, width), rb)
+        assert got.data_ptr() % 16 and torch.equal(got, want) and bool((flat[[0, -1]] == 7).all())
+
+
 def test_no_tokens(dev):
     _say("layer without tokens, product without rows")
     w1, w2 = _weights((2, 64, 64), 32, 1, False, False), _weights((2, 32, 64), 32, 2, False, False)

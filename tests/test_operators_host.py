@@ -159,6 +159,21 @@ def test_gemm_w4_refusals(weights, change, code, match):
     _refused("mk_gemm_w4", _args(capi.GemmW4Args, dict(GEMM, W=_weights(**weights)), change), code, match)
 
 
+@pytest.mark.parametrize("out_type,off", [(0, 2), (0, 1), (1, 1), (2, 1)])
+def test_w4_outputs_are_aligned_to_their_elements(out_type, off):
+    if out_type < 2:
+        _refused("mk_gemm_w4", _args(capi.GemmW4Args, dict(GEMM, W=_weights(), C=P + off, out_type=out_type), {}), EINVAL,
+                 "elements")
+    _refused("mk_moe_grouped_gemm_w4", _args(capi.MoeGroupedGemmW4Args,
+                                             dict(GROUPED, W=_weights(), out=P + off, out_type=out_type), {}), EINVAL, "elements")
+
+
+@pytest.mark.parametrize("change", [dict(act=P + 4), dict(y_expert=P + 4), dict(tokens=P + 8)])
+def test_ffn_w4_scratch_alignment(change):
+    a = dict(FFN, w1=_weights(K=256, N=64), w2=_weights(K=32, N=256))
+    _refused("mk_moe_ffn_combine_w4", _args(capi.MoeFfnW4Args, a, change), EINVAL, "16-byte")
+
+
 def test_pack_refusals():
     _refused("mk_w4_pack", _args(capi.W4PackArgs, dict(codes=P, scales=P, zeros=P, out=_weights()), {}), EINVAL, "one side")
     _refused("mk_w4_quantize", _args(capi.W4QuantizeArgs, dict(W=P, codes=P, scales=P, K=8, N=8, group=16, num_experts=1),
