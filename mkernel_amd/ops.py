@@ -239,7 +239,13 @@ def moe_build_indices_dev(topk_ids: torch.Tensor, gates: torch.Tensor, e0: int, 
     returned tensors are views trimmed to R / R_pad rows (the same dict
     layout as moe_build_indices, as device tensors).  With sync=False nothing
     is read back: the tables stay at their capacity and "sizes" holds the
-    device int64 {R, R_pad} for moe_ffn_combine(..., sizes=...)."""
+    device int64 {R, R_pad} for moe_ffn_combine(..., sizes=...).
+    All tables are pieces of one buffer, which holds the build's workspace too
+    and lives as long as any of them (about 32 bytes per row of the capacity;
+    clone() a table to keep or store it alone).  The tables by row
+    (pull_indices, row_expert, row_weight, row_to_slot, row_to_owner,
+    slot_to_row) start at multiples of 512 bytes where row_block is a multiple
+    of 128, the others at multiples of 4."""
     if topk_ids.dtype != torch.int32 or gates.dtype != torch.float32 or not topk_ids.is_cuda:
         raise ValueError("topk_ids must be int32 and gates float32 device tensors")
     ids = topk_ids.contiguous()
@@ -250,19 +256,22 @@ def moe_build_indices_dev(topk_ids: torch.Tensor, gates: torch.Tensor, e0: int, 
     # row count for the grouped GEMMs
     cap = (T * k + n_local * (row_block - 1) + row_block - 1) // row_block * row_block
     wsb = int(capi.lib().mk_moe_index_workspace_bytes(T, k, n_local))
-    # one allocation for the tables and the workspace: 13 took most of the call
+    # one allocation for the tables and the workspace: 13 took most of the call.  Behind the sizes' 512 bytes the
+    # row tables: whole row blocks, so that each starts where an allocation might
     nb = (cap + row_block - 1) // row_block
-    parts = (4, n_local, n_local, 3 * cap, cap, nb, nb, cap, T + 1, cap, cap, max(cap, 1), max(wsb, 4) // 4)
+    parts = (4, 124, 3 * cap, cap, cap, cap, cap, max(cap, 1), n_local, n_local, nb, nb, T + 1, max(wsb, 4) // 4)
     buf = torch.empty(sum(parts), dtype=torch.int32, device=dev)
     # ("unsafe": pieces that autograd does not know as views, which tables need not be; 4.1 us with views, so 2.9)
-    sizes, padded, local_rb, pull, row_expert, rb_expert, rb_rows, weight, offset, to_slot, to_owner, to_row, _ = \
+    sizes, _, pull, row_expert, weight, to_slot, to_owner, to_row, padded, local_rb, rb_expert, rb_rows, offset, _ = \
         torch.unsafe_split_with_sizes(buf, parts)
     t = dict(zip(_INDEX_TABLES, (padded, local_rb, pull.view(cap, 3), row_expert, rb_expert, rb_rows,
                                  weight.view(torch.float32), offset, to_slot, to_owner, to_row)))
     sizes = sizes.view(torch.int64)  # both words are written by the build
-    at, *tables, ws = itertools.accumulate((4 * n for n in parts[:-1]), initial=buf.data_ptr())
+    at, _, a_pull, a_expert, a_weight, a_slot, a_owner, a_row, a_padded, a_local, a_rb, a_rows, a_offset, ws = \
+        itertools.accumulate((4 * n for n in parts[:-1]), initial=buf.data_ptr())
     capi.call_values("mk_moe_build_indices_dev", MoeIndexDevArgs, _stream(), ids.data_ptr(), g.data_ptr(), T, k, e0,
-                     n_local, row_block, cap, ws, wsb, at, *tables)
+                     n_local, row_block, cap, ws, wsb, at, a_padded, a_local, a_pull, a_expert, a_rb, a_rows, a_weight,
+                     a_offset, a_slot, a_owner, a_row)
     if not sync:
         t["sizes"] = sizes
         return t

@@ -228,3 +228,27 @@ def test_index_dev_random_routings(dev):
         _say(f"moe index dev random case={case} T={T} topk={topk} E={experts} e0={e0} n_local={n_local} rb={row_block}")
         ids, gates = wl.zipf_routing(T, experts, min(topk, experts), float(rng.choice([0.0, 1.1])), 700 + case)
         _check(dev, ids, gates, e0, n_local, row_block)
+
+
+@pytest.mark.parametrize("T,k,n_local,row_block", [(1, 1, 1, 128), (37, 3, 5, 128), (1001, 8, 33, 128), (64, 8, 32, 256),
+                                                   (7, 2, 3, 32), (5, 1, 1, 1), (0, 2, 3, 128), (0, 1, 1, 1)])
+def test_index_dev_tables_in_one_buffer(dev, T, k, n_local, row_block):
+    """The tables share a buffer: each is its own piece of it (writing one changes no other), and those by row
+    start at multiples of 512 bytes where row_block is a multiple of 128."""
+    _say(f"moe index dev pieces T={T} k={k} n_local={n_local} row_block={row_block}")
+    ids = torch.randint(0, n_local + 1, (T, k), dtype=torch.int32, generator=torch.Generator().manual_seed(T)).to(dev)
+    gates = torch.rand((T, k), device=dev)
+    if T == 0:  # a batch of no tokens is refused (its ids have no address)
+        with pytest.raises(capi.MkError, match="null"):
+            ops.moe_build_indices_dev(ids, gates, 0, n_local, row_block, sync=False)
+        return
+    t = ops.moe_build_indices_dev(ids, gates, 0, n_local, row_block, sync=False)
+    cap = t["pull_indices"].shape[0]
+    if row_block % 128 == 0:
+        for f in ("pull_indices", "row_expert", "row_weight", "row_to_slot", "row_to_owner", "slot_to_row"):
+            assert t[f].data_ptr() % 512 == 0 and t[f].is_contiguous(), f
+    assert t["sizes"].data_ptr() % 8 == 0
+    spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size()) for x in t.values() if x.numel())
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+    assert t["owner_offset"].shape == (T + 1,) and t["row_weight"].shape == (cap,) and t["row_weight"].dtype == torch.float32
+    _check(dev, ids.cpu().numpy(), gates.cpu().numpy(), 0, n_local, row_block)
