@@ -615,7 +615,9 @@ int mk_w4_pack(const mk_w4_pack_args* args, void* stream);
 
 /* Codes and scales of bf16 weights [E, K, N], without zero points: scale =
  * bf16(largest magnitude of the group / 7), code = round(w / scale) + 8 cut to
- * 0 .. 15 (8 where the scale is 0). */
+ * 0 .. 15 (8 where the scale is 0).  With a NaN in a group its scale is NaN, so
+ * that all its weights are; with an infinity it is infinite, and the infinities
+ * keep their sign. */
 typedef struct mk_w4_quantize_args {
   const void* W;        /* bf16 [E, K, N] */
   void* codes;          /* uint8 [E, K, N] */

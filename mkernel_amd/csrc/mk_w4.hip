@@ -582,7 +582,7 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* codes, cons
 }
 
 // One thread per group and column: scale = bf16(largest magnitude / 7), code =
-// round(w / scale) + 8.
+// round(w / scale) + 8.  A NaN in a group is its largest magnitude.
 __global__ __launch_bounds__(256) void w4_quantize_kernel(const uint16_t* W, int64_t K, int64_t N, int group,
                                                           int64_t groups, int64_t count, uint8_t* codes,
                                                           uint16_t* scales) {
@@ -591,12 +591,15 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(const uint16_t* W, int
     const int64_t k0 = g * group, k1 = min(K, k0 + group);
     auto value = [&](int64_t k) { return __uint_as_float((uint32_t)W[(e * K + k) * N + n] << 16); };
     float most = 0.f;
-    for (int64_t k = k0; k < k1; ++k) most = fmaxf(most, fabsf(value(k)));
+    for (int64_t k = k0; k < k1; ++k) {
+      const float v = fabsf(value(k));
+      most = v > most || v != v ? v : most;  // (once NaN it stays: no comparison with it holds)
+    }
     const __bf16 s = (__bf16)(most / 7.f);
     const float scale = (float)s;
     scales[i] = __builtin_bit_cast(uint16_t, s);
     for (int64_t k = k0; k < k1; ++k) {
-      const float q = scale > 0.f ? rintf(value(k) / scale) : 0.f;
+      const float v = value(k), q = !(scale > 0.f) ? 0.f : isinf(v) ? v : rintf(v / scale);
       codes[(e * K + k) * N + n] = (uint8_t)((int)fminf(fmaxf(q, -8.f), 7.f) + 8);
     }
   }

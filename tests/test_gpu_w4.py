@@ -167,6 +167,32 @@ def test_quantize(dev, shape, group):
         assert bool(((got - want).abs() <= _bound(x, (codes, scales), group, want)).all())
 
 
+def test_quantize_not_finite(dev):
+    """A NaN makes its group's scale NaN, an infinity infinite; no other group's codes or scales change, and the
+    weights they stand for are NaN and infinite where they were."""
+    _say("quantize NaN and infinities")
+    K, N, group = 136, 40, 64
+    W = wl.randn_bf16((K, N), 3)
+    codes, scales = ops.w4_quantize(W.to(dev), group)
+    bad = W.clone()
+    bad[3, 5], bad[70, 6], bad[71, 6], bad[135, 7], bad[0, 8] = (float(v) for v in ("nan", "inf", "-inf", "-inf", "nan"))
+    bad[1, 8] = float("inf")
+    c2, s2 = ops.w4_quantize(bad.to(dev), group)
+    hit = torch.zeros((3, N), dtype=torch.bool)
+    hit[0, 5] = hit[1, 6] = hit[2, 7] = hit[0, 8] = True
+    rows = hit[torch.arange(K) // group].to(dev)
+    assert torch.equal(c2[~rows], codes[~rows]) and torch.equal(s2[~hit.to(dev)], scales[~hit.to(dev)])
+    back = (c2.float() - 8) * s2.float()[torch.arange(K, device=dev) // group]
+    back = back.cpu()
+    assert back[:64, 5].isnan().all() and back[:64, 8].isnan().all() and torch.isinf(s2[[1, 2], [6, 7]]).all()
+    assert back[70, 6] == float("inf") and back[71, 6] == -float("inf") and back[135, 7] == -float("inf")
+    # through a product: whole columns are not finite, others as they were
+    x = wl.randn_bf16((3, K), 4).to(dev)
+    got, want = ops.gemm_w4(x, ops.w4_pack(c2, s2, group)), ops.gemm_w4(x, ops.w4_pack(codes, scales, group))
+    cols = hit.any(0).to(dev)
+    assert not torch.isfinite(got[:, cols]).any() and torch.equal(got[:, ~cols], want[:, ~cols])
+
+
 def _tables(dev, counts, E):
     """Tables of experts with these row counts, in 128-row blocks."""
     blocks = [(c + 127) // 128 for c in counts]
