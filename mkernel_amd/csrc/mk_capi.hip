@@ -1088,15 +1088,23 @@ int mk_moe_route(const mk_moe_route_args* a, void* stream) {
   return e == hipSuccess ? MK_OK : hip_fail(e, "mk_moe_route launch");
 }
 
-// Whether two matrices of T rows of E elements share none, or are one and the same.
+// Whether two matrices share no byte: `rows` rows of `width` bytes, `ld` bytes apart.
+struct ByteRows {
+  const void* p;
+  int64_t rows, ld, width;
+};
+static bool apart(const ByteRows& a, const ByteRows& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  if (x + (uintptr_t)((a.rows - 1) * a.ld + a.width) <= y || y + (uintptr_t)((b.rows - 1) * b.ld + b.width) <= x) return true;
+  // columns of one wider matrix: the later one's begin behind the earlier one's, and end before its next row
+  const uintptr_t ld = (uintptr_t)(a.ld > 0 ? a.ld : 1), at = (x < y ? y - x : x - y) % ld;
+  const uintptr_t first = (uintptr_t)(x < y ? a.width : b.width), then = (uintptr_t)(x < y ? b.width : a.width);
+  return a.rows > 1 && b.rows > 1 && a.ld == b.ld && at >= first && at + then <= ld;
+}
+
+// The same for two matrices of T rows of E elements, or whether they are one and the same.
 static bool apart_or_same(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t T, int64_t E, int64_t size) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  if (x == y && (lda == ldb || T == 1)) return true;
-  const uintptr_t bytes_a = (uintptr_t)(((T - 1) * lda + E) * size), bytes_b = (uintptr_t)(((T - 1) * ldb + E) * size);
-  if (x + bytes_a <= y || y + bytes_b <= x) return true;
-  // columns of one wider matrix
-  const uintptr_t ld = (uintptr_t)(lda * size), at = (x < y ? y - x : x - y) % (ld ? ld : 1), row = (uintptr_t)(E * size);
-  return T > 1 && lda == ldb && at >= row && at + row <= ld;
+  return (a == b && (lda == ldb || T == 1)) || apart({a, T, lda * size, E * size}, {b, T, ldb * size, E * size});
 }
 
 int mk_moe_route_backward(const mk_moe_route_backward_args* a, void* stream) {
@@ -1227,6 +1235,9 @@ int mk_gemm_w4(const mk_gemm_w4_args* a, void* stream) {
   if (!a->A || !a->C) return fail(MK_EINVAL, "mk_gemm_w4: null argument");
   if (!aligned16(a->A)) return fail(MK_EINVAL, "mk_gemm_w4: A must be 16-byte aligned");
   if (!w4_out_aligned(a->C, a->out_type)) return fail(MK_EINVAL, "mk_gemm_w4: C must be aligned to its elements");
+  const int64_t size = a->out_type == 0 ? 4 : 2;
+  if (!apart({a->A, a->M, a->lda * 2, a->W.K * 2}, {a->C, a->M, a->ldc * size, a->W.N * size}))
+    return fail(MK_EINVAL, "mk_gemm_w4: C overlaps A");
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   mk::W4KParams p = w4_params(a->W, a->A, a->C, a->M, a->lda, a->ldc);
@@ -1271,11 +1282,18 @@ static int prepare_grouped_w4(const char* fn, const mk_moe_grouped_gemm_w4_args*
   return MK_OK;
 }
 
+// Whether a checked expert product's result lies apart from what it reads.
+static bool grouped_w4_apart(const mk::W4KParams& p) {
+  const int64_t rows = p.gather_pull ? p.gather_rows : p.M, ldc = p.ldc * (p.out_type == 0 ? 4 : 2);
+  return apart({p.A, rows, p.lda * 2, p.lda * 2}, {p.C, p.M, ldc, ldc});
+}
+
 int mk_moe_grouped_gemm_w4(const mk_moe_grouped_gemm_w4_args* a, void* stream) {
   if (!a) return fail(MK_EINVAL, "mk_moe_grouped_gemm_w4: null argument");
   mk::W4KParams p;
   if (int rc = prepare_grouped_w4("mk_moe_grouped_gemm_w4", a, &p)) return rc;
   if (a->R_pad == 0) return MK_OK;
+  if (!grouped_w4_apart(p)) return fail(MK_EINVAL, "mk_moe_grouped_gemm_w4: out overlaps A");
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   hipError_t e = mk::launch_w4(p, d.cus, static_cast<hipStream_t>(stream));
@@ -1306,6 +1324,12 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* a, void* stream) {
                               a->num_tokens, a->w1.K, a->out_dtype, 1, (uint32_t)a->R_pad};
   if (rows && !aligned16(a->y_expert)) return fail(MK_EINVAL, "%s: y_expert must be 16-byte aligned", fn);
   if (a->num_tokens > 0 && !aligned16(a->y_out)) return fail(MK_EINVAL, "%s: y_out must be 16-byte aligned", fn);
+  if (rows) {
+    const int64_t H = a->w1.K, out = a->out_dtype == 0 ? 4 * H : 2 * H;
+    if (!grouped_w4_apart(p1) || !grouped_w4_apart(p2) ||
+        (a->num_tokens > 0 && !apart({a->y_expert, a->R_pad, 4 * H, 4 * H}, {a->y_out, a->num_tokens, out, out})))
+      return fail(MK_EINVAL, "%s: tokens, act, y_expert and y_out overlap one after the other", fn);
+  }
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from mkernel_amd import ops, workloads as wl
+from mkernel_amd import capi, ops, workloads as wl
 
 pytestmark = pytest.mark.gpu
 D = torch.float64
@@ -500,6 +500,39 @@ def test_outputs_at_odd_places(dev, dtype):
         flat = torch.full((128 * width + 2,), 7.0, dtype=dtype, device=dev)
         got = ops.moe_grouped_gemm_w4(x, p, flat[1:-1].view(128, width), rb)
         assert got.data_ptr() % 16 and torch.equal(got, want) and bool((flat[[0, -1]] == 7).all())
+
+
+def test_result_beside_its_input(dev):
+    """Results in the same memory as their input but apart from it: other columns of the same rows, the rows
+    behind; the layer's output over its tokens.  In place is refused."""
+    _say("results beside inputs")
+    M, K, N = 40, 264, 100
+    w = _weights((K, N), 64, 3, True, True)
+    p, x = _pack(dev, w, 64), _whole((M, K), 1).to(dev)
+    want = ops.gemm_w4(x, p)
+    for first in (True, False):  # out before or behind x in a row
+        rows = torch.full((M, 400), 7.0, dtype=torch.bfloat16, device=dev)
+        a, out = (rows[:, 104:104 + K], rows[:, 1:101]) if first else (rows[:, :K], rows[:, K:K + N])
+        a.copy_(x)
+        assert torch.equal(ops.gemm_w4(a, p, out=out), want) and torch.equal(a, x)
+    flat = torch.full((M * K + M * N,), 7.0, dtype=torch.bfloat16, device=dev)
+    flat[:M * K] = x.view(-1)
+    assert torch.equal(ops.gemm_w4(flat[:M * K].view(M, K), p, out=flat[M * K:].view(M, N)), want)
+    square = _pack(dev, _weights((K, K), 64, 4, False, True), 64)
+    with pytest.raises(capi.MkError, match="overlaps"):
+        ops.gemm_w4(x, square, out=x)
+    T, H, I, E = 9, 64, 32, 4
+    xs, logits, w1, w2 = _layer(dev, T, H, I, E, 0, E, 2, 32, 5)
+    p1, p2, xd = _pack(dev, w1, 32), _pack(dev, w2, 32), xs.to(dev)
+    want, ids, gates = _run_layer(dev, xd, logits.to(dev), p1, p2, 0, E, 2, torch.bfloat16)
+    t = ops.moe_build_indices_dev(ids, gates, 0, E)
+    args = xd, t["pull_indices"], t["row_weight"], t["owner_offset"], t["slot_to_row"], p1, p2
+    act = torch.empty((t["R_pad"], 2 * I), dtype=torch.bfloat16, device=dev)
+    ye = torch.empty((t["R_pad"], H), device=dev)
+    with pytest.raises(capi.MkError, match="overlap"):
+        ops.moe_ffn_combine_w4(*args, act, ye, ye.view(torch.bfloat16).view(-1)[:T * H].view(T, H), t["rb_expert"],
+                               t["rb_rows"])
+    assert torch.equal(ops.moe_ffn_combine_w4(*args, act, ye, xd, t["rb_expert"], t["rb_rows"]), want)
 
 
 def test_no_tokens(dev):

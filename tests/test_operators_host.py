@@ -174,6 +174,27 @@ def test_ffn_w4_scratch_alignment(change):
     _refused("mk_moe_ffn_combine_w4", _args(capi.MoeFfnW4Args, a, change), EINVAL, "16-byte")
 
 
+# A is 4 rows of 512 bytes, C 4 rows of 64 columns
+@pytest.mark.parametrize("change", [
+    dict(C=P), dict(C=P + 1024), dict(C=P + 4 * 512 - 2), dict(C=P - 3 * 128 - 126), dict(C=P + 512, ldc=256),
+    dict(lda=512, ldc=512, C=P + 510), dict(lda=512, ldc=512, C=P + 1024 - 126), dict(lda=512, ldc=256, out_type=0, C=P + 800),
+    dict(M=1, C=P + 510)])
+def test_gemm_w4_overlap(change):
+    """A result that shares elements with A, which other workgroups may still read."""
+    _refused("mk_gemm_w4", _args(capi.GemmW4Args, dict(GEMM, M=4, W=_weights()), change), EINVAL, "overlaps")
+
+
+def test_expert_products_overlap():
+    far = P + (1 << 30)  # never read
+    for change in (dict(out=P), dict(out=P + 128 * 512 - 2), dict(out=P - 128 * 128 + 2), dict(PULL, n_src_rows=2, out=P + 1022)):
+        _refused("mk_moe_grouped_gemm_w4", _args(capi.MoeGroupedGemmW4Args, dict(GROUPED, W=_weights()), change), EINVAL,
+                 "overlaps")
+    for change in (dict(act=P), dict(act=P + 496), dict(act=far, y_expert=far), dict(act=far, y_expert=far + 128 * 128 - 16),
+                   dict(act=far, y_expert=far - 128 * 1024 + 16), dict(act=far, y_expert=2 * far, y_out=2 * far + 1024)):
+        a = dict(FFN, w1=_weights(K=256, N=64), w2=_weights(K=32, N=256))
+        _refused("mk_moe_ffn_combine_w4", _args(capi.MoeFfnW4Args, a, change), EINVAL, "overlap")
+
+
 def test_pack_refusals():
     _refused("mk_w4_pack", _args(capi.W4PackArgs, dict(codes=P, scales=P, zeros=P, out=_weights()), {}), EINVAL, "one side")
     _refused("mk_w4_quantize", _args(capi.W4QuantizeArgs, dict(W=P, codes=P, scales=P, K=8, N=8, group=16, num_experts=1),
