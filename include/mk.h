@@ -568,7 +568,8 @@ int mk_moe_route_backward(const mk_moe_route_backward_args* args, void* stream);
  * R_pad (sizes[1] when sizes is set, R_pad then being the capacity) are
  * neither read nor written; with R_pad 0 every table of rows may be NULL, and
  * dgates is 0.  dy_expert may be NULL, and rb_rows then too; it may be y_expert
- * itself, whose padding rows are then zeroed as well.
+ * itself, whose padding rows are then zeroed as well, but shares no other memory
+ * with y_expert or dy.
  * Each sum is added in a fixed order.  At most 32 choices.  No counterpart in
  * the reference, which has no backward pass. */
 typedef struct mk_moe_combine_backward_args {

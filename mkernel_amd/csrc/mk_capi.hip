@@ -1145,6 +1145,12 @@ int mk_moe_combine_backward(const mk_moe_combine_backward_args* a, void* stream)
     return fail(MK_EINVAL, "mk_moe_combine_backward: null argument");
   if (!aligned16(a->dy) || !aligned16(a->y_expert) || !aligned16(a->dy_expert))
     return fail(MK_EINVAL, "mk_moe_combine_backward: dy, y_expert and dy_expert must be 16-byte aligned");
+  if (rows && a->dy_expert) {
+    const int64_t row = a->H * 2, dy_row = a->dy_dtype == 0 ? 4 * a->H : row;
+    if (!apart_or_same(a->y_expert, a->H, a->dy_expert, a->H, a->R_pad, a->H, 2) ||
+        (a->num_tokens > 0 && !apart({a->dy, a->num_tokens, dy_row, dy_row}, {a->dy_expert, a->R_pad, row, row})))
+      return fail(MK_EINVAL, "mk_moe_combine_backward: dy_expert overlaps dy, or y_expert in part");
+  }
   DevInfo d;
   if (int rc = device_info(&d)) return rc;
   mk::CombineBwdKParams p{a->dy, static_cast<const uint16_t*>(a->y_expert), a->topk_ids, a->row_weight,

@@ -134,6 +134,15 @@ def test_combine_backward_refusals(change, code, match):
     _refused("mk_moe_combine_backward", _args(capi.MoeCombineBackwardArgs, COMBINE, change), code, match)
 
 
+@pytest.mark.parametrize("change", [
+    dict(dy_expert=P + 128 * 128 - 16), dict(dy_expert=P + 16), dict(dy_expert=P - 16), dict(dy=P + (1 << 20), dy_expert=P + (1 << 20)),
+    dict(dy=P + (1 << 20), dy_expert=P + (1 << 20) + 4 * 256 - 16),
+    dict(dy=P + (1 << 20), dy_expert=P + (1 << 20) + 4 * 128 - 16, dy_dtype=1), dict(dy=P, dy_expert=P)])
+def test_combine_backward_overlap(change):
+    """dy_expert over a part of y_expert, or over dy (4 tokens of 64 columns)."""
+    _refused("mk_moe_combine_backward", _args(capi.MoeCombineBackwardArgs, COMBINE, change), EINVAL, "overlaps")
+
+
 def _weights(**change):
     return _args(capi.W4WeightsC, dict(packed=P, K=256, N=64, group=128, num_experts=1), change)
 
