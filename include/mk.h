@@ -629,10 +629,10 @@ typedef struct mk_w4_quantize_args {
 int mk_w4_quantize(const mk_w4_quantize_args* args, void* stream);
 
 /* C[M, N] = A[M, K] @ w (num_experts 1), fp32 sums, bf16 or fp32 output.  For
- * few rows (16 at a time, and the weights expanded for each 16); K % 8 == 0,
- * lda % 8 == 0, A 16-byte aligned; C aligned to its elements, apart from A (it
- * may be other columns of the same rows); any M up to 2^20
- * and any N.  A group's sum is that of
+ * few rows: the weights are expanded for every 16 of them (32 where that leaves
+ * work for every CU).  K % 8 == 0, lda % 8 == 0, A 16-byte aligned; C aligned to
+ * its elements, apart from A (it may be other columns of the same rows); any M
+ * up to 2^20 and any N.  A group's sum is that of
  * A * (16 + code) - A * (16 + zero), exact products: its fp32 roundings are
  * relative to at most 31 times the group's sum of |A|, and an infinity in a row
  * of A, or a group whose |A| sum to more than 2^123, makes that row of C NaN or
@@ -653,8 +653,8 @@ int mk_gemm_w4(const mk_gemm_w4_args* args, void* stream);
  * only the rb_rows real rows of a block are computed, other rows of out stay as
  * they are.  out is fp32, bf16, or a bf16 pair: a row holds its values rounded
  * to bf16 and behind them what the rounding left, again in bf16 (17 bits of
- * significand, so that an activation between two products loses nothing that a
- * bf16 result shows); such rows are read with a_parts 2.  A is 16-byte aligned,
+ * significand: off by 2^-17 of the value at most, a 512th of a bf16 result's
+ * own rounding); such rows are read with a_parts 2.  A is 16-byte aligned,
  * out to its elements, and apart from A.  gather_pull,
  * n_src_rows, tokens_per_src, devs_per_node and sizes as in
  * mk_moe_grouped_gemm_args. */
@@ -677,8 +677,8 @@ int mk_moe_grouped_gemm_w4(const mk_moe_grouped_gemm_w4_args* args, void* stream
 
 /* The local MoE layer with 4-bit expert weights: GEMM1 + SwiGLU (token rows
  * read through the pull table) -> GEMM2 -> combine, three launches.  The
- * activation goes as a bf16 pair and the expert rows in fp32, so y_out is
- * rounded once.  act and y_expert are written on real rows only.  act lies apart
+ * activation goes as a bf16 pair (17 bits) and the expert rows in fp32, so
+ * y_out's is the only rounding to 8 bits.  act and y_expert are written on real rows only.  act lies apart
  * from tokens, y_expert from act, y_out from y_expert (y_out may be tokens). */
 typedef struct mk_moe_ffn_w4_args {
   const void* tokens;           /* bf16 [n_src_rows, H] */

@@ -11,12 +11,16 @@
 // so results do not depend on timing either.
 //
 // What bounds it: a small batch the chain of launch, loads, ranking and stores
-// (1 x 256, 8 choices 3.1 us; 4096 x 256 fp32 with sums 8 and 6 us, gradient 8),
-// a large one the vector instructions: 131001 x 60 bf16, 4 choices, with sums,
-// 13.8 us, 477 of them per 16 tokens, which keep the units busy for four fifths
-// of a wave's life (its 20 MB are 4 us); the sums over workgroups 7.2 us, the
-// gradient 14.3 (447 instructions, and two dependent loads before them).  16384
-// x 256 bf16, 8 choices, without sums: 6.6 us.
+// (1 x 256, 8 choices 3.2 us; 4096 x 256 fp32 with sums 8 to 9 and 6 us, gradient
+// 8; its 128 workgroups leave half of the CUs idle).  A large one, 131001 x 60
+// bf16, 4 choices, with sums, 13.9 us for 20 MB that a copy moves in 4: 477 vector
+// instructions per 16 tokens, whose issue is 7 us and keeps the units busy for 73 %
+// of the waves' life.  The sums over workgroups take 7.1 us, the gradient 14.3 (447
+// instructions, 62 %; its waves wait for two thirds of their life, on the choices'
+// logits, which are loaded after the choices).  fp32 logits take 134 to 138
+// registers where bf16 takes 105, so a CU holds one workgroup of 8 waves with sums
+// instead of two: 131001 x 60 fp32 26.5 us forward and 15.6 back, bf16 19.8 and
+// 12.5 (calls back to back).  16384 x 256 bf16, 8 choices, without sums: 6.6 us.
 #include <algorithm>
 #include <type_traits>
 #include <utility>

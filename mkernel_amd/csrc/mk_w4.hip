@@ -20,13 +20,16 @@
 // of x, and needs that column's scale only.  The waves of a workgroup share a
 // column tile and split K; their sums meet in LDS in wave order.
 //
-// What bounds it: for few rows the weights' bytes.  1 x 8192 x 3584: 5.7 us for
+// What bounds it: for few rows the weights' bytes.  1 x 8192 x 3584: 5.8 us for
 // 15 MB, 3 of them launch and first loads; 64 tokens on 18 experts of 7168 x
-// 4096 (273 MB, not in a cache): 62 us, 4.4 TB/s, where a kernel that only reads
+// 4096 (273 MB, not in a cache): 61 us, 4.5 TB/s, where a kernel that only reads
 // them takes 46.  With more rows a step's instructions beside (128 x 64 weights
-// against 16 rows: 170 vector instructions, two thirds of them the expansion, and
-// 20 MFMAs; against 32 rows 250 and 40): 64 x 3584 x 8192 in 11.2 us is 335
-// TFLOP/s.
+// against 16 rows: 166 to 183 vector instructions, 128 of them the expansion, and
+// 20 MFMAs; against 32 rows 230 to 270 and 40, by group): 64 x 3584 x 8192 in
+// 10.9 us (in a graph) is 345 TFLOP/s.  The expansion is paid once per 16 or 32 rows: bf16
+// weights through mk_gemm are as fast at 128 rows of 3584 x 8192 (19 us) and
+// twice as fast at 1024 (108 and 55); the experts' layer of 7168 / 2048 takes as
+// long as its bf16 form at 1024 tokens (600 us) and twice as long at 4096.
 #include <algorithm>
 #include <type_traits>
 
@@ -327,8 +330,10 @@ __device__ __forceinline__ int block_rows(const W4KParams& p, int64_t b) {
 }
 
 // Waves of a workgroup, and those that a CU holds (by registers): the grid of a
-// launch.  Items of two row tiles with 12 waves spill (64 x 3584 x 8192 12.9 us,
-// with 8 11.2).
+// launch.  Items of two row tiles take 188 to 195 registers in groups of 32 and
+// 64: with 12 waves they spill (64 x 3584 x 8192 12.9 us, with 8 11.2).  In
+// groups of 128 they take 155 to 162, which 12 waves have room for; that was not
+// tried, nor were four row tiles.
 constexpr int group_waves(int nt, int mt) { return nt == 1 || mt == 2 ? 8 : 4; }
 constexpr int waves_per_cu(int nt, int mt) { return nt == 1 ? 16 : mt == 2 ? 8 : 12; }
 
@@ -680,6 +685,7 @@ hipError_t launch_w4(const W4KParams& args, int cus, hipStream_t stream) {
   // (64 x 7168 x 2048) 13.9, 9.3, 11.6; 640 (16 x 4096 x 10240) 12.3, 9.4, 8.6;
   // 1024 (32 x 3584 x 8192) -, 10.3, 8.2, 10.1; 1280 (64 x 3584 x 5120) -, -,
   // 12.2, 10.1; 2048 (64 x 3584 x 8192) -, 16.7, 13.6, 11.2.
+  // (Measured with codes expanded to 128 + q, see expand().)
   const int64_t tiles = (p.M + 15) / 16 * p.tile_cols;
   const int wide = p.rb_expert ? (p.swiglu && p.tile_cols % 2 ? 2 : 4)
                    : p.M <= 4 || tiles <= cus ? 1 : tiles <= 2 * (int64_t)cus ? 2 : 4;
