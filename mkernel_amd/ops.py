@@ -536,7 +536,8 @@ def moe_combine_backward(dy: torch.Tensor, y_expert: torch.Tensor, ids: torch.Te
     combine's output), with the tables of moe_build_indices(_dev)(ids, ...,
     e0, n_local) at row_block 128.  dgates is 0 for experts of other ranks.
     With sizes (moe_build_indices_dev(sync=False)) the rows are a capacity and
-    those behind the routed ones are left as they are."""
+    those behind the routed ones are left as they are.  dy_expert may be
+    y_expert itself, but shares no other memory with y_expert or dy."""
     _tensor(dy, "dy", _LOGITS, dim=2)
     dev = dy.device
     T, H = dy.shape
