@@ -701,6 +701,187 @@ typedef struct mk_moe_ffn_w4_args {
 int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Dense products of any size with what follows them, and their gradients.
+ *
+ * Common to the entry points from here to mk_vocab_loss_backward: bf16
+ * operands, fp32 sums, one rounding at the end.  Any sizes and row strides (of
+ * at least the row's width, at most 2^21 elements); operands aligned to their
+ * elements.  Operands whose rows do not start at 16-byte boundaries, or whose
+ * rows' ends do not fill 16 bytes where the sum runs along them, are laid out
+ * anew in the workspace first.  Results may not overlap what is read, unless
+ * said otherwise.  Sums are added in an order that depends on sizes alone.
+ * `workspace`: mk_*_workspace_bytes(args) bytes, 16-byte aligned, holding
+ * nothing between calls (the pointers in args have to be set for the question,
+ * the workspace's own need not).  `tickets`: MK_PRODUCT_TICKETS 32-bit words,
+ * zero before their first use, left zero by every call; launches that share
+ * them must be ordered. */
+#define MK_PRODUCT_TICKETS 1024
+
+#define MK_ACT_NONE 0
+#define MK_ACT_RELU 1
+#define MK_ACT_GELU 2      /* x * Phi(x) */
+#define MK_ACT_GELU_TANH 3 /* x/2 * (1 + tanh(sqrt(2/pi) * (x + 0.044715 x^3))) */
+#define MK_ACT_SILU 4      /* x / (1 + e^-x) */
+
+/* C = act(A @ B + bias) + residual; pre, where set, gets A @ B + bias (bf16) for
+ * the backward pass.  residual may be C itself (same type and stride).  From one
+ * row (K is then cut into parts that fill the chip) to any number. */
+typedef struct mk_gemm_act_args {
+  const void* A;         /* bf16 [M, lda] */
+  const void* B;         /* bf16 [K, ldb] */
+  void* C;               /* [M, ldc] */
+  const void* bias;      /* [N] or NULL */
+  const void* residual;  /* [M, ldr] or NULL */
+  void* pre;             /* bf16 [M, ldp] or NULL */
+  int64_t M, N, K;
+  int64_t lda, ldb, ldc, ldr, ldp;
+  int32_t act;           /* MK_ACT_* */
+  int32_t c_type, bias_type, residual_type; /* 0 fp32, 1 bf16 */
+  void* workspace;
+  int64_t workspace_bytes;
+  void* tickets;
+} mk_gemm_act_args;
+int64_t mk_gemm_act_workspace_bytes(const mk_gemm_act_args* args);
+int mk_gemm_act(const mk_gemm_act_args* args, void* stream);
+
+/* Gradients of mk_gemm_act (the residual's is dC itself): with
+ * dpre = dC * act'(pre),
+ *   dA = dpre @ B^T (bf16),  dB = A^T @ dpre,  dbias = column sums of dpre (fp32).
+ * Each of the three may be NULL.  pre is needed with an activation; dpre is then
+ * rounded to bf16 for the two products (matrix cores take nothing wider at their
+ * rate; dA and dB are off by about 1.4 of their own rounding), not for dbias.
+ * accumulate: dB and dbias are added to what they hold (gradients of several
+ * batches). */
+typedef struct mk_gemm_act_backward_args {
+  const void* dC;        /* bf16 [M, lddc] */
+  const void* A;         /* bf16 [M, lda]; needed for dB */
+  const void* B;         /* bf16 [K, ldb]; needed for dA */
+  const void* pre;       /* bf16 [M, ldp]; NULL with MK_ACT_NONE */
+  void* dA;              /* bf16 [M, ldda] or NULL */
+  void* dB;              /* [K, lddb] or NULL */
+  float* dbias;          /* [N] or NULL */
+  int64_t M, N, K;
+  int64_t lddc, lda, ldb, ldp, ldda, lddb;
+  int32_t act, db_type;  /* db_type 0 fp32, 1 bf16 */
+  int32_t accumulate;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* tickets;
+} mk_gemm_act_backward_args;
+int64_t mk_gemm_act_backward_workspace_bytes(const mk_gemm_act_backward_args* args);
+int mk_gemm_act_backward(const mk_gemm_act_backward_args* args, void* stream);
+
+/* Expert products on ragged rows: the rows of expert e are the counts[e] rows
+ * behind those of the experts before it (padded_tokens_per_expert of an index
+ * build, at row_block 1 or any other).  Counts are read on the device; below 0
+ * they count as 0, and rows from R on, which the counts may name, are not there.
+ * Rows behind the last expert's are neither read nor written, whatever they hold.
+ *   mode 0: out[r] = A[r] @ W[e]                        (out [R, N])
+ *   mode 1: out[r] = silu(g) * u, (g | u) = A[r] @ W[e] (out [R, N/2]), and h,
+ *           where set, gets (g | u) in bf16 [R, N] for the backward pass. */
+typedef struct mk_moe_ragged_gemm_args {
+  const void* A;          /* bf16 [R, lda] */
+  const void* W;          /* bf16 [E, K, N] */
+  const int32_t* counts;  /* [E] */
+  void* out;              /* bf16 [R, ldo] */
+  void* h;                /* bf16 [R, ldh] or NULL */
+  int64_t R, K, N;
+  int64_t lda, ldo, ldh;
+  int32_t num_experts, mode;
+  void* workspace;
+  int64_t workspace_bytes;
+} mk_moe_ragged_gemm_args;
+int64_t mk_moe_ragged_gemm_workspace_bytes(const mk_moe_ragged_gemm_args* args);
+int mk_moe_ragged_gemm(const mk_moe_ragged_gemm_args* args, void* stream);
+
+/* Gradient of the rows: dA[r] = dy[r] @ W[e]^T ([R, K]); with h (that product's
+ * A was silu(g) * u of it, h = (g | u) [R, 2K] as mode 1 gave it) the gradient of
+ * h instead: out = dh [R, 2K], in one pass.  out may be h. */
+typedef struct mk_moe_ragged_dgrad_args {
+  const void* dy;         /* bf16 [R, lddy] */
+  const void* W;          /* bf16 [E, K, N] */
+  const int32_t* counts;  /* [E] */
+  const void* h;          /* bf16 [R, ldh] or NULL */
+  void* out;              /* bf16 [R, ldo] */
+  int64_t R, K, N;
+  int64_t lddy, ldh, ldo;
+  int32_t num_experts;
+  void* workspace;
+  int64_t workspace_bytes;
+} mk_moe_ragged_dgrad_args;
+int64_t mk_moe_ragged_dgrad_workspace_bytes(const mk_moe_ragged_dgrad_args* args);
+int mk_moe_ragged_dgrad(const mk_moe_ragged_dgrad_args* args, void* stream);
+
+/* Gradient of the weights: dW[e] = A_e^T @ dy_e, zeros for an expert without
+ * rows; accumulate: added to what dW holds. */
+typedef struct mk_moe_ragged_wgrad_args {
+  const void* A;          /* bf16 [R, lda] */
+  const void* dy;         /* bf16 [R, lddy] */
+  const int32_t* counts;  /* [E] */
+  void* dW;               /* [E, K, N] */
+  int64_t R, K, N;
+  int64_t lda, lddy;
+  int32_t num_experts;
+  int32_t dw_type;        /* 0 fp32, 1 bf16 */
+  int32_t accumulate;
+  void* workspace;
+  int64_t workspace_bytes;
+} mk_moe_ragged_wgrad_args;
+int64_t mk_moe_ragged_wgrad_workspace_bytes(const mk_moe_ragged_wgrad_args* args);
+int mk_moe_ragged_wgrad(const mk_moe_ragged_wgrad_args* args, void* stream);
+
+/* Cross entropy over a vocabulary, or one rank's shard [vocab_begin,
+ * vocab_begin + V) of it, without keeping the logits x @ W: per token
+ *   lse = log sum_v e^logit,  target = the label's logit (0 where another shard
+ *   has it),  loss = lse - target.
+ * Shards are joined by lse = log sum e^lse_i and the sum of the targets.  Tokens
+ * whose label is ignore_index have zeros in all three, whatever their x holds. */
+typedef struct mk_vocab_loss_args {
+  const void* x;          /* bf16 [T, ldx] */
+  const void* W;          /* bf16 [H, ldw] */
+  const void* labels;     /* [T] int32 or int64 */
+  float* lse;             /* [T] */
+  float* target;          /* [T] */
+  float* loss;            /* [T] or NULL */
+  int64_t T, H, V;
+  int64_t ldx, ldw;
+  int64_t vocab_begin, ignore_index;
+  int32_t labels_type;    /* 0 int32, 1 int64 */
+  void* workspace;
+  int64_t workspace_bytes;
+  void* tickets;
+} mk_vocab_loss_args;
+int64_t mk_vocab_loss_workspace_bytes(const mk_vocab_loss_args* args);
+int mk_vocab_loss(const mk_vocab_loss_args* args, void* stream);
+
+/* Gradients: with dl = (e^(logit - lse) - [v = label]) * dloss (lse over all
+ * shards), 0 for ignored tokens,
+ *   dx = dl @ W^T (of a shard: its part of the sum),  dW = x^T @ dl.
+ * Logits are computed anew, a piece of the vocabulary at a time (piece_columns, a
+ * multiple of 256; 0: the library's choice), dl goes through the workspace in
+ * bf16.  Either result may be NULL; accumulate: dW is added to. */
+typedef struct mk_vocab_loss_backward_args {
+  const void* x;          /* bf16 [T, ldx] */
+  const void* W;          /* bf16 [H, ldw] */
+  const void* labels;
+  const float* lse;       /* [T] */
+  const float* dloss;     /* [T] */
+  void* dx;               /* [T, lddx] or NULL */
+  void* dW;               /* [H, lddw] or NULL */
+  int64_t T, H, V;
+  int64_t ldx, ldw, lddx, lddw;
+  int64_t vocab_begin, ignore_index;
+  int64_t piece_columns;
+  int32_t labels_type, dx_type, dw_type; /* types 0 fp32, 1 bf16 */
+  int32_t accumulate;
+  void* workspace;
+  int64_t workspace_bytes;
+  void* tickets;
+} mk_vocab_loss_backward_args;
+int64_t mk_vocab_loss_backward_workspace_bytes(const mk_vocab_loss_backward_args* args);
+int mk_vocab_loss_backward(const mk_vocab_loss_backward_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* K-split workspace size.  When the output tiles do not fill the last round
  * of the persistent grid (tiles % compute workgroups != 0), the GEMM entry
  * points split each tile of that tail round along K over 2-4 workgroups;

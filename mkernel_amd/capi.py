@@ -44,6 +44,20 @@ EXPORTS = (
     "mk_gemm_w4",
     "mk_moe_grouped_gemm_w4",
     "mk_moe_ffn_combine_w4",
+    "mk_gemm_act_workspace_bytes",
+    "mk_gemm_act",
+    "mk_gemm_act_backward_workspace_bytes",
+    "mk_gemm_act_backward",
+    "mk_moe_ragged_gemm_workspace_bytes",
+    "mk_moe_ragged_gemm",
+    "mk_moe_ragged_dgrad_workspace_bytes",
+    "mk_moe_ragged_dgrad",
+    "mk_moe_ragged_wgrad_workspace_bytes",
+    "mk_moe_ragged_wgrad",
+    "mk_vocab_loss_workspace_bytes",
+    "mk_vocab_loss",
+    "mk_vocab_loss_backward_workspace_bytes",
+    "mk_vocab_loss_backward",
     "mk_query_workspace_bytes",
     "mk_probe_mfma_ceiling",
     "mk_probe_threads",
@@ -52,6 +66,12 @@ EXPORTS = (
     "mk_abi_version",
     "mk_epoch_advance",
 )
+
+# entry points with a workspace of mk_..._workspace_bytes(args) bytes
+_PRODUCTS = ("mk_gemm_act", "mk_gemm_act_backward", "mk_moe_ragged_gemm", "mk_moe_ragged_dgrad", "mk_moe_ragged_wgrad",
+             "mk_vocab_loss", "mk_vocab_loss_backward")
+PRODUCT_TICKETS = 1024  # include/mk.h MK_PRODUCT_TICKETS
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # MK_ACT_*
 
 vp = C.c_void_p
 i64 = C.c_int64
@@ -192,6 +212,52 @@ class MoeGroupedGemmW4Args(C.Structure):
                 ("tokens_per_src", i32), ("devs_per_node", i32), ("sizes", vp)]
 
 
+class GemmActArgs(C.Structure):
+    _fields_ = [("A", vp), ("B", vp), ("C", vp), ("bias", vp), ("residual", vp), ("pre", vp), ("M", i64), ("N", i64),
+                ("K", i64), ("lda", i64), ("ldb", i64), ("ldc", i64), ("ldr", i64), ("ldp", i64), ("act", i32),
+                ("c_type", i32), ("bias_type", i32), ("residual_type", i32), ("workspace", vp),
+                ("workspace_bytes", i64), ("tickets", vp)]
+
+
+class GemmActBackwardArgs(C.Structure):
+    _fields_ = [("dC", vp), ("A", vp), ("B", vp), ("pre", vp), ("dA", vp), ("dB", vp), ("dbias", vp), ("M", i64),
+                ("N", i64), ("K", i64), ("lddc", i64), ("lda", i64), ("ldb", i64), ("ldp", i64), ("ldda", i64),
+                ("lddb", i64), ("act", i32), ("db_type", i32), ("accumulate", i32), ("workspace", vp),
+                ("workspace_bytes", i64), ("tickets", vp)]
+
+
+class MoeRaggedGemmArgs(C.Structure):
+    _fields_ = [("A", vp), ("W", vp), ("counts", vp), ("out", vp), ("h", vp), ("R", i64), ("K", i64), ("N", i64),
+                ("lda", i64), ("ldo", i64), ("ldh", i64), ("num_experts", i32), ("mode", i32), ("workspace", vp),
+                ("workspace_bytes", i64)]
+
+
+class MoeRaggedDgradArgs(C.Structure):
+    _fields_ = [("dy", vp), ("W", vp), ("counts", vp), ("h", vp), ("out", vp), ("R", i64), ("K", i64), ("N", i64),
+                ("lddy", i64), ("ldh", i64), ("ldo", i64), ("num_experts", i32), ("workspace", vp),
+                ("workspace_bytes", i64)]
+
+
+class MoeRaggedWgradArgs(C.Structure):
+    _fields_ = [("A", vp), ("dy", vp), ("counts", vp), ("dW", vp), ("R", i64), ("K", i64), ("N", i64), ("lda", i64),
+                ("lddy", i64), ("num_experts", i32), ("dw_type", i32), ("accumulate", i32), ("workspace", vp),
+                ("workspace_bytes", i64)]
+
+
+class VocabLossArgs(C.Structure):
+    _fields_ = [("x", vp), ("W", vp), ("labels", vp), ("lse", vp), ("target", vp), ("loss", vp), ("T", i64),
+                ("H", i64), ("V", i64), ("ldx", i64), ("ldw", i64), ("vocab_begin", i64), ("ignore_index", i64),
+                ("labels_type", i32), ("workspace", vp), ("workspace_bytes", i64), ("tickets", vp)]
+
+
+class VocabLossBackwardArgs(C.Structure):
+    _fields_ = [("x", vp), ("W", vp), ("labels", vp), ("lse", vp), ("dloss", vp), ("dx", vp), ("dW", vp), ("T", i64),
+                ("H", i64), ("V", i64), ("ldx", i64), ("ldw", i64), ("lddx", i64), ("lddw", i64),
+                ("vocab_begin", i64), ("ignore_index", i64), ("piece_columns", i64), ("labels_type", i32),
+                ("dx_type", i32), ("dw_type", i32), ("accumulate", i32), ("workspace", vp),
+                ("workspace_bytes", i64), ("tickets", vp)]
+
+
 class MoeFfnW4Args(C.Structure):
     _fields_ = [("tokens", vp), ("pull_indices", vp), ("rb_expert", vp), ("rb_rows", vp), ("row_weight", vp),
                 ("owner_offset", vp), ("slot_to_row", vp), ("w1", W4WeightsC), ("w2", W4WeightsC), ("act", vp),
@@ -213,9 +279,12 @@ def lib() -> C.CDLL:
         for name in ("mk_gemm", "mk_ag_gemm", "mk_ag_gemm_noalloc", "mk_gemm_rs", "mk_gemm_ar", "mk_gemm_ar_two_shot", "mk_moe_permute", "mk_moe_grouped_gemm",
                      "mk_moe_combine", "mk_moe_ffn_combine", "mk_moe_route", "mk_moe_route_backward",
                      "mk_moe_combine_backward", "mk_w4_pack", "mk_w4_quantize", "mk_gemm_w4",
-                     "mk_moe_grouped_gemm_w4", "mk_moe_ffn_combine_w4"):
+                     "mk_moe_grouped_gemm_w4", "mk_moe_ffn_combine_w4", *_PRODUCTS):
             getattr(L, name).argtypes = [vp, vp]
             getattr(L, name).restype = C.c_int
+        for name in _PRODUCTS:
+            getattr(L, name + "_workspace_bytes").argtypes = [vp]
+            getattr(L, name + "_workspace_bytes").restype = i64
         L.mk_moe_index_sizes.argtypes = [vp, i32, i32, i32, i32, i32, C.POINTER(i64), C.POINTER(i64)]
         L.mk_moe_index_sizes.restype = C.c_int
         L.mk_moe_build_indices.argtypes = [vp, vp, i32, i32, i32, i32, i32, C.POINTER(MoeIndex)]
@@ -311,3 +380,17 @@ def call_values(fn: str, cls, stream: int, *values) -> None:
     rc = f(args, stream or None)
     if rc:
         check(fn, rc)
+
+
+def workspace_bytes(fn: str, cls, *values) -> int:
+    """What fn's workspace has to hold for these arguments (without the
+    workspace's own, which come last)."""
+    key = fn + "_workspace_bytes"
+    f = _functions.get(key)
+    if f is None:
+        f = _functions[key] = getattr(lib(), key)
+    pack = _packers.get(cls) or _packer(cls)
+    n = f(pack(*values, *(0,) * (len(cls._fields_) - len(values))))
+    if n < 0:
+        raise MkError(fn, int(n), lib().mk_last_error_string().decode())
+    return n

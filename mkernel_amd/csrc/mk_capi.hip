@@ -1347,3 +1347,619 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* a, void* stream) {
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Products with what follows them (mk_product.h)
+// ---------------------------------------------------------------------------
+namespace {
+
+constexpr int64_t kMaxLd = 1 << 21, kMaxRows = 1 << 30;
+
+// The pieces of a workspace, one behind the other.  A call's body runs twice:
+// once to count (nothing is queued), once to work.
+struct Space {
+  char* base = nullptr;
+  bool counting = true;
+  int64_t used = 0, peak = 0;
+  void* take(int64_t bytes) {
+    const int64_t at = used;
+    used += (bytes + 255) / 256 * 256;
+    peak = std::max(peak, used);
+    return counting ? nullptr : base + at;
+  }
+};
+
+template <class F>
+int64_t count_space(F body) {
+  Space sp;
+  const int rc = body(sp);
+  return rc ? -1 : sp.peak;
+}
+
+template <class F>
+int with_space(const char* fn, void* ws, int64_t bytes, F body) {
+  Space sp;
+  if (int rc = body(sp)) return rc;
+  if (sp.peak > 0 && (!ws || bytes < sp.peak))
+    return fail(MK_EINVAL, "%s: the workspace must hold %lld bytes", fn, (long long)sp.peak);
+  if (!aligned16(ws)) return fail(MK_EINVAL, "%s: the workspace must be 16-byte aligned", fn);
+  Space work;
+  work.base = static_cast<char*>(ws);
+  work.counting = false;
+  return body(work);
+}
+
+struct Products {
+  const char* fn;
+  Space& sp;
+  int cus;
+  uint32_t* tickets;  // null: no K is cut
+  hipStream_t stream;
+
+  int launched(hipError_t e) const { return e == hipSuccess ? MK_OK : hip_fail(e, fn); }
+
+  // One product; b_cols: columns of B that its tiles cover (SwiGLU: gate and up).
+  int run(int order, int epi, mk::ProductParams p, int64_t tile_cols, int* tile = nullptr) {
+    if (p.M == 0 || p.N == 0) return MK_OK;
+    const int groups = p.ragged ? p.E : 1;
+    const mk::ProductPlan plan =
+        mk::plan_product(p.M, tile_cols, p.K, groups, p.ragged, order == mk::kProdRightGrad, tickets != nullptr, cus);
+    if (tile) *tile = plan.tile;
+    const mk::ProductShape& s = mk::kProductShapes[plan.tile];
+    p.split = plan.split;
+    p.group_m = 8;
+    p.tickets = tickets;
+    const int bn = epi == mk::kProdSwiglu ? s.bn / 2 : s.bn;
+    const int64_t tn = (p.N + bn - 1) / bn, tm = (p.M + s.bm - 1) / s.bm;
+    // of ragged rows at most: each group's last tile may hold one row
+    const int64_t tiles = (p.ragged == 1 ? std::min(tm + groups - 1, p.M) : tm) * tn * (p.ragged == 2 ? groups : 1);
+    if (tiles * p.split >= (1LL << 31)) return fail(MK_ESHAPE, "%s: too many tiles", fn);
+    p.tiles_m = (int)tm;
+    p.tiles_n = (int)tn;
+    const int64_t mark = sp.used;
+    if (p.split > 1) p.parts = static_cast<float*>(sp.take(tiles * p.split * s.bm * s.bn * 4));
+    sp.used = mark;  // the next launch may use them again
+    if (sp.counting) return MK_OK;
+    const int64_t grid = tiles * p.split;
+    return launched(order == mk::kProdForward    ? mk::launch_product_forward(p, epi, plan.tile, grid, stream)
+                    : order == mk::kProdLeftGrad ? mk::launch_product_left_grad(p, epi, plan.tile, grid, stream)
+                                                 : mk::launch_product_right_grad(p, plan.tile, grid, stream));
+  }
+
+  // Rows as an operand takes them: 16-byte aligned; `whole`: ending with a unit or zeros (k-contiguous operands).
+  // Laid out anew where they are not; groups of `rows` rows each, `stride` apart, in `parts` pieces of columns.
+  int rows(const uint16_t*& src, int64_t n, int64_t cols, int64_t& ld, bool whole, int groups = 1, int64_t* stride = nullptr,
+           const int* counts = nullptr, int parts = 1) {
+    if (n == 1) ld = (cols + 7) / 8 * 8;
+    const int64_t piece = cols / parts;
+    if (aligned16(src) && ld % 8 == 0 && (!whole || cols % 8 == 0) && (parts == 1 || piece % 8 == 0) &&
+        (!stride || groups == 1 || *stride % 8 == 0))
+      return MK_OK;
+    mk::RepackParams r = {};
+    r.src = src;
+    r.rows = n;
+    r.cols = piece;
+    r.ld = n == 1 ? cols : ld;
+    r.width = (piece + 7) / 8 * 8;
+    r.parts = parts;
+    r.src_stride = stride ? *stride : 0;
+    ld = r.width * parts;
+    r.dst_stride = n * ld;
+    r.E = groups;
+    r.counts = counts;
+    r.dst = static_cast<uint16_t*>(sp.take(groups * r.dst_stride * 2));
+    if (stride) *stride = r.dst_stride;
+    src = r.dst;
+    return sp.counting ? MK_OK : launched(mk::launch_repack(r, stream));
+  }
+};
+
+bool vec_rows(const void* p, int64_t ld, int type) { return aligned16(p) && ld % (type == 0 ? 4 : 8) == 0; }
+
+const uint16_t* u16(const void* p) { return static_cast<const uint16_t*>(p); }
+
+// Row strides of at least the width and at most kMaxLd, the pointer aligned to its elements.
+int check_rows(const char* fn, const char* name, const void* p, int64_t rows, int64_t width, int64_t ld, int size) {
+  if (rows == 0 || width == 0) return MK_OK;
+  if (!p) return fail(MK_EINVAL, "%s: %s is null", fn, name);
+  if (ld < width || ld > kMaxLd)
+    return fail(MK_ESHAPE, "%s: rows of %s must be %lld to %lld elements apart", fn, name, (long long)width, (long long)kMaxLd);
+  if (reinterpret_cast<uintptr_t>(p) % size) return fail(MK_EINVAL, "%s: %s must be aligned to its elements", fn, name);
+  return MK_OK;
+}
+
+int check_sizes(const char* fn, int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 0 || M > kMaxRows || N > kMaxLd || K > kMaxRows)
+    return fail(MK_ESHAPE, "%s: bad sizes (%lld x %lld x %lld)", fn, (long long)M, (long long)N, (long long)K);
+  return MK_OK;
+}
+
+bool is_type(int t) { return t == 0 || t == 1; }
+int size_of(int t) { return t == 0 ? 4 : 2; }
+
+struct Matrix {
+  const char* name;
+  const void* p;
+  int64_t rows, width, ld;  // elements
+  int size;
+  bool empty() const { return !p || rows <= 0 || width <= 0; }
+  ByteRows bytes() const { return {p, rows, ld * size, width * size}; }
+};
+
+// Every matrix has fitting rows, and results lie apart from everything else (`same`: pairs that may be one and the same).
+int check_matrices(const char* fn, std::initializer_list<Matrix> in, std::initializer_list<Matrix> out,
+                   const void* same_in = nullptr, const void* same_out = nullptr) {
+  for (const Matrix& m : in)
+    if (int rc = check_rows(fn, m.name, m.p, m.rows, m.width, m.ld, m.size)) return rc;
+  for (const Matrix& m : out)
+    if (int rc = check_rows(fn, m.name, m.p, m.rows, m.width, m.ld, m.size)) return rc;
+  for (const Matrix* o = out.begin(); o != out.end(); ++o) {
+    if (o->empty()) continue;
+    for (const Matrix& m : in) {
+      if (m.empty() || apart(m.bytes(), o->bytes())) continue;
+      if (m.p == same_in && o->p == same_out && m.p == o->p && m.size == o->size && (m.ld == o->ld || m.rows == 1)) continue;
+      return fail(MK_EINVAL, "%s: %s overlaps %s", fn, o->name, m.name);
+    }
+    for (const Matrix* q = out.begin(); q != o; ++q)
+      if (!q->empty() && !apart(q->bytes(), o->bytes())) return fail(MK_EINVAL, "%s: %s overlaps %s", fn, o->name, q->name);
+  }
+  return MK_OK;
+}
+
+// ---- C = act(A @ B + bias) + residual ----
+
+int check_gemm_act(const char* fn, const mk_gemm_act_args* a) {
+  if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
+  if (int rc = check_sizes(fn, a->M, a->N, a->K)) return rc;
+  if (a->act < 0 || a->act > MK_ACT_SILU) return fail(MK_EINVAL, "%s: act must be 0 .. %d", fn, MK_ACT_SILU);
+  if (!is_type(a->c_type) || !is_type(a->bias_type) || !is_type(a->residual_type))
+    return fail(MK_EINVAL, "%s: types must be 0 or 1", fn);
+  const bool res = a->residual, pre = a->pre;
+  return check_matrices(fn,
+                        {{"A", a->A, a->M, a->K, a->lda, 2},
+                         {"B", a->B, a->K, a->N, a->ldb, 2},
+                         {"bias", a->bias, a->bias ? 1 : 0, a->N, a->N, size_of(a->bias_type)},
+                         {"residual", a->residual, res ? a->M : 0, a->N, a->ldr, size_of(a->residual_type)}},
+                        {{"C", a->C, a->M, a->N, a->ldc, size_of(a->c_type)}, {"pre", a->pre, pre ? a->M : 0, a->N, a->ldp, 2}},
+                        a->residual, a->C);
+}
+
+int gemm_act_body(const mk_gemm_act_args* a, Products g) {
+  if (a->M == 0 || a->N == 0) return MK_OK;
+  mk::ProductParams p = {};
+  p.A = u16(a->A); p.B = u16(a->B);
+  p.lda = a->lda; p.ldb = a->ldb;
+  p.M = a->M; p.N = a->N; p.K = a->K; p.b_cols = a->N;
+  if (a->K > 0) {
+    if (int rc = g.rows(p.A, a->M, a->K, p.lda, true)) return rc;
+    if (int rc = g.rows(p.B, a->K, a->N, p.ldb, false)) return rc;
+  }
+  p.act = a->act;
+  p.C = a->C; p.ldc = a->ldc; p.c_f32 = a->c_type == 0;
+  p.bias = a->bias; p.bias_f32 = a->bias_type == 0;
+  p.res = a->residual; p.ldr = a->ldr; p.res_f32 = a->residual_type == 0;
+  p.pre = static_cast<uint16_t*>(a->pre); p.ldp = a->ldp;
+  p.vec = (vec_rows(a->C, a->ldc, a->c_type) ? mk::kVecC : 0) | (vec_rows(a->residual, a->ldr, a->residual_type) ? mk::kVecRes : 0) |
+          (vec_rows(a->pre, a->ldp, 1) ? mk::kVecPre : 0) | (aligned16(a->bias) ? mk::kVecBias : 0);
+  return g.run(mk::kProdForward, mk::kProdStore, p, a->N);
+}
+
+// ---- its gradients ----
+
+int check_gemm_act_backward(const char* fn, const mk_gemm_act_backward_args* a) {
+  if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
+  if (int rc = check_sizes(fn, a->M, a->N, a->K)) return rc;
+  if (a->act < 0 || a->act > MK_ACT_SILU) return fail(MK_EINVAL, "%s: act must be 0 .. %d", fn, MK_ACT_SILU);
+  if (!is_type(a->db_type)) return fail(MK_EINVAL, "%s: db_type must be 0 or 1", fn);
+  if (!a->dA && !a->dB && !a->dbias) return fail(MK_EINVAL, "%s: dA, dB or dbias must be set", fn);
+  const bool act = a->act != MK_ACT_NONE, da = a->dA, db = a->dB;
+  return check_matrices(fn,
+                        {{"dC", a->dC, a->M, a->N, a->lddc, 2},
+                         {"A", a->A, db ? a->M : 0, a->K, a->lda, 2},
+                         {"B", a->B, da ? a->K : 0, a->N, a->ldb, 2},
+                         {"pre", a->pre, act ? a->M : 0, a->N, a->ldp, 2}},
+                        {{"dA", a->dA, da ? a->M : 0, a->K, a->ldda, 2},
+                         {"dB", a->dB, db ? a->K : 0, a->N, a->lddb, size_of(a->db_type)},
+                         {"dbias", a->dbias, a->dbias ? 1 : 0, a->N, a->N, 4}});
+}
+
+int gemm_act_backward_body(const mk_gemm_act_backward_args* a, Products g) {
+  const uint16_t* d = u16(a->dC);
+  int64_t ldd = a->M == 1 ? (a->N + 7) / 8 * 8 : a->lddc;
+  const bool act = a->act != MK_ACT_NONE;
+  // both products read dpre's rows, one of them along the sum
+  const bool copy = (a->dA || a->dB) && (act || !aligned16(d) || ldd % 8 || a->N % 8);
+  if (copy || a->dbias) {
+    mk::ActGradParams p = {};
+    p.dC = d; p.ldc = a->lddc; p.vec_c = vec_rows(d, a->lddc, 1);
+    p.pre = u16(a->pre); p.ldp = a->ldp; p.vec_p = vec_rows(a->pre, a->ldp, 1);
+    p.M = a->M; p.N = a->N; p.act = a->act;
+    p.row_blocks = mk::act_grad_blocks(a->M, a->N);
+    if (copy) {
+      ldd = p.width = (a->N + 7) / 8 * 8;
+      d = p.dpre = static_cast<uint16_t*>(g.sp.take(a->M * p.width * 2));
+    }
+    if (a->dbias) {
+      p.part = static_cast<float*>(g.sp.take(p.row_blocks * a->N * 4));
+      p.dbias = a->dbias;
+      p.accumulate = a->accumulate;
+    }
+    if (!g.sp.counting)
+      if (int rc = g.launched(mk::launch_act_grad(p, g.stream))) return rc;
+  }
+  if (a->dA) {
+    mk::ProductParams p = {};
+    p.A = d; p.lda = ldd;
+    p.B = u16(a->B); p.ldb = a->ldb;
+    p.M = a->M; p.N = a->K; p.K = a->N;
+    if (a->M > 0 && a->N > 0)
+      if (int rc = g.rows(p.B, a->K, a->N, p.ldb, true)) return rc;
+    p.C = a->dA; p.ldc = a->ldda;
+    p.vec = vec_rows(a->dA, a->ldda, 1) ? mk::kVecC : 0;
+    if (int rc = g.run(mk::kProdLeftGrad, mk::kProdStore, p, a->K)) return rc;
+  }
+  if (a->dB) {
+    mk::ProductParams p = {};
+    p.A = u16(a->A); p.lda = a->lda;
+    p.B = d; p.ldb = ldd; p.b_cols = a->N;
+    p.M = a->K; p.N = a->N; p.K = a->M;
+    if (a->M > 0 && a->N > 0)
+      if (int rc = g.rows(p.A, a->M, a->K, p.lda, false)) return rc;
+    p.C = a->dB; p.ldc = a->lddb; p.c_f32 = a->db_type == 0;
+    p.vec = vec_rows(a->dB, a->lddb, a->db_type) ? mk::kVecC | mk::kVecRes : 0;
+    if (a->accumulate) {
+      p.res = a->dB; p.ldr = a->lddb; p.res_f32 = p.c_f32;
+    }
+    if (int rc = g.run(mk::kProdRightGrad, mk::kProdStore, p, a->N)) return rc;
+  }
+  return MK_OK;
+}
+
+// ---- expert products on ragged rows ----
+
+int check_ragged(const char* fn, int64_t R, int64_t K, int64_t N, int32_t E, const void* counts) {
+  if (int rc = check_sizes(fn, R, N, K)) return rc;
+  if (K == 0 || N == 0 || K > kMaxLd) return fail(MK_ESHAPE, "%s: K and N must be 1 .. %lld", fn, (long long)kMaxLd);
+  if (E <= 0 || E > mk::kMaxExperts) return fail(MK_ESHAPE, "%s: 1 .. %d experts", fn, mk::kMaxExperts);
+  if (!counts) return fail(MK_EINVAL, "%s: counts is null", fn);
+  return MK_OK;
+}
+
+int check_ragged_gemm(const char* fn, const mk_moe_ragged_gemm_args* a) {
+  if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
+  if (a->mode != 0 && a->mode != 1) return fail(MK_EINVAL, "%s: mode must be 0 or 1", fn);
+  if (int rc = check_ragged(fn, a->R, a->K, a->N, a->num_experts, a->counts)) return rc;
+  if (a->mode == 1 && a->N % 2) return fail(MK_ESHAPE, "%s: N must be even with SwiGLU", fn);
+  if (a->mode == 0 && a->h) return fail(MK_EINVAL, "%s: h belongs to mode 1", fn);
+  return check_matrices(fn, {{"A", a->A, a->R, a->K, a->lda, 2}, {"W", a->W, a->num_experts * a->K, a->N, a->N, 2}},
+                        {{"out", a->out, a->R, a->mode ? a->N / 2 : a->N, a->ldo, 2}, {"h", a->h, a->h ? a->R : 0, a->N, a->ldh, 2}});
+}
+
+int ragged_gemm_body(const mk_moe_ragged_gemm_args* a, Products g) {
+  if (a->R == 0) return MK_OK;
+  mk::ProductParams p = {};
+  p.A = u16(a->A); p.lda = a->lda;
+  p.B = u16(a->W); p.ldb = a->N; p.b_stride = a->K * a->N;
+  p.M = a->R; p.K = a->K;
+  p.counts = a->counts; p.E = a->num_experts; p.ragged = 1;
+  if (int rc = g.rows(p.A, a->R, a->K, p.lda, true)) return rc;
+  if (int rc = g.rows(p.B, a->K, a->N, p.ldb, false, a->num_experts, &p.b_stride, a->counts, a->mode ? 2 : 1)) return rc;
+  p.b_cols = p.ldb;
+  p.C = a->out; p.ldc = a->ldo;
+  p.vec = vec_rows(a->out, a->ldo, 1) ? mk::kVecC : 0;
+  if (a->mode == 0) {
+    p.N = p.b_cols = a->N;
+    return g.run(mk::kProdForward, mk::kProdStore, p, a->N);
+  }
+  p.N = a->N / 2;
+  p.up = (int)(p.b_cols / 2);  // as the rows lie: behind the gates, or where they were laid out anew
+  p.pre = static_cast<uint16_t*>(a->h); p.ldp = a->ldh;
+  if (vec_rows(a->h, a->ldh, 1) && p.N % 8 == 0) p.vec |= mk::kVecPre;
+  return g.run(mk::kProdForward, mk::kProdSwiglu, p, a->N);
+}
+
+int check_ragged_dgrad(const char* fn, const mk_moe_ragged_dgrad_args* a) {
+  if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
+  if (int rc = check_ragged(fn, a->R, a->K, a->N, a->num_experts, a->counts)) return rc;
+  const int64_t width = a->h ? 2 * a->K : a->K;
+  return check_matrices(fn,
+                        {{"dy", a->dy, a->R, a->N, a->lddy, 2},
+                         {"W", a->W, a->num_experts * a->K, a->N, a->N, 2},
+                         {"h", a->h, a->h ? a->R : 0, width, a->ldh, 2}},
+                        {{"out", a->out, a->R, width, a->ldo, 2}}, a->h, a->out);
+}
+
+int ragged_dgrad_body(const mk_moe_ragged_dgrad_args* a, Products g) {
+  if (a->R == 0) return MK_OK;
+  mk::ProductParams p = {};
+  p.A = u16(a->dy); p.lda = a->lddy;
+  p.B = u16(a->W); p.ldb = a->N; p.b_stride = a->K * a->N;
+  p.M = a->R; p.N = a->K; p.K = a->N;
+  p.counts = a->counts; p.E = a->num_experts; p.ragged = 1;
+  if (int rc = g.rows(p.A, a->R, a->N, p.lda, true)) return rc;
+  if (int rc = g.rows(p.B, a->K, a->N, p.ldb, true, a->num_experts, &p.b_stride, a->counts)) return rc;
+  p.C = a->out; p.ldc = a->ldo;
+  p.res = a->h; p.ldr = a->ldh;
+  const bool halves = !a->h || a->K % 8 == 0;
+  p.vec = (vec_rows(a->out, a->ldo, 1) && halves ? mk::kVecC : 0) | (vec_rows(a->h, a->ldh, 1) && halves ? mk::kVecRes : 0);
+  return g.run(mk::kProdLeftGrad, a->h ? mk::kProdSwigluGrad : mk::kProdStore, p, a->K);
+}
+
+int check_ragged_wgrad(const char* fn, const mk_moe_ragged_wgrad_args* a) {
+  if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
+  if (int rc = check_ragged(fn, a->R, a->K, a->N, a->num_experts, a->counts)) return rc;
+  if (!is_type(a->dw_type)) return fail(MK_EINVAL, "%s: dw_type must be 0 or 1", fn);
+  return check_matrices(fn, {{"A", a->A, a->R, a->K, a->lda, 2}, {"dy", a->dy, a->R, a->N, a->lddy, 2}},
+                        {{"dW", a->dW, a->num_experts * a->K, a->N, a->N, size_of(a->dw_type)}});
+}
+
+int ragged_wgrad_body(const mk_moe_ragged_wgrad_args* a, Products g) {
+  mk::ProductParams p = {};
+  p.A = u16(a->A); p.lda = a->lda;
+  p.B = u16(a->dy); p.ldb = a->lddy; p.b_cols = a->N;
+  p.M = a->K; p.N = a->N; p.K = a->R;
+  p.counts = a->counts; p.E = a->num_experts; p.ragged = 2;
+  if (a->R > 0) {
+    if (int rc = g.rows(p.A, a->R, a->K, p.lda, false)) return rc;
+    if (int rc = g.rows(p.B, a->R, a->N, p.ldb, false)) return rc;
+  }
+  p.C = a->dW; p.ldc = a->N; p.c_stride = a->K * a->N; p.c_f32 = a->dw_type == 0;
+  p.vec = vec_rows(a->dW, a->N, a->dw_type) && p.c_stride % 8 == 0 ? mk::kVecC | mk::kVecRes : 0;
+  if (a->accumulate) {
+    p.res = a->dW; p.ldr = a->N; p.res_f32 = p.c_f32;
+  }
+  return g.run(mk::kProdRightGrad, mk::kProdStore, p, a->N);
+}
+
+// ---- cross entropy over a vocabulary ----
+
+int check_vocab(const char* fn, int64_t T, int64_t H, int64_t V, int64_t begin, int labels_type, const void* labels,
+                const void* lse) {
+  if (int rc = check_sizes(fn, T, V, H)) return rc;
+  if (H == 0 || V == 0 || H > kMaxLd) return fail(MK_ESHAPE, "%s: H and V must be 1 .. %lld", fn, (long long)kMaxLd);
+  if (T > kMaxLd) return fail(MK_ESHAPE, "%s: at most %lld tokens", fn, (long long)kMaxLd);
+  if (begin < 0) return fail(MK_EINVAL, "%s: vocab_begin must not be negative", fn);
+  if (!is_type(labels_type)) return fail(MK_EINVAL, "%s: labels_type must be 0 or 1", fn);
+  if (T > 0 && (!labels || !lse)) return fail(MK_EINVAL, "%s: null argument", fn);
+  if (T > 0 && reinterpret_cast<uintptr_t>(labels) % (labels_type ? 8 : 4))
+    return fail(MK_EINVAL, "%s: labels must be aligned to their elements", fn);
+  return MK_OK;
+}
+
+int check_vocab_loss(const char* fn, const mk_vocab_loss_args* a) {
+  if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
+  if (int rc = check_vocab(fn, a->T, a->H, a->V, a->vocab_begin, a->labels_type, a->labels, a->lse)) return rc;
+  const int64_t n = a->T > 0 ? 1 : 0, w = a->T;
+  return check_matrices(fn, {{"x", a->x, a->T, a->H, a->ldx, 2}, {"W", a->W, a->H, a->V, a->ldw, 2},
+                             {"labels", a->labels, n, w, w, a->labels_type ? 8 : 4}},
+                        {{"lse", a->lse, n, w, w, 4}, {"target", a->target, n, w, w, 4},
+                         {"loss", a->loss, a->loss ? n : 0, w, w, 4}});
+}
+
+void fill_vocab(mk::ProductParams& p, const void* labels, int type, int64_t ignore, int64_t begin, int64_t V) {
+  p.labels = labels;
+  p.labels64 = type;
+  p.ignore = ignore;
+  p.label0 = begin;
+  p.vocab = V;
+}
+
+// Columns of a piece: its rows of [rows, columns] in bf16 take at most 128 MB (half of the last-level cache), a
+// multiple of 256.
+int64_t piece_of(int64_t rows, int64_t V) {
+  const int64_t most = std::max<int64_t>(256, (64LL << 20) / std::max<int64_t>(rows, 1) / 256 * 256);
+  return std::min(most, (V + 255) / 256 * 256);
+}
+
+int vocab_loss_body(const mk_vocab_loss_args* a, Products g) {
+  if (a->T == 0) return MK_OK;
+  mk::ProductParams p = {};
+  p.A = u16(a->x); p.lda = a->ldx;
+  p.M = a->T; p.K = a->H;
+  if (int rc = g.rows(p.A, a->T, a->H, p.lda, true)) return rc;
+  fill_vocab(p, a->labels, a->labels_type, a->ignore_index, a->vocab_begin, a->V);
+  p.target = a->target;
+  // weights that have to be laid out anew go piece by piece
+  const bool direct = aligned16(a->W) && a->ldw % 8 == 0;
+  const int64_t piece = direct ? a->V : piece_of(a->H, a->V);
+  const int64_t most_groups = (a->V + 63) / 64 + 8 * ((a->V + piece - 1) / piece);
+  float2* stats = static_cast<float2*>(g.sp.take(most_groups * a->T * 8));
+  int64_t groups = 0;
+  for (int64_t c0 = 0; c0 < a->V; c0 += piece) {
+    const int64_t mark = g.sp.used;
+    p.N = p.b_cols = std::min(piece, a->V - c0);
+    p.B = u16(a->W) + c0;
+    p.ldb = a->ldw;
+    if (int rc = g.rows(p.B, a->H, p.N, p.ldb, false)) return rc;
+    p.first_col = c0;
+    p.stats = g.sp.counting ? nullptr : stats + groups * a->T;
+    int tile = 0;
+    if (int rc = g.run(mk::kProdForward, mk::kProdStats, p, p.N, &tile)) return rc;
+    const mk::ProductShape& s = mk::kProductShapes[tile];
+    groups += (p.N + s.bn - 1) / s.bn * s.waves_n;
+    g.sp.used = mark;
+  }
+  if (g.sp.counting) return MK_OK;
+  mk::VocabJoinParams j = {stats, groups, a->T, a->labels, a->labels_type, a->ignore_index, a->vocab_begin, a->V,
+                           a->target, a->lse, a->loss};
+  return g.launched(mk::launch_vocab_join(j, g.stream));
+}
+
+int check_vocab_backward(const char* fn, const mk_vocab_loss_backward_args* a) {
+  if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
+  if (int rc = check_vocab(fn, a->T, a->H, a->V, a->vocab_begin, a->labels_type, a->labels, a->lse)) return rc;
+  if (!is_type(a->dx_type) || !is_type(a->dw_type)) return fail(MK_EINVAL, "%s: types must be 0 or 1", fn);
+  if (a->piece_columns < 0 || a->piece_columns % 256) return fail(MK_EINVAL, "%s: piece_columns must be a multiple of 256", fn);
+  if (a->T > 0 && !a->dloss) return fail(MK_EINVAL, "%s: dloss is null", fn);
+  if (!a->dx && !a->dW) return fail(MK_EINVAL, "%s: dx or dW must be set", fn);
+  const int64_t n = a->T > 0 ? 1 : 0, w = a->T;
+  return check_matrices(fn, {{"x", a->x, a->T, a->H, a->ldx, 2}, {"W", a->W, a->H, a->V, a->ldw, 2},
+                             {"lse", a->lse, n, w, w, 4}, {"dloss", a->dloss, n, w, w, 4},
+                             {"labels", a->labels, n, w, w, a->labels_type ? 8 : 4}},
+                        {{"dx", a->dx, a->dx ? a->T : 0, a->H, a->lddx, size_of(a->dx_type)},
+                         {"dW", a->dW, a->dW ? a->H : 0, a->V, a->lddw, size_of(a->dw_type)}});
+}
+
+int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
+  const int64_t T = a->T, H = a->H, V = a->V;
+  if (T == 0) {  // dW: a sum of nothing
+    if (!a->dW || a->accumulate) return MK_OK;
+    mk::ProductParams p = {};
+    p.M = H; p.N = p.b_cols = V;
+    p.lda = p.ldb = 8;
+    p.C = a->dW; p.ldc = a->lddw; p.c_f32 = a->dw_type == 0;
+    return g.run(mk::kProdRightGrad, mk::kProdStore, p, V);
+  }
+  const bool direct = aligned16(a->W) && a->ldw % 8 == 0 && V % 8 == 0;
+  int64_t piece = a->piece_columns ? std::min(a->piece_columns, (V + 255) / 256 * 256) : piece_of(direct ? T : std::max(T, H), V);
+  // x with the rows of tokens without a loss as zeros: what they hold would meet the zeros of dl otherwise
+  const int64_t ldx = (H + 7) / 8 * 8;
+  mk::RepackParams r = {};
+  r.src = u16(a->x); r.rows = T; r.cols = H; r.ld = T == 1 ? H : a->ldx; r.width = ldx; r.parts = 1; r.E = 1;
+  r.labels = a->labels; r.labels64 = a->labels_type; r.ignore = a->ignore_index;
+  uint16_t* x = r.dst = static_cast<uint16_t*>(g.sp.take(T * ldx * 2));
+  uint16_t* dl = static_cast<uint16_t*>(g.sp.take(T * piece * 2));
+  float* sum = nullptr;  // of dx over the pieces
+  int64_t lds = H;
+  if (a->dx && V > piece) {
+    if (a->dx_type == 0) {
+      sum = static_cast<float*>(a->dx);
+      lds = a->lddx;
+    } else {
+      lds = (H + 3) / 4 * 4;
+      sum = static_cast<float*>(g.sp.take(T * lds * 4));
+    }
+  }
+  if (!g.sp.counting)
+    if (int rc = g.launched(mk::launch_repack(r, g.stream))) return rc;
+  for (int64_t c0 = 0; c0 < V; c0 += piece) {
+    const int64_t mark = g.sp.used, n = std::min(piece, V - c0);
+    const uint16_t* w = u16(a->W) + c0;
+    int64_t ldw = a->ldw;
+    if (!direct)
+      if (int rc = g.rows(w, H, n, ldw, true)) return rc;
+    mk::ProductParams p = {};
+    p.A = x; p.lda = ldx;
+    p.B = w; p.ldb = ldw; p.b_cols = n;
+    p.M = T; p.N = n; p.K = H;
+    fill_vocab(p, a->labels, a->labels_type, a->ignore_index, a->vocab_begin, V);
+    p.first_col = c0;
+    p.lse = a->lse; p.dloss = a->dloss;
+    p.C = dl; p.ldc = piece;
+    if (int rc = g.run(mk::kProdForward, mk::kProdDlogits, p, n)) return rc;
+    if (a->dx) {
+      const bool last = c0 + n == V;
+      mk::ProductParams q = {};
+      q.A = dl; q.lda = piece;
+      q.B = w; q.ldb = ldw;
+      q.M = T; q.N = H; q.K = n;
+      if (c0 > 0) {
+        q.res = sum; q.ldr = lds; q.res_f32 = 1;
+        if (g.sp.counting || vec_rows(sum, lds, 0)) q.vec |= mk::kVecRes;
+      }
+      q.C = last ? a->dx : sum;
+      q.ldc = last ? a->lddx : lds;
+      q.c_f32 = !last || a->dx_type == 0;
+      if (vec_rows(q.C, q.ldc, q.c_f32 ? 0 : 1)) q.vec |= mk::kVecC;
+      if (int rc = g.run(mk::kProdLeftGrad, mk::kProdStore, q, H)) return rc;
+    }
+    if (a->dW) {
+      mk::ProductParams q = {};
+      q.A = x; q.lda = ldx;
+      q.B = dl; q.ldb = piece; q.b_cols = n;
+      q.M = H; q.N = n; q.K = T;
+      q.C = static_cast<char*>(a->dW) + c0 * size_of(a->dw_type);
+      q.ldc = a->lddw; q.c_f32 = a->dw_type == 0;
+      if (vec_rows(q.C, q.ldc, a->dw_type)) q.vec = mk::kVecC | mk::kVecRes;
+      if (a->accumulate) {
+        q.res = q.C; q.ldr = q.ldc; q.res_f32 = q.c_f32;
+      }
+      if (int rc = g.run(mk::kProdRightGrad, mk::kProdStore, q, n)) return rc;
+    }
+    g.sp.used = mark;
+  }
+  return MK_OK;
+}
+
+uint32_t* tickets_of(void* t) { return static_cast<uint32_t*>(t); }
+
+// The two entry points of an operator: `check`, then `body` to count or to work.
+template <class A, class Check, class Body>
+int64_t product_bytes(const char* fn, const A* a, Check check, Body body, bool cut) {
+  if (check(fn, a)) return -1;
+  DevInfo d;
+  if (device_info(&d)) return -1;
+  static uint32_t any[1];
+  return count_space([&](Space& sp) { return body(a, Products{fn, sp, d.cus, cut ? any : nullptr, nullptr}); });
+}
+
+template <class A, class Check, class Body>
+int product_call(const char* fn, const A* a, Check check, Body body, void* tickets, bool cut, void* stream) {
+  if (int rc = check(fn, a)) return rc;
+  if (cut && (!tickets || reinterpret_cast<uintptr_t>(tickets) % 4))
+    return fail(MK_EINVAL, "%s: tickets must be %d words", fn, MK_PRODUCT_TICKETS);
+  DevInfo d;
+  if (int rc = device_info(&d)) return rc;
+  return with_space(fn, a->workspace, a->workspace_bytes, [&](Space& sp) {
+    return body(a, Products{fn, sp, d.cus, cut ? tickets_of(tickets) : nullptr, static_cast<hipStream_t>(stream)});
+  });
+}
+
+static_assert(MK_PRODUCT_TICKETS == mk::kProductTickets, "tickets");
+
+}  // namespace
+
+extern "C" {
+
+int64_t mk_gemm_act_workspace_bytes(const mk_gemm_act_args* a) {
+  return product_bytes("mk_gemm_act_workspace_bytes", a, check_gemm_act, gemm_act_body, true);
+}
+int mk_gemm_act(const mk_gemm_act_args* a, void* stream) {
+  return product_call("mk_gemm_act", a, check_gemm_act, gemm_act_body, a ? a->tickets : nullptr, true, stream);
+}
+
+int64_t mk_gemm_act_backward_workspace_bytes(const mk_gemm_act_backward_args* a) {
+  return product_bytes("mk_gemm_act_backward_workspace_bytes", a, check_gemm_act_backward, gemm_act_backward_body, true);
+}
+int mk_gemm_act_backward(const mk_gemm_act_backward_args* a, void* stream) {
+  return product_call("mk_gemm_act_backward", a, check_gemm_act_backward, gemm_act_backward_body,
+                      a ? a->tickets : nullptr, true, stream);
+}
+
+int64_t mk_moe_ragged_gemm_workspace_bytes(const mk_moe_ragged_gemm_args* a) {
+  return product_bytes("mk_moe_ragged_gemm_workspace_bytes", a, check_ragged_gemm, ragged_gemm_body, false);
+}
+int mk_moe_ragged_gemm(const mk_moe_ragged_gemm_args* a, void* stream) {
+  return product_call("mk_moe_ragged_gemm", a, check_ragged_gemm, ragged_gemm_body, nullptr, false, stream);
+}
+
+int64_t mk_moe_ragged_dgrad_workspace_bytes(const mk_moe_ragged_dgrad_args* a) {
+  return product_bytes("mk_moe_ragged_dgrad_workspace_bytes", a, check_ragged_dgrad, ragged_dgrad_body, false);
+}
+int mk_moe_ragged_dgrad(const mk_moe_ragged_dgrad_args* a, void* stream) {
+  return product_call("mk_moe_ragged_dgrad", a, check_ragged_dgrad, ragged_dgrad_body, nullptr, false, stream);
+}
+
+int64_t mk_moe_ragged_wgrad_workspace_bytes(const mk_moe_ragged_wgrad_args* a) {
+  return product_bytes("mk_moe_ragged_wgrad_workspace_bytes", a, check_ragged_wgrad, ragged_wgrad_body, false);
+}
+int mk_moe_ragged_wgrad(const mk_moe_ragged_wgrad_args* a, void* stream) {
+  return product_call("mk_moe_ragged_wgrad", a, check_ragged_wgrad, ragged_wgrad_body, nullptr, false, stream);
+}
+
+int64_t mk_vocab_loss_workspace_bytes(const mk_vocab_loss_args* a) {
+  return product_bytes("mk_vocab_loss_workspace_bytes", a, check_vocab_loss, vocab_loss_body, true);
+}
+int mk_vocab_loss(const mk_vocab_loss_args* a, void* stream) {
+  return product_call("mk_vocab_loss", a, check_vocab_loss, vocab_loss_body, a ? a->tickets : nullptr, true, stream);
+}
+
+int64_t mk_vocab_loss_backward_workspace_bytes(const mk_vocab_loss_backward_args* a) {
+  return product_bytes("mk_vocab_loss_backward_workspace_bytes", a, check_vocab_backward, vocab_loss_backward_body, true);
+}
+int mk_vocab_loss_backward(const mk_vocab_loss_backward_args* a, void* stream) {
+  return product_call("mk_vocab_loss_backward", a, check_vocab_backward, vocab_loss_backward_body,
+                      a ? a->tickets : nullptr, true, stream);
+}
+
+}  // extern "C"

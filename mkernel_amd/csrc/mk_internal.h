@@ -6,6 +6,7 @@
 
 #include "mk_map.h"
 #include "mk_plan.h"
+#include "mk_product_plan.h"
 
 namespace mk {
 
@@ -255,6 +256,92 @@ hipError_t launch_w4_pack(const uint8_t* codes, const uint16_t* scales, const ui
                           int64_t E, int group, unsigned char* packed, hipStream_t stream);
 hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E, int group, uint8_t* codes,
                               uint16_t* scales, hipStream_t stream);
+
+// Products with what follows them (mk_product.h, mk_product.hip).
+enum ProductEpilogue : int { kProdStore = 0, kProdSwiglu = 1, kProdSwigluGrad = 2, kProdStats = 3, kProdDlogits = 4 };
+enum ProductOrder : int { kProdForward = 0, kProdLeftGrad = 1, kProdRightGrad = 2 };
+enum ProductAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+// which rows of the epilogue start at 16-byte boundaries
+enum ProductVec : int { kVecC = 1, kVecRes = 2, kVecPre = 4, kVecBias = 8 };
+struct ProductParams {
+  const uint16_t* A;
+  const uint16_t* B;
+  int64_t lda, ldb;
+  int64_t M, N, K;          // of C; with ragged 1 M, with ragged 2 K is the rows of the buffers
+  int64_t b_cols;           // valid columns of a k-strided B
+  // groups
+  const int* counts;
+  int E, ragged;            // 0 none, 1 rows of A and C, 2 rows of A and B
+  int64_t b_stride, c_stride;  // elements between groups' B (ragged 1) and C (ragged 2)
+  // tiles
+  int tiles_m, tiles_n, group_m, split;
+  uint32_t* tickets;        // one per tile, zero between launches
+  float* parts;             // a tile per part
+  // epilogue
+  int vec, act;
+  void* C;                  // SwiGLU: [M, N]; its gradient: [M, 2 N]
+  int64_t ldc;
+  int c_f32;
+  const void* bias;
+  int bias_f32;
+  const void* res;          // added behind the activation (may be C); SwiGLU's gradient: [M, 2 N] gate | up
+  int64_t ldr;
+  int res_f32;
+  uint16_t* pre;            // store: sum + bias; SwiGLU: [M, 2 N] gate | up
+  int64_t ldp;
+  int up;                   // SwiGLU: B's first up column
+  // vocabulary
+  const void* labels;
+  int labels64;
+  int64_t ignore, label0, vocab, first_col;
+  float2* stats;            // [column groups][M]
+  float* target;
+  const float* lse;
+  const float* dloss;
+};
+hipError_t launch_product_forward(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
+hipError_t launch_product_left_grad(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
+hipError_t launch_product_right_grad(const ProductParams& p, int tile, int64_t grid, hipStream_t stream);
+// Rows of bf16 into rows of a multiple of 8 elements, zeros behind the last: `parts` pieces of `cols` columns each,
+// one behind the other, every piece filled up to `width`; groups (counts, E) that have no rows are left out.
+// labels: rows whose label is `ignore` become zeros.
+struct RepackParams {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t rows, cols, ld, src_stride, dst_stride;  // strides between the groups' matrices
+  int64_t width;
+  int parts, E;
+  const int* counts;
+  const void* labels;
+  int labels64;
+  int64_t ignore;
+};
+hipError_t launch_repack(const RepackParams& p, hipStream_t stream);
+// dpre = dC * act'(pre), bf16 rows of `width` (null: not kept), and the columns' sums of it
+struct ActGradParams {
+  const uint16_t* dC;
+  const uint16_t* pre;
+  uint16_t* dpre;
+  int64_t M, N, ldc, ldp, width;
+  int act, vec_c, vec_p;
+  float* part;              // [row_blocks][N], null: no sums
+  float* dbias;
+  int accumulate;
+  int64_t row_blocks;       // set by act_grad_blocks
+};
+int64_t act_grad_blocks(int64_t M, int64_t N);
+hipError_t launch_act_grad(const ActGradParams& p, hipStream_t stream);
+struct VocabJoinParams {
+  const float2* stats;
+  int64_t groups, T;
+  const void* labels;
+  int labels64;
+  int64_t ignore, label0, vocab;
+  float* target;
+  float* lse;
+  float* loss;
+};
+hipError_t launch_vocab_join(const VocabJoinParams& p, hipStream_t stream);
 
 int64_t index_workspace_bytes(int T, int topk, int n_local);
 hipError_t launch_mfma_ceiling(int64_t iters, int n_wg, uint32_t seed, float* sink, uint64_t* clocks,

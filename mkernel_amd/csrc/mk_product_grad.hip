@@ -1,0 +1,25 @@
+// mk_product_grad.hip — the products of a backward pass (mk_product.h): of the
+// activations (rows against the rows of the weights) and of the weights (columns
+// against columns), without a transposed copy of either.
+#include "mk_product.h"
+
+namespace mk {
+
+hipError_t launch_product_left_grad(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream) {
+  switch (epi) {
+    case kProdStore: return launch_product_tile<true, true, kProdStore>(p, tile, grid, stream);
+    case kProdSwigluGrad: return launch_product_tile<true, true, kProdSwigluGrad>(p, tile, grid, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_product_right_grad(const ProductParams& p, int tile, int64_t grid, hipStream_t stream) {
+  switch (tile) {
+    case kProd64: return launch_product_cfg<ProdTile64, false, false, kProdStore>(p, grid, stream);
+    case kProd128: return launch_product_cfg<ProdTile128, false, false, kProdStore>(p, grid, stream);
+    case kProd256: return launch_product_cfg<ProdTile256, false, false, kProdStore>(p, grid, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace mk

@@ -15,9 +15,11 @@ import numpy as np
 import torch
 
 from . import capi
-from .capi import (AgGemmArgs, GemmAr2Args, GemmArArgs, GemmArgs, GemmRsArgs, GemmW4Args, MoeCombineArgs,
-                   MoeCombineBackwardArgs, MoeFfnArgs, MoeFfnW4Args, MoeGroupedGemmArgs, MoeGroupedGemmW4Args, MoeIndex,
-                   MoeIndexDevArgs, MoePermuteArgs, MoeRouteArgs, MoeRouteBackwardArgs, W4PackArgs, W4QuantizeArgs)
+from .capi import (AgGemmArgs, GemmActArgs, GemmActBackwardArgs, GemmAr2Args, GemmArArgs, GemmArgs, GemmRsArgs,
+                   GemmW4Args, MoeCombineArgs, MoeCombineBackwardArgs, MoeFfnArgs, MoeFfnW4Args, MoeGroupedGemmArgs,
+                   MoeGroupedGemmW4Args, MoeIndex, MoeIndexDevArgs, MoePermuteArgs, MoeRaggedDgradArgs,
+                   MoeRaggedGemmArgs, MoeRaggedWgradArgs, MoeRouteArgs, MoeRouteBackwardArgs, VocabLossArgs,
+                   VocabLossBackwardArgs, W4PackArgs, W4QuantizeArgs)
 
 
 def _ptr(t: torch.Tensor | None) -> int:
@@ -787,6 +789,314 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
                      y_out.data_ptr(), T, n, R_pad, n if tokens_per_src is None else tokens_per_src, devs_per_node,
                      y_out.dtype is torch.bfloat16, _ptr(sizes))
     return y_out
+
+
+# ------------------------------------------------------------------- products with what follows them
+_tickets: dict = {}
+
+
+def _ticket_words(index: int, stream: int) -> int:
+    """The zeroed words by which the parts of a product's K meet: one set per
+    (device, stream), left zeroed by every launch.  Inside a graph's capture a
+    set of its own, whose zeros are recorded with it: graphs may then run beside
+    each other and beside eager calls."""
+    if torch.cuda.is_current_stream_capturing():
+        # torch keeps it for the graph, whose private pool it comes from
+        return torch.zeros(capi.PRODUCT_TICKETS, dtype=torch.int32, device=torch.device("cuda", index)).data_ptr()
+    t = _tickets.get((index, stream))
+    if t is None:
+        t = _tickets[index, stream] = torch.zeros(capi.PRODUCT_TICKETS, dtype=torch.int32,
+                                                  device=torch.device("cuda", index))
+    return t.data_ptr()
+
+
+def _product(fn: str, cls, device, cut: bool, *values) -> None:
+    """Calls an entry point whose arguments end with a workspace (and, with
+    cut, tickets)."""
+    n = capi.workspace_bytes(fn, cls, *values)
+    # the caching allocator reuses it in stream order, a graph's capture keeps it
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    stream = _raw_stream(device.index)
+    tail = (_ticket_words(device.index, stream),) if cut else ()
+    capi.call_values(fn, cls, stream, *values, 0 if ws is None else ws.data_ptr(), n, *tail)
+
+
+def _rows(t, name: str, dtypes, shape, device) -> None:
+    """A matrix with contiguous rows, any distance apart."""
+    if not (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == shape and t.device == device
+            and t.is_contiguous()):
+        _tensor(t, name, dtypes, shape, rows=True, device=device)
+
+
+def _matrix(t, name: str) -> tuple:
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.bfloat16 and t.is_cuda and t.dim() == 2
+            and t.is_contiguous()):
+        _tensor(t, name, _BF16, rows=True)
+    return t.shape
+
+
+def _act(act: str) -> int:
+    if act not in capi.ACTS:
+        raise ValueError(f"act must be one of {', '.join(capi.ACTS)}")
+    return capi.ACTS[act]
+
+
+def _result(out, name: str, dtype, shape, device):
+    """out, checked, or a new tensor of that type."""
+    if out is None:
+        if dtype not in _LOGITS:
+            raise ValueError(f"{name} is float32 or bfloat16")
+        return torch.empty(shape, dtype=dtype, device=device)
+    _rows(out, name, _LOGITS, shape, device)
+    return out
+
+
+def _code(t) -> int:
+    return int(t is not None and t.dtype is torch.bfloat16)
+
+
+def gemm_act(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
+             residual: torch.Tensor | None = None, out: torch.Tensor | None = None, pre: torch.Tensor | None = None,
+             out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """out = act(A @ B + bias) + residual in one pass (mk_gemm_act): A bf16
+    [M, K], B bf16 [K, N], fp32 sums, one rounding.  Any sizes, from one row on;
+    rows need only be contiguous each (operands whose rows do not start at
+    16-byte boundaries are laid out anew first, which costs a copy).  act: none,
+    relu, gelu, gelu_tanh or silu.  bias [N] and residual [M, N]: bfloat16 or
+    float32; out: bfloat16 or float32 (out_dtype where none is given), may be the
+    residual itself, overlaps nothing else.  pre (bf16 [M, N]) receives A @ B +
+    bias for gemm_act_backward.  Nothing is recorded for autograd."""
+    M, K = _matrix(A, "A")
+    dev = A.device
+    if _matrix(B, "B")[0] != K or B.device != dev:
+        raise ValueError(f"B must be [{K}, N] on {dev}")
+    N = B.shape[1]
+    code = _act(act)
+    if bias is not None and not (_is(bias, torch.bfloat16, (N,), dev) or _is(bias, torch.float32, (N,), dev)):
+        _tensor(bias, "bias", _LOGITS, (N,), device=dev)
+    if residual is not None:
+        _rows(residual, "residual", _LOGITS, (M, N), dev)
+    if pre is not None:
+        _rows(pre, "pre", _BF16, (M, N), dev)
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return gemm_act(A, B, bias, act, residual, out, pre, out_dtype)
+    out = _result(out, "out", out_dtype, (M, N), dev)
+    if out.numel() == 0:
+        return out
+    _product("mk_gemm_act", GemmActArgs, dev, True, A.data_ptr(), B.data_ptr(), out.data_ptr(), _ptr(bias),
+             _ptr(residual), _ptr(pre), M, N, K, _ld(A), _ld(B), _ld(out), 0 if residual is None else _ld(residual),
+             0 if pre is None else _ld(pre), code, _code(out), _code(bias), _code(residual))
+    return out
+
+
+def gemm_act_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor, pre: torch.Tensor | None = None,
+                      act: str = "none", need_dA: bool = True, need_dB: bool = True, need_dbias: bool = True,
+                      dA: torch.Tensor | None = None, dB: torch.Tensor | None = None,
+                      dbias: torch.Tensor | None = None, dB_dtype: torch.dtype = torch.bfloat16,
+                      accumulate: bool = False) -> tuple:
+    """Gradients of gemm_act (mk_gemm_act_backward): (dA bf16, dB bfloat16 or
+    float32, dbias float32), None for what is not needed; the residual's is dC
+    itself (bf16 [M, N]).  pre: what the forward call kept, needed with an
+    activation.  dpre = dC * act'(pre) is rounded to bf16 for dA and dB (not for
+    dbias), without an activation it is dC.  accumulate: dB and dbias, which are
+    then given, are added to."""
+    M, N = _matrix(dC, "dC")
+    dev = dC.device
+    K = _matrix(A, "A")[1]
+    if A.shape[0] != M or A.device != dev or _matrix(B, "B") != (K, N) or B.device != dev:
+        raise ValueError(f"A must be [{M}, K] and B [K, {N}] on {dev}")
+    code = _act(act)
+    if code:
+        if pre is None:
+            raise ValueError("pre is needed with an activation")
+        _rows(pre, "pre", _BF16, (M, N), dev)
+    if not (need_dA or need_dB or need_dbias):
+        return None, None, None
+    if accumulate and ((need_dB and dB is None) or (need_dbias and dbias is None)):
+        raise ValueError("accumulate needs dB and dbias")
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return gemm_act_backward(dC, A, B, pre, act, need_dA, need_dB, need_dbias, dA, dB, dbias, dB_dtype,
+                                     accumulate)
+    if need_dA and dA is not None:
+        _rows(dA, "dA", _BF16, (M, K), dev)
+    dA = _result(dA, "dA", torch.bfloat16, (M, K), dev) if need_dA else None
+    dB = _result(dB, "dB", dB_dtype, (K, N), dev) if need_dB else None
+    if not need_dbias:
+        dbias = None
+    elif dbias is None:
+        dbias = torch.empty(N, dtype=torch.float32, device=dev)
+    elif not _is(dbias, torch.float32, (N,), dev):
+        _tensor(dbias, "dbias", _F32, (N,), device=dev)
+    _product("mk_gemm_act_backward", GemmActBackwardArgs, dev, True, dC.data_ptr(), A.data_ptr(), B.data_ptr(),
+             _ptr(pre) if code else 0, _ptr(dA), _ptr(dB), _ptr(dbias), M, N, K, _ld(dC), _ld(A), _ld(B),
+             _ld(pre) if code else 0, 0 if dA is None else _ld(dA), 0 if dB is None else _ld(dB), code, _code(dB),
+             bool(accumulate))
+    return dA, dB, dbias
+
+
+def _experts(W, counts, device) -> tuple:
+    if not (isinstance(W, torch.Tensor) and W.dtype is torch.bfloat16 and W.device == device and W.dim() == 3
+            and W.is_contiguous()):
+        _tensor(W, "W", _BF16, dim=3, device=device)
+    if not _is(counts, torch.int32, (W.shape[0],), device):
+        _tensor(counts, "counts", _I32, (W.shape[0],), device=device)
+    return W.shape
+
+
+def moe_ragged_gemm(A: torch.Tensor, W: torch.Tensor, counts: torch.Tensor, mode: int = 0,
+                    out: torch.Tensor | None = None, h: torch.Tensor | None = None) -> torch.Tensor:
+    """Expert products on ragged rows (mk_moe_ragged_gemm): A bf16 [R, K] holds
+    counts[e] rows for expert e, one expert behind the other (counts int32 [E] on
+    the device, e.g. padded_tokens_per_expert of moe_build_indices_dev, at
+    row_block 1 or any other; nothing is read back), W bf16 [E, K, N].
+    mode 0: out = A @ W[e] (bf16 [R, N]); mode 1: out = silu(g) * u with (g | u) =
+    A @ W[e] (bf16 [R, N / 2]), and h (bf16 [R, N]) receives (g | u) for the
+    backward pass.  Any sizes.  Rows behind the experts' are neither read nor
+    written (new results hold whatever was there)."""
+    R, K = _matrix(A, "A")
+    dev = A.device
+    if _experts(W, counts, dev)[1] != K:
+        raise ValueError(f"W must be [E, {K}, N]")
+    E, _, N = W.shape
+    if mode not in (0, 1) or (mode == 1 and N % 2):
+        raise ValueError("mode must be 0, or 1 with an even N")
+    if h is not None:
+        if mode == 0:
+            raise ValueError("h belongs to mode 1")
+        _rows(h, "h", _BF16, (R, N), dev)
+    shape = (R, N // 2 if mode else N)
+    if out is not None:
+        _rows(out, "out", _BF16, shape, dev)
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return moe_ragged_gemm(A, W, counts, mode, out, h)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    _product("mk_moe_ragged_gemm", MoeRaggedGemmArgs, dev, False, A.data_ptr(), W.data_ptr(), counts.data_ptr(),
+             out.data_ptr(), _ptr(h), R, K, N, _ld(A), _ld(out), 0 if h is None else _ld(h), E, mode)
+    return out
+
+
+def moe_ragged_gemm_dgrad(dy: torch.Tensor, W: torch.Tensor, counts: torch.Tensor, h: torch.Tensor | None = None,
+                          out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of moe_ragged_gemm's rows (mk_moe_ragged_dgrad): dA = dy @ W[e]^T
+    (bf16 [R, K]).  With h (bf16 [R, 2K], as mode 1 kept it in front of this
+    product): the gradient of h itself, bf16 [R, 2K], in the same pass; out may
+    then be h."""
+    R, N = _matrix(dy, "dy")
+    dev = dy.device
+    if _experts(W, counts, dev)[2] != N:
+        raise ValueError(f"W must be [E, K, {N}]")
+    E, K, _ = W.shape
+    shape = (R, 2 * K if h is not None else K)
+    if h is not None:
+        _rows(h, "h", _BF16, shape, dev)
+    if out is not None:
+        _rows(out, "out", _BF16, shape, dev)
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return moe_ragged_gemm_dgrad(dy, W, counts, h, out)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    _product("mk_moe_ragged_dgrad", MoeRaggedDgradArgs, dev, False, dy.data_ptr(), W.data_ptr(), counts.data_ptr(),
+             _ptr(h), out.data_ptr(), R, K, N, _ld(dy), 0 if h is None else _ld(h), _ld(out), E)
+    return out
+
+
+def moe_ragged_gemm_wgrad(A: torch.Tensor, dy: torch.Tensor, counts: torch.Tensor, out: torch.Tensor | None = None,
+                          out_dtype: torch.dtype = torch.bfloat16, accumulate: bool = False) -> torch.Tensor:
+    """Gradient of moe_ragged_gemm's weights (mk_moe_ragged_wgrad): dW[e] = A_e^T
+    @ dy_e, bfloat16 or float32 [E, K, N]; zeros for an expert without rows.
+    accumulate: out is added to."""
+    R, K = _matrix(A, "A")
+    dev = A.device
+    if _matrix(dy, "dy")[0] != R or dy.device != dev:
+        raise ValueError(f"dy must be [{R}, N] on {dev}")
+    N = dy.shape[1]
+    if not (isinstance(counts, torch.Tensor) and counts.dim() == 1 and _is(counts, torch.int32, counts.shape, dev)):
+        _tensor(counts, "counts", _I32, dim=1, device=dev)
+    E = counts.shape[0]
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+    else:
+        _tensor(out, "out", _LOGITS, (E, K, N), device=dev)
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return moe_ragged_gemm_wgrad(A, dy, counts, out, out_dtype, accumulate)
+    if out is None:
+        if out_dtype not in _LOGITS:
+            raise ValueError("out is float32 or bfloat16")
+        out = torch.empty((E, K, N), dtype=out_dtype, device=dev)
+    _product("mk_moe_ragged_wgrad", MoeRaggedWgradArgs, dev, False, A.data_ptr(), dy.data_ptr(), counts.data_ptr(),
+             out.data_ptr(), R, K, N, _ld(A), _ld(dy), E, _code(out), bool(accumulate))
+    return out
+
+
+def _vocab(x, W, labels) -> tuple:
+    T, H = _matrix(x, "x")
+    dev = x.device
+    if _matrix(W, "W")[0] != H or W.device != dev:
+        raise ValueError(f"W must be [{H}, V] on {dev}")
+    if not (_is(labels, torch.int64, (T,), dev) or _is(labels, torch.int32, (T,), dev)):
+        _tensor(labels, "labels", (torch.int32, torch.int64), (T,), device=dev)
+    return T, H, W.shape[1], dev, labels.dtype is torch.int64
+
+
+def vocab_loss(x: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, vocab_begin: int = 0,
+               ignore_index: int = -100) -> dict:
+    """Cross entropy of the logits x @ W, which are never stored (mk_vocab_loss):
+    x bf16 [T, H], W bf16 [H, V], labels int32 or int64 [T].  Returns float32 [T]
+    "lse" = log sum exp of the logits, "target" = the label's logit and "loss" =
+    lse - target; all 0 for tokens whose label is ignore_index, whatever their
+    rows of x hold.  One rank's shard of a vocabulary: W holds the columns from
+    vocab_begin on, and target is 0 where another rank has the label; the ranks'
+    lse are joined by torch.logsumexp, their targets by a sum, and the loss is
+    the difference."""
+    T, H, V, dev, wide = _vocab(x, W, labels)
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return vocab_loss(x, W, labels, vocab_begin, ignore_index)
+    lse, target, loss = torch.empty((3, T), dtype=torch.float32, device=dev).unbind(0)
+    _product("mk_vocab_loss", VocabLossArgs, dev, True, x.data_ptr(), W.data_ptr(), labels.data_ptr(), lse.data_ptr(),
+             target.data_ptr(), loss.data_ptr(), T, H, V, _ld(x), _ld(W), vocab_begin, ignore_index, wide)
+    return {"loss": loss, "lse": lse, "target": target}
+
+
+def vocab_loss_backward(x: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor,
+                        dloss: torch.Tensor, vocab_begin: int = 0, ignore_index: int = -100, need_dx: bool = True,
+                        need_dW: bool = True, dx: torch.Tensor | None = None, dW: torch.Tensor | None = None,
+                        dx_dtype: torch.dtype = torch.bfloat16, dW_dtype: torch.dtype = torch.bfloat16,
+                        accumulate: bool = False, piece_columns: int = 0) -> tuple:
+    """Gradients of vocab_loss's loss (mk_vocab_loss_backward): (dx [T, H], dW
+    [H, V]), bfloat16 or float32, None for what is not needed, from dloss
+    (float32 [T]) and lse (of a shard: the joined one).  The logits are computed
+    anew, a piece of the vocabulary at a time (piece_columns, a multiple of 256;
+    0: as many as keep the piece's gradient of the logits below 128 MB); that
+    gradient is rounded to bf16 between the products.  A shard's dx is its part
+    of a sum over the ranks (dx_dtype=torch.float32 for that).  accumulate: dW,
+    which is then given, is added to."""
+    T, H, V, dev, wide = _vocab(x, W, labels)
+    for t, name in ((lse, "lse"), (dloss, "dloss")):
+        if not _is(t, torch.float32, (T,), dev):
+            _tensor(t, name, _F32, (T,), device=dev)
+    if not (need_dx or need_dW):
+        return None, None
+    if accumulate and need_dW and dW is None:
+        raise ValueError("accumulate needs dW")
+    if dev.index != _device_index():
+        with torch.cuda.device(dev):
+            return vocab_loss_backward(x, W, labels, lse, dloss, vocab_begin, ignore_index, need_dx, need_dW, dx, dW,
+                                       dx_dtype, dW_dtype, accumulate, piece_columns)
+    dx = _result(dx, "dx", dx_dtype, (T, H), dev) if need_dx else None
+    dW = _result(dW, "dW", dW_dtype, (H, V), dev) if need_dW else None
+    _product("mk_vocab_loss_backward", VocabLossBackwardArgs, dev, True, x.data_ptr(), W.data_ptr(), labels.data_ptr(),
+             lse.data_ptr(), dloss.data_ptr(), _ptr(dx), _ptr(dW), T, H, V, _ld(x), _ld(W),
+             0 if dx is None else _ld(dx), 0 if dW is None else _ld(dW), vocab_begin, ignore_index, piece_columns,
+             wide, _code(dx), _code(dW), bool(accumulate))
+    return dx, dW
 
 
 def probe_mfma_ceiling(iters: int = 20000, num_wg: int = 0, reps: int = 3) -> dict:
