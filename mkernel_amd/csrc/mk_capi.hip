@@ -1411,16 +1411,18 @@ struct Products {
     p.tickets = tickets;
     const int bn = epi == mk::kProdSwiglu ? s.bn / 2 : s.bn;
     const int64_t tn = (p.N + bn - 1) / bn, tm = (p.M + s.bm - 1) / s.bm;
-    // of ragged rows at most: each group's last tile may hold one row
-    const int64_t tiles = (p.ragged == 1 ? std::min(tm + groups - 1, p.M) : tm) * tn * (p.ragged == 2 ? groups : 1);
-    if (tiles * p.split >= (1LL << 31)) return fail(MK_ESHAPE, "%s: too many tiles", fn);
     p.tiles_m = (int)tm;
     p.tiles_n = (int)tn;
+    p.whole = (int)plan.whole;
+    int64_t grid = plan.whole + (plan.tiles - plan.whole) * plan.split;
+    // ragged: at most that many workgroups for one of the 8 XCDs, of rows when every group's last tile holds one
+    if (p.ragged == 1) grid = 8 * ((tn + 7) / 8) * std::min(tm + groups - 1, p.M);
+    if (p.ragged == 2) grid = 8 * ((tm * tn + 7) / 8) * groups;
+    if (grid >= (1LL << 31)) return fail(MK_ESHAPE, "%s: too many tiles", fn);
     const int64_t mark = sp.used;
-    if (p.split > 1) p.parts = static_cast<float*>(sp.take(tiles * p.split * s.bm * s.bn * 4));
+    if (p.split > 1) p.parts = static_cast<float*>(sp.take((plan.tiles - plan.whole) * p.split * s.bm * s.bn * 4));
     sp.used = mark;  // the next launch may use them again
     if (sp.counting) return MK_OK;
-    const int64_t grid = tiles * p.split;
     return launched(order == mk::kProdForward    ? mk::launch_product_forward(p, epi, plan.tile, grid, stream)
                     : order == mk::kProdLeftGrad ? mk::launch_product_left_grad(p, epi, plan.tile, grid, stream)
                                                  : mk::launch_product_right_grad(p, plan.tile, grid, stream));

@@ -274,8 +274,9 @@ struct ProductParams {
   int E, ragged;            // 0 none, 1 rows of A and C, 2 rows of A and B
   int64_t b_stride, c_stride;  // elements between groups' B (ragged 1) and C (ragged 2)
   // tiles
-  int tiles_m, tiles_n, group_m, split;
-  uint32_t* tickets;        // one per tile, zero between launches
+  int tiles_m, tiles_n, group_m;
+  int whole, split;         // tiles from `whole` on are cut into `split` parts along K
+  uint32_t* tickets;        // one per cut tile, zero between launches
   float* parts;             // a tile per part
   // epilogue
   int vec, act;

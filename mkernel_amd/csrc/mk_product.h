@@ -26,6 +26,8 @@
 // rows in fp32 and comes back as 8 neighbouring columns a lane, so that every
 // load and store of the epilogue covers whole row segments.
 #pragma once
+#include <type_traits>
+
 #include "mk_device.h"
 #include "mk_internal.h"
 #include "mk_once.h"
@@ -69,11 +71,10 @@ struct Operand {
   static constexpr uint32_t ROW = UPR * 16;
   uint32_t src[INST];   // byte offset of this lane's unit from the stage's base
   uint32_t rd[KC ? BK / 16 : F];
-  const uint16_t* base;  // of the next stage to load (KS), of the tile (KC)
+  u32x4_t rsrc;         // KC: the tile's rows; KS: a whole stage's k-rows, the base moves on with every stage
+  uint32_t koff;        // KC: byte offset of the next stage
   int64_t ld;
-  uint32_t bytes, koff;
-  int64_t left;          // k-rows behind the next stage's first (KS)
-  int cols;              // valid columns of a k-row (KS)
+  int cols;             // KS: valid columns of a k-row
 
   // LDS row and unit of DMA lane l of the wave's instruction i
   __device__ __forceinline__ static void where(int wave, int lane, int i, int& row, int& c) {
@@ -88,13 +89,11 @@ struct Operand {
                                        int wave, int lane, Col col) {
     ld = ld_;
     if constexpr (KC) {
-      base = p;
-      bytes = rows_or_cols > 0 ? ((uint32_t)(((rows_or_cols - 1) * ld + K) * 2) + 15u) & ~15u : 0u;
+      rsrc = make_rsrc_v(p, rows_or_cols > 0 ? ((uint32_t)(((rows_or_cols - 1) * ld + K) * 2) + 15u) & ~15u : 0u);
       koff = (uint32_t)(k0 * 2);
     } else {
-      base = p + k0 * ld;
-      left = K - k0;
       cols = (int)rows_or_cols;
+      rsrc = make_rsrc_v(p + k0 * ld, stage_bytes(BK));
     }
 #pragma unroll
     for (int i = 0; i < INST; ++i) {
@@ -131,29 +130,36 @@ struct Operand {
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
-  // The next stage into LDS; `kleft`: elements of K from its first on.
-  __device__ __forceinline__ void issue(uint32_t lds, int wave, int lane, int kleft) {
+  // bytes of the first `rows` k-rows of a stage, to a whole unit (KS)
+  __device__ __forceinline__ uint32_t stage_bytes(int rows) const {
+    return ((uint32_t)(((rows - 1) * ld + cols) * 2) + 15u) & ~15u;
+  }
+  // The next stage into LDS.
+  __device__ __forceinline__ void issue(uint32_t lds) {
     if constexpr (KC) {
-      const u32x4_t r = make_rsrc_v(base, bytes);
-      if (kleft < BK) {
-        uint32_t v[INST];
-#pragma unroll
-        for (int i = 0; i < INST; ++i) {
-          int row, c;
-          where(wave, lane, i, row, c);
-          v[i] = c * 8 < kleft ? src[i] : 0x80000000u;
-        }
-        dma16_run<INST>(r, lds, v, koff);
-      } else {
-        dma16_run<INST>(r, lds, src, koff);
-      }
+      dma16_run<INST>(rsrc, lds, src, koff);
       koff += BK * 2;
     } else {
-      const int rows = left < BK ? (int)left : BK;
-      const u32x4_t r = make_rsrc_v(base, rows > 0 ? ((uint32_t)(((rows - 1) * ld + cols) * 2) + 15u) & ~15u : 0u);
-      dma16_run<INST>(r, lds, src, 0u);
-      base += BK * ld;
-      left -= BK;
+      dma16_run<INST>(rsrc, lds, src, 0u);
+      const uint64_t at = ((uint64_t)rsrc[1] << 32 | rsrc[0]) + (uint64_t)(BK * 2) * (uint64_t)ld;
+      rsrc[0] = (uint32_t)at;
+      rsrc[1] = (uint32_t)(at >> 32);
+    }
+  }
+  // The last stage, of 0 < kleft < BK elements of K.
+  __device__ __forceinline__ void issue_short(uint32_t lds, int wave, int lane, int kleft) {
+    if constexpr (KC) {
+      uint32_t v[INST];
+#pragma unroll
+      for (int i = 0; i < INST; ++i) {
+        int row, c;
+        where(wave, lane, i, row, c);
+        v[i] = c * 8 < kleft ? src[i] : 0x80000000u;
+      }
+      dma16_run<INST>(rsrc, lds, v, koff);
+    } else {
+      rsrc[2] = stage_bytes(kleft);
+      dma16_run<INST>(rsrc, lds, src, 0u);
     }
   }
 };
@@ -274,117 +280,125 @@ __device__ __forceinline__ int64_t label_of(const ProductParams& p, int64_t m) {
 // The kernel
 // ---------------------------------------------------------------------------
 
-// Running sums over the groups: rows of group e and of those before it, and the row tiles before it.  64 groups a
-// step, sums by shuffles.  Calls f(lane's group index or more than E, rows, rows before, tiles, tiles before) for
-// each 64; returns all tiles.
-template <int BM, class F>
-__device__ __forceinline__ int64_t scan_groups(const int* counts, int E, int64_t M, F f) {
+// A group and the workgroup's tile among the group's.
+struct GroupTile {
+  int e, beg, rows;  // its rows are beg .. beg + rows
+  int tm, tn;
+};
+
+// Inclusive sums over the wave's lanes; MOST: sums stop there (all values up to 2^30).
+template <bool MOST = false>
+__device__ __forceinline__ uint32_t lanes_below(uint32_t v, uint32_t most = 0) {
   const int ln = threadIdx.x & 63;
-  int64_t rows0 = 0, tiles0 = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    int64_t n = e0 + ln < E ? max(counts[e0 + ln], 0) : 0;
-    int64_t incl = n;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(incl, d, 64);
-      if (ln >= d) incl += y;
-    }
-    // rows behind the buffers' last belong to nobody
-    const int64_t beg = min(rows0 + incl - n, M), end = min(rows0 + incl, M);
-    const int64_t tiles = (end - beg + BM - 1) / BM;
-    int64_t t = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(t, d, 64);
-      if (ln >= d) t += y;
-    }
-    f(e0, beg, end - beg, tiles0 + t - tiles, tiles);
-    rows0 += __shfl(incl, 63, 64);
-    tiles0 += __shfl(t, 63, 64);
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(v, d, 64);
+    if (ln >= d) v = MOST ? min(v + y, most) : v + y;
   }
-  return tiles0;
+  return v;
 }
 
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-  return (int64_t)((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)v) |
-                   (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32)) << 32);
+// Tile i of XCD x, of all groups' tiles: false where there are fewer.
+//
+// The counts are what the device holds, so every workgroup adds them up by itself: 64 groups a step, sums over lanes.
+// Every group's tiles are dealt to all XCDs, ragged 1 by columns (an XCD has all row tiles of a column, which share
+// its weights in L2), ragged 2 by runs of an eighth: with whole groups per XCD, one with half of the rows kept one
+// XCD busy while seven idled (gradient of 32 experts' weights, one of them with 47 % of 7643 rows, 877 us; even
+// groups 385).  Groups of more rows than a tile (products are what bounds them) and of fewer (their weights, or their
+// result, are) take turns in proportion, so that the chip has work of both kinds at any time.
+template <int BM>
+__device__ __forceinline__ bool find_group_tile(const ProductParams& p, int x, int i, GroupTile& out) {
+  const int ln = threadIdx.x & 63, E = p.E;
+  const uint32_t M = (uint32_t)(p.ragged == 1 ? p.M : p.K), per = (uint32_t)(p.ragged == 1 ? p.tiles_n : p.tiles_m * p.tiles_n);
+  uint32_t beg, rows, nt, first, w, large, small;  // of the lane's group: its rows, row tiles, first column or tile,
+                                                   // tiles; sums
+  uint32_t carry = 0, carry_l = 0, carry_s = 0;
+  uint32_t prev_l = 0, prev_s = 0;  // the sums in front of the step
+  auto step = [&](int e0) {
+    prev_l = carry_l;
+    prev_s = carry_s;
+    const int e = e0 + ln;
+    const uint32_t n = e < E ? (uint32_t)min(max((int64_t)p.counts[e], (int64_t)0), (int64_t)M) : 0;
+    const uint32_t incl = min(carry + lanes_below<true>(n, M), M);  // rows behind the buffers' last are nobody's
+    const uint32_t before = __shfl_up(incl, 1, 64);
+    beg = ln == 0 ? carry : before;
+    rows = incl - beg;
+    bool many;
+    if (p.ragged == 1) {
+      nt = (rows + BM - 1) / BM;
+      many = nt > 1;
+    } else {
+      nt = e < E ? 1 : 0;
+      many = rows > 256;
+    }
+    const uint64_t y = (uint32_t)(x + e) & 7;
+    first = (uint32_t)(y * per / 8);
+    w = ((uint32_t)((y + 1) * per / 8) - first) * nt;
+    large = carry_l + lanes_below(many ? w : 0);
+    small = carry_s + lanes_below(many ? 0 : w);
+    carry = __builtin_amdgcn_readlane(incl, 63);
+    carry_l = __builtin_amdgcn_readlane(large, 63);
+    carry_s = __builtin_amdgcn_readlane(small, 63);
+  };
+  for (int e0 = 0; e0 < E; e0 += 64) step(e0);
+  const uint32_t n_l = carry_l, n = carry_l + carry_s;
+  if ((uint32_t)i >= n) return false;
+  const uint32_t both = 2 * min(n_l, carry_s);
+  const bool of_large = (uint32_t)i < both ? !(i & 1) : n_l > carry_s;
+  const uint32_t idx = (uint32_t)i < both ? i / 2 : i - both / 2;
+  carry = carry_l = carry_s = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    if (E > 64) step(e0);  // else as it stands
+    const uint64_t behind = __ballot((of_large ? large : small) > idx);
+    if (!behind) continue;
+    const int l = __builtin_ctzll(behind);  // (groups without such tiles have the sum of the group before)
+    const uint32_t up_to = __shfl(of_large ? large : small, max(l - 1, 0), 64);
+    // the sum up to the group: of the lane before, or of the steps before
+    const uint32_t prev = l > 0 ? up_to : of_large ? prev_l : prev_s;
+    out.e = e0 + l;
+    out.beg = __builtin_amdgcn_readlane(beg, l);
+    out.rows = __builtin_amdgcn_readlane(rows, l);
+    const uint32_t j = idx - prev, f = __builtin_amdgcn_readlane(first, l);
+    if (p.ragged == 1) {
+      const uint32_t t = __builtin_amdgcn_readlane(nt, l), c = __builtin_amdgcn_readlane(w, l) / t;
+      out.tm = (int)(j / c);
+      out.tn = (int)(f + j % c);
+    } else {
+      decode_grouped((int)(f + j), p.tiles_m, p.tiles_n, p.group_m, out.tm, out.tn);
+    }
+    return true;
+  }
+  return false;
 }
+
+// A tile's place: of its group, in C, and which part of its K.
+struct TileSpot {
+  const uint16_t* A;
+  const uint16_t* B;
+  int64_t M, K;      // rows of the group (the matrix), length of the sum
+  int64_t crow;      // first row of the group in C (ragged 1)
+  int64_t coff;      // element offset of the group's C (ragged 2)
+  int tm, tn;        // in tiles of the launch's shape
+  int64_t m0;
+  uint32_t t, part;  // among the tiles that are cut
+  int parts;
+};
 
 template <class C, bool AKC, bool BKC, int EPI>
-__global__ __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(1, C::WAVES_PER_SIMD)))
-void product_kernel(ProductParams p) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+__device__ __forceinline__ void product_tile(const ProductParams& p, const TileSpot& at, char* smem) {
   constexpr bool kSwiglu = EPI == kProdSwiglu;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
-
-  // ---- which tile ----
-  int64_t M = p.M, K = p.K, G = gridDim.x;
-  const uint16_t* A = p.A;
-  const uint16_t* B = p.B;
-  int64_t crow = 0;  // first row of the group in C (ragged 1)
-  int64_t coff = 0;  // element offset of the group's C (ragged 2)
-  if (p.ragged == 1) {
-    const int64_t tiles = scan_groups<C::BM>(p.counts, p.E, p.M, [](int, int64_t, int64_t, int64_t, int64_t) {});
-    G = uniform64(tiles) * p.tiles_n * p.split;
-    if (blockIdx.x >= G) return;
-  }
-  // workgroups are dealt round-robin to the 8 XCDs: each XCD gets a contiguous run of ids, hence neighbouring
-  // tiles, for its L2
-  const uint32_t g = (uint32_t)G, xcd = blockIdx.x & 7;
-  const uint32_t id = xcd * (g >> 3) + min(xcd, g & 7) + (blockIdx.x >> 3);
-  const uint32_t t = id / p.split, part = id - t * p.split;
-  int tm, tn;
-  if (p.ragged == 1) {
-    // group by group, column by column: a group's row tiles share each column of its weights
-    const int64_t rt = t / p.tiles_n;
-    int e = 0;
-    int64_t beg = 0, rows = 0, first = 0, n = 1;
-    scan_groups<C::BM>(p.counts, p.E, p.M, [&](int e0, int64_t b, int64_t r, int64_t t0, int64_t tl) {
-      const uint64_t mine = __ballot(rt >= t0 && rt < t0 + tl);
-      if (mine) {
-        const int l = __builtin_ctzll(mine);
-        e = e0 + l;
-        beg = __shfl(b, l, 64);
-        rows = __shfl(r, l, 64);
-        first = __shfl(t0, l, 64);
-        n = __shfl(tl, l, 64);
-      }
-    });
-    e = __builtin_amdgcn_readfirstlane(e);
-    crow = uniform64(beg);
-    M = uniform64(rows);
-    const int q = (int)(t - uniform64(first) * p.tiles_n), nt = (int)uniform64(n);
-    tm = q % nt;
-    tn = q / nt;
-    A += crow * p.lda;
-    B += e * p.b_stride;
-  } else if (p.ragged == 2) {
-    const int per = p.tiles_m * p.tiles_n, e = t / per;
-    int64_t beg = 0, rows = 0;
-    scan_groups<C::BM>(p.counts, p.E, p.K, [&](int e0, int64_t b, int64_t r, int64_t, int64_t) {
-      if (e >= e0 && e < e0 + 64) {
-        beg = __shfl(b, e - e0, 64);
-        rows = __shfl(r, e - e0, 64);
-      }
-    });
-    beg = uniform64(beg);
-    K = uniform64(rows);
-    A += beg * p.lda;
-    B += beg * p.ldb;
-    coff = e * p.c_stride;
-    decode_grouped(t - e * per, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-  } else {
-    decode_grouped((int)t, p.tiles_m, p.tiles_n, p.group_m, tm, tn);
-  }
-  tm = __builtin_amdgcn_readfirstlane(tm);
-  tn = __builtin_amdgcn_readfirstlane(tn);
-  const int64_t m0 = (int64_t)tm * C::BM;
+  const uint16_t* A = at.A;
+  const uint16_t* B = at.B;
+  const int64_t M = at.M, K = at.K, crow = at.crow, coff = at.coff, m0 = at.m0;
+  const uint32_t t = at.t, part = at.part;
+  const int parts = at.parts, tn = at.tn;
   const int n0 = tn * (kSwiglu ? C::BN / 2 : C::BN);  // SwiGLU: of the output's columns
   const int64_t nk = (K + C::BK - 1) / C::BK;
-  const int64_t s0 = part * nk / p.split;
-  const int ns = (int)((part + 1) * nk / p.split - s0);
+  const int64_t s0 = part * nk / parts;
+  const int ns = (int)((part + 1) * nk / parts - s0);
   const int64_t k0 = s0 * C::BK;
 
   // ---- operands ----
@@ -414,50 +428,62 @@ void product_kernel(ProductParams p) {
     for (int j = 0; j < C::FN; ++j)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
-  uint32_t wr = 0;
-  int64_t kleft = K - k0;
+  // whole stages, and what the sum's last one holds if it is shorter
+  const int nf = (int)min<int64_t>(ns, (K - k0) / C::BK), rest = ns > nf ? (int)(K - k0 - (int64_t)nf * C::BK) : 0;
+  uint32_t wr = lds_base, rd = 0;
+  const uint32_t a_lds = wave * (C::A_INST * 1024), b_lds = C::A_BYTES + wave * (C::B_INST * 1024);
+  auto next_slot = [](uint32_t o, uint32_t base) { return o + C::STAGE == base + C::S * C::STAGE ? base : o + C::STAGE; };
   auto issue = [&] {
-    const int kl = kleft < C::BK ? (int)kleft : C::BK;
-    a.issue(lds_base + wr + wave * (C::A_INST * 1024), wave, lane, kl);
-    b.issue(lds_base + wr + C::A_BYTES + wave * (C::B_INST * 1024), wave, lane, kl);
-    kleft -= C::BK;
-    wr = wr + C::STAGE == C::S * C::STAGE ? 0u : wr + C::STAGE;
+    a.issue(wr + a_lds);
+    b.issue(wr + b_lds);
+    wr = next_slot(wr, lds_base);
   };
-  if (ns > 0) {
+  auto issue_short = [&] {
+    a.issue_short(wr + a_lds, wave, lane, rest);
+    b.issue_short(wr + b_lds, wave, lane, rest);
+  };
+  // stage j, which may be the short one or none
+  auto issue_any = [&](int j) {
+    if (j < nf) issue();
+    else if (j < ns) issue_short();
+  };
+  // Row blocks of 32 that hold a row: a wave leaves the others' reads and matrix instructions out, which is what makes
+  // tall tiles stream a small group's weights as fast as flat ones would.
+  const int active = (int)min<int64_t>(max<int64_t>((M - m0 - wm * C::WTM + 31) / 32, 0), C::FM);
+  auto main_loop = [&](auto blocks_) {
+    constexpr int F = decltype(blocks_)::value;
     if constexpr (C::PP) {
       // Two groups of four waves, one wave of each on every SIMD: while one
       // reads a stage's operands from LDS (and loads the stage S - 1 ahead into
       // the slot that the stage before left), the other runs its matrix
       // instructions, so each SIMD's matrix core is fed while the partner loads.
-      bf16x8 af[C::KSTEPS][C::FM], bf[C::KSTEPS][C::FN];
-      uint32_t rd = 0;
+      // The loops over whole stages hold no test but their own: a memory step
+      // has to fit beside the 512 cycles of the partner's matrix instructions.
+      bf16x8 af[C::KSTEPS][F > 0 ? F : 1], bf[C::KSTEPS][C::FN];
       auto read_stage = [&] {
-        const char* sA = smem + rd;
-        const char* sB = sA + C::A_BYTES;
+        if constexpr (F > 0) {
+          const char* sA = smem + rd;
+          const char* sB = sA + C::A_BYTES;
 #pragma unroll
-        for (int kk = 0; kk < C::KSTEPS; ++kk) {
+          for (int kk = 0; kk < C::KSTEPS; ++kk) {
 #pragma unroll
-          for (int i = 0; i < C::FM; ++i) af[kk][i] = a.read(sA, kk, i);
+            for (int i = 0; i < F; ++i) af[kk][i] = a.read(sA, kk, i);
 #pragma unroll
-          for (int j = 0; j < C::FN; ++j) bf[kk][j] = b.read(sB, kk, j);
+            for (int j = 0; j < C::FN; ++j) bf[kk][j] = b.read(sB, kk, j);
+          }
+          rd = next_slot(rd, 0u);
         }
-        rd = rd + C::STAGE == C::S * C::STAGE ? 0u : rd + C::STAGE;
       };
       auto mfma = [&] {
 #pragma unroll
         for (int kk = 0; kk < C::KSTEPS; ++kk)
 #pragma unroll
-          for (int i = 0; i < C::FM; ++i)
+          for (int i = 0; i < F; ++i)
 #pragma unroll
             for (int j = 0; j < C::FN; ++j)
               acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[kk][j], af[kk][i], acc[i][j], 0, 0, 0);
       };
-      const bool first = wave < C::WAVES / 2;
-      auto mem_step = [&](int j) {
-        if (first && j + C::S - 1 < ns) issue();
-        read_stage();
-        if (!first && j + C::S - 1 < ns) issue();
-      };
+      // stage j + 1 has landed: S - 2 younger ones may be in flight, or as many as there are
       auto wait_next = [&](int j) {
         if (j + C::S - 1 < ns) wait_vm<(C::S - 2) * C::LOADS>();
         else if (j + 1 < ns) wait_stage<C::S + 1, C::LOADS>(min(C::S - 2, ns - 2 - j));
@@ -467,75 +493,110 @@ void product_kernel(ProductParams p) {
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
       };
-#pragma unroll
-      for (int s = 0; s < C::S - 1; ++s)
-        if (s < ns) issue();
-      wait_stage<C::S + 1, C::LOADS>(min(C::S - 2, ns - 1));
-      __syncthreads();
-      if (first) {
-        mem_step(0);
-        for (int j = 0; j < ns; ++j) {
+      int j = 0;
+      if (wave < C::WAVES / 2) {
+#pragma clang loop unroll(disable)
+        for (; j + C::S - 1 < nf; ++j) {
+          issue();
+          read_stage();
+          bar();
+          mfma();
+          wait_vm<(C::S - 2) * C::LOADS>();
+          bar();
+        }
+#pragma clang loop unroll(disable)
+        for (; j < ns; ++j) {
+          issue_any(j + C::S - 1);
+          read_stage();
           bar();
           mfma();
           wait_next(j);
           bar();
-          if (j + 1 < ns) mem_step(j + 1);
         }
       } else {
-        for (int j = 0; j < ns; ++j) {
+#pragma clang loop unroll(disable)
+        for (; j + C::S - 1 < nf; ++j) {
           bar();
-          mem_step(j);
+          read_stage();
+          issue();
+          wait_vm<(C::S - 2) * C::LOADS>();
+          bar();
+          mfma();
+        }
+#pragma clang loop unroll(disable)
+        for (; j < ns; ++j) {
+          bar();
+          read_stage();
+          issue_any(j + C::S - 1);
           wait_next(j);
           bar();
           mfma();
         }
       }
-      __syncthreads();
     } else {
-      uint32_t rd = 0;
+      // All of a stage's reads go out before its matrix instructions: left alone, the compiler spares registers and
+      // waits for one read after another (512 x 4096 x 4096 on 128 x 128 tiles 41.8 us so).
       auto compute = [&] {
-        const char* sA = smem + rd;
-        const char* sB = sA + C::A_BYTES;
+        if constexpr (F > 0) {
+          const char* sA = smem + rd;
+          const char* sB = sA + C::A_BYTES;
+          bf16x8 af[C::KSTEPS][F > 0 ? F : 1], bf[C::KSTEPS][C::FN];
 #pragma unroll
-        for (int kk = 0; kk < C::KSTEPS; ++kk) {
-          bf16x8 af[C::FM], bf[C::FN];
+          for (int kk = 0; kk < C::KSTEPS; ++kk) {
 #pragma unroll
-          for (int i = 0; i < C::FM; ++i) af[i] = a.read(sA, kk, i);
+            for (int i = 0; i < F; ++i) af[kk][i] = a.read(sA, kk, i);
 #pragma unroll
-          for (int j = 0; j < C::FN; ++j) bf[j] = b.read(sB, kk, j);
+            for (int j = 0; j < C::FN; ++j) bf[kk][j] = b.read(sB, kk, j);
+          }
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < C::FM; ++i)
+          for (int kk = 0; kk < C::KSTEPS; ++kk)
 #pragma unroll
-            for (int j = 0; j < C::FN; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[j], af[i], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+              for (int j = 0; j < C::FN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[kk][j], af[kk][i], acc[i][j], 0, 0, 0);
+          rd = next_slot(rd, 0u);
         }
-        rd = rd + C::STAGE == C::S * C::STAGE ? 0u : rd + C::STAGE;
       };
-#pragma unroll
-      for (int s = 0; s < C::S - 1; ++s)
-        if (s < ns) issue();
       // Each barrier says that every wave's share of stage j has landed and that every wave has read stage j - 1,
       // whose slot the next DMA overwrites.
       int j = 0;
-      for (; j + C::S - 1 < ns; ++j) {
+#pragma clang loop unroll(disable)
+      for (; j + C::S - 1 < nf; ++j) {
         wait_vm<(C::S - 2) * C::LOADS>();
         __syncthreads();
         issue();
         compute();
       }
+#pragma clang loop unroll(disable)
       for (; j < ns; ++j) {
-        wait_stage<C::S + 1, C::LOADS>(ns - 1 - j);
+        wait_stage<C::S + 1, C::LOADS>(min(C::S - 2, ns - 1 - j));
         __syncthreads();
+        issue_any(j + C::S - 1);
         compute();
       }
-      __syncthreads();  // the ring is free: the exchange and the epilogue use it
     }
+  };
+  if (ns > 0) {
+#pragma unroll
+    for (int s = 0; s < C::S - 1; ++s) issue_any(s);
+    if constexpr (C::PP) {
+      wait_stage<C::S + 1, C::LOADS>(min(C::S - 2, ns - 1));
+      __syncthreads();
+    }
+    // (every variant passes the same barriers)
+    if (active > C::FM / 2) main_loop(std::integral_constant<int, C::FM>{});
+    else if (C::FM >= 4 && active > C::FM / 4) main_loop(std::integral_constant<int, C::FM / 2>{});
+    else if (C::FM >= 2 && active > 0) main_loop(std::integral_constant<int, (C::FM + 3) / 4>{});
+    else main_loop(std::integral_constant<int, 0>{});
+    __syncthreads();  // the ring is free: the exchange and the epilogue use it
   }
 
   // ---- parts of the tile's K ----
-  if (p.split > 1) {
+  if (parts > 1) {
     constexpr int64_t TILE = (int64_t)C::BM * C::BN;
-    float* slot0 = p.parts + (int64_t)t * p.split * TILE;
+    float* slot0 = p.parts + (int64_t)t * parts * TILE;
     {
       const __amdgpu_buffer_rsrc_t r = make_rsrc(slot0 + part * TILE, (uint32_t)(TILE * 4));
 #pragma unroll
@@ -552,13 +613,13 @@ void product_kernel(ProductParams p) {
     int* sh = reinterpret_cast<int*>(smem);
     if (tid == 0) {
       const uint32_t n = __hip_atomic_fetch_add(p.tickets + t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (n == p.split - 1u) __hip_atomic_store(p.tickets + t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (n == parts - 1u) __hip_atomic_store(p.tickets + t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       sh[0] = (int)n;
     }
     __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(sh[0]) != p.split - 1) return;
+    if (__builtin_amdgcn_readfirstlane(sh[0]) != parts - 1) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    for (int q = 0; q < p.split; ++q) {
+    for (int q = 0; q < parts; ++q) {
       const __amdgpu_buffer_rsrc_t r = make_rsrc(slot0 + q * TILE, (uint32_t)(TILE * 4));
       // eight loads in flight: more take registers that the sums need
       constexpr int AT_ONCE = C::UNITS < 8 ? C::UNITS : 8;
@@ -703,35 +764,94 @@ void product_kernel(ProductParams p) {
   }
 }
 
-template <class C, bool AKC, bool BKC, int EPI>
+// FLAT: the shape for row tiles of at most its height (of small groups), C's otherwise; both as wide.
+template <class C, class FLAT, bool AKC, bool BKC, int EPI>
+__global__ __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(1, C::WAVES_PER_SIMD)))
+void product_kernel(ProductParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  // Workgroups are dealt round-robin to the 8 XCDs: each XCD gets neighbouring tiles, for its L2.
+  TileSpot at = {p.A, p.B, p.M, p.K, 0, 0, 0, 0, 0, 0, 0, 1};
+  if (p.ragged) {
+    GroupTile g;
+    if (!find_group_tile<C::BM>(p, blockIdx.x & 7, blockIdx.x >> 3, g)) return;
+    at.tm = g.tm;
+    at.tn = g.tn;
+    at.A += (int64_t)g.beg * p.lda;
+    if (p.ragged == 1) {
+      at.crow = g.beg;
+      at.M = g.rows;
+      at.B += g.e * p.b_stride;
+    } else {
+      at.K = g.rows;
+      at.B += (int64_t)g.beg * p.ldb;
+      at.coff = g.e * p.c_stride;
+    }
+  } else {
+    // tiles below p.whole, then the parts of the others
+    const bool whole = blockIdx.x < (uint32_t)p.whole;
+    const uint32_t b = whole ? blockIdx.x : blockIdx.x - p.whole, n = whole ? p.whole : gridDim.x - p.whole;
+    const uint32_t xcd = b & 7, id = xcd * (n >> 3) + min(xcd, n & 7) + (b >> 3);
+    at.t = id;
+    if (!whole) {
+      at.parts = p.split;
+      at.t = id / at.parts;
+      at.part = id - at.t * at.parts;
+    }
+    decode_grouped((int)(whole ? at.t : at.t + p.whole), p.tiles_m, p.tiles_n, p.group_m, at.tm, at.tn);
+  }
+  at.tm = __builtin_amdgcn_readfirstlane(at.tm);
+  at.tn = __builtin_amdgcn_readfirstlane(at.tn);
+  at.m0 = (int64_t)at.tm * C::BM;
+  if constexpr (!std::is_void_v<FLAT>) {
+    static_assert(FLAT::BN == C::BN && FLAT::NT == C::NT, "flat tiles");
+    if (p.ragged == 1 && at.M - at.m0 <= FLAT::BM) {
+      product_tile<FLAT, AKC, BKC, EPI>(p, at, smem);
+      return;
+    }
+  }
+  product_tile<C, AKC, BKC, EPI>(p, at, smem);
+}
+
+template <class C, class FLAT, bool AKC, bool BKC, int EPI>
 hipError_t launch_product_cfg(const ProductParams& p, int64_t grid, hipStream_t stream) {
   static PerDeviceFlag attr_set;
+  uint32_t lds = C::LDS_BYTES;
+  if constexpr (!std::is_void_v<FLAT>) lds = std::max<uint32_t>(lds, FLAT::LDS_BYTES);
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return e;
   if (!attr_set.is_set(dev)) {
-    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<C, AKC, BKC, EPI>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS_BYTES);
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(&product_kernel<C, FLAT, AKC, BKC, EPI>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
     attr_set.set(dev);
   }
-  hipLaunchKernelGGL((product_kernel<C, AKC, BKC, EPI>), dim3((unsigned)grid), dim3(C::NT), C::LDS_BYTES, stream, p);
+  hipLaunchKernelGGL((product_kernel<C, FLAT, AKC, BKC, EPI>), dim3((unsigned)grid), dim3(C::NT), lds, stream, p);
   return hipGetLastError();
 }
 
 // The tile shapes, in the order of ProductTile.
 using ProdTile32 = PCfg<32, 128, 1, 2, 64, 4>;
-using ProdTile64 = PCfg<64, 128, 2, 2, 64, 3>;
+using ProdTile64 = PCfg<64, 64, 2, 1, 64, 4>;
+using ProdTile64w = PCfg<64, 128, 2, 2, 64, 3>;
 using ProdTile128 = PCfg<128, 128, 4, 2, 64, 2>;
 using ProdTile256 = PCfg<256, 256, 2, 4, 32, 4, true>;
+// of 256-row tiles that hold 128 rows or fewer: the ring holds more of B's stages, 64 KB or more in flight instead of
+// 48; rows along the sum come in whole 128-byte lines
+template <bool BKC>
+using ProdFlat256 = std::conditional_t<BKC, PCfg<128, 256, 2, 4, 64, 3>, PCfg<128, 256, 2, 4, 32, 6>>;
 
 template <bool AKC, bool BKC, int EPI>
 hipError_t launch_product_tile(const ProductParams& p, int tile, int64_t grid, hipStream_t stream) {
   switch (tile) {
-    case kProd32: return launch_product_cfg<ProdTile32, AKC, BKC, EPI>(p, grid, stream);
-    case kProd64: return launch_product_cfg<ProdTile64, AKC, BKC, EPI>(p, grid, stream);
-    case kProd128: return launch_product_cfg<ProdTile128, AKC, BKC, EPI>(p, grid, stream);
-    case kProd256: return launch_product_cfg<ProdTile256, AKC, BKC, EPI>(p, grid, stream);
+    case kProd32: return launch_product_cfg<ProdTile32, void, AKC, BKC, EPI>(p, grid, stream);
+    case kProd64: return launch_product_cfg<ProdTile64, void, AKC, BKC, EPI>(p, grid, stream);
+    case kProd64w: return launch_product_cfg<ProdTile64w, void, AKC, BKC, EPI>(p, grid, stream);
+    case kProd128: return launch_product_cfg<ProdTile128, void, AKC, BKC, EPI>(p, grid, stream);
+    case kProd256:
+      // only the epilogues of expert products see small groups
+      if constexpr (EPI <= kProdSwigluGrad) return launch_product_cfg<ProdTile256, ProdFlat256<BKC>, AKC, BKC, EPI>(p, grid, stream);
+      else return launch_product_cfg<ProdTile256, void, AKC, BKC, EPI>(p, grid, stream);
   }
   return hipErrorInvalidValue;
 }

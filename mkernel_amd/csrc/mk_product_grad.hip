@@ -15,9 +15,10 @@ hipError_t launch_product_left_grad(const ProductParams& p, int epi, int tile, i
 
 hipError_t launch_product_right_grad(const ProductParams& p, int tile, int64_t grid, hipStream_t stream) {
   switch (tile) {
-    case kProd64: return launch_product_cfg<ProdTile64, false, false, kProdStore>(p, grid, stream);
-    case kProd128: return launch_product_cfg<ProdTile128, false, false, kProdStore>(p, grid, stream);
-    case kProd256: return launch_product_cfg<ProdTile256, false, false, kProdStore>(p, grid, stream);
+    case kProd64: return launch_product_cfg<ProdTile64, void, false, false, kProdStore>(p, grid, stream);
+    case kProd64w: return launch_product_cfg<ProdTile64w, void, false, false, kProdStore>(p, grid, stream);
+    case kProd128: return launch_product_cfg<ProdTile128, void, false, false, kProdStore>(p, grid, stream);
+    case kProd256: return launch_product_cfg<ProdTile256, void, false, false, kProdStore>(p, grid, stream);
   }
   return hipErrorInvalidValue;
 }
