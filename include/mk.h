@@ -28,6 +28,7 @@ extern "C" {
 #define MK_ESHAPE (-2)   /* shape not supported by the tiling */
 #define MK_EDEVICE (-3)  /* no usable device / wrong architecture */
 #define MK_ETIMEOUT (-4) /* a bounded flag wait expired (error word set) */
+#define MK_EWORKSPACE (-5) /* the workspace is too small: nothing was queued (mk_gemm_act and the entry points behind it) */
 
 #define MK_ROW_BLOCK 128 /* flag / expert-padding granularity (rows) */
 
@@ -715,7 +716,7 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* args, void* stream);
  * the workspace's own need not).  `tickets`: MK_PRODUCT_TICKETS 32-bit words,
  * zero before their first use, left zero by every call; launches that share
  * them must be ordered. */
-#define MK_PRODUCT_TICKETS 1024
+#define MK_PRODUCT_TICKETS 8192
 
 #define MK_ACT_NONE 0
 #define MK_ACT_RELU 1

@@ -70,7 +70,7 @@ EXPORTS = (
 # entry points with a workspace of mk_..._workspace_bytes(args) bytes
 _PRODUCTS = ("mk_gemm_act", "mk_gemm_act_backward", "mk_moe_ragged_gemm", "mk_moe_ragged_dgrad", "mk_moe_ragged_wgrad",
              "mk_vocab_loss", "mk_vocab_loss_backward")
-PRODUCT_TICKETS = 1024  # include/mk.h MK_PRODUCT_TICKETS
+PRODUCT_TICKETS = 8192  # include/mk.h MK_PRODUCT_TICKETS
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # MK_ACT_*
 
 vp = C.c_void_p
@@ -366,6 +366,12 @@ def _packer(cls):
 
 def call_values(fn: str, cls, stream: int, *values) -> None:
     """call(fn, cls(*values), stream); a null pointer is 0 (or None)."""
+    rc = _call(fn, cls, stream, values)
+    if rc:
+        check(fn, rc)
+
+
+def _call(fn, cls, stream, values):
     f = _functions.get(fn)
     if f is None:
         f = _functions[fn] = getattr(lib(), fn)
@@ -377,9 +383,18 @@ def call_values(fn: str, cls, stream: int, *values) -> None:
             raise ValueError(f"{fn}: {err}") from None
         block = cls(*values)
         args = C.addressof(block)
-    rc = f(args, stream or None)
-    if rc:
+    return f(args, stream or None)
+
+
+EWORKSPACE = -5  # include/mk.h MK_EWORKSPACE
+
+
+def call_with_workspace(fn: str, cls, stream: int, *values) -> bool:
+    """call_values, but False where the workspace is too small."""
+    rc = _call(fn, cls, stream, values)
+    if rc and rc != EWORKSPACE:
         check(fn, rc)
+    return not rc
 
 
 def workspace_bytes(fn: str, cls, *values) -> int:

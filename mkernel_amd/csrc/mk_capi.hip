@@ -1381,7 +1381,7 @@ int with_space(const char* fn, void* ws, int64_t bytes, F body) {
   Space sp;
   if (int rc = body(sp)) return rc;
   if (sp.peak > 0 && (!ws || bytes < sp.peak))
-    return fail(MK_EINVAL, "%s: the workspace must hold %lld bytes", fn, (long long)sp.peak);
+    return fail(MK_EWORKSPACE, "%s: the workspace must hold %lld bytes", fn, (long long)sp.peak);
   if (!aligned16(ws)) return fail(MK_EINVAL, "%s: the workspace must be 16-byte aligned", fn);
   Space work;
   work.base = static_cast<char*>(ws);
@@ -1416,7 +1416,8 @@ struct Products {
     p.whole = (int)plan.whole;
     int64_t grid = plan.whole + (plan.tiles - plan.whole) * plan.split;
     // ragged: at most that many workgroups for one of the 8 XCDs, of rows when every group's last tile holds one
-    if (p.ragged == 1) grid = 8 * ((tn + 7) / 8) * std::min(tm + groups - 1, p.M);
+    // (a group of t row tiles: ceil(tn / 8) t, or ceil(tn / 4) ceil(t / 2) <= ceil(tn / 8) (t + 1))
+    if (p.ragged == 1) grid = 8 * ((tn + 7) / 8) * std::min(tm + 2 * groups - 1, 2 * p.M);
     if (p.ragged == 2) grid = 8 * ((tm * tn + 7) / 8) * groups;
     if (grid >= (1LL << 31)) return fail(MK_ESHAPE, "%s: too many tiles", fn);
     const int64_t mark = sp.used;
@@ -1528,11 +1529,12 @@ int check_gemm_act(const char* fn, const mk_gemm_act_args* a) {
 
 int gemm_act_body(const mk_gemm_act_args* a, Products g) {
   if (a->M == 0 || a->N == 0) return MK_OK;
+  const bool few = mk::product_few_rows(a->M, a->N, a->K, aligned16(a->B) && (a->ldb % 8 == 0 || a->K <= 1));
   mk::ProductParams p = {};
   p.A = u16(a->A); p.B = u16(a->B);
   p.lda = a->lda; p.ldb = a->ldb;
   p.M = a->M; p.N = a->N; p.K = a->K; p.b_cols = a->N;
-  if (a->K > 0) {
+  if (a->K > 0 && !few) {
     if (int rc = g.rows(p.A, a->M, a->K, p.lda, true)) return rc;
     if (int rc = g.rows(p.B, a->K, a->N, p.ldb, false)) return rc;
   }
@@ -1543,6 +1545,7 @@ int gemm_act_body(const mk_gemm_act_args* a, Products g) {
   p.pre = static_cast<uint16_t*>(a->pre); p.ldp = a->ldp;
   p.vec = (vec_rows(a->C, a->ldc, a->c_type) ? mk::kVecC : 0) | (vec_rows(a->residual, a->ldr, a->residual_type) ? mk::kVecRes : 0) |
           (vec_rows(a->pre, a->ldp, 1) ? mk::kVecPre : 0) | (aligned16(a->bias) ? mk::kVecBias : 0);
+  if (few) return g.sp.counting ? MK_OK : g.launched(mk::launch_product_few_rows(p, g.stream));
   return g.run(mk::kProdForward, mk::kProdStore, p, a->N);
 }
 
@@ -1764,7 +1767,7 @@ int vocab_loss_body(const mk_vocab_loss_args* a, Products g) {
   // weights that have to be laid out anew go piece by piece
   const bool direct = aligned16(a->W) && a->ldw % 8 == 0;
   const int64_t piece = direct ? a->V : piece_of(a->H, a->V);
-  const int64_t most_groups = (a->V + 63) / 64 + 8 * ((a->V + piece - 1) / piece);
+  const int64_t most_groups = (a->V + 63) / 64 + (a->V + piece - 1) / piece;  // no tile is narrower
   float2* stats = static_cast<float2*>(g.sp.take(most_groups * a->T * 8));
   int64_t groups = 0;
   for (int64_t c0 = 0; c0 < a->V; c0 += piece) {
@@ -1778,7 +1781,7 @@ int vocab_loss_body(const mk_vocab_loss_args* a, Products g) {
     int tile = 0;
     if (int rc = g.run(mk::kProdForward, mk::kProdStats, p, p.N, &tile)) return rc;
     const mk::ProductShape& s = mk::kProductShapes[tile];
-    groups += (p.N + s.bn - 1) / s.bn * s.waves_n;
+    groups += (p.N + s.bn - 1) / s.bn;
     g.sp.used = mark;
   }
   if (g.sp.counting) return MK_OK;
@@ -1907,7 +1910,7 @@ int product_call(const char* fn, const A* a, Check check, Body body, void* ticke
   });
 }
 
-static_assert(MK_PRODUCT_TICKETS == mk::kProductTickets, "tickets");
+static_assert(MK_PRODUCT_TICKETS == mk::kProductTickets * mk::kTicketStride, "tickets");
 
 }  // namespace
 

@@ -276,7 +276,7 @@ struct ProductParams {
   // tiles
   int tiles_m, tiles_n, group_m;
   int whole, split;         // tiles from `whole` on are cut into `split` parts along K
-  uint32_t* tickets;        // one per cut tile, zero between launches
+  uint32_t* tickets;        // one per cut tile, kTicketStride words apart, zero between launches
   float* parts;             // a tile per part
   // epilogue
   int vec, act;
@@ -295,7 +295,7 @@ struct ProductParams {
   const void* labels;
   int labels64;
   int64_t ignore, label0, vocab, first_col;
-  float2* stats;            // [column groups][M]
+  float2* stats;            // [column tiles][M]
   float* target;
   const float* lse;
   const float* dloss;
@@ -303,6 +303,8 @@ struct ProductParams {
 hipError_t launch_product_forward(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
 hipError_t launch_product_left_grad(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
 hipError_t launch_product_right_grad(const ProductParams& p, int tile, int64_t grid, hipStream_t stream);
+// Forward, plain epilogue, one row or two: operands of any alignment.
+hipError_t launch_product_few_rows(const ProductParams& p, hipStream_t stream);
 // Rows of bf16 into rows of a multiple of 8 elements, zeros behind the last: `parts` pieces of `cols` columns each,
 // one behind the other, every piece filled up to `width`; groups (counts, E) that have no rows are left out.
 // labels: rows whose label is `ignore` become zeros.

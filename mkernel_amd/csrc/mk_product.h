@@ -46,7 +46,8 @@ struct PCfg {
   static constexpr int A_INST = A_BYTES / 1024 / WAVES, B_INST = B_BYTES / 1024 / WAVES, LOADS = A_INST + B_INST;
   static constexpr int PITCH = WTN * 4 + 16;  // bytes of an epilogue row
   static constexpr uint32_t EPI_BYTES = WAVES * 32 * PITCH;
-  static constexpr uint32_t LDS_BYTES = S * STAGE > EPI_BYTES ? S * STAGE : EPI_BYTES;
+  static constexpr uint32_t STATS_BYTES = WN * BM * 8;  // behind them, of the vocabulary's epilogue
+  static constexpr uint32_t LDS_BYTES = S * STAGE > EPI_BYTES + STATS_BYTES ? S * STAGE : EPI_BYTES + STATS_BYTES;
   static constexpr int PER_CU = 160 * 1024 / LDS_BYTES;
   static constexpr int WAVES_PER_SIMD = PER_CU * WAVES / 4 > 0 ? PER_CU * WAVES / 4 : 1;
   static constexpr int UNITS = FM * FN * 4;  // 16-byte units of sums per thread
@@ -268,6 +269,13 @@ __device__ __forceinline__ void for_act(int act, F f) {
   }
 }
 
+// (largest, sum of exponentials relative to it) of two sets of columns.
+__device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
+  const float to = fmaxf(a.x, b.x);
+  const float ref = to == -INFINITY ? 0.f : to;  // all of it -inf: sums are 0 (or NaN, which stays)
+  return {to, a.y * __expf(a.x - ref) + b.y * __expf(b.x - ref)};
+}
+
 // Label of token m among this call's columns, -1: another shard's, -2: no loss.
 __device__ __forceinline__ int64_t label_of(const ProductParams& p, int64_t m) {
   const int64_t l = p.labels64 ? static_cast<const int64_t*>(p.labels)[m] : static_cast<const int*>(p.labels)[m];
@@ -286,15 +294,18 @@ struct GroupTile {
   int tm, tn;
 };
 
-// Inclusive sums over the wave's lanes; MOST: sums stop there (all values up to 2^30).
+// Inclusive sums over the wave's lanes; MOST: sums stop there (all values up to 2^30).  By lane shifts inside the vector
+// unit (1, 2, 4, 8 lanes within rows of 16, then the last lanes of rows to those behind): six shuffles through LDS, one
+// after another, took a third of a microsecond.
 template <bool MOST = false>
 __device__ __forceinline__ uint32_t lanes_below(uint32_t v, uint32_t most = 0) {
-  const int ln = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t y = __shfl_up(v, d, 64);
-    if (ln >= d) v = MOST ? min(v + y, most) : v + y;
-  }
+  auto add = [&](uint32_t y) { v = MOST ? min(v + y, most) : v + y; };
+  add(__builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));   // row_shr 1
+  add(__builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));   // row_shr 2
+  add(__builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));   // row_shr 4
+  add(__builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));   // row_shr 8
+  add(__builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));  // row_bcast 15, into rows 1 and 3
+  add(__builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));  // row_bcast 31, into rows 2 and 3
   return v;
 }
 
@@ -302,16 +313,16 @@ __device__ __forceinline__ uint32_t lanes_below(uint32_t v, uint32_t most = 0) {
 //
 // The counts are what the device holds, so every workgroup adds them up by itself: 64 groups a step, sums over lanes.
 // Every group's tiles are dealt to all XCDs, ragged 1 by columns (an XCD has all row tiles of a column, which share
-// its weights in L2), ragged 2 by runs of an eighth: with whole groups per XCD, one with half of the rows kept one
+// its weights in L2; from four row tiles on, half of them and twice the columns), ragged 2 by runs of an eighth: with whole groups per XCD, one with half of the rows kept one
 // XCD busy while seven idled (gradient of 32 experts' weights, one of them with 47 % of 7643 rows, 877 us; even
 // groups 385).  Groups of more rows than a tile (products are what bounds them) and of fewer (their weights, or their
-// result, are) take turns in proportion, so that the chip has work of both kinds at any time.
+// result, are) take turns while there are both, so that the chip has work of both kinds.
 template <int BM>
 __device__ __forceinline__ bool find_group_tile(const ProductParams& p, int x, int i, GroupTile& out) {
   const int ln = threadIdx.x & 63, E = p.E;
   const uint32_t M = (uint32_t)(p.ragged == 1 ? p.M : p.K), per = (uint32_t)(p.ragged == 1 ? p.tiles_n : p.tiles_m * p.tiles_n);
-  uint32_t beg, rows, nt, first, w, large, small;  // of the lane's group: its rows, row tiles, first column or tile,
-                                                   // tiles; sums
+  // of the lane's group: its rows; its row tiles, first column (ragged 2: tile) and tiles on this XCD; sums of those
+  uint32_t beg, rows, row0, nt, first, w, large, small;
   uint32_t carry = 0, carry_l = 0, carry_s = 0;
   uint32_t prev_l = 0, prev_s = 0;  // the sums in front of the step
   auto step = [&](int e0) {
@@ -320,20 +331,17 @@ __device__ __forceinline__ bool find_group_tile(const ProductParams& p, int x, i
     const int e = e0 + ln;
     const uint32_t n = e < E ? (uint32_t)min(max((int64_t)p.counts[e], (int64_t)0), (int64_t)M) : 0;
     const uint32_t incl = min(carry + lanes_below<true>(n, M), M);  // rows behind the buffers' last are nobody's
-    const uint32_t before = __shfl_up(incl, 1, 64);
-    beg = ln == 0 ? carry : before;
+    beg = __builtin_amdgcn_update_dpp(carry, incl, 0x138, 0xf, 0xf, false);  // wave_shr 1, the carry into lane 0
     rows = incl - beg;
-    bool many;
-    if (p.ragged == 1) {
-      nt = (rows + BM - 1) / BM;
-      many = nt > 1;
-    } else {
-      nt = e < E ? 1 : 0;
-      many = rows > 256;
-    }
     const uint64_t y = (uint32_t)(x + e) & 7;
-    first = (uint32_t)(y * per / 8);
-    w = ((uint32_t)((y + 1) * per / 8) - first) * nt;
+    const uint32_t tiles = p.ragged == 1 ? (rows + BM - 1) / BM : e < E;
+    const bool many = p.ragged == 1 ? tiles > 1 : rows > 256, halves = p.ragged == 1 && tiles >= 4;
+    const uint32_t sh = halves ? 2 : 3;
+    const uint64_t yc = halves ? y & 3 : y, yr = halves ? y >> 2 : 0;
+    row0 = yr ? tiles / 2 : 0;
+    nt = halves ? (yr ? tiles - tiles / 2 : tiles / 2) : tiles;
+    first = (uint32_t)(yc * per >> sh);
+    w = ((uint32_t)((yc + 1) * per >> sh) - first) * nt;
     large = carry_l + lanes_below(many ? w : 0);
     small = carry_s + lanes_below(many ? 0 : w);
     carry = __builtin_amdgcn_readlane(incl, 63);
@@ -352,7 +360,7 @@ __device__ __forceinline__ bool find_group_tile(const ProductParams& p, int x, i
     const uint64_t behind = __ballot((of_large ? large : small) > idx);
     if (!behind) continue;
     const int l = __builtin_ctzll(behind);  // (groups without such tiles have the sum of the group before)
-    const uint32_t up_to = __shfl(of_large ? large : small, max(l - 1, 0), 64);
+    const uint32_t up_to = __builtin_amdgcn_readlane(of_large ? large : small, max(l - 1, 0));
     // the sum up to the group: of the lane before, or of the steps before
     const uint32_t prev = l > 0 ? up_to : of_large ? prev_l : prev_s;
     out.e = e0 + l;
@@ -361,7 +369,7 @@ __device__ __forceinline__ bool find_group_tile(const ProductParams& p, int x, i
     const uint32_t j = idx - prev, f = __builtin_amdgcn_readlane(first, l);
     if (p.ragged == 1) {
       const uint32_t t = __builtin_amdgcn_readlane(nt, l), c = __builtin_amdgcn_readlane(w, l) / t;
-      out.tm = (int)(j / c);
+      out.tm = (int)(__builtin_amdgcn_readlane(row0, l) + j / c);
       out.tn = (int)(f + j % c);
     } else {
       decode_grouped((int)(f + j), p.tiles_m, p.tiles_n, p.group_m, out.tm, out.tn);
@@ -597,6 +605,10 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
   if (parts > 1) {
     constexpr int64_t TILE = (int64_t)C::BM * C::BN;
     float* slot0 = p.parts + (int64_t)t * parts * TILE;
+    // 16-byte unit u of thread tid; rows behind the last are neither written nor read (offsets past the buffer's end)
+    uint32_t off[C::FM];
+#pragma unroll
+    for (int i = 0; i < C::FM; ++i) off[i] = m0 + wm * C::WTM + 32 * i + (lane & 31) < M ? tid * 16 : 0x80000000u;
     {
       const __amdgpu_buffer_rsrc_t r = make_rsrc(slot0 + part * TILE, (uint32_t)(TILE * 4));
 #pragma unroll
@@ -605,37 +617,48 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = acc[u / (C::FN * 4)][(u / 4) % C::FN][4 * (u % 4) + i];
         // SC1: performed at agent scope once vmcnt says that it is stored
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), r, tid * 16, u * C::NT * 16, 0x10);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), r, off[u / (C::FN * 4)], u * C::NT * 16, 0x10);
       }
     }
     wait_vmem_all();
     __syncthreads();
     int* sh = reinterpret_cast<int*>(smem);
     if (tid == 0) {
-      const uint32_t n = __hip_atomic_fetch_add(p.tickets + t, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (n == parts - 1u) __hip_atomic_store(p.tickets + t, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const uint32_t n = __hip_atomic_fetch_add(p.tickets + t * kTicketStride, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (n == parts - 1u) __hip_atomic_store(p.tickets + t * kTicketStride, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       sh[0] = (int)n;
     }
     __syncthreads();
     if (__builtin_amdgcn_readfirstlane(sh[0]) != parts - 1) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    for (int q = 0; q < parts; ++q) {
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(slot0 + q * TILE, (uint32_t)(TILE * 4));
-      // eight loads in flight: more take registers that the sums need
-      constexpr int AT_ONCE = C::UNITS < 8 ? C::UNITS : 8;
+    // Parts are added in order, the loads of several (of a large tile's part: of many units) in flight together: one
+    // latency per part made 1 x 2048 x 2048 on 8 parts 10.8 us.
+    constexpr int AT_ONCE = C::WAVES_PER_SIMD >= 4 ? 8 : 32;  // as the registers allow
+    constexpr int UNITS_AT_ONCE = C::UNITS < 16 ? C::UNITS : 16, PARTS_AT_ONCE = C::UNITS < 16 ? AT_ONCE / C::UNITS : 1;
+    for (int q0 = 0; q0 < parts; q0 += PARTS_AT_ONCE) {
 #pragma unroll
-      for (int u0 = 0; u0 < C::UNITS; u0 += AT_ONCE) {
-        f32x4 v[AT_ONCE];
+      for (int u0 = 0; u0 < C::UNITS; u0 += UNITS_AT_ONCE) {
+        f32x4 v[PARTS_AT_ONCE][UNITS_AT_ONCE];
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
-          v[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, tid * 16, (u0 + u) * C::NT * 16, 0));
+        for (int q = 0; q < PARTS_AT_ONCE; ++q) {
+          const __amdgpu_buffer_rsrc_t r = make_rsrc(slot0 + min(q0 + q, parts - 1) * TILE, (uint32_t)(TILE * 4));
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
+          for (int u = 0; u < UNITS_AT_ONCE; ++u)
+            v[q][u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    r, off[(u0 + u) / (C::FN * 4)], (u0 + u) * C::NT * 16, 0));
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int w = u0 + u;
-            const float x = acc[w / (C::FN * 4)][(w / 4) % C::FN][4 * (w % 4) + i];
-            acc[w / (C::FN * 4)][(w / 4) % C::FN][4 * (w % 4) + i] = q == 0 ? v[u][i] : x + v[u][i];
+        for (int q = 0; q < PARTS_AT_ONCE; ++q)
+          if (q0 + q < parts) {
+#pragma unroll
+            for (int u = 0; u < UNITS_AT_ONCE; ++u)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int w = u0 + u;
+                const float x = acc[w / (C::FN * 4)][(w / 4) % C::FN][4 * (w % 4) + i];
+                acc[w / (C::FN * 4)][(w / 4) % C::FN][4 * (w % 4) + i] = q0 + q == 0 ? v[q][u][i] : x + v[q][u][i];
+              }
           }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -653,6 +676,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
   const int64_t row0 = m0 + wm * C::WTM;                                  // in the group
   const int64_t col = n0 + wn * (kSwiglu ? C::WTN / 2 : C::WTN) + cc * 8;  // of the lane's first element
   const int nc = (int)min<int64_t>(max<int64_t>(p.N - col, 0), 8);
+  float2* wave_stats = reinterpret_cast<float2*>(smem + C::EPI_BYTES);
   float bias[8];
   if constexpr (EPI == kProdStore) {
     if (p.bias && nc > 0) load8(p.bias, col, p.bias_f32, p.vec & kVecBias, nc, bias);
@@ -736,7 +760,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
 #pragma unroll
         for (int d = 1; d < LPR; d <<= 1) sum += __shfl_xor(sum, d, 64);
         if (m < M) {
-          if (cc == 0) p.stats[(int64_t)(tn * C::WN + wn) * p.M + m] = float2{mx, sum};
+          if (cc == 0) wave_stats[wn * C::BM + wm * C::WTM + i * 32 + lr] = float2{mx, sum};
           const int64_t at = label_of(p, m) - col;
           if (at >= 0 && at < nc) {
 #pragma unroll
@@ -762,11 +786,21 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
     }
     wait_lgkm_all();  // this block's reads are done before the next block's writes
   }
+  if constexpr (EPI == kProdStats) {
+    // the waves' columns of a row, joined in order
+    __syncthreads();
+    for (int r = tid; r < C::BM && m0 + r < M; r += C::NT) {
+      float2 s = wave_stats[r];
+#pragma unroll
+      for (int w = 1; w < C::WN; ++w) s = join_stats(s, wave_stats[w * C::BM + r]);
+      p.stats[(int64_t)tn * p.M + m0 + r] = s;
+    }
+  }
 }
 
 // FLAT: the shape for row tiles of at most its height (of small groups), C's otherwise; both as wide.
 template <class C, class FLAT, bool AKC, bool BKC, int EPI>
-__global__ __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(1, C::WAVES_PER_SIMD)))
+__global__ __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(C::WAVES_PER_SIMD, C::WAVES_PER_SIMD)))
 void product_kernel(ProductParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // Workgroups are dealt round-robin to the 8 XCDs: each XCD gets neighbouring tiles, for its L2.

@@ -7,32 +7,130 @@
 namespace mk {
 namespace {
 
-// One workgroup copies rows blockIdx.x * 4 .. of group blockIdx.y, a row per wave.
+// 16 bytes that start at any element
+typedef uint32_t words_at_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// ---------------------------------------------------------------------------
+// One row or two against B [K, N], where latency counts (or B's rows allow no
+// 16-byte loads): a workgroup has 32 or 64 columns and all of K, a wave's load
+// covers 16 or 8 k-rows, so no sums cross workgroups and each lane's loads for
+// 8 k-rows are in flight together.  Sums on the vector units: 8 columns a lane,
+// then over the lanes of a column by shuffles, then over the waves through LDS.
+// us in a graph, weights from HBM, against 32-row tiles with K in parts: 1 x 512 x
+// 1024 3.9 and 6.1, 1 x 2048 x 2048 7.0 and 8.9, 2 x 1024 x 1024 about 6 and 7; a
+// longer K turns it round (1 x 4096 x 4096 18.7 and 14.7: as many bytes in flight,
+// but a workgroup's K goes through one CU), four rows too (4 x 2048 x 2048 10.9, 9.0).
+// ---------------------------------------------------------------------------
+constexpr int kFewWaves = 8;
+
+template <int ROWS, int COLS>
+__global__ __launch_bounds__(64 * kFewWaves) void product_few_rows_kernel(ProductParams p) {
+  __shared__ float sums[kFewWaves][ROWS][COLS];
+  constexpr int LANES = COLS / 8, KROWS = 64 / LANES;  // lanes of a k-row, k-rows of a wave's load
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // each XCD has neighbouring columns
+  const uint32_t n = gridDim.x, xcd = blockIdx.x & 7, id = xcd * (n >> 3) + min(xcd, n & 7) + (blockIdx.x >> 3);
+  // the last columns' loads end with the row: a workgroup's columns start at col0, some of them its neighbour's
+  const int64_t col0 = max<int64_t>(min<int64_t>((int64_t)id * COLS, p.N - COLS), 0);
+  const int64_t col = min<int64_t>(col0 + lane % LANES * 8, p.N - 8);  // (N is 8 or more)
+  float acc[ROWS][8];
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) acc[m][c] = 0.f;
+  // a lane has 8 neighbouring k-rows at a time, whose elements of A are one load
+  constexpr int U = 8;
+  for (int64_t k0 = (int64_t)(wave * KROWS + lane / LANES) * U; k0 < p.K; k0 += (int64_t)kFewWaves * KROWS * U) {
+    words_at_any w[U], x[ROWS];
+    const bool whole = k0 + U <= p.K;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      w[u] = *reinterpret_cast<const words_at_any*>(p.B + (whole ? k0 + u : min(k0 + u, p.K - 1)) * p.ldb + col);
+    if (whole) {
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) x[m] = *reinterpret_cast<const words_at_any*>(p.A + min<int64_t>(m, p.M - 1) * p.lda + k0);
+    } else {
+      // k-rows behind the last are zeros on both sides
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k0 + u >= p.K) w[u] = words_at_any{0, 0, 0, 0};
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) {
+        x[m] = words_at_any{0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (k0 + u < p.K) x[m][u / 2] |= (uint32_t)p.A[min<int64_t>(m, p.M - 1) * p.lda + k0 + u] << (16 * (u & 1));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) {
+        const float a = u & 1 ? bf16_hi(x[m][u / 2]) : bf16_lo(x[m][u / 2]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[m][2 * i] += a * bf16_lo(w[u][i]);
+          acc[m][2 * i + 1] += a * bf16_hi(w[u][i]);
+        }
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < ROWS; ++m)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+#pragma unroll
+      for (int d = LANES; d < 64; d <<= 1) acc[m][c] += __shfl_xor(acc[m][c], d, 64);
+      if (lane < LANES) sums[wave][m][col - col0 + c] = acc[m][c];  // (lanes of one column have the same sum)
+    }
+  __syncthreads();
+  if (threadIdx.x >= ROWS * COLS) return;
+  const int m = threadIdx.x / COLS, c = threadIdx.x % COLS;
+  const int64_t at = col0 + c;
+  if (m >= p.M || at < (int64_t)id * COLS || at >= p.N) return;  // a neighbour has its columns
+  float x = 0.f;
+#pragma unroll
+  for (int w = 0; w < kFewWaves; ++w) x += sums[w][m][c];
+  auto get = [](const void* q, int64_t i, int f32) {
+    return f32 ? static_cast<const float*>(q)[i] : __uint_as_float((uint32_t)static_cast<const uint16_t*>(q)[i] << 16);
+  };
+  if (p.bias) x += get(p.bias, at, p.bias_f32);
+  if (p.pre) p.pre[m * p.ldp + at] = (uint16_t)pack_bf16x2(x, 0.f);
+  if (p.act) for_act(p.act, [&](auto a_) { x = act_of<decltype(a_)::value>(x); });
+  if (p.res) x += get(p.res, m * p.ldr + at, p.res_f32);
+  if (p.c_f32) static_cast<float*>(p.C)[m * p.ldc + at] = x;
+  else static_cast<uint16_t*>(p.C)[m * p.ldc + at] = (uint16_t)pack_bf16x2(x, 0.f);
+}
+
+// A wave copies 512 columns of a row; one workgroup four rows of group blockIdx.z, columns from 2048 * blockIdx.y on.
+// (Loads of single elements moved 1.4 TB/s, a 1024 x 5003 matrix in 14.3 us.)
 __global__ __launch_bounds__(256) void repack_kernel(RepackParams p) {
   const int lane = threadIdx.x & 63;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= p.rows || (p.counts && p.counts[blockIdx.y] <= 0)) return;
-  const uint16_t* src = p.src + blockIdx.y * p.src_stride + row * p.ld;
-  uint16_t* dst = p.dst + blockIdx.y * p.dst_stride + row * p.width * p.parts;
+  if (row >= p.rows || (p.counts && p.counts[blockIdx.z] <= 0)) return;
+  const uint16_t* src = p.src + blockIdx.z * p.src_stride + row * p.ld;
+  uint16_t* dst = p.dst + blockIdx.z * p.dst_stride + row * p.width * p.parts;
   bool off = false;
   if (p.labels)
     off = (p.labels64 ? static_cast<const int64_t*>(p.labels)[row] : static_cast<const int*>(p.labels)[row]) == p.ignore;
-  const bool vec = !((reinterpret_cast<uintptr_t>(p.src) & 15) || p.ld % 8 || p.cols % 8 || p.src_stride % 8);
   for (int part = 0; part < p.parts; ++part, src += p.cols, dst += p.width) {
-    for (int64_t c = lane * 8; c < p.width; c += 512) {
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (!off) {
-        if (vec) {
-          const uint4 v = *reinterpret_cast<const uint4*>(src + c);
-          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-        } else {
-          // (eight 2-byte loads: lanes of a wave cover the same lines, which stay in L1)
+    words_at_any w[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c + i < p.cols) w[i / 2] |= (uint32_t)src[c + i] << (16 * (i & 1));
-        }
+    for (int u = 0; u < 4; ++u) {
+      const int64_t c = blockIdx.y * 2048 + u * 512 + lane * 8;
+      w[u] = words_at_any{0, 0, 0, 0};
+      if (off || c >= p.cols) continue;
+      if (c + 8 <= p.cols) {
+        w[u] = *reinterpret_cast<const words_at_any*>(src + c);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i < p.cols) w[u][i / 2] |= (uint32_t)src[c + i] << (16 * (i & 1));
       }
-      *reinterpret_cast<uint4*>(dst + c) = uint4{w[0], w[1], w[2], w[3]};
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t c = blockIdx.y * 2048 + u * 512 + lane * 8;
+      if (c < p.width) *reinterpret_cast<uint4*>(dst + c) = uint4{w[u][0], w[u][1], w[u][2], w[u][3]};
     }
   }
 }
@@ -96,31 +194,27 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const float* part, int
   }
 }
 
-// lse = max + log sum of the column groups' (max, sum of exponentials) pairs: 32 tokens a workgroup, eight slices of
-// the groups each, joined in order.
-__global__ __launch_bounds__(256) void vocab_join_kernel(VocabJoinParams p) {
-  __shared__ float2 part[8][32];
-  const int tok = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int64_t m = (int64_t)blockIdx.x * 32 + tok;
-  float mx = -INFINITY, sum = 0.f;
-  auto join = [&](float2 v) {
-    const float to = fmaxf(mx, v.x);
-    const float ref = to == -INFINITY ? 0.f : to;  // all of it -inf: sums are 0 (or NaN, which stays)
-    sum = sum * __expf(mx - ref) + v.y * __expf(v.x - ref);
-    mx = to;
-  };
+constexpr int kJoinTokens = 16, kJoinSlices = 32;
+
+// lse = max + log sum of the column groups' (max, sum of exponentials) pairs: 16 tokens a workgroup (a line of pairs),
+// 32 slices of the groups each, joined in order.
+__global__ __launch_bounds__(512) void vocab_join_kernel(VocabJoinParams p) {
+  __shared__ float2 part[kJoinSlices][kJoinTokens];
+  const int tok = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens;
+  const int64_t m = (int64_t)blockIdx.x * kJoinTokens + tok;
+  float2 s = {-INFINITY, 0.f};
   if (m < p.T) {
-    const int64_t g1 = (slice + 1) * p.groups / 8;
-#pragma unroll 4
-    for (int64_t g = slice * p.groups / 8; g < g1; ++g) join(p.stats[g * p.T + m]);
+    const int64_t g1 = (slice + 1) * p.groups / kJoinSlices;
+#pragma unroll 8
+    for (int64_t g = slice * p.groups / kJoinSlices; g < g1; ++g) s = join_stats(s, p.stats[g * p.T + m]);
   }
-  part[slice][tok] = float2{mx, sum};
+  part[slice][tok] = s;
   __syncthreads();
   if (slice != 0 || m >= p.T) return;
-  for (int s = 1; s < 8; ++s) join(part[s][tok]);
+  for (int i = 1; i < kJoinSlices; ++i) s = join_stats(s, part[i][tok]);
   const int64_t l = p.labels64 ? static_cast<const int64_t*>(p.labels)[m] : static_cast<const int*>(p.labels)[m];
   const bool none = l == p.ignore, here = !none && l >= p.label0 && l - p.label0 < p.vocab;
-  const float lse = none ? 0.f : mx + logf(sum), target = here ? p.target[m] : 0.f;
+  const float lse = none ? 0.f : s.x + logf(s.y), target = here ? p.target[m] : 0.f;
   p.lse[m] = lse;
   p.target[m] = target;
   if (p.loss) p.loss[m] = none ? 0.f : lse - target;
@@ -128,9 +222,23 @@ __global__ __launch_bounds__(256) void vocab_join_kernel(VocabJoinParams p) {
 
 }  // namespace
 
+hipError_t launch_product_few_rows(const ProductParams& p, hipStream_t stream) {
+  // 64 columns where that is a workgroup for every CU: whole lines (1 x 512 x 16384 10.4 us with 32, 7.0 with 64;
+  // 1 x 2048 x 2048 7.0 and 7.2)
+  const bool wide = p.N >= 64 * 256;
+  const int cols = wide ? 64 : 32;
+  const dim3 grid((unsigned)((p.N + cols - 1) / cols)), block(64 * kFewWaves);
+  if (p.M == 1 && wide) hipLaunchKernelGGL((product_few_rows_kernel<1, 64>), grid, block, 0, stream, p);
+  else if (p.M == 1) hipLaunchKernelGGL((product_few_rows_kernel<1, 32>), grid, block, 0, stream, p);
+  else if (wide) hipLaunchKernelGGL((product_few_rows_kernel<2, 64>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((product_few_rows_kernel<2, 32>), grid, block, 0, stream, p);
+  return hipGetLastError();
+}
+
 hipError_t launch_repack(const RepackParams& p, hipStream_t stream) {
   if (p.rows == 0 || p.E == 0 || p.width == 0) return hipSuccess;
-  hipLaunchKernelGGL(repack_kernel, dim3((unsigned)((p.rows + 3) / 4), (unsigned)p.E), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(repack_kernel, dim3((unsigned)((p.rows + 3) / 4), (unsigned)((p.width + 2047) / 2048), (unsigned)p.E),
+                     dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -154,7 +262,8 @@ hipError_t launch_act_grad(const ActGradParams& p, hipStream_t stream) {
 
 hipError_t launch_vocab_join(const VocabJoinParams& p, hipStream_t stream) {
   if (p.T == 0) return hipSuccess;
-  hipLaunchKernelGGL(vocab_join_kernel, dim3((unsigned)((p.T + 31) / 32)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(vocab_join_kernel, dim3((unsigned)((p.T + kJoinTokens - 1) / kJoinTokens)), dim3(kJoinTokens * kJoinSlices), 0,
+                     stream, p);
   return hipGetLastError();
 }
 

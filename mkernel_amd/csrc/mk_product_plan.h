@@ -9,25 +9,32 @@
 namespace mk {
 
 enum ProductTile : int { kProd32 = 0, kProd64 = 1, kProd64w = 2, kProd128 = 3, kProd256 = 4, kProdTiles = 5 };
-constexpr int kProductTickets = 1024;  // tiles of a launch whose K is cut into parts, at most
+constexpr int kProductTickets = 256;  // tiles of a launch whose K is cut into parts, at most
+constexpr int kTicketStride = 32;     // words between them: a line each
 
 // The tile shapes and what they cost, in us.  A launch runs in rounds of per_cu x CUs workgroups; a round takes
 //   round + K/16 x slope(x),  slope = one + load min(x, 1) + more max(x - 1, 0),  x = the round's workgroups per CU
 // (a full chip clocks lower and shares its caches).  `start` comes once, `area` for a million results (their stores),
 // and where the last round's tiles are cut: meet + part per part, and `exchange` for a MB of partial sums.  Fitted to
-// 923 launches of 79 shapes of 1 .. 8192 rows, 64 .. 8192 columns and K on one MI355X; the tile and cut that it picks
-// take 2 % longer than the best of those tried in the mean (worst 33 %).
+// 1318 launches of 79 shapes of 1 .. 8192 rows, 64 .. 8192 columns and K on one MI355X; the tile and cut that it picks
+// take 4 % longer than the best of those tried in the mean (worst 33 %).
 struct ProductShape {
-  int bm, bn, per_cu, waves_n;
+  int bm, bn, per_cu;
   double start, round, one, load, more, meet, part, area, exchange;
 };
 constexpr ProductShape kProductShapes[kProdTiles] = {
-    {32, 128, 2, 2, 4.10, 0.00, 0.078, 0.002, 0.061, 0.63, 0.41, 10.2, 0.55},
-    {64, 64, 2, 1, 2.25, 2.20, 0.069, 0.020, 0.038, 0.73, 0.39, 0.58, 0.33},
-    {64, 128, 2, 2, 3.52, 1.10, 0.071, 0.044, 0.069, 1.10, 0.39, 0.56, 0.39},
-    {128, 128, 2, 2, 1.60, 2.87, 0.098, 0.120, 0.045, 2.06, 0.53, 0.46, 0.36},
-    {256, 256, 1, 4, 6.59, 0.85, 0.142, 0.293, 0.0, 5.56, 2.01, 0.74, 0.14},
+    {32, 128, 2, 3.96, 0.00, 0.077, 0.013, 0.128, 0.80, 0.39, 8.62, 0.12},
+    {64, 64, 2, 3.14, 1.08, 0.068, 0.015, 0.055, 1.01, 0.34, 0.98, 0.16},
+    {64, 128, 2, 4.35, 0.00, 0.071, 0.040, 0.083, 1.32, 0.30, 0.79, 0.32},
+    {128, 128, 2, 4.41, 0.00, 0.098, 0.117, 0.071, 1.83, 0.31, 0.74, 0.29},
+    {256, 256, 1, 7.32, 0.00, 0.139, 0.288, 0.0, 4.28, 1.23, 0.94, 0.16},
 };
+
+// One row or two go to the kernel that has all of K in one workgroup where K is short, or where B would have to be laid
+// out anew (which takes three times the bytes).
+inline bool product_few_rows(int64_t M, int64_t N, int64_t K, bool aligned) {
+  return M <= 2 && N >= 8 && (M * K <= 2048 || !aligned);
+}
 
 struct ProductPlan {
   int tile, split;
@@ -53,7 +60,7 @@ inline ProductPlan plan_product(int64_t M, int64_t cols, int64_t K, int64_t grou
     const double k16 = (double)(ragged == 2 ? K / std::max<int64_t>(groups, 1) : K) / 16;
     // whole rounds, and the last one's tiles in parts
     const int64_t rest = tiles % slots, rounds = tiles / slots;
-    for (int split = 1; split <= 16; ++split) {
+    for (int split : {1, 2, 3, 4, 6, 8, 12, 16}) {
       // groups' sums have lengths that the host does not know, rows' tiles a number that it does not: not cut
       if (split > 1 && (!cut || ragged || rest == 0 || rest * split > slots || rest > kProductTickets || k16 < 8.0 * split))
         break;

@@ -29,6 +29,7 @@ def _ptr(t: torch.Tensor | None) -> int:
 # current_stream(i).cuda_stream without the Stream object, where torch has these
 # (they are not part of its public interface)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_capturing = torch.cuda.is_current_stream_capturing
 _device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
@@ -792,33 +793,42 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
 
 
 # ------------------------------------------------------------------- products with what follows them
-_tickets: dict = {}
+# Tickets (zeroed words by which the parts of a product's K meet, left zeroed by every launch) and behind them a small
+# workspace: one set per (device, stream), whose launches are ordered.
+_SPACE = 4 << 20
+_spaces: dict = {}
 
 
-def _ticket_words(index: int, stream: int) -> int:
-    """The zeroed words by which the parts of a product's K meet: one set per
-    (device, stream), left zeroed by every launch.  Inside a graph's capture a
-    set of its own, whose zeros are recorded with it: graphs may then run beside
-    each other and beside eager calls."""
-    if torch.cuda.is_current_stream_capturing():
-        # torch keeps it for the graph, whose private pool it comes from
-        return torch.zeros(capi.PRODUCT_TICKETS, dtype=torch.int32, device=torch.device("cuda", index)).data_ptr()
-    t = _tickets.get((index, stream))
+def _space(index: int, stream: int) -> int:
+    t = _spaces.get((index, stream))
     if t is None:
-        t = _tickets[index, stream] = torch.zeros(capi.PRODUCT_TICKETS, dtype=torch.int32,
-                                                  device=torch.device("cuda", index))
+        n = capi.PRODUCT_TICKETS * 4
+        t = torch.empty(n + _SPACE, dtype=torch.uint8, device=torch.device("cuda", index))
+        t[:n].zero_()
+        _spaces[index, stream] = t
     return t.data_ptr()
 
 
 def _product(fn: str, cls, device, cut: bool, *values) -> None:
     """Calls an entry point whose arguments end with a workspace (and, with
-    cut, tickets)."""
+    cut, tickets): the stream's small one where that is enough, else memory of
+    its own, which the caching allocator reuses in stream order.  Inside a
+    graph's capture both are the graph's (torch keeps what it allocates there
+    for it), the tickets' zeros recorded with it: graphs may then run beside
+    each other and beside eager calls."""
+    index = device.index
+    stream = _raw_stream(index)
+    if _capturing():
+        at = torch.zeros(capi.PRODUCT_TICKETS, dtype=torch.int32, device=device) if cut else None
+        tickets = (at.data_ptr(),) if cut else ()
+    else:
+        at = _space(index, stream)
+        tickets = (at,) if cut else ()
+        if capi.call_with_workspace(fn, cls, stream, *values, at + capi.PRODUCT_TICKETS * 4, _SPACE, *tickets):
+            return
     n = capi.workspace_bytes(fn, cls, *values)
-    # the caching allocator reuses it in stream order, a graph's capture keeps it
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    stream = _raw_stream(device.index)
-    tail = (_ticket_words(device.index, stream),) if cut else ()
-    capi.call_values(fn, cls, stream, *values, 0 if ws is None else ws.data_ptr(), n, *tail)
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    capi.call_values(fn, cls, stream, *values, ws.data_ptr(), n, *tickets)
 
 
 def _rows(t, name: str, dtypes, shape, device) -> None:
