@@ -46,7 +46,7 @@ struct PCfg {
   static constexpr int A_INST = A_BYTES / 1024 / WAVES, B_INST = B_BYTES / 1024 / WAVES, LOADS = A_INST + B_INST;
   static constexpr int PITCH = WTN * 4 + 16;  // bytes of an epilogue row
   static constexpr uint32_t EPI_BYTES = WAVES * 32 * PITCH;
-  static constexpr uint32_t STATS_BYTES = WN * BM * 8;  // behind them, of the vocabulary's epilogue
+  static constexpr uint32_t STATS_BYTES = WN * BM * 8 + BM * 16;  // behind them, of the vocabulary's epilogues
   static constexpr uint32_t LDS_BYTES = S * STAGE > EPI_BYTES + STATS_BYTES ? S * STAGE : EPI_BYTES + STATS_BYTES;
   static constexpr int PER_CU = 160 * 1024 / LDS_BYTES;
   static constexpr int WAVES_PER_SIMD = PER_CU * WAVES / 4 > 0 ? PER_CU * WAVES / 4 : 1;
@@ -169,32 +169,55 @@ struct Operand {
 // Epilogue helpers: 8 neighbouring elements of a row
 // ---------------------------------------------------------------------------
 
+// As they come from memory, to be unpacked when they are needed.
+struct Raw8 {
+  uint4 a, b;  // b: the second half of fp32 values
+};
+
 // n < 8: the first n only, others 0.  vec: rows start at 16-byte boundaries.
-__device__ __forceinline__ void load8(const void* p, int64_t at, bool f32, bool vec, int n, float (&x)[8]) {
+__device__ __forceinline__ Raw8 load8_raw(const void* p, int64_t at, bool f32, bool vec, int n) {
+  Raw8 v = {{0, 0, 0, 0}, {0, 0, 0, 0}};
   if (f32) {
-    const float* s = static_cast<const float*>(p) + at;
+    const uint32_t* s = static_cast<const uint32_t*>(p) + at;
     if (vec && n >= 8) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(s), b = *reinterpret_cast<const f32x4*>(s + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = a[i];
-        x[4 + i] = b[i];
-      }
+      v.a = *reinterpret_cast<const uint4*>(s);
+      v.b = *reinterpret_cast<const uint4*>(s + 4);
     } else {
+      uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = i < n ? s[i] : 0.f;
+      for (int i = 0; i < 8; ++i) w[i] = i < n ? s[i] : 0u;
+      v.a = uint4{w[0], w[1], w[2], w[3]};
+      v.b = uint4{w[4], w[5], w[6], w[7]};
     }
   } else {
     const uint16_t* s = static_cast<const uint16_t*>(p) + at;
     if (vec && n >= 8) {
-      const uint4 v = *reinterpret_cast<const uint4*>(s);
-      x[0] = bf16_lo(v.x); x[1] = bf16_hi(v.x); x[2] = bf16_lo(v.y); x[3] = bf16_hi(v.y);
-      x[4] = bf16_lo(v.z); x[5] = bf16_hi(v.z); x[6] = bf16_lo(v.w); x[7] = bf16_hi(v.w);
+      v.a = *reinterpret_cast<const uint4*>(s);
     } else {
+      uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = i < n ? __uint_as_float((uint32_t)s[i] << 16) : 0.f;
+      for (int i = 0; i < 8; ++i) w[i] = i < n ? s[i] : 0u;
+      v.a = uint4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
     }
   }
+  return v;
+}
+__device__ __forceinline__ void unpack8(const Raw8& v, bool f32, float (&x)[8]) {
+  if (f32) {
+    const uint32_t w[8] = {v.a.x, v.a.y, v.a.z, v.a.w, v.b.x, v.b.y, v.b.z, v.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+  } else {
+    const uint32_t w[4] = {v.a.x, v.a.y, v.a.z, v.a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = bf16_lo(w[i]);
+      x[2 * i + 1] = bf16_hi(w[i]);
+    }
+  }
+}
+__device__ __forceinline__ void load8(const void* p, int64_t at, bool f32, bool vec, int n, float (&x)[8]) {
+  unpack8(load8_raw(p, at, f32, vec, n), f32, x);
 }
 
 __device__ __forceinline__ void store8(void* p, int64_t at, bool f32, bool vec, int n, const float (&x)[8]) {
@@ -275,6 +298,12 @@ __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
   const float ref = to == -INFINITY ? 0.f : to;  // all of it -inf: sums are 0 (or NaN, which stays)
   return {to, a.y * __expf(a.x - ref) + b.y * __expf(b.x - ref)};
 }
+
+struct TokenRow {
+  int label;
+  float lse, dloss;
+  int unused;
+};
 
 // Label of token m among this call's columns, -1: another shard's, -2: no loss.
 __device__ __forceinline__ int64_t label_of(const ProductParams& p, int64_t m) {
@@ -428,6 +457,20 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
   });
 
   // ---- main loop ----
+  // vocabulary: a thread has one row's label (as a column of the tile; -1 elsewhere, -2 no loss) and numbers, loaded
+  // before the products and kept in LDS for the epilogue (loaded there, one latency per eight rows, they took 12 us)
+  TokenRow token = {-1, 0.f, 0.f, 0};
+  if constexpr (EPI == kProdStats || EPI == kProdDlogits) {
+    static_assert(C::NT >= C::BM, "a row per thread");
+    if (tid < C::BM && m0 + tid < M) {
+      const int64_t label = label_of(p, m0 + tid), c = label - p.first_col - n0;
+      token.label = label < 0 ? (int)label : c >= 0 && c < C::BN ? (int)c : -1;
+      if constexpr (EPI == kProdDlogits) {
+        token.lse = p.lse[m0 + tid];
+        token.dloss = p.dloss[m0 + tid];
+      }
+    }
+  }
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
   f32x16 acc[C::FM][C::FN];
 #pragma unroll
@@ -676,7 +719,12 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
   const int64_t row0 = m0 + wm * C::WTM;                                  // in the group
   const int64_t col = n0 + wn * (kSwiglu ? C::WTN / 2 : C::WTN) + cc * 8;  // of the lane's first element
   const int nc = (int)min<int64_t>(max<int64_t>(p.N - col, 0), 8);
-  float2* wave_stats = reinterpret_cast<float2*>(smem + C::EPI_BYTES);
+  TokenRow* tokens = reinterpret_cast<TokenRow*>(smem + C::EPI_BYTES);
+  float2* wave_stats = reinterpret_cast<float2*>(tokens + C::BM);
+  if constexpr (EPI == kProdStats || EPI == kProdDlogits) {
+    if (tid < C::BM) tokens[tid] = token;
+    __syncthreads();
+  }
   float bias[8];
   if constexpr (EPI == kProdStore) {
     if (p.bias && nc > 0) load8(p.bias, col, p.bias_f32, p.vec & kVecBias, nc, bias);
@@ -684,6 +732,28 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
 #pragma unroll
   for (int i = 0; i < C::FM; ++i) {
     if (row0 + i * 32 >= M) break;
+    constexpr int STEPS = 32 / RPI;
+    auto row_of = [&](int r) { return row0 + i * 32 + r * RPI + rr; };
+    // what the epilogue reads of memory, all of the block's in flight before anything waits
+    constexpr int READS = EPI == kProdStore || EPI == kProdSwigluGrad ? STEPS : 1;
+    Raw8 extra[READS];
+    if constexpr (EPI == kProdStore) {
+      if (p.res) {
+#pragma unroll
+        for (int r = 0; r < STEPS; ++r)
+          if (row_of(r) < M && nc > 0)
+            extra[r] = load8_raw(p.res, coff + (crow + row_of(r)) * p.ldr + col, p.res_f32, p.vec & kVecRes, nc);
+      }
+    }
+    if constexpr (EPI == kProdSwigluGrad) {
+#pragma unroll
+      for (int r = 0; r < STEPS; ++r)
+        if (row_of(r) < M && nc > 0) {
+          const int64_t at = (crow + row_of(r)) * p.ldr + col;
+          extra[r].a = load8_raw(p.res, at, false, p.vec & kVecRes, nc).a;
+          extra[r].b = load8_raw(p.res, at + p.N, false, p.vec & kVecRes, nc).a;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < C::FN; ++j)
 #pragma unroll
@@ -694,94 +764,121 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
         *reinterpret_cast<f32x4*>(reg + ml * C::PITCH + (32 * j + 8 * q + 4 * kg) * 4) = w;
       }
     wait_lgkm_all();
-    for (int r = 0; r < 32 / RPI; ++r) {
-      const int lr = r * RPI + rr;
-      const int64_t m = row0 + i * 32 + lr;
-      const char* s = reg + lr * C::PITCH + cc * 32;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(s), hi = *reinterpret_cast<const f32x4*>(s + 16);
-      float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if constexpr (EPI == kProdStore) {
-        if (m >= M || nc <= 0) continue;
-        if (p.bias) {
+    auto read = [&](int r, float (&x)[8]) {
+      const f32x4* s = reinterpret_cast<const f32x4*>(reg + (r * RPI + rr) * C::PITCH + cc * 32);
 #pragma unroll
-          for (int v = 0; v < 8; ++v) x[v] += bias[v];
-        }
-        if (p.pre) store8(p.pre, m * p.ldp + col, false, p.vec & kVecPre, nc, x);
-        if (p.act) for_act(p.act, [&](auto a_) {
+      for (int v = 0; v < 4; ++v) {
+        x[v] = s[0][v];
+        x[4 + v] = s[1][v];
+      }
+    };
+    if constexpr (EPI == kProdStore) {
+      if (!p.res || p.bias || p.pre || p.act) {
+#pragma clang loop unroll(disable)
+        for (int r = 0; r < STEPS; ++r) {
+          const int64_t m = row_of(r);
+          if (m >= M || nc <= 0) continue;
+          float x[8];
+          read(r, x);
+          if (p.bias) {
 #pragma unroll
-          for (int v = 0; v < 8; ++v) x[v] = act_of<decltype(a_)::value>(x[v]);
-        });
-        if (p.res) {
-          float y[8];
-          load8(p.res, coff + (crow + m) * p.ldr + col, p.res_f32, p.vec & kVecRes, nc, y);
+            for (int v = 0; v < 8; ++v) x[v] += bias[v];
+          }
+          if (p.pre) store8(p.pre, m * p.ldp + col, false, p.vec & kVecPre, nc, x);
+          if (p.act) for_act(p.act, [&](auto a_) {
 #pragma unroll
-          for (int v = 0; v < 8; ++v) x[v] += y[v];
-        }
-        store8(p.C, coff + (crow + m) * p.ldc + col, p.c_f32, p.vec & kVecC, nc, x);
-      } else if constexpr (kSwiglu) {
-        if (m >= M || nc <= 0) continue;
-        const f32x4 ul = *reinterpret_cast<const f32x4*>(s + C::WTN * 2), uh = *reinterpret_cast<const f32x4*>(s + C::WTN * 2 + 16);
-        const float u[8] = {ul[0], ul[1], ul[2], ul[3], uh[0], uh[1], uh[2], uh[3]};
-        if (p.pre) {
-          const int64_t at = (crow + m) * p.ldp + col;
-          store8(p.pre, at, false, p.vec & kVecPre, nc, x);
-          store8(p.pre, at + p.N, false, p.vec & kVecPre, nc, u);
-        }
-#pragma unroll
-        for (int v = 0; v < 8; ++v) x[v] = act_of<kActSilu>(x[v]) * u[v];
-        store8(p.C, (crow + m) * p.ldc + col, false, p.vec & kVecC, nc, x);
-      } else if constexpr (EPI == kProdSwigluGrad) {
-        // x = d out / d act of columns col ..; the gate's gradient goes to column col, the up's to N + col
-        if (m >= M || nc <= 0) continue;
-        float ga[8], up[8];
-        const int64_t at = (crow + m) * p.ldr + col;
-        load8(p.res, at, false, p.vec & kVecRes, nc, ga);
-        load8(p.res, at + p.N, false, p.vec & kVecRes, nc, up);
-#pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          const float sg = sigmoid(ga[v]), d = x[v];
-          x[v] = d * up[v] * sg * (1.f + ga[v] * (1.f - sg));
-          up[v] = d * ga[v] * sg;
-        }
-        const int64_t to = (crow + m) * p.ldc + col;
-        store8(p.C, to, false, p.vec & kVecC, nc, x);
-        store8(p.C, to + p.N, false, p.vec & kVecC, nc, up);
-      } else if constexpr (EPI == kProdStats) {
-        // largest logit and sum of exponentials of the wave's columns, and the label's logit
-        float mx = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < 8; ++v) mx = v < nc ? fmaxf(mx, x[v]) : mx;
-#pragma unroll
-        for (int d = 1; d < LPR; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-        float sum = 0.f;
-        const float ref = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-        for (int v = 0; v < 8; ++v) sum += v < nc ? __expf(x[v] - ref) : 0.f;
-#pragma unroll
-        for (int d = 1; d < LPR; d <<= 1) sum += __shfl_xor(sum, d, 64);
-        if (m < M) {
-          if (cc == 0) wave_stats[wn * C::BM + wm * C::WTM + i * 32 + lr] = float2{mx, sum};
-          const int64_t at = label_of(p, m) - col;
-          if (at >= 0 && at < nc) {
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              if (v == at) p.target[m] = x[v];
+            for (int v = 0; v < 8; ++v) x[v] = act_of<decltype(a_)::value>(x[v]);
+          });
+          if (p.res) {  // back to where they were: the residual is added below
+            f32x4* s = reinterpret_cast<f32x4*>(reg + (r * RPI + rr) * C::PITCH + cc * 32);
+            s[0] = f32x4{x[0], x[1], x[2], x[3]};
+            s[1] = f32x4{x[4], x[5], x[6], x[7]};
+          } else {
+            store8(p.C, coff + (crow + m) * p.ldc + col, p.c_f32, p.vec & kVecC, nc, x);
           }
         }
-      } else {  // kProdDlogits
-        if (m >= M) continue;
-        const int64_t label = label_of(p, m);
-        const float w = label == -2 ? 0.f : p.dloss[m], lse = p.lse[m];
-        const int64_t at = label - p.first_col - col;
+      }
+      if (p.res) {
 #pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          float d = __expf(x[v] - lse);
-          if (v == at) d -= 1.f;
-          // (a token without a loss, or a column behind the last, has none of it, whatever its logits are)
-          x[v] = label == -2 || v >= nc ? 0.f : d * w;
+        for (int r = 0; r < STEPS; ++r) {
+          const int64_t m = row_of(r);
+          if (m >= M || nc <= 0) continue;
+          float x[8], y[8];
+          read(r, x);
+          unpack8(extra[r], p.res_f32, y);
+#pragma unroll
+          for (int v = 0; v < 8; ++v) x[v] += y[v];
+          store8(p.C, coff + (crow + m) * p.ldc + col, p.c_f32, p.vec & kVecC, nc, x);
         }
-        // the scratch rows are whole units: columns behind the last are zeros, as the products behind read them
-        if (col < p.ldc) store8(p.C, m * p.ldc + col, false, true, 8, x);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < STEPS; ++r) {
+        const int64_t m = row_of(r);
+        float x[8];
+        read(r, x);
+        if constexpr (kSwiglu) {
+          if (m >= M || nc <= 0) continue;
+          const f32x4* s = reinterpret_cast<const f32x4*>(reg + (r * RPI + rr) * C::PITCH + C::WTN * 2 + cc * 32);
+          const float u[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]};
+          if (p.pre) {
+            const int64_t at = (crow + m) * p.ldp + col;
+            store8(p.pre, at, false, p.vec & kVecPre, nc, x);
+            store8(p.pre, at + p.N, false, p.vec & kVecPre, nc, u);
+          }
+#pragma unroll
+          for (int v = 0; v < 8; ++v) x[v] = act_of<kActSilu>(x[v]) * u[v];
+          store8(p.C, (crow + m) * p.ldc + col, false, p.vec & kVecC, nc, x);
+        } else if constexpr (EPI == kProdSwigluGrad) {
+          // x = d out / d act of columns col ..; the gate's gradient goes to column col, the up's to N + col
+          if (m >= M || nc <= 0) continue;
+          float ga[8], up[8];
+          unpack8(Raw8{extra[r].a, {}}, false, ga);
+          unpack8(Raw8{extra[r].b, {}}, false, up);
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            const float sg = sigmoid(ga[v]), d = x[v];
+            x[v] = d * up[v] * sg * (1.f + ga[v] * (1.f - sg));
+            up[v] = d * ga[v] * sg;
+          }
+          const int64_t to = (crow + m) * p.ldc + col;
+          store8(p.C, to, false, p.vec & kVecC, nc, x);
+          store8(p.C, to + p.N, false, p.vec & kVecC, nc, up);
+        } else if constexpr (EPI == kProdStats) {
+          // largest logit and sum of exponentials of the wave's columns, and the label's logit
+          float mx = -INFINITY;
+#pragma unroll
+          for (int v = 0; v < 8; ++v) mx = v < nc ? fmaxf(mx, x[v]) : mx;
+#pragma unroll
+          for (int d = 1; d < LPR; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+          float sum = 0.f;
+          const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+          for (int v = 0; v < 8; ++v) sum += v < nc ? __expf(x[v] - ref) : 0.f;
+#pragma unroll
+          for (int d = 1; d < LPR; d <<= 1) sum += __shfl_xor(sum, d, 64);
+          const int lr = wm * C::WTM + i * 32 + r * RPI + rr, at = tokens[lr].label - (wn * C::WTN + cc * 8);
+          if (cc == 0) wave_stats[wn * C::BM + lr] = float2{mx, sum};
+          if (m < M && at >= 0 && at < nc) {
+            float z = x[0];
+#pragma unroll
+            for (int v = 1; v < 8; ++v) z = v == at ? x[v] : z;
+            p.target[m] = z;
+          }
+        } else {  // kProdDlogits
+          if (m >= M) continue;
+          const TokenRow t = tokens[wm * C::WTM + i * 32 + r * RPI + rr];
+          const int at = t.label - (wn * C::WTN + cc * 8);
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            float d = __expf(x[v] - t.lse);
+            if (v == at) d -= 1.f;
+            // (a token without a loss, or a column behind the last, has none of it, whatever its logits are)
+            x[v] = t.label == -2 || v >= nc ? 0.f : d * t.dloss;
+          }
+          // the scratch rows are whole units: columns behind the last are zeros, as the products behind read them
+          if (col < p.ldc) store8(p.C, m * p.ldc + col, false, true, 8, x);
+        }
       }
     }
     wait_lgkm_all();  // this block's reads are done before the next block's writes

@@ -524,3 +524,10 @@ def test_vocab_loss_gradient_against_differences():
         off = float((dl * move).sum()) * 2.0 ** -8 + 2.0 ** -13 * abs(want)
         assert abs(slope - want) <= off, (i, slope, want, off)
         assert off < 0.5 * abs(want)  # (so that another factor would be seen)
+
+
+def test_vocab_loss_pieces_of_laid_out_weights():
+    """An odd vocabulary whose weights are laid out anew in several pieces, forward and back; labels in each."""
+    T, H, V = 5, 4096, 33001
+    labels = torch.tensor([0, 16383, 16384, 32768, 33000])
+    _check_vocab(T, H, V, labels, randn(T, H, seed=99), randn(H, V, seed=100, scale=2 * H ** -0.5))
