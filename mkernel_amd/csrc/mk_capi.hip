@@ -1402,8 +1402,12 @@ struct Products {
   int run(int order, int epi, mk::ProductParams p, int64_t tile_cols, int* tile = nullptr) {
     if (p.M == 0 || p.N == 0) return MK_OK;
     const int groups = p.ragged ? p.E : 1;
-    const mk::ProductPlan plan =
-        mk::plan_product(p.M, tile_cols, p.K, groups, p.ragged, order == mk::kProdRightGrad, tickets != nullptr, cus);
+    if (epi == mk::kProdStore && !p.bias && !p.act && !p.pre && !p.res) {
+      if (!p.c_f32) epi = mk::kProdPlain;
+      else if (order == mk::kProdRightGrad) epi = mk::kProdPlain32;
+    }
+    const mk::ProductPlan plan = mk::plan_product(p.M, tile_cols, p.K, groups, p.ragged, order == mk::kProdRightGrad,
+                                                  epi != mk::kProdStore, tickets != nullptr, cus);
     if (tile) *tile = plan.tile;
     const mk::ProductShape& s = mk::kProductShapes[plan.tile];
     p.split = plan.split;
@@ -1426,7 +1430,7 @@ struct Products {
     if (sp.counting) return MK_OK;
     return launched(order == mk::kProdForward    ? mk::launch_product_forward(p, epi, plan.tile, grid, stream)
                     : order == mk::kProdLeftGrad ? mk::launch_product_left_grad(p, epi, plan.tile, grid, stream)
-                                                 : mk::launch_product_right_grad(p, plan.tile, grid, stream));
+                                                 : mk::launch_product_right_grad(p, epi, plan.tile, grid, stream));
   }
 
   // Rows as an operand takes them: 16-byte aligned; `whole`: ending with a unit or zeros (k-contiguous operands).

@@ -258,7 +258,8 @@ hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E
                               uint16_t* scales, hipStream_t stream);
 
 // Products with what follows them (mk_product.h, mk_product.hip).
-enum ProductEpilogue : int { kProdStore = 0, kProdSwiglu = 1, kProdSwigluGrad = 2, kProdStats = 3, kProdDlogits = 4 };
+enum ProductEpilogue : int { kProdStore = 0, kProdSwiglu = 1, kProdSwigluGrad = 2, kProdStats = 3, kProdDlogits = 4,
+                             kProdPlain = 5, kProdPlain32 = 6 };  // kProdStore without anything but bf16 or fp32 results
 enum ProductOrder : int { kProdForward = 0, kProdLeftGrad = 1, kProdRightGrad = 2 };
 enum ProductAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
 // which rows of the epilogue start at 16-byte boundaries
@@ -302,7 +303,7 @@ struct ProductParams {
 };
 hipError_t launch_product_forward(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
 hipError_t launch_product_left_grad(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
-hipError_t launch_product_right_grad(const ProductParams& p, int tile, int64_t grid, hipStream_t stream);
+hipError_t launch_product_right_grad(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
 // Forward, plain epilogue, one row or two: operands of any alignment.
 hipError_t launch_product_few_rows(const ProductParams& p, hipStream_t stream);
 // Rows of bf16 into rows of a multiple of 8 elements, zeros behind the last: `parts` pieces of `cols` columns each,

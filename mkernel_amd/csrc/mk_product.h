@@ -220,28 +220,54 @@ __device__ __forceinline__ void load8(const void* p, int64_t at, bool f32, bool 
   unpack8(load8_raw(p, at, f32, vec, n), f32, x);
 }
 
-__device__ __forceinline__ void store8(void* p, int64_t at, bool f32, bool vec, int n, const float (&x)[8]) {
+// The same for four elements, n <= 4 of them there.
+__device__ __forceinline__ uint4 load4_raw(const void* p, int64_t at, bool f32, bool vec, int n) {
+  uint32_t w[4] = {0, 0, 0, 0};
   if (f32) {
-    float* d = static_cast<float*>(p) + at;
-    if (vec && n >= 8) {
-      *reinterpret_cast<f32x4*>(d) = f32x4{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<f32x4*>(d + 4) = f32x4{x[4], x[5], x[6], x[7]};
-    } else {
+    const uint32_t* s = static_cast<const uint32_t*>(p) + at;
+    if (vec && n >= 4) return *reinterpret_cast<const uint4*>(s);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) d[i] = x[i];
-    }
+    for (int i = 0; i < 4; ++i) w[i] = i < n ? s[i] : 0u;
   } else {
-    uint16_t* d = static_cast<uint16_t*>(p) + at;
-    const uint4 v = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
-    if (vec && n >= 8) {
-      *reinterpret_cast<uint4*>(d) = v;
-    } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) d[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+    const uint16_t* s = static_cast<const uint16_t*>(p) + at;
+    if (vec && n >= 4) {
+      const uint2 v = *reinterpret_cast<const uint2*>(s);
+      return uint4{v.x, v.y, 0, 0};
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i / 2] |= (i < n ? (uint32_t)s[i] : 0u) << (16 * (i & 1));
+  }
+  return uint4{w[0], w[1], w[2], w[3]};
+}
+__device__ __forceinline__ f32x4 unpack4(const uint4& v, bool f32) {
+  if (f32) return f32x4{__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w)};
+  return f32x4{bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)};
+}
+
+// NT: past the caches, for results that nothing reads soon (16384 x 8192
+// x 3584 850 us without, 799 with).
+template <bool NT = false>
+__device__ __forceinline__ void store8(void* p, int64_t at, bool vec, int n, const float (&x)[8]) {
+  uint16_t* d = static_cast<uint16_t*>(p) + at;
+  const uint4 v = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+  if (vec && n >= 8) {
+    if constexpr (NT) __builtin_nontemporal_store(u32x4_t{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_t*>(d));
+    else *reinterpret_cast<uint4*>(d) = v;
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) d[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+  }
+}
+
+__device__ __forceinline__ void store4(float* d, bool vec, int n, f32x4 x) {
+  if (vec && n == 4) {
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(d));
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (v < n) d[v] = x[v];
   }
 }
 
@@ -676,8 +702,8 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     // Parts are added in order, the loads of several (of a large tile's part: of many units) in flight together: one
     // latency per part made 1 x 2048 x 2048 on 8 parts 10.8 us.
-    constexpr int AT_ONCE = C::WAVES_PER_SIMD >= 4 ? 8 : 32;  // as the registers allow
-    constexpr int UNITS_AT_ONCE = C::UNITS < 16 ? C::UNITS : 16, PARTS_AT_ONCE = C::UNITS < 16 ? AT_ONCE / C::UNITS : 1;
+    constexpr int AT_ONCE = C::WAVES_PER_SIMD >= 4 ? 8 : C::UNITS < 16 ? 32 : 16;  // loads, as the registers allow
+    constexpr int UNITS_AT_ONCE = C::UNITS < AT_ONCE ? C::UNITS : AT_ONCE, PARTS_AT_ONCE = AT_ONCE / UNITS_AT_ONCE;
     for (int q0 = 0; q0 < parts; q0 += PARTS_AT_ONCE) {
 #pragma unroll
       for (int u0 = 0; u0 < C::UNITS; u0 += UNITS_AT_ONCE) {
@@ -737,12 +763,27 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
     // what the epilogue reads of memory, all of the block's in flight before anything waits
     constexpr int READS = EPI == kProdStore || EPI == kProdSwigluGrad ? STEPS : 1;
     Raw8 extra[READS];
+    // fp32 results go four columns a lane, so that an instruction covers whole lines here too (eight columns a lane, in
+    // two halves, wrote half lines: 60 experts' 2056 x 2768 gradients 346 us, 517 past the caches)
+    constexpr int LPR4 = C::WTN / 4, STEPS4 = 32 * LPR4 / 64;
+    const int cc4 = l % LPR4 * 4;
+    const int64_t col4 = n0 + wn * C::WTN + cc4;
+    const int nc4 = (int)min<int64_t>(max<int64_t>(p.N - col4, 0), 4);
+    auto row4_of = [&](int r) { return row0 + i * 32 + r * (64 / LPR4) + l / LPR4; };
     if constexpr (EPI == kProdStore) {
-      if (p.res) {
+      if (p.res && !p.c_f32) {
 #pragma unroll
         for (int r = 0; r < STEPS; ++r)
           if (row_of(r) < M && nc > 0)
             extra[r] = load8_raw(p.res, coff + (crow + row_of(r)) * p.ldr + col, p.res_f32, p.vec & kVecRes, nc);
+      } else if (p.res) {
+#pragma unroll
+        for (int r = 0; r < STEPS4; ++r)
+          if (row4_of(r) < M && nc4 > 0) {
+            const uint4 v = load4_raw(p.res, coff + (crow + row4_of(r)) * p.ldr + col4, p.res_f32, p.vec & kVecRes, nc4);
+            if (r & 1) extra[r / 2].b = v;
+            else extra[r / 2].a = v;
+          }
       }
     }
     if constexpr (EPI == kProdSwigluGrad) {
@@ -773,7 +814,8 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
       }
     };
     if constexpr (EPI == kProdStore) {
-      if (!p.res || p.bias || p.pre || p.act) {
+      const bool later = p.res || p.c_f32;  // what is added last, and the results, in a loop of their own
+      if (!later || p.bias || p.pre || p.act) {
 #pragma clang loop unroll(disable)
         for (int r = 0; r < STEPS; ++r) {
           const int64_t m = row_of(r);
@@ -784,21 +826,31 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
 #pragma unroll
             for (int v = 0; v < 8; ++v) x[v] += bias[v];
           }
-          if (p.pre) store8(p.pre, m * p.ldp + col, false, p.vec & kVecPre, nc, x);
+          if (p.pre) store8<true>(p.pre, m * p.ldp + col, p.vec & kVecPre, nc, x);
           if (p.act) for_act(p.act, [&](auto a_) {
 #pragma unroll
             for (int v = 0; v < 8; ++v) x[v] = act_of<decltype(a_)::value>(x[v]);
           });
-          if (p.res) {  // back to where they were: the residual is added below
+          if (later) {  // back to where they were
             f32x4* s = reinterpret_cast<f32x4*>(reg + (r * RPI + rr) * C::PITCH + cc * 32);
             s[0] = f32x4{x[0], x[1], x[2], x[3]};
             s[1] = f32x4{x[4], x[5], x[6], x[7]};
           } else {
-            store8(p.C, coff + (crow + m) * p.ldc + col, p.c_f32, p.vec & kVecC, nc, x);
+            store8<true>(p.C, coff + (crow + m) * p.ldc + col, p.vec & kVecC, nc, x);
           }
         }
+        if (later) wait_lgkm_all();
       }
-      if (p.res) {
+      if (p.c_f32) {
+#pragma unroll
+        for (int r = 0; r < STEPS4; ++r) {
+          const int64_t m = row4_of(r);
+          if (m >= M || nc4 <= 0) continue;
+          f32x4 x = *reinterpret_cast<const f32x4*>(reg + (r * (64 / LPR4) + l / LPR4) * C::PITCH + cc4 * 4);
+          if (p.res) x += unpack4(r & 1 ? extra[r / 2].b : extra[r / 2].a, p.res_f32);
+          store4(static_cast<float*>(p.C) + coff + (crow + m) * p.ldc + col4, p.vec & kVecC, nc4, x);
+        }
+      } else if (p.res) {
 #pragma unroll
         for (int r = 0; r < STEPS; ++r) {
           const int64_t m = row_of(r);
@@ -808,8 +860,16 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
           unpack8(extra[r], p.res_f32, y);
 #pragma unroll
           for (int v = 0; v < 8; ++v) x[v] += y[v];
-          store8(p.C, coff + (crow + m) * p.ldc + col, p.c_f32, p.vec & kVecC, nc, x);
+          store8<true>(p.C, coff + (crow + m) * p.ldc + col, p.vec & kVecC, nc, x);
         }
+      }
+    } else if constexpr (EPI == kProdPlain32) {
+#pragma unroll
+      for (int r = 0; r < STEPS4; ++r) {
+        const int64_t m = row4_of(r);
+        if (m >= M || nc4 <= 0) continue;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(reg + (r * (64 / LPR4) + l / LPR4) * C::PITCH + cc4 * 4);
+        store4(static_cast<float*>(p.C) + coff + (crow + m) * p.ldc + col4, p.vec & kVecC, nc4, x);
       }
     } else {
 #pragma unroll
@@ -817,18 +877,20 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
         const int64_t m = row_of(r);
         float x[8];
         read(r, x);
-        if constexpr (kSwiglu) {
+        if constexpr (EPI == kProdPlain) {
+          if (m < M && nc > 0) store8<true>(p.C, coff + (crow + m) * p.ldc + col, p.vec & kVecC, nc, x);
+        } else if constexpr (kSwiglu) {
           if (m >= M || nc <= 0) continue;
           const f32x4* s = reinterpret_cast<const f32x4*>(reg + (r * RPI + rr) * C::PITCH + C::WTN * 2 + cc * 32);
           const float u[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]};
           if (p.pre) {
             const int64_t at = (crow + m) * p.ldp + col;
-            store8(p.pre, at, false, p.vec & kVecPre, nc, x);
-            store8(p.pre, at + p.N, false, p.vec & kVecPre, nc, u);
+            store8<true>(p.pre, at, p.vec & kVecPre, nc, x);
+            store8<true>(p.pre, at + p.N, p.vec & kVecPre, nc, u);
           }
 #pragma unroll
           for (int v = 0; v < 8; ++v) x[v] = act_of<kActSilu>(x[v]) * u[v];
-          store8(p.C, (crow + m) * p.ldc + col, false, p.vec & kVecC, nc, x);
+          store8<true>(p.C, (crow + m) * p.ldc + col, p.vec & kVecC, nc, x);
         } else if constexpr (EPI == kProdSwigluGrad) {
           // x = d out / d act of columns col ..; the gate's gradient goes to column col, the up's to N + col
           if (m >= M || nc <= 0) continue;
@@ -842,8 +904,8 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
             up[v] = d * ga[v] * sg;
           }
           const int64_t to = (crow + m) * p.ldc + col;
-          store8(p.C, to, false, p.vec & kVecC, nc, x);
-          store8(p.C, to + p.N, false, p.vec & kVecC, nc, up);
+          store8<true>(p.C, to, p.vec & kVecC, nc, x);
+          store8<true>(p.C, to + p.N, p.vec & kVecC, nc, up);
         } else if constexpr (EPI == kProdStats) {
           // largest logit and sum of exponentials of the wave's columns, and the label's logit
           float mx = -INFINITY;
@@ -877,7 +939,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
             x[v] = t.label == -2 || v >= nc ? 0.f : d * t.dloss;
           }
           // the scratch rows are whole units: columns behind the last are zeros, as the products behind read them
-          if (col < p.ldc) store8(p.C, m * p.ldc + col, false, true, 8, x);
+          if (col < p.ldc) store8(p.C, m * p.ldc + col, true, 8, x);
         }
       }
     }
@@ -967,6 +1029,8 @@ using ProdTile64 = PCfg<64, 64, 2, 1, 64, 4>;
 using ProdTile64w = PCfg<64, 128, 2, 2, 64, 3>;
 using ProdTile128 = PCfg<128, 128, 4, 2, 64, 2>;
 using ProdTile256 = PCfg<256, 256, 2, 4, 32, 4, true>;
+// gradients of weights: two workgroups per CU, one's stores beside the other's products
+using ProdTile128w = PCfg<128, 256, 2, 4, 32, 3, true>;
 // of 256-row tiles that hold 128 rows or fewer: the ring holds more of B's stages, 64 KB or more in flight instead of
 // 48; rows along the sum come in whole 128-byte lines
 template <bool BKC>
@@ -981,7 +1045,7 @@ hipError_t launch_product_tile(const ProductParams& p, int tile, int64_t grid, h
     case kProd128: return launch_product_cfg<ProdTile128, void, AKC, BKC, EPI>(p, grid, stream);
     case kProd256:
       // only the epilogues of expert products see small groups
-      if constexpr (EPI <= kProdSwigluGrad) return launch_product_cfg<ProdTile256, ProdFlat256<BKC>, AKC, BKC, EPI>(p, grid, stream);
+      if constexpr (EPI != kProdStats && EPI != kProdDlogits) return launch_product_cfg<ProdTile256, ProdFlat256<BKC>, AKC, BKC, EPI>(p, grid, stream);
       else return launch_product_cfg<ProdTile256, void, AKC, BKC, EPI>(p, grid, stream);
   }
   return hipErrorInvalidValue;

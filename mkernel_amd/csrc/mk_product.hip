@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p) {
         if (i >= nc) d[i] = 0.f;
         s[i] += d[i];
       }
-      if (p.dpre && col < p.width) store8(p.dpre, r * p.width + col, false, true, 8, d);
+      if (p.dpre && col < p.width) store8(p.dpre, r * p.width + col, true, 8, d);
     }
   });
   if (!p.part) return;

@@ -8,7 +8,7 @@
 
 namespace mk {
 
-enum ProductTile : int { kProd32 = 0, kProd64 = 1, kProd64w = 2, kProd128 = 3, kProd256 = 4, kProdTiles = 5 };
+enum ProductTile : int { kProd32 = 0, kProd64 = 1, kProd64w = 2, kProd128 = 3, kProd256 = 4, kProd128w = 5, kProdTiles = 6 };
 constexpr int kProductTickets = 256;  // tiles of a launch whose K is cut into parts, at most
 constexpr int kTicketStride = 32;     // words between them: a line each
 
@@ -16,18 +16,19 @@ constexpr int kTicketStride = 32;     // words between them: a line each
 //   round + K/16 x slope(x),  slope = one + load min(x, 1) + more max(x - 1, 0),  x = the round's workgroups per CU
 // (a full chip clocks lower and shares its caches).  `start` comes once, `area` for a million results (their stores),
 // and where the last round's tiles are cut: meet + part per part, and `exchange` for a MB of partial sums.  Fitted to
-// 1318 launches of 79 shapes of 1 .. 8192 rows, 64 .. 8192 columns and K on one MI355X; the tile and cut that it picks
+// 1392 launches of 79 shapes of 1 .. 8192 rows, 64 .. 8192 columns and K on one MI355X; the tile and cut that it picks
 // take 4 % longer than the best of those tried in the mean (worst 33 %).
 struct ProductShape {
   int bm, bn, per_cu;
   double start, round, one, load, more, meet, part, area, exchange;
 };
 constexpr ProductShape kProductShapes[kProdTiles] = {
-    {32, 128, 2, 3.96, 0.00, 0.077, 0.013, 0.128, 0.80, 0.39, 8.62, 0.12},
-    {64, 64, 2, 3.14, 1.08, 0.068, 0.015, 0.055, 1.01, 0.34, 0.98, 0.16},
-    {64, 128, 2, 4.35, 0.00, 0.071, 0.040, 0.083, 1.32, 0.30, 0.79, 0.32},
-    {128, 128, 2, 4.41, 0.00, 0.098, 0.117, 0.071, 1.83, 0.31, 0.74, 0.29},
-    {256, 256, 1, 7.32, 0.00, 0.139, 0.288, 0.0, 4.28, 1.23, 0.94, 0.16},
+    {32, 128, 2, 4.14, 0.00, 0.077, 0.012, 0.125, 0.84, 0.39, 9.00, 0.11},
+    {64, 64, 2, 3.31, 1.07, 0.070, 0.014, 0.048, 1.08, 0.34, 0.91, 0.16},
+    {64, 128, 2, 4.48, 0.00, 0.071, 0.040, 0.081, 1.42, 0.28, 0.69, 0.33},
+    {128, 128, 2, 3.04, 1.45, 0.098, 0.115, 0.071, 1.91, 0.31, 0.56, 0.29},
+    {256, 256, 1, 6.27, 1.53, 0.137, 0.287, 0.0, 4.28, 1.26, 0.92, 0.15},
+    {128, 256, 2, 5.48, 0.00, 0.171, 0.061, 0.233, 0.0, 2.91, 0.34, 0.38},
 };
 
 // One row or two go to the kernel that has all of K in one workgroup where K is short, or where B would have to be laid
@@ -43,15 +44,17 @@ struct ProductPlan {
 };
 
 // M rows (ragged 1: in `groups` groups, about as many each), `cols` columns of B (SwiGLU: gate and up together), K
-// (ragged 2: of all groups).  cut: whether K may be cut.
+// (ragged 2: of all groups).  plain: results go as they are.
+// cut: whether K may be cut.
 inline ProductPlan plan_product(int64_t M, int64_t cols, int64_t K, int64_t groups, int ragged, bool right_grad,
-                                bool cut, int cus) {
+                                bool plain, bool cut, int cus) {
   ProductPlan best = {};
   bool found = false;
   for (int i = 0; i < kProdTiles; ++i) {
     const ProductShape& s = kProductShapes[i];
     // (tiles of 32 rows stream weights of groups more slowly: 64 tokens' 27 experts of 7168 x 4096 242 us, 214 with 64)
     if ((right_grad || ragged) && s.bm == 32) continue;
+    if (i == kProd128w && !(right_grad && plain)) continue;
     const int64_t tn = (cols + s.bn - 1) / s.bn;
     // a group's rows fill its last tile by half in the mean; of the tallest, rows that are not there cost little
     const int64_t spare = ragged == 1 ? (groups - 1) * (s.bm == 256 ? 64 : s.bm / 2) : 0;
