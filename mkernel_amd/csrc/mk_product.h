@@ -51,6 +51,8 @@ struct PCfg {
   static constexpr int PER_CU = 160 * 1024 / LDS_BYTES;
   static constexpr int WAVES_PER_SIMD = PER_CU * WAVES / 4 > 0 ? PER_CU * WAVES / 4 : 1;
   static constexpr int UNITS = FM * FN * 4;  // 16-byte units of sums per thread
+  // operands of the next stage in registers too, where there are as many
+  static constexpr int AHEAD = !PP && WAVES_PER_SIMD <= 2 ? 1 : 0;
   static_assert(WTM % 32 == 0 && WTN % 64 == 0 && A_INST >= 1 && B_INST >= 1, "tile too small for the wave grid");
   static_assert(A_INST * 1024 * WAVES == A_BYTES && B_INST * 1024 * WAVES == B_BYTES, "DMA shares");
   static_assert(LDS_BYTES <= 160 * 1024 && (S - 1) * LOADS < 64 && S <= 7, "ring");
@@ -611,47 +613,92 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
         }
       }
     } else {
-      // All of a stage's reads go out before its matrix instructions: left alone, the compiler spares registers and
-      // waits for one read after another (512 x 4096 x 4096 on 128 x 128 tiles 41.8 us so).
-      auto compute = [&] {
+      // All of a stage's reads go out before matrix instructions: left alone, the compiler spares registers and waits
+      // for one read after another.
+      bf16x8 af[C::AHEAD + 1][C::KSTEPS][F > 0 ? F : 1], bf[C::AHEAD + 1][C::KSTEPS][C::FN];
+      auto read_stage = [&](auto buf_) {
+        constexpr int buf = decltype(buf_)::value;
         if constexpr (F > 0) {
           const char* sA = smem + rd;
           const char* sB = sA + C::A_BYTES;
-          bf16x8 af[C::KSTEPS][F > 0 ? F : 1], bf[C::KSTEPS][C::FN];
 #pragma unroll
           for (int kk = 0; kk < C::KSTEPS; ++kk) {
 #pragma unroll
-            for (int i = 0; i < F; ++i) af[kk][i] = a.read(sA, kk, i);
+            for (int i = 0; i < F; ++i) af[buf][kk][i] = a.read(sA, kk, i);
 #pragma unroll
-            for (int j = 0; j < C::FN; ++j) bf[kk][j] = b.read(sB, kk, j);
+            for (int j = 0; j < C::FN; ++j) bf[buf][kk][j] = b.read(sB, kk, j);
           }
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int kk = 0; kk < C::KSTEPS; ++kk)
-#pragma unroll
-            for (int i = 0; i < F; ++i)
-#pragma unroll
-              for (int j = 0; j < C::FN; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[kk][j], af[kk][i], acc[i][j], 0, 0, 0);
           rd = next_slot(rd, 0u);
+          __builtin_amdgcn_sched_barrier(0);
         }
       };
-      // Each barrier says that every wave's share of stage j has landed and that every wave has read stage j - 1,
-      // whose slot the next DMA overwrites.
+      auto mfma = [&](auto buf_) {
+        constexpr int buf = decltype(buf_)::value;
+#pragma unroll
+        for (int kk = 0; kk < C::KSTEPS; ++kk)
+#pragma unroll
+          for (int i = 0; i < F; ++i)
+#pragma unroll
+            for (int j = 0; j < C::FN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf[buf][kk][j], af[buf][kk][i], acc[i][j], 0, 0, 0);
+      };
+      using B0 = std::integral_constant<int, 0>;
+      using B1 = std::integral_constant<int, C::AHEAD>;
       int j = 0;
-#pragma clang loop unroll(disable)
-      for (; j + C::S - 1 < nf; ++j) {
-        wait_vm<(C::S - 2) * C::LOADS>();
+      if constexpr (C::AHEAD) {
+        // A stage's operands are read into registers while the matrix instructions of the one before run.  The barrier
+        // of step j says that stage j + 1 has landed and that every wave has read stage j, whose slot takes stage j + S.
+        issue_any(C::S - 1);
+        wait_stage<C::S + 1, C::LOADS>(min(C::S - 1, ns - 1));
         __syncthreads();
-        issue();
-        compute();
-      }
+        read_stage(B0{});
+        auto step = [&](auto cur, auto next) {
+          wait_vm<(C::S - 2) * C::LOADS>();
+          __syncthreads();
+          issue();
+          read_stage(next);
+          mfma(cur);
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        auto step_any = [&](auto cur, auto next, int j) {
+          if (j + 1 < ns) {
+            wait_stage<C::S + 1, C::LOADS>(min(C::S - 2, ns - 2 - j));
+            __syncthreads();
+            issue_any(j + C::S);
+            read_stage(next);
+          }
+          mfma(cur);
+          __builtin_amdgcn_sched_barrier(0);
+        };
 #pragma clang loop unroll(disable)
-      for (; j < ns; ++j) {
-        wait_stage<C::S + 1, C::LOADS>(min(C::S - 2, ns - 1 - j));
-        __syncthreads();
-        issue_any(j + C::S - 1);
-        compute();
+        for (; j + 1 + C::S < nf; j += 2) {
+          step(B0{}, B1{});
+          step(B1{}, B0{});
+        }
+#pragma clang loop unroll(disable)
+        for (; j < ns; j += 2) {
+          step_any(B0{}, B1{}, j);
+          if (j + 1 < ns) step_any(B1{}, B0{}, j + 1);
+        }
+      } else {
+        // Each barrier says that every wave's share of stage j has landed and that every wave has read stage j - 1,
+        // whose slot the next DMA overwrites.
+#pragma clang loop unroll(disable)
+        for (; j + C::S - 1 < nf; ++j) {
+          wait_vm<(C::S - 2) * C::LOADS>();
+          __syncthreads();
+          issue();
+          read_stage(B0{});
+          mfma(B0{});
+        }
+#pragma clang loop unroll(disable)
+        for (; j < ns; ++j) {
+          wait_stage<C::S + 1, C::LOADS>(min(C::S - 2, ns - 1 - j));
+          __syncthreads();
+          issue_any(j + C::S - 1);
+          read_stage(B0{});
+          mfma(B0{});
+        }
       }
     }
   };

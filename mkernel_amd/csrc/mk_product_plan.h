@@ -23,12 +23,12 @@ struct ProductShape {
   double start, round, one, load, more, meet, part, area, exchange;
 };
 constexpr ProductShape kProductShapes[kProdTiles] = {
-    {32, 128, 2, 4.14, 0.00, 0.077, 0.012, 0.125, 0.84, 0.39, 9.00, 0.11},
-    {64, 64, 2, 3.31, 1.07, 0.070, 0.014, 0.048, 1.08, 0.34, 0.91, 0.16},
-    {64, 128, 2, 4.48, 0.00, 0.071, 0.040, 0.081, 1.42, 0.28, 0.69, 0.33},
-    {128, 128, 2, 3.04, 1.45, 0.098, 0.115, 0.071, 1.91, 0.31, 0.56, 0.29},
-    {256, 256, 1, 6.27, 1.53, 0.137, 0.287, 0.0, 4.28, 1.26, 0.92, 0.15},
-    {128, 256, 2, 5.48, 0.00, 0.171, 0.061, 0.233, 0.0, 2.91, 0.34, 0.38},
+    {32, 128, 2, 3.68, 0.00, 0.076, 0.015, 0.129, 0.95, 0.39, 5.42, 0.13},
+    {64, 64, 2, 2.97, 0.84, 0.071, 0.012, 0.052, 1.17, 0.34, 0.69, 0.17},
+    {64, 128, 2, 3.81, 0.00, 0.071, 0.040, 0.084, 1.46, 0.30, 0.53, 0.30},
+    {128, 128, 2, 2.66, 1.12, 0.099, 0.113, 0.079, 1.94, 0.32, 0.47, 0.29},
+    {256, 256, 1, 4.95, 1.00, 0.141, 0.266, 0.0, 4.41, 1.32, 0.86, 0.13},
+    {128, 256, 2, 5.37, 0.00, 0.167, 0.073, 0.231, 2.95, 0.90, 0.36, 0.31},
 };
 
 // One row or two go to the kernel that has all of K in one workgroup where K is short, or where B would have to be laid
