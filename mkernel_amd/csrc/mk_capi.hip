@@ -1626,12 +1626,13 @@ int gemm_act_backward_body(const mk_gemm_act_backward_args* a, Products g) {
 
 // ---- expert products on ragged rows ----
 
+Matrix counts_of(const int32_t* counts, int32_t E) { return {"counts", counts, 1, E, E, 4}; }
+
 int check_ragged(const char* fn, int64_t R, int64_t K, int64_t N, int32_t E, const void* counts) {
   if (int rc = check_sizes(fn, R, N, K)) return rc;
   if (K == 0 || N == 0 || K > kMaxLd) return fail(MK_ESHAPE, "%s: K and N must be 1 .. %lld", fn, (long long)kMaxLd);
   if (E <= 0 || E > mk::kMaxExperts) return fail(MK_ESHAPE, "%s: 1 .. %d experts", fn, mk::kMaxExperts);
-  if (!counts) return fail(MK_EINVAL, "%s: counts is null", fn);
-  return MK_OK;
+  return counts ? MK_OK : fail(MK_EINVAL, "%s: counts is null", fn);
 }
 
 int check_ragged_gemm(const char* fn, const mk_moe_ragged_gemm_args* a) {
@@ -1640,7 +1641,8 @@ int check_ragged_gemm(const char* fn, const mk_moe_ragged_gemm_args* a) {
   if (int rc = check_ragged(fn, a->R, a->K, a->N, a->num_experts, a->counts)) return rc;
   if (a->mode == 1 && a->N % 2) return fail(MK_ESHAPE, "%s: N must be even with SwiGLU", fn);
   if (a->mode == 0 && a->h) return fail(MK_EINVAL, "%s: h belongs to mode 1", fn);
-  return check_matrices(fn, {{"A", a->A, a->R, a->K, a->lda, 2}, {"W", a->W, a->num_experts * a->K, a->N, a->N, 2}},
+  return check_matrices(fn, {{"A", a->A, a->R, a->K, a->lda, 2}, {"W", a->W, a->num_experts * a->K, a->N, a->N, 2},
+                             counts_of(a->counts, a->num_experts)},
                         {{"out", a->out, a->R, a->mode ? a->N / 2 : a->N, a->ldo, 2}, {"h", a->h, a->h ? a->R : 0, a->N, a->ldh, 2}});
 }
 
@@ -1674,7 +1676,8 @@ int check_ragged_dgrad(const char* fn, const mk_moe_ragged_dgrad_args* a) {
   return check_matrices(fn,
                         {{"dy", a->dy, a->R, a->N, a->lddy, 2},
                          {"W", a->W, a->num_experts * a->K, a->N, a->N, 2},
-                         {"h", a->h, a->h ? a->R : 0, width, a->ldh, 2}},
+                         {"h", a->h, a->h ? a->R : 0, width, a->ldh, 2},
+                         counts_of(a->counts, a->num_experts)},
                         {{"out", a->out, a->R, width, a->ldo, 2}}, a->h, a->out);
 }
 
@@ -1698,7 +1701,8 @@ int check_ragged_wgrad(const char* fn, const mk_moe_ragged_wgrad_args* a) {
   if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
   if (int rc = check_ragged(fn, a->R, a->K, a->N, a->num_experts, a->counts)) return rc;
   if (!is_type(a->dw_type)) return fail(MK_EINVAL, "%s: dw_type must be 0 or 1", fn);
-  return check_matrices(fn, {{"A", a->A, a->R, a->K, a->lda, 2}, {"dy", a->dy, a->R, a->N, a->lddy, 2}},
+  return check_matrices(fn, {{"A", a->A, a->R, a->K, a->lda, 2}, {"dy", a->dy, a->R, a->N, a->lddy, 2},
+                             counts_of(a->counts, a->num_experts)},
                         {{"dW", a->dW, a->num_experts * a->K, a->N, a->N, size_of(a->dw_type)}});
 }
 

@@ -211,3 +211,12 @@ def test_plans_hold_for_any_size(plans):
             assert 0 < tiles - whole <= 256 and (tiles - whole) * s <= per_cu * 256 and s <= 16 and K >= 128 * s - 15
         else:
             assert whole == tiles
+
+
+@pytest.mark.parametrize("name,out", [("mk_moe_ragged_gemm", "out"), ("mk_moe_ragged_dgrad", "out"), ("mk_moe_ragged_wgrad", "dW")])
+def test_results_over_the_counts_are_refused(name, out):
+    """Workgroups read the counts while others store results already."""
+    for at, what in ((7 * FAR, "overlaps counts"), (7 * FAR + 14, "overlaps counts"), (7 * FAR + 2, "counts must be aligned")):
+        a = _args(name, {"counts": at if "aligned" in what else 7 * FAR, out: 8 * FAR if "aligned" in what else at})
+        assert getattr(capi.lib(), name)(C.byref(a), None) == EINVAL
+        assert what in capi.lib().mk_last_error_string().decode()
