@@ -705,8 +705,8 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* args, void* stream);
 /* Dense products of any size with what follows them, and their gradients.
  *
  * Common to the entry points from here to mk_vocab_loss_backward: bf16
- * operands, fp32 sums, one rounding at the end.  Any sizes and row strides (of
- * at least the row's width, at most 2^21 elements); operands aligned to their
+ * operands, fp32 sums, one rounding at the end.  Any sizes up to 2^25 rows and
+ * row strides (of at least the row's width, at most 2^21 elements); operands aligned to their
  * elements.  Operands whose rows do not start at 16-byte boundaries, or whose
  * rows' ends do not fill 16 bytes where the sum runs along them, are laid out
  * anew in the workspace first.  Results may not overlap what is read, unless

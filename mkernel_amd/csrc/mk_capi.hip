@@ -1353,7 +1353,8 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* a, void* stream) {
 // ---------------------------------------------------------------------------
 namespace {
 
-constexpr int64_t kMaxLd = 1 << 21, kMaxRows = 1 << 30;
+// a launch has fewer than 2^32 threads in a dimension: 64 a row, where rows are laid out anew
+constexpr int64_t kMaxLd = 1 << 21, kMaxRows = 1 << 25;
 
 // The pieces of a workspace, one behind the other.  A call's body runs twice:
 // once to count (nothing is queued), once to work.
@@ -1423,7 +1424,7 @@ struct Products {
     // (a group of t row tiles: ceil(tn / 8) t, or ceil(tn / 4) ceil(t / 2) <= ceil(tn / 8) (t + 1))
     if (p.ragged == 1) grid = 8 * ((tn + 7) / 8) * std::min(tm + 2 * groups - 1, 2 * p.M);
     if (p.ragged == 2) grid = 8 * ((tm * tn + 7) / 8) * groups;
-    if (grid >= (1LL << 31)) return fail(MK_ESHAPE, "%s: too many tiles", fn);
+    if (grid >= (1LL << 32) / 512) return fail(MK_ESHAPE, "%s: too many tiles", fn);  // of 512 threads or fewer
     const int64_t mark = sp.used;
     if (p.split > 1) p.parts = static_cast<float*>(sp.take((plan.tiles - plan.whole) * p.split * s.bm * s.bn * 4));
     sp.used = mark;  // the next launch may use them again

@@ -220,3 +220,12 @@ def test_results_over_the_counts_are_refused(name, out):
         a = _args(name, {"counts": at if "aligned" in what else 7 * FAR, out: 8 * FAR if "aligned" in what else at})
         assert getattr(capi.lib(), name)(C.byref(a), None) == EINVAL
         assert what in capi.lib().mk_last_error_string().decode()
+
+
+@pytest.mark.parametrize("name,rows", [("mk_gemm_act", "M"), ("mk_gemm_act_backward", "M"), ("mk_moe_ragged_gemm", "R"),
+                                       ("mk_moe_ragged_dgrad", "R"), ("mk_moe_ragged_wgrad", "R")])
+def test_rows_beyond_a_launch_are_refused(name, rows):
+    """More rows than a kernel that has 64 threads for each can be launched for."""
+    a = _args(name, {rows: (1 << 25) + 1})
+    assert getattr(capi.lib(), name)(C.byref(a), None) == ESHAPE
+    assert "sizes" in capi.lib().mk_last_error_string().decode()
