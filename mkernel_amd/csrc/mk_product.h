@@ -300,6 +300,8 @@ __device__ __forceinline__ float act_slope(float x) {
   } else if constexpr (ACT == kActGelu) {
     return normal_cdf(x) + x * 0.3989422804014327f * __expf(-0.5f * x * x);
   } else if constexpr (ACT == kActGeluTanh) {
+    // (beyond 30 it is 0 or 1 to the last bit; squares of numbers beyond 2^64 would be infinite)
+    x = x > 30.f ? 30.f : x < -30.f ? -30.f : x;
     const float s = sigmoid(1.5957691216057308f * (x + 0.044715f * x * x * x));
     return s + x * s * (1.f - s) * 1.5957691216057308f * (1.f + 0.134145f * x * x);
   } else if constexpr (ACT == kActSilu) {

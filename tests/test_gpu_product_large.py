@@ -319,6 +319,18 @@ def test_other_current_device_and_refusals():
             bad()
 
 
+def test_slopes_of_far_arguments():
+    """dpre = act'(pre) at arguments whose powers leave fp32: 0 or 1 there, for every activation."""
+    pre = torch.tensor([[-3e38, -1e30, -1e20, -1e10, -300.0, -40.0, 40.0, 300.0, 1e10, 1e20, 1e30, 3e38]]).to(BF16).cuda()
+    n = pre.shape[1]
+    one = torch.ones(1, n, dtype=BF16, device="cuda")
+    want = (pre > 0).float()[0]
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        db = ops.gemm_act_backward(one, one[:, :1], torch.zeros(1, n, dtype=BF16, device="cuda"), pre, act)[2]
+        # -40 e^-40 is the largest of what is not 0; at 1 a reciprocal (a step) and three roundings
+        assert (db - want).abs().le(2e-16 + 5 * U * want).all(), (act, db)
+
+
 # ---------------------------------------------------------------- a training step of the expert layer
 @pytest.mark.parametrize("row_block", [1, 128])
 def test_expert_layer_training_step(row_block):
