@@ -10,6 +10,7 @@ import contextlib
 import ctypes as C
 import itertools
 import math
+import threading
 
 import numpy as np
 import torch
@@ -794,18 +795,26 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
 
 # ------------------------------------------------------------------- products with what follows them
 # Tickets (zeroed words by which the parts of a product's K meet, left zeroed by every launch) and behind them a small
-# workspace: one set per (device, stream), whose launches are ordered.
+# workspace: one set per thread, device and stream, whose launches are ordered (the launches of two threads' calls on
+# one stream may come between each other).
 _SPACE = 4 << 20
-_spaces: dict = {}
+
+
+class _Spaces(threading.local):
+    def __init__(self):
+        self.of = {}
+
+
+_spaces = _Spaces()
 
 
 def _space(index: int, stream: int) -> int:
-    t = _spaces.get((index, stream))
+    t = _spaces.of.get((index, stream))
     if t is None:
         n = capi.PRODUCT_TICKETS * 4
         t = torch.empty(n + _SPACE, dtype=torch.uint8, device=torch.device("cuda", index))
         t[:n].zero_()
-        _spaces[index, stream] = t
+        _spaces.of[index, stream] = t
     return t.data_ptr()
 
 

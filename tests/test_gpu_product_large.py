@@ -331,6 +331,29 @@ def test_slopes_of_far_arguments():
         assert (db - want).abs().le(2e-16 + 5 * U * want).all(), (act, db)
 
 
+def test_two_threads_on_one_stream():
+    """Calls whose operands are laid out anew in the workspace, from two threads at once."""
+    import threading
+    A, B = randn(300, 2811), [randn(2811, 205, seed=s) for s in (1, 2)]
+    want = [ops.gemm_act(A, b) for b in B]
+    torch.cuda.synchronize()
+    got, start = [[], []], threading.Barrier(2)
+
+    def work(i):
+        start.wait()
+        for _ in range(200):
+            got[i].append(ops.gemm_act(A, B[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert len(g) == 200 and all(torch.equal(x, w) for x in g)
+
+
 # ---------------------------------------------------------------- a training step of the expert layer
 @pytest.mark.parametrize("row_block", [1, 128])
 def test_expert_layer_training_step(row_block):
