@@ -836,7 +836,9 @@ int mk_moe_ragged_wgrad(const mk_moe_ragged_wgrad_args* args, void* stream);
  *   lse = log sum_v e^logit,  target = the label's logit (0 where another shard
  *   has it),  loss = lse - target.
  * Shards are joined by lse = log sum e^lse_i and the sum of the targets.  Tokens
- * whose label is ignore_index have zeros in all three, whatever their x holds. */
+ * whose label is ignore_index have zeros in all three, whatever their x holds (the
+ * join of such zeros is for the caller to set to 0; the backward pass gives these
+ * tokens zeros whatever their lse and dloss are). */
 typedef struct mk_vocab_loss_args {
   const void* x;          /* bf16 [T, ldx] */
   const void* W;          /* bf16 [H, ldw] */

@@ -1073,7 +1073,9 @@ def vocab_loss(x: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, vocab_beg
     rows of x hold.  One rank's shard of a vocabulary: W holds the columns from
     vocab_begin on, and target is 0 where another rank has the label; the ranks'
     lse are joined by torch.logsumexp, their targets by a sum, and the loss is
-    the difference."""
+    the difference (ignored tokens, whose zeros join to the logarithm of the
+    ranks' number, are set to 0 by the caller; the backward pass gives them zeros
+    whatever their lse and dloss are)."""
     T, H, V, dev, wide = _vocab(x, W, labels)
     if dev.index != _device_index():
         with torch.cuda.device(dev):

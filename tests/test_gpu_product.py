@@ -531,3 +531,21 @@ def test_vocab_loss_pieces_of_laid_out_weights():
     T, H, V = 5, 4096, 33001
     labels = torch.tensor([0, 16383, 16384, 32768, 33000])
     _check_vocab(T, H, V, labels, randn(T, H, seed=99), randn(H, V, seed=100, scale=2 * H ** -0.5))
+
+
+def test_vocab_loss_backward_of_ignored_tokens():
+    """Zeros, whatever their rows, lse and dloss hold (a shard's joined lse of them is not 0)."""
+    T, H, V = 40, 72, 333
+    labels = _labels(T, V, 97)
+    off = torch.arange(T) % 3 == 1
+    labels[off] = -100
+    x, W, labels, off = randn(T, H, seed=98), randn(H, V, seed=99, scale=0.3), labels.cuda(), off.cuda()
+    lse = ops.vocab_loss(x, W, labels)["lse"]
+    dloss = torch.full((T,), 0.25, device="cuda")
+    want = ops.vocab_loss_backward(x, W, labels, lse, dloss, dx_dtype=F32, dW_dtype=F32)
+    assert (want[0][off] == 0).all()
+    for bad in (float("nan"), float("inf"), -float("inf"), 0.6931):
+        got = ops.vocab_loss_backward(torch.where(off[:, None], bad, x.float()).to(BF16), W, labels,
+                                      torch.where(off, bad, lse), torch.where(off, bad, dloss), dx_dtype=F32,
+                                      dW_dtype=F32)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
