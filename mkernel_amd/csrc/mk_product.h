@@ -540,8 +540,14 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
       // instructions, so each SIMD's matrix core is fed while the partner loads.
       // The loops over whole stages hold no test but their own: a memory step
       // has to fit beside the 512 cycles of the partner's matrix instructions.
+      // (Reads or loads between the matrix instructions, which shorten it, cost
+      // more there: 16384 x 8192 x 3584 755 to 835 us instead of 734.)  In forward
+      // products its waves go first: 734 us without, 724 with; gradients took as
+      // long or 1 % longer so.
+      constexpr bool FIRST = AKC && !BKC;
       bf16x8 af[C::KSTEPS][F > 0 ? F : 1], bf[C::KSTEPS][C::FN];
       auto read_stage = [&] {
+        if constexpr (FIRST) __builtin_amdgcn_s_setprio(1);
         if constexpr (F > 0) {
           const char* sA = smem + rd;
           const char* sB = sA + C::A_BYTES;
@@ -556,6 +562,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
         }
       };
       auto mfma = [&] {
+        if constexpr (FIRST) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int kk = 0; kk < C::KSTEPS; ++kk)
 #pragma unroll
