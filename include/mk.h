@@ -862,7 +862,8 @@ int mk_vocab_loss(const mk_vocab_loss_args* args, void* stream);
  *   dx = dl @ W^T (of a shard: its part of the sum),  dW = x^T @ dl.
  * Logits are computed anew, a piece of the vocabulary at a time (piece_columns, a
  * multiple of 256; 0: the library's choice), dl goes through the workspace in
- * bf16.  Either result may be NULL; accumulate: dW is added to. */
+ * bf16 (without the significand of the largest dloss, which the fp32 sums take
+ * back: of a mean's equal dloss no common rounding stays).  Either result may be NULL; accumulate: dW is added to. */
 typedef struct mk_vocab_loss_backward_args {
   const void* x;          /* bf16 [T, ldx] */
   const void* W;          /* bf16 [H, ldw] */

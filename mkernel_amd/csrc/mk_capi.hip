@@ -1831,7 +1831,9 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
   mk::RepackParams r = {};
   r.src = u16(a->x); r.rows = T; r.cols = H; r.ld = T == 1 ? H : a->ldx; r.width = ldx; r.parts = 1; r.E = 1;
   r.labels = a->labels; r.labels64 = a->labels_type; r.ignore = a->ignore_index;
+  r.dloss = a->dloss;
   uint16_t* x = r.dst = static_cast<uint16_t*>(g.sp.take(T * ldx * 2));
+  float* scale = r.scale = static_cast<float*>(g.sp.take(4));
   uint16_t* dl = static_cast<uint16_t*>(g.sp.take(T * piece * 2));
   float* sum = nullptr;  // of dx over the pieces
   int64_t lds = H;
@@ -1858,7 +1860,7 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
     p.M = T; p.N = n; p.K = H;
     fill_vocab(p, a->labels, a->labels_type, a->ignore_index, a->vocab_begin, V);
     p.first_col = c0;
-    p.lse = a->lse; p.dloss = a->dloss;
+    p.lse = a->lse; p.dloss = a->dloss; p.scale = scale;
     p.C = dl; p.ldc = piece;
     if (int rc = g.run(mk::kProdForward, mk::kProdDlogits, p, n)) return rc;
     if (a->dx) {
@@ -1867,6 +1869,7 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
       q.A = dl; q.lda = piece;
       q.B = w; q.ldb = ldw;
       q.M = T; q.N = H; q.K = n;
+      q.scale = scale;
       if (c0 > 0) {
         q.res = sum; q.ldr = lds; q.res_f32 = 1;
         if (g.sp.counting || vec_rows(sum, lds, 0)) q.vec |= mk::kVecRes;
@@ -1882,6 +1885,7 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
       q.A = x; q.lda = ldx;
       q.B = dl; q.ldb = piece; q.b_cols = n;
       q.M = H; q.N = n; q.K = T;
+      q.scale = scale;
       q.C = static_cast<char*>(a->dW) + c0 * size_of(a->dw_type);
       q.ldc = a->lddw; q.c_f32 = a->dw_type == 0;
       if (vec_rows(q.C, q.ldc, a->dw_type)) q.vec = mk::kVecC | mk::kVecRes;

@@ -300,6 +300,7 @@ struct ProductParams {
   float* target;
   const float* lse;
   const float* dloss;
+  const float* scale;       // one number that dloss is divided by and the gradients' sums multiplied with, or null
 };
 hipError_t launch_product_forward(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
 hipError_t launch_product_left_grad(const ProductParams& p, int epi, int tile, int64_t grid, hipStream_t stream);
@@ -319,6 +320,8 @@ struct RepackParams {
   const void* labels;
   int labels64;
   int64_t ignore;
+  const float* dloss;       // with labels: `scale` gets 1 <= the significand < 2 of the largest finite |dloss| there
+  float* scale;
 };
 hipError_t launch_repack(const RepackParams& p, hipStream_t stream);
 // dpre = dC * act'(pre), bf16 rows of `width` (null: not kept), and the columns' sums of it

@@ -497,9 +497,17 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
       token.label = label < 0 ? (int)label : c >= 0 && c < C::BN ? (int)c : -1;
       if constexpr (EPI == kProdDlogits) {
         token.lse = p.lse[m0 + tid];
-        token.dloss = p.dloss[m0 + tid];
+        // bf16 rounds this token's gradients of the logits; where every token has the same dloss (a mean's 1 / T), those
+        // of the labels, about -dloss, would all be off by the same, up to 2^-8 of it: without its significand they are
+        // about a power of two, and the products' sums take it back
+        token.dloss = p.dloss[m0 + tid] / *p.scale;
       }
     }
+  }
+  constexpr bool SCALED = !(AKC && !BKC);  // gradients
+  float scale = 1.f;
+  if constexpr (SCALED) {
+    if (p.scale) scale = *p.scale;
   }
   const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
   f32x16 acc[C::FM][C::FN];
@@ -857,7 +865,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
       for (int q = 0; q < 4; ++q) {
         f32x4 w;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) w[v] = acc[i][j][4 * q + v];
+        for (int v = 0; v < 4; ++v) w[v] = SCALED ? acc[i][j][4 * q + v] * scale : acc[i][j][4 * q + v];
         *reinterpret_cast<f32x4*>(reg + ml * C::PITCH + (32 * j + 8 * q + 4 * kg) * 4) = w;
       }
     wait_lgkm_all();

@@ -103,15 +103,35 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_rows_kernel(Produc
 
 // A wave copies 512 columns of a row; one workgroup four rows of group blockIdx.z, columns from 2048 * blockIdx.y on.
 // (Loads of single elements moved 1.4 TB/s, a 1024 x 5003 matrix in 14.3 us.)
+__device__ __forceinline__ bool ignored(const RepackParams& p, int64_t row) {
+  return (p.labels64 ? static_cast<const int64_t*>(p.labels)[row] : static_cast<const int*>(p.labels)[row]) == p.ignore;
+}
+
 __global__ __launch_bounds__(256) void repack_kernel(RepackParams p) {
   const int lane = threadIdx.x & 63;
+  if (p.scale && blockIdx.x == 0 && blockIdx.y == 0) {
+    __shared__ uint32_t largest[4];
+    uint32_t most = 0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < p.rows; i += 256) {
+      const uint32_t b = __float_as_uint(p.dloss[i]) & 0x7fffffffu;
+      if (b < 0x7f800000u && !ignored(p, i)) most = max(most, b);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+    if (lane == 0) largest[threadIdx.x >> 6] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      most = max(max(largest[0], largest[1]), max(largest[2], largest[3]));
+      *p.scale = most < 0x00800000u ? 1.f : __uint_as_float((most & 0x007fffffu) | 0x3f800000u);
+    }
+  }
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= p.rows || (p.counts && p.counts[blockIdx.z] <= 0)) return;
   const uint16_t* src = p.src + blockIdx.z * p.src_stride + row * p.ld;
   uint16_t* dst = p.dst + blockIdx.z * p.dst_stride + row * p.width * p.parts;
   bool off = false;
-  if (p.labels)
-    off = (p.labels64 ? static_cast<const int64_t*>(p.labels)[row] : static_cast<const int*>(p.labels)[row]) == p.ignore;
+  if (p.labels) off = ignored(p, row);
   for (int part = 0; part < p.parts; ++part, src += p.cols, dst += p.width) {
     words_at_any w[4];
 #pragma unroll

@@ -1096,7 +1096,9 @@ def vocab_loss_backward(x: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, 
     (float32 [T]) and lse (of a shard: the joined one).  The logits are computed
     anew, a piece of the vocabulary at a time (piece_columns, a multiple of 256;
     0: as many as keep the piece's gradient of the logits below 128 MB); that
-    gradient is rounded to bf16 between the products.  A shard's dx is its part
+    gradient is rounded to bf16 between the products (dloss without the
+    significand of its largest, which the sums take back, so that a mean's equal
+    dloss leaves no common rounding).  A shard's dx is its part
     of a sum over the ranks (dx_dtype=torch.float32 for that).  accumulate: dW,
     which is then given, is added to."""
     T, H, V, dev, wide = _vocab(x, W, labels)

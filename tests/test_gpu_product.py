@@ -549,3 +549,43 @@ def test_vocab_loss_backward_of_ignored_tokens():
                                       torch.where(off, bad, lse), torch.where(off, bad, dloss), dx_dtype=F32,
                                       dW_dtype=F32)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("every", [1.0 / 509, 1.0039, 1.0, 0.25 + 2.0 ** -10])
+@pytest.mark.parametrize("piece", [0, 512])
+def test_vocab_loss_backward_keeps_the_scale(every, piece):
+    """One dloss for all tokens, whatever its significand: the gradients are not longer or shorter than they should be.
+    The factor of the nearest multiple of the right gradient is off by the labels' entries of dl, -(1 - p) times a power
+    of two, whose rounding is off by p at most where p < 2^-9 (to 1), by the other entries' roundings, random and of
+    2^-9 each, over the root of their number, and by the sums' of at most 2^-14."""
+    T, H, V = 509, 64, 4000
+    labels = _labels(T, V, 100).cuda()
+    x, W = randn(T, H, seed=101), randn(H, V, seed=102, scale=0.3 * H ** -0.5)
+    lse = ops.vocab_loss(x, W, labels)["lse"]
+    dloss = torch.full((T,), every, device="cuda")
+    dx, dW = ops.vocab_loss_backward(x, W, labels, lse, dloss, dx_dtype=F32, dW_dtype=F32, piece_columns=piece)
+    p = torch.softmax(d(x) @ d(W), 1)
+    most = float(p.max())
+    assert most < 2.0 ** -9
+    p[torch.arange(T), labels.cpu()] -= 1
+    dl = p * d(dloss)[:, None]
+    for got, want in ((d(dx), dl @ d(W).t()), (d(dW), d(x).t() @ dl)):
+        factor = float((got * want).sum() / (want * want).sum())
+        assert abs(factor - 1) <= most + 2.0 ** -9 / T ** 0.5 + 2.0 ** -14, factor
+
+
+def test_vocab_loss_backward_of_unlike_dloss():
+    """Largest, smallest, infinite, NaN and zero dloss beside each other: each row of dx is its token's alone."""
+    T, H, V = 24, 40, 300
+    labels = _labels(T, V, 103).cuda()
+    x, W = randn(T, H, seed=104), randn(H, V, seed=105, scale=0.3)
+    lse = ops.vocab_loss(x, W, labels)["lse"]
+    dloss = torch.tensor([1.5, 1e-30, 3e30, float("inf"), float("nan"), 0.0, -2.75, 1e-3] * 3, device="cuda")
+    dx = d(ops.vocab_loss_backward(x, W, labels, lse, dloss, need_dW=False, dx_dtype=F32)[0])
+    p = torch.softmax(d(x) @ d(W), 1)
+    p[torch.arange(T), labels.cpu()] -= 1
+    finite = torch.isfinite(dloss).cpu()
+    dl = p * d(dloss)[:, None]
+    tol = 2.0 ** -7 * dl.abs() @ d(W).abs().t()
+    assert ((dx - dl @ d(W).t()).abs()[finite] <= tol[finite]).all()
+    assert not torch.isfinite(dx[~finite]).any()
