@@ -112,7 +112,7 @@ def _args(name, change):
     return a
 
 
-@pytest.mark.parametrize("name,change,code,match", REFUSALS, ids=lambda v: str(v)[:40])
+@pytest.mark.parametrize("name,change,code,match", REFUSALS, ids=[f"{r[0]}-{i}" for i, r in enumerate(REFUSALS)])
 def test_refusals(name, change, code, match):
     L, a = capi.lib(), _args(name, change)
     assert getattr(L, name)(C.byref(a), None) == code, L.mk_last_error_string()
