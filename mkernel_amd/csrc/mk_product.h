@@ -325,7 +325,7 @@ __device__ __forceinline__ void for_act(int act, F f) {
 // (largest, sum of exponentials relative to it) of two sets of columns.
 __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
   const float to = fmaxf(a.x, b.x);
-  const float ref = to == -INFINITY ? 0.f : to;  // all of it -inf: sums are 0 (or NaN, which stays)
+  const float ref = fabsf(to) == INFINITY ? 0.f : to;  // all of it -inf: sums are 0 (NaN stays); one inf: so is the sum
   return {to, a.y * __expf(a.x - ref) + b.y * __expf(b.x - ref)};
 }
 
@@ -978,7 +978,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
 #pragma unroll
           for (int d = 1; d < LPR; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
           float sum = 0.f;
-          const float ref = mx == -INFINITY ? 0.f : mx;
+          const float ref = fabsf(mx) == INFINITY ? 0.f : mx;
 #pragma unroll
           for (int v = 0; v < 8; ++v) sum += v < nc ? __expf(x[v] - ref) : 0.f;
 #pragma unroll

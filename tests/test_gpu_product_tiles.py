@@ -74,3 +74,21 @@ def test_vocab_loss(T, H, V, piece):
     near(dx, want, HALF[BF16] * (want.abs() + tol) + tol + 1e-300)
     want, tol = xs.to(F64).t() @ dl, xs.to(F64).abs().t() @ (de + (T + 1) * U * dl.abs())
     near(dW, want, HALF[BF16] * (want.abs() + tol) + tol)
+
+
+@pytest.mark.parametrize("T,H,V", [(3, 40, 17), (33, 100, 515), (130, 257, 1003), (600, 72, 9000), (2100, 64, 32000)])
+def test_vocab_loss_of_infinite_logits(T, H, V):
+    """log sum exp is inf where a logit is (the loss too, unless it is the label's own), and -inf where all are."""
+    x, W = randn(T, H, seed=22), randn(H, V, seed=23)
+    W[0], W[1] = W[0].abs() + 1, -(W[1].abs() + 1)
+    W[2] = 1.0
+    W[2, V // 2:] = -1.0
+    labels = torch.arange(T, device="cuda") % (V // 2) + V // 2
+    x[0, 0], x[1, 1], x[2, 2] = float("inf"), float("inf"), float("inf")  # all logits inf; all -inf; some of both
+    r = ops.vocab_loss(x, W, labels)
+    inf = float("inf")
+    assert r["lse"][:3].tolist() == [inf, -inf, inf] and r["target"][:3].tolist() == [inf, -inf, -inf]
+    assert r["loss"][:2].isnan().all() and r["loss"][2] == inf
+    assert r["lse"][3:].isfinite().all() and r["loss"][3:].isfinite().all()
+    rest = ops.vocab_loss(x[3:], W, labels[3:])["lse"] if T > 3 else None
+    assert rest is None or torch.allclose(rest, r["lse"][3:], rtol=1e-5, atol=1e-5)
