@@ -718,6 +718,13 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* args, void* stream);
  * them must be ordered. */
 #define MK_PRODUCT_TICKETS 8192
 
+/* What lies between two products of a backward pass (dpre, dl) is held in bf16,
+ * which one product takes, or as fp32's three bf16 parts (x rounded, the rest
+ * rounded, the rest), a product each: three times the operations. */
+#define MK_BETWEEN_RESULT 0 /* for each result as its own type: three parts for fp32 */
+#define MK_BETWEEN_BF16 1
+#define MK_BETWEEN_FP32 2
+
 #define MK_ACT_NONE 0
 #define MK_ACT_RELU 1
 #define MK_ACT_GELU 2      /* x * Phi(x) */
@@ -748,9 +755,12 @@ int mk_gemm_act(const mk_gemm_act_args* args, void* stream);
 /* Gradients of mk_gemm_act (the residual's is dC itself): with
  * dpre = dC * act'(pre),
  *   dA = dpre @ B^T (bf16),  dB = A^T @ dpre,  dbias = column sums of dpre (fp32).
- * Each of the three may be NULL.  pre is needed with an activation; dpre is then
- * rounded to bf16 for the two products (matrix cores take nothing wider at their
- * rate; dA and dB are off by about 1.4 of their own rounding), not for dbias.
+ * Each of the three may be NULL.  pre is needed with an activation; `between`
+ * says how dpre goes into the two products (matrix cores take nothing wider than
+ * bf16 at their rate).  In bf16 each product is off by up to 2^-8 of itself
+ * (4096 cubed, silu: error of bf16 dA and dB 0.0023 in norm, 0.0017 without),
+ * which is thousands of times an fp32 result's own rounding.  dbias takes dpre as
+ * it is; without an activation, and with relu, bf16 holds it exactly.
  * accumulate: dB and dbias are added to what they hold (gradients of several
  * batches). */
 typedef struct mk_gemm_act_backward_args {
@@ -764,7 +774,7 @@ typedef struct mk_gemm_act_backward_args {
   int64_t M, N, K;
   int64_t lddc, lda, ldb, ldp, ldda, lddb;
   int32_t act, db_type;  /* db_type 0 fp32, 1 bf16 */
-  int32_t accumulate;
+  int16_t accumulate, between; /* MK_BETWEEN_* */
   void* workspace;
   int64_t workspace_bytes;
   void* tickets;

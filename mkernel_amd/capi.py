@@ -71,11 +71,13 @@ EXPORTS = (
 _PRODUCTS = ("mk_gemm_act", "mk_gemm_act_backward", "mk_moe_ragged_gemm", "mk_moe_ragged_dgrad", "mk_moe_ragged_wgrad",
              "mk_vocab_loss", "mk_vocab_loss_backward")
 PRODUCT_TICKETS = 8192  # include/mk.h MK_PRODUCT_TICKETS
+BETWEEN = {"result": 0, "bf16": 1, "fp32": 2}  # MK_BETWEEN_*
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # MK_ACT_*
 
 vp = C.c_void_p
 i64 = C.c_int64
 i32 = C.c_int32
+i16 = C.c_int16
 u32 = C.c_uint32
 f32 = C.c_float
 
@@ -222,7 +224,7 @@ class GemmActArgs(C.Structure):
 class GemmActBackwardArgs(C.Structure):
     _fields_ = [("dC", vp), ("A", vp), ("B", vp), ("pre", vp), ("dA", vp), ("dB", vp), ("dbias", vp), ("M", i64),
                 ("N", i64), ("K", i64), ("lddc", i64), ("lda", i64), ("ldb", i64), ("ldp", i64), ("ldda", i64),
-                ("lddb", i64), ("act", i32), ("db_type", i32), ("accumulate", i32), ("workspace", vp),
+                ("lddb", i64), ("act", i32), ("db_type", i32), ("accumulate", i16), ("between", i16), ("workspace", vp),
                 ("workspace_bytes", i64), ("tickets", vp)]
 
 
@@ -339,7 +341,7 @@ def call(fn: str, args: C.Structure, stream: int) -> None:
 # which the library and its launch take 3.8.  Values struct refuses (ctypes
 # wraps integers out of a field's range) go through the Structure, so every
 # call means what it meant.
-_FORMAT = {vp: "P", i64: "q", i32: "i", u32: "I", f32: "f"}
+_FORMAT = {vp: "P", i64: "q", i32: "i", u32: "I", i16: "h", f32: "f"}
 _packers: dict = {}
 _functions: dict = {}
 

@@ -1434,6 +1434,27 @@ struct Products {
                                                  : mk::launch_product_right_grad(p, epi, plan.tile, grid, stream));
   }
 
+  // The product of the sum of `terms` operands, the left one's or the right one's, `stride` elements apart, each smaller
+  // than the one before by bf16's rounding: the smallest first, each added to the sum so far.  `sum`: fp32 [M, lds].
+  int run_terms(int order, const mk::ProductParams& p, int64_t tile_cols, bool left, int terms, int64_t stride, float* sum,
+                int64_t lds) {
+    const bool vec = aligned16(sum) && lds % 4 == 0;
+    for (int t = terms - 1; t >= 0; --t) {
+      mk::ProductParams q = p;
+      if (!sp.counting) (left ? q.A : q.B) += t * stride;
+      if (t < terms - 1) {
+        q.res = sum; q.ldr = lds; q.res_f32 = 1;
+        q.vec = (q.vec & ~mk::kVecRes) | (vec ? mk::kVecRes : 0);
+      }
+      if (t > 0) {
+        q.C = sum; q.ldc = lds; q.c_f32 = 1;
+        q.vec = (q.vec & ~mk::kVecC) | (vec ? mk::kVecC : 0);
+      }
+      if (int rc = run(order, mk::kProdStore, q, tile_cols)) return rc;
+    }
+    return MK_OK;
+  }
+
   // Rows as an operand takes them: 16-byte aligned; `whole`: ending with a unit or zeros (k-contiguous operands).
   // Laid out anew where they are not; groups of `rows` rows each, `stride` apart, in `parts` pieces of columns.
   int rows(const uint16_t*& src, int64_t n, int64_t cols, int64_t& ld, bool whole, int groups = 1, int64_t* stride = nullptr,
@@ -1462,6 +1483,11 @@ struct Products {
   }
 };
 
+// Into how many parts a number between two products goes, for a result of type `type`.
+int between_terms(int32_t between, int32_t type) {
+  return between == MK_BETWEEN_FP32 || (between == MK_BETWEEN_RESULT && type == 0) ? 3 : 1;
+}
+
 bool vec_rows(const void* p, int64_t ld, int type) { return aligned16(p) && ld % (type == 0 ? 4 : 8) == 0; }
 
 const uint16_t* u16(const void* p) { return static_cast<const uint16_t*>(p); }
@@ -1483,6 +1509,7 @@ int check_sizes(const char* fn, int64_t M, int64_t N, int64_t K) {
 }
 
 bool is_type(int t) { return t == 0 || t == 1; }
+bool is_between(int b) { return b >= MK_BETWEEN_RESULT && b <= MK_BETWEEN_FP32; }
 int size_of(int t) { return t == 0 ? 4 : 2; }
 
 struct Matrix {
@@ -1561,6 +1588,7 @@ int check_gemm_act_backward(const char* fn, const mk_gemm_act_backward_args* a) 
   if (int rc = check_sizes(fn, a->M, a->N, a->K)) return rc;
   if (a->act < 0 || a->act > MK_ACT_SILU) return fail(MK_EINVAL, "%s: act must be 0 .. %d", fn, MK_ACT_SILU);
   if (!is_type(a->db_type)) return fail(MK_EINVAL, "%s: db_type must be 0 or 1", fn);
+  if (!is_between(a->between)) return fail(MK_EINVAL, "%s: between must be 0 .. %d", fn, MK_BETWEEN_FP32);
   if (!a->dA && !a->dB && !a->dbias) return fail(MK_EINVAL, "%s: dA, dB or dbias must be set", fn);
   const bool act = a->act != MK_ACT_NONE, da = a->dA, db = a->dB;
   return check_matrices(fn,
@@ -1579,6 +1607,10 @@ int gemm_act_backward_body(const mk_gemm_act_backward_args* a, Products g) {
   const bool act = a->act != MK_ACT_NONE;
   // both products read dpre's rows, one of them along the sum
   const bool copy = (a->dA || a->dB) && (act || !aligned16(d) || ldd % 8 || a->N % 8);
+  // (a slope of 0 or 1 leaves dC's own bits)
+  const bool wider = act && a->act != MK_ACT_RELU;
+  const int terms_a = wider && a->dA ? between_terms(a->between, 1) : 1;
+  const int terms_b = wider && a->dB ? between_terms(a->between, a->db_type) : 1;
   if (copy || a->dbias) {
     mk::ActGradParams p = {};
     p.dC = d; p.ldc = a->lddc; p.vec_c = vec_rows(d, a->lddc, 1);
@@ -1587,7 +1619,8 @@ int gemm_act_backward_body(const mk_gemm_act_backward_args* a, Products g) {
     p.row_blocks = mk::act_grad_blocks(a->M, a->N);
     if (copy) {
       ldd = p.width = (a->N + 7) / 8 * 8;
-      d = p.dpre = static_cast<uint16_t*>(g.sp.take(a->M * p.width * 2));
+      p.terms = std::max(terms_a, terms_b);
+      d = p.dpre = static_cast<uint16_t*>(g.sp.take(p.terms * a->M * p.width * 2));
     }
     if (a->dbias) {
       p.part = static_cast<float*>(g.sp.take(p.row_blocks * a->N * 4));
@@ -1606,7 +1639,10 @@ int gemm_act_backward_body(const mk_gemm_act_backward_args* a, Products g) {
       if (int rc = g.rows(p.B, a->K, a->N, p.ldb, true)) return rc;
     p.C = a->dA; p.ldc = a->ldda;
     p.vec = vec_rows(a->dA, a->ldda, 1) ? mk::kVecC : 0;
-    if (int rc = g.run(mk::kProdLeftGrad, mk::kProdStore, p, a->K)) return rc;
+    const int64_t mark = g.sp.used, lds = (a->K + 3) / 4 * 4;
+    float* sum = terms_a > 1 ? static_cast<float*>(g.sp.take(a->M * lds * 4)) : nullptr;
+    if (int rc = g.run_terms(mk::kProdLeftGrad, p, a->K, true, terms_a, a->M * ldd, sum, lds)) return rc;
+    g.sp.used = mark;
   }
   if (a->dB) {
     mk::ProductParams p = {};
@@ -1620,7 +1656,13 @@ int gemm_act_backward_body(const mk_gemm_act_backward_args* a, Products g) {
     if (a->accumulate) {
       p.res = a->dB; p.ldr = a->lddb; p.res_f32 = p.c_f32;
     }
-    if (int rc = g.run(mk::kProdRightGrad, mk::kProdStore, p, a->N)) return rc;
+    float* sum = static_cast<float*>(a->dB);
+    int64_t lds = a->lddb;
+    if (terms_b > 1 && a->db_type != 0) {
+      lds = (a->N + 3) / 4 * 4;
+      sum = static_cast<float*>(g.sp.take(a->K * lds * 4));
+    }
+    if (int rc = g.run_terms(mk::kProdRightGrad, p, a->N, false, terms_b, a->M * ldd, sum, lds)) return rc;
   }
   return MK_OK;
 }

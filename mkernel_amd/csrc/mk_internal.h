@@ -324,13 +324,14 @@ struct RepackParams {
   float* scale;
 };
 hipError_t launch_repack(const RepackParams& p, hipStream_t stream);
-// dpre = dC * act'(pre), bf16 rows of `width` (null: not kept), and the columns' sums of it
+// dpre = dC * act'(pre), bf16 rows of `width` (null: not kept; in `terms` parts, M * width elements apart, that add up
+// to it), and the columns' sums of it
 struct ActGradParams {
   const uint16_t* dC;
   const uint16_t* pre;
   uint16_t* dpre;
   int64_t M, N, ldc, ldp, width;
-  int act, vec_c, vec_p;
+  int act, vec_c, vec_p, terms;
   float* part;              // [row_blocks][N], null: no sums
   float* dbias;
   int accumulate;

@@ -263,6 +263,13 @@ __device__ __forceinline__ void store8(void* p, int64_t at, bool vec, int n, con
   }
 }
 
+// What bf16's rounding leaves of a number, exactly; nothing of what is infinite or NaN there.  (fp32's 24 bits are a
+// rounded number's 8, those of the rest and those of what is left then.)
+__device__ __forceinline__ float bf16_rest(float x) {
+  const float r = bf16_lo(pack_bf16x2(x, 0.f));
+  return fabsf(r) < INFINITY ? x - r : 0.f;
+}
+
 __device__ __forceinline__ void store4(float* d, bool vec, int n, f32x4 x) {
   if (vec && n == 4) {
     __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(d));

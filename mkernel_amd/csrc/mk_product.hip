@@ -181,7 +181,13 @@ __global__ __launch_bounds__(256) void act_grad_kernel(ActGradParams p) {
         if (i >= nc) d[i] = 0.f;
         s[i] += d[i];
       }
-      if (p.dpre && col < p.width) store8(p.dpre, r * p.width + col, true, 8, d);
+      if (!p.dpre || col >= p.width) continue;
+      store8(p.dpre, r * p.width + col, true, 8, d);
+      for (int t = 1; t < p.terms; ++t) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = bf16_rest(d[i]);
+        store8(p.dpre, (t * p.M + r) * p.width + col, true, 8, d);
+      }
     }
   });
   if (!p.part) return;

@@ -860,6 +860,13 @@ def _act(act: str) -> int:
     return capi.ACTS[act]
 
 
+def _between(dtype, name: str) -> int:
+    """How a number between two products is held (MK_BETWEEN_*)."""
+    if dtype not in (None, *_LOGITS):
+        raise ValueError(f"{name} must be torch.bfloat16, torch.float32 or None")
+    return capi.BETWEEN["result" if dtype is None else "bf16" if dtype is torch.bfloat16 else "fp32"]
+
+
 def _result(out, name: str, dtype, shape, device):
     """out, checked, or a new tensor of that type."""
     if out is None:
@@ -913,19 +920,23 @@ def gemm_act_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor, pre: t
                       act: str = "none", need_dA: bool = True, need_dB: bool = True, need_dbias: bool = True,
                       dA: torch.Tensor | None = None, dB: torch.Tensor | None = None,
                       dbias: torch.Tensor | None = None, dB_dtype: torch.dtype = torch.bfloat16,
-                      accumulate: bool = False) -> tuple:
+                      accumulate: bool = False, dpre_dtype: torch.dtype | None = None) -> tuple:
     """Gradients of gemm_act (mk_gemm_act_backward): (dA bf16, dB bfloat16 or
     float32, dbias float32), None for what is not needed; the residual's is dC
     itself (bf16 [M, N]).  pre: what the forward call kept, needed with an
-    activation.  dpre = dC * act'(pre) is rounded to bf16 for dA and dB (not for
-    dbias), without an activation it is dC.  accumulate: dB and dbias, which are
-    then given, are added to."""
+    activation.  dpre_dtype: how dpre = dC * act'(pre) goes into the products of dA
+    and dB; in bfloat16, one product each, they are off by up to 2^-8 of each
+    element of it, in float32 by nothing, which takes three products each.  None:
+    float32 for a float32 dB, else bfloat16.  (dbias takes dpre as it is; without an
+    activation it is dC, with relu bfloat16 holds it.)  accumulate: dB and dbias,
+    which are then given, are added to."""
     M, N = _matrix(dC, "dC")
     dev = dC.device
     K = _matrix(A, "A")[1]
     if A.shape[0] != M or A.device != dev or _matrix(B, "B") != (K, N) or B.device != dev:
         raise ValueError(f"A must be [{M}, K] and B [K, {N}] on {dev}")
     code = _act(act)
+    between = _between(dpre_dtype, "dpre_dtype")
     if code:
         if pre is None:
             raise ValueError("pre is needed with an activation")
@@ -937,7 +948,7 @@ def gemm_act_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor, pre: t
     if dev.index != _device_index():
         with torch.cuda.device(dev):
             return gemm_act_backward(dC, A, B, pre, act, need_dA, need_dB, need_dbias, dA, dB, dbias, dB_dtype,
-                                     accumulate)
+                                     accumulate, dpre_dtype)
     if need_dA and dA is not None:
         _rows(dA, "dA", _BF16, (M, K), dev)
     dA = _result(dA, "dA", torch.bfloat16, (M, K), dev) if need_dA else None
@@ -951,7 +962,7 @@ def gemm_act_backward(dC: torch.Tensor, A: torch.Tensor, B: torch.Tensor, pre: t
     _product("mk_gemm_act_backward", GemmActBackwardArgs, dev, True, dC.data_ptr(), A.data_ptr(), B.data_ptr(),
              _ptr(pre) if code else 0, _ptr(dA), _ptr(dB), _ptr(dbias), M, N, K, _ld(dC), _ld(A), _ld(B),
              _ld(pre) if code else 0, 0 if dA is None else _ld(dA), 0 if dB is None else _ld(dB), code, _code(dB),
-             bool(accumulate))
+             bool(accumulate), between)
     return dA, dB, dbias
 
 
