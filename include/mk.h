@@ -871,9 +871,12 @@ int mk_vocab_loss(const mk_vocab_loss_args* args, void* stream);
  * shards), 0 for ignored tokens,
  *   dx = dl @ W^T (of a shard: its part of the sum),  dW = x^T @ dl.
  * Logits are computed anew, a piece of the vocabulary at a time (piece_columns, a
- * multiple of 256; 0: the library's choice), dl goes through the workspace in
- * bf16 (without the significand of the largest dloss, which the fp32 sums take
- * back: of a mean's equal dloss no common rounding stays).  Either result may be NULL; accumulate: dW is added to. */
+ * multiple of 256; 0: the library's choice); dl goes through the workspace as
+ * `between` says.  In bf16 each of its elements is off by up to 2^-8 of itself
+ * (without the significand of the largest dloss, which the fp32 sums take back: of
+ * a mean's equal dloss no common rounding stays; of several distinct ones, the
+ * labels' elements of the others keep one each).  Either result may be NULL;
+ * accumulate: dW is added to. */
 typedef struct mk_vocab_loss_backward_args {
   const void* x;          /* bf16 [T, ldx] */
   const void* W;          /* bf16 [H, ldw] */
@@ -887,7 +890,7 @@ typedef struct mk_vocab_loss_backward_args {
   int64_t vocab_begin, ignore_index;
   int64_t piece_columns;
   int32_t labels_type, dx_type, dw_type; /* types 0 fp32, 1 bf16 */
-  int32_t accumulate;
+  int16_t accumulate, between; /* MK_BETWEEN_* */
   void* workspace;
   int64_t workspace_bytes;
   void* tickets;

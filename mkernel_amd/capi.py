@@ -256,7 +256,7 @@ class VocabLossBackwardArgs(C.Structure):
     _fields_ = [("x", vp), ("W", vp), ("labels", vp), ("lse", vp), ("dloss", vp), ("dx", vp), ("dW", vp), ("T", i64),
                 ("H", i64), ("V", i64), ("ldx", i64), ("ldw", i64), ("lddx", i64), ("lddw", i64),
                 ("vocab_begin", i64), ("ignore_index", i64), ("piece_columns", i64), ("labels_type", i32),
-                ("dx_type", i32), ("dw_type", i32), ("accumulate", i32), ("workspace", vp),
+                ("dx_type", i32), ("dw_type", i32), ("accumulate", i16), ("between", i16), ("workspace", vp),
                 ("workspace_bytes", i64), ("tickets", vp)]
 
 

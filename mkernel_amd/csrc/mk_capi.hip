@@ -1845,6 +1845,7 @@ int check_vocab_backward(const char* fn, const mk_vocab_loss_backward_args* a) {
   if (!a) return fail(MK_EINVAL, "%s: null argument", fn);
   if (int rc = check_vocab(fn, a->T, a->H, a->V, a->vocab_begin, a->labels_type, a->labels, a->lse)) return rc;
   if (!is_type(a->dx_type) || !is_type(a->dw_type)) return fail(MK_EINVAL, "%s: types must be 0 or 1", fn);
+  if (!is_between(a->between)) return fail(MK_EINVAL, "%s: between must be 0 .. %d", fn, MK_BETWEEN_FP32);
   if (a->piece_columns < 0 || a->piece_columns % 256) return fail(MK_EINVAL, "%s: piece_columns must be a multiple of 256", fn);
   if (a->T > 0 && !a->dloss) return fail(MK_EINVAL, "%s: dloss is null", fn);
   if (!a->dx && !a->dW) return fail(MK_EINVAL, "%s: dx or dW must be set", fn);
@@ -1876,10 +1877,13 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
   r.dloss = a->dloss;
   uint16_t* x = r.dst = static_cast<uint16_t*>(g.sp.take(T * ldx * 2));
   float* scale = r.scale = static_cast<float*>(g.sp.take(4));
-  uint16_t* dl = static_cast<uint16_t*>(g.sp.take(T * piece * 2));
-  float* sum = nullptr;  // of dx over the pieces
+  const int terms_x = a->dx ? between_terms(a->between, a->dx_type) : 1;
+  const int terms_w = a->dW ? between_terms(a->between, a->dw_type) : 1, terms = std::max(terms_x, terms_w);
+  uint16_t* dl = static_cast<uint16_t*>(g.sp.take(terms * T * piece * 2));
+  float* sum_w = a->dW && terms_w > 1 && a->dw_type != 0 ? static_cast<float*>(g.sp.take(H * piece * 4)) : nullptr;
+  float* sum = nullptr;  // of dx over the pieces and dl's parts
   int64_t lds = H;
-  if (a->dx && V > piece) {
+  if (a->dx && (V > piece || terms_x > 1)) {
     if (a->dx_type == 0) {
       sum = static_cast<float*>(a->dx);
       lds = a->lddx;
@@ -1903,8 +1907,8 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
     fill_vocab(p, a->labels, a->labels_type, a->ignore_index, a->vocab_begin, V);
     p.first_col = c0;
     p.lse = a->lse; p.dloss = a->dloss; p.scale = scale;
-    p.C = dl; p.ldc = piece;
-    if (int rc = g.run(mk::kProdForward, mk::kProdDlogits, p, n)) return rc;
+    p.C = dl; p.ldc = piece; p.c_stride = T * piece;
+    if (int rc = g.run(mk::kProdForward, terms > 1 ? mk::kProdDlogits3 : mk::kProdDlogits, p, n)) return rc;
     if (a->dx) {
       const bool last = c0 + n == V;
       mk::ProductParams q = {};
@@ -1920,7 +1924,7 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
       q.ldc = last ? a->lddx : lds;
       q.c_f32 = !last || a->dx_type == 0;
       if (vec_rows(q.C, q.ldc, q.c_f32 ? 0 : 1)) q.vec |= mk::kVecC;
-      if (int rc = g.run(mk::kProdLeftGrad, mk::kProdStore, q, H)) return rc;
+      if (int rc = g.run_terms(mk::kProdLeftGrad, q, H, true, terms_x, T * piece, sum, lds)) return rc;
     }
     if (a->dW) {
       mk::ProductParams q = {};
@@ -1934,7 +1938,8 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
       if (a->accumulate) {
         q.res = q.C; q.ldr = q.ldc; q.res_f32 = q.c_f32;
       }
-      if (int rc = g.run(mk::kProdRightGrad, mk::kProdStore, q, n)) return rc;
+      float* to = sum_w || g.sp.counting ? sum_w : static_cast<float*>(q.C);
+      if (int rc = g.run_terms(mk::kProdRightGrad, q, n, false, terms_w, T * piece, to, a->dw_type ? piece : a->lddw)) return rc;
     }
     g.sp.used = mark;
   }

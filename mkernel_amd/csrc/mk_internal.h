@@ -259,7 +259,8 @@ hipError_t launch_w4_quantize(const uint16_t* W, int64_t K, int64_t N, int64_t E
 
 // Products with what follows them (mk_product.h, mk_product.hip).
 enum ProductEpilogue : int { kProdStore = 0, kProdSwiglu = 1, kProdSwigluGrad = 2, kProdStats = 3, kProdDlogits = 4,
-                             kProdPlain = 5, kProdPlain32 = 6 };  // kProdStore without anything but bf16 or fp32 results
+                             kProdPlain = 5, kProdPlain32 = 6,  // kProdStore without anything but bf16 or fp32 results
+                             kProdDlogits3 = 7 };  // three parts of the logits' gradient
 enum ProductOrder : int { kProdForward = 0, kProdLeftGrad = 1, kProdRightGrad = 2 };
 enum ProductAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
 // which rows of the epilogue start at 16-byte boundaries
@@ -273,7 +274,7 @@ struct ProductParams {
   // groups
   const int* counts;
   int E, ragged;            // 0 none, 1 rows of A and C, 2 rows of A and B
-  int64_t b_stride, c_stride;  // elements between groups' B (ragged 1) and C (ragged 2)
+  int64_t b_stride, c_stride;  // elements between groups' B (ragged 1) and C (ragged 2), or the parts of a gradient
   // tiles
   int tiles_m, tiles_n, group_m;
   int whole, split;         // tiles from `whole` on are cut into `split` parts along K

@@ -460,7 +460,7 @@ struct TileSpot {
 
 template <class C, bool AKC, bool BKC, int EPI>
 __device__ __forceinline__ void product_tile(const ProductParams& p, const TileSpot& at, char* smem) {
-  constexpr bool kSwiglu = EPI == kProdSwiglu;
+  constexpr bool kSwiglu = EPI == kProdSwiglu, kDlogits = EPI == kProdDlogits || EPI == kProdDlogits3;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / C::WN, wn = wave % C::WN;
@@ -497,12 +497,12 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
   // vocabulary: a thread has one row's label (as a column of the tile; -1 elsewhere, -2 no loss) and numbers, loaded
   // before the products and kept in LDS for the epilogue (loaded there, one latency per eight rows, they took 12 us)
   TokenRow token = {-1, 0.f, 0.f, 0};
-  if constexpr (EPI == kProdStats || EPI == kProdDlogits) {
+  if constexpr (EPI == kProdStats || kDlogits) {
     static_assert(C::NT >= C::BM, "a row per thread");
     if (tid < C::BM && m0 + tid < M) {
       const int64_t label = label_of(p, m0 + tid), c = label - p.first_col - n0;
       token.label = label < 0 ? (int)label : c >= 0 && c < C::BN ? (int)c : -1;
-      if constexpr (EPI == kProdDlogits) {
+      if constexpr (kDlogits) {
         token.lse = p.lse[m0 + tid];
         // bf16 rounds this token's gradients of the logits; where every token has the same dloss (a mean's 1 / T), those
         // of the labels, about -dloss, would all be off by the same, up to 2^-8 of it: without its significand they are
@@ -818,7 +818,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
   const int nc = (int)min<int64_t>(max<int64_t>(p.N - col, 0), 8);
   TokenRow* tokens = reinterpret_cast<TokenRow*>(smem + C::EPI_BYTES);
   float2* wave_stats = reinterpret_cast<float2*>(tokens + C::BM);
-  if constexpr (EPI == kProdStats || EPI == kProdDlogits) {
+  if constexpr (EPI == kProdStats || kDlogits) {
     if (tid < C::BM) tokens[tid] = token;
     __syncthreads();
   }
@@ -998,7 +998,8 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
             for (int v = 1; v < 8; ++v) z = v == at ? x[v] : z;
             p.target[m] = z;
           }
-        } else {  // kProdDlogits
+        } else {  // kDlogits
+          static_assert(kDlogits, "epilogue");
           if (m >= M) continue;
           const TokenRow t = tokens[wm * C::WTM + i * 32 + r * RPI + rr];
           const int at = t.label - (wn * C::WTN + cc * 8);
@@ -1010,7 +1011,17 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
             x[v] = t.label == -2 || v >= nc ? 0.f : d * t.dloss;
           }
           // the scratch rows are whole units: columns behind the last are zeros, as the products behind read them
-          if (col < p.ldc) store8(p.C, m * p.ldc + col, true, 8, x);
+          if (col < p.ldc) {
+            store8(p.C, m * p.ldc + col, true, 8, x);
+            if constexpr (EPI == kProdDlogits3) {
+#pragma unroll
+              for (int t = 1; t < 3; ++t) {
+#pragma unroll
+                for (int v = 0; v < 8; ++v) x[v] = bf16_rest(x[v]);
+                store8(p.C, t * p.c_stride + m * p.ldc + col, true, 8, x);
+              }
+            }
+          }
         }
       }
     }
@@ -1116,7 +1127,7 @@ hipError_t launch_product_tile(const ProductParams& p, int tile, int64_t grid, h
     case kProd128: return launch_product_cfg<ProdTile128, void, AKC, BKC, EPI>(p, grid, stream);
     case kProd256:
       // only the epilogues of expert products see small groups
-      if constexpr (EPI != kProdStats && EPI != kProdDlogits) return launch_product_cfg<ProdTile256, ProdFlat256<BKC>, AKC, BKC, EPI>(p, grid, stream);
+      if constexpr (EPI != kProdStats && EPI != kProdDlogits && EPI != kProdDlogits3) return launch_product_cfg<ProdTile256, ProdFlat256<BKC>, AKC, BKC, EPI>(p, grid, stream);
       else return launch_product_cfg<ProdTile256, void, AKC, BKC, EPI>(p, grid, stream);
   }
   return hipErrorInvalidValue;

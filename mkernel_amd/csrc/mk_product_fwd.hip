@@ -11,6 +11,7 @@ hipError_t launch_product_forward(const ProductParams& p, int epi, int tile, int
     case kProdSwiglu: return launch_product_tile<true, false, kProdSwiglu>(p, tile, grid, stream);
     case kProdStats: return launch_product_tile<true, false, kProdStats>(p, tile, grid, stream);
     case kProdDlogits: return launch_product_tile<true, false, kProdDlogits>(p, tile, grid, stream);
+    case kProdDlogits3: return launch_product_tile<true, false, kProdDlogits3>(p, tile, grid, stream);
   }
   return hipErrorInvalidValue;
 }

@@ -1101,21 +1101,26 @@ def vocab_loss_backward(x: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, 
                         dloss: torch.Tensor, vocab_begin: int = 0, ignore_index: int = -100, need_dx: bool = True,
                         need_dW: bool = True, dx: torch.Tensor | None = None, dW: torch.Tensor | None = None,
                         dx_dtype: torch.dtype = torch.bfloat16, dW_dtype: torch.dtype = torch.bfloat16,
-                        accumulate: bool = False, piece_columns: int = 0) -> tuple:
+                        accumulate: bool = False, piece_columns: int = 0,
+                        dl_dtype: torch.dtype | None = None) -> tuple:
     """Gradients of vocab_loss's loss (mk_vocab_loss_backward): (dx [T, H], dW
     [H, V]), bfloat16 or float32, None for what is not needed, from dloss
     (float32 [T]) and lse (of a shard: the joined one).  The logits are computed
     anew, a piece of the vocabulary at a time (piece_columns, a multiple of 256;
-    0: as many as keep the piece's gradient of the logits below 128 MB); that
-    gradient is rounded to bf16 between the products (dloss without the
-    significand of its largest, which the sums take back, so that a mean's equal
-    dloss leaves no common rounding).  A shard's dx is its part
-    of a sum over the ranks (dx_dtype=torch.float32 for that).  accumulate: dW,
-    which is then given, is added to."""
+    0: as many as keep the piece's gradient of the logits below 128 MB).  dl_dtype:
+    how that gradient goes into the products of dx and dW.  In bfloat16, one
+    product each, each element is off by up to 2^-8 of itself (without the
+    significand of the largest dloss, which the sums take back, so that a mean's
+    equal dloss leaves no common rounding; of several distinct dloss the others
+    keep one each, at their labels); in float32 by nothing, which takes three
+    products each.  None: float32 for a float32 result, bfloat16 for a bfloat16
+    one.  A shard's dx is its part of a sum over the ranks (dx_dtype=torch.float32
+    for that).  accumulate: dW, which is then given, is added to."""
     T, H, V, dev, wide = _vocab(x, W, labels)
     for t, name in ((lse, "lse"), (dloss, "dloss")):
         if not _is(t, torch.float32, (T,), dev):
             _tensor(t, name, _F32, (T,), device=dev)
+    between = _between(dl_dtype, "dl_dtype")
     if not (need_dx or need_dW):
         return None, None
     if accumulate and need_dW and dW is None:
@@ -1123,13 +1128,13 @@ def vocab_loss_backward(x: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, 
     if dev.index != _device_index():
         with torch.cuda.device(dev):
             return vocab_loss_backward(x, W, labels, lse, dloss, vocab_begin, ignore_index, need_dx, need_dW, dx, dW,
-                                       dx_dtype, dW_dtype, accumulate, piece_columns)
+                                       dx_dtype, dW_dtype, accumulate, piece_columns, dl_dtype)
     dx = _result(dx, "dx", dx_dtype, (T, H), dev) if need_dx else None
     dW = _result(dW, "dW", dW_dtype, (H, V), dev) if need_dW else None
     _product("mk_vocab_loss_backward", VocabLossBackwardArgs, dev, True, x.data_ptr(), W.data_ptr(), labels.data_ptr(),
              lse.data_ptr(), dloss.data_ptr(), _ptr(dx), _ptr(dW), T, H, V, _ld(x), _ld(W),
              0 if dx is None else _ld(dx), 0 if dW is None else _ld(dW), vocab_begin, ignore_index, piece_columns,
-             wide, _code(dx), _code(dW), bool(accumulate))
+             wide, _code(dx), _code(dW), bool(accumulate), between)
     return dx, dW
 
 

@@ -7,7 +7,7 @@ from mkernel_amd import capi
 from test_product_host import EINVAL, _args
 
 
-@pytest.mark.parametrize("name", ["mk_gemm_act_backward"])
+@pytest.mark.parametrize("name", ["mk_gemm_act_backward", "mk_vocab_loss_backward"])
 @pytest.mark.parametrize("between", [-1, 3, 99])
 def test_refusals(name, between):
     L, a = capi.lib(), _args(name, dict(between=between))
