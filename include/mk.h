@@ -715,7 +715,8 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* args, void* stream);
  * nothing between calls (the pointers in args have to be set for the question,
  * the workspace's own need not).  `tickets`: MK_PRODUCT_TICKETS 32-bit words,
  * zero before their first use, left zero by every call; launches that share
- * them must be ordered. */
+ * them must be ordered.  mk_*_ticket_words(args) is how many of them the call
+ * touches: 0 where no sum is cut (any address but NULL will do then). */
 #define MK_PRODUCT_TICKETS 8192
 
 /* What lies between two products of a backward pass (dpre, dl) is held in bf16,
@@ -750,6 +751,7 @@ typedef struct mk_gemm_act_args {
   void* tickets;
 } mk_gemm_act_args;
 int64_t mk_gemm_act_workspace_bytes(const mk_gemm_act_args* args);
+int64_t mk_gemm_act_ticket_words(const mk_gemm_act_args* args);
 int mk_gemm_act(const mk_gemm_act_args* args, void* stream);
 
 /* Gradients of mk_gemm_act (the residual's is dC itself): with
@@ -780,6 +782,7 @@ typedef struct mk_gemm_act_backward_args {
   void* tickets;
 } mk_gemm_act_backward_args;
 int64_t mk_gemm_act_backward_workspace_bytes(const mk_gemm_act_backward_args* args);
+int64_t mk_gemm_act_backward_ticket_words(const mk_gemm_act_backward_args* args);
 int mk_gemm_act_backward(const mk_gemm_act_backward_args* args, void* stream);
 
 /* Expert products on ragged rows: the rows of expert e are the counts[e] rows
@@ -865,6 +868,7 @@ typedef struct mk_vocab_loss_args {
   void* tickets;
 } mk_vocab_loss_args;
 int64_t mk_vocab_loss_workspace_bytes(const mk_vocab_loss_args* args);
+int64_t mk_vocab_loss_ticket_words(const mk_vocab_loss_args* args);
 int mk_vocab_loss(const mk_vocab_loss_args* args, void* stream);
 
 /* Gradients: with dl = (e^(logit - lse) - [v = label]) * dloss (lse over all
@@ -896,6 +900,7 @@ typedef struct mk_vocab_loss_backward_args {
   void* tickets;
 } mk_vocab_loss_backward_args;
 int64_t mk_vocab_loss_backward_workspace_bytes(const mk_vocab_loss_backward_args* args);
+int64_t mk_vocab_loss_backward_ticket_words(const mk_vocab_loss_backward_args* args);
 int mk_vocab_loss_backward(const mk_vocab_loss_backward_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */

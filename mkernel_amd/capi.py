@@ -45,8 +45,10 @@ EXPORTS = (
     "mk_moe_grouped_gemm_w4",
     "mk_moe_ffn_combine_w4",
     "mk_gemm_act_workspace_bytes",
+    "mk_gemm_act_ticket_words",
     "mk_gemm_act",
     "mk_gemm_act_backward_workspace_bytes",
+    "mk_gemm_act_backward_ticket_words",
     "mk_gemm_act_backward",
     "mk_moe_ragged_gemm_workspace_bytes",
     "mk_moe_ragged_gemm",
@@ -55,8 +57,10 @@ EXPORTS = (
     "mk_moe_ragged_wgrad_workspace_bytes",
     "mk_moe_ragged_wgrad",
     "mk_vocab_loss_workspace_bytes",
+    "mk_vocab_loss_ticket_words",
     "mk_vocab_loss",
     "mk_vocab_loss_backward_workspace_bytes",
+    "mk_vocab_loss_backward_ticket_words",
     "mk_vocab_loss_backward",
     "mk_query_workspace_bytes",
     "mk_probe_mfma_ceiling",
@@ -70,6 +74,8 @@ EXPORTS = (
 # entry points with a workspace of mk_..._workspace_bytes(args) bytes
 _PRODUCTS = ("mk_gemm_act", "mk_gemm_act_backward", "mk_moe_ragged_gemm", "mk_moe_ragged_dgrad", "mk_moe_ragged_wgrad",
              "mk_vocab_loss", "mk_vocab_loss_backward")
+# ... and of those the ones that take tickets, mk_..._ticket_words(args) of them
+_CUT_PRODUCTS = ("mk_gemm_act", "mk_gemm_act_backward", "mk_vocab_loss", "mk_vocab_loss_backward")
 PRODUCT_TICKETS = 8192  # include/mk.h MK_PRODUCT_TICKETS
 BETWEEN = {"result": 0, "bf16": 1, "fp32": 2}  # MK_BETWEEN_*
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # MK_ACT_*
@@ -287,6 +293,9 @@ def lib() -> C.CDLL:
         for name in _PRODUCTS:
             getattr(L, name + "_workspace_bytes").argtypes = [vp]
             getattr(L, name + "_workspace_bytes").restype = i64
+        for name in _CUT_PRODUCTS:
+            getattr(L, name + "_ticket_words").argtypes = [vp]
+            getattr(L, name + "_ticket_words").restype = i64
         L.mk_moe_index_sizes.argtypes = [vp, i32, i32, i32, i32, i32, C.POINTER(i64), C.POINTER(i64)]
         L.mk_moe_index_sizes.restype = C.c_int
         L.mk_moe_build_indices.argtypes = [vp, vp, i32, i32, i32, i32, i32, C.POINTER(MoeIndex)]
@@ -402,7 +411,16 @@ def call_with_workspace(fn: str, cls, stream: int, *values) -> bool:
 def workspace_bytes(fn: str, cls, *values) -> int:
     """What fn's workspace has to hold for these arguments (without the
     workspace's own, which come last)."""
-    key = fn + "_workspace_bytes"
+    return _ask(fn, "_workspace_bytes", cls, values)
+
+
+def ticket_words(fn: str, cls, *values) -> int:
+    """How many tickets fn touches for these arguments."""
+    return _ask(fn, "_ticket_words", cls, values)
+
+
+def _ask(fn, what, cls, values) -> int:
+    key = fn + what
     f = _functions.get(key)
     if f is None:
         f = _functions[key] = getattr(lib(), key)

@@ -1361,6 +1361,7 @@ constexpr int64_t kMaxLd = 1 << 21, kMaxRows = 1 << 25;
 struct Space {
   char* base = nullptr;
   bool counting = true;
+  bool cut = false;  // a launch has parts, which take tickets
   int64_t used = 0, peak = 0;
   void* take(int64_t bytes) {
     const int64_t at = used;
@@ -1369,13 +1370,6 @@ struct Space {
     return counting ? nullptr : base + at;
   }
 };
-
-template <class F>
-int64_t count_space(F body) {
-  Space sp;
-  const int rc = body(sp);
-  return rc ? -1 : sp.peak;
-}
 
 template <class F>
 int with_space(const char* fn, void* ws, int64_t bytes, F body) {
@@ -1426,6 +1420,7 @@ struct Products {
     if (p.ragged == 2) grid = 8 * ((tm * tn + 7) / 8) * groups;
     if (grid >= (1LL << 32) / 512) return fail(MK_ESHAPE, "%s: too many tiles", fn);  // of 512 threads or fewer
     const int64_t mark = sp.used;
+    if (p.split > 1) sp.cut = true;
     if (p.split > 1) p.parts = static_cast<float*>(sp.take((plan.tiles - plan.whole) * p.split * s.bm * s.bn * 4));
     sp.used = mark;  // the next launch may use them again
     if (sp.counting) return MK_OK;
@@ -1948,14 +1943,26 @@ int vocab_loss_backward_body(const mk_vocab_loss_backward_args* a, Products g) {
 
 uint32_t* tickets_of(void* t) { return static_cast<uint32_t*>(t); }
 
-// The two entry points of an operator: `check`, then `body` to count or to work.
+// The entry points of an operator: `check`, then `body` to count or to work.
+template <class A, class Check, class Body>
+bool count_product(const char* fn, const A* a, Check check, Body body, bool cut, Space& sp) {
+  if (check(fn, a)) return false;
+  DevInfo d;
+  if (device_info(&d)) return false;
+  static uint32_t any[1];
+  return body(a, Products{fn, sp, d.cus, cut ? any : nullptr, nullptr}) == MK_OK;
+}
+
 template <class A, class Check, class Body>
 int64_t product_bytes(const char* fn, const A* a, Check check, Body body, bool cut) {
-  if (check(fn, a)) return -1;
-  DevInfo d;
-  if (device_info(&d)) return -1;
-  static uint32_t any[1];
-  return count_space([&](Space& sp) { return body(a, Products{fn, sp, d.cus, cut ? any : nullptr, nullptr}); });
+  Space sp;
+  return count_product(fn, a, check, body, cut, sp) ? sp.peak : -1;
+}
+
+template <class A, class Check, class Body>
+int64_t product_tickets(const char* fn, const A* a, Check check, Body body) {
+  Space sp;
+  return count_product(fn, a, check, body, true, sp) ? (sp.cut ? MK_PRODUCT_TICKETS : 0) : -1;
 }
 
 template <class A, class Check, class Body>
@@ -1979,12 +1986,18 @@ extern "C" {
 int64_t mk_gemm_act_workspace_bytes(const mk_gemm_act_args* a) {
   return product_bytes("mk_gemm_act_workspace_bytes", a, check_gemm_act, gemm_act_body, true);
 }
+int64_t mk_gemm_act_ticket_words(const mk_gemm_act_args* a) {
+  return product_tickets("mk_gemm_act_ticket_words", a, check_gemm_act, gemm_act_body);
+}
 int mk_gemm_act(const mk_gemm_act_args* a, void* stream) {
   return product_call("mk_gemm_act", a, check_gemm_act, gemm_act_body, a ? a->tickets : nullptr, true, stream);
 }
 
 int64_t mk_gemm_act_backward_workspace_bytes(const mk_gemm_act_backward_args* a) {
   return product_bytes("mk_gemm_act_backward_workspace_bytes", a, check_gemm_act_backward, gemm_act_backward_body, true);
+}
+int64_t mk_gemm_act_backward_ticket_words(const mk_gemm_act_backward_args* a) {
+  return product_tickets("mk_gemm_act_backward_ticket_words", a, check_gemm_act_backward, gemm_act_backward_body);
 }
 int mk_gemm_act_backward(const mk_gemm_act_backward_args* a, void* stream) {
   return product_call("mk_gemm_act_backward", a, check_gemm_act_backward, gemm_act_backward_body,
@@ -2015,12 +2028,18 @@ int mk_moe_ragged_wgrad(const mk_moe_ragged_wgrad_args* a, void* stream) {
 int64_t mk_vocab_loss_workspace_bytes(const mk_vocab_loss_args* a) {
   return product_bytes("mk_vocab_loss_workspace_bytes", a, check_vocab_loss, vocab_loss_body, true);
 }
+int64_t mk_vocab_loss_ticket_words(const mk_vocab_loss_args* a) {
+  return product_tickets("mk_vocab_loss_ticket_words", a, check_vocab_loss, vocab_loss_body);
+}
 int mk_vocab_loss(const mk_vocab_loss_args* a, void* stream) {
   return product_call("mk_vocab_loss", a, check_vocab_loss, vocab_loss_body, a ? a->tickets : nullptr, true, stream);
 }
 
 int64_t mk_vocab_loss_backward_workspace_bytes(const mk_vocab_loss_backward_args* a) {
   return product_bytes("mk_vocab_loss_backward_workspace_bytes", a, check_vocab_backward, vocab_loss_backward_body, true);
+}
+int64_t mk_vocab_loss_backward_ticket_words(const mk_vocab_loss_backward_args* a) {
+  return product_tickets("mk_vocab_loss_backward_ticket_words", a, check_vocab_backward, vocab_loss_backward_body);
 }
 int mk_vocab_loss_backward(const mk_vocab_loss_backward_args* a, void* stream) {
   return product_call("mk_vocab_loss_backward", a, check_vocab_backward, vocab_loss_backward_body,

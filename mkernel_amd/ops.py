@@ -798,6 +798,7 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
 # workspace: one set per thread, device and stream, whose launches are ordered (the launches of two threads' calls on
 # one stream may come between each other).
 _SPACE = 4 << 20
+_UNTOUCHED = 16  # in place of tickets that a call does not touch
 
 
 class _Spaces(threading.local):
@@ -823,13 +824,15 @@ def _product(fn: str, cls, device, cut: bool, *values) -> None:
     cut, tickets): the stream's small one where that is enough, else memory of
     its own, which the caching allocator reuses in stream order.  Inside a
     graph's capture both are the graph's (torch keeps what it allocates there
-    for it), the tickets' zeros recorded with it: graphs may then run beside
-    each other and beside eager calls."""
+    for it), the tickets' zeros recorded with it where the call touches them:
+    graphs may then run beside each other and beside eager calls."""
     index = device.index
     stream = _raw_stream(index)
     if _capturing():
-        at = torch.zeros(capi.PRODUCT_TICKETS, dtype=torch.int32, device=device) if cut else None
-        tickets = (at.data_ptr(),) if cut else ()
+        # (tickets that are not touched: any address)
+        words = capi.ticket_words(fn, cls, *values) if cut else 0
+        at = torch.zeros(words, dtype=torch.int32, device=device) if words else None
+        tickets = (at.data_ptr() if words else _UNTOUCHED,) if cut else ()
     else:
         at = _space(index, stream)
         tickets = (at,) if cut else ()

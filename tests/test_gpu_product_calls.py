@@ -1,9 +1,10 @@
 """How the products' entry points keep what lies between their launches: the
 small workspaces of threads and streams, and what a graph's capture records."""
+import ctypes
 import threading
 
-import torch
 import pytest
+import torch
 
 from mkernel_amd import capi, ops
 from test_gpu_product_large import randn
@@ -43,3 +44,40 @@ def test_two_threads_share_no_small_workspace():
     for g, w in zip(got, want):
         assert len(g) == 300 and all(torch.equal(x, w) for x in g)
     assert len({*at, ops._space(A.device.index, torch.cuda.current_stream().cuda_stream)}) == 3
+
+
+def _nodes(call):
+    """Nodes of a captured call, and the graph with its results."""
+    hip = ctypes.CDLL("libamdhip64.so")
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        out = call()
+    n = ctypes.c_size_t(0)
+    assert hip.hipGraphGetNodes(ctypes.c_void_p(g.raw_cuda_graph()), None, ctypes.byref(n)) == 0
+    g.instantiate()
+    return n.value, g, out
+
+
+def test_captured_calls_record_no_tickets_they_do_not_touch():
+    """A product whose K is not cut is one node, with a fill of the tickets in front of it where it is."""
+    one = randn(1, 2048, seed=5), randn(2048, 2048, seed=6), randn(2048, seed=7)
+    some = randn(256, 96, seed=8), randn(96, 512, seed=9)
+    cut = randn(20, 4096, seed=10), randn(4096, 600, seed=11)
+    x, V = randn(200, 64, seed=12), randn(64, 520, seed=13)
+    labels = torch.arange(200, device="cuda")
+    dloss = torch.full((200,), 0.005, device="cuda")
+    lse = ops.vocab_loss(x, V, labels)["lse"]
+    calls = [(1, lambda: [ops.gemm_act(one[0], one[1], bias=one[2], act="silu")]), (1, lambda: [ops.gemm_act(*some)]),
+             (2, lambda: [ops.gemm_act(*cut)]),
+             (2, lambda: list(ops.vocab_loss(x, V, labels).values())),  # statistics, their join
+             (4, lambda: list(ops.vocab_loss_backward(x, V, labels, lse, dloss)))]  # rows of x, dl, dx, dW
+    for want, call in calls:
+        eager = call()
+        n, g, out = _nodes(call)
+        assert n == want, (want, n)
+        for _ in range(4):
+            for t in out:
+                t.fill_(float("nan"))
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, eager))
