@@ -1393,17 +1393,21 @@ struct Products {
 
   int launched(hipError_t e) const { return e == hipSuccess ? MK_OK : hip_fail(e, fn); }
 
-  // One product; b_cols: columns of B that its tiles cover (SwiGLU: gate and up).
-  int run(int order, int epi, mk::ProductParams p, int64_t tile_cols, int* tile = nullptr) {
+  // tile_cols: columns of B that a product's tiles cover (SwiGLU: gate and up).
+  mk::ProductPlan plan_of(int order, int epi, const mk::ProductParams& p, int64_t tile_cols) const {
+    return mk::plan_product(p.M, tile_cols, p.K, p.ragged ? p.E : 1, p.ragged, order == mk::kProdRightGrad,
+                            epi != mk::kProdStore, tickets != nullptr, cus);
+  }
+
+  // One product.
+  int run(int order, int epi, mk::ProductParams p, int64_t tile_cols) {
     if (p.M == 0 || p.N == 0) return MK_OK;
     const int groups = p.ragged ? p.E : 1;
     if (epi == mk::kProdStore && !p.bias && !p.act && !p.pre && !p.res) {
       if (!p.c_f32) epi = mk::kProdPlain;
       else if (order == mk::kProdRightGrad) epi = mk::kProdPlain32;
     }
-    const mk::ProductPlan plan = mk::plan_product(p.M, tile_cols, p.K, groups, p.ragged, order == mk::kProdRightGrad,
-                                                  epi != mk::kProdStore, tickets != nullptr, cus);
-    if (tile) *tile = plan.tile;
+    const mk::ProductPlan plan = plan_of(order, epi, p, tile_cols);
     const mk::ProductShape& s = mk::kProductShapes[plan.tile];
     p.split = plan.split;
     p.group_m = 8;
@@ -1813,21 +1817,24 @@ int vocab_loss_body(const mk_vocab_loss_args* a, Products g) {
   // weights that have to be laid out anew go piece by piece
   const bool direct = aligned16(a->W) && a->ldw % 8 == 0;
   const int64_t piece = direct ? a->V : piece_of(a->H, a->V);
-  const int64_t most_groups = (a->V + 63) / 64 + (a->V + piece - 1) / piece;  // no tile is narrower
-  float2* stats = static_cast<float2*>(g.sp.take(most_groups * a->T * 8));
-  int64_t groups = 0;
-  for (int64_t c0 = 0; c0 < a->V; c0 += piece) {
-    const int64_t mark = g.sp.used;
+  auto groups_of = [&](int64_t c0) {  // column tiles of the piece
     p.N = p.b_cols = std::min(piece, a->V - c0);
+    const int bn = mk::kProductShapes[g.plan_of(mk::kProdForward, mk::kProdStats, p, p.N).tile].bn;
+    return (p.N + bn - 1) / bn;
+  };
+  int64_t groups = 0;
+  for (int64_t c0 = 0; c0 < a->V; c0 += piece) groups += groups_of(c0);
+  float2* stats = static_cast<float2*>(g.sp.take(groups * a->T * 8));
+  groups = 0;
+  for (int64_t c0 = 0; c0 < a->V; c0 += piece) {
+    const int64_t mark = g.sp.used, n = groups_of(c0);
     p.B = u16(a->W) + c0;
     p.ldb = a->ldw;
     if (int rc = g.rows(p.B, a->H, p.N, p.ldb, false)) return rc;
     p.first_col = c0;
     p.stats = g.sp.counting ? nullptr : stats + groups * a->T;
-    int tile = 0;
-    if (int rc = g.run(mk::kProdForward, mk::kProdStats, p, p.N, &tile)) return rc;
-    const mk::ProductShape& s = mk::kProductShapes[tile];
-    groups += (p.N + s.bn - 1) / s.bn;
+    if (int rc = g.run(mk::kProdForward, mk::kProdStats, p, p.N)) return rc;
+    groups += n;
     g.sp.used = mark;
   }
   if (g.sp.counting) return MK_OK;

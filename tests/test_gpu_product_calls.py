@@ -81,3 +81,12 @@ def test_captured_calls_record_no_tickets_they_do_not_touch():
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_vocab_loss_workspace_holds_the_tiles_statistics():
+    """8 bytes a token for each column tile that the launch has, 256 wide for a large batch, and no more.  (Addresses
+    are not read for the question.)"""
+    T, H, V, at = 32768, 512, 131072, 1 << 40
+    n = capi.workspace_bytes("mk_vocab_loss", capi.VocabLossArgs, at, 2 * at, 3 * at, 4 * at, 5 * at, 6 * at, T, H, V, H, V, 0,
+                             -100, 1)
+    assert n == T * V // 256 * 8
