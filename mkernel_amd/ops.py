@@ -79,11 +79,13 @@ def split_workspace(device=None, stream=None) -> torch.Tensor:
 
 
 def release_split_workspaces() -> None:
-    """Free every cached default K-split workspace (after synchronizing
-    every device that has one, so no queued launch still uses them)."""
-    for dev in {k[0] for k in _split_ws}:
+    """Free every cached default K-split workspace, and the calling thread's
+    tickets and small workspaces of the products (after synchronizing every
+    device that has one, so no queued launch still uses them)."""
+    for dev in {k[0] for k in _split_ws} | {torch.device("cuda", k[0]) for k in _spaces.of}:
         torch.cuda.synchronize(dev)
     _split_ws.clear()
+    _spaces.of.clear()
 
 
 def _ws(split_ws, device) -> tuple:
@@ -796,7 +798,7 @@ def moe_ffn_combine_w4(tokens: torch.Tensor, pull: torch.Tensor, row_weight: tor
 # ------------------------------------------------------------------- products with what follows them
 # Tickets (zeroed words by which the parts of a product's K meet, left zeroed by every launch) and behind them a small
 # workspace: one set per thread, device and stream, whose launches are ordered (the launches of two threads' calls on
-# one stream may come between each other).
+# one stream may come between each other).  They go with their thread, or by release_split_workspaces.
 _SPACE = 4 << 20
 _UNTOUCHED = 16  # in place of tickets that a call does not touch
 

@@ -90,3 +90,19 @@ def test_vocab_loss_workspace_holds_the_tiles_statistics():
     n = capi.workspace_bytes("mk_vocab_loss", capi.VocabLossArgs, at, 2 * at, 3 * at, 4 * at, 5 * at, 6 * at, T, H, V, H, V, 0,
                              -100, 1)
     assert n == T * V // 256 * 8
+
+
+def test_small_workspaces_are_given_back():
+    A, B = randn(300, 1501), randn(1501, 205, seed=1)
+    want = ops.gemm_act(A, B)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        assert torch.equal(ops.gemm_act(A, B), want)
+    torch.cuda.synchronize()
+    sets = len(ops._spaces.of)
+    before = torch.cuda.memory_allocated()
+    ops.release_split_workspaces()
+    assert sets >= 2 and before - torch.cuda.memory_allocated() >= sets * ops._SPACE
+    for _ in range(2):
+        assert torch.equal(ops.gemm_act(A, B), want)  # (tickets are zeroed anew)
