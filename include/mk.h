@@ -705,12 +705,14 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* args, void* stream);
 /* Dense products of any size with what follows them, and their gradients.
  *
  * Common to the entry points from here to mk_vocab_loss_backward: bf16
- * operands, fp32 sums, one rounding at the end.  Any sizes up to 2^25 rows and
- * row strides (of at least the row's width, at most 2^21 elements); operands aligned to their
- * elements.  Operands whose rows do not start at 16-byte boundaries, or whose
+ * operands, fp32 sums, one rounding at the end.  Any sizes up to 2^25 rows (2^21
+ * tokens of the loss) and row strides (of at least the row's width, at most 2^21
+ * elements); operands aligned to their elements.  Operands whose rows do not start at 16-byte boundaries, or whose
  * rows' ends do not fill 16 bytes where the sum runs along them, are laid out
  * anew in the workspace first.  Results may not overlap what is read, unless
- * said otherwise.  Sums are added in an order that depends on sizes alone.
+ * said otherwise.  Sums are added in an order that depends on sizes, on the
+ * operands' alignment and strides and on the device's number of CUs, never on
+ * timing.
  * `workspace`: mk_*_workspace_bytes(args) bytes, 16-byte aligned, holding
  * nothing between calls (the pointers in args have to be set for the question,
  * the workspace's own need not).  `tickets`: MK_PRODUCT_TICKETS 32-bit words,
@@ -733,8 +735,8 @@ int mk_moe_ffn_combine_w4(const mk_moe_ffn_w4_args* args, void* stream);
 #define MK_ACT_SILU 4      /* x / (1 + e^-x) */
 
 /* C = act(A @ B + bias) + residual; pre, where set, gets A @ B + bias (bf16) for
- * the backward pass.  residual may be C itself (same type and stride).  From one
- * row (K is then cut into parts that fill the chip) to any number. */
+ * the backward pass.  residual may be C itself (same type and stride).  Where
+ * nothing follows a bf16 product of whole tiles, mk_gemm is as fast or faster. */
 typedef struct mk_gemm_act_args {
   const void* A;         /* bf16 [M, lda] */
   const void* B;         /* bf16 [K, ldb] */
@@ -789,7 +791,8 @@ int mk_gemm_act_backward(const mk_gemm_act_backward_args* args, void* stream);
  * behind those of the experts before it (padded_tokens_per_expert of an index
  * build, at row_block 1 or any other).  Counts are read on the device; below 0
  * they count as 0, and rows from R on, which the counts may name, are not there.
- * Rows behind the last expert's are neither read nor written, whatever they hold.
+ * Rows behind the last expert's are not written, and nothing that they hold is in
+ * a result (where A is laid out anew they are copied with it).
  *   mode 0: out[r] = A[r] @ W[e]                        (out [R, N])
  *   mode 1: out[r] = silu(g) * u, (g | u) = A[r] @ W[e] (out [R, N/2]), and h,
  *           where set, gets (g | u) in bf16 [R, N] for the backward pass. */
@@ -875,7 +878,8 @@ int mk_vocab_loss(const mk_vocab_loss_args* args, void* stream);
  * shards), 0 for ignored tokens,
  *   dx = dl @ W^T (of a shard: its part of the sum),  dW = x^T @ dl.
  * Logits are computed anew, a piece of the vocabulary at a time (piece_columns, a
- * multiple of 256; 0: the library's choice); dl goes through the workspace as
+ * multiple of 256; 0: as many as keep dl in bf16 at 128 MB or less, at least 256);
+ * dl goes through the workspace as
  * `between` says.  In bf16 each of its elements is off by up to 2^-8 of itself
  * (without the significand of the largest dloss, which the fp32 sums take back: of
  * a mean's equal dloss no common rounding stays; of several distinct ones, the

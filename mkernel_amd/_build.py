@@ -16,8 +16,8 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmk.so"
-SOURCES = ["mk_gemm.hip", "mk_gemm_small.hip", "mk_moe.hip", "mk_moe_index.hip", "mk_route.hip", "mk_w4.hip", "mk_product.hip", "mk_product_fwd.hip",
-           "mk_product_grad.hip", "mk_probe.hip", "mk_capi.hip"]
+SOURCES = ["mk_gemm.hip", "mk_gemm_small.hip", "mk_moe.hip", "mk_moe_index.hip", "mk_route.hip", "mk_w4.hip",
+           "mk_product.hip", "mk_product_fwd.hip", "mk_product_grad.hip", "mk_probe.hip", "mk_capi.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -1799,8 +1799,8 @@ void fill_vocab(mk::ProductParams& p, const void* labels, int type, int64_t igno
   p.vocab = V;
 }
 
-// Columns of a piece: its rows of [rows, columns] in bf16 take at most 128 MB (half of the last-level cache), a
-// multiple of 256.
+// Columns of a piece: its rows of [rows, columns] in bf16 take at most 128 MB (half of the last-level cache); a
+// multiple of 256, and 256 at least (beyond 2^18 rows more than that, up to 1 GB at 2^21).
 int64_t piece_of(int64_t rows, int64_t V) {
   const int64_t most = std::max<int64_t>(256, (64LL << 20) / std::max<int64_t>(rows, 1) / 256 * 256);
   return std::min(most, (V + 255) / 256 * 256);

@@ -379,14 +379,16 @@ __device__ __forceinline__ uint32_t lanes_below(uint32_t v, uint32_t most = 0) {
 //
 // The counts are what the device holds, so every workgroup adds them up by itself: 64 groups a step, sums over lanes.
 // Every group's tiles are dealt to all XCDs, ragged 1 by columns (an XCD has all row tiles of a column, which share
-// its weights in L2; from four row tiles on, half of them and twice the columns), ragged 2 by runs of an eighth: with whole groups per XCD, one with half of the rows kept one
-// XCD busy while seven idled (gradient of 32 experts' weights, one of them with 47 % of 7643 rows, 877 us; even
-// groups 385).  Groups of more rows than a tile (products are what bounds them) and of fewer (their weights, or their
-// result, are) take turns while there are both, so that the chip has work of both kinds.
+// its weights in L2; from four row tiles on, half of them and twice the columns), ragged 2 by runs of an eighth: with
+// whole groups per XCD, one with half of the rows kept one XCD busy while seven idled (gradient of 32 experts' weights,
+// one of them with 47 % of 7643 rows, 877 us; even groups 385).  Groups of more rows than a tile (products are what
+// bounds them) and of fewer (their weights, or their result, are) take turns while there are both, so that the chip has
+// work of both kinds.
 template <int BM>
 __device__ __forceinline__ bool find_group_tile(const ProductParams& p, int x, int i, GroupTile& out) {
   const int ln = threadIdx.x & 63, E = p.E;
-  const uint32_t M = (uint32_t)(p.ragged == 1 ? p.M : p.K), per = (uint32_t)(p.ragged == 1 ? p.tiles_n : p.tiles_m * p.tiles_n);
+  const uint32_t M = (uint32_t)(p.ragged == 1 ? p.M : p.K);
+  const uint32_t per = (uint32_t)(p.ragged == 1 ? p.tiles_n : p.tiles_m * p.tiles_n);
   // of the lane's group: its rows; its row tiles, first column (ragged 2: tile) and tiles on this XCD; sums of those
   uint32_t beg, rows, row0, nt, first, w, large, small;
   uint32_t carry = 0, carry_l = 0, carry_s = 0;
@@ -1013,7 +1015,7 @@ __device__ __forceinline__ void product_tile(const ProductParams& p, const TileS
           // the scratch rows are whole units: columns behind the last are zeros, as the products behind read them
           if (col < p.ldc) {
             store8(p.C, m * p.ldc + col, true, 8, x);
-            if constexpr (EPI == kProdDlogits3) {
+            if constexpr (EPI == kProdDlogits3) {  // (4096 x 4096 x 16384: 493 us, 473 with the first part alone)
 #pragma unroll
               for (int t = 1; t < 3; ++t) {
 #pragma unroll
@@ -1127,8 +1129,10 @@ hipError_t launch_product_tile(const ProductParams& p, int tile, int64_t grid, h
     case kProd128: return launch_product_cfg<ProdTile128, void, AKC, BKC, EPI>(p, grid, stream);
     case kProd256:
       // only the epilogues of expert products see small groups
-      if constexpr (EPI != kProdStats && EPI != kProdDlogits && EPI != kProdDlogits3) return launch_product_cfg<ProdTile256, ProdFlat256<BKC>, AKC, BKC, EPI>(p, grid, stream);
-      else return launch_product_cfg<ProdTile256, void, AKC, BKC, EPI>(p, grid, stream);
+      if constexpr (EPI != kProdStats && EPI != kProdDlogits && EPI != kProdDlogits3)
+        return launch_product_cfg<ProdTile256, ProdFlat256<BKC>, AKC, BKC, EPI>(p, grid, stream);
+      else
+        return launch_product_cfg<ProdTile256, void, AKC, BKC, EPI>(p, grid, stream);
   }
   return hipErrorInvalidValue;
 }

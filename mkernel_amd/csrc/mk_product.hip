@@ -101,12 +101,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void product_few_rows_kernel(Produc
   else static_cast<uint16_t*>(p.C)[m * p.ldc + at] = (uint16_t)pack_bf16x2(x, 0.f);
 }
 
-// A wave copies 512 columns of a row; one workgroup four rows of group blockIdx.z, columns from 2048 * blockIdx.y on.
-// (Loads of single elements moved 1.4 TB/s, a 1024 x 5003 matrix in 14.3 us.)
+// Whether a token has no loss.
 __device__ __forceinline__ bool ignored(const RepackParams& p, int64_t row) {
   return (p.labels64 ? static_cast<const int64_t*>(p.labels)[row] : static_cast<const int*>(p.labels)[row]) == p.ignore;
 }
 
+// A wave copies 512 columns of a row; one workgroup four rows of group blockIdx.z, columns from 2048 * blockIdx.y on.
+// (Loads of single elements moved 1.4 TB/s, a 1024 x 5003 matrix in 14.3 us.)
+// The first workgroup finds the scale of dloss too (4096 tokens 24 us, 12.6 without).
 __global__ __launch_bounds__(256) void repack_kernel(RepackParams p) {
   const int lane = threadIdx.x & 63;
   if (p.scale && blockIdx.x == 0 && blockIdx.y == 0) {

@@ -1,6 +1,6 @@
 // mk_product_plan.h — which tile a product runs on and in how many parts along K:
-// the host's choice, from sizes alone (no HIP headers, so that it can be checked
-// without a GPU).
+// the host's choice, from sizes and the number of CUs (no HIP headers, so that it
+// can be checked without a GPU).
 #pragma once
 #include <stdint.h>
 
@@ -16,8 +16,9 @@ constexpr int kTicketStride = 32;     // words between them: a line each
 //   round + K/16 x slope(x),  slope = one + load min(x, 1) + more max(x - 1, 0),  x = the round's workgroups per CU
 // (a full chip clocks lower and shares its caches).  `start` comes once, `area` for a million results (their stores),
 // and where the last round's tiles are cut: meet + part per part, and `exchange` for a MB of partial sums.  Fitted to
-// 1392 launches of 79 shapes of 1 .. 8192 rows, 64 .. 8192 columns and K on one MI355X; the tile and cut that it picks
-// take 4 % longer than the best of those tried in the mean (worst 33 %).
+// 1392 launches of 79 shapes of 1 .. 8192 rows, 64 .. 8192 columns and K on one MI355X; among these the tile and cut
+// that it picks take 4 % longer than the best of those tried in the mean (worst 33 %).  Odd sizes and short sums take 25
+// to 60 % longer than it says (1003 x 2811 x 1501 22 us and 28, a gradient 1024 x 520 x 5003 14 and 22).
 struct ProductShape {
   int bm, bn, per_cu;
   double start, round, one, load, more, meet, part, area, exchange;

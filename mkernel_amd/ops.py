@@ -896,7 +896,8 @@ def gemm_act(A: torch.Tensor, B: torch.Tensor, bias: torch.Tensor | None = None,
     relu, gelu, gelu_tanh or silu.  bias [N] and residual [M, N]: bfloat16 or
     float32; out: bfloat16 or float32 (out_dtype where none is given), may be the
     residual itself, overlaps nothing else.  pre (bf16 [M, N]) receives A @ B +
-    bias for gemm_act_backward.  Nothing is recorded for autograd."""
+    bias for gemm_act_backward.  Where nothing follows a bfloat16 product of whole
+    tiles, gemm is as fast or faster.  Nothing is recorded for autograd."""
     M, K = _matrix(A, "A")
     dev = A.device
     if _matrix(B, "B")[0] != K or B.device != dev:
@@ -988,8 +989,8 @@ def moe_ragged_gemm(A: torch.Tensor, W: torch.Tensor, counts: torch.Tensor, mode
     row_block 1 or any other; nothing is read back), W bf16 [E, K, N].
     mode 0: out = A @ W[e] (bf16 [R, N]); mode 1: out = silu(g) * u with (g | u) =
     A @ W[e] (bf16 [R, N / 2]), and h (bf16 [R, N]) receives (g | u) for the
-    backward pass.  Any sizes.  Rows behind the experts' are neither read nor
-    written (new results hold whatever was there)."""
+    backward pass.  Any sizes.  Rows behind the experts' are not written (new
+    results hold whatever was there), and nothing that they hold is in a result."""
     R, K = _matrix(A, "A")
     dev = A.device
     if _experts(W, counts, dev)[1] != K:
@@ -1112,7 +1113,8 @@ def vocab_loss_backward(x: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, 
     [H, V]), bfloat16 or float32, None for what is not needed, from dloss
     (float32 [T]) and lse (of a shard: the joined one).  The logits are computed
     anew, a piece of the vocabulary at a time (piece_columns, a multiple of 256;
-    0: as many as keep the piece's gradient of the logits below 128 MB).  dl_dtype:
+    0: as many as keep the piece's gradient of the logits in bfloat16 at 128 MB or
+    less, at least 256).  dl_dtype:
     how that gradient goes into the products of dx and dW.  In bfloat16, one
     product each, each element is off by up to 2^-8 of itself (without the
     significand of the largest dloss, which the sums take back, so that a mean's
