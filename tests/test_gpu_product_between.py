@@ -203,3 +203,29 @@ def test_vocab_loss_backward_choices():
         ops.vocab_loss_backward(x, W, labels, lse, dloss, dl_dtype=torch.float16)
     dx, dW = ops.vocab_loss_backward(x[:0], W, labels[:0], lse[:0], dloss[:0], dx_dtype=F32, dW_dtype=F32)
     assert dx.shape == (0, H) and (dW == 0).all()
+
+
+def test_captured_calls_of_three_parts():
+    """In a graph, replayed between eager calls of the same."""
+    M, K, N = 200, 96, 136
+    dC, A, B, pre, *_ = _backward(M, K, N, "silu", BF16, BF16)
+    T, H, V = 100, 65, 600
+    x, W, labels = randn(T, H, seed=147), randn(H, V, seed=148, scale=0.3), _labels(T, V, 149).cuda()
+    lse, dloss = ops.vocab_loss(x, W, labels)["lse"], torch.full((T,), 1.0 / T, device="cuda")
+
+    def calls():
+        return [*ops.gemm_act_backward(dC, A, B, pre=pre, act="silu", dB_dtype=F32, dpre_dtype=F32),
+                *ops.vocab_loss_backward(x, W, labels, lse, dloss, dx_dtype=F32, piece_columns=256, dl_dtype=F32)]
+
+    want = calls()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = calls()
+    for _ in range(5):
+        for t in out:
+            t.fill_(float("nan"))
+        g.replay()
+        eager = calls()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(out, want, eager))

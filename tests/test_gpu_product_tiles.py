@@ -92,3 +92,29 @@ def test_vocab_loss_of_infinite_logits(T, H, V):
     assert r["lse"][3:].isfinite().all() and r["loss"][3:].isfinite().all()
     rest = ops.vocab_loss(x[3:], W, labels[3:])["lse"] if T > 3 else None
     assert rest is None or torch.allclose(rest, r["lse"][3:], rtol=1e-5, atol=1e-5)
+
+
+def test_vocab_loss_of_a_long_batch():
+    """More tokens than 128 MB of dl have room for at 256 columns, the least that a piece has."""
+    T, H, V = 300001, 24, 700
+    x, W = randn(T, H, seed=24), randn(H, V, seed=25, scale=2 * H ** -0.5)
+    labels = torch.arange(T, device="cuda") * 7919 % V
+    labels[::5] = -100
+    on = labels >= 0
+    r = ops.vocab_loss(x, W, labels)
+    z, err = product(x, W)
+    lse = torch.logsumexp(z, 1)
+    tol = err.amax(1) + (V / 64 + 200) * U + 4 * U * lse.abs()
+    near(r["lse"], torch.where(on, lse, 0.0), torch.where(on, tol, 0.0) + 1e-300)
+    dloss = torch.full((T,), 1.0 / T, device="cuda")
+    dx, dW = ops.vocab_loss_backward(x, W, labels, r["lse"], dloss)
+    p = torch.exp(z - lse[:, None])
+    w = torch.where(on, dloss.to(F64), 0.0)[:, None]
+    pe = p * (err + tol[:, None] + (6 * (z - lse[:, None]).abs().clamp(max=90) + 4) * U) * w
+    p.scatter_add_(1, labels.clamp(min=0)[:, None], torch.full((T, 1), -1.0, dtype=F64, device="cuda"))
+    dl = p * w
+    de = pe + 2.0 ** -8 * (dl.abs() + pe) + 2.0 ** -126
+    want, tol = dl @ W.to(F64).t(), (de + (V + 8) * U * dl.abs()) @ W.to(F64).abs().t()
+    near(dx, want, HALF[BF16] * (want.abs() + tol) + tol + 1e-300)
+    want, tol = x.to(F64).t() @ dl, x.to(F64).abs().t() @ (de + (T + 1) * U * dl.abs())
+    near(dW, want, HALF[BF16] * (want.abs() + tol) + tol)
