@@ -285,7 +285,8 @@ def lib() -> C.CDLL:
                                "(or python -m mkernel_amd._build) first")
         L = C.CDLL(str(LIB_PATH))
         for name in ("mk_gemm", "mk_ag_gemm", "mk_ag_gemm_noalloc", "mk_gemm_rs", "mk_gemm_ar", "mk_gemm_ar_two_shot",
-                     "mk_moe_permute", "mk_moe_grouped_gemm", "mk_moe_combine", "mk_moe_ffn_combine", "mk_moe_route", "mk_moe_route_backward",
+                     "mk_moe_permute", "mk_moe_grouped_gemm", "mk_moe_combine", "mk_moe_ffn_combine", "mk_moe_route",
+                     "mk_moe_route_backward",
                      "mk_moe_combine_backward", "mk_w4_pack", "mk_w4_quantize", "mk_gemm_w4",
                      "mk_moe_grouped_gemm_w4", "mk_moe_ffn_combine_w4", *_PRODUCTS):
             getattr(L, name).argtypes = [vp, vp]
